@@ -141,3 +141,5 @@ void sx_host_bind_scratch(sx_engine *e, sx::AttnFusedArgs &a);
 // inside a stream capture.
 float *sx_host_inv_freq(sx_engine *e, uint32_t rot, float theta, sx_status *st);
 sx_status sx_host_cuda_status(cudaError_t e, const char *what);
+// Arguments common to the paged 8-bit cache's operators (sx_kv8_append.cu).
+sx_status sx_host_check_kv8(const char *what, const sx_kv8 *c, sx_dtype t, uint32_t num_q);

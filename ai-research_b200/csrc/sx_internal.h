@@ -335,6 +335,9 @@ struct ArchiveArgs {
 cudaError_t prepare_archive_kernels();
 cudaError_t launch_archive_integrate(const ArchiveArgs &a, cudaStream_t s);
 
+// Paged 8-bit KV cache (sx_kv8_append.cu)
+cudaError_t prepare_kv8_append();
+
 // Batch-prefill Q4_0 projection GEMM (sx_prefill.cu): y[t][n] = x[t][:] . bf16(deq(w[n][:]))
 cudaError_t prepare_prefill_kernel();
 cudaError_t launch_prefill_q4(const void *w, const void *x, float *y, uint32_t t, uint32_t n,

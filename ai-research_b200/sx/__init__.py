@@ -34,6 +34,14 @@ QUANT_Q4 = 2
 
 ENGINE_KV_F32 = 1
 
+DTYPE_F32 = 0
+DTYPE_BF16 = 1
+KV8_K_EQ_V = 1
+KV8_V_NORM = 2
+NO_PAGE = 0xFFFFFFFF
+NO_TOKEN = 0xFFFFFFFF
+STREAM_LEGACY = 1  # cudaStreamLegacy: CUDA's default stream as an Engine.set_stream argument
+
 
 class SxError(RuntimeError):
     def __init__(self, status: int, message: str):
@@ -83,6 +91,31 @@ class QuiescenceGatePC(C.Structure):
     _fields_ = [("hidden_size", C.c_uint32), ("threshold_sq", C.c_float),
                 ("base_cmd_idx", C.c_uint32), ("num_cmds", C.c_uint32),
                 ("targets", C.c_uint32 * 16)]
+
+
+class KV8(C.Structure):
+    """sx_kv8: a paged 8-bit cache of one layer, over caller-owned device tensors (kept alive by
+    this object): data [num_pages][num_kv][page_tokens / 16][2][16 head_dim] bytes, scale
+    [num_pages][num_kv][page_tokens / 16][2] f32, table [num_seqs][max_pages] page ids."""
+
+    _fields_ = [("data", C.c_void_p), ("scale", C.c_void_p), ("table", C.c_void_p)] + [
+        (n, C.c_uint32) for n in ("num_pages", "page_tokens", "max_pages", "num_seqs", "num_kv",
+                                  "head_dim")]
+
+    def __init__(self, data, scale, table, page_tokens: int, num_kv: int, head_dim: int):
+        page = page_tokens * num_kv * 2 * head_dim
+        num_pages = data.numel() * data.element_size() // page
+        if num_pages * page != data.numel() * data.element_size():
+            raise ValueError("KV8: data does not hold whole pages")
+        if scale.numel() != num_pages * num_kv * (page_tokens // 16) * 2 or scale.element_size() != 4:
+            raise ValueError("KV8: scale must hold one f32 per record")
+        if table.dim() != 2 or table.element_size() != 4:
+            raise ValueError("KV8: table must be [num_seqs][max_pages] 32-bit page ids")
+        if not (data.is_contiguous() and scale.is_contiguous() and table.is_contiguous()):
+            raise ValueError("KV8: data, scale and table must be contiguous")
+        self._keep = (data, scale, table)
+        super().__init__(_ptr(data), _ptr(scale), _ptr(table), num_pages, page_tokens,
+                         table.shape[1], table.shape[0], num_kv, head_dim)
 
 
 class TpShard(C.Structure):
@@ -284,6 +317,21 @@ _SIGS = {
     "sx_model_vcache": (_P, [_P, _U32]),
     "sx_model_weight_bytes": (_U64, [_P]),
     "sx_model_kernels_per_token": (_U32, [_P, _I]),
+    "sx_pages_create": (_S, [_U32, _U32, _U32, _U32, C.POINTER(_P)]),
+    "sx_pages_destroy": (None, [_P]),
+    "sx_pages_extend": (_S, [_P, _U32, _U32]),
+    "sx_pages_truncate": (_S, [_P, _U32, _U32]),
+    "sx_pages_release_before": (_S, [_P, _U32, _U32]),
+    "sx_pages_length": (_U32, [_P, _U32]),
+    "sx_pages_free_count": (_U32, [_P]),
+    "sx_pages_table": (_P, [_P]),
+    "sx_dispatch_kv8_append": (_S, [_P, C.POINTER(KV8), _I, _P, _P, _P, _U32, _U32, _U32, _P, _P,
+                                    _P, _P, _P, _U32, _U32, _P, _U32, _U32, _F]),
+    "sx_dispatch_kv8_attn": (_S, [_P, C.POINTER(KV8), _I, _P, _P, _U32, _U32, _P, _P, _U32, _U32,
+                                  _U32, _F]),
+    "sx_dispatch_probs": (_S, [_P, _P, _U32, _P, _U32, _U32, _U32, _F]),
+    "sx_dispatch_verify": (_S, [_P, _P, _U32, _P, _U32, _P, _P, _P, _P, _P, _P, _U32, _U32,
+                                _U32]),
     "sx_archive_create": (_S, [_P, _U32, _P, C.POINTER(_P)]),
     "sx_archive_destroy": (None, [_P]),
     "sx_archive_integrate": (_S, [_P, _P, _U64, _P, _P]),
@@ -400,6 +448,45 @@ class Ring:
         out = np.zeros(self.total_slots, np.uint32)
         n = lib().sx_ring_active_slots(self.h, layer, clock, out.ctypes.data)
         return out[:n].copy()
+
+
+class Pages:
+    """sx_pages: which pages of a KV8 pool hold which sequence (host bookkeeping)."""
+
+    def __init__(self, num_pages: int, page_tokens: int, num_seqs: int, max_pages: int):
+        h = C.c_void_p()
+        check(lib().sx_pages_create(num_pages, page_tokens, num_seqs, max_pages, C.byref(h)))
+        self.h = h
+        self.num_seqs, self.max_pages = num_seqs, max_pages
+
+    def close(self):
+        if getattr(self, "h", None):
+            lib().sx_pages_destroy(self.h)
+            self.h = None
+
+    __del__ = _quiet_close
+
+    def extend(self, seq: int, length: int) -> None:
+        check(lib().sx_pages_extend(self.h, seq, length))
+
+    def truncate(self, seq: int, length: int) -> None:
+        check(lib().sx_pages_truncate(self.h, seq, length))
+
+    def release_before(self, seq: int, pos: int) -> None:
+        check(lib().sx_pages_release_before(self.h, seq, pos))
+
+    def length(self, seq: int) -> int:
+        return int(lib().sx_pages_length(self.h, seq))
+
+    @property
+    def free_count(self) -> int:
+        return int(lib().sx_pages_free_count(self.h))
+
+    def table(self) -> np.ndarray:
+        """A copy of the page table, [num_seqs][max_pages] uint32."""
+        n = self.num_seqs * self.max_pages
+        src = (C.c_uint32 * n).from_address(lib().sx_pages_table(self.h))
+        return np.array(src, np.uint32).reshape(self.num_seqs, self.max_pages)
 
 
 class Engine:
@@ -562,6 +649,40 @@ class Engine:
 
     def argmax(self, logits, n, out):
         check(lib().sx_dispatch_argmax(self.h, _ptr(logits), n, _ptr(out)))
+
+    # --- speculative decoding over a paged 8-bit KV cache
+    def kv8_append(self, cache: "KV8", dtype, q_in, k_in, v_in, q_out, row_start, kv_len, tokens,
+                   num_q, inv_freq, rotary_dim, q_norm_w=None, k_norm_w=None, v_norm=False,
+                   k_eq_v=False, eps=1e-6, q_ld=0, k_ld=0, v_ld=0):
+        """sx_dispatch_kv8_append: norm, rotation and quantised append of `tokens` rows (row
+        strides in elements; 0: contiguous rows)."""
+        kv = cache.num_kv * cache.head_dim
+        check(lib().sx_dispatch_kv8_append(
+            self.h, C.byref(cache), dtype, _ptr(q_in), _ptr(k_in), _ptr(v_in),
+            q_ld or num_q * cache.head_dim, k_ld or kv, v_ld or kv, _ptr(q_norm_w),
+            _ptr(k_norm_w), _ptr(q_out), _ptr(row_start), _ptr(kv_len), tokens, num_q,
+            _ptr(inv_freq), rotary_dim,
+            (KV8_V_NORM if v_norm else 0) | (KV8_K_EQ_V if k_eq_v else 0), eps))
+
+    def kv8_attn(self, cache: "KV8", dtype, q, out, row_start, kv_len, tokens, num_q, scale,
+                 window=0, q_ld=0, out_ld=0):
+        """sx_dispatch_kv8_attn: attention of `tokens` rows over the paged 8-bit cache."""
+        row = num_q * cache.head_dim
+        check(lib().sx_dispatch_kv8_attn(
+            self.h, C.byref(cache), dtype, _ptr(q), _ptr(out), q_ld or row, out_ld or row,
+            _ptr(row_start), _ptr(kv_len), tokens, num_q, window, scale))
+
+    def probs(self, logits, probs, rows, n, temperature=1.0, logits_ld=0, probs_ld=0):
+        """sx_dispatch_probs: softmax(logits / temperature) of f32 rows."""
+        check(lib().sx_dispatch_probs(self.h, _ptr(logits), logits_ld, _ptr(probs), probs_ld, rows,
+                                      n, temperature))
+
+    def verify(self, target, draft, tok, u_accept, u_sample, out, accepted, seqs, drafts, vocab,
+               n_draft=None, target_ld=0, draft_ld=0):
+        """sx_dispatch_verify: acceptance of drafted tokens and the draw of the next one."""
+        check(lib().sx_dispatch_verify(
+            self.h, _ptr(target), target_ld, _ptr(draft), draft_ld, _ptr(tok), _ptr(n_draft),
+            _ptr(u_accept), _ptr(u_sample), _ptr(out), _ptr(accepted), seqs, drafts, vocab))
 
     def unpack_q4(self, w_packed, out, m, k):
         check(lib().sx_dispatch_unpack_q4(self.h, _ptr(w_packed), _ptr(out), m, k))

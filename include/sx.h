@@ -514,6 +514,127 @@ SX_API sx_status sx_comm_set_wait_ns(sx_comm *c, uint64_t wait_ns);
 SX_API sx_status sx_model_create_tp(sx_engine *e, const sx_model_config *cfg, sx_comm *comm,
                                     sx_model **out);
 
+/* ---------------------------------------------------------------------------------------
+ * Speculative decoding over a paged 8-bit KV cache (new: the reference keeps one ring of bf16
+ * or f32 K/V per session and decodes greedily).  One serving step of many sequences appends the
+ * new rows' keys and values (sx_dispatch_kv8_append), attends (sx_dispatch_kv8_attn), turns the
+ * logits into probabilities (sx_dispatch_probs) and checks the drafted tokens against them
+ * (sx_dispatch_verify).  All four are asynchronous on the engine stream, allocate nothing and
+ * can be captured in a CUDA graph; lengths, page ids and tokens are read on the device.
+ * ------------------------------------------------------------------------------------- */
+/* Page bookkeeping (host): which pages of a pool hold which sequence.  Only ids live here. */
+typedef struct sx_pages sx_pages;
+#define SX_NO_PAGE 0xFFFFFFFFu
+/* num_pages pages of page_tokens tokens for num_seqs sequences of up to max_pages pages each;
+ * every sequence starts empty. */
+SX_API sx_status sx_pages_create(uint32_t num_pages, uint32_t page_tokens, uint32_t num_seqs,
+                                 uint32_t max_pages, sx_pages **out);
+SX_API void sx_pages_destroy(sx_pages *p);
+/* Sequence seq grows to len tokens (no-op when it is that long): its missing pages are taken from
+ * the free ones, last freed first.  SX_ERR_OOM, with nothing changed, when there are too few. */
+SX_API sx_status sx_pages_extend(sx_pages *p, uint32_t seq, uint32_t len);
+/* Sequence seq shrinks to len tokens (rejected drafts; 0 ends it): pages past them are freed. */
+SX_API sx_status sx_pages_truncate(sx_pages *p, uint32_t seq, uint32_t len);
+/* Pages of seq that lie wholly before token pos are freed (a window has passed them). */
+SX_API sx_status sx_pages_release_before(sx_pages *p, uint32_t seq, uint32_t pos);
+SX_API uint32_t sx_pages_length(const sx_pages *p, uint32_t seq);
+SX_API uint32_t sx_pages_free_count(const sx_pages *p);
+/* [num_seqs][max_pages] page ids, SX_NO_PAGE where there is none; owned by p, to be copied to the
+ * device before the step that uses it. */
+SX_API const uint32_t *sx_pages_table(const sx_pages *p);
+
+typedef enum { SX_F32 = 0, SX_BF16 = 1 } sx_dtype;
+
+/* A paged 8-bit cache of one layer in device memory.  Every 16 tokens of one kv head are a K
+ * record and a V record of 16 head_dim e4m3 bytes; a stored value is its e4m3 number times the
+ * record's scale, a power of two in 2^-60 .. 2^60.  The bytes stand in the order in which the
+ * attention's matrix instructions take them: token t (0..15) and element d at byte
+ *   K: 512 (d / 32) + 16 (4 (t % 8) + (d % 32) / 8) + 8 (t / 8) + d % 8
+ *   V: 512 (d / 32) + 16 (4 ((d % 32) / 4) + (t % 8) / 2) + 4 (d % 4) + t % 2 + 2 (t / 8)
+ * of its record.  Position j of sequence b is token j % page_tokens of page
+ * table[b * max_pages + j / page_tokens]. */
+typedef struct {
+  void *data;            /* [num_pages][num_kv][page_tokens / 16][2 (K, V)][16 head_dim] bytes,
+                            16-byte aligned                                                    */
+  float *scale;          /* [num_pages][num_kv][page_tokens / 16][2 (K, V)], 8-byte aligned    */
+  const uint32_t *table; /* [num_seqs][max_pages]                                              */
+  uint32_t num_pages;
+  uint32_t page_tokens;  /* a multiple of 16, up to 1024                                       */
+  uint32_t max_pages;    /* max_pages * page_tokens < 2^31                                     */
+  uint32_t num_seqs;     /* up to 4096                                                         */
+  uint32_t num_kv;
+  uint32_t head_dim;     /* 64, 128, 256 or 512                                                */
+} sx_kv8;
+#define SX_KV8_K_EQ_V 1u /* v is the raw k (attention_k_eq_v)  */
+#define SX_KV8_V_NORM 2u /* v is RMS-normalised without a gain */
+
+/* New rows into the cache.  Rows row_start[b] .. row_start[b + 1] of q_in / k_in / v_in (dtype t,
+ * row strides q_ld / k_ld / v_ld elements) are the last tokens of sequence b, which is kv_len[b]
+ * tokens long with them: row r sits at position kv_len[b] - row_start[b + 1] + r.  q heads and k
+ * heads are RMS-normalised with their gains (NULL: not) and rotated over the first rotary_dim
+ * elements, pairs (i, i + rotary_dim / 2) by the angle f32(position) * inv_freq[i] (f32, see
+ * sx_rope_inv_freq); q goes to q_out ([tokens][num_q * head_dim], dtype t; num_q 0: no q), k and
+ * v to their pages.  A record's scale is the smallest power of two 2^e with max |x| <= 448 2^e
+ * over what it holds; when new tokens raise it the older ones are rounded again to the new scale
+ * (exact but for e4m3 subnormals), and a record whose first token is new starts empty: its scale
+ * is the new tokens' and the slots after them hold zeros.  A NaN is stored as NaN and an infinity
+ * as the largest value.  Sequences whose rows or length do not fit (row_start falling or past
+ * `tokens`, more rows than kv_len, kv_len past the table, page id >= num_pages) are skipped and
+ * raise SX_ERR_DEVICE at the next sx_engine_sync.  One call must not name a page twice among the
+ * pages it writes.  Vectors 16-byte aligned, strides multiples of 16 bytes. */
+SX_API sx_status sx_dispatch_kv8_append(sx_engine *e, const sx_kv8 *c, sx_dtype t,
+                                        const void *q_in, const void *k_in, const void *v_in,
+                                        uint32_t q_ld, uint32_t k_ld, uint32_t v_ld,
+                                        const float *q_norm_w, const float *k_norm_w, void *q_out,
+                                        const uint32_t *row_start, const uint32_t *kv_len,
+                                        uint32_t tokens, uint32_t num_q, const float *inv_freq,
+                                        uint32_t rotary_dim, uint32_t flags, float eps);
+
+/* Attention of rows q ([tokens] rows of num_q * head_dim, dtype t, row stride q_ld elements) over
+ * the cache; rows, positions and lengths as in sx_dispatch_kv8_append (which runs first).  Row at
+ * position pos of sequence b sees keys j <= pos, with window > 0 only j > pos - window:
+ *   out = sum_j p_j V_j,  p = softmax_j(scale * q . K_j);  a row that sees nothing is zero.
+ * out has dtype t and row stride out_ld.  Pages that no row of a call sees are not read, nor are
+ * their table entries.  Masked keys do not count whatever their pages hold, NaN included; a row
+ * that sees a V record's NaN is NaN, at least in the elements that hold it.  A bad page id masks its tokens and, like bad
+ * rows and lengths (which leave their rows unwritten), raises SX_ERR_DEVICE.  Products of 16-bit
+ * operands with f32 sums: e4m3 is exact in f16; q and p are split into two f16 terms for SX_F32
+ * (22 bits) and rounded to f16 for SX_BF16.  Vectors 16-byte aligned, strides multiples of
+ * 16 bytes; num_q a multiple of num_kv, at most 64 q heads per kv head. */
+SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, sx_dtype t, const void *q,
+                                      void *out, uint32_t q_ld, uint32_t out_ld,
+                                      const uint32_t *row_start, const uint32_t *kv_len,
+                                      uint32_t tokens, uint32_t num_q, uint32_t window,
+                                      float scale);
+
+/* probs[r] = softmax(logits[r] / temperature) for `rows` rows of n f32 (strides in floats, 0: n);
+ * temperature > 0.  A row of -inf alone gives zeros; a NaN or +inf gives NaN.  In place allowed
+ * when the strides are equal. */
+SX_API sx_status sx_dispatch_probs(sx_engine *e, const float *logits, uint32_t logits_ld,
+                                   float *probs, uint32_t probs_ld, uint32_t rows, uint32_t n,
+                                   float temperature);
+
+#define SX_NO_TOKEN 0xFFFFFFFFu
+/* Verification of drafted tokens.  Sequence b has n_draft[b] <= drafts drafted tokens
+ * tok[b][0..] (n_draft NULL: `drafts` each); row i of target[b] ([seqs][drafts + 1] rows of vocab
+ * probabilities, row stride target_ld floats) is the target's distribution in the place of draft
+ * i, row n_draft[b] the one after them; draft[b] ([seqs][drafts] rows, stride draft_ld) are the
+ * distributions the tokens were drawn from (NULL: chosen without chance, q = 1 at the token).
+ * Draft i is accepted while u_accept[b][i] * q_i(tok_i) < p_i(tok_i) (f32 product).  The next
+ * token is drawn with u_sample[b] in [0, 1) from max(p - q, 0) of the first refused place, or from
+ * row n_draft[b] when all were accepted: with weights floor(min(w, 1) 2^38) (NaN and negative: 0),
+ * their sum S and goal floor(S floor(u 2^24) / 2^24), the first index whose cumulative weight
+ * exceeds the goal -- whole numbers, so no order of summation changes the token.  Where the
+ * difference has no weight the target's row itself is used, and SX_NO_TOKEN where that has none.
+ * out[b][0 .. drafts]: the accepted tokens, the drawn one, then SX_NO_TOKEN; accepted[b]: how many
+ * were accepted.  A token id >= vocab is refused; n_draft[b] > drafts counts as drafts; both
+ * raise SX_ERR_DEVICE.  vocab <= 2^24; strides 0: vocab. */
+SX_API sx_status sx_dispatch_verify(sx_engine *e, const float *target, uint32_t target_ld,
+                                    const float *draft, uint32_t draft_ld, const uint32_t *tok,
+                                    const uint32_t *n_draft, const float *u_accept,
+                                    const float *u_sample, uint32_t *out, uint32_t *accepted,
+                                    uint32_t seqs, uint32_t drafts, uint32_t vocab);
+
 #ifdef __cplusplus
 }
 #endif
