@@ -613,6 +613,8 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
       size_t o_done = take(256);
       size_t o_amax = take(sx::argmax_scratch_bytes());
       size_t o_pbar = take(256);
+      size_t o_kpart = take(sx::kv8_part_bytes(e->num_sms));
+      size_t o_kcnt = take((size_t)e->num_sms * 4);
       e->scratch_bytes = off;
       st = cuda_status(cudaMalloc(&e->scratch, e->scratch_bytes), "engine scratch");
       if (st) break;
@@ -626,6 +628,8 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
       e->done_cnt = reinterpret_cast<uint32_t *>(b + o_done);
       e->argmax_part = b + o_amax;
       e->persist_bar = reinterpret_cast<uint32_t *>(b + o_pbar);
+      e->kv8_part = reinterpret_cast<float *>(b + o_kpart);
+      e->kv8_cnt = reinterpret_cast<uint32_t *>(b + o_kcnt);
       st = cuda_status(cudaMemset(e->scratch, 0, e->scratch_bytes), "engine scratch zero");
       if (st) break;
     }
@@ -646,6 +650,8 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
     st = cuda_status(sx::prepare_prefill_kernel(), "prefill kernel attributes");
     if (st) break;
     st = cuda_status(sx::prepare_kv8_append(), "kv8 append kernel attributes");
+    if (st) break;
+    st = cuda_status(sx::prepare_kv8_attn(), "kv8 attention kernel attributes");
   } while (0);
   if (st != SX_OK) {
     sx_engine_destroy(e);

@@ -337,6 +337,9 @@ cudaError_t launch_archive_integrate(const ArchiveArgs &a, cudaStream_t s);
 
 // Paged 8-bit KV cache (sx_kv8_append.cu)
 cudaError_t prepare_kv8_append();
+// and its attention (sx_kv8_attn.cu): scratch for the parts of split problems
+cudaError_t prepare_kv8_attn();
+size_t kv8_part_bytes(int num_sms);
 
 // Batch-prefill Q4_0 projection GEMM (sx_prefill.cu): y[t][n] = x[t][:] . bf16(deq(w[n][:]))
 cudaError_t prepare_prefill_kernel();

@@ -2,12 +2,35 @@
 //
 //   out_r = sum_j p_j V_j,  p = softmax_j(scale q_r . K_j),  j <= pos(r), j > pos(r) - window
 //
-// One warp per row and q head walks the row's keys with a running maximum and sum.
+// The rows that share a kv head (n new tokens x G q heads) are packed, and the two products run
+// transposed on mma.m16n8k16: S^T = K Q^T with 16 tokens as the rows of A, O^T = V^T P^T with 16
+// elements of the head as the rows of A.  The cache's records are those A operands byte for byte
+// (sx_kv8.cuh), so a block of 16 tokens goes shared memory -> registers -> f16 -> MMA, and eight
+// packed rows fill the instruction's N without waste.  P^T leaves the first product with tokens
+// along the lanes' rows and enters the second with tokens along K: movmatrix transposes it.
+//
+// Values: e4m3 is exact in f16.  q is scaled by a power of two per row to at most 2 and split into
+// two f16 terms (22 bits) for f32 rows; bf16 rows need one.  The running maximum m is that of
+// x + log2(v scale), x the score in log2 units, so that p' = 2^(x + log2(v scale) - m + 10) is at
+// most 2^10, carries the V record's scale and keeps 14 binades of subnormal-free f16 below the
+// largest contribution; the softmax's sum takes p' / v scale in f32.
+//
+// Split: the batch's work is a line of 16-token blocks -- for each sequence, kv head and group of
+// packed rows the blocks it sees -- cut into equal runs, one per CTA, computed on the device from
+// the lengths, so a ragged batch and one long sequence balance alike.  The warps of a CTA take
+// blocks in turn, each with its own ring of bulk copies and its own maximum, sum and output; they
+// merge in shared memory at the end of a problem, and CTAs that share a problem through the
+// workspace: the last to arrive merges (its order is that of the CTAs, so results repeat).
 #include "sx_host.h"
 #include "sx_kv8.cuh"
 
 namespace sx {
 namespace {
+
+constexpr int kDecWarps = 8;
+constexpr int kDecThreads = kDecWarps * 32;
+constexpr float kPOffset = 10.0f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct Kv8AttnArgs {
   sx_kv8 c;
@@ -15,75 +38,624 @@ struct Kv8AttnArgs {
   void *out;
   uint32_t q_ld, out_ld;
   const uint32_t *row_start, *kv_len;
-  uint32_t tokens, num_q, window;
+  uint32_t tokens, num_q, window, gqa, min_run;
   float scale;
+  float *part;      // [2 grid][8 NT] x {m, l}, then [2 grid][8 NT][D]
+  uint32_t *cnt;    // [grid], zero at rest
   uint32_t *err;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv8_attn_kernel(Kv8AttnArgs a) {
-  constexpr int kPer = D / 32;
-  const int lane = threadIdx.x & 31;
-  const uint32_t t = blockIdx.x, h = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (h >= a.num_q) return;
-  const uint32_t b = warp_last_le(a.c.num_seqs, t, [&](uint32_t i) { return a.row_start[i]; });
-  Kv8Rows r;
-  if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r)) {
-    if (lane == 0) raise_error(a.err, kDevBadParams);
-    return;
+SX_DEV float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+  return r;
+}
+SX_DEV uint32_t movmatrix_trans(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
+}
+SX_DEV uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// what f16 rounding left of the pair
+SX_DEV uint32_t pack_f16_rest(float lo, float hi, uint32_t rounded) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&rounded));
+  return pack_f16(lo - f.x, hi - f.y);
+}
+
+// The blocks of 16 tokens that rows of a sequence see.
+SX_DEV void seen_blocks(const Kv8Rows &r, uint32_t window, uint32_t *first, uint32_t *count) {
+  const uint32_t pos0 = r.len - r.n;  // of the first row
+  *first = (window && pos0 + 1 > window ? pos0 + 1 - window : 0) / kKv8Block;
+  *count = r.n ? (r.len - 1) / kKv8Block - *first + 1 : 0;
+}
+
+template <int D, int NT, bool SPLIT>
+struct DecShape {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kPieces = D / 32;
+  static constexpr int kSub = D >= 256 ? 1 : 256 / D;         // blocks a warp takes at a time
+  static constexpr int kBlockBytes = 32 * D;                  // K and V record
+  static constexpr int kStageBytes = kSub * kBlockBytes;
+  static constexpr int kStages = D == 512 ? 1 : 3;
+  static constexpr int kRing = kDecWarps * kStages * kStageBytes;
+  static constexpr int kLdO = D + 4;
+  static constexpr int kMerge = kDecWarps * kRows * kLdO * 4; // shares the ring's memory
+  static constexpr int kArea = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kQ = NT * kPieces * 512 * (SPLIT ? 2 : 1);
+  static constexpr int kSmem = kArea + kQ;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs a) {
+  constexpr bool kSplit = sizeof(T) == 4;
+  using S = DecShape<D, NT, kSplit>;
+  constexpr int kSub = S::kSub, kStages = S::kStages, kPieces = S::kPieces, kRows = S::kRows;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t full_bar[kDecWarps * kStages];
+  __shared__ uint64_t scan[kDecWarps], found_off;
+  __shared__ uint32_t found_b, last_flag;
+  __shared__ float row_mul[kRows], wm[kDecWarps][kRows], wl[kDecWarps][kRows];
+  __shared__ float fac[kDecWarps][kRows], row_inv[kRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  uint8_t *const qf = smem + S::kArea;
+  uint8_t *const ring = smem + warp * kStages * S::kStageBytes;
+  const uint32_t ring_u = smem_u32(ring), bar_u = smem_u32(full_bar + warp * kStages);
+  if (lane == 0) {
+    for (int s = 0; s < kStages; ++s) mbar_init(bar_u + 8 * s, 1);
+    fence_mbar_init();
   }
-  if (t < r.r0 || t >= r.r0 + r.n) return;
-  const uint32_t pos = r.len - r.n + (t - r.r0), kvh = h / (a.num_q / a.c.num_kv);
-  const uint32_t j0 = a.window && pos >= a.window ? pos - a.window + 1 : 0;
-  const T *q = static_cast<const T *>(a.q) + (size_t)t * a.q_ld + (size_t)h * D;
-  float qr[kPer], o[kPer], m = -INFINITY, l = 0.0f;
+
+  // ---- this CTA's run of the line of blocks
+  auto cost = [&](uint32_t b, Kv8Rows *r, uint32_t *first, uint32_t *count) -> uint64_t {
+    const bool ok = kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, r);
+    if (!ok) r->n = 0;
+    seen_blocks(*r, a.window, first, count);
+    const uint32_t groups = (r->n * a.gqa + kRows - 1) / kRows;
+    return (uint64_t)*count * groups * a.c.num_kv;
+  };
+  uint64_t begin, end;
+  {
+    Kv8Rows r;
+    uint32_t f, n;
+    const uint32_t per = (a.c.num_seqs + kDecThreads - 1) / kDecThreads;
+    const uint32_t b0 = threadIdx.x * per, b1 = min(a.c.num_seqs, b0 + per);
+    uint64_t mine = 0;
+    for (uint32_t b = b0; b < b1; ++b) {
+      if (blockIdx.x == 0 && !kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r))
+        raise_error(a.err, kDevBadParams);
+      mine += cost(b, &r, &f, &n);
+    }
+    uint64_t incl = mine;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    qr[i] = (float)q[32 * i + lane];
-    o[i] = 0.0f;
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    uint64_t before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    before += incl - mine;
+    uint64_t run = (total + gridDim.x - 1) / gridDim.x;
+    run = run > a.min_run ? run : a.min_run;
+    begin = run * blockIdx.x;
+    end = begin + run < total ? begin + run : total;
+    if (begin >= end) return;
+    if (begin >= before && begin < before + mine) {
+      uint64_t off = begin - before;
+      for (uint32_t b = b0; b < b1; ++b) {
+        const uint64_t n_b = cost(b, &r, &f, &n);
+        if (off < n_b) {
+          found_b = b;
+          found_off = off;
+          break;
+        }
+        off -= n_b;
+      }
+    }
+    __syncthreads();
   }
-  for (uint32_t j = j0; j <= pos; ++j) {
-    const uint32_t page = a.c.table[(size_t)b * a.c.max_pages + j / a.c.page_tokens];
-    if (page >= a.c.num_pages) {
-      if (lane == 0) raise_error(a.err, kDevBadSlot);
+  const uint64_t run = gridDim.x == 1 ? end : (blockIdx.x ? begin / blockIdx.x : end);  // run length
+
+  uint32_t issued = 0, taken = 0;  // stages of this warp's ring, over all segments
+  uint32_t b = found_b;
+  uint64_t off = found_off, at = begin;
+  bool first_seg = true;
+  while (at < end) {
+    Kv8Rows r;
+    uint32_t first, count;
+    const uint64_t n_b = cost(b, &r, &first, &count);
+    if (n_b == 0) {
+      ++b;
       continue;
     }
-    const size_t rec = (((size_t)page * a.c.num_kv + kvh) * (a.c.page_tokens / 16) + j % a.c.page_tokens / 16) * 2;
-    const uint8_t *k = static_cast<const uint8_t *>(a.c.data) + rec * (16 * D);
-    const uint32_t s = j % 16;
-    float part = 0.0f, v[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const uint32_t e = lane;
-      const uint32_t kb = k[512 * i + 16 * (4 * (s % 8) + e / 8) + 8 * (s / 8) + e % 8];
-      const uint32_t vb = k[16 * D + 512 * i + 16 * (4 * (e / 4) + s % 8 / 2) + 4 * (e % 4) + s % 2 + 2 * (s / 8)];
-      const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(kb | vb << 8), __NV_E4M3)));
-      part = fmaf(qr[i], f.x, part);
-      v[i] = f.y;
+    const uint32_t problem = (uint32_t)(off / count), groups = (r.n * a.gqa + kRows - 1) / kRows;
+    const uint32_t s0 = (uint32_t)(off % count);
+    const uint32_t s1 = end - at < count - s0 ? s0 + (uint32_t)(end - at) : count;
+    const uint32_t h = problem / groups, row0 = problem % groups * kRows;  // packed rows
+    const uint32_t rows = min((uint32_t)kRows, r.n * a.gqa - row0);
+    const uint32_t pos0 = r.len - r.n;
+    const uint32_t tok_lo = row0 / a.gqa, tok_hi = (row0 + rows - 1) / a.gqa;
+
+    // ---- copies: entry j is the warp's j-th block of the segment, 32 entries at a time in lanes
+    const uint32_t *table = a.c.table + (size_t)b * a.c.max_pages;
+    const uint32_t steps = (s1 - s0 + kDecWarps * kSub - 1) / (kDecWarps * kSub);
+    auto block_of = [&](uint32_t j) { return s0 + (j / kSub * kDecWarps + warp) * kSub + j % kSub; };
+    struct Entry {
+      uint64_t rec;  // record pair index; ~0: nothing to read
+      float ks, vs;
+    };
+    auto entry = [&](uint32_t j) -> Entry {
+      Entry e{~0ull, 0.0f, 1.0f};
+      const uint32_t s = block_of(j);
+      if (s >= s1) return e;
+      const uint32_t blk = first + s;
+      const uint32_t page = table[blk * kKv8Block / a.c.page_tokens];
+      if (page >= a.c.num_pages) {
+        raise_error(a.err, kDevBadSlot);
+        return e;
+      }
+      const uint32_t per = a.c.page_tokens / kKv8Block;
+      e.rec = ((uint64_t)page * a.c.num_kv + h) * per + blk % per;
+      const float2 f = *reinterpret_cast<const float2 *>(a.c.scale + 2 * e.rec);
+      e.ks = f.x;
+      e.vs = f.y;
+      return e;
+    };
+    Entry cur = entry(lane), nxt = entry(32 + lane);
+    uint32_t batch = 0;   // cur holds entries [32 batch, + 32)
+    uint32_t to_issue = 0;  // next step to issue
+    auto issue = [&]() {
+      const uint32_t j0 = to_issue * kSub;
+      const Entry &e = j0 / 32 == batch ? cur : nxt;
+      const bool mine = (uint32_t)lane - j0 % 32 < (uint32_t)kSub && e.rec != ~0ull;
+      const uint32_t n = __popc(__ballot_sync(0xffffffffu, mine));
+      const uint32_t st = issued % kStages;
+      if (lane == 0) mbar_arrive_expect_tx(bar_u + 8 * st, n * S::kBlockBytes);
+      __syncwarp();
+      if (mine)
+        bulk_g2s(ring_u + st * S::kStageBytes + (lane - j0 % 32) * S::kBlockBytes,
+                 static_cast<const uint8_t *>(a.c.data) + e.rec * S::kBlockBytes, S::kBlockBytes,
+                 bar_u + 8 * st);
+      ++issued;
+      ++to_issue;
+    };
+    if (!first_seg) {  // the merge of the segment before is done with the ring
+      fence_proxy_async();
+      __syncthreads();
     }
-    const float z = warp_sum(part) * a.c.scale[rec] * a.scale;
-    const float mn = fmaxf(m, z), corr = m == -INFINITY ? 0.0f : expf(m - mn);
-    const float p = expf(z - mn), pv = p * a.c.scale[rec + 1];
-    l = fmaf(l, corr, p);
+    while (to_issue < steps && to_issue < (uint32_t)kStages) issue();
+
+    // ---- q: power-of-two scaled f16 terms as B operands
+    for (uint32_t i = warp; i < (uint32_t)kRows; i += kDecWarps) {
+      float x[D / 32];
+      const uint32_t pr = row0 + i;
+      if (i < rows) {
+        const T *src = static_cast<const T *>(a.q) + (size_t)(r.r0 + pr / a.gqa) * a.q_ld +
+                       (size_t)(h * a.gqa + pr % a.gqa) * D;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) o[i] = fmaf(o[i], corr, pv * v[i]);
-    m = mn;
+        for (int k = 0; k < D / 64; ++k) {
+          float v[2];
+          load_vec<T, 2>(src + 64 * k + 2 * lane, v);
+          x[2 * k] = v[0];
+          x[2 * k + 1] = v[1];
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) x[k] = 0.0f;
+      }
+      float m = 0.0f;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) m = fmaxf(m, fabsf(x[k]));
+      m = warp_max(m);
+      int e = (int)(__float_as_uint(m) >> 23) - 127;
+      if (m == 0.0f || e == 128) e = 0;  // nothing to scale; an infinity stays one
+      e = min(max(e, -126), 126);
+      const float inv = exp2_int(-e);
+      if (lane == 0) row_mul[i] = a.scale * kLog2e * exp2_int(e);
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) {
+        const uint32_t d = 64 * k + 2 * lane;  // elements d, d + 1 of piece d / 32
+        uint8_t *dst = qf + ((i / 8) * kPieces + d / 32) * 512 + (4 * (i % 8) + d % 32 / 8) * 16 + d % 8 * 2;
+        const float v0 = x[2 * k] * inv, v1 = x[2 * k + 1] * inv;
+        const uint32_t hi = pack_f16(v0, v1);
+        *reinterpret_cast<uint32_t *>(dst) = hi;
+        if constexpr (kSplit)
+          *reinterpret_cast<uint32_t *>(dst + S::kQ / 2) = pack_f16_rest(v0, v1, hi);
+      }
+    }
+    __syncthreads();
+
+    float o[kPieces][2][NT][4], mx[NT][2], ls[NT][2], mul[NT][2];
+    uint32_t see_lo[NT][2], see_hi[NT][2];  // keys [lo, hi] of this lane's packed rows
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t i = 8 * t + 2 * c + k;
+        mul[t][k] = row_mul[i];
+        mx[t][k] = -INFINITY;
+        ls[t][k] = 0.0f;
+        const uint32_t pos = pos0 + (row0 + min(i, rows - 1)) / a.gqa;
+        see_hi[t][k] = pos;
+        see_lo[t][k] = a.window && pos >= a.window ? pos - a.window + 1 : 0;
+      }
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[p][mt][t][k] = 0.0f;
+    // blocks inside [all_lo, all_hi] are seen whole by every row
+    const uint32_t all_hi = pos0 + tok_lo;
+    const uint32_t all_lo = a.window && pos0 + tok_hi >= a.window ? pos0 + tok_hi - a.window + 1 : 0;
+
+    for (uint32_t step = 0; step < steps; ++step) {
+      const uint32_t j0 = step * kSub;
+      if (j0 / 32 != batch) {
+        cur = nxt;
+        ++batch;
+        nxt = entry(32 * (batch + 1) + lane);
+      }
+      float ks[kSub], vs[kSub];
+      bool have[kSub];
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        const int src = (int)(j0 % 32) + i;
+        ks[i] = __shfl_sync(0xffffffffu, cur.ks, src);
+        vs[i] = __shfl_sync(0xffffffffu, cur.vs, src);
+        have[i] = __shfl_sync(0xffffffffu, (int)(cur.rec != ~0ull), src) != 0;
+      }
+      const uint32_t st = taken % kStages;
+      if (!mbar_wait_bounded(bar_u + 8 * st, (taken / kStages) & 1)) raise_error(a.err, kDevWaitTimeout);
+      uint8_t *const kv = ring + st * S::kStageBytes;
+
+      // ---- S^T = K Q^T
+      float s[kSub][NT][kSplit ? 2 : 1][4];
+#pragma unroll
+      for (int i = 0; i < kSub; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int w = 0; w < (kSplit ? 2 : 1); ++w)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[i][t][w][k] = 0.0f;
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p) {
+        uint4 q[NT][kSplit ? 2 : 1];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int w = 0; w < (kSplit ? 2 : 1); ++w)
+            q[t][w] = *reinterpret_cast<const uint4 *>(qf + w * (S::kQ / 2) + (t * kPieces + p) * 512 + lane * 16);
+#pragma unroll
+        for (int i = 0; i < kSub; ++i) {
+          const uint4 k4 = *reinterpret_cast<const uint4 *>(kv + i * S::kBlockBytes + p * 512 + lane * 16);
+          const uint32_t a0[4] = {e4m3x2_f16x2(k4.x & 0xFFFF), e4m3x2_f16x2(k4.z & 0xFFFF),
+                                  e4m3x2_f16x2(k4.x >> 16), e4m3x2_f16x2(k4.z >> 16)};
+          const uint32_t a1[4] = {e4m3x2_f16x2(k4.y & 0xFFFF), e4m3x2_f16x2(k4.w & 0xFFFF),
+                                  e4m3x2_f16x2(k4.y >> 16), e4m3x2_f16x2(k4.w >> 16)};
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int w = 0; w < (kSplit ? 2 : 1); ++w) {
+              mma_f16_16816(s[i][t][w], a0, q[t][w].x, q[t][w].y);
+              mma_f16_16816(s[i][t][w], a1, q[t][w].z, q[t][w].w);
+            }
+        }
+      }
+
+      // ---- scores, masks, running maximum
+      float lv[kSub], top[NT][2];
+      uint32_t keep_v[kSub];  // V bytes of this lane's tokens that count (all but in masked blocks)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) top[t][0] = top[t][1] = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        lv[i] = (float)kv8_scale_exponent(vs[i]);
+        keep_v[i] = 0xFFFFFFFFu;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float x = s[i][t][0][k];
+            if constexpr (kSplit) x += s[i][t][1][k];
+            s[i][t][0][k] = fmaf(x * ks[i], mul[t][k & 1], lv[i]);
+          }
+        const uint32_t key0 = (first + block_of(j0 + i)) * kKv8Block;
+        if (!have[i] || key0 < all_lo || key0 + kKv8Block - 1 > all_hi) {
+          // Some row does not see all of the block.  A token no row sees is taken out of V (its
+          // bytes may be anything); one whose V holds a NaN is taken out too and makes the
+          // rows that do see it NaN.
+          uint32_t nan = 0;
+          if (have[i]) {
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) {
+              const uint4 v = *reinterpret_cast<const uint4 *>(kv + i * S::kBlockBytes + 16 * D + p * 512 + lane * 16);
+              nan |= ((v.x & 0x7F7F7F7Fu) + 0x01010101u) | ((v.y & 0x7F7F7F7Fu) + 0x01010101u) |
+                     ((v.z & 0x7F7F7F7Fu) + 0x01010101u) | ((v.w & 0x7F7F7F7Fu) + 0x01010101u);
+            }
+            nan &= 0x80808080u;
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) nan |= __shfl_xor_sync(0xffffffffu, nan, w);
+            keep_v[i] = ~((nan >> 7) * 0xFFu);
+          } else {
+            keep_v[i] = 0;
+          }
+          // token g is byte g % 2 of the lanes with c = g / 2, token g + 8 two bytes on
+          const uint32_t nan_g = __shfl_sync(0xffffffffu, nan, g / 2) >> (8 * (g & 1));
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t key = key0 + g + (k >> 1) * 8;
+              const bool seen = have[i] && key >= see_lo[t][k & 1] && key <= see_hi[t][k & 1];
+              float x = s[i][t][0][k];
+              if ((nan_g >> (16 * (k >> 1))) & 0x80u) x = NAN;
+              s[i][t][0][k] = seen ? x : -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top[t][k & 1] = fmaxf(top[t][k & 1], s[i][t][0][k]);
+      }
+      bool moved = false;
+      float shift[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float m = top[t][k];
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+          top[t][k] = fmaxf(m, mx[t][k]);
+          moved |= top[t][k] != mx[t][k];
+          shift[t][k] = top[t][k] == -INFINITY ? 0.0f : top[t][k] - kPOffset;
+        }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float f = mx[t][k] == -INFINITY ? 0.0f : ex2(mx[t][k] - top[t][k]);
+            mx[t][k] = top[t][k];
+            ls[t][k] *= f;
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) {
+                o[p][mt][t][k] *= f;
+                o[p][mt][t][k + 2] *= f;
+              }
+          }
+      }
+
+      // ---- P^T as B operands
+      uint32_t pb[kSub][NT][kSplit ? 2 : 1][2];
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) {
+        const float unv = ex2(-lv[i]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float pr[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) pr[k] = ex2(s[i][t][0][k] - shift[t][k & 1]);
+          ls[t][0] = fmaf(pr[0] + pr[2], unv, ls[t][0]);
+          ls[t][1] = fmaf(pr[1] + pr[3], unv, ls[t][1]);
+          const uint32_t p0 = pack_f16(pr[0], pr[1]), p1 = pack_f16(pr[2], pr[3]);
+          pb[i][t][0][0] = movmatrix_trans(p0);
+          pb[i][t][0][1] = movmatrix_trans(p1);
+          if constexpr (kSplit) {
+            pb[i][t][1][0] = movmatrix_trans(pack_f16_rest(pr[0], pr[1], p0));
+            pb[i][t][1][1] = movmatrix_trans(pack_f16_rest(pr[2], pr[3], p1));
+          }
+        }
+      }
+
+      // ---- O^T += V^T P^T
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+        for (int i = 0; i < kSub; ++i) {
+          uint4 v = *reinterpret_cast<const uint4 *>(kv + i * S::kBlockBytes + 16 * D + p * 512 + lane * 16);
+          v.x &= keep_v[i]; v.y &= keep_v[i]; v.z &= keep_v[i]; v.w &= keep_v[i];
+          const uint32_t a0[4] = {e4m3x2_f16x2(v.x & 0xFFFF), e4m3x2_f16x2(v.y & 0xFFFF),
+                                  e4m3x2_f16x2(v.x >> 16), e4m3x2_f16x2(v.y >> 16)};
+          const uint32_t a1[4] = {e4m3x2_f16x2(v.z & 0xFFFF), e4m3x2_f16x2(v.w & 0xFFFF),
+                                  e4m3x2_f16x2(v.z >> 16), e4m3x2_f16x2(v.w >> 16)};
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int w = 0; w < (kSplit ? 2 : 1); ++w) {
+              mma_f16_16816(o[p][0][t], a0, pb[i][t][w][0], pb[i][t][w][1]);
+              mma_f16_16816(o[p][1][t], a1, pb[i][t][w][0], pb[i][t][w][1]);
+            }
+        }
+      ++taken;
+      __syncwarp();
+      if (to_issue < steps) issue();
+    }
+
+    // ---- merge the warps
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float l = ls[t][k];
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+        if (g == 0) {
+          wm[warp][8 * t + 2 * c + k] = mx[t][k];
+          wl[warp][8 * t + 2 * c + k] = l;
+        }
+      }
+    __syncthreads();  // every warp's ring is free
+    float *const mo = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          *reinterpret_cast<float4 *>(mo + (size_t)(warp * kRows + 8 * t + 2 * c + k) * S::kLdO + 32 * p + 4 * g) =
+              make_float4(o[p][0][t][k], o[p][0][t][k + 2], o[p][1][t][k], o[p][1][t][k + 2]);
+    const bool whole = s0 == 0 && s1 == count;
+    const uint32_t slot = 2 * blockIdx.x + (first_seg ? 0 : 1);
+    float *const part_ml = a.part, *const part_o = a.part + (size_t)2 * gridDim.x * kRows * 2;
+    if (threadIdx.x < kRows) {
+      const uint32_t i = threadIdx.x;
+      float m = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) m = fmaxf(m, wm[w][i]);
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) {
+        const float f = wm[w][i] == -INFINITY ? 0.0f : ex2(wm[w][i] - m);
+        fac[w][i] = f;
+        l += wl[w][i] * f;
+      }
+      if (whole) {
+        row_inv[i] = l == 0.0f ? 0.0f : 1.0f / l;
+      } else {
+        row_inv[i] = 1.0f;
+        part_ml[((size_t)slot * kRows + i) * 2] = m;
+        part_ml[((size_t)slot * kRows + i) * 2 + 1] = l;
+      }
+    }
+    __syncthreads();
+    auto out_row = [&](uint32_t i) {
+      const uint32_t pr = row0 + i;
+      return static_cast<T *>(a.out) + (size_t)(r.r0 + pr / a.gqa) * a.out_ld + (size_t)(h * a.gqa + pr % a.gqa) * D;
+    };
+    for (uint32_t x = threadIdx.x; x < rows * (D / 4); x += kDecThreads) {
+      const uint32_t i = x / (D / 4), d = x % (D / 4) * 4;
+      float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int w = 0; w < kDecWarps; ++w) {
+        const float4 v = *reinterpret_cast<const float4 *>(mo + (size_t)(w * kRows + i) * S::kLdO + d);
+        const float f = fac[w][i];
+        sum.x = fmaf(v.x, f, sum.x);
+        sum.y = fmaf(v.y, f, sum.y);
+        sum.z = fmaf(v.z, f, sum.z);
+        sum.w = fmaf(v.w, f, sum.w);
+      }
+      if (whole) {
+        const float inv = row_inv[i], y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+        store_vec<T, 4>(out_row(i) + d, y);
+      } else {
+        *reinterpret_cast<float4 *>(part_o + ((size_t)slot * kRows + i) * D + d) = sum;
+      }
+    }
+    if (!whole) {
+      // CTAs c0 .. c1 hold parts of this problem; c0 counts them
+      const uint64_t p0 = at - s0;  // where the problem begins on the line
+      const uint32_t c0 = (uint32_t)(p0 / run), c1 = (uint32_t)((p0 + count - 1) / run);
+      const uint32_t slot0 = 2 * c0 + (p0 > run * c0 ? 1 : 0);
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) last_flag = atomicAdd(a.cnt + c0, 1u) == c1 - c0;
+      __syncthreads();
+      if (last_flag) {
+        __threadfence();
+        auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : 2 * (c0 + k); };
+        const uint32_t n = c1 - c0 + 1;
+        // one warp per row for the maxima, then all threads over the rows' elements
+        for (uint32_t i = warp; i < rows; i += kDecWarps) {
+          float m = -INFINITY, l = 0.0f;
+          for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, __ldcg(part_ml + ((size_t)slot_of(k) * kRows + i) * 2));
+          m = warp_max(m);
+          for (uint32_t k = lane; k < n; k += 32) {
+            const float *ml = part_ml + ((size_t)slot_of(k) * kRows + i) * 2;
+            const float mk = __ldcg(ml);
+            l += __ldcg(ml + 1) * (mk == -INFINITY ? 0.0f : ex2(mk - m));
+          }
+          l = warp_sum(l);
+          if (lane == 0) {
+            wm[0][i] = m;
+            row_inv[i] = l == 0.0f ? 0.0f : 1.0f / l;
+          }
+        }
+        __syncthreads();
+        for (uint32_t x = threadIdx.x; x < rows * (D / 4); x += kDecThreads) {
+          const uint32_t i = x / (D / 4), d = x % (D / 4) * 4;
+          const float m = wm[0][i];
+          float4 sum = make_float4(0, 0, 0, 0);
+          for (uint32_t k = 0; k < n; ++k) {
+            const float mk = __ldcg(part_ml + ((size_t)slot_of(k) * kRows + i) * 2);
+            const float f = mk == -INFINITY ? 0.0f : ex2(mk - m);
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_o + ((size_t)slot_of(k) * kRows + i) * D + d));
+            sum.x = fmaf(v.x, f, sum.x);
+            sum.y = fmaf(v.y, f, sum.y);
+            sum.z = fmaf(v.z, f, sum.z);
+            sum.w = fmaf(v.w, f, sum.w);
+          }
+          const float inv = row_inv[i], y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+          store_vec<T, 4>(out_row(i) + d, y);
+        }
+        if (threadIdx.x == 0) a.cnt[c0] = 0;
+      }
+    }
+    first_seg = false;
+    at += s1 - s0;
+    off += s1 - s0;
+    if (off == n_b) {
+      off = 0;
+      ++b;
+    }
   }
-  T *out = static_cast<T *>(a.out) + (size_t)t * a.out_ld + (size_t)h * D;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) out[32 * i + lane] = (T)(l == 0.0f ? 0.0f : o[i] / l);
 }
 
 using AttnKernel = void (*)(Kv8AttnArgs);
-AttnKernel attn_kernel(sx_dtype t, uint32_t d) {
-  if (t == SX_F32)
-    return d == 64 ? kv8_attn_kernel<float, 64> : d == 128 ? kv8_attn_kernel<float, 128>
-         : d == 256 ? kv8_attn_kernel<float, 256> : kv8_attn_kernel<float, 512>;
-  return d == 64 ? kv8_attn_kernel<__nv_bfloat16, 64> : d == 128 ? kv8_attn_kernel<__nv_bfloat16, 128>
-       : d == 256 ? kv8_attn_kernel<__nv_bfloat16, 256> : kv8_attn_kernel<__nv_bfloat16, 512>;
+struct DecVariant {
+  AttnKernel fn;
+  uint32_t smem, rows;
+};
+template <typename T, int D, int NT>
+DecVariant variant() {
+  return {kv8_decode_kernel<T, D, NT>, (uint32_t)DecShape<D, NT, sizeof(T) == 4>::kSmem, 8 * NT};
+}
+// Variant i (0, 1, 2: 8, 16, 32 packed rows) of a head size: the output of 8 NT rows takes
+// D NT / 4 registers per thread, of which there may be 128.
+template <typename T>
+DecVariant variant(uint32_t d, uint32_t i) {
+  switch (d) {
+    case 64: return i == 0 ? variant<T, 64, 1>() : i == 1 ? variant<T, 64, 2>() : variant<T, 64, 4>();
+    case 128: return i == 0 ? variant<T, 128, 1>() : i == 1 ? variant<T, 128, 2>() : variant<T, 128, 4>();
+    case 256: return i == 0 ? variant<T, 256, 1>() : variant<T, 256, 2>();
+    default: return variant<T, 512, 1>();
+  }
+}
+DecVariant dec_variant(sx_dtype t, uint32_t d, uint32_t i) {
+  return t == SX_F32 ? variant<float>(d, i) : variant<__nv_bfloat16>(d, i);
 }
 
+constexpr uint32_t kMinRun = 16;  // blocks: two per warp
+
 }  // namespace
+
+// Two partial results per CTA of the decode kernel, each up to 4096 / head_dim rows.
+size_t kv8_part_bytes(int num_sms) { return (size_t)2 * num_sms * (64 * 2 + 4096) * sizeof(float); }
+
+cudaError_t prepare_kv8_attn() {
+  for (uint32_t d : {64u, 128u, 256u, 512u})
+    for (sx_dtype t : {SX_F32, SX_BF16})
+      for (uint32_t i = 0; i < 3; ++i) {
+        const DecVariant v = dec_variant(t, d, i);
+        const cudaError_t e = cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem);
+        if (e != cudaSuccess) return e;
+      }
+  return cudaSuccess;
+}
+
 }  // namespace sx
 
 extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, sx_dtype t,
@@ -108,7 +680,26 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
   if (tokens == 0 || c->num_seqs == 0) return SX_OK;
   cudaError_t ce = cudaSetDevice(e->device);
   if (ce != cudaSuccess) return sx_host_cuda_status(ce, "cudaSetDevice");
-  sx::Kv8AttnArgs a{*c, q, out, q_ld, out_ld, row_start, kv_len, tokens, num_q, window, scale, e->err_dev};
-  sx::attn_kernel(t, c->head_dim)<<<dim3(tokens, (num_q + 3) / 4), 128, 0, e->stream>>>(a);
+  sx::Kv8AttnArgs a{};
+  a.c = *c;
+  a.q = q;
+  a.out = out;
+  a.q_ld = q_ld;
+  a.out_ld = out_ld;
+  a.row_start = row_start;
+  a.kv_len = kv_len;
+  a.tokens = tokens;
+  a.num_q = num_q;
+  a.window = window;
+  a.gqa = num_q / c->num_kv;
+  a.min_run = sx::kMinRun;
+  a.scale = scale;
+  a.part = e->kv8_part;
+  a.cnt = e->kv8_cnt;
+  a.err = e->err_dev;
+  // packed rows of an average sequence
+  const uint64_t avg = (uint64_t)((tokens + c->num_seqs - 1) / c->num_seqs) * a.gqa;
+  const sx::DecVariant v = sx::dec_variant(t, c->head_dim, avg <= 8 ? 0 : avg <= 16 ? 1 : 2);
+  v.fn<<<e->num_sms, sx::kDecThreads, v.smem, e->stream>>>(a);
   return sx_host_cuda_status(cudaGetLastError(), "kv8_attn launch");
 }
