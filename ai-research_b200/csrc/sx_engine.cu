@@ -614,7 +614,7 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
       size_t o_amax = take(sx::argmax_scratch_bytes());
       size_t o_pbar = take(256);
       size_t o_kpart = take(sx::kv8_part_bytes(e->num_sms));
-      size_t o_kcnt = take((size_t)e->num_sms * 4);
+      size_t o_kcnt = take((size_t)e->num_sms * 2 * 4);
       e->scratch_bytes = off;
       st = cuda_status(cudaMalloc(&e->scratch, e->scratch_bytes), "engine scratch");
       if (st) break;

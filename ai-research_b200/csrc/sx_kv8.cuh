@@ -70,10 +70,13 @@ SX_DEV uint32_t e4m3_pack4(float a, float b, float c, float d) {
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
   return lo | hi << 16;
 }
-// two e4m3 bytes -> f16x2 (exact)
-SX_DEV uint32_t e4m3x2_f16x2(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-  return (uint32_t)h.x | (uint32_t)h.y << 16;
+// four e4m3 bytes -> two f16x2 (exact).  The conversion takes a register's half as it is: half a
+// cycle per SM and pair, against 1.5 when the half is first cut out in 32 bits.
+SX_DEV void e4m3x4_f16(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %2;\n cvt.rn.f16x2.e4m3x2 %0, l;\n"
+      " cvt.rn.f16x2.e4m3x2 %1, h;\n}\n"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 SX_DEV float4 e4m3_unpack4(uint32_t w) {
   const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);

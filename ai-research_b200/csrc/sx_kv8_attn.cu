@@ -16,19 +16,22 @@
 // largest contribution; the softmax's sum takes p' / v scale in f32.
 //
 // Split: the batch's work is a line of 16-token blocks -- for each sequence, kv head and group of
-// packed rows the blocks it sees -- cut into equal runs, one per CTA, computed on the device from
-// the lengths, so a ragged batch and one long sequence balance alike.  The warps of a CTA take
-// blocks in turn, each with its own ring of bulk copies and its own maximum, sum and output; they
-// merge in shared memory at the end of a problem, and CTAs that share a problem through the
-// workspace: the last to arrive merges (its order is that of the CTAs, so results repeat).
+// packed rows the blocks it sees and kOverhead more, for what starting and ending it costs -- cut
+// into equal runs, one per CTA, computed on the device from the lengths, so a ragged batch and one
+// long sequence balance alike.  The warps of a CTA take blocks in turn, each with its own ring of
+// bulk copies (a K or a V record a stage) and its own maximum, sum and output; they merge in shared
+// memory at the end of a problem, and CTAs that share a problem through the workspace: the last to
+// arrive merges (its order is that of the CTAs, so results repeat).
 #include "sx_host.h"
 #include "sx_kv8.cuh"
+#include "sx_launch.cuh"
 
 namespace sx {
 namespace {
 
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
+constexpr uint32_t kOverhead = 8;  // blocks a problem's start and end are worth
 constexpr float kPOffset = 10.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -59,6 +62,13 @@ SX_DEV uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&h);
 }
+// Count an arrival on behalf of a CTA whose threads met at a barrier before: their writes are
+// released by it, and those of the CTAs counted before are acquired.
+SX_DEV uint32_t arrive_acq_rel(uint32_t *cnt) {
+  uint32_t r;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;\n" : "=r"(r) : "l"(cnt) : "memory");
+  return r;
+}
 // what f16 rounding left of the pair
 SX_DEV uint32_t pack_f16_rest(float lo, float hi, uint32_t rounded) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&rounded));
@@ -72,120 +82,122 @@ SX_DEV void seen_blocks(const Kv8Rows &r, uint32_t window, uint32_t *first, uint
   *count = r.n ? (r.len - 1) / kKv8Block - *first + 1 : 0;
 }
 
+// Shapes of the kernel for head size D and 8 NT packed rows.  The output takes D NT / 4 registers
+// per thread: up to 64 two CTAs fit an SM and hide each other's starts and ends, with 128 one.
 template <int D, int NT, bool SPLIT>
 struct DecShape {
   static constexpr int kRows = 8 * NT;
   static constexpr int kPieces = D / 32;
-  static constexpr int kSub = D >= 256 ? 1 : 256 / D;         // blocks a warp takes at a time
-  static constexpr int kBlockBytes = 32 * D;                  // K and V record
-  static constexpr int kStageBytes = kSub * kBlockBytes;
-  static constexpr int kStages = D == 512 ? 1 : 3;
-  static constexpr int kRing = kDecWarps * kStages * kStageBytes;
+  static constexpr int kCtas = D * NT <= 256 ? 2 : 1;         // per SM
+  static constexpr int kSub = D * NT >= 256 ? 1 : 256 / (D * NT);  // blocks a warp takes at a time
+  static constexpr int kRecord = 16 * D;
+  static constexpr int kStageBytes = kSub * kRecord;
+  static constexpr int kRing = (kCtas == 2 ? 12 : 24) * 1024; // of one warp
+  static constexpr int kStages = kRing / kStageBytes;
   static constexpr int kLdO = D + 4;
-  static constexpr int kMerge = kDecWarps * kRows * kLdO * 4; // shares the ring's memory
-  static constexpr int kArea = kRing > kMerge ? kRing : kMerge;
+  static constexpr int kMerge = kDecWarps * kRows * kLdO * 4; // shares the rings' memory
+  static constexpr int kArea = kDecWarps * kRing > kMerge ? kDecWarps * kRing : kMerge;
   static constexpr int kQ = NT * kPieces * 512 * (SPLIT ? 2 : 1);
   static constexpr int kSmem = kArea + kQ;
 };
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs a) {
+__global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>::kCtas))
+    kv8_decode_kernel(Kv8AttnArgs a) {
   constexpr bool kSplit = sizeof(T) == 4;
   using S = DecShape<D, NT, kSplit>;
   constexpr int kSub = S::kSub, kStages = S::kStages, kPieces = S::kPieces, kRows = S::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t full_bar[kDecWarps * kStages];
-  __shared__ uint64_t scan[kDecWarps], found_off;
-  __shared__ uint32_t found_b, last_flag;
+  __shared__ uint32_t last_flag;
   __shared__ float row_mul[kRows], wm[kDecWarps][kRows], wl[kDecWarps][kRows];
   __shared__ float fac[kDecWarps][kRows], row_inv[kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   uint8_t *const qf = smem + S::kArea;
-  uint8_t *const ring = smem + warp * kStages * S::kStageBytes;
+  uint8_t *const ring = smem + warp * S::kRing;
   const uint32_t ring_u = smem_u32(ring), bar_u = smem_u32(full_bar + warp * kStages);
   if (lane == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(bar_u + 8 * s, 1);
     fence_mbar_init();
   }
 
-  // ---- this CTA's run of the line of blocks
-  auto cost = [&](uint32_t b, Kv8Rows *r, uint32_t *first, uint32_t *count) -> uint64_t {
-    const bool ok = kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, r);
-    if (!ok) r->n = 0;
-    seen_blocks(*r, a.window, first, count);
-    const uint32_t groups = (r->n * a.gqa + kRows - 1) / kRows;
-    return (uint64_t)*count * groups * a.c.num_kv;
+  __syncwarp();
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- this CTA's run of the line of blocks; every warp finds it alike
+  auto problems_of = [&](const Kv8Rows &r) {
+    return (r.n * a.gqa + kRows - 1) / kRows * a.c.num_kv;
   };
-  uint64_t begin, end;
-  {
+  auto cost = [&](uint32_t b) -> uint64_t {
     Kv8Rows r;
-    uint32_t f, n;
-    const uint32_t per = (a.c.num_seqs + kDecThreads - 1) / kDecThreads;
-    const uint32_t b0 = threadIdx.x * per, b1 = min(a.c.num_seqs, b0 + per);
-    uint64_t mine = 0;
-    for (uint32_t b = b0; b < b1; ++b) {
-      if (blockIdx.x == 0 && !kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r))
-        raise_error(a.err, kDevBadParams);
-      mine += cost(b, &r, &f, &n);
+    if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r)) {
+      if (blockIdx.x == 0 && warp == 0) raise_error(a.err, kDevBadParams);
+      return 0;
     }
+    uint32_t first, count;
+    seen_blocks(r, a.window, &first, &count);
+    return r.n ? (uint64_t)(count + kOverhead) * problems_of(r) : 0;
+  };
+  uint64_t begin, end, run, at;  // at: where the sequence of the next problem starts
+  uint32_t b;
+  {
+    const uint32_t per = (a.c.num_seqs + 31) / 32;
+    const uint32_t b0 = lane * per, b1 = min(a.c.num_seqs, b0 + per);
+    uint64_t mine = 0;
+    for (uint32_t i = b0; i < b1; ++i) mine += cost(i);
     uint64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    if (lane == 31) scan[warp] = incl;
-    __syncthreads();
-    uint64_t before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-      if (w < warp) before += scan[w];
-      total += scan[w];
-    }
-    before += incl - mine;
-    uint64_t run = (total + gridDim.x - 1) / gridDim.x;
+    const uint64_t total = __shfl_sync(0xffffffffu, incl, 31);
+    run = (total + gridDim.x - 1) / gridDim.x;
     run = run > a.min_run ? run : a.min_run;
     begin = run * blockIdx.x;
     end = begin + run < total ? begin + run : total;
     if (begin >= end) return;
-    if (begin >= before && begin < before + mine) {
-      uint64_t off = begin - before;
-      for (uint32_t b = b0; b < b1; ++b) {
-        const uint64_t n_b = cost(b, &r, &f, &n);
-        if (off < n_b) {
-          found_b = b;
-          found_off = off;
-          break;
-        }
-        off -= n_b;
+    const uint32_t who = __popc(__ballot_sync(0xffffffffu, incl <= begin));  // its lane holds begin
+    at = incl - mine;
+    b = b0;
+    if (lane == (int)who)
+      for (uint64_t n; (n = cost(b)) <= begin - at; at += n) ++b;
+    at = __shfl_sync(0xffffffffu, at, who);
+    b = __shfl_sync(0xffffffffu, b, who);
+  }
+
+  uint32_t issued = 0, taken = 0;  // stages of this warp's ring, over all problems
+  Kv8Rows r;
+  uint32_t first = 0, count = 0, left = 0, problem = 0;  // problems of b that are left
+  bool fresh = true;  // the first sequence: its first problems may lie before the run
+  bool merged = false;
+  for (; at < end; at += count + kOverhead, --left, ++problem) {
+    while (left == 0) {  // the next sequence with rows
+      const bool ok = kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r);
+      ++b;
+      if (!ok || r.n == 0) continue;
+      seen_blocks(r, a.window, &first, &count);
+      left = problems_of(r);
+      problem = 0;
+      if (fresh) {
+        problem = (uint32_t)((begin - at) / (count + kOverhead));
+        left -= problem;
+        at += (uint64_t)problem * (count + kOverhead);
+        fresh = false;
       }
     }
-    __syncthreads();
-  }
-  const uint64_t run = gridDim.x == 1 ? end : (blockIdx.x ? begin / blockIdx.x : end);  // run length
-
-  uint32_t issued = 0, taken = 0;  // stages of this warp's ring, over all segments
-  uint32_t b = found_b;
-  uint64_t off = found_off, at = begin;
-  bool first_seg = true;
-  while (at < end) {
-    Kv8Rows r;
-    uint32_t first, count;
-    const uint64_t n_b = cost(b, &r, &first, &count);
-    if (n_b == 0) {
-      ++b;
-      continue;
-    }
-    const uint32_t problem = (uint32_t)(off / count), groups = (r.n * a.gqa + kRows - 1) / kRows;
-    const uint32_t s0 = (uint32_t)(off % count);
-    const uint32_t s1 = end - at < count - s0 ? s0 + (uint32_t)(end - at) : count;
+    const uint32_t s0 = begin > at ? (uint32_t)(begin - at) : 0;
+    const uint32_t s1 = end - at < count ? (uint32_t)(end - at) : count;
+    if (s0 >= s1) continue;  // only its overhead lies in the run
+    const uint32_t groups = (r.n * a.gqa + kRows - 1) / kRows;
     const uint32_t h = problem / groups, row0 = problem % groups * kRows;  // packed rows
     const uint32_t rows = min((uint32_t)kRows, r.n * a.gqa - row0);
     const uint32_t pos0 = r.len - r.n;
     const uint32_t tok_lo = row0 / a.gqa, tok_hi = (row0 + rows - 1) / a.gqa;
 
     // ---- copies: entry j is the warp's j-th block of the segment, 32 entries at a time in lanes
-    const uint32_t *table = a.c.table + (size_t)b * a.c.max_pages;
+    const uint32_t *table = a.c.table + (size_t)(b - 1) * a.c.max_pages;
     const uint32_t steps = (s1 - s0 + kDecWarps * kSub - 1) / (kDecWarps * kSub);
     auto block_of = [&](uint32_t j) { return s0 + (j / kSub * kDecWarps + warp) * kSub + j % kSub; };
     struct Entry {
@@ -209,48 +221,51 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs 
       e.vs = f.y;
       return e;
     };
+    // rows of q come first: their loads run beside the page table's
+    float qx[(kRows + kDecWarps - 1) / kDecWarps][D / 32];
+#pragma unroll
+    for (int i = 0; i < kRows / kDecWarps; ++i) {
+      const uint32_t pr = row0 + warp + i * kDecWarps;
+      const bool in = warp + i * kDecWarps < rows;
+      const T *src = static_cast<const T *>(a.q) + (size_t)(r.r0 + pr / a.gqa) * a.q_ld +
+                     (size_t)(h * a.gqa + pr % a.gqa) * D;
+#pragma unroll
+      for (int k = 0; k < D / 64; ++k) {
+        float v[2] = {0.0f, 0.0f};
+        if (in) load_vec<T, 2>(src + 64 * k + 2 * lane, v);
+        qx[i][2 * k] = v[0];
+        qx[i][2 * k + 1] = v[1];
+      }
+    }
     Entry cur = entry(lane), nxt = entry(32 + lane);
-    uint32_t batch = 0;   // cur holds entries [32 batch, + 32)
-    uint32_t to_issue = 0;  // next step to issue
+    uint32_t batch = 0;     // cur holds entries [32 batch, + 32)
+    uint32_t to_issue = 0;  // next record to issue: 2 step (K), 2 step + 1 (V)
     auto issue = [&]() {
-      const uint32_t j0 = to_issue * kSub;
+      const uint32_t j0 = to_issue / 2 * kSub;
       const Entry &e = j0 / 32 == batch ? cur : nxt;
       const bool mine = (uint32_t)lane - j0 % 32 < (uint32_t)kSub && e.rec != ~0ull;
       const uint32_t n = __popc(__ballot_sync(0xffffffffu, mine));
       const uint32_t st = issued % kStages;
-      if (lane == 0) mbar_arrive_expect_tx(bar_u + 8 * st, n * S::kBlockBytes);
+      if (lane == 0) mbar_arrive_expect_tx(bar_u + 8 * st, n * S::kRecord);
       __syncwarp();
       if (mine)
-        bulk_g2s(ring_u + st * S::kStageBytes + (lane - j0 % 32) * S::kBlockBytes,
-                 static_cast<const uint8_t *>(a.c.data) + e.rec * S::kBlockBytes, S::kBlockBytes,
-                 bar_u + 8 * st);
+        bulk_g2s(ring_u + st * S::kStageBytes + (lane - j0 % 32) * S::kRecord,
+                 static_cast<const uint8_t *>(a.c.data) + (2 * e.rec + (to_issue & 1)) * S::kRecord,
+                 S::kRecord, bar_u + 8 * st);
       ++issued;
       ++to_issue;
     };
-    if (!first_seg) {  // the merge of the segment before is done with the ring
+    if (merged) {  // the merge of the problem before is done with the ring
       fence_proxy_async();
       __syncthreads();
     }
-    while (to_issue < steps && to_issue < (uint32_t)kStages) issue();
+    while (to_issue < 2 * steps && to_issue < (uint32_t)kStages) issue();
 
     // ---- q: power-of-two scaled f16 terms as B operands
-    for (uint32_t i = warp; i < (uint32_t)kRows; i += kDecWarps) {
-      float x[D / 32];
-      const uint32_t pr = row0 + i;
-      if (i < rows) {
-        const T *src = static_cast<const T *>(a.q) + (size_t)(r.r0 + pr / a.gqa) * a.q_ld +
-                       (size_t)(h * a.gqa + pr % a.gqa) * D;
 #pragma unroll
-        for (int k = 0; k < D / 64; ++k) {
-          float v[2];
-          load_vec<T, 2>(src + 64 * k + 2 * lane, v);
-          x[2 * k] = v[0];
-          x[2 * k + 1] = v[1];
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) x[k] = 0.0f;
-      }
+    for (int ii = 0; ii < kRows / kDecWarps; ++ii) {
+      const uint32_t i = warp + ii * kDecWarps;
+      const float (&x)[D / 32] = qx[ii];
       float m = 0.0f;
 #pragma unroll
       for (int k = 0; k < D / 32; ++k) m = fmaxf(m, fabsf(x[k]));
@@ -315,18 +330,27 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs 
         vs[i] = __shfl_sync(0xffffffffu, cur.vs, src);
         have[i] = __shfl_sync(0xffffffffu, (int)(cur.rec != ~0ull), src) != 0;
       }
-      const uint32_t st = taken % kStages;
-      if (!mbar_wait_bounded(bar_u + 8 * st, (taken / kStages) & 1)) raise_error(a.err, kDevWaitTimeout);
-      uint8_t *const kv = ring + st * S::kStageBytes;
+      auto stage = [&]() -> uint8_t * {  // the next record, once it is there
+        const uint32_t st = taken % kStages;
+        if (!mbar_wait_bounded(bar_u + 8 * st, (taken / kStages) & 1)) raise_error(a.err, kDevWaitTimeout);
+        ++taken;
+        return ring + st * S::kStageBytes;
+      };
+      auto release = [&]() {  // a record has been read: its stage takes the next copy
+        __syncwarp();
+        if (to_issue < 2 * steps) issue();
+      };
+      const uint8_t *const kr = stage();
 
       // ---- S^T = K Q^T
-      float s[kSub][NT][kSplit ? 2 : 1][4];
+      // (two chains of accumulators: an MMA's result is 24 cycles away)
+      float s[kSub][NT][2][4];
 #pragma unroll
       for (int i = 0; i < kSub; ++i)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int w = 0; w < (kSplit ? 2 : 1); ++w)
+          for (int w = 0; w < 2; ++w)
 #pragma unroll
             for (int k = 0; k < 4; ++k) s[i][t][w][k] = 0.0f;
 #pragma unroll
@@ -339,37 +363,37 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs 
             q[t][w] = *reinterpret_cast<const uint4 *>(qf + w * (S::kQ / 2) + (t * kPieces + p) * 512 + lane * 16);
 #pragma unroll
         for (int i = 0; i < kSub; ++i) {
-          const uint4 k4 = *reinterpret_cast<const uint4 *>(kv + i * S::kBlockBytes + p * 512 + lane * 16);
-          const uint32_t a0[4] = {e4m3x2_f16x2(k4.x & 0xFFFF), e4m3x2_f16x2(k4.z & 0xFFFF),
-                                  e4m3x2_f16x2(k4.x >> 16), e4m3x2_f16x2(k4.z >> 16)};
-          const uint32_t a1[4] = {e4m3x2_f16x2(k4.y & 0xFFFF), e4m3x2_f16x2(k4.w & 0xFFFF),
-                                  e4m3x2_f16x2(k4.y >> 16), e4m3x2_f16x2(k4.w >> 16)};
+          const uint4 k4 = *reinterpret_cast<const uint4 *>(kr + i * S::kRecord + p * 512 + lane * 16);
+          uint32_t a0[4], a1[4];
+          e4m3x4_f16(k4.x, a0[0], a0[2]);
+          e4m3x4_f16(k4.y, a1[0], a1[2]);
+          e4m3x4_f16(k4.z, a0[1], a0[3]);
+          e4m3x4_f16(k4.w, a1[1], a1[3]);
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int w = 0; w < (kSplit ? 2 : 1); ++w) {
-              mma_f16_16816(s[i][t][w], a0, q[t][w].x, q[t][w].y);
-              mma_f16_16816(s[i][t][w], a1, q[t][w].z, q[t][w].w);
+              mma_f16_16816(s[i][t][0], a0, q[t][w].x, q[t][w].y);
+              mma_f16_16816(s[i][t][1], a1, q[t][w].z, q[t][w].w);
             }
         }
       }
 
+      release();
+
       // ---- scores, masks, running maximum
+      uint8_t *const vr = stage();
       float lv[kSub], top[NT][2];
-      uint32_t keep_v[kSub];  // V bytes of this lane's tokens that count (all but in masked blocks)
 #pragma unroll
       for (int t = 0; t < NT; ++t) top[t][0] = top[t][1] = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kSub; ++i) {
         lv[i] = (float)kv8_scale_exponent(vs[i]);
-        keep_v[i] = 0xFFFFFFFFu;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            float x = s[i][t][0][k];
-            if constexpr (kSplit) x += s[i][t][1][k];
-            s[i][t][0][k] = fmaf(x * ks[i], mul[t][k & 1], lv[i]);
+            s[i][t][0][k] = fmaf((s[i][t][0][k] + s[i][t][1][k]) * ks[i], mul[t][k & 1], lv[i]);
           }
         const uint32_t key0 = (first + block_of(j0 + i)) * kKv8Block;
         if (!have[i] || key0 < all_lo || key0 + kKv8Block - 1 > all_hi) {
@@ -377,19 +401,29 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs 
           // bytes may be anything); one whose V holds a NaN is taken out too and makes the
           // rows that do see it NaN.
           uint32_t nan = 0;
+          uint4 *const own = reinterpret_cast<uint4 *>(vr + i * S::kRecord) + lane;  // + 32 p
           if (have[i]) {
 #pragma unroll
             for (int p = 0; p < kPieces; ++p) {
-              const uint4 v = *reinterpret_cast<const uint4 *>(kv + i * S::kBlockBytes + 16 * D + p * 512 + lane * 16);
+              const uint4 v = own[32 * p];
               nan |= ((v.x & 0x7F7F7F7Fu) + 0x01010101u) | ((v.y & 0x7F7F7F7Fu) + 0x01010101u) |
                      ((v.z & 0x7F7F7F7Fu) + 0x01010101u) | ((v.w & 0x7F7F7F7Fu) + 0x01010101u);
             }
             nan &= 0x80808080u;
 #pragma unroll
             for (int w = 4; w < 32; w <<= 1) nan |= __shfl_xor_sync(0xffffffffu, nan, w);
-            keep_v[i] = ~((nan >> 7) * 0xFFu);
           } else {
-            keep_v[i] = 0;
+            nan = 0x80808080u;  // nothing was read: whatever the stage holds goes
+          }
+          if (__any_sync(0xffffffffu, nan != 0)) {
+            const uint32_t keep = ~((nan >> 7) * 0xFFu);
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) {
+              uint4 v = own[32 * p];
+              v.x &= keep; v.y &= keep; v.z &= keep; v.w &= keep;
+              own[32 * p] = v;
+            }
+            fence_proxy_async();  // before the stage's next copy
           }
           // token g is byte g % 2 of the lanes with c = g / 2, token g + 8 two bytes on
           const uint32_t nan_g = __shfl_sync(0xffffffffu, nan, g / 2) >> (8 * (g & 1));
@@ -467,12 +501,12 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs 
       for (int p = 0; p < kPieces; ++p)
 #pragma unroll
         for (int i = 0; i < kSub; ++i) {
-          uint4 v = *reinterpret_cast<const uint4 *>(kv + i * S::kBlockBytes + 16 * D + p * 512 + lane * 16);
-          v.x &= keep_v[i]; v.y &= keep_v[i]; v.z &= keep_v[i]; v.w &= keep_v[i];
-          const uint32_t a0[4] = {e4m3x2_f16x2(v.x & 0xFFFF), e4m3x2_f16x2(v.y & 0xFFFF),
-                                  e4m3x2_f16x2(v.x >> 16), e4m3x2_f16x2(v.y >> 16)};
-          const uint32_t a1[4] = {e4m3x2_f16x2(v.z & 0xFFFF), e4m3x2_f16x2(v.w & 0xFFFF),
-                                  e4m3x2_f16x2(v.z >> 16), e4m3x2_f16x2(v.w >> 16)};
+          const uint4 v = *reinterpret_cast<const uint4 *>(vr + i * S::kRecord + p * 512 + lane * 16);
+          uint32_t a0[4], a1[4];
+          e4m3x4_f16(v.x, a0[0], a0[2]);
+          e4m3x4_f16(v.y, a0[1], a0[3]);
+          e4m3x4_f16(v.z, a1[0], a1[2]);
+          e4m3x4_f16(v.w, a1[1], a1[3]);
 #pragma unroll
           for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -481,9 +515,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs 
               mma_f16_16816(o[p][1][t], a1, pb[i][t][w][0], pb[i][t][w][1]);
             }
         }
-      ++taken;
-      __syncwarp();
-      if (to_issue < steps) issue();
+      release();
     }
 
     // ---- merge the warps
@@ -510,7 +542,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs 
           *reinterpret_cast<float4 *>(mo + (size_t)(warp * kRows + 8 * t + 2 * c + k) * S::kLdO + 32 * p + 4 * g) =
               make_float4(o[p][0][t][k], o[p][0][t][k + 2], o[p][1][t][k], o[p][1][t][k + 2]);
     const bool whole = s0 == 0 && s1 == count;
-    const uint32_t slot = 2 * blockIdx.x + (first_seg ? 0 : 1);
+    // a problem that starts inside the run, or at its head: at most one of each leaves a part
+    const uint32_t slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
     float *const part_ml = a.part, *const part_o = a.part + (size_t)2 * gridDim.x * kRows * 2;
     if (threadIdx.x < kRows) {
       const uint32_t i = threadIdx.x;
@@ -557,15 +590,12 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs 
     }
     if (!whole) {
       // CTAs c0 .. c1 hold parts of this problem; c0 counts them
-      const uint64_t p0 = at - s0;  // where the problem begins on the line
-      const uint32_t c0 = (uint32_t)(p0 / run), c1 = (uint32_t)((p0 + count - 1) / run);
-      const uint32_t slot0 = 2 * c0 + (p0 > run * c0 ? 1 : 0);
-      __threadfence();
+      const uint32_t c0 = (uint32_t)(at / run), c1 = (uint32_t)((at + count - 1) / run);
+      const uint32_t slot0 = 2 * c0 + (at > run * c0 ? 1 : 0);
       __syncthreads();
-      if (threadIdx.x == 0) last_flag = atomicAdd(a.cnt + c0, 1u) == c1 - c0;
+      if (threadIdx.x == 0) last_flag = arrive_acq_rel(a.cnt + c0) == c1 - c0;
       __syncthreads();
       if (last_flag) {
-        __threadfence();
         auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : 2 * (c0 + k); };
         const uint32_t n = c1 - c0 + 1;
         // one warp per row for the maxima, then all threads over the rows' elements
@@ -604,24 +634,19 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(Kv8AttnArgs 
         if (threadIdx.x == 0) a.cnt[c0] = 0;
       }
     }
-    first_seg = false;
-    at += s1 - s0;
-    off += s1 - s0;
-    if (off == n_b) {
-      off = 0;
-      ++b;
-    }
+    merged = true;
   }
 }
 
 using AttnKernel = void (*)(Kv8AttnArgs);
 struct DecVariant {
   AttnKernel fn;
-  uint32_t smem, rows;
+  uint32_t smem, ctas;
 };
 template <typename T, int D, int NT>
 DecVariant variant() {
-  return {kv8_decode_kernel<T, D, NT>, (uint32_t)DecShape<D, NT, sizeof(T) == 4>::kSmem, 8 * NT};
+  using S = DecShape<D, NT, sizeof(T) == 4>;
+  return {kv8_decode_kernel<T, D, NT>, (uint32_t)S::kSmem, (uint32_t)S::kCtas};
 }
 // Variant i (0, 1, 2: 8, 16, 32 packed rows) of a head size: the output of 8 NT rows takes
 // D NT / 4 registers per thread, of which there may be 128.
@@ -638,12 +663,13 @@ DecVariant dec_variant(sx_dtype t, uint32_t d, uint32_t i) {
   return t == SX_F32 ? variant<float>(d, i) : variant<__nv_bfloat16>(d, i);
 }
 
-constexpr uint32_t kMinRun = 16;  // blocks: two per warp
+constexpr uint32_t kMinRun = 32;  // blocks, a problem's overhead included
 
 }  // namespace
 
-// Two partial results per CTA of the decode kernel, each up to 4096 / head_dim rows.
-size_t kv8_part_bytes(int num_sms) { return (size_t)2 * num_sms * (64 * 2 + 4096) * sizeof(float); }
+// Two parts per CTA of the decode kernel: up to 32 rows of {m, l}, and 4096 output values with one
+// CTA per SM, half as many with two.
+size_t kv8_part_bytes(int num_sms) { return (size_t)2 * num_sms * (2 * 32 * 2 + 4096) * sizeof(float); }
 
 cudaError_t prepare_kv8_attn() {
   for (uint32_t d : {64u, 128u, 256u, 512u})
@@ -700,6 +726,7 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
   // packed rows of an average sequence
   const uint64_t avg = (uint64_t)((tokens + c->num_seqs - 1) / c->num_seqs) * a.gqa;
   const sx::DecVariant v = sx::dec_variant(t, c->head_dim, avg <= 8 ? 0 : avg <= 16 ? 1 : 2);
-  v.fn<<<e->num_sms, sx::kDecThreads, v.smem, e->stream>>>(a);
-  return sx_host_cuda_status(cudaGetLastError(), "kv8_attn launch");
+  return sx_host_cuda_status(
+      sx::launch_chained(v.fn, dim3(e->num_sms * v.ctas), dim3(sx::kDecThreads), v.smem, e->stream, 1, a),
+      "kv8_attn launch");
 }
