@@ -652,6 +652,8 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
     st = cuda_status(sx::prepare_kv8_append(), "kv8 append kernel attributes");
     if (st) break;
     st = cuda_status(sx::prepare_kv8_attn(), "kv8 attention kernel attributes");
+    if (st) break;
+    st = cuda_status(sx::prepare_sample_kernels(), "probability kernel attributes");
   } while (0);
   if (st != SX_OK) {
     sx_engine_destroy(e);

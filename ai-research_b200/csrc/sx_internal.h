@@ -340,6 +340,8 @@ cudaError_t prepare_kv8_append();
 // and its attention (sx_kv8_attn.cu): scratch for the parts of split problems
 cudaError_t prepare_kv8_attn();
 size_t kv8_part_bytes(int num_sms);
+// Probabilities and verification (sx_sample.cu)
+cudaError_t prepare_sample_kernels();
 
 // Batch-prefill Q4_0 projection GEMM (sx_prefill.cu): y[t][n] = x[t][:] . bf16(deq(w[n][:]))
 cudaError_t prepare_prefill_kernel();

@@ -1,46 +1,165 @@
 // sx_sample.cu -- logits to probabilities, and verification of drafted tokens against them
 // (include/sx.h, sx_dispatch_probs and sx_dispatch_verify).
-#include "sx_host.h"
+//
+// Both walk rows of a vocabulary (1 MiB at 262144 tokens) and are bound by reading them, so a row
+// is spread over a thread-block cluster: its CTAs exchange one partial result each through
+// distributed shared memory, and the row is read once.
 #include "sx_common.cuh"
+#include "sx_host.h"
+#include "sx_launch.cuh"
 
 namespace sx {
 namespace {
 
-constexpr int kSampleThreads = 1024;
+constexpr int kSampleThreads = 512;
+constexpr int kSampleWarps = kSampleThreads / 32;
+constexpr uint32_t kMaxCluster = 16;
 
+SX_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+SX_DEV uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(r));
+  return r;
+}
+SX_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+}
+// store to the same shared variable of cluster rank r
+SX_DEV void st_cluster_u64(uint64_t *p, uint32_t r, uint64_t v) {
+  asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n"
+               " st.shared::cluster.u64 [a], %2;\n}\n" ::"r"(smem_u32(p)),
+               "r"(r), "l"(v)
+               : "memory");
+}
+SX_DEV float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// elements [i, i + 4) of a row of n; `fill` past its end
+SX_DEV float4 load4(const float *p, uint32_t i, uint32_t n, bool aligned, float fill) {
+  if (aligned && i + 4 <= n) return *reinterpret_cast<const float4 *>(p + i);
+  float4 v = make_float4(fill, fill, fill, fill);
+  if (i < n) v.x = p[i];
+  if (i + 1 < n) v.y = p[i + 1];
+  if (i + 2 < n) v.z = p[i + 2];
+  if (i + 3 < n) v.w = p[i + 3];
+  return v;
+}
+SX_DEV void store4(float *p, uint32_t i, uint32_t n, bool aligned, float4 v) {
+  if (aligned && i + 4 <= n) {
+    *reinterpret_cast<float4 *>(p + i) = v;
+    return;
+  }
+  if (i < n) p[i] = v.x;
+  if (i + 1 < n) p[i + 1] = v.y;
+  if (i + 2 < n) p[i + 2] = v.z;
+  if (i + 3 < n) p[i + 3] = v.w;
+}
+SX_DEV bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// ---------------------------------------------------------------------------------------
+// p = 2^(c (z - max)) / sum, c = log2(e) / temperature.
 struct ProbsArgs {
   const float *z;
   float *p;
   uint32_t z_ld, p_ld, n;
-  float temperature;
+  float c;
 };
 
-// max that keeps a NaN
-SX_DEV float max_nan(float a, float b) { return a != a ? a : (b != b ? b : fmaxf(a, b)); }
-
+// NV > 0: a thread holds NV float4 of the row in registers, so the row is read once; NV = 0: rows
+// of any length, read a second time (from L2) for the division.
+template <int NV>
 __global__ void __launch_bounds__(kSampleThreads) probs_kernel(ProbsArgs a) {
-  __shared__ float red[32];
-  const float *z = a.z + (size_t)blockIdx.x * a.z_ld;
-  float *p = a.p + (size_t)blockIdx.x * a.p_ld;
+  __shared__ float red_m[kSampleWarps], red_s[kSampleWarps];
+  __shared__ uint64_t part[kMaxCluster];  // {max, sum} of every CTA of the row
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  float m = -INFINITY;
-  for (uint32_t i = threadIdx.x; i < a.n; i += blockDim.x) m = max_nan(m, z[i]);
-  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) red[warp] = m;
+  const uint32_t rank = cluster_rank(), ctas = cluster_size(), row = blockIdx.x / ctas;
+  const float *z = a.z + (size_t)row * a.z_ld;
+  float *p = a.p + (size_t)row * a.p_ld;
+  const bool az = aligned16(z), ap = aligned16(p);
+  pdl_launch_dependents();
+  pdl_wait();
+
+  float4 x[NV > 0 ? NV : 1];
+  float m = -INFINITY, s = 0.0f;
+  const uint32_t seg = NV > 0 ? kSampleThreads * 4 * NV : (a.n + ctas - 1) / ctas + 3 & ~3u;
+  const uint32_t i0 = rank * seg + threadIdx.x * 4;
+  auto local = [&](float top) { return top == -INFINITY ? 0.0f : top; };
+  auto exps = [&](float4 v, float top) {
+    return make_float4(ex2((v.x - top) * a.c), ex2((v.y - top) * a.c), ex2((v.z - top) * a.c),
+                       ex2((v.w - top) * a.c));
+  };
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) x[k] = load4(z, i0 + k * kSampleThreads * 4, a.n, az, -INFINITY);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) m = fmaxf(fmaxf(m, fmaxf(x[k].x, x[k].y)), fmaxf(x[k].z, x[k].w));
+  } else {
+    const uint32_t end = min(a.n, (rank + 1) * seg);
+    for (uint32_t i = i0; i < end; i += kSampleThreads * 4) {
+      const float4 v = load4(z, i, end, az, -INFINITY);
+      const float t = fmaxf(m, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+      if (t > m) {
+        s *= m == -INFINITY ? 0.0f : ex2((m - t) * a.c);
+        m = t;
+      }
+      const float4 e = exps(v, local(m));
+      s += (e.x + e.y) + (e.z + e.w);
+    }
+  }
+  const float mine = m;
+  m = warp_max(m);
+  if (lane == 0) red_m[warp] = m;
   __syncthreads();
-  m = red[lane];
-  for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  m = warp_max(red_m[lane % kSampleWarps]);
+  if constexpr (NV > 0) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      x[k] = exps(x[k], local(m));
+      s += (x[k].x + x[k].y) + (x[k].z + x[k].w);
+    }
+  } else {
+    s *= mine == -INFINITY ? 1.0f : ex2((mine - m) * a.c);
+  }
+  s = warp_sum(s);
+  if (lane == 0) red_s[warp] = s;
   __syncthreads();
-  const float shift = m == -INFINITY ? 0.0f : m;
-  float s = 0.0f;
-  for (uint32_t i = threadIdx.x; i < a.n; i += blockDim.x) s += expf(__fdiv_rn(z[i] - shift, a.temperature));
-  s = block_sum(s, red);
-  for (uint32_t i = threadIdx.x; i < a.n; i += blockDim.x) {
-    const float e = expf(__fdiv_rn(z[i] - shift, a.temperature));
-    p[i] = m == -INFINITY ? 0.0f : __fdiv_rn(e, s);
+  s = lane < kSampleWarps ? red_s[lane] : 0.0f;
+  s = warp_sum(s);
+  float top = m, sum = s;
+  if (ctas > 1) {
+    if (threadIdx.x < ctas)
+      st_cluster_u64(part + rank, threadIdx.x, (uint64_t)__float_as_uint(s) << 32 | __float_as_uint(m));
+    cluster_sync();
+    const uint64_t v = part[lane % ctas];
+    const float mk = __uint_as_float((uint32_t)v), sk = __uint_as_float((uint32_t)(v >> 32));
+    top = warp_max(mk);
+    sum = warp_sum((uint32_t)lane < ctas ? sk * (mk == -INFINITY ? 1.0f : ex2((mk - top) * a.c)) : 0.0f);
+  }
+  // a row of -inf alone has sum 0 and stays 0; a NaN or +inf has made the sum NaN
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  if constexpr (NV > 0) {
+    const float f = (m == -INFINITY ? 1.0f : ex2((m - top) * a.c)) * inv;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      store4(p, i0 + k * kSampleThreads * 4, a.n, ap,
+             make_float4(x[k].x * f, x[k].y * f, x[k].z * f, x[k].w * f));
+  } else {
+    const uint32_t end = min(a.n, (rank + 1) * seg);
+    for (uint32_t i = i0; i < end; i += kSampleThreads * 4) {
+      const float4 e = exps(load4(z, i, end, az, -INFINITY), local(top));
+      store4(p, i, end, ap, make_float4(e.x * inv, e.y * inv, e.z * inv, e.w * inv));
+    }
   }
 }
 
+// ---------------------------------------------------------------------------------------
 struct VerifyArgs {
   const float *p, *q;
   const uint32_t *tok, *n_draft;
@@ -58,80 +177,183 @@ SX_DEV uint64_t warp_sum_u64(uint64_t v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+SX_DEV uint64_t warp_scan_u64(uint64_t v) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t u = __shfl_up_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) >= o) v += u;
+  }
+  return v;
+}
+
+// One cluster per sequence.  The row is cut into one contiguous run per warp, a run into lines of
+// 128 tokens (a float4 per lane); the warp keeps the sum of every line, lane i those of lines i,
+// i + 32, ..., so that once the total is known the token is found by three prefix sums (warps,
+// lines, tokens) and one line is read again.
+constexpr uint32_t kLine = 128;
 
 __global__ void __launch_bounds__(kSampleThreads) verify_kernel(VerifyArgs a) {
-  __shared__ uint64_t sums[32];
-  __shared__ uint32_t drawn;
-  const uint32_t b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ uint64_t warp_sums[kSampleWarps];
+  __shared__ uint64_t part[2][kMaxCluster];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t rank = cluster_rank(), ctas = cluster_size(), b = blockIdx.x / ctas;
   const float *p = a.p + (size_t)b * (a.drafts + 1) * a.p_ld;
   const float *q = a.q ? a.q + (size_t)b * a.drafts * a.q_ld : nullptr;
   const uint32_t *tok = a.tok + (size_t)b * a.drafts;
+  pdl_launch_dependents();
+  pdl_wait();
+  const bool lead = rank == 0 && threadIdx.x == 0;
+  const float us = a.u_sample[b];
   uint32_t nd = a.drafts;
   if (a.n_draft) {
     nd = a.n_draft[b];
     if (nd > a.drafts) {
-      if (threadIdx.x == 0) raise_error(a.err, kDevBadParams);
+      if (lead) raise_error(a.err, kDevBadParams);
       nd = a.drafts;
     }
   }
+  // ---- how many drafts are accepted: a lane each, every warp alike
   uint32_t m = 0;
-  for (; m < nd; ++m) {
-    const uint32_t x = tok[m];
-    if (x >= a.vocab) {
-      if (threadIdx.x == 0) raise_error(a.err, kDevBadParams);
+  for (; m < nd; m += 32) {
+    const uint32_t i = m + lane;
+    bool ok = false, bad = false;
+    if (i < nd) {
+      const uint32_t x = tok[i];
+      bad = x >= a.vocab;
+      if (!bad) {
+        const float qx = q ? q[(size_t)i * a.q_ld + x] : 1.0f;
+        ok = __fmul_rn(a.u_accept[(size_t)b * a.drafts + i], qx) < p[(size_t)i * a.p_ld + x];
+      }
+    }
+    const uint32_t no = __ballot_sync(0xffffffffu, !ok);
+    if (no) {
+      const uint32_t at = __ffs(no) - 1;
+      if (rank == 0 && warp == 0 && lane == (int)at && bad) raise_error(a.err, kDevBadParams);
+      m += at;
       break;
     }
-    const float qx = q ? q[(size_t)m * a.q_ld + x] : 1.0f;
-    if (!(__fmul_rn(a.u_accept[(size_t)b * a.drafts + m], qx) < p[(size_t)m * a.p_ld + x])) break;
   }
+  m = min(m, nd);
+  const bool refused = m < nd;
   const float *pr = p + (size_t)m * a.p_ld;
-  const float *qr = m < nd && q ? q + (size_t)m * a.q_ld : nullptr;
-  const uint32_t gone = m < nd && !q ? tok[m] : SX_NO_TOKEN;
-  if (threadIdx.x == 0) drawn = SX_NO_TOKEN;
+  const float *qr = refused && q ? q + (size_t)m * a.q_ld : nullptr;
+  const uint32_t gone = refused && !q ? tok[m] : SX_NO_TOKEN;  // q = 1 there, 0 elsewhere
+  const bool ap = aligned16(pr), aq = aligned16(qr);
+
+  const uint32_t lines = (a.vocab + kLine - 1) / kLine;
+  const uint32_t per = (lines + ctas * kSampleWarps - 1) / (ctas * kSampleWarps);  // lines of a warp
+  const uint32_t l0 = min(lines, (rank * kSampleWarps + warp) * per), l1 = min(lines, l0 + per);
+  uint32_t drawn = SX_NO_TOKEN;
+  bool here = false, none = true;  // this lane found the token; nothing has any weight
+#pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {  // the difference; if it has no weight, the row itself
-    auto weight = [&](uint32_t i) -> uint64_t {
-      if (pass == 1) return whole(pr[i]);
-      return whole(qr ? __fsub_rn(pr[i], qr[i]) : i == gone ? 0.0f : pr[i]);
+    auto weights = [&](uint32_t line, uint64_t (&w)[4]) {
+      const uint32_t i = line * kLine + 4 * lane;
+      float4 v = load4(pr, i, a.vocab, ap, 0.0f);
+      if (pass == 0) {
+        if (qr) {
+          const float4 d = load4(qr, i, a.vocab, aq, 0.0f);
+          v = make_float4(__fsub_rn(v.x, d.x), __fsub_rn(v.y, d.y), __fsub_rn(v.z, d.z), __fsub_rn(v.w, d.w));
+        } else if (gone - i < 4) {
+          if (gone == i) v.x = 0.0f;
+          if (gone == i + 1) v.y = 0.0f;
+          if (gone == i + 2) v.z = 0.0f;
+          if (gone == i + 3) v.w = 0.0f;
+        }
+      }
+      w[0] = whole(v.x);
+      w[1] = whole(v.y);
+      w[2] = whole(v.z);
+      w[3] = whole(v.w);
     };
-    // thread's run of consecutive tokens
-    const uint32_t per = (a.vocab + blockDim.x - 1) / blockDim.x;
-    const uint32_t i0 = min(a.vocab, threadIdx.x * per), i1 = min(a.vocab, i0 + per);
-    uint64_t mine = 0;
-    for (uint32_t i = i0; i < i1; ++i) mine += weight(i);
-    uint64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= (uint32_t)o) incl += v;
+    // Sums of the warp's lines.  Past 32 lines a lane keeps those of groups of lines: lane i the
+    // lines [l0 + i step, + step).
+    const uint32_t step = (l1 - l0 + 31) / 32;
+    uint64_t kept = 0;
+    for (uint32_t i = 0; i < 32 && l0 + i * step < l1; ++i) {
+      uint64_t sum = 0;
+#pragma unroll 4
+      for (uint32_t l = l0 + i * step; l < min(l1, l0 + (i + 1) * step); ++l) {
+        uint64_t w[4];
+        weights(l, w);
+        sum += (w[0] + w[1]) + (w[2] + w[3]);
+      }
+      sum = warp_sum_u64(sum);
+      if (lane == (int)i) kept = sum;
     }
+    const uint64_t incl = warp_scan_u64(kept);
+    const uint64_t mine = __shfl_sync(0xffffffffu, incl, 31);
+    if (lane == 31) warp_sums[warp] = mine;
     __syncthreads();
-    if (lane == 31) sums[warp] = incl;
-    __syncthreads();
-    uint64_t before = warp_sum_u64(lane < warp ? sums[lane] : 0ull);
-    const uint64_t total = warp_sum_u64(sums[lane]);
-    if (total == 0) continue;
-    const uint64_t u = (uint64_t)(a.u_sample[b] * 16777216.0f);
+    const uint64_t ws = lane < kSampleWarps ? warp_sums[lane] : 0;
+    const uint64_t cta = warp_sum_u64(ws);
+    const uint64_t before_warp = warp_sum_u64(lane < warp ? ws : 0);
+    if (threadIdx.x < ctas) st_cluster_u64(&part[pass][rank], threadIdx.x, cta);
+    cluster_sync();
+    const uint64_t ps = (uint32_t)lane < ctas ? part[pass][lane] : 0;
+    const uint64_t total = warp_sum_u64(ps);
+    if (total == 0) continue;  // the same in every CTA
+    none = false;
+    const uint64_t before = warp_sum_u64((uint32_t)lane < rank ? ps : 0) + before_warp;
+    const uint64_t u = (uint64_t)(us * 16777216.0f);
     const uint64_t goal = (total >> 24) * u + (((total & 0xFFFFFFull) * u) >> 24);
-    before += incl - mine;
-    if (before <= goal && goal < before + mine) {
-      uint64_t c = before;
-      for (uint32_t i = i0; i < i1; ++i) {
-        c += weight(i);
-        if (c > goal) {
-          drawn = i;
+    if (before <= goal && goal < before + mine) {  // this warp's run
+      const uint32_t who = __popc(__ballot_sync(0xffffffffu, before + incl <= goal));
+      uint64_t c = before + __shfl_sync(0xffffffffu, incl - kept, who);
+      for (uint32_t l = l0 + who * step; l < l1; ++l) {
+        uint64_t w[4];
+        weights(l, w);
+        const uint64_t sum = (w[0] + w[1]) + (w[2] + w[3]), in = warp_scan_u64(sum);
+        const uint64_t line = __shfl_sync(0xffffffffu, in, 31);
+        if (goal < c + line) {
+          uint64_t t = c + in - sum;
+          here = t <= goal && goal < t + sum;
+          drawn = l * kLine + 4 * lane;
+#pragma unroll
+          for (int k = 0; k < 3; ++k) {
+            t += w[k];
+            if (t <= goal) ++drawn;
+            else break;
+          }
           break;
         }
+        c += line;
       }
     }
     break;
   }
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i <= a.drafts; i += blockDim.x)
-    a.out[(size_t)b * (a.drafts + 1) + i] = i < m ? tok[i] : i == m ? drawn : SX_NO_TOKEN;
-  if (threadIdx.x == 0) a.accepted[b] = m;
+  uint32_t *out = a.out + (size_t)b * (a.drafts + 1);
+  if (here) out[m] = drawn;
+  if (rank == 0) {
+    for (uint32_t i = threadIdx.x; i <= a.drafts; i += kSampleThreads)
+      if (i != m || none) out[i] = i < m ? tok[i] : SX_NO_TOKEN;
+    if (threadIdx.x == 0) a.accepted[b] = m;
+  }
+}
+
+using ProbsKernel = void (*)(ProbsArgs);
+// float4 per thread of the single-CTA forms; longer rows take 8 in as many CTAs as it needs
+ProbsKernel probs_variant(uint32_t n, uint32_t *ctas) {
+  *ctas = 1;
+  if (n <= 2048) return probs_kernel<1>;
+  if (n <= 2 * 2048) return probs_kernel<2>;
+  if (n <= 4 * 2048) return probs_kernel<4>;
+  const uint32_t need = (n + 8 * 2048 - 1) / (8 * 2048);
+  while (*ctas < need && *ctas < kMaxCluster) *ctas *= 2;
+  return need <= kMaxCluster ? probs_kernel<8> : probs_kernel<0>;
 }
 
 }  // namespace
+
+cudaError_t prepare_sample_kernels() {
+  const void *k[] = {(const void *)probs_kernel<0>, (const void *)probs_kernel<8>, (const void *)verify_kernel};
+  for (const void *f : k) {
+    const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
 }  // namespace sx
 
 extern "C" {
@@ -145,16 +367,20 @@ SX_API sx_status sx_dispatch_probs(sx_engine *e, const float *logits, uint32_t l
   };
   if (!e || !logits || !probs) return bad("null engine, logits or probs");
   if (n == 0 || n > (1u << 24)) return bad("n must be 1 .. 2^24");
-  if (!(temperature > 0.0f) || !(temperature < 3.0e38f)) return bad("temperature must be positive and finite");
+  if (!(temperature >= 1e-30f) || !(temperature <= 1e30f)) return bad("temperature must be 1e-30 .. 1e30");
   if ((logits_ld && logits_ld < n) || (probs_ld && probs_ld < n)) return bad("strides are shorter than a row");
   if (logits == probs && (logits_ld ? logits_ld : n) != (probs_ld ? probs_ld : n))
     return bad("in place needs equal strides");
+  if (rows >= (1u << 26)) return bad("too many rows");
   if (rows == 0) return SX_OK;
   cudaError_t ce = cudaSetDevice(e->device);
   if (ce != cudaSuccess) return sx_host_cuda_status(ce, "cudaSetDevice");
-  sx::ProbsArgs a{logits, probs, logits_ld ? logits_ld : n, probs_ld ? probs_ld : n, n, temperature};
-  sx::probs_kernel<<<rows, sx::kSampleThreads, 0, e->stream>>>(a);
-  return sx_host_cuda_status(cudaGetLastError(), "probs launch");
+  sx::ProbsArgs a{logits, probs, logits_ld ? logits_ld : n, probs_ld ? probs_ld : n, n,
+                  1.4426950408889634f / temperature};
+  uint32_t ctas;
+  const sx::ProbsKernel k = sx::probs_variant(n, &ctas);
+  return sx_host_cuda_status(
+      sx::launch_chained(k, dim3(rows * ctas), dim3(sx::kSampleThreads), 0, e->stream, ctas, a), "probs launch");
 }
 
 SX_API sx_status sx_dispatch_verify(sx_engine *e, const float *target, uint32_t target_ld,
@@ -172,13 +398,18 @@ SX_API sx_status sx_dispatch_verify(sx_engine *e, const float *target, uint32_t 
   if (drafts > 1024) return bad("at most 1024 drafts");
   if ((target_ld && target_ld < vocab) || (draft_ld && draft_ld < vocab))
     return bad("strides are shorter than a row");
+  if (seqs >= (1u << 26)) return bad("too many sequences");
   if (seqs == 0) return SX_OK;
   cudaError_t ce = cudaSetDevice(e->device);
   if (ce != cudaSuccess) return sx_host_cuda_status(ce, "cudaSetDevice");
   sx::VerifyArgs a{target, drafts ? draft : nullptr, tok, n_draft, u_accept, u_sample, out, accepted,
                    target_ld ? target_ld : vocab, draft_ld ? draft_ld : vocab, drafts, vocab, e->err_dev};
-  sx::verify_kernel<<<seqs, sx::kSampleThreads, 0, e->stream>>>(a);
-  return sx_host_cuda_status(cudaGetLastError(), "verify launch");
+  // a CTA per 8192 tokens of the vocabulary
+  uint32_t ctas = 1;
+  while (ctas < sx::kMaxCluster && ctas * 8192 < vocab) ctas *= 2;
+  return sx_host_cuda_status(
+      sx::launch_chained(sx::verify_kernel, dim3(seqs * ctas), dim3(sx::kSampleThreads), 0, e->stream, ctas, a),
+      "verify launch");
 }
 
 }  // extern "C"

@@ -608,7 +608,7 @@ SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, sx_dtype t,
                                       float scale);
 
 /* probs[r] = softmax(logits[r] / temperature) for `rows` rows of n f32 (strides in floats, 0: n);
- * temperature > 0.  A row of -inf alone gives zeros; a NaN or +inf gives NaN.  In place allowed
+ * temperature 1e-30 .. 1e30.  A row of -inf alone gives zeros; a NaN or +inf gives NaN.  In place allowed
  * when the strides are equal. */
 SX_API sx_status sx_dispatch_probs(sx_engine *e, const float *logits, uint32_t logits_ld,
                                    float *probs, uint32_t probs_ld, uint32_t rows, uint32_t n,
