@@ -25,9 +25,8 @@ SX_DEV uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(r));
   return r;
 }
-SX_DEV void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
-}
+SX_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory"); }
+SX_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
 // store to the same shared variable of cluster rank r
 SX_DEV void st_cluster_u64(uint64_t *p, uint32_t r, uint64_t v) {
   asm volatile("{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %0, %1;\n"
@@ -83,6 +82,7 @@ __global__ void __launch_bounds__(kSampleThreads) probs_kernel(ProbsArgs a) {
   const float *z = a.z + (size_t)row * a.z_ld;
   float *p = a.p + (size_t)row * a.p_ld;
   const bool az = aligned16(z), ap = aligned16(p);
+  cluster_arrive();  // met before the first store to another CTA: it has started by then
   pdl_launch_dependents();
   pdl_wait();
 
@@ -133,10 +133,12 @@ __global__ void __launch_bounds__(kSampleThreads) probs_kernel(ProbsArgs a) {
   s = lane < kSampleWarps ? red_s[lane] : 0.0f;
   s = warp_sum(s);
   float top = m, sum = s;
+  cluster_wait();
   if (ctas > 1) {
     if (threadIdx.x < ctas)
       st_cluster_u64(part + rank, threadIdx.x, (uint64_t)__float_as_uint(s) << 32 | __float_as_uint(m));
-    cluster_sync();
+    cluster_arrive();
+    cluster_wait();
     const uint64_t v = part[lane % ctas];
     const float mk = __uint_as_float((uint32_t)v), sk = __uint_as_float((uint32_t)(v >> 32));
     top = warp_max(mk);
@@ -169,8 +171,12 @@ struct VerifyArgs {
   uint32_t *err;
 };
 
-// a probability as a multiple of 2^-38 (NaN and negative: 0)
-SX_DEV uint64_t whole(float w) { return w > 0.0f ? (uint64_t)(fminf(w, 1.0f) * 0x1p38f) : 0ull; }
+// floor(min(w, 1) 2^38), NaN and negative 0: 2^14 + w rounded toward zero in 64 bits has exactly
+// that many units of 2^-38 past 2^14, and its bits count them.
+constexpr uint64_t kWholeZero = 0x40D0000000000000ull;  // bits of 2^14
+SX_DEV uint64_t whole_bits(float w) {
+  return (uint64_t)__double_as_longlong(__dadd_rz((double)fminf(fmaxf(w, 0.0f), 1.0f), 16384.0));
+}
 
 SX_DEV uint64_t warp_sum_u64(uint64_t v) {
 #pragma unroll
@@ -200,6 +206,7 @@ __global__ void __launch_bounds__(kSampleThreads) verify_kernel(VerifyArgs a) {
   const float *p = a.p + (size_t)b * (a.drafts + 1) * a.p_ld;
   const float *q = a.q ? a.q + (size_t)b * a.drafts * a.q_ld : nullptr;
   const uint32_t *tok = a.tok + (size_t)b * a.drafts;
+  cluster_arrive();  // met before the first store to another CTA
   pdl_launch_dependents();
   pdl_wait();
   const bool lead = rank == 0 && threadIdx.x == 0;
@@ -247,39 +254,45 @@ __global__ void __launch_bounds__(kSampleThreads) verify_kernel(VerifyArgs a) {
   bool here = false, none = true;  // this lane found the token; nothing has any weight
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {  // the difference; if it has no weight, the row itself
-    auto weights = [&](uint32_t line, uint64_t (&w)[4]) {
+    // values of a line, and their weights
+    auto fetch = [&](uint32_t line, float4 &v, float4 &d) {
       const uint32_t i = line * kLine + 4 * lane;
-      float4 v = load4(pr, i, a.vocab, ap, 0.0f);
-      if (pass == 0) {
-        if (qr) {
-          const float4 d = load4(qr, i, a.vocab, aq, 0.0f);
-          v = make_float4(__fsub_rn(v.x, d.x), __fsub_rn(v.y, d.y), __fsub_rn(v.z, d.z), __fsub_rn(v.w, d.w));
-        } else if (gone - i < 4) {
-          if (gone == i) v.x = 0.0f;
-          if (gone == i + 1) v.y = 0.0f;
-          if (gone == i + 2) v.z = 0.0f;
-          if (gone == i + 3) v.w = 0.0f;
-        }
-      }
-      w[0] = whole(v.x);
-      w[1] = whole(v.y);
-      w[2] = whole(v.z);
-      w[3] = whole(v.w);
+      v = load4(pr, i, a.vocab, ap, 0.0f);
+      d = pass == 0 && qr ? load4(qr, i, a.vocab, aq, 0.0f) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     };
-    // Sums of the warp's lines.  Past 32 lines a lane keeps those of groups of lines: lane i the
-    // lines [l0 + i step, + step).
-    const uint32_t step = (l1 - l0 + 31) / 32;
-    uint64_t kept = 0;
-    for (uint32_t i = 0; i < 32 && l0 + i * step < l1; ++i) {
-      uint64_t sum = 0;
-#pragma unroll 4
-      for (uint32_t l = l0 + i * step; l < min(l1, l0 + (i + 1) * step); ++l) {
+    auto weights = [&](uint32_t line, float4 v, float4 d, uint64_t (&w)[4]) {
+      const uint32_t i = line * kLine + 4 * lane;
+      w[0] = whole_bits(__fsub_rn(v.x, d.x)) - kWholeZero;
+      w[1] = whole_bits(__fsub_rn(v.y, d.y)) - kWholeZero;
+      w[2] = whole_bits(__fsub_rn(v.z, d.z)) - kWholeZero;
+      w[3] = whole_bits(__fsub_rn(v.w, d.w)) - kWholeZero;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (pass == 0 && gone == i + k) w[k] = 0;
+    };
+    // Sums of groups of `step` of the warp's lines (four, or more so that 32 groups hold the run),
+    // four lines in flight; lane i keeps that of group i.
+    const uint32_t step = 4 * ((l1 - l0 + 127) / 128);
+    uint64_t kept = 0, sum = 0;
+    uint32_t in_group = 0, group = 0;
+    for (uint32_t l = l0; l < l1; l += 4) {
+      float4 v[4], d[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) fetch(l + k, v[k], d[k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
         uint64_t w[4];
-        weights(l, w);
-        sum += (w[0] + w[1]) + (w[2] + w[3]);
+        weights(l + k, v[k], d[k], w);
+        if (l + k < l1) sum += (w[0] + w[1]) + (w[2] + w[3]);
       }
-      sum = warp_sum_u64(sum);
-      if (lane == (int)i) kept = sum;
+      in_group += 4;
+      if (in_group == step || l + 4 >= l1) {
+        sum = warp_sum_u64(sum);
+        if (lane == (int)group) kept = sum;
+        ++group;
+        sum = 0;
+        in_group = 0;
+      }
     }
     const uint64_t incl = warp_scan_u64(kept);
     const uint64_t mine = __shfl_sync(0xffffffffu, incl, 31);
@@ -288,8 +301,10 @@ __global__ void __launch_bounds__(kSampleThreads) verify_kernel(VerifyArgs a) {
     const uint64_t ws = lane < kSampleWarps ? warp_sums[lane] : 0;
     const uint64_t cta = warp_sum_u64(ws);
     const uint64_t before_warp = warp_sum_u64(lane < warp ? ws : 0);
+    if (pass == 0) cluster_wait();
     if (threadIdx.x < ctas) st_cluster_u64(&part[pass][rank], threadIdx.x, cta);
-    cluster_sync();
+    cluster_arrive();
+    cluster_wait();
     const uint64_t ps = (uint32_t)lane < ctas ? part[pass][lane] : 0;
     const uint64_t total = warp_sum_u64(ps);
     if (total == 0) continue;  // the same in every CTA
@@ -300,24 +315,26 @@ __global__ void __launch_bounds__(kSampleThreads) verify_kernel(VerifyArgs a) {
     if (before <= goal && goal < before + mine) {  // this warp's run
       const uint32_t who = __popc(__ballot_sync(0xffffffffu, before + incl <= goal));
       uint64_t c = before + __shfl_sync(0xffffffffu, incl - kept, who);
-      for (uint32_t l = l0 + who * step; l < l1; ++l) {
-        uint64_t w[4];
-        weights(l, w);
-        const uint64_t sum = (w[0] + w[1]) + (w[2] + w[3]), in = warp_scan_u64(sum);
-        const uint64_t line = __shfl_sync(0xffffffffu, in, 31);
-        if (goal < c + line) {
-          uint64_t t = c + in - sum;
-          here = t <= goal && goal < t + sum;
-          drawn = l * kLine + 4 * lane;
+      for (uint32_t l = l0 + who * step; l < l1 && drawn == SX_NO_TOKEN; l += 4) {
+        float4 v[4], d[4];
 #pragma unroll
-          for (int k = 0; k < 3; ++k) {
-            t += w[k];
-            if (t <= goal) ++drawn;
-            else break;
+        for (int k = 0; k < 4; ++k) fetch(l + k, v[k], d[k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint64_t w[4];
+          weights(l + k, v[k], d[k], w);
+          const uint64_t sum = (w[0] + w[1]) + (w[2] + w[3]), in = warp_scan_u64(sum);
+          const uint64_t line = __shfl_sync(0xffffffffu, in, 31);
+          if (drawn == SX_NO_TOKEN && goal < c + line) {
+            uint64_t t = c + in - sum;
+            here = t <= goal && goal < t + sum;
+            drawn = (l + k) * kLine + 4 * lane;
+            if (t + w[0] <= goal) ++drawn;
+            if (t + w[0] + w[1] <= goal) ++drawn;
+            if (t + w[0] + w[1] + w[2] <= goal) ++drawn;
           }
-          break;
+          c += line;
         }
-        c += line;
       }
     }
     break;
@@ -332,15 +349,19 @@ __global__ void __launch_bounds__(kSampleThreads) verify_kernel(VerifyArgs a) {
 }
 
 using ProbsKernel = void (*)(ProbsArgs);
-// float4 per thread of the single-CTA forms; longer rows take 8 in as many CTAs as it needs
-ProbsKernel probs_variant(uint32_t n, uint32_t *ctas) {
-  *ctas = 1;
-  if (n <= 2048) return probs_kernel<1>;
-  if (n <= 2 * 2048) return probs_kernel<2>;
-  if (n <= 4 * 2048) return probs_kernel<4>;
-  const uint32_t need = (n + 8 * 2048 - 1) / (8 * 2048);
-  while (*ctas < need && *ctas < kMaxCluster) *ctas *= 2;
-  return need <= kMaxCluster ? probs_kernel<8> : probs_kernel<0>;
+struct ProbsVariant {
+  ProbsKernel fn;
+  uint32_t ctas;
+};
+// Up to 8192 logits one CTA holds the row in registers, up to 16 x 16384 as many CTAs as it needs
+// do; past that they read it twice.
+ProbsVariant probs_variant(uint32_t n) {
+  if (n <= 2048) return {probs_kernel<1>, 1};
+  if (n <= 2 * 2048) return {probs_kernel<2>, 1};
+  if (n <= 4 * 2048) return {probs_kernel<4>, 1};
+  uint32_t ctas = 1;
+  while (ctas < kMaxCluster && ctas * (8 * 2048) < n) ctas *= 2;
+  return {n <= ctas * (8 * 2048) ? probs_kernel<8> : probs_kernel<0>, ctas};
 }
 
 }  // namespace
@@ -377,10 +398,10 @@ SX_API sx_status sx_dispatch_probs(sx_engine *e, const float *logits, uint32_t l
   if (ce != cudaSuccess) return sx_host_cuda_status(ce, "cudaSetDevice");
   sx::ProbsArgs a{logits, probs, logits_ld ? logits_ld : n, probs_ld ? probs_ld : n, n,
                   1.4426950408889634f / temperature};
-  uint32_t ctas;
-  const sx::ProbsKernel k = sx::probs_variant(n, &ctas);
+  const sx::ProbsVariant v = sx::probs_variant(n);
   return sx_host_cuda_status(
-      sx::launch_chained(k, dim3(rows * ctas), dim3(sx::kSampleThreads), 0, e->stream, ctas, a), "probs launch");
+      sx::launch_chained(v.fn, dim3(rows * v.ctas), dim3(sx::kSampleThreads), 0, e->stream, v.ctas, a),
+      "probs launch");
 }
 
 SX_API sx_status sx_dispatch_verify(sx_engine *e, const float *target, uint32_t target_ld,
@@ -404,9 +425,9 @@ SX_API sx_status sx_dispatch_verify(sx_engine *e, const float *target, uint32_t 
   if (ce != cudaSuccess) return sx_host_cuda_status(ce, "cudaSetDevice");
   sx::VerifyArgs a{target, drafts ? draft : nullptr, tok, n_draft, u_accept, u_sample, out, accepted,
                    target_ld ? target_ld : vocab, draft_ld ? draft_ld : vocab, drafts, vocab, e->err_dev};
-  // a CTA per 8192 tokens of the vocabulary
+  // a CTA per 8192 tokens of the vocabulary, while they fit the GPU at once (two per SM)
   uint32_t ctas = 1;
-  while (ctas < sx::kMaxCluster && ctas * 8192 < vocab) ctas *= 2;
+  while (ctas < sx::kMaxCluster && ctas * 8192 < vocab && (uint64_t)seqs * ctas * 2 <= 2ull * e->num_sms) ctas *= 2;
   return sx_host_cuda_status(
       sx::launch_chained(sx::verify_kernel, dim3(seqs * ctas), dim3(sx::kSampleThreads), 0, e->stream, ctas, a),
       "verify launch");
