@@ -7,12 +7,19 @@
 //
 // A record belongs to one CTA, which sees all of its new tokens, so the scale needs no atomics:
 // unit u is one 16-token block of one sequence, a CTA takes one unit and a group of kv heads with
-// their q heads.  The angles of a unit's tokens are computed once and kept in shared memory.
-// With sequence b's rows at row_start[b], units row_start[b] / 16 + 2 b .. belong to it: n rows
-// touch at most n / 16 + 2 blocks, so the grid follows from the row and sequence counts alone and
-// nothing is read back.
+// their q heads.  With sequence b's rows at row_start[b], units row_start[b] / 16 + 2 b .. belong to
+// it: n rows touch at most n / 16 + 2 blocks, so the grid follows from the row and sequence counts
+// alone and nothing is read back.
+//
+// Bound by the rows' bytes, and close behind by instructions: a vector of 256 has 45 cycles of an SM
+// at the copy rate.  A warp takes whole vectors; lane l holds elements 64 k + 2 l, + 1 of every
+// chunk k, so that a rotation over the first 64 touches one chunk (its pairs meet by one shuffle)
+// and one whose half is a multiple of 64 needs no exchange.  The angles are computed once per unit.
+// K and V stay in registers until the block's maxima have met in shared memory, are converted by
+// their owners, and leave through a byte tile that turns rows of tokens into the record's pieces.
 #include "sx_host.h"
 #include "sx_kv8.cuh"
+#include "sx_launch.cuh"
 
 namespace sx {
 namespace {
@@ -32,29 +39,149 @@ struct AppendArgs {
   uint32_t *err;
 };
 
-// x / rms(x) * w, in the engine's order of operations (qkv_rope)
-template <int N>
-SX_DEV void normalise(float (&x)[N], float eps, uint32_t dim) {
+// shared memory: the byte tile (or a row of f32 per warp, for rotations whose pairs meet there),
+// the gains of q and k, the angles' cosines and sines
+SX_HD constexpr uint32_t append_tile_bytes(uint32_t d) {
+  return 2 * kKv8Block * (d + 32) > kAppWarps * d * 4 ? 2 * kKv8Block * (d + 32) : kAppWarps * d * 4;
+}
+
+// A lane's part of a vector as it stands in memory: one word (bf16) or two (f32) per chunk.
+template <typename T, int C>
+struct Raw {
+  static constexpr int kWords = sizeof(T) == 4 ? 2 : 1;
+  uint32_t w[C][kWords];
+  SX_DEV void load(const T *p, uint32_t lane) {
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      if constexpr (kWords == 2) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(p + 64 * k + 2 * lane);
+        w[k][0] = u.x;
+        w[k][1] = u.y;
+      } else {
+        w[k][0] = *reinterpret_cast<const uint32_t *>(p + 64 * k + 2 * lane);
+      }
+    }
+  }
+  SX_DEV void unpack(float (&x)[C][2]) const {
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+      x[k][0] = __uint_as_float(kWords == 2 ? w[k][0] : w[k][0] << 16);
+      x[k][1] = __uint_as_float(kWords == 2 ? w[k][kWords - 1] : w[k][0] & 0xFFFF0000u);
+    }
+  }
+};
+template <typename T, int C>
+SX_DEV void store_vector(T *p, uint32_t lane, const float (&x)[C][2]) {
+#pragma unroll
+  for (int k = 0; k < C; ++k) store_vec<T, 2>(p + 64 * k + 2 * lane, x[k]);
+}
+
+// x / rms(x)
+template <int C>
+SX_DEV void normalise(float (&x)[C][2], float eps) {
   float ss = 0.0f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) ss = fmaf(x[i], x[i], ss);
-  ss = warp_sum(ss);
-  const float rs = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)dim), eps)));
+  for (int k = 0; k < C; ++k) ss = fmaf(x[k][0], x[k][0], fmaf(x[k][1], x[k][1], ss));
+  const float rs = rsqrtf(warp_sum(ss) * (1.0f / (64 * C)) + eps);
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = __fmul_rn(x[i], rs);
+  for (int k = 0; k < C; ++k) {
+    x[k][0] = __fmul_rn(x[k][0], rs);
+    x[k][1] = __fmul_rn(x[k][1], rs);
+  }
+}
+template <int C>
+SX_DEV void gain(float (&x)[C][2], const float *w, uint32_t lane) {
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const float2 g = *reinterpret_cast<const float2 *>(w + 64 * k + 2 * lane);
+    x[k][0] = __fmul_rn(x[k][0], g.x);
+    x[k][1] = __fmul_rn(x[k][1], g.y);
+  }
+}
+// (x0, x1) turned by the angle with cosine and sine f: every product and sum rounded, as the engine
+SX_DEV float turn_low(float x0, float x1, float2 f) { return __fsub_rn(__fmul_rn(x0, f.x), __fmul_rn(x1, f.y)); }
+SX_DEV float turn_high(float x0, float x1, float2 f) { return __fadd_rn(__fmul_rn(x0, f.y), __fmul_rn(x1, f.x)); }
+
+// half = 64 H: the pairs are chunks k and k + H of one lane
+template <int H, int C>
+SX_DEV void rotate_chunks(float (&x)[C][2], const float2 *ct, uint32_t lane) {
+  if constexpr (2 * H <= C) {
+#pragma unroll
+    for (int k = 0; k < H; ++k)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float2 f = ct[64 * k + 2 * lane + j];
+        const float x0 = x[k][j], x1 = x[k + H][j];
+        x[k][j] = turn_low(x0, x1, f);
+        x[k + H][j] = turn_high(x0, x1, f);
+      }
+  }
+}
+// Any rotation: half up to 32 and even stays in chunk 0; the odd ones meet in buf (D floats).
+template <int C>
+SX_DEV void rotate(float (&x)[C][2], uint32_t half, const float2 *ct, float *buf, uint32_t lane) {
+  if (half == 0) return;
+  if (half <= 32 && half % 2 == 0) {
+    const uint32_t o = half / 2;
+    const bool low = lane < o, high = !low && lane < 2 * o;
+    const uint32_t peer = low ? lane + o : high ? lane - o : lane;
+    const float y0 = __shfl_sync(0xffffffffu, x[0][0], peer), y1 = __shfl_sync(0xffffffffu, x[0][1], peer);
+    if (low) {
+      x[0][0] = turn_low(x[0][0], y0, ct[2 * lane]);
+      x[0][1] = turn_low(x[0][1], y1, ct[2 * lane + 1]);
+    } else if (high) {
+      x[0][0] = turn_high(y0, x[0][0], ct[2 * lane - half]);
+      x[0][1] = turn_high(y1, x[0][1], ct[2 * lane + 1 - half]);
+    }
+  } else if (half == 64) {
+    rotate_chunks<1>(x, ct, lane);
+  } else if (half == 128) {
+    rotate_chunks<2>(x, ct, lane);
+  } else if (half == 256) {
+    rotate_chunks<4>(x, ct, lane);
+  } else {
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < C; ++k) *reinterpret_cast<float2 *>(buf + 64 * k + 2 * lane) = make_float2(x[k][0], x[k][1]);
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < C; ++k)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t d = 64 * k + 2 * lane + j;
+        if (d < half)
+          x[k][j] = turn_low(x[k][j], buf[d + half], ct[d]);
+        else if (d < 2 * half)
+          x[k][j] = turn_high(buf[d - half], x[k][j], ct[d - half]);
+      }
+  }
+}
+
+// four rows' words of 4 bytes -> four words of one byte each row (a 4 x 4 byte transposition)
+SX_DEV void transpose4(uint32_t (&w)[4]) {
+  const uint32_t a = prmt(w[0], w[1], 0x5140), b = prmt(w[2], w[3], 0x5140);  // bytes 0, 1
+  const uint32_t c = prmt(w[0], w[1], 0x7362), d = prmt(w[2], w[3], 0x7362);  // bytes 2, 3
+  w[0] = prmt(a, b, 0x5410);
+  w[1] = prmt(a, b, 0x7632);
+  w[2] = prmt(c, d, 0x5410);
+  w[3] = prmt(c, d, 0x7632);
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kAppWarps * 32) kv8_append_kernel(AppendArgs a) {
-  constexpr int kPer = D / 32;                                  // elements of a vector per lane
-  constexpr int kVec = kPer < 16 / (int)sizeof(T) ? kPer : 16 / (int)sizeof(T);
-  constexpr int kLd = D + 4;  // tile row stride: the 16-byte reads below hit all banks once
-  extern __shared__ float sh[];
-  __shared__ float amax[2][kKv8Block];
-  float *tile = sh;                                             // [2][16][kLd]; q rows: [warps][D]
-  float2 *cs = reinterpret_cast<float2 *>(sh + 2 * kKv8Block * kLd);  // [16][rot / 2]
+__global__ void __launch_bounds__(kAppWarps * 32, D <= 256 ? 3 : 2) kv8_append_kernel(AppendArgs a) {
+  constexpr int kChunks = D / 64;
+  constexpr int kLd = D + 32;  // bytes of a tile row
+  extern __shared__ __align__(16) uint8_t sh[];
+  __shared__ float amax[2][2][kKv8Block];  // [parity][K, V][token]
+  uint8_t *const tile = sh;                // [K, V][16][kLd]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float *const buf = reinterpret_cast<float *>(sh) + warp * D;
+  float *const q_w = reinterpret_cast<float *>(sh + append_tile_bytes(D)), *const k_w = q_w + D;
+  float2 *const cs = reinterpret_cast<float2 *>(k_w + D);  // [16][half]
   const uint32_t half = a.rot / 2;
+  const bool by_buf = half != 0 && !(half <= 32 && half % 2 == 0) && half != 64 && half != 128 && half != 256;
+  pdl_launch_dependents();
+  pdl_wait();
 
   const uint32_t u = blockIdx.x;
   const uint32_t b = warp_last_le(a.c.num_seqs, u, [&](uint32_t i) { return a.row_start[i] / 16 + 2 * i; });
@@ -78,184 +205,174 @@ __global__ void __launch_bounds__(kAppWarps * 32) kv8_append_kernel(AppendArgs a
   const uint32_t in_page = blk % (a.c.page_tokens / kKv8Block);
 
   for (uint32_t i = threadIdx.x; i < cnt * half; i += blockDim.x) {
-    const uint32_t t = i / half, f = i % half;
+    const uint32_t t = i / half, f = i - t * half;
     float s, c;
     sincosf(__fmul_rn((float)(lo + t), a.inv_freq[f]), &s, &c);
     cs[i] = make_float2(c, s);
   }
+  for (uint32_t i = threadIdx.x; i < D; i += blockDim.x) {
+    if (a.q_w) q_w[i] = a.q_w[i];
+    if (a.k_w) k_w[i] = a.k_w[i];
+  }
   __syncthreads();
 
-  // a lane's elements of a vector: chunk i is [(32 i + lane) kVec, + kVec)
-  auto load = [&](const void *base, size_t off, float (&x)[kPer]) {
-#pragma unroll
-    for (int i = 0; i < kPer / kVec; ++i) {
-      float v[kVec];
-      load_vec<T, kVec>(static_cast<const T *>(base) + off + (32 * i + lane) * kVec, v);
-#pragma unroll
-      for (int j = 0; j < kVec; ++j) x[i * kVec + j] = v[j];
-    }
-  };
-  auto gain = [&](const float *w, float (&x)[kPer]) {
-#pragma unroll
-    for (int i = 0; i < kPer / kVec; ++i)
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        x[i * kVec + j] = __fmul_rn(x[i * kVec + j], w[(32 * i + lane) * kVec + j]);
-  };
-  // rotate token t's vector: the pairs meet in buf (one warp's row of D floats)
-  auto rotate = [&](float (&x)[kPer], float *buf, uint32_t t) {
-    if (half == 0) return;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) buf[(32 * (i / kVec) + lane) * kVec + i % kVec] = x[i];
-    __syncwarp();
-    const float2 *ct = cs + t * half;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const uint32_t d = (32 * (i / kVec) + lane) * kVec + i % kVec;
-      if (d < half) {
-        const float2 f = ct[d];
-        x[i] = __fsub_rn(__fmul_rn(x[i], f.x), __fmul_rn(buf[d + half], f.y));
-      } else if (d < 2 * half) {
-        const float2 f = ct[d - half];
-        x[i] = __fadd_rn(__fmul_rn(buf[d - half], f.y), __fmul_rn(x[i], f.x));
-      }
-    }
-  };
-
+  // Tokens over warps: warp w takes tokens w % tw and w % tw + 8, and with few tokens the vectors
+  // of one (K, V, then q heads) are dealt to the warps that share it.
+  uint32_t tw = 8;
+  while (tw > 1 && tw / 2 >= cnt) tw /= 2;
+  const uint32_t tok = warp % tw, sub = warp / tw, subs = kAppWarps / tw;
   const uint32_t h0 = blockIdx.y * a.heads_per_cta;
   const uint32_t h1 = min(a.c.num_kv, h0 + a.heads_per_cta);
-  // ---- q rows
-  const uint32_t nq = (h1 - h0) * a.gqa;
-  for (uint32_t i = warp; i < cnt * nq; i += kAppWarps) {
-    const uint32_t t = i / nq, h = h0 * a.gqa + i % nq;
-    float x[kPer];
-    load(a.q, (size_t)(row0 + t) * a.q_ld + (size_t)h * D, x);
-    if (a.q_w) {
-      normalise(x, a.eps, D);
-      gain(a.q_w, x);
-    }
-    rotate(x, tile + warp * D, t);
-    T *dst = static_cast<T *>(a.q_out) + ((size_t)(row0 + t) * a.c.num_kv * a.gqa + h) * D;
-#pragma unroll
-    for (int j = 0; j < kPer / kVec; ++j) {
-      float v[kVec];
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) v[e] = x[j * kVec + e];
-      store_vec<T, kVec>(dst + (32 * j + lane) * kVec, v);
-    }
-  }
-
-  // ---- K and V records
+  const size_t q_row = (size_t)a.c.num_kv * a.gqa * D;
   for (uint32_t h = h0; h < h1; ++h) {
-    __syncthreads();  // the tile is free
-    for (uint32_t i = warp; i < 2 * cnt; i += kAppWarps) {
-      const uint32_t t = i >> 1, is_v = i & 1;
-      float *row = tile + (is_v * kKv8Block + t0 + t) * kLd;
-      float x[kPer];
-      if (is_v && !a.k_eq_v)
-        load(a.v, (size_t)(row0 + t) * a.v_ld + (size_t)h * D, x);
-      else
-        load(a.k, (size_t)(row0 + t) * a.k_ld + (size_t)h * D, x);
-      if (is_v) {
-        if (a.v_norm) normalise(x, a.eps, D);
-      } else {
-        if (a.k_w) {
-          normalise(x, a.eps, D);
-          gain(a.k_w, x);
-        }
-        rotate(x, row, t);
-        __syncwarp();
-      }
-      float m = 0.0f;
+    const uint32_t par = (h - h0) & 1;
+    float x[2][2][kChunks][2];  // [token][K, V]
+    {
+      Raw<T, kChunks> raw[2][2];
 #pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        row[(32 * (j / kVec) + lane) * kVec + j % kVec] = x[j];
-        m = fmaxf(m, fabsf(x[j]));  // a NaN does not count
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t t = tok + 8 * i;
+          if (t >= cnt || (uint32_t)w % subs != sub) continue;
+          const bool from_v = w == 1 && !a.k_eq_v;
+          raw[i][w].load(static_cast<const T *>(from_v ? a.v : a.k) +
+                             (size_t)(row0 + t) * (from_v ? a.v_ld : a.k_ld) + (size_t)h * D, lane);
+        }
+      if (by_buf) __syncthreads();  // the rows of buf lie over the tile
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t t = tok + 8 * i;
+          if (t >= cnt || (uint32_t)w % subs != sub) continue;
+          raw[i][w].unpack(x[i][w]);
+          if (w == 1) {
+            if (a.v_norm) normalise(x[i][w], a.eps);
+          } else {
+            if (a.k_w) {
+              normalise(x[i][w], a.eps);
+              gain(x[i][w], k_w, lane);
+            }
+            rotate(x[i][w], half, cs + t * half, buf, lane);
+          }
+          float m = 0.0f;
+#pragma unroll
+          for (int k = 0; k < kChunks; ++k)  // a NaN does not count
+            m = fmaxf(m, fmaxf(fabsf(x[i][w][k][0]), fabsf(x[i][w][k][1])));
+          m = warp_max(m);
+          if (lane == 0) amax[par][w][t] = m;
+        }
+    }
+    // ---- q heads of kv head h
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t t = tok + 8 * i;
+      if (t >= cnt) continue;
+      const T *src = static_cast<const T *>(a.q) + (size_t)(row0 + t) * a.q_ld + (size_t)h * a.gqa * D;
+      T *dst = static_cast<T *>(a.q_out) + (size_t)(row0 + t) * q_row + (size_t)h * a.gqa * D;
+      // vector 2 + g of the token belongs to warp (2 + g) % subs
+      uint32_t g = (sub + subs - 2 % subs) % subs;
+      Raw<T, kChunks> next;
+      if (g < a.gqa) next.load(src + (size_t)g * D, lane);
+      for (; g < a.gqa; g += subs) {
+        float y[kChunks][2];
+        next.unpack(y);
+        if (g + subs < a.gqa) next.load(src + (size_t)(g + subs) * D, lane);
+        if (a.q_w) {
+          normalise(y, a.eps);
+          gain(y, q_w, lane);
+        }
+        rotate(y, half, cs + t * half, buf, lane);
+        store_vector(dst + (size_t)g * D, lane, y);
       }
-      m = warp_max(m);
-      if (lane == 0) amax[is_v][t] = m;
     }
     __syncthreads();
+    // ---- the block's scales, and the owners' conversion
     const size_t rec = (((size_t)page * a.c.num_kv + h) * (a.c.page_tokens / kKv8Block) + in_page) * 2;
+    int e_old[2], e[2];
+    {
+      const uint32_t t = lane & 15;
+      float m = t < cnt ? amax[par][lane >> 4][t] : 0.0f;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      float m = 0.0f;
-      for (uint32_t t = 0; t < cnt; ++t) m = fmaxf(m, amax[w][t]);
-      const int e_old = fresh ? kKv8MinExp : kv8_scale_exponent(a.c.scale[rec + w]);
-      const int e = max(e_old, kv8_exponent(m));
-      const float inv = exp2_int(-e), shrink = exp2_int(e_old - e);
-      uint8_t *out = static_cast<uint8_t *>(a.c.data) + (rec + w) * (size_t)(kKv8Block * D);
-      const float *src = tile + w * kKv8Block * kLd;
-      // scale is read by all before one thread writes it (the barrier below)
-      for (uint32_t i = threadIdx.x; i < D; i += blockDim.x) {  // 16-byte pieces of the record
-        const uint32_t p = i >> 5, g = (i & 31) >> 2, c = i & 3;
-        uint4 old = make_uint4(0, 0, 0, 0);
-        uint32_t v[4];
-        if (w == 0) {
-          const bool n0 = g >= t0 && g < t0 + cnt, n1 = g + 8 >= t0 && g + 8 < t0 + cnt;
-          if (!fresh) {
-            if (!n0 && !n1 && e == e_old) continue;
-            if (!n0 || !n1) old = *reinterpret_cast<const uint4 *>(out + 16 * i);
-          }
-          v[0] = old.x; v[1] = old.y; v[2] = old.z; v[3] = old.w;
+      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      int was = kKv8MinExp;
+      if (!fresh) was = kv8_scale_exponent(a.c.scale[rec + (lane >> 4)]);
+      const int now = max(was, kv8_exponent(m));
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const bool is_new = q < 2 ? n0 : n1;
-            if (is_new) {
-              const float4 f = *reinterpret_cast<const float4 *>(src + (g + 8 * (q >> 1)) * kLd + 32 * p + 8 * c + 4 * (q & 1));
-              v[q] = e4m3_pack4(f.x * inv, f.y * inv, f.z * inv, f.w * inv);
-            } else if (e != e_old) {
-              const float4 f = e4m3_unpack4(v[q]);
-              v[q] = e4m3_pack4(f.x * shrink, f.y * shrink, f.z * shrink, f.w * shrink);
-            }
-          }
-        } else {
-          uint32_t is_new = 0;  // byte mask of the new tokens among 2 c, 2 c + 1, 2 c + 8, 2 c + 9
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const uint32_t t = 2 * c + (s & 1) + 8 * (s >> 1);
-            if (t >= t0 && t < t0 + cnt) is_new |= 0xFFu << (8 * s);
-          }
-          if (!fresh) {
-            if (is_new == 0 && e == e_old) continue;
-            if (is_new != 0xFFFFFFFFu) old = *reinterpret_cast<const uint4 *>(out + 16 * i);
-          }
-          v[0] = old.x; v[1] = old.y; v[2] = old.z; v[3] = old.w;
-          float f[4][4];  // [token][element]
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            const uint32_t t = 2 * c + (s & 1) + 8 * (s >> 1);
-            float4 x = make_float4(0, 0, 0, 0);
-            if ((is_new >> (8 * s)) & 1) x = *reinterpret_cast<const float4 *>(src + t * kLd + 32 * p + 4 * g);
-            f[s][0] = x.x; f[s][1] = x.y; f[s][2] = x.z; f[s][3] = x.w;
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (e != e_old) {
-              const float4 o = e4m3_unpack4(v[q]);
-              v[q] = e4m3_pack4(o.x * shrink, o.y * shrink, o.z * shrink, o.w * shrink);
-            }
-            const uint32_t n = e4m3_pack4(f[0][q] * inv, f[1][q] * inv, f[2][q] * inv, f[3][q] * inv);
-            v[q] = (n & is_new) | (v[q] & ~is_new);
-          }
-        }
-        *reinterpret_cast<uint4 *>(out + 16 * i) = make_uint4(v[0], v[1], v[2], v[3]);
+      for (int w = 0; w < 2; ++w) {
+        e_old[w] = __shfl_sync(0xffffffffu, was, 16 * w);
+        e[w] = __shfl_sync(0xffffffffu, now, 16 * w);
       }
     }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t t = tok + 8 * i;
+        if (t >= cnt || (uint32_t)w % subs != sub) continue;
+        const float inv = exp2_int(-e[w]);
+        uint8_t *row = tile + (w * kKv8Block + t0 + t) * kLd + 2 * lane;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k)
+          *reinterpret_cast<uint16_t *>(row + 64 * k) = (uint16_t)__nv_cvt_float2_to_fp8x2(
+              make_float2(x[i][w][k][0] * inv, x[i][w][k][1] * inv), __NV_SATFINITE, __NV_E4M3);
+      }
     __syncthreads();
-    if (threadIdx.x < 2) {
-      const uint32_t w = threadIdx.x;
-      float m = 0.0f;
-      for (uint32_t t = 0; t < cnt; ++t) m = fmaxf(m, amax[w][t]);
-      const int e_old = fresh ? kKv8MinExp : kv8_scale_exponent(a.c.scale[rec + w]);
-      a.c.scale[rec + w] = exp2_int(max(e_old, kv8_exponent(m)));
+    if (threadIdx.x < 2) a.c.scale[rec + threadIdx.x] = exp2_int(threadIdx.x ? e[1] : e[0]);
+    // ---- 16-byte pieces of the K record, then of the V record
+    uint8_t *const out = static_cast<uint8_t *>(a.c.data) + rec * (size_t)(kKv8Block * D);
+    for (uint32_t i = threadIdx.x; i < 2 * D; i += blockDim.x) {
+      const uint32_t w = i / D, p = i % D >> 5, g = (i & 31) >> 2, c = i & 3;
+      const uint8_t *src = tile + w * kKv8Block * kLd + 32 * p;
+      uint32_t v[4], is_new[4];  // the piece and which of its bytes are new
+      if (w == 0) {
+        const uint2 lo8 = *reinterpret_cast<const uint2 *>(src + g * kLd + 8 * c);
+        const uint2 hi8 = *reinterpret_cast<const uint2 *>(src + (g + 8) * kLd + 8 * c);
+        v[0] = lo8.x; v[1] = lo8.y; v[2] = hi8.x; v[3] = hi8.y;
+        is_new[0] = is_new[1] = g >= t0 && g < t0 + cnt ? 0xFFFFFFFFu : 0u;
+        is_new[2] = is_new[3] = g + 8 >= t0 && g + 8 < t0 + cnt ? 0xFFFFFFFFu : 0u;
+      } else {
+        uint32_t m = 0;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const uint32_t t = 2 * c + (s & 1) + 8 * (s >> 1);
+          v[s] = *reinterpret_cast<const uint32_t *>(src + t * kLd + 4 * g);
+          if (t >= t0 && t < t0 + cnt) m |= 0xFFu << (8 * s);
+        }
+        transpose4(v);
+        is_new[0] = is_new[1] = is_new[2] = is_new[3] = m;
+      }
+      uint4 *dst = reinterpret_cast<uint4 *>(out + 16 * i);
+      if ((is_new[0] & is_new[2]) != 0xFFFFFFFFu) {
+        uint4 old = make_uint4(0, 0, 0, 0);
+        if (!fresh) {
+          const int grow = w ? e[1] - e_old[1] : e[0] - e_old[0];
+          if (is_new[0] == 0 && is_new[2] == 0 && grow == 0) continue;
+          old = *dst;
+          if (grow != 0) {
+            const float shrink = exp2_int(-grow);
+            uint32_t o[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float4 f = e4m3_unpack4(o[k]);
+              o[k] = e4m3_pack4(f.x * shrink, f.y * shrink, f.z * shrink, f.w * shrink);
+            }
+            old = make_uint4(o[0], o[1], o[2], o[3]);
+          }
+        }
+        v[0] = (v[0] & is_new[0]) | (old.x & ~is_new[0]);
+        v[1] = (v[1] & is_new[1]) | (old.y & ~is_new[1]);
+        v[2] = (v[2] & is_new[2]) | (old.z & ~is_new[2]);
+        v[3] = (v[3] & is_new[3]) | (old.w & ~is_new[3]);
+      }
+      *dst = make_uint4(v[0], v[1], v[2], v[3]);
     }
   }
 }
 
 size_t append_smem(uint32_t d, uint32_t rot) {
-  return 2 * kKv8Block * (d + 4) * sizeof(float) + (size_t)kKv8Block * (rot / 2) * sizeof(float2);
+  return append_tile_bytes(d) + 2 * d * sizeof(float) + (size_t)kKv8Block * (rot / 2) * sizeof(float2);
 }
 
 using AppendKernel = void (*)(AppendArgs);
@@ -352,10 +469,16 @@ extern "C" SX_API sx_status sx_dispatch_kv8_append(
   a.inv_freq = inv_freq;
   a.eps = eps;
   a.err = e->err_dev;
-  a.heads_per_cta = 1;
+  // All kv heads of a unit in one CTA compute its angles once; with few units the heads are spread
+  // until every SM has work.
   const uint32_t units = tokens / sx::kKv8Block + 2 * c->num_seqs;
+  a.heads_per_cta = c->num_kv;
+  while (a.heads_per_cta > 1 && (uint64_t)units * ((c->num_kv + a.heads_per_cta - 1) / a.heads_per_cta) <
+                                    6ull * e->num_sms)
+    a.heads_per_cta = (a.heads_per_cta + 1) / 2;
   const dim3 grid(units, (c->num_kv + a.heads_per_cta - 1) / a.heads_per_cta);
-  sx::append_kernel(t, c->head_dim)<<<grid, sx::kAppWarps * 32,
-                                      sx::append_smem(c->head_dim, rotary_dim), e->stream>>>(a);
-  return sx_host_cuda_status(cudaGetLastError(), "kv8_append launch");
+  return sx_host_cuda_status(
+      sx::launch_chained(sx::append_kernel(t, c->head_dim), grid, dim3(sx::kAppWarps * 32),
+                         sx::append_smem(c->head_dim, rotary_dim), e->stream, 1, a),
+      "kv8_append launch");
 }

@@ -198,7 +198,7 @@ SX_DEV uint64_t warp_scan_u64(uint64_t v) {  // inclusive
 // lines, tokens) and one line is read again.
 constexpr uint32_t kLine = 128;
 
-__global__ void __launch_bounds__(kSampleThreads) verify_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kSampleThreads, 2) verify_kernel(VerifyArgs a) {
   __shared__ uint64_t warp_sums[kSampleWarps];
   __shared__ uint64_t part[2][kMaxCluster];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
