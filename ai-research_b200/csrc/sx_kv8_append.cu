@@ -12,11 +12,12 @@
 // alone and nothing is read back.
 //
 // Bound by the rows' bytes, and close behind by instructions: a vector of 256 has 45 cycles of an SM
-// at the copy rate.  A warp takes whole vectors; lane l holds elements 64 k + 2 l, + 1 of every
-// chunk k, so that a rotation over the first 64 touches one chunk (its pairs meet by one shuffle)
-// and one whose half is a multiple of 64 needs no exchange.  The angles are computed once per unit.
-// K and V stay in registers until the block's maxima have met in shared memory, are converted by
-// their owners, and leave through a byte tile that turns rows of tokens into the record's pieces.
+// at the copy rate.  A warp takes whole vectors; lane l holds elements 128 k + 4 l .. + 3 of every
+// chunk k (64 k + 2 l for heads of 64), so that a rotation whose half is a multiple of the chunk
+// needs no exchange and a shorter one meets its pairs by shuffles within chunk 0.  The angles are
+// computed once per unit.  K and V stay in registers until the block's maxima have met in shared
+// memory, are converted by their owners, and leave through a byte tile that turns rows of tokens
+// into the record's pieces.
 #include "sx_host.h"
 #include "sx_kv8.cuh"
 #include "sx_launch.cuh"
@@ -45,117 +46,152 @@ SX_HD constexpr uint32_t append_tile_bytes(uint32_t d) {
   return 2 * kKv8Block * (d + 32) > kAppWarps * d * 4 ? 2 * kKv8Block * (d + 32) : kAppWarps * d * 4;
 }
 
-// A lane's part of a vector as it stands in memory: one word (bf16) or two (f32) per chunk.
-template <typename T, int C>
+// Head size D: chunks of 32 lanes x V elements.
+template <int D>
+struct Lane {
+  static constexpr int kVec = D >= 128 ? 4 : 2;
+  static constexpr int kChunk = 32 * kVec;
+  static constexpr int kChunks = D / kChunk;
+};
+template <int D>
+using Elems = float[Lane<D>::kChunks][Lane<D>::kVec];
+
+// A lane's part of a vector as it stands in memory.
+template <typename T, int D>
 struct Raw {
-  static constexpr int kWords = sizeof(T) == 4 ? 2 : 1;
-  uint32_t w[C][kWords];
+  static constexpr int kWords = Lane<D>::kVec * (int)sizeof(T) / 4;
+  uint32_t w[Lane<D>::kChunks][kWords];
   SX_DEV void load(const T *p, uint32_t lane) {
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      if constexpr (kWords == 2) {
-        const uint2 u = *reinterpret_cast<const uint2 *>(p + 64 * k + 2 * lane);
-        w[k][0] = u.x;
-        w[k][1] = u.y;
+    for (int k = 0; k < Lane<D>::kChunks; ++k) {
+      const T *src = p + Lane<D>::kChunk * k + Lane<D>::kVec * lane;
+      if constexpr (kWords == 4) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(src);
+        w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
+      } else if constexpr (kWords == 2) {
+        const uint2 u = *reinterpret_cast<const uint2 *>(src);
+        w[k][0] = u.x; w[k][1] = u.y;
       } else {
-        w[k][0] = *reinterpret_cast<const uint32_t *>(p + 64 * k + 2 * lane);
+        w[k][0] = *reinterpret_cast<const uint32_t *>(src);
       }
     }
   }
-  SX_DEV void unpack(float (&x)[C][2]) const {
+  SX_DEV void unpack(Elems<D> &x) const {
 #pragma unroll
-    for (int k = 0; k < C; ++k) {
-      x[k][0] = __uint_as_float(kWords == 2 ? w[k][0] : w[k][0] << 16);
-      x[k][1] = __uint_as_float(kWords == 2 ? w[k][kWords - 1] : w[k][0] & 0xFFFF0000u);
-    }
+    for (int k = 0; k < Lane<D>::kChunks; ++k)
+#pragma unroll
+      for (int j = 0; j < Lane<D>::kVec; ++j) {
+        if constexpr (sizeof(T) == 4)
+          x[k][j] = __uint_as_float(w[k][j]);
+        else
+          x[k][j] = __uint_as_float(j & 1 ? w[k][j / 2] & 0xFFFF0000u : w[k][j / 2] << 16);
+      }
   }
 };
-template <typename T, int C>
-SX_DEV void store_vector(T *p, uint32_t lane, const float (&x)[C][2]) {
+template <typename T, int D>
+SX_DEV void store_vector(T *p, uint32_t lane, const Elems<D> &x) {
 #pragma unroll
-  for (int k = 0; k < C; ++k) store_vec<T, 2>(p + 64 * k + 2 * lane, x[k]);
+  for (int k = 0; k < Lane<D>::kChunks; ++k)
+    store_vec<T, Lane<D>::kVec>(p + Lane<D>::kChunk * k + Lane<D>::kVec * lane, x[k]);
 }
 
 // x / rms(x)
-template <int C>
-SX_DEV void normalise(float (&x)[C][2], float eps) {
+template <int D>
+SX_DEV void normalise(Elems<D> &x, float eps) {
   float ss = 0.0f;
 #pragma unroll
-  for (int k = 0; k < C; ++k) ss = fmaf(x[k][0], x[k][0], fmaf(x[k][1], x[k][1], ss));
-  const float rs = rsqrtf(warp_sum(ss) * (1.0f / (64 * C)) + eps);
+  for (int k = 0; k < Lane<D>::kChunks; ++k)
 #pragma unroll
-  for (int k = 0; k < C; ++k) {
-    x[k][0] = __fmul_rn(x[k][0], rs);
-    x[k][1] = __fmul_rn(x[k][1], rs);
+    for (int j = 0; j < Lane<D>::kVec; ++j) ss = fmaf(x[k][j], x[k][j], ss);
+  const float rs = rsqrtf(warp_sum(ss) * (1.0f / D) + eps);
+#pragma unroll
+  for (int k = 0; k < Lane<D>::kChunks; ++k)
+#pragma unroll
+    for (int j = 0; j < Lane<D>::kVec; ++j) x[k][j] = __fmul_rn(x[k][j], rs);
+}
+template <int D>
+SX_DEV void gain(Elems<D> &x, const float *w, uint32_t lane) {
+#pragma unroll
+  for (int k = 0; k < Lane<D>::kChunks; ++k) {
+    float g[Lane<D>::kVec];
+    load_vec<float, Lane<D>::kVec>(w + Lane<D>::kChunk * k + Lane<D>::kVec * lane, g);
+#pragma unroll
+    for (int j = 0; j < Lane<D>::kVec; ++j) x[k][j] = __fmul_rn(x[k][j], g[j]);
   }
 }
-template <int C>
-SX_DEV void gain(float (&x)[C][2], const float *w, uint32_t lane) {
-#pragma unroll
-  for (int k = 0; k < C; ++k) {
-    const float2 g = *reinterpret_cast<const float2 *>(w + 64 * k + 2 * lane);
-    x[k][0] = __fmul_rn(x[k][0], g.x);
-    x[k][1] = __fmul_rn(x[k][1], g.y);
-  }
-}
-// (x0, x1) turned by the angle with cosine and sine f: every product and sum rounded, as the engine
-SX_DEV float turn_low(float x0, float x1, float2 f) { return __fsub_rn(__fmul_rn(x0, f.x), __fmul_rn(x1, f.y)); }
-SX_DEV float turn_high(float x0, float x1, float2 f) { return __fadd_rn(__fmul_rn(x0, f.y), __fmul_rn(x1, f.x)); }
 
-// half = 64 H: the pairs are chunks k and k + H of one lane
-template <int H, int C>
-SX_DEV void rotate_chunks(float (&x)[C][2], const float2 *ct, uint32_t lane) {
-  if constexpr (2 * H <= C) {
-#pragma unroll
-    for (int k = 0; k < H; ++k)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float2 f = ct[64 * k + 2 * lane + j];
-        const float x0 = x[k][j], x1 = x[k + H][j];
-        x[k][j] = turn_low(x0, x1, f);
-        x[k + H][j] = turn_high(x0, x1, f);
-      }
-  }
-}
-// Any rotation: half up to 32 and even stays in chunk 0; the odd ones meet in buf (D floats).
-template <int C>
-SX_DEV void rotate(float (&x)[C][2], uint32_t half, const float2 *ct, float *buf, uint32_t lane) {
-  if (half == 0) return;
-  if (half <= 32 && half % 2 == 0) {
-    const uint32_t o = half / 2;
-    const bool low = lane < o, high = !low && lane < 2 * o;
-    const uint32_t peer = low ? lane + o : high ? lane - o : lane;
-    const float y0 = __shfl_sync(0xffffffffu, x[0][0], peer), y1 = __shfl_sync(0xffffffffu, x[0][1], peer);
-    if (low) {
-      x[0][0] = turn_low(x[0][0], y0, ct[2 * lane]);
-      x[0][1] = turn_low(x[0][1], y1, ct[2 * lane + 1]);
-    } else if (high) {
-      x[0][0] = turn_high(y0, x[0][0], ct[2 * lane - half]);
-      x[0][1] = turn_high(y1, x[0][1], ct[2 * lane + 1 - half]);
+// The rotation of one lane's elements.  Angles of a token: [cosines of the pairs | their sines].
+template <int D>
+struct Turn {
+  static constexpr int kVec = Lane<D>::kVec, kChunk = Lane<D>::kChunk, kChunks = Lane<D>::kChunks;
+  uint32_t half, mode;     // 0 none, 1 shuffles in chunk 0, 2 chunks of a lane, 3 by memory
+  uint32_t peer, at;       // mode 1: the lane of the partners, this lane's first pair
+  bool low, in;            //         first of the pairs; rotated at all
+  SX_DEV Turn(uint32_t half_, uint32_t lane) : half(half_), peer(lane), at(0), low(false), in(false) {
+    mode = half == 0 ? 0 : half % kChunk == 0 ? 2 : 2 * half <= (uint32_t)kChunk && half % kVec == 0 ? 1 : 3;
+    if (mode == 1) {
+      const uint32_t o = half / kVec;
+      low = lane < o;
+      in = lane < 2 * o;
+      peer = low ? lane + o : in ? lane - o : lane;
+      at = in ? kVec * (low ? lane : lane - o) : 0;
     }
-  } else if (half == 64) {
-    rotate_chunks<1>(x, ct, lane);
-  } else if (half == 128) {
-    rotate_chunks<2>(x, ct, lane);
-  } else if (half == 256) {
-    rotate_chunks<4>(x, ct, lane);
-  } else {
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < C; ++k) *reinterpret_cast<float2 *>(buf + 64 * k + 2 * lane) = make_float2(x[k][0], x[k][1]);
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < C; ++k)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint32_t d = 64 * k + 2 * lane + j;
-        if (d < half)
-          x[k][j] = turn_low(x[k][j], buf[d + half], ct[d]);
-        else if (d < 2 * half)
-          x[k][j] = turn_high(buf[d - half], x[k][j], ct[d - half]);
-      }
   }
-}
+  // every product and sum rounded by itself, as the engine's own rotation
+  template <int H>
+  SX_DEV void chunks(Elems<D> &x, const float *cs, uint32_t lane) const {
+    if constexpr (2 * H <= kChunks) {
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        float c[kVec], s[kVec];
+        load_vec<float, kVec>(cs + kChunk * k + kVec * lane, c);
+        load_vec<float, kVec>(cs + half + kChunk * k + kVec * lane, s);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const float x0 = x[k][j], x1 = x[k + H][j];
+          x[k][j] = __fsub_rn(__fmul_rn(x0, c[j]), __fmul_rn(x1, s[j]));
+          x[k + H][j] = __fadd_rn(__fmul_rn(x0, s[j]), __fmul_rn(x1, c[j]));
+        }
+      }
+    }
+  }
+  SX_DEV void operator()(Elems<D> &x, const float *cs, float *buf, uint32_t lane) const {
+    if (mode == 0) return;
+    if (mode == 1) {
+      float c[kVec], s[kVec];
+      load_vec<float, kVec>(cs + at, c);
+      load_vec<float, kVec>(cs + half + at, s);
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const float y = __fmul_rn(__shfl_sync(0xffffffffu, x[0][j], peer), s[j]);
+        const float r = __fadd_rn(__fmul_rn(x[0][j], c[j]), low ? -y : y);
+        if (in) x[0][j] = r;
+      }
+    } else if (mode == 2) {
+      if (half == kChunk)
+        chunks<1>(x, cs, lane);
+      else if (half == 2 * kChunk)
+        chunks<2>(x, cs, lane);
+    } else {
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) buf[kChunk * k + kVec * lane + j] = x[k][j];
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < kChunks; ++k)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const uint32_t d = kChunk * k + kVec * lane + j;
+          if (d < half)
+            x[k][j] = __fsub_rn(__fmul_rn(x[k][j], cs[d]), __fmul_rn(buf[d + half], cs[half + d]));
+          else if (d < 2 * half)
+            x[k][j] = __fadd_rn(__fmul_rn(buf[d - half], cs[d]), __fmul_rn(x[k][j], cs[d - half]));
+        }
+    }
+  }
+};
 
 // four rows' words of 4 bytes -> four words of one byte each row (a 4 x 4 byte transposition)
 SX_DEV void transpose4(uint32_t (&w)[4]) {
@@ -167,133 +203,112 @@ SX_DEV void transpose4(uint32_t (&w)[4]) {
   w[3] = prmt(c, d, 0x7632);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAppWarps * 32, D <= 256 ? 3 : 2) kv8_append_kernel(AppendArgs a) {
-  constexpr int kChunks = D / 64;
+// One 16-token block of one sequence.
+struct Unit {
+  uint32_t row0, cnt, t0;  // its new rows, how many, the first one's place in the block
+  uint32_t page, in_page;  // page and block of the page
+};
+
+// The kv heads [h0, h1) of a unit with their q heads.  FULL: all 16 tokens are new.
+template <typename T, int D, bool FULL>
+SX_DEV void append_heads(const AppendArgs &a, const Unit &u, uint32_t h0, uint32_t h1, uint8_t *sh,
+                         float (*amax)[2][kKv8Block]) {
+  constexpr int kChunks = Lane<D>::kChunks, kVec = Lane<D>::kVec, kChunk = Lane<D>::kChunk;
   constexpr int kLd = D + 32;  // bytes of a tile row
-  extern __shared__ __align__(16) uint8_t sh[];
-  __shared__ float amax[2][2][kKv8Block];  // [parity][K, V][token]
-  uint8_t *const tile = sh;                // [K, V][16][kLd]
+  uint8_t *const tile = sh;    // [K, V][16][kLd]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   float *const buf = reinterpret_cast<float *>(sh) + warp * D;
-  float *const q_w = reinterpret_cast<float *>(sh + append_tile_bytes(D)), *const k_w = q_w + D;
-  float2 *const cs = reinterpret_cast<float2 *>(k_w + D);  // [16][half]
-  const uint32_t half = a.rot / 2;
-  const bool by_buf = half != 0 && !(half <= 32 && half % 2 == 0) && half != 64 && half != 128 && half != 256;
-  pdl_launch_dependents();
-  pdl_wait();
-
-  const uint32_t u = blockIdx.x;
-  const uint32_t b = warp_last_le(a.c.num_seqs, u, [&](uint32_t i) { return a.row_start[i] / 16 + 2 * i; });
-  Kv8Rows r;
-  if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r)) {
-    if (threadIdx.x == 0) raise_error(a.err, kDevBadParams);
-    return;
-  }
-  const uint32_t pos0 = r.len - r.n;  // position of the sequence's first new row
-  const uint32_t rel = u - (r.r0 / 16 + 2 * b);
-  const uint32_t blk = pos0 / kKv8Block + rel;
-  if (r.n == 0 || blk * kKv8Block >= r.len) return;
-  const uint32_t lo = max(pos0, blk * kKv8Block), hi = min(r.len, (blk + 1) * kKv8Block);
-  const uint32_t row0 = r.r0 + (lo - pos0), cnt = hi - lo, t0 = lo % kKv8Block;
+  const float *const q_w = reinterpret_cast<const float *>(sh + append_tile_bytes(D)), *const k_w = q_w + D;
+  const float *const angles = k_w + D;  // [16][2 half]
+  const uint32_t cnt = FULL ? kKv8Block : u.cnt, t0 = FULL ? 0 : u.t0;
   const bool fresh = t0 == 0;
-  const uint32_t page = a.c.table[(size_t)b * a.c.max_pages + blk * kKv8Block / a.c.page_tokens];
-  if (page >= a.c.num_pages) {
-    if (threadIdx.x == 0) raise_error(a.err, kDevBadSlot);
-    return;
-  }
-  const uint32_t in_page = blk % (a.c.page_tokens / kKv8Block);
-
-  for (uint32_t i = threadIdx.x; i < cnt * half; i += blockDim.x) {
-    const uint32_t t = i / half, f = i - t * half;
-    float s, c;
-    sincosf(__fmul_rn((float)(lo + t), a.inv_freq[f]), &s, &c);
-    cs[i] = make_float2(c, s);
-  }
-  for (uint32_t i = threadIdx.x; i < D; i += blockDim.x) {
-    if (a.q_w) q_w[i] = a.q_w[i];
-    if (a.k_w) k_w[i] = a.k_w[i];
-  }
-  __syncthreads();
+  const Turn<D> turn(a.rot / 2, lane);
 
   // Tokens over warps: warp w takes tokens w % tw and w % tw + 8, and with few tokens the vectors
-  // of one (K, V, then q heads) are dealt to the warps that share it.
+  // of one (K, V, then q heads) are dealt to the warps that share it (tw and subs: powers of two).
   uint32_t tw = 8;
-  while (tw > 1 && tw / 2 >= cnt) tw /= 2;
-  const uint32_t tok = warp % tw, sub = warp / tw, subs = kAppWarps / tw;
-  const uint32_t h0 = blockIdx.y * a.heads_per_cta;
-  const uint32_t h1 = min(a.c.num_kv, h0 + a.heads_per_cta);
-  const size_t q_row = (size_t)a.c.num_kv * a.gqa * D;
+  if (!FULL)
+    while (tw > 1 && tw / 2 >= cnt) tw /= 2;
+  const uint32_t tok = warp & (tw - 1), sub = FULL ? 0 : warp / tw, subs = FULL ? 1 : kAppWarps / tw;
+  auto skip = [&](int i, int w) { return !FULL && (tok + 8 * i >= cnt || (w & (subs - 1)) != sub); };
+  const T *rows[2][2], *q_src[2];
+  T *q_dst[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const size_t row = u.row0 + tok + 8 * i;
+    rows[i][0] = static_cast<const T *>(a.k) + row * a.k_ld;
+    rows[i][1] = a.k_eq_v ? rows[i][0] : static_cast<const T *>(a.v) + row * a.v_ld;
+    q_src[i] = static_cast<const T *>(a.q) + row * a.q_ld;
+    q_dst[i] = static_cast<T *>(a.q_out) + row * ((size_t)a.c.num_kv * a.gqa * D);
+  }
   for (uint32_t h = h0; h < h1; ++h) {
     const uint32_t par = (h - h0) & 1;
-    float x[2][2][kChunks][2];  // [token][K, V]
+    float x[2][2][kChunks][kVec];  // [token][K, V]
     {
-      Raw<T, kChunks> raw[2][2];
+      Raw<T, D> raw[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          if (!skip(i, w)) raw[i][w].load(rows[i][w] + (size_t)h * D, lane);
+      if (turn.mode == 3) __syncthreads();  // the rows of buf lie over the tile
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
+          if (skip(i, w)) continue;
           const uint32_t t = tok + 8 * i;
-          if (t >= cnt || (uint32_t)w % subs != sub) continue;
-          const bool from_v = w == 1 && !a.k_eq_v;
-          raw[i][w].load(static_cast<const T *>(from_v ? a.v : a.k) +
-                             (size_t)(row0 + t) * (from_v ? a.v_ld : a.k_ld) + (size_t)h * D, lane);
-        }
-      if (by_buf) __syncthreads();  // the rows of buf lie over the tile
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t t = tok + 8 * i;
-          if (t >= cnt || (uint32_t)w % subs != sub) continue;
           raw[i][w].unpack(x[i][w]);
           if (w == 1) {
-            if (a.v_norm) normalise(x[i][w], a.eps);
+            if (a.v_norm) normalise<D>(x[i][w], a.eps);
           } else {
             if (a.k_w) {
-              normalise(x[i][w], a.eps);
-              gain(x[i][w], k_w, lane);
+              normalise<D>(x[i][w], a.eps);
+              gain<D>(x[i][w], k_w, lane);
             }
-            rotate(x[i][w], half, cs + t * half, buf, lane);
+            turn(x[i][w], angles + t * a.rot, buf, lane);
           }
           float m = 0.0f;
 #pragma unroll
-          for (int k = 0; k < kChunks; ++k)  // a NaN does not count
-            m = fmaxf(m, fmaxf(fabsf(x[i][w][k][0]), fabsf(x[i][w][k][1])));
+          for (int k = 0; k < kChunks; ++k)
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) m = fmaxf(m, fabsf(x[i][w][k][j]));  // a NaN does not count
           m = warp_max(m);
           if (lane == 0) amax[par][w][t] = m;
         }
     }
-    // ---- q heads of kv head h
+    // ---- q heads of kv head h, the next one's load in flight
+    {
+      // vector 2 + g of a token belongs to warp (2 + g) % subs
+      const uint32_t g0 = (sub - 2) & (subs - 1);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t t = tok + 8 * i;
-      if (t >= cnt) continue;
-      const T *src = static_cast<const T *>(a.q) + (size_t)(row0 + t) * a.q_ld + (size_t)h * a.gqa * D;
-      T *dst = static_cast<T *>(a.q_out) + (size_t)(row0 + t) * q_row + (size_t)h * a.gqa * D;
-      // vector 2 + g of the token belongs to warp (2 + g) % subs
-      uint32_t g = (sub + subs - 2 % subs) % subs;
-      Raw<T, kChunks> next;
-      if (g < a.gqa) next.load(src + (size_t)g * D, lane);
-      for (; g < a.gqa; g += subs) {
-        float y[kChunks][2];
-        next.unpack(y);
-        if (g + subs < a.gqa) next.load(src + (size_t)(g + subs) * D, lane);
-        if (a.q_w) {
-          normalise(y, a.eps);
-          gain(y, q_w, lane);
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t t = tok + 8 * i;
+        if (!FULL && t >= cnt) continue;
+        const T *src = q_src[i] + (size_t)h * a.gqa * D;
+        T *dst = q_dst[i] + (size_t)h * a.gqa * D;
+        Raw<T, D> next;
+        if (g0 < a.gqa) next.load(src + g0 * D, lane);
+        for (uint32_t g = g0; g < a.gqa; g += subs) {
+          Elems<D> y;
+          next.unpack(y);
+          if (g + subs < a.gqa) next.load(src + (g + subs) * D, lane);
+          if (a.q_w) {
+            normalise<D>(y, a.eps);
+            gain<D>(y, q_w, lane);
+          }
+          turn(y, angles + t * a.rot, buf, lane);
+          store_vector<T, D>(dst + g * D, lane, y);
         }
-        rotate(y, half, cs + t * half, buf, lane);
-        store_vector(dst + (size_t)g * D, lane, y);
       }
     }
     __syncthreads();
     // ---- the block's scales, and the owners' conversion
-    const size_t rec = (((size_t)page * a.c.num_kv + h) * (a.c.page_tokens / kKv8Block) + in_page) * 2;
+    const size_t rec = (((size_t)u.page * a.c.num_kv + h) * (a.c.page_tokens / kKv8Block) + u.in_page) * 2;
     int e_old[2], e[2];
     {
       const uint32_t t = lane & 15;
-      float m = t < cnt ? amax[par][lane >> 4][t] : 0.0f;
+      float m = FULL || t < cnt ? amax[par][lane >> 4][t] : 0.0f;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       int was = kKv8MinExp;
@@ -309,20 +324,24 @@ __global__ void __launch_bounds__(kAppWarps * 32, D <= 256 ? 3 : 2) kv8_append_k
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        const uint32_t t = tok + 8 * i;
-        if (t >= cnt || (uint32_t)w % subs != sub) continue;
+        if (skip(i, w)) continue;
         const float inv = exp2_int(-e[w]);
-        uint8_t *row = tile + (w * kKv8Block + t0 + t) * kLd + 2 * lane;
+        uint8_t *row = tile + (w * kKv8Block + t0 + tok + 8 * i) * kLd + kVec * lane;
 #pragma unroll
-        for (int k = 0; k < kChunks; ++k)
-          *reinterpret_cast<uint16_t *>(row + 64 * k) = (uint16_t)__nv_cvt_float2_to_fp8x2(
-              make_float2(x[i][w][k][0] * inv, x[i][w][k][1] * inv), __NV_SATFINITE, __NV_E4M3);
+        for (int k = 0; k < kChunks; ++k) {
+          if constexpr (kVec == 4)
+            *reinterpret_cast<uint32_t *>(row + kChunk * k) =
+                e4m3_pack4(x[i][w][k][0] * inv, x[i][w][k][1] * inv, x[i][w][k][2] * inv, x[i][w][k][3] * inv);
+          else
+            *reinterpret_cast<uint16_t *>(row + kChunk * k) = (uint16_t)__nv_cvt_float2_to_fp8x2(
+                make_float2(x[i][w][k][0] * inv, x[i][w][k][1] * inv), __NV_SATFINITE, __NV_E4M3);
+        }
       }
     __syncthreads();
     if (threadIdx.x < 2) a.c.scale[rec + threadIdx.x] = exp2_int(threadIdx.x ? e[1] : e[0]);
     // ---- 16-byte pieces of the K record, then of the V record
     uint8_t *const out = static_cast<uint8_t *>(a.c.data) + rec * (size_t)(kKv8Block * D);
-    for (uint32_t i = threadIdx.x; i < 2 * D; i += blockDim.x) {
+    for (uint32_t i = threadIdx.x; i < 2 * D; i += kAppWarps * 32) {
       const uint32_t w = i / D, p = i % D >> 5, g = (i & 31) >> 2, c = i & 3;
       const uint8_t *src = tile + w * kKv8Block * kLd + 32 * p;
       uint32_t v[4], is_new[4];  // the piece and which of its bytes are new
@@ -344,7 +363,7 @@ __global__ void __launch_bounds__(kAppWarps * 32, D <= 256 ? 3 : 2) kv8_append_k
         is_new[0] = is_new[1] = is_new[2] = is_new[3] = m;
       }
       uint4 *dst = reinterpret_cast<uint4 *>(out + 16 * i);
-      if ((is_new[0] & is_new[2]) != 0xFFFFFFFFu) {
+      if (!FULL && (is_new[0] & is_new[2]) != 0xFFFFFFFFu) {
         uint4 old = make_uint4(0, 0, 0, 0);
         if (!fresh) {
           const int grow = w ? e[1] - e_old[1] : e[0] - e_old[0];
@@ -371,8 +390,61 @@ __global__ void __launch_bounds__(kAppWarps * 32, D <= 256 ? 3 : 2) kv8_append_k
   }
 }
 
+template <typename T, int D>
+__global__ void __launch_bounds__(kAppWarps * 32, D <= 256 ? 3 : 2) kv8_append_kernel(AppendArgs a) {
+  extern __shared__ __align__(16) uint8_t sh[];
+  __shared__ float amax[2][2][kKv8Block];  // [parity][K, V][token]
+  pdl_launch_dependents();
+  pdl_wait();
+
+  const uint32_t u = blockIdx.x;
+  const uint32_t b = warp_last_le(a.c.num_seqs, u, [&](uint32_t i) { return a.row_start[i] / 16 + 2 * i; });
+  Kv8Rows r;
+  if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r)) {
+    if (threadIdx.x == 0) raise_error(a.err, kDevBadParams);
+    return;
+  }
+  const uint32_t pos0 = r.len - r.n;  // position of the sequence's first new row
+  const uint32_t rel = u - (r.r0 / 16 + 2 * b);
+  const uint32_t blk = pos0 / kKv8Block + rel;
+  if (r.n == 0 || blk * kKv8Block >= r.len) return;
+  const uint32_t lo = max(pos0, blk * kKv8Block), hi = min(r.len, (blk + 1) * kKv8Block);
+  Unit unit;
+  unit.row0 = r.r0 + (lo - pos0);
+  unit.cnt = hi - lo;
+  unit.t0 = lo % kKv8Block;
+  unit.page = a.c.table[(size_t)b * a.c.max_pages + blk * kKv8Block / a.c.page_tokens];
+  unit.in_page = blk % (a.c.page_tokens / kKv8Block);
+  if (unit.page >= a.c.num_pages) {
+    if (threadIdx.x == 0) raise_error(a.err, kDevBadSlot);
+    return;
+  }
+
+  float *const q_w = reinterpret_cast<float *>(sh + append_tile_bytes(D)), *const k_w = q_w + D;
+  float *const angles = k_w + D;
+  const uint32_t half = a.rot / 2;
+  for (uint32_t i = threadIdx.x; i < unit.cnt * half; i += blockDim.x) {
+    const uint32_t t = i / half, f = i - t * half;
+    float s, c;
+    sincosf(__fmul_rn((float)(lo + t), a.inv_freq[f]), &s, &c);
+    angles[t * a.rot + f] = c;
+    angles[t * a.rot + half + f] = s;
+  }
+  for (uint32_t i = threadIdx.x; i < D; i += blockDim.x) {
+    if (a.q_w) q_w[i] = a.q_w[i];
+    if (a.k_w) k_w[i] = a.k_w[i];
+  }
+  __syncthreads();
+  const uint32_t h0 = blockIdx.y * a.heads_per_cta;
+  const uint32_t h1 = min(a.c.num_kv, h0 + a.heads_per_cta);
+  if (unit.cnt == kKv8Block)
+    append_heads<T, D, true>(a, unit, h0, h1, sh, amax);
+  else
+    append_heads<T, D, false>(a, unit, h0, h1, sh, amax);
+}
+
 size_t append_smem(uint32_t d, uint32_t rot) {
-  return append_tile_bytes(d) + 2 * d * sizeof(float) + (size_t)kKv8Block * (rot / 2) * sizeof(float2);
+  return append_tile_bytes(d) + 2 * d * sizeof(float) + (size_t)kKv8Block * rot * sizeof(float);
 }
 
 using AppendKernel = void (*)(AppendArgs);
@@ -474,7 +546,7 @@ extern "C" SX_API sx_status sx_dispatch_kv8_append(
   const uint32_t units = tokens / sx::kKv8Block + 2 * c->num_seqs;
   a.heads_per_cta = c->num_kv;
   while (a.heads_per_cta > 1 && (uint64_t)units * ((c->num_kv + a.heads_per_cta - 1) / a.heads_per_cta) <
-                                    6ull * e->num_sms)
+                                    12ull * e->num_sms)
     a.heads_per_cta = (a.heads_per_cta + 1) / 2;
   const dim3 grid(units, (c->num_kv + a.heads_per_cta - 1) / a.heads_per_cta);
   return sx_host_cuda_status(
