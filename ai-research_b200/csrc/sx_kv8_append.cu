@@ -12,12 +12,13 @@
 // alone and nothing is read back.
 //
 // Bound by the rows' bytes, and close behind by instructions: a vector of 256 has 45 cycles of an SM
-// at the copy rate.  A warp takes whole vectors; lane l holds elements 128 k + 4 l .. + 3 of every
-// chunk k (64 k + 2 l for heads of 64), so that a rotation whose half is a multiple of the chunk
-// needs no exchange and a shorter one meets its pairs by shuffles within chunk 0.  The angles are
-// computed once per unit.  K and V stay in registers until the block's maxima have met in shared
-// memory, are converted by their owners, and leave through a byte tile that turns rows of tokens
-// into the record's pieces.
+// at the copy rate.  Half a warp takes a vector (a token of the unit each, when all 16 are new):
+// its sums are four shuffle steps for two vectors at once.  Lane l of the half holds elements
+// 64 k + 4 l .. + 3 of every chunk k, so that a rotation whose half is a multiple of 64 needs no
+// exchange and a shorter one meets its pairs by shuffles within chunk 0.  The angles are computed
+// once per unit.  K and V stay in registers until the block's maxima have met in shared memory, are
+// converted by their owners, and leave through a byte tile that turns rows of tokens into the
+// record's pieces.
 #include "sx_host.h"
 #include "sx_kv8.cuh"
 #include "sx_launch.cuh"
@@ -25,7 +26,8 @@
 namespace sx {
 namespace {
 
-constexpr int kAppWarps = 8;
+constexpr int kAppThreads = 256;
+constexpr int kWorkers = kAppThreads / 16;  // half warps
 
 struct AppendArgs {
   sx_kv8 c;
@@ -40,47 +42,53 @@ struct AppendArgs {
   uint32_t *err;
 };
 
-// shared memory: the byte tile (or a row of f32 per warp, for rotations whose pairs meet there),
+// shared memory: the byte tile (or a row of f32 per worker, for rotations whose pairs meet there),
 // the gains of q and k, the angles' cosines and sines
-SX_HD constexpr uint32_t append_tile_bytes(uint32_t d) {
-  return 2 * kKv8Block * (d + 32) > kAppWarps * d * 4 ? 2 * kKv8Block * (d + 32) : kAppWarps * d * 4;
+SX_HD constexpr uint32_t append_tile_bytes(uint32_t d, bool rows) {
+  return rows ? kWorkers * d * 4 : 2 * kKv8Block * (d + 32);
 }
 
-// Head size D: chunks of 32 lanes x V elements.
+// Head size D: chunks of 16 lanes x 4 elements.
+constexpr int kVec = 4, kChunk = 64;
 template <int D>
-struct Lane {
-  static constexpr int kVec = D >= 128 ? 4 : 2;
-  static constexpr int kChunk = 32 * kVec;
-  static constexpr int kChunks = D / kChunk;
-};
-template <int D>
-using Elems = float[Lane<D>::kChunks][Lane<D>::kVec];
+using Elems = float[D / kChunk][kVec];
+
+// the lanes of this thread's half warp, and sums and maxima over them
+SX_DEV uint32_t half_mask() { return 0xFFFFu << (threadIdx.x & 16); }
+SX_DEV float half_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(half_mask(), v, o);
+  return v;
+}
+SX_DEV float half_max(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(half_mask(), v, o));
+  return v;
+}
 
 // A lane's part of a vector as it stands in memory.
 template <typename T, int D>
 struct Raw {
-  static constexpr int kWords = Lane<D>::kVec * (int)sizeof(T) / 4;
-  uint32_t w[Lane<D>::kChunks][kWords];
-  SX_DEV void load(const T *p, uint32_t lane) {
+  static constexpr int kWords = kVec * (int)sizeof(T) / 4;
+  uint32_t w[D / kChunk][kWords];
+  SX_DEV void load(const T *p, uint32_t l) {
 #pragma unroll
-    for (int k = 0; k < Lane<D>::kChunks; ++k) {
-      const T *src = p + Lane<D>::kChunk * k + Lane<D>::kVec * lane;
+    for (int k = 0; k < D / kChunk; ++k) {
+      const T *src = p + kChunk * k + kVec * l;
       if constexpr (kWords == 4) {
         const uint4 u = *reinterpret_cast<const uint4 *>(src);
         w[k][0] = u.x; w[k][1] = u.y; w[k][2] = u.z; w[k][3] = u.w;
-      } else if constexpr (kWords == 2) {
+      } else {
         const uint2 u = *reinterpret_cast<const uint2 *>(src);
         w[k][0] = u.x; w[k][1] = u.y;
-      } else {
-        w[k][0] = *reinterpret_cast<const uint32_t *>(src);
       }
     }
   }
   SX_DEV void unpack(Elems<D> &x) const {
 #pragma unroll
-    for (int k = 0; k < Lane<D>::kChunks; ++k)
+    for (int k = 0; k < D / kChunk; ++k)
 #pragma unroll
-      for (int j = 0; j < Lane<D>::kVec; ++j) {
+      for (int j = 0; j < kVec; ++j) {
         if constexpr (sizeof(T) == 4)
           x[k][j] = __uint_as_float(w[k][j]);
         else
@@ -89,10 +97,9 @@ struct Raw {
   }
 };
 template <typename T, int D>
-SX_DEV void store_vector(T *p, uint32_t lane, const Elems<D> &x) {
+SX_DEV void store_vector(T *p, uint32_t l, const Elems<D> &x) {
 #pragma unroll
-  for (int k = 0; k < Lane<D>::kChunks; ++k)
-    store_vec<T, Lane<D>::kVec>(p + Lane<D>::kChunk * k + Lane<D>::kVec * lane, x[k]);
+  for (int k = 0; k < D / kChunk; ++k) store_vec<T, kVec>(p + kChunk * k + kVec * l, x[k]);
 }
 
 // x / rms(x)
@@ -100,52 +107,55 @@ template <int D>
 SX_DEV void normalise(Elems<D> &x, float eps) {
   float ss = 0.0f;
 #pragma unroll
-  for (int k = 0; k < Lane<D>::kChunks; ++k)
+  for (int k = 0; k < D / kChunk; ++k)
 #pragma unroll
-    for (int j = 0; j < Lane<D>::kVec; ++j) ss = fmaf(x[k][j], x[k][j], ss);
-  const float rs = rsqrtf(warp_sum(ss) * (1.0f / D) + eps);
+    for (int j = 0; j < kVec; ++j) ss = fmaf(x[k][j], x[k][j], ss);
+  const float rs = rsqrtf(half_sum(ss) * (1.0f / D) + eps);
 #pragma unroll
-  for (int k = 0; k < Lane<D>::kChunks; ++k)
+  for (int k = 0; k < D / kChunk; ++k)
 #pragma unroll
-    for (int j = 0; j < Lane<D>::kVec; ++j) x[k][j] = __fmul_rn(x[k][j], rs);
+    for (int j = 0; j < kVec; ++j) x[k][j] = __fmul_rn(x[k][j], rs);
 }
 template <int D>
-SX_DEV void gain(Elems<D> &x, const float *w, uint32_t lane) {
+SX_DEV void gain(Elems<D> &x, const float *w, uint32_t l) {
 #pragma unroll
-  for (int k = 0; k < Lane<D>::kChunks; ++k) {
-    float g[Lane<D>::kVec];
-    load_vec<float, Lane<D>::kVec>(w + Lane<D>::kChunk * k + Lane<D>::kVec * lane, g);
+  for (int k = 0; k < D / kChunk; ++k) {
+    float g[kVec];
+    load_vec<float, kVec>(w + kChunk * k + kVec * l, g);
 #pragma unroll
-    for (int j = 0; j < Lane<D>::kVec; ++j) x[k][j] = __fmul_rn(x[k][j], g[j]);
+    for (int j = 0; j < kVec; ++j) x[k][j] = __fmul_rn(x[k][j], g[j]);
   }
 }
 
 // The rotation of one lane's elements.  Angles of a token: [cosines of the pairs | their sines].
-template <int D>
+enum TurnMode : int { kTurnShuffle, kTurnChunks, kTurnMemory };
+inline TurnMode turn_mode(uint32_t half) {
+  if (half <= kChunk / 2 && half % kVec == 0) return kTurnShuffle;
+  return half == 64 || half == 128 || half == 256 ? kTurnChunks : kTurnMemory;
+}
+template <int D, TurnMode MODE>
 struct Turn {
-  static constexpr int kVec = Lane<D>::kVec, kChunk = Lane<D>::kChunk, kChunks = Lane<D>::kChunks;
-  uint32_t half, mode;     // 0 none, 1 shuffles in chunk 0, 2 chunks of a lane, 3 by memory
-  uint32_t peer, at;       // mode 1: the lane of the partners, this lane's first pair
-  bool low, in;            //         first of the pairs; rotated at all
-  SX_DEV Turn(uint32_t half_, uint32_t lane) : half(half_), peer(lane), at(0), low(false), in(false) {
-    mode = half == 0 ? 0 : half % kChunk == 0 ? 2 : 2 * half <= (uint32_t)kChunk && half % kVec == 0 ? 1 : 3;
-    if (mode == 1) {
+  uint32_t half;
+  uint32_t peer, at;  // shuffles: the lane of the partners, this lane's first pair
+  bool low, in;       //           first of the pairs; rotated at all
+  SX_DEV Turn(uint32_t half_, uint32_t l) : half(half_), peer(0), at(0), low(false), in(false) {
+    if (MODE == kTurnShuffle) {
       const uint32_t o = half / kVec;
-      low = lane < o;
-      in = lane < 2 * o;
-      peer = low ? lane + o : in ? lane - o : lane;
-      at = in ? kVec * (low ? lane : lane - o) : 0;
+      low = l < o;
+      in = l < 2 * o;
+      peer = (threadIdx.x & 16) | (low ? l + o : in ? l - o : l);
+      at = in ? kVec * (low ? l : l - o) : 0;
     }
   }
   // every product and sum rounded by itself, as the engine's own rotation
   template <int H>
-  SX_DEV void chunks(Elems<D> &x, const float *cs, uint32_t lane) const {
-    if constexpr (2 * H <= kChunks) {
+  SX_DEV void chunks(Elems<D> &x, const float *cs, uint32_t l) const {
+    if constexpr (2 * H <= D / kChunk) {
 #pragma unroll
       for (int k = 0; k < H; ++k) {
         float c[kVec], s[kVec];
-        load_vec<float, kVec>(cs + kChunk * k + kVec * lane, c);
-        load_vec<float, kVec>(cs + half + kChunk * k + kVec * lane, s);
+        load_vec<float, kVec>(cs + kChunk * k + kVec * l, c);
+        load_vec<float, kVec>(cs + half + kChunk * k + kVec * l, s);
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
           const float x0 = x[k][j], x1 = x[k + H][j];
@@ -155,35 +165,37 @@ struct Turn {
       }
     }
   }
-  SX_DEV void operator()(Elems<D> &x, const float *cs, float *buf, uint32_t lane) const {
-    if (mode == 0) return;
-    if (mode == 1) {
+  SX_DEV void operator()(Elems<D> &x, const float *cs, float *buf, uint32_t l) const {
+    if constexpr (MODE == kTurnShuffle) {
+      if (half == 0) return;  // no angles to read either
       float c[kVec], s[kVec];
       load_vec<float, kVec>(cs + at, c);
       load_vec<float, kVec>(cs + half + at, s);
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
-        const float y = __fmul_rn(__shfl_sync(0xffffffffu, x[0][j], peer), s[j]);
+        const float y = __fmul_rn(__shfl_sync(half_mask(), x[0][j], peer), s[j]);
         const float r = __fadd_rn(__fmul_rn(x[0][j], c[j]), low ? -y : y);
         if (in) x[0][j] = r;
       }
-    } else if (mode == 2) {
-      if (half == kChunk)
-        chunks<1>(x, cs, lane);
-      else if (half == 2 * kChunk)
-        chunks<2>(x, cs, lane);
+    } else if constexpr (MODE == kTurnChunks) {
+      if (half == 64)
+        chunks<1>(x, cs, l);
+      else if (half == 128)
+        chunks<2>(x, cs, l);
+      else
+        chunks<4>(x, cs, l);
     } else {
-      __syncwarp();
+      __syncwarp(half_mask());
 #pragma unroll
-      for (int k = 0; k < kChunks; ++k)
+      for (int k = 0; k < D / kChunk; ++k)
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) buf[kChunk * k + kVec * lane + j] = x[k][j];
-      __syncwarp();
+        for (int j = 0; j < kVec; ++j) buf[kChunk * k + kVec * l + j] = x[k][j];
+      __syncwarp(half_mask());
 #pragma unroll
-      for (int k = 0; k < kChunks; ++k)
+      for (int k = 0; k < D / kChunk; ++k)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
-          const uint32_t d = kChunk * k + kVec * lane + j;
+          const uint32_t d = kChunk * k + kVec * l + j;
           if (d < half)
             x[k][j] = __fsub_rn(__fmul_rn(x[k][j], cs[d]), __fmul_rn(buf[d + half], cs[half + d]));
           else if (d < 2 * half)
@@ -210,107 +222,90 @@ struct Unit {
 };
 
 // The kv heads [h0, h1) of a unit with their q heads.  FULL: all 16 tokens are new.
-template <typename T, int D, bool FULL>
+template <typename T, int D, TurnMode MODE, bool FULL>
 SX_DEV void append_heads(const AppendArgs &a, const Unit &u, uint32_t h0, uint32_t h1, uint8_t *sh,
                          float (*amax)[2][kKv8Block]) {
-  constexpr int kChunks = Lane<D>::kChunks, kVec = Lane<D>::kVec, kChunk = Lane<D>::kChunk;
   constexpr int kLd = D + 32;  // bytes of a tile row
   uint8_t *const tile = sh;    // [K, V][16][kLd]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float *const buf = reinterpret_cast<float *>(sh) + warp * D;
-  const float *const q_w = reinterpret_cast<const float *>(sh + append_tile_bytes(D)), *const k_w = q_w + D;
-  const float *const angles = k_w + D;  // [16][2 half]
+  const int lane = threadIdx.x & 31;
+  const uint32_t worker = threadIdx.x >> 4, l = threadIdx.x & 15;
+  float *const buf = reinterpret_cast<float *>(sh) + worker * D;
+  const float *const q_w = reinterpret_cast<const float *>(sh + append_tile_bytes(D, MODE == kTurnMemory));
+  const float *const k_w = q_w + D, *const angles = k_w + D;  // [16][2 half]
   const uint32_t cnt = FULL ? kKv8Block : u.cnt, t0 = FULL ? 0 : u.t0;
   const bool fresh = t0 == 0;
-  const Turn<D> turn(a.rot / 2, lane);
+  const Turn<D, MODE> turn(a.rot / 2, l);
 
-  // Tokens over warps: warp w takes tokens w % tw and w % tw + 8, and with few tokens the vectors
-  // of one (K, V, then q heads) are dealt to the warps that share it (tw and subs: powers of two).
-  uint32_t tw = 8;
+  // Worker w takes token w % tw; with few tokens the vectors of one (K, V, then q heads) are dealt
+  // to the workers that share it (tw and subs: powers of two).
+  uint32_t tw = kWorkers;
   if (!FULL)
     while (tw > 1 && tw / 2 >= cnt) tw /= 2;
-  const uint32_t tok = warp & (tw - 1), sub = FULL ? 0 : warp / tw, subs = FULL ? 1 : kAppWarps / tw;
-  auto skip = [&](int i, int w) { return !FULL && (tok + 8 * i >= cnt || (w & (subs - 1)) != sub); };
-  const T *rows[2][2], *q_src[2];
-  T *q_dst[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const size_t row = u.row0 + tok + 8 * i;
-    rows[i][0] = static_cast<const T *>(a.k) + row * a.k_ld;
-    rows[i][1] = a.k_eq_v ? rows[i][0] : static_cast<const T *>(a.v) + row * a.v_ld;
-    q_src[i] = static_cast<const T *>(a.q) + row * a.q_ld;
-    q_dst[i] = static_cast<T *>(a.q_out) + row * ((size_t)a.c.num_kv * a.gqa * D);
-  }
+  const uint32_t t = worker & (tw - 1), sub = FULL ? 0 : worker / tw, subs = FULL ? 1 : kWorkers / tw;
+  auto mine = [&](uint32_t w) { return FULL || (t < cnt && (w & (subs - 1)) == sub); };
+  const size_t row = u.row0 + t;
+  const T *const k_row = static_cast<const T *>(a.k) + row * a.k_ld;
+  const T *const v_row = a.k_eq_v ? k_row : static_cast<const T *>(a.v) + row * a.v_ld;
+  const T *const q_row = static_cast<const T *>(a.q) + row * a.q_ld;
+  T *const q_dst = static_cast<T *>(a.q_out) + row * ((size_t)a.c.num_kv * a.gqa * D);
+  const float *const cs = angles + t * a.rot;
   for (uint32_t h = h0; h < h1; ++h) {
     const uint32_t par = (h - h0) & 1;
-    float x[2][2][kChunks][kVec];  // [token][K, V]
-    {
-      Raw<T, D> raw[2][2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int w = 0; w < 2; ++w)
-          if (!skip(i, w)) raw[i][w].load(rows[i][w] + (size_t)h * D, lane);
-      if (turn.mode == 3) __syncthreads();  // the rows of buf lie over the tile
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if (skip(i, w)) continue;
-          const uint32_t t = tok + 8 * i;
-          raw[i][w].unpack(x[i][w]);
-          if (w == 1) {
-            if (a.v_norm) normalise<D>(x[i][w], a.eps);
-          } else {
-            if (a.k_w) {
-              normalise<D>(x[i][w], a.eps);
-              gain<D>(x[i][w], k_w, lane);
-            }
-            turn(x[i][w], angles + t * a.rot, buf, lane);
-          }
-          float m = 0.0f;
-#pragma unroll
-          for (int k = 0; k < kChunks; ++k)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) m = fmaxf(m, fabsf(x[i][w][k][j]));  // a NaN does not count
-          m = warp_max(m);
-          if (lane == 0) amax[par][w][t] = m;
-        }
-    }
+    Raw<T, D> raw[2];  // K, V: on their way while the q heads are worked on
+    if (mine(0)) raw[0].load(k_row + (size_t)h * D, l);
+    if (mine(1)) raw[1].load(v_row + (size_t)h * D, l);
+    if (MODE == kTurnMemory) __syncthreads();  // the rows of buf lie over the tile
     // ---- q heads of kv head h, the next one's load in flight
-    {
-      // vector 2 + g of a token belongs to warp (2 + g) % subs
-      const uint32_t g0 = (sub - 2) & (subs - 1);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t t = tok + 8 * i;
-        if (!FULL && t >= cnt) continue;
-        const T *src = q_src[i] + (size_t)h * a.gqa * D;
-        T *dst = q_dst[i] + (size_t)h * a.gqa * D;
-        Raw<T, D> next;
-        if (g0 < a.gqa) next.load(src + g0 * D, lane);
-        for (uint32_t g = g0; g < a.gqa; g += subs) {
-          Elems<D> y;
-          next.unpack(y);
-          if (g + subs < a.gqa) next.load(src + (g + subs) * D, lane);
-          if (a.q_w) {
-            normalise<D>(y, a.eps);
-            gain<D>(y, q_w, lane);
-          }
-          turn(y, angles + t * a.rot, buf, lane);
-          store_vector<T, D>(dst + g * D, lane, y);
+    if (FULL || t < cnt) {
+      // vector 2 + g of a token belongs to worker (2 + g) % subs of it
+      uint32_t g = (sub - 2) & (subs - 1);
+      const T *src = q_row + (size_t)(h * a.gqa + g) * D;
+      T *dst = q_dst + (size_t)(h * a.gqa + g) * D;
+      Raw<T, D> next;
+      if (g < a.gqa) next.load(src, l);
+      for (; g < a.gqa; g += subs, dst += subs * D) {
+        Elems<D> y;
+        next.unpack(y);
+        src += subs * D;
+        if (g + subs < a.gqa) next.load(src, l);
+        if (a.q_w) {
+          normalise<D>(y, a.eps);
+          gain<D>(y, q_w, l);
         }
+        turn(y, cs, buf, l);
+        store_vector<T, D>(dst, l, y);
       }
+    }
+    // ---- K and V
+    Elems<D> x[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if (!mine(w)) continue;
+      raw[w].unpack(x[w]);
+      if (w == 1) {
+        if (a.v_norm) normalise<D>(x[w], a.eps);
+      } else {
+        if (a.k_w) {
+          normalise<D>(x[w], a.eps);
+          gain<D>(x[w], k_w, l);
+        }
+        turn(x[w], cs, buf, l);
+      }
+      float m = 0.0f;
+#pragma unroll
+      for (int k = 0; k < D / kChunk; ++k)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) m = fmaxf(m, fabsf(x[w][k][j]));  // a NaN does not count
+      m = half_max(m);
+      if (l == 0) amax[par][w][t] = m;
     }
     __syncthreads();
     // ---- the block's scales, and the owners' conversion
     const size_t rec = (((size_t)u.page * a.c.num_kv + h) * (a.c.page_tokens / kKv8Block) + u.in_page) * 2;
     int e_old[2], e[2];
     {
-      const uint32_t t = lane & 15;
-      float m = FULL || t < cnt ? amax[par][lane >> 4][t] : 0.0f;
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float m = FULL || l < cnt ? amax[par][lane >> 4][l] : 0.0f;
+      m = half_max(m);
       int was = kKv8MinExp;
       if (!fresh) was = kv8_scale_exponent(a.c.scale[rec + (lane >> 4)]);
       const int now = max(was, kv8_exponent(m));
@@ -321,27 +316,20 @@ SX_DEV void append_heads(const AppendArgs &a, const Unit &u, uint32_t h0, uint32
       }
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int w = 0; w < 2; ++w) {
+      if (!mine(w)) continue;
+      const float inv = exp2_int(-e[w]);
+      uint8_t *dst = tile + (w * kKv8Block + t0 + t) * kLd + kVec * l;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        if (skip(i, w)) continue;
-        const float inv = exp2_int(-e[w]);
-        uint8_t *row = tile + (w * kKv8Block + t0 + tok + 8 * i) * kLd + kVec * lane;
-#pragma unroll
-        for (int k = 0; k < kChunks; ++k) {
-          if constexpr (kVec == 4)
-            *reinterpret_cast<uint32_t *>(row + kChunk * k) =
-                e4m3_pack4(x[i][w][k][0] * inv, x[i][w][k][1] * inv, x[i][w][k][2] * inv, x[i][w][k][3] * inv);
-          else
-            *reinterpret_cast<uint16_t *>(row + kChunk * k) = (uint16_t)__nv_cvt_float2_to_fp8x2(
-                make_float2(x[i][w][k][0] * inv, x[i][w][k][1] * inv), __NV_SATFINITE, __NV_E4M3);
-        }
-      }
+      for (int k = 0; k < D / kChunk; ++k)
+        *reinterpret_cast<uint32_t *>(dst + kChunk * k) =
+            e4m3_pack4(x[w][k][0] * inv, x[w][k][1] * inv, x[w][k][2] * inv, x[w][k][3] * inv);
+    }
     __syncthreads();
     if (threadIdx.x < 2) a.c.scale[rec + threadIdx.x] = exp2_int(threadIdx.x ? e[1] : e[0]);
     // ---- 16-byte pieces of the K record, then of the V record
     uint8_t *const out = static_cast<uint8_t *>(a.c.data) + rec * (size_t)(kKv8Block * D);
-    for (uint32_t i = threadIdx.x; i < 2 * D; i += kAppWarps * 32) {
+    for (uint32_t i = threadIdx.x; i < 2 * D; i += kAppThreads) {
       const uint32_t w = i / D, p = i % D >> 5, g = (i & 31) >> 2, c = i & 3;
       const uint8_t *src = tile + w * kKv8Block * kLd + 32 * p;
       uint32_t v[4], is_new[4];  // the piece and which of its bytes are new
@@ -349,15 +337,15 @@ SX_DEV void append_heads(const AppendArgs &a, const Unit &u, uint32_t h0, uint32
         const uint2 lo8 = *reinterpret_cast<const uint2 *>(src + g * kLd + 8 * c);
         const uint2 hi8 = *reinterpret_cast<const uint2 *>(src + (g + 8) * kLd + 8 * c);
         v[0] = lo8.x; v[1] = lo8.y; v[2] = hi8.x; v[3] = hi8.y;
-        is_new[0] = is_new[1] = g >= t0 && g < t0 + cnt ? 0xFFFFFFFFu : 0u;
-        is_new[2] = is_new[3] = g + 8 >= t0 && g + 8 < t0 + cnt ? 0xFFFFFFFFu : 0u;
+        is_new[0] = is_new[1] = g - t0 < cnt ? 0xFFFFFFFFu : 0u;
+        is_new[2] = is_new[3] = g + 8 - t0 < cnt ? 0xFFFFFFFFu : 0u;
       } else {
         uint32_t m = 0;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           const uint32_t t = 2 * c + (s & 1) + 8 * (s >> 1);
           v[s] = *reinterpret_cast<const uint32_t *>(src + t * kLd + 4 * g);
-          if (t >= t0 && t < t0 + cnt) m |= 0xFFu << (8 * s);
+          if (t - t0 < cnt) m |= 0xFFu << (8 * s);
         }
         transpose4(v);
         is_new[0] = is_new[1] = is_new[2] = is_new[3] = m;
@@ -390,8 +378,9 @@ SX_DEV void append_heads(const AppendArgs &a, const Unit &u, uint32_t h0, uint32
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kAppWarps * 32, D <= 256 ? 3 : 2) kv8_append_kernel(AppendArgs a) {
+template <typename T, int D, TurnMode MODE>
+__global__ void __launch_bounds__(kAppThreads, D * sizeof(T) <= 512 ? 4 : D <= 256 ? 3 : 2)
+    kv8_append_kernel(AppendArgs a) {
   extern __shared__ __align__(16) uint8_t sh[];
   __shared__ float amax[2][2][kKv8Block];  // [parity][K, V][token]
   pdl_launch_dependents();
@@ -420,7 +409,7 @@ __global__ void __launch_bounds__(kAppWarps * 32, D <= 256 ? 3 : 2) kv8_append_k
     return;
   }
 
-  float *const q_w = reinterpret_cast<float *>(sh + append_tile_bytes(D)), *const k_w = q_w + D;
+  float *const q_w = reinterpret_cast<float *>(sh + append_tile_bytes(D, MODE == kTurnMemory)), *const k_w = q_w + D;
   float *const angles = k_w + D;
   const uint32_t half = a.rot / 2;
   for (uint32_t i = threadIdx.x; i < unit.cnt * half; i += blockDim.x) {
@@ -438,33 +427,45 @@ __global__ void __launch_bounds__(kAppWarps * 32, D <= 256 ? 3 : 2) kv8_append_k
   const uint32_t h0 = blockIdx.y * a.heads_per_cta;
   const uint32_t h1 = min(a.c.num_kv, h0 + a.heads_per_cta);
   if (unit.cnt == kKv8Block)
-    append_heads<T, D, true>(a, unit, h0, h1, sh, amax);
+    append_heads<T, D, MODE, true>(a, unit, h0, h1, sh, amax);
   else
-    append_heads<T, D, false>(a, unit, h0, h1, sh, amax);
+    append_heads<T, D, MODE, false>(a, unit, h0, h1, sh, amax);
 }
 
 size_t append_smem(uint32_t d, uint32_t rot) {
-  return append_tile_bytes(d) + 2 * d * sizeof(float) + (size_t)kKv8Block * rot * sizeof(float);
+  return append_tile_bytes(d, turn_mode(rot / 2) == kTurnMemory) + 2 * d * sizeof(float) +
+         (size_t)kKv8Block * rot * sizeof(float);
 }
 
 using AppendKernel = void (*)(AppendArgs);
-AppendKernel append_kernel(sx_dtype t, uint32_t d) {
-  if (t == SX_F32)
-    return d == 64 ? kv8_append_kernel<float, 64> : d == 128 ? kv8_append_kernel<float, 128>
-         : d == 256 ? kv8_append_kernel<float, 256> : kv8_append_kernel<float, 512>;
-  return d == 64 ? kv8_append_kernel<__nv_bfloat16, 64> : d == 128 ? kv8_append_kernel<__nv_bfloat16, 128>
-       : d == 256 ? kv8_append_kernel<__nv_bfloat16, 256> : kv8_append_kernel<__nv_bfloat16, 512>;
+template <typename T, int D>
+AppendKernel append_kernel(uint32_t half) {
+  switch (turn_mode(half)) {
+    case kTurnShuffle: return kv8_append_kernel<T, D, kTurnShuffle>;
+    case kTurnChunks: return kv8_append_kernel<T, D, kTurnChunks>;
+    default: return kv8_append_kernel<T, D, kTurnMemory>;
+  }
+}
+template <typename T>
+AppendKernel append_kernel(uint32_t d, uint32_t half) {
+  return d == 64 ? append_kernel<T, 64>(half) : d == 128 ? append_kernel<T, 128>(half)
+       : d == 256 ? append_kernel<T, 256>(half) : append_kernel<T, 512>(half);
+}
+AppendKernel append_kernel(sx_dtype t, uint32_t d, uint32_t half) {
+  return t == SX_F32 ? append_kernel<float>(d, half) : append_kernel<__nv_bfloat16>(d, half);
 }
 
 }  // namespace
 
 cudaError_t prepare_kv8_append() {
   for (uint32_t d : {64u, 128u, 256u, 512u})
-    for (sx_dtype t : {SX_F32, SX_BF16}) {
-      const cudaError_t e = cudaFuncSetAttribute(
-          append_kernel(t, d), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)append_smem(d, d));
-      if (e != cudaSuccess) return e;
-    }
+    for (sx_dtype t : {SX_F32, SX_BF16})
+      for (uint32_t half : {0u, 64u, 1u}) {  // one of each rotation
+        const cudaError_t e = cudaFuncSetAttribute(append_kernel(t, d, half),
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   (int)(append_tile_bytes(d, true) + append_smem(d, d)));
+        if (e != cudaSuccess) return e;
+      }
   return cudaSuccess;
 }
 
@@ -550,7 +551,7 @@ extern "C" SX_API sx_status sx_dispatch_kv8_append(
     a.heads_per_cta = (a.heads_per_cta + 1) / 2;
   const dim3 grid(units, (c->num_kv + a.heads_per_cta - 1) / a.heads_per_cta);
   return sx_host_cuda_status(
-      sx::launch_chained(sx::append_kernel(t, c->head_dim), grid, dim3(sx::kAppWarps * 32),
+      sx::launch_chained(sx::append_kernel(t, c->head_dim, rotary_dim / 2), grid, dim3(sx::kAppThreads),
                          sx::append_smem(c->head_dim, rotary_dim), e->stream, 1, a),
       "kv8_append launch");
 }
