@@ -6,6 +6,7 @@
 //   descriptor set         -> ordered tuple of device buffers
 //   vkQueueSubmit + fence  -> cudaGraphLaunch + deadline-bounded cudaStreamQuery poll
 // Nothing here falls back to the CPU: every op is a CUDA kernel from csrc/.
+#include <algorithm>
 #include <chrono>
 #include <cmath>
 #include <cstdarg>
@@ -613,7 +614,7 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
       size_t o_done = take(256);
       size_t o_amax = take(sx::argmax_scratch_bytes());
       size_t o_pbar = take(256);
-      size_t o_kpart = take(sx::kv8_part_bytes(e->num_sms));
+      size_t o_kpart = take(std::max(sx::kv8_part_bytes(e->num_sms), sx::kv8_prompt_part_bytes(e->num_sms)));
       size_t o_kcnt = take((size_t)e->num_sms * 2 * 4);
       e->scratch_bytes = off;
       st = cuda_status(cudaMalloc(&e->scratch, e->scratch_bytes), "engine scratch");
@@ -652,6 +653,8 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
     st = cuda_status(sx::prepare_kv8_append(), "kv8 append kernel attributes");
     if (st) break;
     st = cuda_status(sx::prepare_kv8_attn(), "kv8 attention kernel attributes");
+    if (st) break;
+    st = cuda_status(sx::prepare_kv8_prompt(), "kv8 prompt attention kernel attributes");
     if (st) break;
     st = cuda_status(sx::prepare_sample_kernels(), "probability kernel attributes");
   } while (0);

@@ -340,6 +340,9 @@ cudaError_t prepare_kv8_append();
 // and its attention (sx_kv8_attn.cu): scratch for the parts of split problems
 cudaError_t prepare_kv8_attn();
 size_t kv8_part_bytes(int num_sms);
+// its form for many rows per kv head (sx_kv8_prompt.cu); the arguments are in sx_kv8.cuh
+cudaError_t prepare_kv8_prompt();
+size_t kv8_prompt_part_bytes(int num_sms);
 // Probabilities and verification (sx_sample.cu)
 cudaError_t prepare_sample_kernels();
 

@@ -130,4 +130,44 @@ SX_DEV void store_vec(T *p, const float (&v)[VEC]) {
     *reinterpret_cast<uint32_t *>(p) = w[0];
 }
 
+// ---- attention
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Kv8AttnArgs {
+  sx_kv8 c;
+  const void *q;
+  void *out;
+  uint32_t q_ld, out_ld;
+  const uint32_t *row_start, *kv_len;
+  uint32_t tokens, num_q, window, gqa, min_run;
+  float scale;
+  float *part;      // parts of split problems: [2 grid][rows] x {m, l}, then [2 grid][rows][D]
+  uint32_t *cnt;    // [grid], zero at rest
+  uint32_t *err;
+};
+
+SX_DEV float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+  return r;
+}
+SX_DEV uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&h);
+}
+// what f16 rounding left of the pair
+SX_DEV uint32_t pack_f16_rest(float lo, float hi, uint32_t rounded) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&rounded));
+  return pack_f16(lo - f.x, hi - f.y);
+}
+
+// Count an arrival on behalf of a CTA whose threads met at a barrier before: their writes are
+// released by it, and those of the CTAs counted before are acquired.
+SX_DEV uint32_t arrive_acq_rel(uint32_t *cnt) {
+  uint32_t r;
+  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;\n" : "=r"(r) : "l"(cnt) : "memory");
+  return r;
+}
+cudaError_t launch_kv8_prompt(Kv8AttnArgs a, sx_dtype t, int num_sms, cudaStream_t s);
+
 }  // namespace sx

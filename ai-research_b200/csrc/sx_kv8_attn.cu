@@ -33,48 +33,12 @@ constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr uint32_t kOverhead = 8;  // blocks a problem's start and end are worth
 constexpr float kPOffset = 10.0f;
-constexpr float kLog2e = 1.4426950408889634f;
 
-struct Kv8AttnArgs {
-  sx_kv8 c;
-  const void *q;
-  void *out;
-  uint32_t q_ld, out_ld;
-  const uint32_t *row_start, *kv_len;
-  uint32_t tokens, num_q, window, gqa, min_run;
-  float scale;
-  float *part;      // [2 grid][8 NT] x {m, l}, then [2 grid][8 NT][D]
-  uint32_t *cnt;    // [grid], zero at rest
-  uint32_t *err;
-};
-
-SX_DEV float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
-  return r;
-}
 SX_DEV uint32_t movmatrix_trans(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
-SX_DEV uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-// Count an arrival on behalf of a CTA whose threads met at a barrier before: their writes are
-// released by it, and those of the CTAs counted before are acquired.
-SX_DEV uint32_t arrive_acq_rel(uint32_t *cnt) {
-  uint32_t r;
-  asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;\n" : "=r"(r) : "l"(cnt) : "memory");
-  return r;
-}
-// what f16 rounding left of the pair
-SX_DEV uint32_t pack_f16_rest(float lo, float hi, uint32_t rounded) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&rounded));
-  return pack_f16(lo - f.x, hi - f.y);
-}
-
 // The blocks of 16 tokens that rows of a sequence see.
 SX_DEV void seen_blocks(const Kv8Rows &r, uint32_t window, uint32_t *first, uint32_t *count) {
   const uint32_t pos0 = r.len - r.n;  // of the first row
@@ -723,8 +687,10 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
   a.part = e->kv8_part;
   a.cnt = e->kv8_cnt;
   a.err = e->err_dev;
-  // packed rows of an average sequence
+  // Packed rows of an average sequence: past 16 the tcgen05 form, which takes 128 at a time.
   const uint64_t avg = (uint64_t)((tokens + c->num_seqs - 1) / c->num_seqs) * a.gqa;
+  if (avg > 16 && c->head_dim <= 256)
+    return sx_host_cuda_status(sx::launch_kv8_prompt(a, t, e->num_sms, e->stream), "kv8_attn launch");
   const sx::DecVariant v = sx::dec_variant(t, c->head_dim, avg <= 8 ? 0 : avg <= 16 ? 1 : 2);
   return sx_host_cuda_status(
       sx::launch_chained(v.fn, dim3(e->num_sms * v.ctas), dim3(sx::kDecThreads), v.smem, e->stream, 1, a),

@@ -1,0 +1,691 @@
+// sx_kv8_prompt.cu -- attention over the paged 8-bit KV cache for many rows per kv head, on
+// tcgen05 tensor cores (include/sx.h, sx_dispatch_kv8_attn).
+//
+//   S = Q K^T (128 packed rows x kTokens keys),  P = 2^(x + log2(v scale) - m + 6),  O += P V
+//
+// 128 packed rows (new tokens x q heads of one kv head) are the M of both products; S and O live in
+// tensor memory, P goes back there as f16 over S and is the second product's A operand.  e4m3 is
+// exact in f16, so K and V are widened on the way to shared memory; f32 rows split Q and P into two
+// f16 terms, with twice the products.  Warps:
+//   0 .. 3   softmax, a thread per row: S from tensor memory twice (maximum, then exponentials), P
+//            back.  The maximum that the exponentials refer to moves only when it grows by 2^8; the
+//            row of O is then rescaled in tensor memory.
+//   4 ..     widen K and V.  A warp takes a pair of blocks (32 tokens): the cache's 16-byte pieces
+//            become 16-byte stores of the 128-byte-swizzled tiles for a fitting order of the tokens
+//            (tile position 32 q + 8 (t % 8 / 2) + 4 half + 2 (t / 8) + t % 2) and of V's elements
+//            (tile row 32 p + 8 (d % 4) + f(d % 32 / 4), f a permutation of 8).  The softmax undoes
+//            the first in its masks and scales, the output the second: both are register indexes.
+//   last     one thread issues the products.
+// Bound by shared memory (the tiles' stores and the products' reads) and exponentials (16 a cycle
+// and SM, as many as a product of head size 128 takes cycles).  Up to head size 128 two CTAs share an
+// SM and fill each other's waits; above, two S tiles let the next product run beside the softmax.
+//
+// Work is the line of sx_kv8_attn.cu with problems of their own length: row group k of a sequence
+// sees pos0 + 128 (k + 1) / G keys at most, so the line counts keys x G, whose sums are closed
+// forms; a tile belongs to the CTA in whose run its first key lies.
+#include "sx_host.h"
+#include "sx_kv8.cuh"
+#include "sx_launch.cuh"
+#include "sx_tcgen05.cuh"
+
+namespace sx {
+namespace {
+
+constexpr uint32_t kRows = 128;      // packed rows of a problem
+constexpr float kPromptOffset = 6.0f, kSlack = 8.0f;
+
+template <int D, bool SPLIT>
+struct PromptShape {
+  static constexpr int kCtas = D <= 128 && !(D == 128 && SPLIT) ? 2 : 1;  // per SM
+  static constexpr int kTokens = D == 256 && SPLIT ? 64 : 128;            // of a tile
+  static constexpr int kS = kCtas == 2 ? 1 : 2;                           // S tiles
+  static constexpr int kWiden = kCtas == 2 ? 4 : 8;                       // warps that widen
+  static constexpr int kThreads = (4 + kWiden + 1) * 32;
+  static constexpr int kTerms = SPLIT ? 2 : 1;
+  static constexpr int kQTerm = (int)kRows * D * 2;
+  static constexpr int kTile = kTokens * D * 2;
+  static constexpr int kSmem = kTerms * kQTerm + 2 * kTile + 1024;        // + alignment
+  // tensor memory columns: S tiles (P over them), low terms of P, O
+  static constexpr int kLow = kS * kTokens;
+  static constexpr int kO = kLow + (SPLIT ? kS * kTokens / 2 : 0);
+  static constexpr int kCols = kO + D <= 256 ? 256 : 512;
+  static_assert(kO + D <= 512 && kCols * kCtas <= 512, "tensor memory");
+};
+
+// Costs on the line: keys x G of a row group, at most `cap` with a window, plus `over`.
+struct GroupCost {
+  uint64_t base, cap, over;  // pos0 * G; the most a group sees; what starting one costs
+  uint32_t groups;
+  SX_DEV uint64_t of(uint32_t k) const {
+    const uint64_t c = base + (uint64_t)kRows * (k + 1);
+    return (c < cap ? c : cap) + over;
+  }
+  SX_DEV uint64_t before(uint32_t k) const {  // of the groups below k
+    uint64_t full = cap > base ? (cap - base) / kRows : 0;  // groups under the cap
+    if (full > k) full = k;
+    return full * base + kRows * (full * (full + 1) / 2) + (k - full) * cap + k * over;
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (PromptShape<D, sizeof(T) == 4>::kCtas))
+    kv8_prompt_kernel(Kv8AttnArgs a) {
+  constexpr bool kSplit = sizeof(T) == 4;
+  using P = PromptShape<D, kSplit>;
+  constexpr int kTokens = P::kTokens, kS = P::kS, kWiden = P::kWiden, kTerms = P::kTerms;
+  constexpr int kTileBlocks = kTokens / kKv8Block;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[6];
+  __shared__ uint32_t tmem_slot, last_flag, nan_mask[2][kTokens / 32];
+  __shared__ volatile uint32_t abort_flag;
+  __shared__ float row_mul[kRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const uint32_t q_tile = (smem_u32(smem_raw) + 1023) & ~1023u;  // [terms][D / 64][128 rows][128 B]
+  const uint32_t k_tile = q_tile + kTerms * P::kQTerm;           // [D / 64][tokens][128 B]
+  const uint32_t v_tile = k_tile + P::kTile;                     // [tokens / 64][D][128 B]
+  const uint32_t bar = smem_u32(bars);
+  const uint32_t k_full = bar, v_full = bar + 8, p_full = bar + 16, pv_done = bar + 24;
+  auto s_done = [&](uint32_t t) { return bar + 32 + 8 * (t % kS); };
+  if (threadIdx.x == 0) {
+    mbar_init(k_full, kWiden);
+    mbar_init(v_full, kWiden);
+    mbar_init(p_full, 4);
+    mbar_init(pv_done, 1);
+    mbar_init(bar + 32, 1);
+    mbar_init(bar + 40, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&tmem_slot), P::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // A wait that runs out ends the CTA's waiting altogether: what follows runs through on whatever
+  // is there, and the error word says so.
+  auto wait = [&](uint32_t b, uint32_t parity) {
+    if (abort_flag) return;
+    if (!mbar_wait_bounded(b, parity & 1)) {
+      abort_flag = 1;
+      raise_error(a.err, kDevWaitTimeout);
+    }
+  };
+
+  // ---- this CTA's run of the line; every warp finds it alike
+  const uint64_t unit = (uint64_t)a.gqa * kTokens;  // line length of a tile
+  auto cost_of = [&](const Kv8Rows &r) {
+    GroupCost k;
+    k.base = (uint64_t)(r.len - r.n) * a.gqa;
+    k.cap = a.window ? (uint64_t)a.window * a.gqa + kRows + 2 * a.gqa : ~0ull >> 1;
+    k.over = unit;
+    k.groups = (r.n * a.gqa + kRows - 1) / kRows;
+    return k;
+  };
+  auto cost = [&](uint32_t i) -> uint64_t {
+    Kv8Rows r;
+    if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, i, &r)) {
+      if (blockIdx.x == 0 && warp == 0) raise_error(a.err, kDevBadParams);
+      return 0;
+    }
+    if (r.n == 0) return 0;
+    const GroupCost k = cost_of(r);
+    return k.before(k.groups) * a.c.num_kv;
+  };
+  uint64_t begin = 0, end = 0, run = 1, at = 0;  // at: where the next problem starts
+  uint32_t b;
+  {
+    const uint32_t per = (a.c.num_seqs + 31) / 32;
+    const uint32_t b0 = lane * per, b1 = min(a.c.num_seqs, b0 + per);
+    uint64_t mine = 0;
+    for (uint32_t i = b0; i < b1; ++i) mine += cost(i);
+    uint64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const uint64_t total = __shfl_sync(0xffffffffu, incl, 31);
+    run = (total + gridDim.x - 1) / gridDim.x;
+    run = run > a.min_run * unit ? run : a.min_run * unit;
+    begin = run * blockIdx.x;
+    end = begin + run < total ? begin + run : total;
+    const uint32_t who = min(31, __popc(__ballot_sync(0xffffffffu, incl <= begin)));
+    at = incl - mine;
+    b = b0;
+    if (lane == (int)who && begin < end)
+      for (uint64_t n; (n = cost(b)) <= begin - at; at += n) ++b;
+    at = __shfl_sync(0xffffffffu, at, who);
+    b = __shfl_sync(0xffffffffu, b, who);
+    if (begin >= end) at = end;  // no run for this CTA
+  }
+
+  uint32_t tiles = 0;  // tiles done, over all problems: every barrier's phase follows from it
+  Kv8Rows r;
+  GroupCost gc;
+  uint32_t left = 0, head = 0, group = 0;
+  uint64_t length = 0;
+  bool fresh = true;  // the first sequence: its first problems may lie before the run
+  for (; at < end; at += length, --left) {
+    if (left != 0) {
+      if (++group == gc.groups) {
+        group = 0;
+        ++head;
+      }
+    }
+    while (left == 0) {  // the next sequence with rows
+      const bool ok = kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r);
+      ++b;
+      if (!ok || r.n == 0) continue;
+      gc = cost_of(r);
+      left = gc.groups * a.c.num_kv;
+      head = group = 0;
+      if (fresh) {
+        fresh = false;
+        const uint64_t per_head = gc.before(gc.groups);
+        head = (uint32_t)((begin - at) / per_head);
+        at += head * per_head;
+        uint32_t lo = 0, hi = gc.groups - 1;  // the last group that starts at or before begin
+        while (lo < hi) {
+          const uint32_t mid = (lo + hi + 1) / 2;
+          if (gc.before(mid) <= begin - at) lo = mid; else hi = mid - 1;
+        }
+        group = lo;
+        at += gc.before(group);
+        left -= head * gc.groups + group;
+      }
+    }
+    length = gc.of(group);
+    const uint32_t row0 = group * kRows, rows = min(kRows, r.n * a.gqa - row0);
+    const uint32_t pos0 = r.len - r.n;
+    const uint32_t pos_lo = pos0 + row0 / a.gqa, pos_hi = pos0 + (row0 + rows - 1) / a.gqa;
+    const uint32_t first = (a.window && pos_lo >= a.window ? pos_lo - a.window + 1 : 0) / kKv8Block;
+    const uint32_t blocks = pos_hi / kKv8Block - first + 1;
+    const uint32_t count = (blocks + kTileBlocks - 1) / kTileBlocks;
+    const uint32_t t0 = begin > at ? (uint32_t)((begin - at + unit - 1) / unit) : 0;
+    const uint64_t until = (end - at + unit - 1) / unit;
+    const uint32_t t1 = until < count ? (uint32_t)until : count;
+    if (t0 >= t1) continue;  // no tile starts in the run
+    const uint32_t n_tiles = t1 - t0;
+    const uint32_t *table = a.c.table + (size_t)(b - 1) * a.c.max_pages;
+    // record pair of block s of the problem; ~0: nothing to read
+    auto record = [&](uint32_t s) -> uint64_t {
+      if (s >= blocks) return ~0ull;
+      const uint32_t per = a.c.page_tokens / kKv8Block, page = table[(first + s) / per];
+      if (page >= a.c.num_pages) {
+        raise_error(a.err, kDevBadSlot);
+        return ~0ull;
+      }
+      return ((uint64_t)page * a.c.num_kv + head) * per + (first + s) % per;
+    };
+    // tiles whose keys every row sees
+    const uint32_t all_hi = pos_lo, all_lo = a.window && pos_hi >= a.window ? pos_hi - a.window + 1 : 0;
+    auto is_mixed = [&](uint32_t t) {
+      const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
+      return key0 < all_lo || key0 + kTokens - 1 > all_hi;
+    };
+
+    // ---- Q: power-of-two scaled f16 terms, K-major 128-byte swizzle
+    {
+      constexpr int kLanes = D / 8, kPass = 32 / kLanes;  // lanes of a row, rows of a warp's pass
+      const uint32_t li = lane % kLanes;
+      for (uint32_t i0 = warp * kPass; i0 < kRows; i0 += P::kThreads / 32 * kPass) {
+        const uint32_t i = i0 + lane / kLanes, pr = row0 + i;
+        const bool in = i < rows;
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+        if (in) {
+          const T *src = static_cast<const T *>(a.q) + (size_t)(r.r0 + pr / a.gqa) * a.q_ld +
+                         (size_t)(head * a.gqa + pr % a.gqa) * D + 8 * li;
+          constexpr int kVec = 16 / (int)sizeof(T);
+#pragma unroll
+          for (int k = 0; k < 8; k += kVec) {
+            float v[kVec];
+            load_vec<T, kVec>(src + k, v);
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) x[k + j] = v[j];
+          }
+        }
+        float m = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[k]));
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        int e = (int)(__float_as_uint(m) >> 23) - 127;
+        if (m == 0.0f || e == 128) e = 0;  // nothing to scale; an infinity stays one
+        e = min(max(e, -126), 126);
+        const float inv = a.scale < 0.0f ? -exp2_int(-e) : exp2_int(-e);
+        if (li == 0) row_mul[i] = fabsf(a.scale) * kLog2e * exp2_int(e);
+        uint32_t hi[4], low[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float v0 = x[2 * k] * inv, v1 = x[2 * k + 1] * inv;
+          hi[k] = pack_f16(v0, v1);
+          if constexpr (kSplit) low[k] = pack_f16_rest(v0, v1, hi[k]);
+        }
+        const uint32_t dst = q_tile + li / 8 * (kRows * 128) + i * 128 + (((li % 8) ^ (i & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
+        if constexpr (kSplit)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + P::kQTerm), "r"(low[0]), "r"(low[1]), "r"(low[2]), "r"(low[3]) : "memory");
+      }
+      fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
+    }
+    __syncthreads();
+
+    if (warp < 4) {
+      // ================================================================ softmax: thread = row
+      const uint32_t i = threadIdx.x, lanes = (uint32_t)(32 * warp) << 16;
+      const float mul = row_mul[i];
+      const uint32_t pos = pos0 + (row0 + min(i, rows - 1)) / a.gqa;
+      const uint32_t see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_n = pos - see_lo;
+      float ref = -INFINITY, l = 0.0f;
+      // scales of a tile's blocks: lane s < kTileBlocks holds block s; a tile ahead
+      auto scales = [&](uint32_t t) -> float2 {
+        float2 f = make_float2(0.0f, 0.0f);  // v scale 0: a block that is not there
+        if (lane < kTileBlocks && t < t1) {
+          const uint64_t rec = record(t * kTileBlocks + lane);
+          if (rec != ~0ull) f = *reinterpret_cast<const float2 *>(a.c.scale + 2 * rec);
+        }
+        return f;
+      };
+      float2 next = scales(t0);
+      for (uint32_t t = t0; t < t1; ++t) {
+        const uint32_t tile = tiles + (t - t0), s_col = tmem + lanes + tile % kS * kTokens;
+        const float2 sc = next;
+        next = scales(t + 1);
+        // masked: some row does not see all of the tile, or a block of it is not there
+        const bool mixed = is_mixed(t);
+        const bool masked = mixed || __any_sync(0xffffffffu, lane < kTileBlocks && sc.y == 0.0f);
+        const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
+        if (mixed) wait(v_full, tile);  // the NaN masks come with V
+        wait(s_done(tile), tile / kS);
+        tc_fence_after();
+        // -- the largest x + log2(v scale)
+        float top = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < kTokens / 32; ++q) {
+          uint32_t s[32];
+          tmem_ld32(s_col + 32 * q, s);
+          float m[2] = {-INFINITY, -INFINITY};
+          float ks[2], vs[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            ks[h] = __shfl_sync(0xffffffffu, sc.x, 2 * q + h);
+            vs[h] = __shfl_sync(0xffffffffu, sc.y, 2 * q + h);
+          }
+          tmem_wait_ld();
+          if (!masked) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) m[(k >> 2) & 1] = fmaxf(m[(k >> 2) & 1], __uint_as_float(s[k]));
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const int h = (k >> 2) & 1;
+              const uint32_t key = key0 + 32 * q + 16 * h + 8 * ((k >> 1) & 1) + 2 * (k >> 3) + (k & 1);
+              if (key - see_lo <= see_n && vs[h] != 0.0f) m[h] = fmaxf(m[h], __uint_as_float(s[k]));
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (m[h] != -INFINITY)
+              top = fmaxf(top, fmaf(m[h], ks[h] * mul, (float)kv8_scale_exponent(vs[h])));
+        }
+        // -- a maximum that outgrew the reference: rescale the row
+        const bool grow = top > ref + kSlack || (ref == -INFINITY && top > ref);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = !grow ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - top);
+          if (grow) ref = top;
+          l *= f;
+          if (t > t0) {
+            wait(pv_done, tile - 1);
+            tc_fence_after();
+#pragma unroll 1
+            for (int d = 0; d < D; d += 32) {
+              uint32_t o[32];
+              tmem_ld32(tmem + lanes + P::kO + d, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st32(tmem + lanes + P::kO + d, o);
+            }
+            tmem_wait_st();
+          }
+        }
+        const float shift = ref == -INFINITY ? 0.0f : ref - kPromptOffset;
+        // -- P over S: chunk q's 16 columns lie in S columns that have been read
+#pragma unroll
+        for (int q = 0; q < kTokens / 32; ++q) {
+          uint32_t s[32];
+          tmem_ld32(s_col + 32 * q, s);
+          float km[2], off[2], unv[2], sum[2] = {0.0f, 0.0f};
+          uint32_t vis[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float ks = __shfl_sync(0xffffffffu, sc.x, 2 * q + h), vs = __shfl_sync(0xffffffffu, sc.y, 2 * q + h);
+            const float lv = (float)kv8_scale_exponent(vs);
+            km[h] = ks * mul;
+            off[h] = lv - shift;
+            unv[h] = ex2(-lv);
+            vis[h] = vs != 0.0f;
+          }
+          tmem_wait_ld();
+          if (!masked) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const int h = (k >> 2) & 1;
+              const float p = ex2(fmaf(__uint_as_float(s[k]), km[h], off[h]));
+              sum[h] += p;
+              s[k] = __float_as_uint(p);
+            }
+          } else {
+            const uint32_t nan = mixed ? nan_mask[tile & 1][q] : 0;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              const int h = (k >> 2) & 1, tok = 16 * h + 8 * ((k >> 1) & 1) + 2 * (k >> 3) + (k & 1);
+              const bool seen = key0 + 32 * q + tok - see_lo <= see_n && vis[h];
+              float p = ex2(fmaf(__uint_as_float(s[k]), km[h], off[h]));
+              if ((nan >> tok) & 1u) p = NAN;
+              p = seen ? p : 0.0f;
+              sum[h] += p;
+              s[k] = __float_as_uint(p);
+            }
+          }
+          l = fmaf(sum[0], unv[0], fmaf(sum[1], unv[1], l));
+          uint32_t hi[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) hi[k] = pack_f16(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+          tmem_st16(s_col + 16 * q, hi);
+          if constexpr (kSplit) {
+            uint32_t low[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              low[k] = pack_f16_rest(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]), hi[k]);
+            tmem_st16(tmem + lanes + P::kLow + tile % kS * (kTokens / 2) + 16 * q, low);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
+      }
+      // ---- the row's output, or its part
+      wait(pv_done, tiles + n_tiles - 1);
+      tc_fence_after();
+      const bool whole = t0 == 0 && t1 == count;
+      const uint32_t slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
+      float *const ml = a.part + ((size_t)slot * kRows + i) * 2;
+      float *const po = a.part + (size_t)2 * gridDim.x * kRows * 2 + ((size_t)slot * kRows + i) * D;
+      const uint32_t pr = row0 + i;
+      T *const out = static_cast<T *>(a.out) + (size_t)(r.r0 + pr / a.gqa) * a.out_ld +
+                     (size_t)(head * a.gqa + pr % a.gqa) * D;
+      const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+      if (!whole && i < rows) {
+        ml[0] = ref;
+        ml[1] = l;
+      }
+#pragma unroll 1
+      for (int d = 0; d < D; d += 32) {
+        uint32_t o[32];
+        tmem_ld32(tmem + lanes + P::kO + d, o);
+        tmem_wait_ld();
+        if (i < rows) {
+          // element 4 g + i of the piece is column 8 i + f(g), f(g) = g / 2 + 4 (g % 2)
+          float y[32];
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            y[k] = __uint_as_float(o[8 * (k & 3) + ((k >> 2) >> 1) + 4 * ((k >> 2) & 1)]) * inv;
+          if (whole) {
+            constexpr int kVec = 16 / (int)sizeof(T);
+#pragma unroll
+            for (int k = 0; k < 32; k += kVec) {
+              float v[kVec];
+#pragma unroll
+              for (int j = 0; j < kVec; ++j) v[j] = y[k + j];
+              store_vec<T, kVec>(out + d + k, v);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<float4 *>(po + d + k) = make_float4(y[k], y[k + 1], y[k + 2], y[k + 3]);
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+    } else if (warp < 4 + kWiden) {
+      // ================================================================ widen K and V
+      constexpr int kPairs = kTokens / 32, kShare = kWiden / kPairs;  // warps of a pair of blocks
+      constexpr int kMine = D / 32 / kShare;                          // pieces of a warp
+      static_assert(kMine >= 2, "pieces come in pairs");
+      const uint32_t ww = warp - 4, pair = ww % kPairs, p0 = ww / kPairs * kMine;
+      struct Recs {
+        uint64_t r[2];
+      };
+      auto recs = [&](uint32_t t) -> Recs {
+        Recs x{{~0ull, ~0ull}};
+        if (t < t1) {
+          x.r[0] = record(t * kTileBlocks + 2 * pair);
+          x.r[1] = record(t * kTileBlocks + 2 * pair + 1);
+        }
+        return x;
+      };
+      uint4 raw_k[2][kMine], raw_v[2][kMine];
+      // K: lanes with odd g take the pieces of a pair in the other order, so that a store's eight
+      // lanes meet all banks
+      auto fetch = [&](const Recs &x, int which, uint4 (&raw)[2][kMine]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + (2 * x.r[h] + which) * (size_t)(16 * D);
+#pragma unroll
+          for (int p = 0; p < kMine; ++p)
+            raw[h][p] = x.r[h] == ~0ull ? make_uint4(0, 0, 0, 0)
+                                        : *reinterpret_cast<const uint4 *>(src + 512 * (p0 + (which ? p : p ^ (g & 1))) + 16 * lane);
+        }
+      };
+      Recs cur = recs(t0);
+      fetch(cur, 0, raw_k);
+      fetch(cur, 1, raw_v);
+      for (uint32_t t = t0; t < t1; ++t) {
+        const uint32_t tile = tiles + (t - t0);
+        const bool mixed = is_mixed(t);
+        const Recs ahead = recs(t + 1);
+        if (tile > 0) wait(s_done(tile - 1), (tile - 1) / kS);  // the product before has read K
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int p = 0; p < kMine; ++p) {
+            const uint32_t piece = p0 + (p ^ (g & 1)), chunk = (piece & 1) * 4 + c;
+            const uint32_t row = 32 * pair + 8 * (g / 2) + 4 * h + (g & 1);
+            const uint32_t base = k_tile + piece / 2 * (kTokens * 128);
+            const uint4 w = raw_k[h][p];
+            uint32_t x[4];
+            e4m3x4_f16(w.x, x[0], x[1]);
+            e4m3x4_f16(w.y, x[2], x[3]);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(base + row * 128 + ((chunk ^ (row & 7)) << 4)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+            e4m3x4_f16(w.z, x[0], x[1]);
+            e4m3x4_f16(w.w, x[2], x[3]);
+            const uint32_t row8 = row + 2;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(base + row8 * 128 + ((chunk ^ (row8 & 7)) << 4)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          }
+        fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
+        __syncwarp();
+        if (lane == 0) mbar_arrive(k_full);
+        fetch(ahead, 0, raw_k);
+
+        if (tile > 0) wait(pv_done, tile - 1);  // the product before has read V
+        if (mixed) {
+          // A NaN would reach rows that do not see its token through 0 x NaN: it is taken out, and
+          // its token marked for the rows that do.
+          if (ww == 0 && lane < kPairs) nan_mask[tile & 1][lane] = 0;
+          asm volatile("bar.sync 1, %0;\n" ::"n"(kWiden * 32) : "memory");
+          uint32_t bits = 0;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int p = 0; p < kMine; ++p) {
+              uint32_t w[4] = {raw_v[h][p].x, raw_v[h][p].y, raw_v[h][p].z, raw_v[h][p].w};
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint32_t n = (((w[k] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+                w[k] &= ~(n * 0xFFu);
+                // bytes are tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9 of block h
+                bits |= ((n & 1u) | ((n >> 7) & 2u) | ((n >> 8) & 0x100u) | ((n >> 15) & 0x200u)) << (2 * c + 16 * h);
+              }
+              raw_v[h][p] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          if (bits) atomicOr(&nan_mask[tile & 1][pair], bits);
+        }
+#pragma unroll
+        for (int p = 0; p < kMine; ++p) {
+          const uint32_t fg = (g >> 1) | ((g & 1) << 2), chunk = (pair & 1) * 4 + c;
+          const uint32_t base = v_tile + pair / 2 * (D * 128) + (32 * (p0 + p) + fg) * 128 + ((chunk ^ fg) << 4);
+          const uint32_t wa[4] = {raw_v[0][p].x, raw_v[0][p].y, raw_v[0][p].z, raw_v[0][p].w};
+          const uint32_t wb[4] = {raw_v[1][p].x, raw_v[1][p].y, raw_v[1][p].z, raw_v[1][p].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {  // element 4 g + k: row 8 k + f(g) of the piece
+            uint32_t x[4];
+            e4m3x4_f16(wa[k], x[0], x[1]);
+            e4m3x4_f16(wb[k], x[2], x[3]);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(base + k * 8 * 128), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full);
+        fetch(ahead, 1, raw_v);
+      }
+    } else if (lane == 0) {
+      // ================================================================ the products
+      constexpr uint32_t s_desc = umma_idesc_f16(kRows, kTokens), o_desc = umma_idesc_f16(kRows, D);
+      auto product_s = [&](uint32_t tile) {
+        wait(k_full, tile);
+        tc_fence_after();
+#pragma unroll
+        for (int w = 0; w < kTerms; ++w)
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)  // 32 bytes of a swizzled row per step of 16
+            umma_f16(tmem + tile % kS * kTokens,
+                     umma_desc_sw128(q_tile + w * P::kQTerm + k / 4 * (kRows * 128)) + 2 * (k % 4),
+                     umma_desc_sw128(k_tile + k / 4 * (kTokens * 128)) + 2 * (k % 4), s_desc, w > 0 || k > 0);
+        umma_commit(s_done(tile));
+      };
+      auto product_o = [&](uint32_t tile, bool add) {
+        wait(v_full, tile);
+        wait(p_full, tile);
+        tc_fence_after();
+#pragma unroll
+        for (int w = 0; w < kTerms; ++w)
+#pragma unroll
+          for (int k = 0; k < kTokens / 16; ++k)
+            umma_f16_ts(tmem + P::kO,
+                        tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens) + 8 * k,
+                        umma_desc_sw128(v_tile + k / 4 * (D * 128)) + 2 * (k % 4), o_desc, add || w > 0 || k > 0);
+        umma_commit(pv_done);
+      };
+      if (kS == 2) product_s(tiles);
+      for (uint32_t j = 0; j < n_tiles; ++j) {
+        if (kS == 1)
+          product_s(tiles + j);
+        else if (j + 1 < n_tiles)
+          product_s(tiles + j + 1);
+        product_o(tiles + j, j > 0);
+      }
+    }
+    tiles += n_tiles;
+    __syncthreads();  // Q, the tiles and O are free; the parts are written
+
+    if (!(t0 == 0 && t1 == count)) {
+      // CTAs c0 .. c1 hold parts of this problem; c0 counts them
+      const uint32_t c0 = (uint32_t)(at / run), c1 = (uint32_t)((at + (count - 1) * unit) / run);
+      const uint32_t slot0 = 2 * c0 + (at > run * c0 ? 1 : 0);
+      if (threadIdx.x == 0) last_flag = arrive_acq_rel(a.cnt + c0) == c1 - c0;
+      __syncthreads();
+      if (last_flag) {
+        const float *ml = a.part, *po = a.part + (size_t)2 * gridDim.x * kRows * 2;
+        auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : 2 * (c0 + k); };
+        const uint32_t n = c1 - c0 + 1;
+        for (uint32_t i = warp; i < rows; i += P::kThreads / 32) {  // a warp per row
+          float m = -INFINITY, l = 0.0f;
+          for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, __ldcg(ml + ((size_t)slot_of(k) * kRows + i) * 2));
+          m = warp_max(m);
+          float sum[D / 32];
+#pragma unroll
+          for (int d = 0; d < D / 32; ++d) sum[d] = 0.0f;
+          for (uint32_t k = 0; k < n; ++k) {
+            const size_t at_row = (size_t)slot_of(k) * kRows + i;
+            const float mk = __ldcg(ml + at_row * 2), f = mk == -INFINITY ? 0.0f : ex2(mk - m);
+            l = fmaf(__ldcg(ml + at_row * 2 + 1), f, l);
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d) {
+              const float2 v = __ldcg(reinterpret_cast<const float2 *>(po + at_row * D + 64 * d + 2 * lane));
+              sum[2 * d] = fmaf(v.x, f, sum[2 * d]);
+              sum[2 * d + 1] = fmaf(v.y, f, sum[2 * d + 1]);
+            }
+          }
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+          const uint32_t pr = row0 + i;
+          T *out = static_cast<T *>(a.out) + (size_t)(r.r0 + pr / a.gqa) * a.out_ld + (size_t)(head * a.gqa + pr % a.gqa) * D;
+#pragma unroll
+          for (int d = 0; d < D / 64; ++d) {
+            const float y[2] = {sum[2 * d] * inv, sum[2 * d + 1] * inv};
+            store_vec<T, 2>(out + 64 * d + 2 * lane, y);
+          }
+        }
+        if (threadIdx.x == 0) a.cnt[c0] = 0;
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, P::kCols);
+  }
+}
+
+using PromptKernel = void (*)(Kv8AttnArgs);
+struct PromptVariant {
+  PromptKernel fn;
+  uint32_t smem, ctas, threads;
+};
+template <typename T, int D>
+PromptVariant prompt_variant() {
+  using P = PromptShape<D, sizeof(T) == 4>;
+  return {kv8_prompt_kernel<T, D>, (uint32_t)P::kSmem, (uint32_t)P::kCtas, (uint32_t)P::kThreads};
+}
+PromptVariant prompt_variant(sx_dtype t, uint32_t d) {
+  if (t == SX_F32)
+    return d == 64 ? prompt_variant<float, 64>() : d == 128 ? prompt_variant<float, 128>() : prompt_variant<float, 256>();
+  return d == 64 ? prompt_variant<__nv_bfloat16, 64>() : d == 128 ? prompt_variant<__nv_bfloat16, 128>()
+       : prompt_variant<__nv_bfloat16, 256>();
+}
+
+}  // namespace
+
+cudaError_t prepare_kv8_prompt() {
+  for (uint32_t d : {64u, 128u, 256u})
+    for (sx_dtype t : {SX_F32, SX_BF16}) {
+      const PromptVariant v = prompt_variant(t, d);
+      const cudaError_t e = cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem);
+      if (e != cudaSuccess) return e;
+    }
+  return cudaSuccess;
+}
+
+// Two parts per CTA of 128 rows: {m, l}, and 128 (two CTAs per SM) or 256 output values a row.
+size_t kv8_prompt_part_bytes(int num_sms) { return (size_t)2 * num_sms * kRows * (2 * 2 + 256) * sizeof(float); }
+
+cudaError_t launch_kv8_prompt(Kv8AttnArgs a, sx_dtype t, int num_sms, cudaStream_t s) {
+  const PromptVariant v = prompt_variant(t, a.c.head_dim);
+  a.min_run = 4;  // tiles: shorter runs cost more to merge than they save
+  return launch_chained(v.fn, dim3(num_sms * v.ctas), dim3(v.threads), v.smem, s, 1, a);
+}
+
+}  // namespace sx
