@@ -7,15 +7,15 @@
 // tensor memory, P goes back there as f16 over S and is the second product's A operand.  e4m3 is
 // exact in f16, so K and V are widened on the way to shared memory; f32 rows split Q and P into two
 // f16 terms, with twice the products.  Warps:
-//   0 .. 3   softmax, a thread per row: S from tensor memory twice (maximum, then exponentials), P
-//            back.  The maximum that the exponentials refer to moves only when it grows by 2^8; the
-//            row of O is then rescaled in tensor memory.
+//   0 .. 3   softmax, a thread per row: S from tensor memory 32 columns at a time, the next ones on
+//            their way, P back.  The maximum that the exponentials refer to moves only when it grows
+//            by 2^8; the row of O, and of P so far, is then rescaled in tensor memory.
 //   4 ..     widen K and V.  A warp takes a pair of blocks (32 tokens): the cache's 16-byte pieces
 //            become 16-byte stores of the 128-byte-swizzled tiles for a fitting order of the tokens
 //            (tile position 32 q + 8 (t % 8 / 2) + 4 half + 2 (t / 8) + t % 2) and of V's elements
 //            (tile row 32 p + 8 (d % 4) + f(d % 32 / 4), f a permutation of 8).  The softmax undoes
 //            the first in its masks and scales, the output the second: both are register indexes.
-//   last     one thread issues the products.
+// A thread of warp 0 issues the products (a warp of their own would cost the others registers).
 // Bound by shared memory (the tiles' stores and the products' reads) and exponentials (16 a cycle
 // and SM, as many as a product of head size 128 takes cycles).  Up to head size 128 two CTAs share an
 // SM and fill each other's waits; above, two S tiles let the next product run beside the softmax.
@@ -40,7 +40,7 @@ struct PromptShape {
   static constexpr int kTokens = D == 256 && SPLIT ? 64 : 128;            // of a tile
   static constexpr int kS = kCtas == 2 ? 1 : 2;                           // S tiles
   static constexpr int kWiden = kCtas == 2 ? 4 : 8;                       // warps that widen
-  static constexpr int kThreads = (4 + kWiden + 1) * 32;
+  static constexpr int kThreads = (4 + kWiden) * 32;
   static constexpr int kTerms = SPLIT ? 2 : 1;
   static constexpr int kQTerm = (int)kRows * D * 2;
   static constexpr int kTile = kTokens * D * 2;
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
   constexpr int kTokens = P::kTokens, kS = P::kS, kWiden = P::kWiden, kTerms = P::kTerms;
   constexpr int kTileBlocks = kTokens / kKv8Block;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[6];
+  __shared__ __align__(8) uint64_t bars[9];
   __shared__ uint32_t tmem_slot, last_flag, nan_mask[2][kTokens / 32];
   __shared__ volatile uint32_t abort_flag;
   __shared__ float row_mul[kRows];
@@ -84,15 +84,25 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
   const uint32_t k_tile = q_tile + kTerms * P::kQTerm;           // [D / 64][tokens][128 B]
   const uint32_t v_tile = k_tile + P::kTile;                     // [tokens / 64][D][128 B]
   const uint32_t bar = smem_u32(bars);
-  const uint32_t k_full = bar, v_full = bar + 8, p_full = bar + 16, pv_done = bar + 24;
-  auto s_done = [&](uint32_t t) { return bar + 32 + 8 * (t % kS); };
+  // Waits are for a phase's parity, so a waiter must be sure of the phase before and ahead of the one
+  // after.  The threads that widen and the one that issues go tile by tile; a softmax warp may be a
+  // tile ahead of another when there are two S tiles, so what it waits for or arrives at has a
+  // barrier for even and one for odd tiles: S of a tile done means that all of two tiles back is.
+  const uint32_t k_full = bar;
+  auto v_full = [&](uint32_t t) { return bar + 8 + 8 * (t & 1); };
+  auto pv_done = [&](uint32_t t) { return bar + 24 + 8 * (t & 1); };
+  auto s_done = [&](uint32_t t) { return bar + 40 + 8 * (t % kS); };
+  auto p_full = [&](uint32_t t) { return bar + 56 + 8 * (t % kS); };
   if (threadIdx.x == 0) {
     mbar_init(k_full, kWiden);
-    mbar_init(v_full, kWiden);
-    mbar_init(p_full, 4);
-    mbar_init(pv_done, 1);
-    mbar_init(bar + 32, 1);
-    mbar_init(bar + 40, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(v_full(i), kWiden);
+      mbar_init(pv_done(i), 1);
+    }
+    for (int i = 0; i < kS; ++i) {
+      mbar_init(s_done(i), 1);
+      mbar_init(p_full(i), 4);
+    }
     abort_flag = 0;
     fence_mbar_init();
   }
@@ -278,6 +288,34 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
     }
     __syncthreads();
 
+    // ---- the products, for one thread
+    constexpr uint32_t s_desc = umma_idesc_f16(kRows, kTokens), o_desc = umma_idesc_f16(kRows, D);
+    auto product_s = [&](uint32_t tile) {
+      wait(k_full, tile);
+      tc_fence_after();
+#pragma unroll
+      for (int w = 0; w < kTerms; ++w)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)  // 32 bytes of a swizzled row per step of 16
+          umma_f16(tmem + tile % kS * kTokens,
+                   umma_desc_sw128(q_tile + w * P::kQTerm + k / 4 * (kRows * 128)) + 2 * (k % 4),
+                   umma_desc_sw128(k_tile + k / 4 * (kTokens * 128)) + 2 * (k % 4), s_desc, w > 0 || k > 0);
+      umma_commit(s_done(tile));
+    };
+    auto product_o = [&](uint32_t tile, bool add) {
+      wait(v_full(tile), tile / 2);
+      wait(p_full(tile), tile / kS);
+      tc_fence_after();
+#pragma unroll
+      for (int w = 0; w < kTerms; ++w)
+#pragma unroll
+        for (int k = 0; k < kTokens / 16; ++k)
+          umma_f16_ts(tmem + P::kO,
+                      tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens) + 8 * k,
+                      umma_desc_sw128(v_tile + k / 4 * (D * 128)) + 2 * (k % 4), o_desc, add || w > 0 || k > 0);
+      umma_commit(pv_done(tile));
+    };
+
     if (warp < 4) {
       // ================================================================ softmax: thread = row
       const uint32_t i = threadIdx.x, lanes = (uint32_t)(32 * warp) << 16;
@@ -295,6 +333,7 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
         return f;
       };
       float2 next = scales(t0);
+      if (threadIdx.x == 0) product_s(tiles);
       for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t tile = tiles + (t - t0), s_col = tmem + lanes + tile % kS * kTokens;
         const float2 sc = next;
@@ -303,119 +342,121 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
         const bool mixed = is_mixed(t);
         const bool masked = mixed || __any_sync(0xffffffffu, lane < kTileBlocks && sc.y == 0.0f);
         const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
-        if (mixed) wait(v_full, tile);  // the NaN masks come with V
         wait(s_done(tile), tile / kS);
+        if (mixed) wait(v_full(tile), tile / 2);  // the NaN masks come with V
         tc_fence_after();
-        // -- the largest x + log2(v scale)
-        float top = -INFINITY;
+        const uint32_t low_col = tmem + lanes + P::kLow + tile % kS * (kTokens / 2);
+        uint32_t s[2][32];
+        tmem_ld32(s_col, s[0]);
+        // P over S: chunk q's 16 columns lie in S columns that have been read
 #pragma unroll
         for (int q = 0; q < kTokens / 32; ++q) {
-          uint32_t s[32];
-          tmem_ld32(s_col + 32 * q, s);
-          float m[2] = {-INFINITY, -INFINITY};
-          float ks[2], vs[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ks[h] = __shfl_sync(0xffffffffu, sc.x, 2 * q + h);
-            vs[h] = __shfl_sync(0xffffffffu, sc.y, 2 * q + h);
-          }
-          tmem_wait_ld();
-          if (!masked) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) m[(k >> 2) & 1] = fmaxf(m[(k >> 2) & 1], __uint_as_float(s[k]));
-          } else {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int h = (k >> 2) & 1;
-              const uint32_t key = key0 + 32 * q + 16 * h + 8 * ((k >> 1) & 1) + 2 * (k >> 3) + (k & 1);
-              if (key - see_lo <= see_n && vs[h] != 0.0f) m[h] = fmaxf(m[h], __uint_as_float(s[k]));
-            }
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (m[h] != -INFINITY)
-              top = fmaxf(top, fmaf(m[h], ks[h] * mul, (float)kv8_scale_exponent(vs[h])));
-        }
-        // -- a maximum that outgrew the reference: rescale the row
-        const bool grow = top > ref + kSlack || (ref == -INFINITY && top > ref);
-        if (__any_sync(0xffffffffu, grow)) {
-          const float f = !grow ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - top);
-          if (grow) ref = top;
-          l *= f;
-          if (t > t0) {
-            wait(pv_done, tile - 1);
-            tc_fence_after();
-#pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-              uint32_t o[32];
-              tmem_ld32(tmem + lanes + P::kO + d, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-              tmem_st32(tmem + lanes + P::kO + d, o);
-            }
-            tmem_wait_st();
-          }
-        }
-        const float shift = ref == -INFINITY ? 0.0f : ref - kPromptOffset;
-        // -- P over S: chunk q's 16 columns lie in S columns that have been read
-#pragma unroll
-        for (int q = 0; q < kTokens / 32; ++q) {
-          uint32_t s[32];
-          tmem_ld32(s_col + 32 * q, s);
-          float km[2], off[2], unv[2], sum[2] = {0.0f, 0.0f};
+          uint32_t (&x)[32] = s[q & 1];
+          float km[2], lv[2], unv[2], m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
           uint32_t vis[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float ks = __shfl_sync(0xffffffffu, sc.x, 2 * q + h), vs = __shfl_sync(0xffffffffu, sc.y, 2 * q + h);
-            const float lv = (float)kv8_scale_exponent(vs);
-            km[h] = ks * mul;
-            off[h] = lv - shift;
-            unv[h] = ex2(-lv);
+            lv[h] = (float)kv8_scale_exponent(vs);
+            km[h] = fmaxf(ks * mul, 1.17549435e-38f);  // -inf stays -inf
+            unv[h] = exp2_int(-kv8_scale_exponent(vs));
             vis[h] = vs != 0.0f;
           }
-          tmem_wait_ld();
-          if (!masked) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int h = (k >> 2) & 1;
-              const float p = ex2(fmaf(__uint_as_float(s[k]), km[h], off[h]));
-              sum[h] += p;
-              s[k] = __float_as_uint(p);
-            }
-          } else {
+          tmem_wait_ld(x);
+          if (q + 1 < kTokens / 32) tmem_ld32(s_col + 32 * (q + 1), s[(q + 1) & 1]);
+          // -- the chunk's largest x + log2(v scale); a masked score becomes -inf
+          if (masked) {
             const uint32_t nan = mixed ? nan_mask[tile & 1][q] : 0;
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
               const int h = (k >> 2) & 1, tok = 16 * h + 8 * ((k >> 1) & 1) + 2 * (k >> 3) + (k & 1);
               const bool seen = key0 + 32 * q + tok - see_lo <= see_n && vis[h];
-              float p = ex2(fmaf(__uint_as_float(s[k]), km[h], off[h]));
-              if ((nan >> tok) & 1u) p = NAN;
-              p = seen ? p : 0.0f;
-              sum[h] += p;
-              s[k] = __float_as_uint(p);
+              if ((nan >> tok) & 1u) x[k] = 0x7FFFFFFFu;
+              if (!seen) x[k] = 0xFF800000u;
             }
+          }
+#pragma unroll
+          for (int k = 0; k < 32; k += 8) {
+            m[0] = fmaxf(m[0], fmaxf(fmaxf(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), fmaxf(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]))));
+            m[1] = fmaxf(m[1], fmaxf(fmaxf(__uint_as_float(x[k + 4]), __uint_as_float(x[k + 5])), fmaxf(__uint_as_float(x[k + 6]), __uint_as_float(x[k + 7]))));
+          }
+          float top = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (m[h] != -INFINITY) top = fmaxf(top, fmaf(m[h], km[h], lv[h]));
+          // -- one that outgrew the reference: rescale what the row has so far
+          const bool grow = top > ref + kSlack || (ref == -INFINITY && top > ref);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float f = !grow ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - top);
+            if (grow) ref = top;
+            l *= f;
+            if (q + 1 < kTokens / 32) tmem_wait_ld(s[(q + 1) & 1]);
+            if (t > t0) {
+              wait(pv_done(tile - 1), (tile - 1) / 2);
+              tc_fence_after();
+#pragma unroll 1
+              for (int d = 0; d < D; d += 16) {
+                uint32_t o[16];
+                tmem_ld16(tmem + lanes + P::kO + d, o);
+                tmem_wait_ld(o);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                tmem_st16(tmem + lanes + P::kO + d, o);
+              }
+            }
+            tmem_wait_st();
+#pragma unroll 1
+            for (int d = 0; d < q * 16 * kTerms; d += 16) {
+              const uint32_t col = d < 16 * q ? s_col + d : low_col + d - 16 * q;
+              uint32_t o[16];
+              tmem_ld16(col, o);
+              tmem_wait_ld(o);
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&o[k]));
+                o[k] = pack_f16(v.x * f, v.y * f);
+              }
+              tmem_st16(col, o);
+            }
+          }
+          const float shift = ref == -INFINITY ? 0.0f : ref - kPromptOffset;
+          const float off[2] = {lv[0] - shift, lv[1] - shift};
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const int h = (k >> 2) & 1;
+            const float p = ex2(fmaf(__uint_as_float(x[k]), km[h], off[h]));
+            sum[h] += p;
+            x[k] = __float_as_uint(p);
           }
           l = fmaf(sum[0], unv[0], fmaf(sum[1], unv[1], l));
           uint32_t hi[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) hi[k] = pack_f16(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+          for (int k = 0; k < 16; ++k) hi[k] = pack_f16(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1]));
           tmem_st16(s_col + 16 * q, hi);
           if constexpr (kSplit) {
-            uint32_t low[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k)
-              low[k] = pack_f16_rest(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]), hi[k]);
-            tmem_st16(tmem + lanes + P::kLow + tile % kS * (kTokens / 2) + 16 * q, low);
+              hi[k] = pack_f16_rest(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1]), hi[k]);
+            tmem_st16(low_col + 16 * q, hi);
+          }
+          // with a second S tile the next product runs beside the rest of this softmax
+          if (kS == 2 && q == kTokens / 64 - 1) {
+            if (threadIdx.x == 0 && t + 1 < t1) product_s(tile + 1);
+            __syncwarp();
           }
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        if (lane == 0) mbar_arrive(p_full(tile));
+        if (threadIdx.x == 0) {
+          product_o(tile, t > t0);
+          if (kS == 1 && t + 1 < t1) product_s(tile + 1);
+        }
+        __syncwarp();
       }
       // ---- the row's output, or its part
-      wait(pv_done, tiles + n_tiles - 1);
+      wait(pv_done(tiles + n_tiles - 1), (tiles + n_tiles - 1) / 2);
       tc_fence_after();
       const bool whole = t0 == 0 && t1 == count;
       const uint32_t slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
@@ -433,7 +474,7 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
       for (int d = 0; d < D; d += 32) {
         uint32_t o[32];
         tmem_ld32(tmem + lanes + P::kO + d, o);
-        tmem_wait_ld();
+        tmem_wait_ld(o);
         if (i < rows) {
           // element 4 g + i of the piece is column 8 i + f(g), f(g) = g / 2 + 4 (g % 2)
           float y[32];
@@ -458,7 +499,7 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
         __syncwarp();
       }
       tc_fence_before();
-    } else if (warp < 4 + kWiden) {
+    } else {
       // ================================================================ widen K and V
       constexpr int kPairs = kTokens / 32, kShare = kWiden / kPairs;  // warps of a pair of blocks
       constexpr int kMine = D / 32 / kShare;                          // pieces of a warp
@@ -518,7 +559,7 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
         if (lane == 0) mbar_arrive(k_full);
         fetch(ahead, 0, raw_k);
 
-        if (tile > 0) wait(pv_done, tile - 1);  // the product before has read V
+        if (tile > 0) wait(pv_done(tile - 1), (tile - 1) / 2);  // the product before has read V
         if (mixed) {
           // A NaN would reach rows that do not see its token through 0 x NaN: it is taken out, and
           // its token marked for the rows that do.
@@ -557,44 +598,8 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
         }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(v_full);
+        if (lane == 0) mbar_arrive(v_full(tile));
         fetch(ahead, 1, raw_v);
-      }
-    } else if (lane == 0) {
-      // ================================================================ the products
-      constexpr uint32_t s_desc = umma_idesc_f16(kRows, kTokens), o_desc = umma_idesc_f16(kRows, D);
-      auto product_s = [&](uint32_t tile) {
-        wait(k_full, tile);
-        tc_fence_after();
-#pragma unroll
-        for (int w = 0; w < kTerms; ++w)
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)  // 32 bytes of a swizzled row per step of 16
-            umma_f16(tmem + tile % kS * kTokens,
-                     umma_desc_sw128(q_tile + w * P::kQTerm + k / 4 * (kRows * 128)) + 2 * (k % 4),
-                     umma_desc_sw128(k_tile + k / 4 * (kTokens * 128)) + 2 * (k % 4), s_desc, w > 0 || k > 0);
-        umma_commit(s_done(tile));
-      };
-      auto product_o = [&](uint32_t tile, bool add) {
-        wait(v_full, tile);
-        wait(p_full, tile);
-        tc_fence_after();
-#pragma unroll
-        for (int w = 0; w < kTerms; ++w)
-#pragma unroll
-          for (int k = 0; k < kTokens / 16; ++k)
-            umma_f16_ts(tmem + P::kO,
-                        tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens) + 8 * k,
-                        umma_desc_sw128(v_tile + k / 4 * (D * 128)) + 2 * (k % 4), o_desc, add || w > 0 || k > 0);
-        umma_commit(pv_done);
-      };
-      if (kS == 2) product_s(tiles);
-      for (uint32_t j = 0; j < n_tiles; ++j) {
-        if (kS == 1)
-          product_s(tiles + j);
-        else if (j + 1 < n_tiles)
-          product_s(tiles + j + 1);
-        product_o(tiles + j, j > 0);
       }
     }
     tiles += n_tiles;

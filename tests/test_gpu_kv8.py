@@ -378,6 +378,34 @@ def test_attn_repeats_bit_for_bit_on_any_stream_and_in_a_graph(eng):
             assert torch.equal(out, other)
 
 
+@pytest.mark.parametrize("dtype,d", [("f32", 64), ("bf16", 64), ("f32", 128), ("bf16", 128), ("f32", 256), ("bf16", 256), ("f32", 512)])
+def test_attn_prompts_repeat_bit_for_bit(eng, dtype, d):
+    """Sequences of several row groups and many tiles, split over CTAs: warps that run ahead of one
+    another must not change anything."""
+    news, lens = [1, 130, 0, 257, 64], [90, 130, 0, 300, 3000]
+    cache, q, out = check_attn(eng, dtype, 8, 1, d, 32, news, lens)
+    start, kv_len, _ = rows_of(news, lens)
+    for _ in range(20):
+        other = torch.empty_like(q)
+        eng.kv8_attn(cache.kv8(), DT[dtype][0], q, other, start, kv_len, sum(news), 8, d ** -0.5)
+        assert torch.equal(out, other)
+    eng.sync()
+
+
+@pytest.mark.parametrize("new", [1, 20])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_attn_scale_zero_and_negative(eng, new, scale):
+    d, total = 64, 100 + new
+    cache = Cache([total], 16, 1, d, 6)
+    q = torch.randn(new, 2 * d, device="cuda")
+    out = torch.empty_like(q)
+    start, kv_len, _ = rows_of([new], [total])
+    eng.kv8_attn(cache.kv8(), sx.DTYPE_F32, q, out, start, kv_len, new, 2, scale)
+    eng.sync()
+    want, mass, dz = want_attn(cache, q, [new], [total], 2, scale, 0)
+    assert ((out.double() - want).abs() <= tolerance("f32", want, mass, dz, d)).all()
+
+
 def test_attn_refusals(eng):
     c = Cache([20], 16, 2, 64, 1)
     q = torch.zeros(1, 4 * 64, device="cuda")
