@@ -7,15 +7,17 @@
 // tensor memory, P goes back there as f16 over S and is the second product's A operand.  e4m3 is
 // exact in f16, so K and V are widened on the way to shared memory; f32 rows split Q and P into two
 // f16 terms, with twice the products.  Warps:
-//   0 .. 3   softmax, a thread per row: S from tensor memory 32 columns at a time, the next ones on
-//            their way, P back.  The maximum that the exponentials refer to moves only when it grows
-//            by 2^8; the row of O, and of P so far, is then rescaled in tensor memory.
+//   0 .. 3   softmax, a thread per row: the row of S from tensor memory, P back.  The maximum that the
+//            exponentials refer to moves only when it grows by 2^8; the row of O is then rescaled in
+//            tensor memory.
 //   4 ..     widen K and V.  A warp takes a pair of blocks (32 tokens): the cache's 16-byte pieces
 //            become 16-byte stores of the 128-byte-swizzled tiles for a fitting order of the tokens
 //            (tile position 32 q + 8 (t % 8 / 2) + 4 half + 2 (t / 8) + t % 2) and of V's elements
 //            (tile row 32 p + 8 (d % 4) + f(d % 32 / 4), f a permutation of 8).  The softmax undoes
 //            the first in its masks and scales, the output the second: both are register indexes.
-// A thread of warp 0 issues the products (a warp of their own would cost the others registers).
+// A thread of warp 0 issues the products (a warp of their own would cost the others registers).  What runs
+// seldom is out of line and loops stay loops: four warps a role do not hide the fetching of 100 KB of
+// instructions (unrolled throughout, the kernel spent 20 cycles an instruction).
 // Bound by shared memory (the tiles' stores and the products' reads) and exponentials (16 a cycle
 // and SM, as many as a product of head size 128 takes cycles).  Up to head size 128 two CTAs share an
 // SM and fill each other's waits; above, two S tiles let the next product run beside the softmax.
@@ -33,6 +35,7 @@ namespace {
 
 constexpr uint32_t kRows = 128;      // packed rows of a problem
 constexpr float kPromptOffset = 6.0f, kSlack = 8.0f;
+constexpr float kMinScale = 1.17549435e-38f;  // a product with a masked -inf stays that
 
 template <int D, bool SPLIT>
 struct PromptShape {
@@ -67,76 +70,87 @@ struct GroupCost {
   }
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (PromptShape<D, sizeof(T) == 4>::kCtas))
-    kv8_prompt_kernel(Kv8AttnArgs a) {
-  constexpr bool kSplit = sizeof(T) == 4;
-  using P = PromptShape<D, kSplit>;
-  constexpr int kTokens = P::kTokens, kS = P::kS, kWiden = P::kWiden, kTerms = P::kTerms;
-  constexpr int kTileBlocks = kTokens / kKv8Block;
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[9];
-  __shared__ uint32_t tmem_slot, last_flag, nan_mask[2][kTokens / 32];
-  __shared__ volatile uint32_t abort_flag;
-  __shared__ float row_mul[kRows];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const uint32_t q_tile = (smem_u32(smem_raw) + 1023) & ~1023u;  // [terms][D / 64][128 rows][128 B]
-  const uint32_t k_tile = q_tile + kTerms * P::kQTerm;           // [D / 64][tokens][128 B]
-  const uint32_t v_tile = k_tile + P::kTile;                     // [tokens / 64][D][128 B]
-  const uint32_t bar = smem_u32(bars);
-  // Waits are for a phase's parity, so a waiter must be sure of the phase before and ahead of the one
-  // after.  The threads that widen and the one that issues go tile by tile; a softmax warp may be a
-  // tile ahead of another when there are two S tiles, so what it waits for or arrives at has a
-  // barrier for even and one for odd tiles: S of a tile done means that all of two tiles back is.
-  const uint32_t k_full = bar;
-  auto v_full = [&](uint32_t t) { return bar + 8 + 8 * (t & 1); };
-  auto pv_done = [&](uint32_t t) { return bar + 24 + 8 * (t & 1); };
-  auto s_done = [&](uint32_t t) { return bar + 40 + 8 * (t % kS); };
-  auto p_full = [&](uint32_t t) { return bar + 56 + 8 * (t % kS); };
-  if (threadIdx.x == 0) {
-    mbar_init(k_full, kWiden);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(v_full(i), kWiden);
-      mbar_init(pv_done(i), 1);
-    }
-    for (int i = 0; i < kS; ++i) {
-      mbar_init(s_done(i), 1);
-      mbar_init(p_full(i), 4);
-    }
-    abort_flag = 0;
-    fence_mbar_init();
-  }
-  if (warp == 0) {
-    tmem_alloc(smem_u32(&tmem_slot), P::kCols);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_slot;
-  pdl_launch_dependents();
-  pdl_wait();
+SX_DEV void st_shared16(uint32_t dst, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+               : "memory");
+}
 
-  // A wait that runs out ends the CTA's waiting altogether: what follows runs through on whatever
-  // is there, and the error word says so.
-  auto wait = [&](uint32_t b, uint32_t parity) {
-    if (abort_flag) return;
-    if (!mbar_wait_bounded(b, parity & 1)) {
-      abort_flag = 1;
-      raise_error(a.err, kDevWaitTimeout);
-    }
-  };
+// Waits are for a phase's parity, so a waiter must be sure of the phase before and ahead of the one
+// after.  The threads that widen and the one that issues go tile by tile; a softmax warp may be a tile
+// ahead of another when there are two S tiles, so what it waits for or arrives at has a barrier for
+// even and one for odd tiles: S of a tile done means that all of two tiles back is.
+template <int S>
+struct PromptBars {
+  uint32_t k_full;
+  SX_DEV explicit PromptBars(uint32_t at) : k_full(at) {}
+  SX_DEV uint32_t v_full(uint32_t t) const { return k_full + 8 + 8 * (t & 1); }
+  SX_DEV uint32_t pv_done(uint32_t t) const { return k_full + 24 + 8 * (t & 1); }
+  SX_DEV uint32_t s_done(uint32_t t) const { return k_full + 40 + 8 * (t % S); }
+  SX_DEV uint32_t p_full(uint32_t t) const { return k_full + 56 + 8 * (t % S); }
+};
 
-  // ---- this CTA's run of the line; every warp finds it alike
-  const uint64_t unit = (uint64_t)a.gqa * kTokens;  // line length of a tile
-  auto cost_of = [&](const Kv8Rows &r) {
-    GroupCost k;
-    k.base = (uint64_t)(r.len - r.n) * a.gqa;
-    k.cap = a.window ? (uint64_t)a.window * a.gqa + kRows + 2 * a.gqa : ~0ull >> 1;
-    k.over = unit;
-    k.groups = (r.n * a.gqa + kRows - 1) / kRows;
-    return k;
-  };
+// This thread's row of `cols` f32 columns of tensor memory times f.  A whole warp calls it, seldom:
+// out of line it stays out of the way of the loop's instructions.
+__device__ __noinline__ void rescale_row(uint32_t col, int cols, float f) {
+#pragma unroll 1
+  for (int d = 0; d < cols; d += 16) {
+    uint32_t o[16];
+    tmem_ld16(col + d, o);
+    tmem_wait_ld(o);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+    tmem_st16(col + d, o);
+  }
+}
+
+enum Role { kSoftmax, kWidenKv };
+
+// What the CTA's threads share.
+template <int TOKENS>
+struct PromptShared {
+  uint64_t bars[9];
+  uint32_t tmem_slot, last_flag, abort_flag;
+  uint32_t nan_mask[2][TOKENS / 32];
+  float row_mul[kRows];
+  float4 block[4][TOKENS / kKv8Block];  // softmax warps: {k scale, log2(v scale), 1 / v scale, there}
+};
+
+// A wait that runs out ends the CTA's waiting altogether: what follows runs through on whatever is
+// there, and the error word says so.
+__device__ __noinline__ void wait_or_abort(uint32_t b, uint32_t parity, volatile uint32_t *abort_flag, uint32_t *err) {
+  if (mbar_try_wait(b, parity & 1) || *abort_flag) return;
+  if (!mbar_wait_bounded(b, parity & 1)) {
+    *abort_flag = 1;
+    raise_error(err, kDevWaitTimeout);
+  }
+}
+
+// block / blocks per page (up to 64): a product with 2^32 / blocks rounded up, at most one too much
+struct PageDiv {
+  uint32_t per, magic;
+  SX_DEV explicit PageDiv(uint32_t page_tokens) : per(page_tokens / kKv8Block), magic(0xFFFFFFFFu / per + 1) {}
+  SX_DEV uint32_t page(uint32_t x) const {
+    const uint32_t q = per == 1 ? x : __umulhi(x, magic);
+    return q * per > x ? q - 1 : q;
+  }
+};
+
+SX_DEV GroupCost cost_of(const Kv8AttnArgs &a, const Kv8Rows &r, uint64_t unit) {
+  GroupCost k;
+  k.base = (uint64_t)(r.len - r.n) * a.gqa;
+  k.cap = a.window ? (uint64_t)a.window * a.gqa + kRows + 2 * a.gqa : ~0ull >> 1;
+  k.over = unit;
+  k.groups = (r.n * a.gqa + kRows - 1) / kRows;
+  return k;
+}
+
+// A CTA's run [begin, end) of the line, the sequence that holds begin and where that starts.
+struct Run {
+  uint64_t begin, end, length, at;
+  uint32_t b;
+};
+__device__ __noinline__ Run find_run(const Kv8AttnArgs &a, uint64_t unit) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto cost = [&](uint32_t i) -> uint64_t {
     Kv8Rows r;
     if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, i, &r)) {
@@ -144,42 +158,175 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
       return 0;
     }
     if (r.n == 0) return 0;
-    const GroupCost k = cost_of(r);
+    const GroupCost k = cost_of(a, r, unit);
     return k.before(k.groups) * a.c.num_kv;
   };
-  uint64_t begin = 0, end = 0, run = 1, at = 0;  // at: where the next problem starts
-  uint32_t b;
-  {
-    const uint32_t per = (a.c.num_seqs + 31) / 32;
-    const uint32_t b0 = lane * per, b1 = min(a.c.num_seqs, b0 + per);
-    uint64_t mine = 0;
-    for (uint32_t i = b0; i < b1; ++i) mine += cost(i);
-    uint64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
-    }
-    const uint64_t total = __shfl_sync(0xffffffffu, incl, 31);
-    run = (total + gridDim.x - 1) / gridDim.x;
-    run = run > a.min_run * unit ? run : a.min_run * unit;
-    begin = run * blockIdx.x;
-    end = begin + run < total ? begin + run : total;
-    const uint32_t who = min(31, __popc(__ballot_sync(0xffffffffu, incl <= begin)));
-    at = incl - mine;
-    b = b0;
-    if (lane == (int)who && begin < end)
-      for (uint64_t n; (n = cost(b)) <= begin - at; at += n) ++b;
-    at = __shfl_sync(0xffffffffu, at, who);
-    b = __shfl_sync(0xffffffffu, b, who);
-    if (begin >= end) at = end;  // no run for this CTA
+  const uint32_t per = (a.c.num_seqs + 31) / 32;
+  const uint32_t b0 = lane * per, b1 = min(a.c.num_seqs, b0 + per);
+  uint64_t mine = 0;
+  for (uint32_t i = b0; i < b1; ++i) mine += cost(i);
+  uint64_t incl = mine;
+#pragma unroll 1
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
   }
+  const uint64_t total = __shfl_sync(0xffffffffu, incl, 31);
+  Run x;
+  x.length = (total + gridDim.x - 1) / gridDim.x;
+  x.length = x.length > a.min_run * unit ? x.length : a.min_run * unit;
+  x.begin = x.length * blockIdx.x;
+  x.end = x.begin + x.length < total ? x.begin + x.length : total;
+  const uint32_t who = min(31, __popc(__ballot_sync(0xffffffffu, incl <= x.begin)));
+  uint64_t at = incl - mine;
+  uint32_t b = b0;
+  if (lane == (int)who && x.begin < x.end)
+    for (uint64_t n; (n = cost(b)) <= x.begin - at; at += n) ++b;
+  x.at = __shfl_sync(0xffffffffu, at, who);
+  x.b = __shfl_sync(0xffffffffu, b, who);
+  if (x.begin >= x.end) x.at = x.end;  // no run for this CTA
+  return x;
+}
+
+// A problem's place: first row of the sequence, first packed row, how many, kv head.
+struct Where {
+  uint32_t r0, row0, rows, head;
+  SX_DEV size_t row(const Kv8AttnArgs &a, uint32_t i) const { return r0 + (row0 + i) / a.gqa; }
+  SX_DEV uint32_t col(const Kv8AttnArgs &a, uint32_t i) const {
+    return (head * a.gqa + (row0 + i) % a.gqa) * a.c.head_dim;
+  }
+};
+
+// Q: power-of-two scaled f16 terms, K-major 128-byte swizzle, by all threads.
+template <typename T, int D>
+__device__ __noinline__ void put_q(const Kv8AttnArgs &a, const Where &w, uint32_t q_tile, float *row_mul) {
+  constexpr bool kSplit = sizeof(T) == 4;
+  using P = PromptShape<D, kSplit>;
+  constexpr int kLanes = D / 8, kPass = 32 / kLanes;  // lanes of a row, rows of a warp's pass
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t li = lane % kLanes;
+#pragma unroll 2
+  for (uint32_t i0 = warp * kPass; i0 < kRows; i0 += P::kThreads / 32 * kPass) {
+    const uint32_t i = i0 + lane / kLanes;
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+    if (i < w.rows) {
+      const T *src = static_cast<const T *>(a.q) + w.row(a, i) * a.q_ld + w.col(a, i) + 8 * li;
+      constexpr int kVec = 16 / (int)sizeof(T);
+#pragma unroll
+      for (int k = 0; k < 8; k += kVec) {
+        float v[kVec];
+        load_vec<T, kVec>(src + k, v);
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) x[k + j] = v[j];
+      }
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[k]));
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    int e = (int)(__float_as_uint(m) >> 23) - 127;
+    if (m == 0.0f || e == 128) e = 0;  // nothing to scale; an infinity stays one
+    e = min(max(e, -126), 126);
+    const float inv = a.scale < 0.0f ? -exp2_int(-e) : exp2_int(-e);
+    if (li == 0) row_mul[i] = fabsf(a.scale) * kLog2e * exp2_int(e);
+    uint32_t hi[4], low[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float v0 = x[2 * k] * inv, v1 = x[2 * k + 1] * inv;
+      hi[k] = pack_f16(v0, v1);
+      if constexpr (kSplit) low[k] = pack_f16_rest(v0, v1, hi[k]);
+    }
+    const uint32_t dst = q_tile + li / 8 * (kRows * 128) + i * 128 + (((li % 8) ^ (i & 7)) << 4);
+    st_shared16(dst, hi);
+    if constexpr (kSplit) st_shared16(dst + P::kQTerm, low);
+  }
+  fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
+}
+
+// The last CTA to finish a part of a problem merges the n parts, a warp per row.
+template <typename T, int D>
+__device__ __noinline__ void merge_parts(const Kv8AttnArgs &a, const Where &w, uint32_t slot0, uint32_t c0, uint32_t n) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const float *ml = a.part, *po = a.part + (size_t)2 * gridDim.x * kRows * 2;
+  auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : 2 * (c0 + k); };
+  for (uint32_t i = warp; i < w.rows; i += blockDim.x / 32) {
+    float m = -INFINITY, l = 0.0f;
+    for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, __ldcg(ml + ((size_t)slot_of(k) * kRows + i) * 2));
+    m = warp_max(m);
+    float sum[D / 32];
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) sum[d] = 0.0f;
+#pragma unroll 1
+    for (uint32_t k = 0; k < n; ++k) {
+      const size_t at_row = (size_t)slot_of(k) * kRows + i;
+      const float mk = __ldcg(ml + at_row * 2), f = mk == -INFINITY ? 0.0f : ex2(mk - m);
+      l = fmaf(__ldcg(ml + at_row * 2 + 1), f, l);
+#pragma unroll
+      for (int d = 0; d < D / 64; ++d) {
+        const float2 v = __ldcg(reinterpret_cast<const float2 *>(po + at_row * D + 64 * d + 2 * lane));
+        sum[2 * d] = fmaf(v.x, f, sum[2 * d]);
+        sum[2 * d + 1] = fmaf(v.y, f, sum[2 * d + 1]);
+      }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *out = static_cast<T *>(a.out) + w.row(a, i) * a.out_ld + w.col(a, i);
+#pragma unroll
+    for (int d = 0; d < D / 64; ++d) {
+      const float y[2] = {sum[2 * d] * inv, sum[2 * d + 1] * inv};
+      store_vec<T, 2>(out + 64 * d + 2 * lane, y);
+    }
+  }
+  if (threadIdx.x == 0) a.cnt[c0] = 0;
+}
+
+// One product, issued by one thread: `steps` of 16 along K, A from shared memory (a_tile) or tensor
+// memory (a_col); 32 bytes of a swizzled row per step, a panel of 64 elements every four.
+__device__ __noinline__ void issue_ss(uint32_t d, uint32_t a_tile, uint32_t a_panel, uint32_t b_tile, uint32_t b_panel,
+                                      uint32_t idesc, int steps, bool add) {
+#pragma unroll 1
+  for (int k = 0; k < steps; k += 4) {
+    const uint64_t x = umma_desc_sw128(a_tile + k / 4 * a_panel), y = umma_desc_sw128(b_tile + k / 4 * b_panel);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) umma_f16(d, x + 2 * j, y + 2 * j, idesc, add || k + j > 0);
+  }
+}
+__device__ __noinline__ void issue_ts(uint32_t d, uint32_t a_col, uint32_t b_tile, uint32_t b_panel, uint32_t idesc,
+                                      int steps, bool add) {
+#pragma unroll 1
+  for (int k = 0; k < steps; k += 4) {
+    const uint64_t y = umma_desc_sw128(b_tile + k / 4 * b_panel);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) umma_f16_ts(d, a_col + 8 * (k + j), y + 2 * j, idesc, add || k + j > 0);
+  }
+}
+
+// One role's way through the CTA's run.
+template <typename T, int D, Role ROLE>
+SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
+                        PromptShared<PromptShape<D, sizeof(T) == 4>::kTokens> &sh) {
+  constexpr bool kSplit = sizeof(T) == 4;
+  using P = PromptShape<D, kSplit>;
+  constexpr int kTokens = P::kTokens, kS = P::kS, kWiden = P::kWiden, kTerms = P::kTerms;
+  constexpr int kTileBlocks = kTokens / kKv8Block;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t q_tile = (smem_u32(smem_raw) + 1023) & ~1023u;  // [terms][D / 64][128 rows][128 B]
+  const uint32_t k_tile = q_tile + kTerms * P::kQTerm;           // [D / 64][tokens][128 B]
+  const uint32_t v_tile = k_tile + P::kTile;                     // [tokens / 64][D][128 B]
+  const PromptBars<kS> bars(smem_u32(sh.bars));
+  const uint32_t tmem = sh.tmem_slot;
+  auto wait = [&](uint32_t b, uint32_t parity) { wait_or_abort(b, parity, &sh.abort_flag, a.err); };
+  const PageDiv div(a.c.page_tokens);
+  const uint64_t unit = (uint64_t)a.gqa * kTokens;  // line length of a tile
+  const uint64_t begin = run.begin, end = run.end;
 
   uint32_t tiles = 0;  // tiles done, over all problems: every barrier's phase follows from it
   Kv8Rows r;
   GroupCost gc;
-  uint32_t left = 0, head = 0, group = 0;
-  uint64_t length = 0;
+  uint64_t at = run.at, length = 0;  // where the next problem starts, its length
+  uint32_t b = run.b, left = 0, head = 0, group = 0;
   bool fresh = true;  // the first sequence: its first problems may lie before the run
   for (; at < end; at += length, --left) {
     if (left != 0) {
@@ -192,7 +339,7 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
       const bool ok = kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r);
       ++b;
       if (!ok || r.n == 0) continue;
-      gc = cost_of(r);
+      gc = cost_of(a, r, unit);
       left = gc.groups * a.c.num_kv;
       head = group = 0;
       if (fresh) {
@@ -223,15 +370,16 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
     if (t0 >= t1) continue;  // no tile starts in the run
     const uint32_t n_tiles = t1 - t0;
     const uint32_t *table = a.c.table + (size_t)(b - 1) * a.c.max_pages;
-    // record pair of block s of the problem; ~0: nothing to read
-    auto record = [&](uint32_t s) -> uint64_t {
-      if (s >= blocks) return ~0ull;
-      const uint32_t per = a.c.page_tokens / kKv8Block, page = table[(first + s) / per];
+    // Block s of the problem: its page (asked for a tile before it is used, so that nothing waits
+    // for the table) and its record pair, ~0 where there is nothing to read.
+    const uint32_t there = min(blocks, t1 * kTileBlocks);
+    auto page_of = [&](uint32_t s) { return s < there ? table[div.page(first + s)] : SX_NO_PAGE; };
+    auto record = [&](uint32_t s, uint32_t page) -> uint64_t {
       if (page >= a.c.num_pages) {
-        raise_error(a.err, kDevBadSlot);
+        if (s < there) raise_error(a.err, kDevBadSlot);
         return ~0ull;
       }
-      return ((uint64_t)page * a.c.num_kv + head) * per + (first + s) % per;
+      return ((uint64_t)page * a.c.num_kv + head) * div.per + (first + s - div.page(first + s) * div.per);
     };
     // tiles whose keys every row sees
     const uint32_t all_hi = pos_lo, all_lo = a.window && pos_hi >= a.window ? pos_hi - a.window + 1 : 0;
@@ -239,204 +387,147 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
       const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
       return key0 < all_lo || key0 + kTokens - 1 > all_hi;
     };
-
-    // ---- Q: power-of-two scaled f16 terms, K-major 128-byte swizzle
-    {
-      constexpr int kLanes = D / 8, kPass = 32 / kLanes;  // lanes of a row, rows of a warp's pass
-      const uint32_t li = lane % kLanes;
-      for (uint32_t i0 = warp * kPass; i0 < kRows; i0 += P::kThreads / 32 * kPass) {
-        const uint32_t i = i0 + lane / kLanes, pr = row0 + i;
-        const bool in = i < rows;
-        float x[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-        if (in) {
-          const T *src = static_cast<const T *>(a.q) + (size_t)(r.r0 + pr / a.gqa) * a.q_ld +
-                         (size_t)(head * a.gqa + pr % a.gqa) * D + 8 * li;
-          constexpr int kVec = 16 / (int)sizeof(T);
-#pragma unroll
-          for (int k = 0; k < 8; k += kVec) {
-            float v[kVec];
-            load_vec<T, kVec>(src + k, v);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) x[k + j] = v[j];
-          }
-        }
-        float m = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[k]));
-#pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        int e = (int)(__float_as_uint(m) >> 23) - 127;
-        if (m == 0.0f || e == 128) e = 0;  // nothing to scale; an infinity stays one
-        e = min(max(e, -126), 126);
-        const float inv = a.scale < 0.0f ? -exp2_int(-e) : exp2_int(-e);
-        if (li == 0) row_mul[i] = fabsf(a.scale) * kLog2e * exp2_int(e);
-        uint32_t hi[4], low[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float v0 = x[2 * k] * inv, v1 = x[2 * k + 1] * inv;
-          hi[k] = pack_f16(v0, v1);
-          if constexpr (kSplit) low[k] = pack_f16_rest(v0, v1, hi[k]);
-        }
-        const uint32_t dst = q_tile + li / 8 * (kRows * 128) + i * 128 + (((li % 8) ^ (i & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(hi[0]), "r"(hi[1]), "r"(hi[2]), "r"(hi[3]) : "memory");
-        if constexpr (kSplit)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + P::kQTerm), "r"(low[0]), "r"(low[1]), "r"(low[2]), "r"(low[3]) : "memory");
-      }
-      fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
-    }
+    const Where where{r.r0, row0, rows, head};
+    put_q<T, D>(a, where, q_tile, sh.row_mul);
     __syncthreads();
 
-    // ---- the products, for one thread
-    constexpr uint32_t s_desc = umma_idesc_f16(kRows, kTokens), o_desc = umma_idesc_f16(kRows, D);
-    auto product_s = [&](uint32_t tile) {
-      wait(k_full, tile);
-      tc_fence_after();
-#pragma unroll
-      for (int w = 0; w < kTerms; ++w)
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)  // 32 bytes of a swizzled row per step of 16
-          umma_f16(tmem + tile % kS * kTokens,
-                   umma_desc_sw128(q_tile + w * P::kQTerm + k / 4 * (kRows * 128)) + 2 * (k % 4),
-                   umma_desc_sw128(k_tile + k / 4 * (kTokens * 128)) + 2 * (k % 4), s_desc, w > 0 || k > 0);
-      umma_commit(s_done(tile));
-    };
-    auto product_o = [&](uint32_t tile, bool add) {
-      wait(v_full(tile), tile / 2);
-      wait(p_full(tile), tile / kS);
-      tc_fence_after();
-#pragma unroll
-      for (int w = 0; w < kTerms; ++w)
-#pragma unroll
-        for (int k = 0; k < kTokens / 16; ++k)
-          umma_f16_ts(tmem + P::kO,
-                      tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens) + 8 * k,
-                      umma_desc_sw128(v_tile + k / 4 * (D * 128)) + 2 * (k % 4), o_desc, add || w > 0 || k > 0);
-      umma_commit(pv_done(tile));
-    };
-
-    if (warp < 4) {
+    if constexpr (ROLE == kSoftmax) {
+      // -- the products, for one thread
+      auto product_s = [&](uint32_t tile) {
+        wait(bars.k_full, tile);
+        tc_fence_after();
+        for (int w = 0; w < kTerms; ++w)
+          issue_ss(tmem + tile % kS * kTokens, q_tile + w * P::kQTerm, kRows * 128, k_tile, kTokens * 128,
+                   umma_idesc_f16(kRows, kTokens), D / 16, w > 0);
+        umma_commit(bars.s_done(tile));
+      };
+      auto product_o = [&](uint32_t tile, bool add) {
+        wait(bars.v_full(tile), tile / 2);
+        wait(bars.p_full(tile), tile / kS);
+        tc_fence_after();
+        for (int w = 0; w < kTerms; ++w)
+          issue_ts(tmem + P::kO, tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens), v_tile, D * 128,
+                   umma_idesc_f16(kRows, D), kTokens / 16, add || w > 0);
+        umma_commit(bars.pv_done(tile));
+      };
       // ================================================================ softmax: thread = row
       const uint32_t i = threadIdx.x, lanes = (uint32_t)(32 * warp) << 16;
-      const float mul = row_mul[i];
+      const float mul = sh.row_mul[i];
       const uint32_t pos = pos0 + (row0 + min(i, rows - 1)) / a.gqa;
       const uint32_t see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_n = pos - see_lo;
       float ref = -INFINITY, l = 0.0f;
-      // scales of a tile's blocks: lane s < kTileBlocks holds block s; a tile ahead
-      auto scales = [&](uint32_t t) -> float2 {
+      float4 *const block = sh.block[warp];
+      // Scales of a tile's blocks, block s in lane s: a tile ahead, their pages two; put where every
+      // thread of the warp reads them while the products run.
+      auto page_at = [&](uint32_t t) { return lane < kTileBlocks ? page_of(t * kTileBlocks + lane) : SX_NO_PAGE; };
+      auto scales = [&](uint32_t t, uint32_t page) -> float2 {
         float2 f = make_float2(0.0f, 0.0f);  // v scale 0: a block that is not there
-        if (lane < kTileBlocks && t < t1) {
-          const uint64_t rec = record(t * kTileBlocks + lane);
+        if (lane < kTileBlocks) {
+          const uint64_t rec = record(t * kTileBlocks + lane, page);
           if (rec != ~0ull) f = *reinterpret_cast<const float2 *>(a.c.scale + 2 * rec);
         }
         return f;
       };
-      float2 next = scales(t0);
+      // the tile's block table; true where some row does not see all of the tile or a block is missing
+      auto set_blocks = [&](uint32_t t, float2 f) {
+        if (lane < kTileBlocks) {
+          const int e = kv8_scale_exponent(f.y);
+          block[lane] = make_float4(f.x, (float)e, exp2_int(-e), f.y != 0.0f ? 1.0f : 0.0f);
+        }
+        __syncwarp();
+        return is_mixed(t) || __any_sync(0xffffffffu, lane < kTileBlocks && f.y == 0.0f);
+      };
       if (threadIdx.x == 0) product_s(tiles);
+      __syncwarp();
+      bool masked = set_blocks(t0, scales(t0, page_at(t0)));
+      float2 next = scales(t0 + 1, page_at(t0 + 1));
+      uint32_t next_page = page_at(t0 + 2);
+#pragma unroll 1
       for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t tile = tiles + (t - t0), s_col = tmem + lanes + tile % kS * kTokens;
-        const float2 sc = next;
-        next = scales(t + 1);
-        // masked: some row does not see all of the tile, or a block of it is not there
-        const bool mixed = is_mixed(t);
-        const bool masked = mixed || __any_sync(0xffffffffu, lane < kTileBlocks && sc.y == 0.0f);
-        const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
-        wait(s_done(tile), tile / kS);
-        if (mixed) wait(v_full(tile), tile / 2);  // the NaN masks come with V
-        tc_fence_after();
         const uint32_t low_col = tmem + lanes + P::kLow + tile % kS * (kTokens / 2);
-        uint32_t s[2][32];
-        tmem_ld32(s_col, s[0]);
-        // P over S: chunk q's 16 columns lie in S columns that have been read
+        const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
+        wait(bars.s_done(tile), tile / kS);
+        const bool mixed = masked && is_mixed(t);
+        if (mixed) wait(bars.v_full(tile), tile / 2);  // the NaN masks come with V
+        __syncwarp();
+        tc_fence_after();
+        // the tokens of chunk q that the row sees, a bit each
+        auto visible = [&](int q) -> uint32_t {
+          const uint32_t k0 = key0 + 32 * q, see_hi = see_lo + see_n + 1;  // seen: see_lo .. see_hi - 1
+          const uint32_t lo = see_lo > k0 ? see_lo - k0 : 0, hi = see_hi > k0 ? see_hi - k0 : 0;
+          uint32_t m = lo < 32 && hi > lo ? (hi < 32 ? (1u << hi) - 1 : ~0u) & (~0u << lo) : 0;
+          if (block[2 * q].w == 0.0f) m &= 0xFFFF0000u;
+          if (block[2 * q + 1].w == 0.0f) m &= 0x0000FFFFu;
+          return m;
+        };
+        // column k of a chunk is token 16 (k / 4 % 2) + 8 (k / 2 % 2) + 2 (k / 8) + k % 2
+        auto mask = [&](uint32_t (&s)[32], uint32_t vis) {
 #pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (!(vis & (1u << (16 * ((k >> 2) & 1) + 8 * ((k >> 1) & 1) + 2 * (k >> 3) + (k & 1))))) s[k] = 0xFF800000u;
+        };
+        // -- the largest x + log2(v scale)
+        float top = -INFINITY;
+#pragma unroll 1
         for (int q = 0; q < kTokens / 32; ++q) {
-          uint32_t (&x)[32] = s[q & 1];
-          float km[2], lv[2], unv[2], m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-          uint32_t vis[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float ks = __shfl_sync(0xffffffffu, sc.x, 2 * q + h), vs = __shfl_sync(0xffffffffu, sc.y, 2 * q + h);
-            lv[h] = (float)kv8_scale_exponent(vs);
-            km[h] = fmaxf(ks * mul, 1.17549435e-38f);  // -inf stays -inf
-            unv[h] = exp2_int(-kv8_scale_exponent(vs));
-            vis[h] = vs != 0.0f;
-          }
-          tmem_wait_ld(x);
-          if (q + 1 < kTokens / 32) tmem_ld32(s_col + 32 * (q + 1), s[(q + 1) & 1]);
-          // -- the chunk's largest x + log2(v scale); a masked score becomes -inf
+          uint32_t s[32];
+          tmem_ld32(s_col + 32 * q, s);
+          const float4 f0 = block[2 * q], f1 = block[2 * q + 1];
+          tmem_wait_ld(s);
           if (masked) {
-            const uint32_t nan = mixed ? nan_mask[tile & 1][q] : 0;
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const int h = (k >> 2) & 1, tok = 16 * h + 8 * ((k >> 1) & 1) + 2 * (k >> 3) + (k & 1);
-              const bool seen = key0 + 32 * q + tok - see_lo <= see_n && vis[h];
-              if ((nan >> tok) & 1u) x[k] = 0x7FFFFFFFu;
-              if (!seen) x[k] = 0xFF800000u;
-            }
+            const uint32_t vis = visible(q);
+            if (mixed && (sh.nan_mask[tile & 1][q] & vis)) l = NAN;
+            mask(s, vis);
           }
+          float m[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int k = 0; k < 32; k += 8) {
-            m[0] = fmaxf(m[0], fmaxf(fmaxf(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), fmaxf(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]))));
-            m[1] = fmaxf(m[1], fmaxf(fmaxf(__uint_as_float(x[k + 4]), __uint_as_float(x[k + 5])), fmaxf(__uint_as_float(x[k + 6]), __uint_as_float(x[k + 7]))));
-          }
-          float top = -INFINITY;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (m[h] != -INFINITY) top = fmaxf(top, fmaf(m[h], km[h], lv[h]));
-          // -- one that outgrew the reference: rescale what the row has so far
-          const bool grow = top > ref + kSlack || (ref == -INFINITY && top > ref);
-          if (__any_sync(0xffffffffu, grow)) {
-            const float f = !grow ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - top);
-            if (grow) ref = top;
-            l *= f;
-            if (q + 1 < kTokens / 32) tmem_wait_ld(s[(q + 1) & 1]);
-            if (t > t0) {
-              wait(pv_done(tile - 1), (tile - 1) / 2);
-              tc_fence_after();
-#pragma unroll 1
-              for (int d = 0; d < D; d += 16) {
-                uint32_t o[16];
-                tmem_ld16(tmem + lanes + P::kO + d, o);
-                tmem_wait_ld(o);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                tmem_st16(tmem + lanes + P::kO + d, o);
-              }
-            }
+          for (int k = 0; k < 32; k += 4)
+            m[(k >> 2) & 1] = fmaxf(fmaxf(m[(k >> 2) & 1], fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 1]))),
+                                    fmaxf(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])));
+          top = fmaxf(top, fmaxf(fmaf(m[0], fmaxf(f0.x * mul, kMinScale), f0.y),
+                                 fmaf(m[1], fmaxf(f1.x * mul, kMinScale), f1.y)));
+        }
+        // -- one that outgrew the reference: rescale the row
+        const bool grow = top > ref + kSlack || (ref == -INFINITY && top > ref);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float f = !grow ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - top);
+          if (grow) ref = top;
+          l *= f;
+          if (t > t0) {
+            wait(bars.pv_done(tile - 1), (tile - 1) / 2);
+            __syncwarp();
+            tc_fence_after();
+            rescale_row(tmem + lanes + P::kO, D, f);
             tmem_wait_st();
+          }
+        }
+        const float shift = ref == -INFINITY ? 0.0f : ref - kPromptOffset;
 #pragma unroll 1
-            for (int d = 0; d < q * 16 * kTerms; d += 16) {
-              const uint32_t col = d < 16 * q ? s_col + d : low_col + d - 16 * q;
-              uint32_t o[16];
-              tmem_ld16(col, o);
-              tmem_wait_ld(o);
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&o[k]));
-                o[k] = pack_f16(v.x * f, v.y * f);
-              }
-              tmem_st16(col, o);
-            }
-          }
-          const float shift = ref == -INFINITY ? 0.0f : ref - kPromptOffset;
-          const float off[2] = {lv[0] - shift, lv[1] - shift};
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const int h = (k >> 2) & 1;
-            const float p = ex2(fmaf(__uint_as_float(x[k]), km[h], off[h]));
-            sum[h] += p;
-            x[k] = __float_as_uint(p);
-          }
-          l = fmaf(sum[0], unv[0], fmaf(sum[1], unv[1], l));
+        for (int q = 0; q < kTokens / 32; ++q) {
+          uint32_t s[32];
+          tmem_ld32(s_col + 32 * q, s);
+          const float4 f[2] = {block[2 * q], block[2 * q + 1]};
+          const float km[2] = {fmaxf(f[0].x * mul, kMinScale), fmaxf(f[1].x * mul, kMinScale)};
+          const float off[2] = {f[0].y - shift, f[1].y - shift};
+          float sum[2] = {0.0f, 0.0f};
           uint32_t hi[16];
+          tmem_wait_ld(s);
+          if (masked) mask(s, visible(q));
 #pragma unroll
-          for (int k = 0; k < 16; ++k) hi[k] = pack_f16(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1]));
-          tmem_st16(s_col + 16 * q, hi);
+          for (int k = 0; k < 32; k += 2) {
+            const int h = (k >> 2) & 1;
+            const float p0 = ex2(fmaf(__uint_as_float(s[k]), km[h], off[h]));
+            const float p1 = ex2(fmaf(__uint_as_float(s[k + 1]), km[h], off[h]));
+            sum[h] += p0 + p1;
+            hi[k / 2] = pack_f16(p0, p1);
+            if constexpr (kSplit) s[k / 2] = pack_f16_rest(p0, p1, hi[k / 2]);
+          }
+          l = fmaf(sum[0], f[0].z, fmaf(sum[1], f[1].z, l));
+          tmem_st16(s_col + 16 * q, hi);  // P over S: columns that have been read
           if constexpr (kSplit) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k)
-              hi[k] = pack_f16_rest(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1]), hi[k]);
+            for (int k = 0; k < 16; ++k) hi[k] = s[k];
             tmem_st16(low_col + 16 * q, hi);
           }
           // with a second S tile the next product runs beside the rest of this softmax
@@ -448,23 +539,25 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full(tile));
+        if (lane == 0) mbar_arrive(bars.p_full(tile));
         if (threadIdx.x == 0) {
           product_o(tile, t > t0);
           if (kS == 1 && t + 1 < t1) product_s(tile + 1);
         }
         __syncwarp();
+        masked = set_blocks(t + 1, next);
+        next = scales(t + 2, next_page);
+        next_page = page_at(t + 3);
       }
       // ---- the row's output, or its part
-      wait(pv_done(tiles + n_tiles - 1), (tiles + n_tiles - 1) / 2);
+      wait(bars.pv_done(tiles + n_tiles - 1), (tiles + n_tiles - 1) / 2);
+      __syncwarp();
       tc_fence_after();
       const bool whole = t0 == 0 && t1 == count;
       const uint32_t slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
       float *const ml = a.part + ((size_t)slot * kRows + i) * 2;
       float *const po = a.part + (size_t)2 * gridDim.x * kRows * 2 + ((size_t)slot * kRows + i) * D;
-      const uint32_t pr = row0 + i;
-      T *const out = static_cast<T *>(a.out) + (size_t)(r.r0 + pr / a.gqa) * a.out_ld +
-                     (size_t)(head * a.gqa + pr % a.gqa) * D;
+      T *const out = static_cast<T *>(a.out) + where.row(a, i) * a.out_ld + where.col(a, i);
       const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
       if (!whole && i < rows) {
         ml[0] = ref;
@@ -500,26 +593,28 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
       }
       tc_fence_before();
     } else {
+      const int g = lane >> 2, c = lane & 3;
       // ================================================================ widen K and V
       constexpr int kPairs = kTokens / 32, kShare = kWiden / kPairs;  // warps of a pair of blocks
       constexpr int kMine = D / 32 / kShare;                          // pieces of a warp
       static_assert(kMine >= 2, "pieces come in pairs");
       const uint32_t ww = warp - 4, pair = ww % kPairs, p0 = ww / kPairs * kMine;
-      struct Recs {
+      struct Two {
         uint64_t r[2];
       };
-      auto recs = [&](uint32_t t) -> Recs {
-        Recs x{{~0ull, ~0ull}};
-        if (t < t1) {
-          x.r[0] = record(t * kTileBlocks + 2 * pair);
-          x.r[1] = record(t * kTileBlocks + 2 * pair + 1);
-        }
-        return x;
+      struct Pages {
+        uint32_t p[2];
       };
-      uint4 raw_k[2][kMine], raw_v[2][kMine];
+      auto pages = [&](uint32_t t) -> Pages {
+        return {{page_of(t * kTileBlocks + 2 * pair), page_of(t * kTileBlocks + 2 * pair + 1)}};
+      };
+      auto recs = [&](uint32_t t, const Pages &x) -> Two {
+        return {{record(t * kTileBlocks + 2 * pair, x.p[0]), record(t * kTileBlocks + 2 * pair + 1, x.p[1])}};
+      };
+      uint4 raw[2][kMine];  // K of a tile, then its V: asked for as soon as the registers are free
       // K: lanes with odd g take the pieces of a pair in the other order, so that a store's eight
       // lanes meet all banks
-      auto fetch = [&](const Recs &x, int which, uint4 (&raw)[2][kMine]) {
+      auto fetch = [&](const Two &x, int which) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + (2 * x.r[h] + which) * (size_t)(16 * D);
@@ -529,14 +624,15 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
                                         : *reinterpret_cast<const uint4 *>(src + 512 * (p0 + (which ? p : p ^ (g & 1))) + 16 * lane);
         }
       };
-      Recs cur = recs(t0);
-      fetch(cur, 0, raw_k);
-      fetch(cur, 1, raw_v);
+      Two now = recs(t0, pages(t0));
+      fetch(now, 0);
+      Pages next = pages(t0 + 1);
       for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t tile = tiles + (t - t0);
         const bool mixed = is_mixed(t);
-        const Recs ahead = recs(t + 1);
-        if (tile > 0) wait(s_done(tile - 1), (tile - 1) / kS);  // the product before has read K
+        const Two ahead = recs(t + 1, next);
+        next = pages(t + 2);
+        if (tile > 0) wait(bars.s_done(tile - 1), (tile - 1) / kS);  // the product before has read K
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -544,33 +640,33 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
             const uint32_t piece = p0 + (p ^ (g & 1)), chunk = (piece & 1) * 4 + c;
             const uint32_t row = 32 * pair + 8 * (g / 2) + 4 * h + (g & 1);
             const uint32_t base = k_tile + piece / 2 * (kTokens * 128);
-            const uint4 w = raw_k[h][p];
+            const uint4 w = raw[h][p];
             uint32_t x[4];
             e4m3x4_f16(w.x, x[0], x[1]);
             e4m3x4_f16(w.y, x[2], x[3]);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(base + row * 128 + ((chunk ^ (row & 7)) << 4)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+            st_shared16(base + row * 128 + ((chunk ^ (row & 7)) << 4), x);
             e4m3x4_f16(w.z, x[0], x[1]);
             e4m3x4_f16(w.w, x[2], x[3]);
             const uint32_t row8 = row + 2;
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(base + row8 * 128 + ((chunk ^ (row8 & 7)) << 4)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+            st_shared16(base + row8 * 128 + ((chunk ^ (row8 & 7)) << 4), x);
           }
         fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
         __syncwarp();
-        if (lane == 0) mbar_arrive(k_full);
-        fetch(ahead, 0, raw_k);
+        if (lane == 0) mbar_arrive(bars.k_full);
+        fetch(now, 1);
 
-        if (tile > 0) wait(pv_done(tile - 1), (tile - 1) / 2);  // the product before has read V
+        if (tile > 0) wait(bars.pv_done(tile - 1), (tile - 1) / 2);  // the product before has read V
         if (mixed) {
           // A NaN would reach rows that do not see its token through 0 x NaN: it is taken out, and
           // its token marked for the rows that do.
-          if (ww == 0 && lane < kPairs) nan_mask[tile & 1][lane] = 0;
+          if (ww == 0 && lane < kPairs) sh.nan_mask[tile & 1][lane] = 0;
           asm volatile("bar.sync 1, %0;\n" ::"n"(kWiden * 32) : "memory");
           uint32_t bits = 0;
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int p = 0; p < kMine; ++p) {
-              uint32_t w[4] = {raw_v[h][p].x, raw_v[h][p].y, raw_v[h][p].z, raw_v[h][p].w};
+              uint32_t w[4] = {raw[h][p].x, raw[h][p].y, raw[h][p].z, raw[h][p].w};
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const uint32_t n = (((w[k] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
@@ -578,80 +674,83 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
                 // bytes are tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9 of block h
                 bits |= ((n & 1u) | ((n >> 7) & 2u) | ((n >> 8) & 0x100u) | ((n >> 15) & 0x200u)) << (2 * c + 16 * h);
               }
-              raw_v[h][p] = make_uint4(w[0], w[1], w[2], w[3]);
+              raw[h][p] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-          if (bits) atomicOr(&nan_mask[tile & 1][pair], bits);
+          if (bits) atomicOr(&sh.nan_mask[tile & 1][pair], bits);
         }
 #pragma unroll
         for (int p = 0; p < kMine; ++p) {
           const uint32_t fg = (g >> 1) | ((g & 1) << 2), chunk = (pair & 1) * 4 + c;
           const uint32_t base = v_tile + pair / 2 * (D * 128) + (32 * (p0 + p) + fg) * 128 + ((chunk ^ fg) << 4);
-          const uint32_t wa[4] = {raw_v[0][p].x, raw_v[0][p].y, raw_v[0][p].z, raw_v[0][p].w};
-          const uint32_t wb[4] = {raw_v[1][p].x, raw_v[1][p].y, raw_v[1][p].z, raw_v[1][p].w};
+          const uint32_t wa[4] = {raw[0][p].x, raw[0][p].y, raw[0][p].z, raw[0][p].w};
+          const uint32_t wb[4] = {raw[1][p].x, raw[1][p].y, raw[1][p].z, raw[1][p].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // element 4 g + k: row 8 k + f(g) of the piece
             uint32_t x[4];
             e4m3x4_f16(wa[k], x[0], x[1]);
             e4m3x4_f16(wb[k], x[2], x[3]);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(base + k * 8 * 128), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+            st_shared16(base + k * 8 * 128, x);
           }
         }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(v_full(tile));
-        fetch(ahead, 1, raw_v);
+        if (lane == 0) mbar_arrive(bars.v_full(tile));
+        fetch(ahead, 0);
+        now = ahead;
       }
     }
     tiles += n_tiles;
     __syncthreads();  // Q, the tiles and O are free; the parts are written
-
     if (!(t0 == 0 && t1 == count)) {
       // CTAs c0 .. c1 hold parts of this problem; c0 counts them
-      const uint32_t c0 = (uint32_t)(at / run), c1 = (uint32_t)((at + (count - 1) * unit) / run);
-      const uint32_t slot0 = 2 * c0 + (at > run * c0 ? 1 : 0);
-      if (threadIdx.x == 0) last_flag = arrive_acq_rel(a.cnt + c0) == c1 - c0;
+      const uint32_t c0 = (uint32_t)(at / run.length), c1 = (uint32_t)((at + (count - 1) * unit) / run.length);
+      if (threadIdx.x == 0) sh.last_flag = arrive_acq_rel(a.cnt + c0) == c1 - c0;
       __syncthreads();
-      if (last_flag) {
-        const float *ml = a.part, *po = a.part + (size_t)2 * gridDim.x * kRows * 2;
-        auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : 2 * (c0 + k); };
-        const uint32_t n = c1 - c0 + 1;
-        for (uint32_t i = warp; i < rows; i += P::kThreads / 32) {  // a warp per row
-          float m = -INFINITY, l = 0.0f;
-          for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, __ldcg(ml + ((size_t)slot_of(k) * kRows + i) * 2));
-          m = warp_max(m);
-          float sum[D / 32];
-#pragma unroll
-          for (int d = 0; d < D / 32; ++d) sum[d] = 0.0f;
-          for (uint32_t k = 0; k < n; ++k) {
-            const size_t at_row = (size_t)slot_of(k) * kRows + i;
-            const float mk = __ldcg(ml + at_row * 2), f = mk == -INFINITY ? 0.0f : ex2(mk - m);
-            l = fmaf(__ldcg(ml + at_row * 2 + 1), f, l);
-#pragma unroll
-            for (int d = 0; d < D / 64; ++d) {
-              const float2 v = __ldcg(reinterpret_cast<const float2 *>(po + at_row * D + 64 * d + 2 * lane));
-              sum[2 * d] = fmaf(v.x, f, sum[2 * d]);
-              sum[2 * d + 1] = fmaf(v.y, f, sum[2 * d + 1]);
-            }
-          }
-          const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-          const uint32_t pr = row0 + i;
-          T *out = static_cast<T *>(a.out) + (size_t)(r.r0 + pr / a.gqa) * a.out_ld + (size_t)(head * a.gqa + pr % a.gqa) * D;
-#pragma unroll
-          for (int d = 0; d < D / 64; ++d) {
-            const float y[2] = {sum[2 * d] * inv, sum[2 * d + 1] * inv};
-            store_vec<T, 2>(out + 64 * d + 2 * lane, y);
-          }
-        }
-        if (threadIdx.x == 0) a.cnt[c0] = 0;
-      }
+      if (sh.last_flag) merge_parts<T, D>(a, where, 2 * c0 + (at > run.length * c0 ? 1 : 0), c0, c1 - c0 + 1);
     }
   }
+}
 
+template <typename T, int D>
+__global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (PromptShape<D, sizeof(T) == 4>::kCtas))
+    kv8_prompt_kernel(Kv8AttnArgs a) {
+  using P = PromptShape<D, sizeof(T) == 4>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ PromptShared<P::kTokens> sh;
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    const PromptBars<P::kS> bars(smem_u32(sh.bars));
+    mbar_init(bars.k_full, P::kWiden);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bars.v_full(i), P::kWiden);
+      mbar_init(bars.pv_done(i), 1);
+    }
+    for (int i = 0; i < P::kS; ++i) {
+      mbar_init(bars.s_done(i), 1);
+      mbar_init(bars.p_full(i), 4);
+    }
+    sh.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&sh.tmem_slot), P::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();
+  pdl_wait();
+  const Run run = find_run(a, (uint64_t)a.gqa * P::kTokens);
+  if (warp < 4)
+    prompt_role<T, D, kSoftmax>(a, run, smem_raw, sh);
+  else
+    prompt_role<T, D, kWidenKv>(a, run, smem_raw, sh);
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, P::kCols);
+    tmem_dealloc(sh.tmem_slot, P::kCols);
   }
 }
 
