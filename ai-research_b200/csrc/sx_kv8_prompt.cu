@@ -15,7 +15,8 @@
 //            (tile position 32 q + 8 (t % 8 / 2) + 4 half + 2 (t / 8) + t % 2) and of V's elements
 //            (tile row 32 p + 8 (d % 4) + f(d % 32 / 4), f a permutation of 8).  The softmax undoes
 //            the first in its masks and scales, the output the second: both are register indexes.
-// A thread of warp 0 issues the products (a warp of their own would cost the others registers).  What runs
+//   last     one thread issues the products.
+// What runs
 // seldom is out of line and loops stay loops: four warps a role do not hide the fetching of 100 KB of
 // instructions (unrolled throughout, the kernel spent 20 cycles an instruction).
 // Bound by shared memory (the tiles' stores and the products' reads) and exponentials (16 a cycle
@@ -43,7 +44,7 @@ struct PromptShape {
   static constexpr int kTokens = D == 256 && SPLIT ? 64 : 128;            // of a tile
   static constexpr int kS = kCtas == 2 ? 1 : 2;                           // S tiles
   static constexpr int kWiden = kCtas == 2 ? 4 : 8;                       // warps that widen
-  static constexpr int kThreads = (4 + kWiden) * 32;
+  static constexpr int kThreads = (4 + kWiden + 1) * 32;
   static constexpr int kTerms = SPLIT ? 2 : 1;
   static constexpr int kQTerm = (int)kRows * D * 2;
   static constexpr int kTile = kTokens * D * 2;
@@ -103,7 +104,7 @@ __device__ __noinline__ void rescale_row(uint32_t col, int cols, float f) {
   }
 }
 
-enum Role { kSoftmax, kWidenKv };
+enum Role { kSoftmax, kWidenKv, kProducts };
 
 // What the CTA's threads share.
 template <int TOKENS>
@@ -392,24 +393,6 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
     __syncthreads();
 
     if constexpr (ROLE == kSoftmax) {
-      // -- the products, for one thread
-      auto product_s = [&](uint32_t tile) {
-        wait(bars.k_full, tile);
-        tc_fence_after();
-        for (int w = 0; w < kTerms; ++w)
-          issue_ss(tmem + tile % kS * kTokens, q_tile + w * P::kQTerm, kRows * 128, k_tile, kTokens * 128,
-                   umma_idesc_f16(kRows, kTokens), D / 16, w > 0);
-        umma_commit(bars.s_done(tile));
-      };
-      auto product_o = [&](uint32_t tile, bool add) {
-        wait(bars.v_full(tile), tile / 2);
-        wait(bars.p_full(tile), tile / kS);
-        tc_fence_after();
-        for (int w = 0; w < kTerms; ++w)
-          issue_ts(tmem + P::kO, tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens), v_tile, D * 128,
-                   umma_idesc_f16(kRows, D), kTokens / 16, add || w > 0);
-        umma_commit(bars.pv_done(tile));
-      };
       // ================================================================ softmax: thread = row
       const uint32_t i = threadIdx.x, lanes = (uint32_t)(32 * warp) << 16;
       const float mul = sh.row_mul[i];
@@ -437,8 +420,6 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         __syncwarp();
         return is_mixed(t) || __any_sync(0xffffffffu, lane < kTileBlocks && f.y == 0.0f);
       };
-      if (threadIdx.x == 0) product_s(tiles);
-      __syncwarp();
       bool masked = set_blocks(t0, scales(t0, page_at(t0)));
       float2 next = scales(t0 + 1, page_at(t0 + 1));
       uint32_t next_page = page_at(t0 + 2);
@@ -530,21 +511,11 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
             for (int k = 0; k < 16; ++k) hi[k] = s[k];
             tmem_st16(low_col + 16 * q, hi);
           }
-          // with a second S tile the next product runs beside the rest of this softmax
-          if (kS == 2 && q == kTokens / 64 - 1) {
-            if (threadIdx.x == 0 && t + 1 < t1) product_s(tile + 1);
-            __syncwarp();
-          }
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.p_full(tile));
-        if (threadIdx.x == 0) {
-          product_o(tile, t > t0);
-          if (kS == 1 && t + 1 < t1) product_s(tile + 1);
-        }
-        __syncwarp();
         masked = set_blocks(t + 1, next);
         next = scales(t + 2, next_page);
         next_page = page_at(t + 3);
@@ -592,7 +563,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         __syncwarp();
       }
       tc_fence_before();
-    } else {
+    } else if constexpr (ROLE == kWidenKv) {
       const int g = lane >> 2, c = lane & 3;
       // ================================================================ widen K and V
       constexpr int kPairs = kTokens / 32, kShare = kWiden / kPairs;  // warps of a pair of blocks
@@ -698,6 +669,32 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         fetch(ahead, 0);
         now = ahead;
       }
+    } else if (lane == 0) {
+      // ================================================================ the products
+      auto product_s = [&](uint32_t tile) {
+        wait(bars.k_full, tile);
+        tc_fence_after();
+        for (int w = 0; w < kTerms; ++w)
+          issue_ss(tmem + tile % kS * kTokens, q_tile + w * P::kQTerm, kRows * 128, k_tile, kTokens * 128,
+                   umma_idesc_f16(kRows, kTokens), D / 16, w > 0);
+        umma_commit(bars.s_done(tile));
+      };
+      auto product_o = [&](uint32_t tile, bool add) {
+        wait(bars.v_full(tile), tile / 2);
+        wait(bars.p_full(tile), tile / kS);
+        tc_fence_after();
+        for (int w = 0; w < kTerms; ++w)
+          issue_ts(tmem + P::kO, tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens), v_tile, D * 128,
+                   umma_idesc_f16(kRows, D), kTokens / 16, add || w > 0);
+        umma_commit(bars.pv_done(tile));
+      };
+      if (kS == 2) product_s(tiles);
+      for (uint32_t j = 0; j < n_tiles; ++j) {
+        // with a second S tile the next product runs beside this tile's softmax
+        if (kS == 1) product_s(tiles + j);
+        else if (j + 1 < n_tiles) product_s(tiles + j + 1);
+        product_o(tiles + j, j > 0);
+      }
     }
     tiles += n_tiles;
     __syncthreads();  // Q, the tiles and O are free; the parts are written
@@ -713,7 +710,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
 
 template <typename T, int D>
 __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (PromptShape<D, sizeof(T) == 4>::kCtas))
-    kv8_prompt_kernel(Kv8AttnArgs a) {
+    kv8_prompt_kernel(const __grid_constant__ Kv8AttnArgs a) {
   using P = PromptShape<D, sizeof(T) == 4>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ PromptShared<P::kTokens> sh;
@@ -744,8 +741,10 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
   const Run run = find_run(a, (uint64_t)a.gqa * P::kTokens);
   if (warp < 4)
     prompt_role<T, D, kSoftmax>(a, run, smem_raw, sh);
-  else
+  else if (warp < 4 + P::kWiden)
     prompt_role<T, D, kWidenKv>(a, run, smem_raw, sh);
+  else
+    prompt_role<T, D, kProducts>(a, run, smem_raw, sh);
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
@@ -754,7 +753,7 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
   }
 }
 
-using PromptKernel = void (*)(Kv8AttnArgs);
+using PromptKernel = void (*)(const Kv8AttnArgs);
 struct PromptVariant {
   PromptKernel fn;
   uint32_t smem, ctas, threads;
