@@ -20,8 +20,9 @@
 // seldom is out of line and loops stay loops: four warps a role do not hide the fetching of 100 KB of
 // instructions (unrolled throughout, the kernel spent 20 cycles an instruction).
 // Bound by shared memory (the tiles' stores and the products' reads) and exponentials (16 a cycle
-// and SM, as many as a product of head size 128 takes cycles).  Up to head size 128 two CTAs share an
-// SM and fill each other's waits; above, two S tiles let the next product run beside the softmax.
+// and SM, as many as a product of head size 128 takes cycles).  Two S, K and V tiles let a tile's first
+// product, and the widening for it, run beside the softmax of the one before; up to head size 128 two
+// CTAs share an SM.
 //
 // Work is the line of sx_kv8_attn.cu with problems of their own length: row group k of a sequence
 // sees pos0 + 128 (k + 1) / G keys at most, so the line counts keys x G, whose sums are closed
@@ -41,14 +42,15 @@ constexpr float kMinScale = 1.17549435e-38f;  // a product with a masked -inf st
 template <int D, bool SPLIT>
 struct PromptShape {
   static constexpr int kCtas = D <= 128 && !(D == 128 && SPLIT) ? 2 : 1;  // per SM
-  static constexpr int kTokens = D == 256 && SPLIT ? 64 : 128;            // of a tile
-  static constexpr int kS = kCtas == 2 ? 1 : 2;                           // S tiles
+  static constexpr int kTokens = D == 128 && SPLIT ? 128 : 64;            // of a tile
+  static constexpr int kStages = D == 256 && SPLIT ? 1 : 2;               // K and V tiles
+  static constexpr int kS = 2;                                            // S tiles
   static constexpr int kWiden = kCtas == 2 ? 4 : 8;                       // warps that widen
   static constexpr int kThreads = (4 + kWiden + 1) * 32;
   static constexpr int kTerms = SPLIT ? 2 : 1;
   static constexpr int kQTerm = (int)kRows * D * 2;
   static constexpr int kTile = kTokens * D * 2;
-  static constexpr int kSmem = kTerms * kQTerm + 2 * kTile + 1024;        // + alignment
+  static constexpr int kSmem = kTerms * kQTerm + kStages * 2 * kTile + 1024;        // + alignment
   // tensor memory columns: S tiles (P over them), low terms of P, O
   static constexpr int kLow = kS * kTokens;
   static constexpr int kO = kLow + (SPLIT ? kS * kTokens / 2 : 0);
@@ -77,17 +79,16 @@ SX_DEV void st_shared16(uint32_t dst, const uint32_t (&v)[4]) {
 }
 
 // Waits are for a phase's parity, so a waiter must be sure of the phase before and ahead of the one
-// after.  The threads that widen and the one that issues go tile by tile; a softmax warp may be a tile
-// ahead of another when there are two S tiles, so what it waits for or arrives at has a barrier for
-// even and one for odd tiles: S of a tile done means that all of two tiles back is.
-template <int S>
+// after.  Every kind of event has a barrier for even and one for odd tiles: roles and softmax warps run
+// a tile ahead of one another, and S of a tile done means that all of two tiles back is.
 struct PromptBars {
-  uint32_t k_full;
-  SX_DEV explicit PromptBars(uint32_t at) : k_full(at) {}
-  SX_DEV uint32_t v_full(uint32_t t) const { return k_full + 8 + 8 * (t & 1); }
-  SX_DEV uint32_t pv_done(uint32_t t) const { return k_full + 24 + 8 * (t & 1); }
-  SX_DEV uint32_t s_done(uint32_t t) const { return k_full + 40 + 8 * (t % S); }
-  SX_DEV uint32_t p_full(uint32_t t) const { return k_full + 56 + 8 * (t % S); }
+  uint32_t at;
+  SX_DEV explicit PromptBars(uint32_t p) : at(p) {}
+  SX_DEV uint32_t k_full(uint32_t t) const { return at + 8 * (t & 1); }        // K, V in place
+  SX_DEV uint32_t v_full(uint32_t t) const { return at + 16 + 8 * (t & 1); }
+  SX_DEV uint32_t p_full(uint32_t t) const { return at + 32 + 8 * (t & 1); }   // P in place
+  SX_DEV uint32_t s_done(uint32_t t) const { return at + 48 + 8 * (t & 1); }   // products done
+  SX_DEV uint32_t pv_done(uint32_t t) const { return at + 64 + 8 * (t & 1); }
 };
 
 // This thread's row of `cols` f32 columns of tensor memory times f.  A whole warp calls it, seldom:
@@ -109,7 +110,7 @@ enum Role { kSoftmax, kWidenKv, kProducts };
 // What the CTA's threads share.
 template <int TOKENS>
 struct PromptShared {
-  uint64_t bars[9];
+  uint64_t bars[10];
   uint32_t tmem_slot, last_flag, abort_flag;
   uint32_t nan_mask[2][TOKENS / 32];
   float row_mul[kRows];
@@ -118,8 +119,8 @@ struct PromptShared {
 
 // A wait that runs out ends the CTA's waiting altogether: what follows runs through on whatever is
 // there, and the error word says so.
-__device__ __noinline__ void wait_or_abort(uint32_t b, uint32_t parity, volatile uint32_t *abort_flag, uint32_t *err) {
-  if (mbar_try_wait(b, parity & 1) || *abort_flag) return;
+__device__ __noinline__ void wait_longer(uint32_t b, uint32_t parity, volatile uint32_t *abort_flag, uint32_t *err) {
+  if (*abort_flag) return;
   if (!mbar_wait_bounded(b, parity & 1)) {
     *abort_flag = 1;
     raise_error(err, kDevWaitTimeout);
@@ -283,25 +284,28 @@ __device__ __noinline__ void merge_parts(const Kv8AttnArgs &a, const Where &w, u
   if (threadIdx.x == 0) a.cnt[c0] = 0;
 }
 
-// One product, issued by one thread: `steps` of 16 along K, A from shared memory (a_tile) or tensor
-// memory (a_col); 32 bytes of a swizzled row per step, a panel of 64 elements every four.
-__device__ __noinline__ void issue_ss(uint32_t d, uint32_t a_tile, uint32_t a_panel, uint32_t b_tile, uint32_t b_panel,
-                                      uint32_t idesc, int steps, bool add) {
-#pragma unroll 1
-  for (int k = 0; k < steps; k += 4) {
-    const uint64_t x = umma_desc_sw128(a_tile + k / 4 * a_panel), y = umma_desc_sw128(b_tile + k / 4 * b_panel);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) umma_f16(d, x + 2 * j, y + 2 * j, idesc, add || k + j > 0);
-  }
+// One product by one thread of the warp that calls it: STEPS of 16 along K, A from shared memory
+// (a_tile) or tensor memory (a_col); 32 bytes of a swizzled row per step, a panel of 64 elements every
+// four.  The whole warp comes here so that descriptors are the same in all lanes.
+SX_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
 }
-__device__ __noinline__ void issue_ts(uint32_t d, uint32_t a_col, uint32_t b_tile, uint32_t b_panel, uint32_t idesc,
-                                      int steps, bool add) {
-#pragma unroll 1
-  for (int k = 0; k < steps; k += 4) {
-    const uint64_t y = umma_desc_sw128(b_tile + k / 4 * b_panel);
+template <int STEPS>
+SX_DEV void issue_ss(uint32_t d, uint32_t a_tile, uint32_t a_panel, uint32_t b_tile, uint32_t b_panel, uint32_t idesc,
+                     bool add) {
+  const uint64_t x = umma_desc_sw128(a_tile), y = umma_desc_sw128(b_tile);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) umma_f16_ts(d, a_col + 8 * (k + j), y + 2 * j, idesc, add || k + j > 0);
-  }
+  for (int k = 0; k < STEPS; ++k)
+    umma_f16(d, x + k / 4 * (a_panel >> 4) + 2 * (k % 4), y + k / 4 * (b_panel >> 4) + 2 * (k % 4), idesc, add || k > 0);
+}
+template <int STEPS>
+SX_DEV void issue_ts(uint32_t d, uint32_t a_col, uint32_t b_tile, uint32_t b_panel, uint32_t idesc, bool add) {
+  const uint64_t y = umma_desc_sw128(b_tile);
+#pragma unroll
+  for (int k = 0; k < STEPS; ++k)
+    umma_f16_ts(d, a_col + 8 * k, y + k / 4 * (b_panel >> 4) + 2 * (k % 4), idesc, add || k > 0);
 }
 
 // One role's way through the CTA's run.
@@ -314,11 +318,14 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
   constexpr int kTileBlocks = kTokens / kKv8Block;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t q_tile = (smem_u32(smem_raw) + 1023) & ~1023u;  // [terms][D / 64][128 rows][128 B]
-  const uint32_t k_tile = q_tile + kTerms * P::kQTerm;           // [D / 64][tokens][128 B]
-  const uint32_t v_tile = k_tile + P::kTile;                     // [tokens / 64][D][128 B]
-  const PromptBars<kS> bars(smem_u32(sh.bars));
+  // K and V tiles: [stages][D / 64][tokens][128 B], [stages][tokens / 64][D][128 B]
+  auto k_tile = [&](uint32_t t) { return q_tile + kTerms * P::kQTerm + t % P::kStages * P::kTile; };
+  auto v_tile = [&](uint32_t t) { return q_tile + kTerms * P::kQTerm + (P::kStages + t % P::kStages) * P::kTile; };
+  const PromptBars bars(smem_u32(sh.bars));
   const uint32_t tmem = sh.tmem_slot;
-  auto wait = [&](uint32_t b, uint32_t parity) { wait_or_abort(b, parity, &sh.abort_flag, a.err); };
+  auto wait = [&](uint32_t b, uint32_t parity) {
+    if (!mbar_try_wait(b, parity & 1)) wait_longer(b, parity, &sh.abort_flag, a.err);
+  };
   const PageDiv div(a.c.page_tokens);
   const uint64_t unit = (uint64_t)a.gqa * kTokens;  // line length of a tile
   const uint64_t begin = run.begin, end = run.end;
@@ -428,7 +435,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         const uint32_t tile = tiles + (t - t0), s_col = tmem + lanes + tile % kS * kTokens;
         const uint32_t low_col = tmem + lanes + P::kLow + tile % kS * (kTokens / 2);
         const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
-        wait(bars.s_done(tile), tile / kS);
+        wait(bars.s_done(tile), tile / 2);
         const bool mixed = masked && is_mixed(t);
         if (mixed) wait(bars.v_full(tile), tile / 2);  // the NaN masks come with V
         __syncwarp();
@@ -568,7 +575,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
       // ================================================================ widen K and V
       constexpr int kPairs = kTokens / 32, kShare = kWiden / kPairs;  // warps of a pair of blocks
       constexpr int kMine = D / 32 / kShare;                          // pieces of a warp
-      static_assert(kMine >= 2, "pieces come in pairs");
+      const uint32_t swap = kMine >= 2 ? lane >> 2 & 1 : 0;
       const uint32_t ww = warp - 4, pair = ww % kPairs, p0 = ww / kPairs * kMine;
       struct Two {
         uint64_t r[2];
@@ -582,36 +589,39 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
       auto recs = [&](uint32_t t, const Pages &x) -> Two {
         return {{record(t * kTileBlocks + 2 * pair, x.p[0]), record(t * kTileBlocks + 2 * pair + 1, x.p[1])}};
       };
-      uint4 raw[2][kMine];  // K of a tile, then its V: asked for as soon as the registers are free
+      uint4 raw_k[2][kMine], raw_v[2][kMine];  // a tile ahead
       // K: lanes with odd g take the pieces of a pair in the other order, so that a store's eight
       // lanes meet all banks
-      auto fetch = [&](const Two &x, int which) {
+      auto fetch = [&](const Two &x, int which, uint4 (&raw)[2][kMine]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + (2 * x.r[h] + which) * (size_t)(16 * D);
 #pragma unroll
           for (int p = 0; p < kMine; ++p)
             raw[h][p] = x.r[h] == ~0ull ? make_uint4(0, 0, 0, 0)
-                                        : *reinterpret_cast<const uint4 *>(src + 512 * (p0 + (which ? p : p ^ (g & 1))) + 16 * lane);
+                                        : *reinterpret_cast<const uint4 *>(src + 512 * (p0 + (which ? p : p ^ swap)) + 16 * lane);
         }
       };
-      Two now = recs(t0, pages(t0));
-      fetch(now, 0);
+      {
+        const Two x = recs(t0, pages(t0));
+        fetch(x, 0, raw_k);
+        fetch(x, 1, raw_v);
+      }
       Pages next = pages(t0 + 1);
       for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t tile = tiles + (t - t0);
         const bool mixed = is_mixed(t);
         const Two ahead = recs(t + 1, next);
         next = pages(t + 2);
-        if (tile > 0) wait(bars.s_done(tile - 1), (tile - 1) / kS);  // the product before has read K
+        if (tile >= P::kStages) wait(bars.s_done(tile - P::kStages), (tile - P::kStages) / 2);  // K has been read
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int p = 0; p < kMine; ++p) {
-            const uint32_t piece = p0 + (p ^ (g & 1)), chunk = (piece & 1) * 4 + c;
+            const uint32_t piece = p0 + (p ^ swap), chunk = (piece & 1) * 4 + c;
             const uint32_t row = 32 * pair + 8 * (g / 2) + 4 * h + (g & 1);
-            const uint32_t base = k_tile + piece / 2 * (kTokens * 128);
-            const uint4 w = raw[h][p];
+            const uint32_t base = k_tile(tile) + piece / 2 * (kTokens * 128);
+            const uint4 w = raw_k[h][p];
             uint32_t x[4];
             e4m3x4_f16(w.x, x[0], x[1]);
             e4m3x4_f16(w.y, x[2], x[3]);
@@ -623,10 +633,10 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
           }
         fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars.k_full);
-        fetch(now, 1);
+        if (lane == 0) mbar_arrive(bars.k_full(tile));
+        fetch(ahead, 0, raw_k);
 
-        if (tile > 0) wait(bars.pv_done(tile - 1), (tile - 1) / 2);  // the product before has read V
+        if (tile >= P::kStages) wait(bars.pv_done(tile - P::kStages), (tile - P::kStages) / 2);  // V has been read
         if (mixed) {
           // A NaN would reach rows that do not see its token through 0 x NaN: it is taken out, and
           // its token marked for the rows that do.
@@ -637,7 +647,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
           for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int p = 0; p < kMine; ++p) {
-              uint32_t w[4] = {raw[h][p].x, raw[h][p].y, raw[h][p].z, raw[h][p].w};
+              uint32_t w[4] = {raw_v[h][p].x, raw_v[h][p].y, raw_v[h][p].z, raw_v[h][p].w};
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const uint32_t n = (((w[k] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
@@ -645,16 +655,16 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
                 // bytes are tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9 of block h
                 bits |= ((n & 1u) | ((n >> 7) & 2u) | ((n >> 8) & 0x100u) | ((n >> 15) & 0x200u)) << (2 * c + 16 * h);
               }
-              raw[h][p] = make_uint4(w[0], w[1], w[2], w[3]);
+              raw_v[h][p] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           if (bits) atomicOr(&sh.nan_mask[tile & 1][pair], bits);
         }
 #pragma unroll
         for (int p = 0; p < kMine; ++p) {
           const uint32_t fg = (g >> 1) | ((g & 1) << 2), chunk = (pair & 1) * 4 + c;
-          const uint32_t base = v_tile + pair / 2 * (D * 128) + (32 * (p0 + p) + fg) * 128 + ((chunk ^ fg) << 4);
-          const uint32_t wa[4] = {raw[0][p].x, raw[0][p].y, raw[0][p].z, raw[0][p].w};
-          const uint32_t wb[4] = {raw[1][p].x, raw[1][p].y, raw[1][p].z, raw[1][p].w};
+          const uint32_t base = v_tile(tile) + pair / 2 * (D * 128) + (32 * (p0 + p) + fg) * 128 + ((chunk ^ fg) << 4);
+          const uint32_t wa[4] = {raw_v[0][p].x, raw_v[0][p].y, raw_v[0][p].z, raw_v[0][p].w};
+          const uint32_t wb[4] = {raw_v[1][p].x, raw_v[1][p].y, raw_v[1][p].z, raw_v[1][p].w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // element 4 g + k: row 8 k + f(g) of the piece
             uint32_t x[4];
@@ -666,34 +676,40 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.v_full(tile));
-        fetch(ahead, 0);
-        now = ahead;
+        fetch(ahead, 1, raw_v);
       }
-    } else if (lane == 0) {
+    } else {
       // ================================================================ the products
       auto product_s = [&](uint32_t tile) {
-        wait(bars.k_full, tile);
+        wait(bars.k_full(tile), tile / 2);
+        __syncwarp();
         tc_fence_after();
-        for (int w = 0; w < kTerms; ++w)
-          issue_ss(tmem + tile % kS * kTokens, q_tile + w * P::kQTerm, kRows * 128, k_tile, kTokens * 128,
-                   umma_idesc_f16(kRows, kTokens), D / 16, w > 0);
-        umma_commit(bars.s_done(tile));
+        if (elect_one()) {
+#pragma unroll
+          for (int w = 0; w < kTerms; ++w)
+            issue_ss<D / 16>(tmem + tile % kS * kTokens, q_tile + w * P::kQTerm, kRows * 128, k_tile(tile), kTokens * 128,
+                             umma_idesc_f16(kRows, kTokens), w > 0);
+          umma_commit(bars.s_done(tile));
+        }
+        __syncwarp();
       };
-      auto product_o = [&](uint32_t tile, bool add) {
-        wait(bars.v_full(tile), tile / 2);
-        wait(bars.p_full(tile), tile / kS);
-        tc_fence_after();
-        for (int w = 0; w < kTerms; ++w)
-          issue_ts(tmem + P::kO, tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens), v_tile, D * 128,
-                   umma_idesc_f16(kRows, D), kTokens / 16, add || w > 0);
-        umma_commit(bars.pv_done(tile));
-      };
-      if (kS == 2) product_s(tiles);
+      product_s(tiles);
+#pragma unroll 1
       for (uint32_t j = 0; j < n_tiles; ++j) {
-        // with a second S tile the next product runs beside this tile's softmax
-        if (kS == 1) product_s(tiles + j);
-        else if (j + 1 < n_tiles) product_s(tiles + j + 1);
-        product_o(tiles + j, j > 0);
+        const uint32_t tile = tiles + j;
+        if (j + 1 < n_tiles) product_s(tile + 1);  // beside this tile's softmax
+        wait(bars.v_full(tile), tile / 2);
+        wait(bars.p_full(tile), tile / 2);
+        __syncwarp();
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int w = 0; w < kTerms; ++w)
+            issue_ts<kTokens / 16>(tmem + P::kO, tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens),
+                                   v_tile(tile), D * 128, umma_idesc_f16(kRows, D), j > 0 || w > 0);
+          umma_commit(bars.pv_done(tile));
+        }
+        __syncwarp();
       }
     }
     tiles += n_tiles;
@@ -716,15 +732,13 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
   __shared__ PromptShared<P::kTokens> sh;
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
-    const PromptBars<P::kS> bars(smem_u32(sh.bars));
-    mbar_init(bars.k_full, P::kWiden);
+    const PromptBars bars(smem_u32(sh.bars));
     for (int i = 0; i < 2; ++i) {
+      mbar_init(bars.k_full(i), P::kWiden);
       mbar_init(bars.v_full(i), P::kWiden);
-      mbar_init(bars.pv_done(i), 1);
-    }
-    for (int i = 0; i < P::kS; ++i) {
-      mbar_init(bars.s_done(i), 1);
       mbar_init(bars.p_full(i), 4);
+      mbar_init(bars.s_done(i), 1);
+      mbar_init(bars.pv_done(i), 1);
     }
     sh.abort_flag = 0;
     fence_mbar_init();
