@@ -114,7 +114,7 @@ struct PromptShared {
   uint32_t tmem_slot, last_flag, abort_flag;
   uint32_t nan_mask[2][TOKENS / 32];
   float row_mul[kRows];
-  float4 block[4][TOKENS / kKv8Block];  // softmax warps: {k scale, log2(v scale), 1 / v scale, there}
+  float4 block[2][TOKENS / kKv8Block];  // of a tile: {k scale, log2(v scale), 1 / v scale, there}
 };
 
 // A wait that runs out ends the CTA's waiting altogether: what follows runs through on whatever is
@@ -377,18 +377,6 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
     const uint32_t t1 = until < count ? (uint32_t)until : count;
     if (t0 >= t1) continue;  // no tile starts in the run
     const uint32_t n_tiles = t1 - t0;
-    const uint32_t *table = a.c.table + (size_t)(b - 1) * a.c.max_pages;
-    // Block s of the problem: its page (asked for a tile before it is used, so that nothing waits
-    // for the table) and its record pair, ~0 where there is nothing to read.
-    const uint32_t there = min(blocks, t1 * kTileBlocks);
-    auto page_of = [&](uint32_t s) { return s < there ? table[div.page(first + s)] : SX_NO_PAGE; };
-    auto record = [&](uint32_t s, uint32_t page) -> uint64_t {
-      if (page >= a.c.num_pages) {
-        if (s < there) raise_error(a.err, kDevBadSlot);
-        return ~0ull;
-      }
-      return ((uint64_t)page * a.c.num_kv + head) * div.per + (first + s - div.page(first + s) * div.per);
-    };
     // tiles whose keys every row sees
     const uint32_t all_hi = pos_lo, all_lo = a.window && pos_hi >= a.window ? pos_hi - a.window + 1 : 0;
     auto is_mixed = [&](uint32_t t) {
@@ -406,40 +394,19 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
       const uint32_t pos = pos0 + (row0 + min(i, rows - 1)) / a.gqa;
       const uint32_t see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_n = pos - see_lo;
       float ref = -INFINITY, l = 0.0f;
-      float4 *const block = sh.block[warp];
-      // Scales of a tile's blocks, block s in lane s: a tile ahead, their pages two; put where every
-      // thread of the warp reads them while the products run.
-      auto page_at = [&](uint32_t t) { return lane < kTileBlocks ? page_of(t * kTileBlocks + lane) : SX_NO_PAGE; };
-      auto scales = [&](uint32_t t, uint32_t page) -> float2 {
-        float2 f = make_float2(0.0f, 0.0f);  // v scale 0: a block that is not there
-        if (lane < kTileBlocks) {
-          const uint64_t rec = record(t * kTileBlocks + lane, page);
-          if (rec != ~0ull) f = *reinterpret_cast<const float2 *>(a.c.scale + 2 * rec);
-        }
-        return f;
-      };
-      // the tile's block table; true where some row does not see all of the tile or a block is missing
-      auto set_blocks = [&](uint32_t t, float2 f) {
-        if (lane < kTileBlocks) {
-          const int e = kv8_scale_exponent(f.y);
-          block[lane] = make_float4(f.x, (float)e, exp2_int(-e), f.y != 0.0f ? 1.0f : 0.0f);
-        }
-        __syncwarp();
-        return is_mixed(t) || __any_sync(0xffffffffu, lane < kTileBlocks && f.y == 0.0f);
-      };
-      bool masked = set_blocks(t0, scales(t0, page_at(t0)));
-      float2 next = scales(t0 + 1, page_at(t0 + 1));
-      uint32_t next_page = page_at(t0 + 2);
 #pragma unroll 1
       for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t tile = tiles + (t - t0), s_col = tmem + lanes + tile % kS * kTokens;
         const uint32_t low_col = tmem + lanes + P::kLow + tile % kS * (kTokens / 2);
         const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
+        const float4 *const block = sh.block[tile & 1];
+        wait(bars.v_full(tile), tile / 2);  // with V come its scales and NaN masks
         wait(bars.s_done(tile), tile / 2);
-        const bool mixed = masked && is_mixed(t);
-        if (mixed) wait(bars.v_full(tile), tile / 2);  // the NaN masks come with V
         __syncwarp();
         tc_fence_after();
+        // masked: some row does not see all of the tile, or a block of it is not there
+        const bool mixed = is_mixed(t);
+        const bool masked = mixed || __any_sync(0xffffffffu, lane < kTileBlocks && block[lane].w == 0.0f);
         // the tokens of chunk q that the row sees, a bit each
         auto visible = [&](int q) -> uint32_t {
           const uint32_t k0 = key0 + 32 * q, see_hi = see_lo + see_n + 1;  // seen: see_lo .. see_hi - 1
@@ -523,9 +490,6 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.p_full(tile));
-        masked = set_blocks(t + 1, next);
-        next = scales(t + 2, next_page);
-        next_page = page_at(t + 3);
       }
       // ---- the row's output, or its part
       wait(bars.pv_done(tiles + n_tiles - 1), (tiles + n_tiles - 1) / 2);
@@ -577,42 +541,61 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
       constexpr int kMine = D / 32 / kShare;                          // pieces of a warp
       const uint32_t swap = kMine >= 2 ? lane >> 2 & 1 : 0;
       const uint32_t ww = warp - 4, pair = ww % kPairs, p0 = ww / kPairs * kMine;
-      struct Two {
-        uint64_t r[2];
+      // Blocks from the run's first tile on, 32 at a time in the lanes: record pair (~0: nothing to
+      // read) and scales.
+      const uint32_t *table = a.c.table + (size_t)(b - 1) * a.c.max_pages;
+      const uint32_t there = min(blocks, t1 * kTileBlocks);
+      struct Entry {
+        uint64_t rec;
+        float ks, vs;
       };
-      struct Pages {
-        uint32_t p[2];
-      };
-      auto pages = [&](uint32_t t) -> Pages {
-        return {{page_of(t * kTileBlocks + 2 * pair), page_of(t * kTileBlocks + 2 * pair + 1)}};
-      };
-      auto recs = [&](uint32_t t, const Pages &x) -> Two {
-        return {{record(t * kTileBlocks + 2 * pair, x.p[0]), record(t * kTileBlocks + 2 * pair + 1, x.p[1])}};
+      auto entry = [&](uint32_t s) -> Entry {
+        Entry e{~0ull, 0.0f, 0.0f};
+        s += t0 * kTileBlocks;
+        if (s >= there) return e;
+        const uint32_t x = first + s, in = div.page(x), page = table[in];
+        if (page >= a.c.num_pages) {
+          raise_error(a.err, kDevBadSlot);
+          return e;
+        }
+        e.rec = ((uint64_t)page * a.c.num_kv + head) * div.per + (x - in * div.per);
+        const float2 f = *reinterpret_cast<const float2 *>(a.c.scale + 2 * e.rec);
+        e.ks = f.x;
+        e.vs = f.y;
+        return e;
       };
       uint4 raw_k[2][kMine], raw_v[2][kMine];  // a tile ahead
       // K: lanes with odd g take the pieces of a pair in the other order, so that a store's eight
       // lanes meet all banks
-      auto fetch = [&](const Two &x, int which, uint4 (&raw)[2][kMine]) {
+      auto fetch = [&](uint64_t rec, int h, int which, uint4 (&raw)[2][kMine]) {
+        const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + (2 * rec + which) * (size_t)(16 * D) + 512 * p0 + 16 * lane;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + (2 * x.r[h] + which) * (size_t)(16 * D);
-#pragma unroll
-          for (int p = 0; p < kMine; ++p)
-            raw[h][p] = x.r[h] == ~0ull ? make_uint4(0, 0, 0, 0)
-                                        : *reinterpret_cast<const uint4 *>(src + 512 * (p0 + (which ? p : p ^ swap)) + 16 * lane);
+        for (int p = 0; p < kMine; ++p) {
+          raw[h][p] = make_uint4(0, 0, 0, 0);
+          if (rec != ~0ull) raw[h][p] = *reinterpret_cast<const uint4 *>(src + 512 * (which ? p : p ^ swap));
         }
       };
-      {
-        const Two x = recs(t0, pages(t0));
-        fetch(x, 0, raw_k);
-        fetch(x, 1, raw_v);
+      Entry cur = entry(lane), nxt = entry(32 + lane);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t rec = __shfl_sync(0xffffffffu, cur.rec, 2 * pair + h);
+        fetch(rec, h, 0, raw_k);
+        fetch(rec, h, 1, raw_v);
       }
-      Pages next = pages(t0 + 1);
+#pragma unroll 1
       for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t tile = tiles + (t - t0);
         const bool mixed = is_mixed(t);
-        const Two ahead = recs(t + 1, next);
-        next = pages(t + 2);
+        // this tile's blocks are entries j .. of cur, the next one's of cur or nxt
+        const uint32_t j = (t - t0) * kTileBlocks % 32;
+        if (j == 0 && t > t0) {
+          cur = nxt;
+          nxt = entry((t - t0) * kTileBlocks + 32 + lane);
+        }
+        uint64_t ahead[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          ahead[h] = __shfl_sync(0xffffffffu, j + kTileBlocks < 32 ? cur.rec : nxt.rec, (j + kTileBlocks + 2 * pair + h) % 32);
         if (tile >= P::kStages) wait(bars.s_done(tile - P::kStages), (tile - P::kStages) / 2);  // K has been read
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -634,9 +617,14 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.k_full(tile));
-        fetch(ahead, 0, raw_k);
+        fetch(ahead[0], 0, 0, raw_k);
+        fetch(ahead[1], 1, 0, raw_k);
 
         if (tile >= P::kStages) wait(bars.pv_done(tile - P::kStages), (tile - P::kStages) / 2);  // V has been read
+        if (p0 == 0 && (uint32_t)lane - j - 2 * pair < 2) {
+          const int e = kv8_scale_exponent(cur.vs);
+          sh.block[tile & 1][lane - j] = make_float4(cur.ks, (float)e, exp2_int(-e), cur.rec != ~0ull ? 1.0f : 0.0f);
+        }
         if (mixed) {
           // A NaN would reach rows that do not see its token through 0 x NaN: it is taken out, and
           // its token marked for the rows that do.
@@ -676,7 +664,8 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.v_full(tile));
-        fetch(ahead, 1, raw_v);
+        fetch(ahead[0], 0, 1, raw_v);
+        fetch(ahead[1], 1, 1, raw_v);
       }
     } else {
       // ================================================================ the products
