@@ -15,10 +15,10 @@
 //            (tile position 32 q + 8 (t % 8 / 2) + 4 half + 2 (t / 8) + t % 2) and of V's elements
 //            (tile row 32 p + 8 (d % 4) + f(d % 32 / 4), f a permutation of 8).  The softmax undoes
 //            the first in its masks and scales, the output the second: both are register indexes.
-//   last     one thread issues the products.
-// What runs
-// seldom is out of line and loops stay loops: four warps a role do not hide the fetching of 100 KB of
-// instructions (unrolled throughout, the kernel spent 20 cycles an instruction).
+//   last     cuts the CTA's run into problems, one ahead, and issues the products.
+// Four warps a role hide little, so what runs seldom is out of line, loops stay loops (unrolled
+// throughout the kernel spent 20 cycles an instruction, fetching), and what describes a problem is in
+// shared memory instead of registers that would be spilled.
 // Bound by shared memory (the tiles' stores and the products' reads) and exponentials (16 a cycle
 // and SM, as many as a product of head size 128 takes cycles).  Two S, K and V tiles let a tile's first
 // product, and the widening for it, run beside the softmax of the one before; up to head size 128 two
@@ -58,6 +58,9 @@ struct PromptShape {
   static_assert(kO + D <= 512 && kCols * kCtas <= 512, "tensor memory");
 };
 
+// What starting and ending a problem costs, in tiles (10 000 cycles, and a tile takes 3000).
+constexpr uint32_t kPromptOver = 3;
+
 // Costs on the line: keys x G of a row group, at most `cap` with a window, plus `over`.
 struct GroupCost {
   uint64_t base, cap, over;  // pos0 * G; the most a group sees; what starting one costs
@@ -84,11 +87,10 @@ SX_DEV void st_shared16(uint32_t dst, const uint32_t (&v)[4]) {
 struct PromptBars {
   uint32_t at;
   SX_DEV explicit PromptBars(uint32_t p) : at(p) {}
-  SX_DEV uint32_t k_full(uint32_t t) const { return at + 8 * (t & 1); }        // K, V in place
-  SX_DEV uint32_t v_full(uint32_t t) const { return at + 16 + 8 * (t & 1); }
-  SX_DEV uint32_t p_full(uint32_t t) const { return at + 32 + 8 * (t & 1); }   // P in place
-  SX_DEV uint32_t s_done(uint32_t t) const { return at + 48 + 8 * (t & 1); }   // products done
-  SX_DEV uint32_t pv_done(uint32_t t) const { return at + 64 + 8 * (t & 1); }
+  SX_DEV uint32_t kv_full(uint32_t t) const { return at + 8 * (t & 1); }        // K and V in place
+  SX_DEV uint32_t p_full(uint32_t t) const { return at + 16 + 8 * (t & 1); }    // P in place
+  SX_DEV uint32_t s_done(uint32_t t) const { return at + 32 + 8 * (t & 1); }    // products done
+  SX_DEV uint32_t pv_done(uint32_t t) const { return at + 48 + 8 * (t & 1); }
 };
 
 // This thread's row of `cols` f32 columns of tensor memory times f.  A whole warp calls it, seldom:
@@ -107,13 +109,30 @@ __device__ __noinline__ void rescale_row(uint32_t col, int cols, float f) {
 
 enum Role { kSoftmax, kWidenKv, kProducts };
 
+// 128 packed rows of one sequence and kv head, and the tiles [t0, t1) of their keys that this CTA takes.
+struct Problem {
+  uint32_t more;                 // 0: the run is over
+  uint32_t r0, row0, rows, head; // first row of the sequence, first packed row, how many, kv head
+  uint32_t seq, pos0;            // the sequence and the position of its first new row
+  uint32_t first, blocks;        // first block that some row sees, how many
+  uint32_t t0, t1;
+  uint32_t all_lo, all_hi;       // keys that every row sees
+  uint32_t slot, slot0, c0, parts;  // this part's place; that of the first part, its CTA, how many
+  SX_DEV size_t row(const Kv8AttnArgs &a, uint32_t i) const { return r0 + (row0 + i) / a.gqa; }
+  SX_DEV uint32_t col(const Kv8AttnArgs &a, uint32_t i) const {
+    return (head * a.gqa + (row0 + i) % a.gqa) * a.c.head_dim;
+  }
+};
+
 // What the CTA's threads share.
 template <int TOKENS>
 struct PromptShared {
-  uint64_t bars[10];
+  uint64_t bars[8];
   uint32_t tmem_slot, last_flag, abort_flag;
   uint32_t nan_mask[2][TOKENS / 32];
+  Problem problem[2];
   float row_mul[kRows];
+  float2 row_merge[kRows];
   float4 block[2][TOKENS / kKv8Block];  // of a tile: {k scale, log2(v scale), 1 / v scale, there}
 };
 
@@ -137,151 +156,245 @@ struct PageDiv {
   }
 };
 
-SX_DEV GroupCost cost_of(const Kv8AttnArgs &a, const Kv8Rows &r, uint64_t unit) {
-  GroupCost k;
-  k.base = (uint64_t)(r.len - r.n) * a.gqa;
-  k.cap = a.window ? (uint64_t)a.window * a.gqa + kRows + 2 * a.gqa : ~0ull >> 1;
-  k.over = unit;
-  k.groups = (r.n * a.gqa + kRows - 1) / kRows;
-  return k;
-}
+// This CTA's run [begin, end) of the line, cut into problems: one warp, all lanes alike.
+struct Schedule {
+  uint64_t unit, begin, end, length, at, step;  // at: where the problem starts, step: its length
+  uint32_t b, left, head, group;                // next sequence; problems left of the one before
+  bool fresh;  // the first sequence: its first problems may lie before the run
+  Kv8Rows r;
+  GroupCost gc;
 
-// A CTA's run [begin, end) of the line, the sequence that holds begin and where that starts.
-struct Run {
-  uint64_t begin, end, length, at;
-  uint32_t b;
-};
-__device__ __noinline__ Run find_run(const Kv8AttnArgs &a, uint64_t unit) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto cost = [&](uint32_t i) -> uint64_t {
-    Kv8Rows r;
-    if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, i, &r)) {
-      if (blockIdx.x == 0 && warp == 0) raise_error(a.err, kDevBadParams);
+  SX_DEV GroupCost cost_of(const Kv8AttnArgs &a, const Kv8Rows &x) const {
+    GroupCost k;
+    k.base = (uint64_t)(x.len - x.n) * a.gqa;
+    k.cap = a.window ? (uint64_t)a.window * a.gqa + kRows + 2 * a.gqa : ~0ull >> 1;
+    k.over = kPromptOver * unit;
+    k.groups = (x.n * a.gqa + kRows - 1) / kRows;
+    return k;
+  }
+  SX_DEV uint64_t cost(const Kv8AttnArgs &a, uint32_t i) const {
+    Kv8Rows x;
+    if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, i, &x)) {
+      if (blockIdx.x == 0) raise_error(a.err, kDevBadParams);
       return 0;
     }
-    if (r.n == 0) return 0;
-    const GroupCost k = cost_of(a, r, unit);
+    if (x.n == 0) return 0;
+    const GroupCost k = cost_of(a, x);
     return k.before(k.groups) * a.c.num_kv;
-  };
-  const uint32_t per = (a.c.num_seqs + 31) / 32;
-  const uint32_t b0 = lane * per, b1 = min(a.c.num_seqs, b0 + per);
-  uint64_t mine = 0;
-  for (uint32_t i = b0; i < b1; ++i) mine += cost(i);
-  uint64_t incl = mine;
-#pragma unroll 1
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
   }
-  const uint64_t total = __shfl_sync(0xffffffffu, incl, 31);
-  Run x;
-  x.length = (total + gridDim.x - 1) / gridDim.x;
-  x.length = x.length > a.min_run * unit ? x.length : a.min_run * unit;
-  x.begin = x.length * blockIdx.x;
-  x.end = x.begin + x.length < total ? x.begin + x.length : total;
-  const uint32_t who = min(31, __popc(__ballot_sync(0xffffffffu, incl <= x.begin)));
-  uint64_t at = incl - mine;
-  uint32_t b = b0;
-  if (lane == (int)who && x.begin < x.end)
-    for (uint64_t n; (n = cost(b)) <= x.begin - at; at += n) ++b;
-  x.at = __shfl_sync(0xffffffffu, at, who);
-  x.b = __shfl_sync(0xffffffffu, b, who);
-  if (x.begin >= x.end) x.at = x.end;  // no run for this CTA
-  return x;
-}
-
-// A problem's place: first row of the sequence, first packed row, how many, kv head.
-struct Where {
-  uint32_t r0, row0, rows, head;
-  SX_DEV size_t row(const Kv8AttnArgs &a, uint32_t i) const { return r0 + (row0 + i) / a.gqa; }
-  SX_DEV uint32_t col(const Kv8AttnArgs &a, uint32_t i) const {
-    return (head * a.gqa + (row0 + i) % a.gqa) * a.c.head_dim;
+  __device__ __noinline__ void start(const Kv8AttnArgs &a, uint32_t tokens) {
+    const int lane = threadIdx.x & 31;
+    unit = (uint64_t)a.gqa * tokens;
+    const uint32_t per = (a.c.num_seqs + 31) / 32;
+    const uint32_t b0 = lane * per, b1 = min(a.c.num_seqs, b0 + per);
+    uint64_t mine = 0;
+    for (uint32_t i = b0; i < b1; ++i) mine += cost(a, i);
+    uint64_t incl = mine;
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const uint64_t total = __shfl_sync(0xffffffffu, incl, 31);
+    length = (total + gridDim.x - 1) / gridDim.x;
+    length = length > a.min_run * unit ? length : a.min_run * unit;
+    begin = length * blockIdx.x;
+    end = begin + length < total ? begin + length : total;
+    const uint32_t who = min(31, __popc(__ballot_sync(0xffffffffu, incl <= begin)));
+    at = incl - mine;
+    b = b0;
+    if (lane == (int)who && begin < end)
+      for (uint64_t n; (n = cost(a, b)) <= begin - at; at += n) ++b;
+    at = __shfl_sync(0xffffffffu, at, who);
+    b = __shfl_sync(0xffffffffu, b, who);
+    if (begin >= end) at = end;  // no run for this CTA
+    left = head = group = 0;
+    step = 0;
+    fresh = true;
+  }
+  // The next problem with a tile in the run.
+  __device__ __noinline__ void next(const Kv8AttnArgs &a, uint32_t tile_blocks, Problem &out) {
+    for (; at < end; at += step, --left) {
+      if (left != 0) {
+        if (++group == gc.groups) {
+          group = 0;
+          ++head;
+        }
+      }
+      while (left == 0 && b < a.c.num_seqs) {  // the next sequence with rows
+        const bool ok = kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r);
+        ++b;
+        if (!ok || r.n == 0) continue;
+        gc = cost_of(a, r);
+        left = gc.groups * a.c.num_kv;
+        head = group = 0;
+        if (fresh) {
+          fresh = false;
+          const uint64_t per_head = gc.before(gc.groups);
+          head = (uint32_t)((begin - at) / per_head);
+          at += head * per_head;
+          uint32_t lo = 0, hi = gc.groups - 1;  // the last group that starts at or before begin
+          while (lo < hi) {
+            const uint32_t mid = (lo + hi + 1) / 2;
+            if (gc.before(mid) <= begin - at) lo = mid; else hi = mid - 1;
+          }
+          group = lo;
+          at += gc.before(group);
+          left -= head * gc.groups + group;
+        }
+      }
+      if (left == 0) {  // the counts changed under the call
+        at = end;
+        break;
+      }
+      step = gc.of(group);
+      Problem p;
+      p.r0 = r.r0;
+      p.row0 = group * kRows;
+      p.rows = min(kRows, r.n * a.gqa - p.row0);
+      p.head = head;
+      p.seq = b - 1;
+      p.pos0 = r.len - r.n;
+      const uint32_t pos_lo = p.pos0 + p.row0 / a.gqa, pos_hi = p.pos0 + (p.row0 + p.rows - 1) / a.gqa;
+      p.first = (a.window && pos_lo >= a.window ? pos_lo - a.window + 1 : 0) / kKv8Block;
+      p.blocks = pos_hi / kKv8Block - p.first + 1;
+      p.all_hi = pos_lo;
+      p.all_lo = a.window && pos_hi >= a.window ? pos_hi - a.window + 1 : 0;
+      const uint32_t count = (p.blocks + tile_blocks - 1) / tile_blocks;
+      p.t0 = begin > at ? (uint32_t)((begin - at + unit - 1) / unit) : 0;
+      const uint64_t until = (end - at + unit - 1) / unit;
+      p.t1 = until < count ? (uint32_t)until : count;
+      if (p.t0 >= p.t1) continue;  // no tile starts in the run
+      // CTAs c0 .. c1 hold parts of this problem
+      p.c0 = (uint32_t)(at / length);
+      p.parts = (uint32_t)((at + (count - 1) * unit) / length) - p.c0 + 1;
+      p.slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
+      p.slot0 = 2 * p.c0 + (at > length * p.c0 ? 1 : 0);
+      p.more = 1;
+      if ((threadIdx.x & 31) == 0) out = p;
+      at += step;
+      --left;
+      return;
+    }
+    if ((threadIdx.x & 31) == 0) out.more = 0;
   }
 };
 
 // Q: power-of-two scaled f16 terms, K-major 128-byte swizzle, by all threads.
 template <typename T, int D>
-__device__ __noinline__ void put_q(const Kv8AttnArgs &a, const Where &w, uint32_t q_tile, float *row_mul) {
+__device__ __noinline__ void put_q(const Kv8AttnArgs &a, const Problem &w, uint32_t q_tile, float *row_mul) {
   constexpr bool kSplit = sizeof(T) == 4;
   using P = PromptShape<D, kSplit>;
-  constexpr int kLanes = D / 8, kPass = 32 / kLanes;  // lanes of a row, rows of a warp's pass
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t li = lane % kLanes;
-#pragma unroll 2
-  for (uint32_t i0 = warp * kPass; i0 < kRows; i0 += P::kThreads / 32 * kPass) {
-    const uint32_t i = i0 + lane / kLanes;
-    float x[8];
+  constexpr uint32_t kLanes = D / 8, kPass = 32 / kLanes;  // lanes of a row, rows of a warp's pass
+  constexpr uint32_t kStep = P::kThreads / 32 * kPass;
+  constexpr int kVec = 16 / (int)sizeof(T), kBatch = kSplit ? 3 : 5;  // rows on their way
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, li = lane % kLanes;
+  uint32_t i = warp * kPass + lane / kLanes;  // this lane's row; its token and q head
+  uint32_t t = (w.row0 + i) / a.gqa, g = w.row0 + i - t * a.gqa;
+  const uint32_t dt = kStep / a.gqa, dg = kStep - dt * a.gqa;
+#pragma unroll 1
+  for (uint32_t i0 = warp * kPass; i0 < kRows; i0 += kBatch * kStep) {
+    uint4 raw[kBatch][8 / kVec];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-    if (i < w.rows) {
-      const T *src = static_cast<const T *>(a.q) + w.row(a, i) * a.q_ld + w.col(a, i) + 8 * li;
-      constexpr int kVec = 16 / (int)sizeof(T);
+    for (int n = 0; n < kBatch; ++n) {
+      const T *src = static_cast<const T *>(a.q) + (size_t)(w.r0 + t) * a.q_ld + (w.head * a.gqa + g) * D + 8 * li;
 #pragma unroll
-      for (int k = 0; k < 8; k += kVec) {
-        float v[kVec];
-        load_vec<T, kVec>(src + k, v);
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) x[k + j] = v[j];
+      for (int k = 0; k < 8 / kVec; ++k) {
+        raw[n][k] = make_uint4(0, 0, 0, 0);
+        if (i + n * kStep < w.rows) raw[n][k] = *reinterpret_cast<const uint4 *>(src + kVec * k);
+      }
+      t += dt;
+      g += dg;
+      if (g >= a.gqa) {
+        g -= a.gqa;
+        ++t;
       }
     }
-    float m = 0.0f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[k]));
+    for (int n = 0; n < kBatch; ++n, i += kStep) {
+      if (i0 + n * kStep >= kRows) break;
+      float x[8], m = 0.0f;
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    int e = (int)(__float_as_uint(m) >> 23) - 127;
-    if (m == 0.0f || e == 128) e = 0;  // nothing to scale; an infinity stays one
-    e = min(max(e, -126), 126);
-    const float inv = a.scale < 0.0f ? -exp2_int(-e) : exp2_int(-e);
-    if (li == 0) row_mul[i] = fabsf(a.scale) * kLog2e * exp2_int(e);
-    uint32_t hi[4], low[4];
+      for (int k = 0; k < 8 / kVec; ++k) {
+        float v[kVec];
+        load_vec<T, kVec>(reinterpret_cast<const T *>(&raw[n][k]), v);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float v0 = x[2 * k] * inv, v1 = x[2 * k + 1] * inv;
-      hi[k] = pack_f16(v0, v1);
-      if constexpr (kSplit) low[k] = pack_f16_rest(v0, v1, hi[k]);
+        for (int j = 0; j < kVec; ++j) x[kVec * k + j] = v[j];
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(x[k]));
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      int e = (int)(__float_as_uint(m) >> 23) - 127;
+      if (m == 0.0f || e == 128) e = 0;  // nothing to scale; an infinity stays one
+      e = min(max(e, -126), 126);
+      const float inv = a.scale < 0.0f ? -exp2_int(-e) : exp2_int(-e);
+      if (li == 0) row_mul[i] = fabsf(a.scale) * kLog2e * exp2_int(e);
+      uint32_t hi[4], low[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float v0 = x[2 * k] * inv, v1 = x[2 * k + 1] * inv;
+        hi[k] = pack_f16(v0, v1);
+        if constexpr (kSplit) low[k] = pack_f16_rest(v0, v1, hi[k]);
+      }
+      const uint32_t dst = q_tile + li / 8 * (kRows * 128) + i * 128 + (((li % 8) ^ (i & 7)) << 4);
+      st_shared16(dst, hi);
+      if constexpr (kSplit) st_shared16(dst + P::kQTerm, low);
     }
-    const uint32_t dst = q_tile + li / 8 * (kRows * 128) + i * 128 + (((li % 8) ^ (i & 7)) << 4);
-    st_shared16(dst, hi);
-    if constexpr (kSplit) st_shared16(dst + P::kQTerm, low);
   }
   fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
 }
 
-// The last CTA to finish a part of a problem merges the n parts, a warp per row.
+// The last CTA to finish a part of a problem merges the parts: a thread per row for the maxima and the
+// sums, then all threads over the rows' values, four at a time with their loads in flight together.
 template <typename T, int D>
-__device__ __noinline__ void merge_parts(const Kv8AttnArgs &a, const Where &w, uint32_t slot0, uint32_t c0, uint32_t n) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const float *ml = a.part, *po = a.part + (size_t)2 * gridDim.x * kRows * 2;
-  auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : 2 * (c0 + k); };
-  for (uint32_t i = warp; i < w.rows; i += blockDim.x / 32) {
+__device__ __noinline__ void merge_parts(const Kv8AttnArgs &a, const Problem &w, float2 (&row)[kRows]) {
+  const float2 *ml = reinterpret_cast<const float2 *>(a.part);
+  const float *po = a.part + (size_t)2 * gridDim.x * kRows * 2;
+  const uint32_t n = w.parts, rows = w.rows;
+  auto slot_of = [&](uint32_t k) { return k == 0 ? w.slot0 : 2 * (w.c0 + k); };
+  if (threadIdx.x < rows) {
     float m = -INFINITY, l = 0.0f;
-    for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, __ldcg(ml + ((size_t)slot_of(k) * kRows + i) * 2));
-    m = warp_max(m);
-    float sum[D / 32];
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d) sum[d] = 0.0f;
-#pragma unroll 1
+#pragma unroll 4
     for (uint32_t k = 0; k < n; ++k) {
-      const size_t at_row = (size_t)slot_of(k) * kRows + i;
-      const float mk = __ldcg(ml + at_row * 2), f = mk == -INFINITY ? 0.0f : ex2(mk - m);
-      l = fmaf(__ldcg(ml + at_row * 2 + 1), f, l);
+      const float2 v = __ldcg(ml + (size_t)slot_of(k) * kRows + threadIdx.x);
+      const float top = fmaxf(m, v.x);  // a part that saw nothing has -inf and weight 0
+      l = l * (m == -INFINITY ? 0.0f : ex2(m - top)) + v.y * (v.x == -INFINITY ? 0.0f : ex2(v.x - top));
+      m = top;
+    }
+    row[threadIdx.x] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
+  }
+  __syncthreads();
+  constexpr uint32_t kCols = D / 4;
+#pragma unroll 1
+  for (uint32_t x0 = threadIdx.x; x0 < rows * kCols; x0 += 4 * blockDim.x) {
+    float4 sum[4];
 #pragma unroll
-      for (int d = 0; d < D / 64; ++d) {
-        const float2 v = __ldcg(reinterpret_cast<const float2 *>(po + at_row * D + 64 * d + 2 * lane));
-        sum[2 * d] = fmaf(v.x, f, sum[2 * d]);
-        sum[2 * d + 1] = fmaf(v.y, f, sum[2 * d + 1]);
+    for (int u = 0; u < 4; ++u) sum[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+    for (uint32_t k = 0; k < n; ++k) {
+      const size_t base = (size_t)slot_of(k) * kRows;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t x = min(x0 + u * blockDim.x, rows * kCols - 1), i = x / kCols;
+        const float mk = __ldcg(&ml[base + i].x);
+        const float4 v = __ldcg(reinterpret_cast<const float4 *>(po + (base + i) * D + x % kCols * 4));
+        const float f = mk == -INFINITY ? 0.0f : ex2(mk - row[i].x);
+        sum[u].x = fmaf(v.x, f, sum[u].x);
+        sum[u].y = fmaf(v.y, f, sum[u].y);
+        sum[u].z = fmaf(v.z, f, sum[u].z);
+        sum[u].w = fmaf(v.w, f, sum[u].w);
       }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T *out = static_cast<T *>(a.out) + w.row(a, i) * a.out_ld + w.col(a, i);
 #pragma unroll
-    for (int d = 0; d < D / 64; ++d) {
-      const float y[2] = {sum[2 * d] * inv, sum[2 * d + 1] * inv};
-      store_vec<T, 2>(out + 64 * d + 2 * lane, y);
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t x = x0 + u * blockDim.x, i = x / kCols;
+      if (x >= rows * kCols) break;
+      const float f = row[i].y, y[4] = {sum[u].x * f, sum[u].y * f, sum[u].z * f, sum[u].w * f};
+      store_vec<T, 4>(static_cast<T *>(a.out) + w.row(a, i) * a.out_ld + w.col(a, i) + x % kCols * 4, y);
     }
   }
-  if (threadIdx.x == 0) a.cnt[c0] = 0;
+  if (threadIdx.x == 0) a.cnt[w.c0] = 0;
 }
 
 // One product by one thread of the warp that calls it: STEPS of 16 along K, A from shared memory
@@ -308,90 +421,52 @@ SX_DEV void issue_ts(uint32_t d, uint32_t a_col, uint32_t b_tile, uint32_t b_pan
     umma_f16_ts(d, a_col + 8 * k, y + k / 4 * (b_panel >> 4) + 2 * (k % 4), idesc, add || k > 0);
 }
 
-// One role's way through the CTA's run.
+// One role's way through the CTA's problems.
 template <typename T, int D, Role ROLE>
-SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
-                        PromptShared<PromptShape<D, sizeof(T) == 4>::kTokens> &sh) {
+SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<PromptShape<D, sizeof(T) == 4>::kTokens> &sh) {
   constexpr bool kSplit = sizeof(T) == 4;
   using P = PromptShape<D, kSplit>;
-  constexpr int kTokens = P::kTokens, kS = P::kS, kWiden = P::kWiden, kTerms = P::kTerms;
+  constexpr int kTokens = P::kTokens, kS = P::kS, kWiden = P::kWiden, kTerms = P::kTerms, kStages = P::kStages;
   constexpr int kTileBlocks = kTokens / kKv8Block;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t q_tile = (smem_u32(smem_raw) + 1023) & ~1023u;  // [terms][D / 64][128 rows][128 B]
   // K and V tiles: [stages][D / 64][tokens][128 B], [stages][tokens / 64][D][128 B]
-  auto k_tile = [&](uint32_t t) { return q_tile + kTerms * P::kQTerm + t % P::kStages * P::kTile; };
-  auto v_tile = [&](uint32_t t) { return q_tile + kTerms * P::kQTerm + (P::kStages + t % P::kStages) * P::kTile; };
+  auto k_tile = [&](uint32_t t) { return q_tile + kTerms * P::kQTerm + t % kStages * P::kTile; };
+  auto v_tile = [&](uint32_t t) { return q_tile + kTerms * P::kQTerm + (kStages + t % kStages) * P::kTile; };
   const PromptBars bars(smem_u32(sh.bars));
   const uint32_t tmem = sh.tmem_slot;
   auto wait = [&](uint32_t b, uint32_t parity) {
     if (!mbar_try_wait(b, parity & 1)) wait_longer(b, parity, &sh.abort_flag, a.err);
   };
-  const PageDiv div(a.c.page_tokens);
-  const uint64_t unit = (uint64_t)a.gqa * kTokens;  // line length of a tile
-  const uint64_t begin = run.begin, end = run.end;
+  Schedule plan;
+  if constexpr (ROLE == kProducts) {
+    plan.start(a, kTokens);
+    plan.next(a, kTileBlocks, sh.problem[0]);
+  }
+  __syncthreads();
 
   uint32_t tiles = 0;  // tiles done, over all problems: every barrier's phase follows from it
-  Kv8Rows r;
-  GroupCost gc;
-  uint64_t at = run.at, length = 0;  // where the next problem starts, its length
-  uint32_t b = run.b, left = 0, head = 0, group = 0;
-  bool fresh = true;  // the first sequence: its first problems may lie before the run
-  for (; at < end; at += length, --left) {
-    if (left != 0) {
-      if (++group == gc.groups) {
-        group = 0;
-        ++head;
-      }
-    }
-    while (left == 0) {  // the next sequence with rows
-      const bool ok = kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r);
-      ++b;
-      if (!ok || r.n == 0) continue;
-      gc = cost_of(a, r, unit);
-      left = gc.groups * a.c.num_kv;
-      head = group = 0;
-      if (fresh) {
-        fresh = false;
-        const uint64_t per_head = gc.before(gc.groups);
-        head = (uint32_t)((begin - at) / per_head);
-        at += head * per_head;
-        uint32_t lo = 0, hi = gc.groups - 1;  // the last group that starts at or before begin
-        while (lo < hi) {
-          const uint32_t mid = (lo + hi + 1) / 2;
-          if (gc.before(mid) <= begin - at) lo = mid; else hi = mid - 1;
-        }
-        group = lo;
-        at += gc.before(group);
-        left -= head * gc.groups + group;
-      }
-    }
-    length = gc.of(group);
-    const uint32_t row0 = group * kRows, rows = min(kRows, r.n * a.gqa - row0);
-    const uint32_t pos0 = r.len - r.n;
-    const uint32_t pos_lo = pos0 + row0 / a.gqa, pos_hi = pos0 + (row0 + rows - 1) / a.gqa;
-    const uint32_t first = (a.window && pos_lo >= a.window ? pos_lo - a.window + 1 : 0) / kKv8Block;
-    const uint32_t blocks = pos_hi / kKv8Block - first + 1;
-    const uint32_t count = (blocks + kTileBlocks - 1) / kTileBlocks;
-    const uint32_t t0 = begin > at ? (uint32_t)((begin - at + unit - 1) / unit) : 0;
-    const uint64_t until = (end - at + unit - 1) / unit;
-    const uint32_t t1 = until < count ? (uint32_t)until : count;
-    if (t0 >= t1) continue;  // no tile starts in the run
-    const uint32_t n_tiles = t1 - t0;
-    // tiles whose keys every row sees
-    const uint32_t all_hi = pos_lo, all_lo = a.window && pos_hi >= a.window ? pos_hi - a.window + 1 : 0;
+#pragma unroll 1
+  for (uint32_t np = 0;; ++np) {
+    const Problem &pr = sh.problem[np & 1];
+    if (!pr.more) break;
+    const uint32_t t0 = pr.t0, t1 = pr.t1, n_tiles = t1 - t0, first = pr.first;
+    // tiles whose keys some row does not see
+    const uint32_t all_lo = pr.all_lo, all_hi = pr.all_hi;
     auto is_mixed = [&](uint32_t t) {
       const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
       return key0 < all_lo || key0 + kTokens - 1 > all_hi;
     };
-    const Where where{r.r0, row0, rows, head};
-    put_q<T, D>(a, where, q_tile, sh.row_mul);
-    __syncthreads();
+    if constexpr (ROLE != kWidenKv) {  // (the warps that widen ask for their first tiles before)
+      put_q<T, D>(a, pr, q_tile, sh.row_mul);
+      __syncthreads();
+    }
 
     if constexpr (ROLE == kSoftmax) {
       // ================================================================ softmax: thread = row
-      const uint32_t i = threadIdx.x, lanes = (uint32_t)(32 * warp) << 16;
+      const uint32_t i = threadIdx.x, lanes = (uint32_t)(32 * warp) << 16, rows = pr.rows;
       const float mul = sh.row_mul[i];
-      const uint32_t pos = pos0 + (row0 + min(i, rows - 1)) / a.gqa;
+      const uint32_t pos = pr.pos0 + (pr.row0 + min(i, rows - 1)) / a.gqa;
       const uint32_t see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_n = pos - see_lo;
       float ref = -INFINITY, l = 0.0f;
 #pragma unroll 1
@@ -400,8 +475,8 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         const uint32_t low_col = tmem + lanes + P::kLow + tile % kS * (kTokens / 2);
         const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
         const float4 *const block = sh.block[tile & 1];
-        wait(bars.v_full(tile), tile / 2);  // with V come its scales and NaN masks
         wait(bars.s_done(tile), tile / 2);
+        wait(bars.kv_full(tile), tile / 2);  // long true; says that the blocks' scales are there
         __syncwarp();
         tc_fence_after();
         // masked: some row does not see all of the tile, or a block of it is not there
@@ -495,16 +570,12 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
       wait(bars.pv_done(tiles + n_tiles - 1), (tiles + n_tiles - 1) / 2);
       __syncwarp();
       tc_fence_after();
-      const bool whole = t0 == 0 && t1 == count;
-      const uint32_t slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
-      float *const ml = a.part + ((size_t)slot * kRows + i) * 2;
-      float *const po = a.part + (size_t)2 * gridDim.x * kRows * 2 + ((size_t)slot * kRows + i) * D;
-      T *const out = static_cast<T *>(a.out) + where.row(a, i) * a.out_ld + where.col(a, i);
+      const bool whole = pr.parts == 1;
+      const size_t at = (size_t)pr.slot * kRows + i;
+      float *const po = a.part + (size_t)2 * gridDim.x * kRows * 2 + at * D;
+      T *const out = static_cast<T *>(a.out) + pr.row(a, i) * a.out_ld + pr.col(a, i);
       const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-      if (!whole && i < rows) {
-        ml[0] = ref;
-        ml[1] = l;
-      }
+      if (!whole && i < rows) reinterpret_cast<float2 *>(a.part)[at] = make_float2(ref, l);
 #pragma unroll 1
       for (int d = 0; d < D; d += 32) {
         uint32_t o[32];
@@ -535,16 +606,13 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
       }
       tc_fence_before();
     } else if constexpr (ROLE == kWidenKv) {
-      const int g = lane >> 2, c = lane & 3;
       // ================================================================ widen K and V
       constexpr int kPairs = kTokens / 32, kShare = kWiden / kPairs;  // warps of a pair of blocks
       constexpr int kMine = D / 32 / kShare;                          // pieces of a warp
-      const uint32_t swap = kMine >= 2 ? lane >> 2 & 1 : 0;
+      const uint32_t g = lane >> 2, c = lane & 3;
       const uint32_t ww = warp - 4, pair = ww % kPairs, p0 = ww / kPairs * kMine;
       // Blocks from the run's first tile on, 32 at a time in the lanes: record pair (~0: nothing to
       // read) and scales.
-      const uint32_t *table = a.c.table + (size_t)(b - 1) * a.c.max_pages;
-      const uint32_t there = min(blocks, t1 * kTileBlocks);
       struct Entry {
         uint64_t rec;
         float ks, vs;
@@ -552,40 +620,57 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
       auto entry = [&](uint32_t s) -> Entry {
         Entry e{~0ull, 0.0f, 0.0f};
         s += t0 * kTileBlocks;
-        if (s >= there) return e;
-        const uint32_t x = first + s, in = div.page(x), page = table[in];
+        if (s >= min(pr.blocks, t1 * kTileBlocks)) return e;
+        const PageDiv div(a.c.page_tokens);
+        const uint32_t x = first + s, in = div.page(x), page = a.c.table[(size_t)pr.seq * a.c.max_pages + in];
         if (page >= a.c.num_pages) {
           raise_error(a.err, kDevBadSlot);
           return e;
         }
-        e.rec = ((uint64_t)page * a.c.num_kv + head) * div.per + (x - in * div.per);
+        e.rec = ((uint64_t)page * a.c.num_kv + pr.head) * div.per + (x - in * div.per);
         const float2 f = *reinterpret_cast<const float2 *>(a.c.scale + 2 * e.rec);
         e.ks = f.x;
         e.vs = f.y;
         return e;
       };
-      uint4 raw_k[2][kMine], raw_v[2][kMine];  // a tile ahead
       // K: lanes with odd g take the pieces of a pair in the other order, so that a store's eight
-      // lanes meet all banks
-      auto fetch = [&](uint64_t rec, int h, int which, uint4 (&raw)[2][kMine]) {
-        const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + (2 * rec + which) * (size_t)(16 * D) + 512 * p0 + 16 * lane;
+      // lanes meet all banks.  A piece's store goes to the lane's offset with bits 5 and 6 turned by
+      // which of its tokens, block and piece it is.
+      const uint32_t swap = kMine >= 2 ? g & 1 : 0;
+      const uint32_t k_lane = p0 / 2 * (kTokens * 128) + (32 * pair + 8 * (g / 2) + (g & 1)) * 128 +
+                              ((kMine >= 2 ? swap : p0 & 1) << 6) + ((c ^ (g & 1)) << 4);
+      const uint32_t fg = (g >> 1) | ((g & 1) << 2);
+      const uint32_t v_lane = pair / 2 * (D * 128) + (32 * p0 + fg) * 128 + ((((pair & 1) * 4 + c) ^ fg) << 4);
+      uint4 raw_k[2][kMine], raw_v[2][kMine];  // a tile ahead
+      auto fetch_k = [&](uint64_t rec, int h) {
+        const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + rec * (32 * D) + 512 * p0 + 16 * lane;
+        const int turn = swap ? 512 : 0;
 #pragma unroll
         for (int p = 0; p < kMine; ++p) {
-          raw[h][p] = make_uint4(0, 0, 0, 0);
-          if (rec != ~0ull) raw[h][p] = *reinterpret_cast<const uint4 *>(src + 512 * (which ? p : p ^ swap));
+          raw_k[h][p] = make_uint4(0, 0, 0, 0);
+          if (rec != ~0ull) raw_k[h][p] = *reinterpret_cast<const uint4 *>(src + 512 * p + (p & 1 ? -turn : turn));
+        }
+      };
+      auto fetch_v = [&](uint64_t rec, int h) {
+        const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + rec * (32 * D) + 16 * D + 512 * p0 + 16 * lane;
+#pragma unroll
+        for (int p = 0; p < kMine; ++p) {
+          raw_v[h][p] = make_uint4(0, 0, 0, 0);
+          if (rec != ~0ull) raw_v[h][p] = *reinterpret_cast<const uint4 *>(src + 512 * p);
         }
       };
       Entry cur = entry(lane), nxt = entry(32 + lane);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint64_t rec = __shfl_sync(0xffffffffu, cur.rec, 2 * pair + h);
-        fetch(rec, h, 0, raw_k);
-        fetch(rec, h, 1, raw_v);
+        fetch_k(rec, h);
+        fetch_v(rec, h);
       }
+      put_q<T, D>(a, pr, q_tile, sh.row_mul);
+      __syncthreads();
 #pragma unroll 1
       for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t tile = tiles + (t - t0);
-        const bool mixed = is_mixed(t);
         // this tile's blocks are entries j .. of cur, the next one's of cur or nxt
         const uint32_t j = (t - t0) * kTileBlocks % 32;
         if (j == 0 && t > t0) {
@@ -596,36 +681,32 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           ahead[h] = __shfl_sync(0xffffffffu, j + kTileBlocks < 32 ? cur.rec : nxt.rec, (j + kTileBlocks + 2 * pair + h) % 32);
-        if (tile >= P::kStages) wait(bars.s_done(tile - P::kStages), (tile - P::kStages) / 2);  // K has been read
+        if (tile >= kStages) {  // the tiles' last contents have been read
+          wait(bars.s_done(tile - kStages), (tile - kStages) / 2);
+          wait(bars.pv_done(tile - kStages), (tile - kStages) / 2);
+        }
+        const uint32_t k_at = k_tile(tile);
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
           for (int p = 0; p < kMine; ++p) {
-            const uint32_t piece = p0 + (p ^ swap), chunk = (piece & 1) * 4 + c;
-            const uint32_t row = 32 * pair + 8 * (g / 2) + 4 * h + (g & 1);
-            const uint32_t base = k_tile(tile) + piece / 2 * (kTokens * 128);
-            const uint4 w = raw_k[h][p];
+            const uint32_t at = k_at + p / 2 * (kTokens * 128) + h * 512 + (k_lane ^ (((p & 1) ^ h) << 6));
+            const uint32_t at8 = k_at + p / 2 * (kTokens * 128) + h * 512 + 256 + (k_lane ^ (((p & 1) ^ h) << 6) ^ 32);
             uint32_t x[4];
-            e4m3x4_f16(w.x, x[0], x[1]);
-            e4m3x4_f16(w.y, x[2], x[3]);
-            st_shared16(base + row * 128 + ((chunk ^ (row & 7)) << 4), x);
-            e4m3x4_f16(w.z, x[0], x[1]);
-            e4m3x4_f16(w.w, x[2], x[3]);
-            const uint32_t row8 = row + 2;
-            st_shared16(base + row8 * 128 + ((chunk ^ (row8 & 7)) << 4), x);
+            e4m3x4_f16(raw_k[h][p].x, x[0], x[1]);
+            e4m3x4_f16(raw_k[h][p].y, x[2], x[3]);
+            st_shared16(at, x);
+            e4m3x4_f16(raw_k[h][p].z, x[0], x[1]);
+            e4m3x4_f16(raw_k[h][p].w, x[2], x[3]);
+            st_shared16(at8, x);
           }
-        fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bars.k_full(tile));
-        fetch(ahead[0], 0, 0, raw_k);
-        fetch(ahead[1], 1, 0, raw_k);
-
-        if (tile >= P::kStages) wait(bars.pv_done(tile - P::kStages), (tile - P::kStages) / 2);  // V has been read
+          fetch_k(ahead[h], h);
+        }
         if (p0 == 0 && (uint32_t)lane - j - 2 * pair < 2) {
           const int e = kv8_scale_exponent(cur.vs);
           sh.block[tile & 1][lane - j] = make_float4(cur.ks, (float)e, exp2_int(-e), cur.rec != ~0ull ? 1.0f : 0.0f);
         }
-        if (mixed) {
+        if (is_mixed(t)) {
           // A NaN would reach rows that do not see its token through 0 x NaN: it is taken out, and
           // its token marked for the rows that do.
           if (ww == 0 && lane < kPairs) sh.nan_mask[tile & 1][lane] = 0;
@@ -647,10 +728,9 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
             }
           if (bits) atomicOr(&sh.nan_mask[tile & 1][pair], bits);
         }
+        const uint32_t v_at = v_tile(tile) + v_lane;
 #pragma unroll
         for (int p = 0; p < kMine; ++p) {
-          const uint32_t fg = (g >> 1) | ((g & 1) << 2), chunk = (pair & 1) * 4 + c;
-          const uint32_t base = v_tile(tile) + pair / 2 * (D * 128) + (32 * (p0 + p) + fg) * 128 + ((chunk ^ fg) << 4);
           const uint32_t wa[4] = {raw_v[0][p].x, raw_v[0][p].y, raw_v[0][p].z, raw_v[0][p].w};
           const uint32_t wb[4] = {raw_v[1][p].x, raw_v[1][p].y, raw_v[1][p].z, raw_v[1][p].w};
 #pragma unroll
@@ -658,19 +738,19 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
             uint32_t x[4];
             e4m3x4_f16(wa[k], x[0], x[1]);
             e4m3x4_f16(wb[k], x[2], x[3]);
-            st_shared16(base + k * 8 * 128, x);
+            st_shared16(v_at + p * 4096 + k * 1024, x);
           }
         }
-        fence_proxy_async();
+        fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars.v_full(tile));
-        fetch(ahead[0], 0, 1, raw_v);
-        fetch(ahead[1], 1, 1, raw_v);
+        if (lane == 0) mbar_arrive(bars.kv_full(tile));
+        fetch_v(ahead[0], 0);
+        fetch_v(ahead[1], 1);
       }
     } else {
       // ================================================================ the products
       auto product_s = [&](uint32_t tile) {
-        wait(bars.k_full(tile), tile / 2);
+        wait(bars.kv_full(tile), tile / 2);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
@@ -683,11 +763,12 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
         __syncwarp();
       };
       product_s(tiles);
+      plan.next(a, kTileBlocks, sh.problem[(np + 1) & 1]);  // (read by all after the barrier below)
 #pragma unroll 1
       for (uint32_t j = 0; j < n_tiles; ++j) {
         const uint32_t tile = tiles + j;
-        if (j + 1 < n_tiles) product_s(tile + 1);  // beside this tile's softmax
-        wait(bars.v_full(tile), tile / 2);
+        // beside this tile's softmax, unless K and V have one tile only
+        if (kStages == 2 && j + 1 < n_tiles) product_s(tile + 1);
         wait(bars.p_full(tile), tile / 2);
         __syncwarp();
         tc_fence_after();
@@ -699,16 +780,15 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, const Run &run, uint8_t *smem_raw,
           umma_commit(bars.pv_done(tile));
         }
         __syncwarp();
+        if (kStages == 1 && j + 1 < n_tiles) product_s(tile + 1);
       }
     }
     tiles += n_tiles;
-    __syncthreads();  // Q, the tiles and O are free; the parts are written
-    if (!(t0 == 0 && t1 == count)) {
-      // CTAs c0 .. c1 hold parts of this problem; c0 counts them
-      const uint32_t c0 = (uint32_t)(at / run.length), c1 = (uint32_t)((at + (count - 1) * unit) / run.length);
-      if (threadIdx.x == 0) sh.last_flag = arrive_acq_rel(a.cnt + c0) == c1 - c0;
+    __syncthreads();  // Q, the tiles and O are free; the parts are written, and the next problem
+    if (pr.parts > 1) {
+      if (threadIdx.x == 0) sh.last_flag = arrive_acq_rel(a.cnt + pr.c0) == pr.parts - 1;
       __syncthreads();
-      if (sh.last_flag) merge_parts<T, D>(a, where, 2 * c0 + (at > run.length * c0 ? 1 : 0), c0, c1 - c0 + 1);
+      if (sh.last_flag) merge_parts<T, D>(a, pr, sh.row_merge);
     }
   }
 }
@@ -723,8 +803,7 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
   if (threadIdx.x == 0) {
     const PromptBars bars(smem_u32(sh.bars));
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bars.k_full(i), P::kWiden);
-      mbar_init(bars.v_full(i), P::kWiden);
+      mbar_init(bars.kv_full(i), P::kWiden);
       mbar_init(bars.p_full(i), 4);
       mbar_init(bars.s_done(i), 1);
       mbar_init(bars.pv_done(i), 1);
@@ -741,13 +820,12 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
   tc_fence_after();
   pdl_launch_dependents();
   pdl_wait();
-  const Run run = find_run(a, (uint64_t)a.gqa * P::kTokens);
   if (warp < 4)
-    prompt_role<T, D, kSoftmax>(a, run, smem_raw, sh);
+    prompt_role<T, D, kSoftmax>(a, smem_raw, sh);
   else if (warp < 4 + P::kWiden)
-    prompt_role<T, D, kWidenKv>(a, run, smem_raw, sh);
+    prompt_role<T, D, kWidenKv>(a, smem_raw, sh);
   else
-    prompt_role<T, D, kProducts>(a, run, smem_raw, sh);
+    prompt_role<T, D, kProducts>(a, smem_raw, sh);
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
@@ -790,7 +868,7 @@ size_t kv8_prompt_part_bytes(int num_sms) { return (size_t)2 * num_sms * kRows *
 
 cudaError_t launch_kv8_prompt(Kv8AttnArgs a, sx_dtype t, int num_sms, cudaStream_t s) {
   const PromptVariant v = prompt_variant(t, a.c.head_dim);
-  a.min_run = 4;  // tiles: shorter runs cost more to merge than they save
+  a.min_run = 6;  // tiles: shorter runs cost more to merge than they save
   return launch_chained(v.fn, dim3(num_sms * v.ctas), dim3(v.threads), v.smem, s, 1, a);
 }
 
