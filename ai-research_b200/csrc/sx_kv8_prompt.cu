@@ -36,17 +36,18 @@ namespace sx {
 namespace {
 
 constexpr uint32_t kRows = 128;      // packed rows of a problem
+constexpr int kSoft = 8;             // softmax warps
 constexpr float kPromptOffset = 6.0f, kSlack = 8.0f;
 constexpr float kMinScale = 1.17549435e-38f;  // a product with a masked -inf stays that
 
 template <int D, bool SPLIT>
 struct PromptShape {
   static constexpr int kCtas = D <= 128 && !(D == 128 && SPLIT) ? 2 : 1;  // per SM
-  static constexpr int kTokens = D == 128 && SPLIT ? 128 : 64;            // of a tile
+  static constexpr int kTokens = 64;                                      // of a tile
   static constexpr int kStages = D == 256 && SPLIT ? 1 : 2;               // K and V tiles
   static constexpr int kS = 2;                                            // S tiles
   static constexpr int kWiden = kCtas == 2 ? 4 : 8;                       // warps that widen
-  static constexpr int kThreads = (4 + kWiden + 1) * 32;
+  static constexpr int kThreads = (kSoft + kWiden + 1) * 32;
   static constexpr int kTerms = SPLIT ? 2 : 1;
   static constexpr int kQTerm = (int)kRows * D * 2;
   static constexpr int kTile = kTokens * D * 2;
@@ -87,11 +88,29 @@ SX_DEV void st_shared16(uint32_t dst, const uint32_t (&v)[4]) {
 struct PromptBars {
   uint32_t at;
   SX_DEV explicit PromptBars(uint32_t p) : at(p) {}
-  SX_DEV uint32_t kv_full(uint32_t t) const { return at + 8 * (t & 1); }        // K and V in place
-  SX_DEV uint32_t p_full(uint32_t t) const { return at + 16 + 8 * (t & 1); }    // P in place
-  SX_DEV uint32_t s_done(uint32_t t) const { return at + 32 + 8 * (t & 1); }    // products done
-  SX_DEV uint32_t pv_done(uint32_t t) const { return at + 48 + 8 * (t & 1); }
+  SX_DEV uint32_t k_full(uint32_t t) const { return at + 8 * (t & 1); }         // K in place
+  SX_DEV uint32_t v_full(uint32_t t) const { return at + 16 + 8 * (t & 1); }    // V in place
+  SX_DEV uint32_t p_full(uint32_t t) const { return at + 32 + 8 * (t & 1); }    // P in place
+  SX_DEV uint32_t s_done(uint32_t t) const { return at + 48 + 8 * (t & 1); }    // products done
+  SX_DEV uint32_t pv_done(uint32_t t) const { return at + 64 + 8 * (t & 1); }
 };
+
+constexpr uint32_t kNoRecord = ~0u;  // (2^32 record pairs of 2 KB are past any memory)
+
+// What stands in for a block that is not there (a branch around its loads would end in copies that
+// wait for them).
+__device__ uint4 g_no_block[32 * 256 / 16];
+
+// Whether any thread of the two warps that share rows says so: one barrier for both to meet at.
+SX_DEV bool pair_any(uint32_t bar, bool mine) {
+  uint32_t any;
+  asm volatile(
+      "{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.or.pred q, %2, 64, p;\nselp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(any)
+      : "r"((uint32_t)mine), "r"(bar)
+      : "memory");
+  return any;
+}
 
 // This thread's row of `cols` f32 columns of tensor memory times f.  A whole warp calls it, seldom:
 // out of line it stays out of the way of the loop's instructions.
@@ -127,13 +146,17 @@ struct Problem {
 // What the CTA's threads share.
 template <int TOKENS>
 struct PromptShared {
-  uint64_t bars[8];
+  uint64_t bars[10];
   uint32_t tmem_slot, last_flag, abort_flag;
   uint32_t nan_mask[2][TOKENS / 32];
   Problem problem[2];
   float row_mul[kRows];
   float2 row_merge[kRows];
-  float4 block[2][TOKENS / kKv8Block];  // of a tile: {k scale, log2(v scale), 1 / v scale, there}
+  float row_top[2][kRows], row_sum[2][kRows];  // of the two halves of a tile's keys
+  // The blocks of 32 tiles: of a widening warp the record pairs (kNoRecord: nothing to read); of a pair
+  // of blocks of a tile {k scale, log2(v scale), 1 / v scale, there}.
+  uint32_t record[8][64];
+  float4 facts[TOKENS / 32][64];
 };
 
 // A wait that runs out ends the CTA's waiting altogether: what follows runs through on whatever is
@@ -463,64 +486,55 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
     }
 
     if constexpr (ROLE == kSoftmax) {
-      // ================================================================ softmax: thread = row
-      const uint32_t i = threadIdx.x, lanes = (uint32_t)(32 * warp) << 16, rows = pr.rows;
+      // ================================================================ softmax: thread = half a row
+      const uint32_t i = threadIdx.x % kRows, half = threadIdx.x / kRows, rows = pr.rows;
+      const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16, pair_bar = 2 + (warp & 3);
       const float mul = sh.row_mul[i];
       const uint32_t pos = pr.pos0 + (pr.row0 + min(i, rows - 1)) / a.gqa;
-      const uint32_t see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_n = pos - see_lo;
+      const uint32_t see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_hi = pos + 1;
       float ref = -INFINITY, l = 0.0f;
 #pragma unroll 1
       for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t tile = tiles + (t - t0), s_col = tmem + lanes + tile % kS * kTokens;
-        const uint32_t low_col = tmem + lanes + P::kLow + tile % kS * (kTokens / 2);
-        const uint32_t key0 = (first + t * kTileBlocks) * kKv8Block;
-        const float4 *const block = sh.block[tile & 1];
+        const bool mixed = is_mixed(t);
         wait(bars.s_done(tile), tile / 2);
-        wait(bars.kv_full(tile), tile / 2);  // long true; says that the blocks' scales are there
+        if (mixed) wait(bars.v_full(tile), tile / 2);  // for the mask of its NaNs
         __syncwarp();
         tc_fence_after();
-        // masked: some row does not see all of the tile, or a block of it is not there
-        const bool mixed = is_mixed(t);
-        const bool masked = mixed || __any_sync(0xffffffffu, lane < kTileBlocks && block[lane].w == 0.0f);
-        // the tokens of chunk q that the row sees, a bit each
-        auto visible = [&](int q) -> uint32_t {
-          const uint32_t k0 = key0 + 32 * q, see_hi = see_lo + see_n + 1;  // seen: see_lo .. see_hi - 1
+        uint32_t s[32];
+        tmem_ld32(s_col + 32 * half, s);
+        // block 2 half holds columns k with k / 4 even, block 2 half + 1 the others
+        const float4 *const block = sh.facts[half] + 2 * (t - t0) % 64;
+        const bool gone0 = block[0].w == 0.0f, gone1 = block[1].w == 0.0f;
+        const float km[2] = {fmaxf(block[0].x * mul, kMinScale), fmaxf(block[1].x * mul, kMinScale)};
+        tmem_wait_ld(s);
+        if (mixed || gone0 || gone1) {  // some row does not see all of the tile, or a block is not there
+          const uint32_t k0 = (first + t * kTileBlocks) * kKv8Block + 32 * half;
           const uint32_t lo = see_lo > k0 ? see_lo - k0 : 0, hi = see_hi > k0 ? see_hi - k0 : 0;
-          uint32_t m = lo < 32 && hi > lo ? (hi < 32 ? (1u << hi) - 1 : ~0u) & (~0u << lo) : 0;
-          if (block[2 * q].w == 0.0f) m &= 0xFFFF0000u;
-          if (block[2 * q + 1].w == 0.0f) m &= 0x0000FFFFu;
-          return m;
-        };
-        // column k of a chunk is token 16 (k / 4 % 2) + 8 (k / 2 % 2) + 2 (k / 8) + k % 2
-        auto mask = [&](uint32_t (&s)[32], uint32_t vis) {
+          uint32_t vis = lo < 32 && hi > lo ? (hi < 32 ? (1u << hi) - 1 : ~0u) & (~0u << lo) : 0;
+          if (gone0) vis &= 0xFFFF0000u;
+          if (gone1) vis &= 0x0000FFFFu;
+          if (mixed && (sh.nan_mask[tile & 1][half] & vis)) l = NAN;
+          // column k is token 16 (k / 4 % 2) + 8 (k / 2 % 2) + 2 (k / 8) + k % 2
 #pragma unroll
           for (int k = 0; k < 32; ++k)
             if (!(vis & (1u << (16 * ((k >> 2) & 1) + 8 * ((k >> 1) & 1) + 2 * (k >> 3) + (k & 1))))) s[k] = 0xFF800000u;
-        };
-        // -- the largest x + log2(v scale)
-        float top = -INFINITY;
-#pragma unroll 1
-        for (int q = 0; q < kTokens / 32; ++q) {
-          uint32_t s[32];
-          tmem_ld32(s_col + 32 * q, s);
-          const float4 f0 = block[2 * q], f1 = block[2 * q + 1];
-          tmem_wait_ld(s);
-          if (masked) {
-            const uint32_t vis = visible(q);
-            if (mixed && (sh.nan_mask[tile & 1][q] & vis)) l = NAN;
-            mask(s, vis);
-          }
-          float m[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            m[(k >> 2) & 1] = fmaxf(fmaxf(m[(k >> 2) & 1], fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 1]))),
-                                    fmaxf(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])));
-          top = fmaxf(top, fmaxf(fmaf(m[0], fmaxf(f0.x * mul, kMinScale), f0.y),
-                                 fmaf(m[1], fmaxf(f1.x * mul, kMinScale), f1.y)));
         }
-        // -- one that outgrew the reference: rescale the row
-        const bool grow = top > ref + kSlack || (ref == -INFINITY && top > ref);
-        if (__any_sync(0xffffffffu, grow)) {
+        // -- the largest x + log2(v scale)
+        float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < 32; k += 4)
+          m[(k >> 2) & 1] = fmaxf(fmaxf(m[(k >> 2) & 1], fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 1]))),
+                                  fmaxf(__uint_as_float(s[k + 2]), __uint_as_float(s[k + 3])));
+        float top = fmaxf(fmaf(m[0], km[0], block[0].y), fmaf(m[1], km[1], block[1].y));
+        // -- one that outgrew the reference: rescale the row.  The vote also says that both halves of
+        // the row have been read, which P overwrites.
+        auto grows = [&] { return top > ref + kSlack || (ref == -INFINITY && top > ref); };
+        if (pair_any(pair_bar, grows())) {
+          sh.row_top[half][i] = top;
+          pair_any(pair_bar, false);
+          top = fmaxf(top, sh.row_top[half ^ 1][i]);
+          const bool grow = grows();
           const float f = !grow ? 1.0f : ref == -INFINITY ? 0.0f : ex2(ref - top);
           if (grow) ref = top;
           l *= f;
@@ -528,45 +542,39 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
             wait(bars.pv_done(tile - 1), (tile - 1) / 2);
             __syncwarp();
             tc_fence_after();
-            rescale_row(tmem + lanes + P::kO, D, f);
+            rescale_row(tmem + lanes + P::kO + half * (D / 2), D / 2, f);
             tmem_wait_st();
           }
         }
         const float shift = ref == -INFINITY ? 0.0f : ref - kPromptOffset;
-#pragma unroll 1
-        for (int q = 0; q < kTokens / 32; ++q) {
-          uint32_t s[32];
-          tmem_ld32(s_col + 32 * q, s);
-          const float4 f[2] = {block[2 * q], block[2 * q + 1]};
-          const float km[2] = {fmaxf(f[0].x * mul, kMinScale), fmaxf(f[1].x * mul, kMinScale)};
-          const float off[2] = {f[0].y - shift, f[1].y - shift};
-          float sum[2] = {0.0f, 0.0f};
-          uint32_t hi[16];
-          tmem_wait_ld(s);
-          if (masked) mask(s, visible(q));
+        const float off[2] = {block[0].y - shift, block[1].y - shift};
+        float sum[2] = {0.0f, 0.0f};
+        uint32_t hi[16];
 #pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const int h = (k >> 2) & 1;
-            const float p0 = ex2(fmaf(__uint_as_float(s[k]), km[h], off[h]));
-            const float p1 = ex2(fmaf(__uint_as_float(s[k + 1]), km[h], off[h]));
-            sum[h] += p0 + p1;
-            hi[k / 2] = pack_f16(p0, p1);
-            if constexpr (kSplit) s[k / 2] = pack_f16_rest(p0, p1, hi[k / 2]);
-          }
-          l = fmaf(sum[0], f[0].z, fmaf(sum[1], f[1].z, l));
-          tmem_st16(s_col + 16 * q, hi);  // P over S: columns that have been read
-          if constexpr (kSplit) {
-#pragma unroll
-            for (int k = 0; k < 16; ++k) hi[k] = s[k];
-            tmem_st16(low_col + 16 * q, hi);
-          }
+        for (int k = 0; k < 32; k += 2) {
+          const int h = (k >> 2) & 1;
+          const float p0 = ex2(fmaf(__uint_as_float(s[k]), km[h], off[h]));
+          const float p1 = ex2(fmaf(__uint_as_float(s[k + 1]), km[h], off[h]));
+          sum[h] += p0 + p1;
+          hi[k / 2] = pack_f16(p0, p1);
+          if constexpr (kSplit) s[k / 2] = pack_f16_rest(p0, p1, hi[k / 2]);
         }
+        tmem_st16(s_col + 16 * half, hi);  // P over S
+        if constexpr (kSplit) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) hi[k] = s[k];
+          tmem_st16(tmem + lanes + P::kLow + tile % kS * (kTokens / 2) + 16 * half, hi);
+        }
+        l = fmaf(sum[0], block[0].z, fmaf(sum[1], block[1].z, l));
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.p_full(tile));
       }
-      // ---- the row's output, or its part
+      // ---- the row's output, or its part: half of the columns a thread
+      sh.row_sum[half][i] = l;
+      pair_any(pair_bar, false);
+      l = sh.row_sum[0][i] + sh.row_sum[1][i];
       wait(bars.pv_done(tiles + n_tiles - 1), (tiles + n_tiles - 1) / 2);
       __syncwarp();
       tc_fence_after();
@@ -575,9 +583,9 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       float *const po = a.part + (size_t)2 * gridDim.x * kRows * 2 + at * D;
       T *const out = static_cast<T *>(a.out) + pr.row(a, i) * a.out_ld + pr.col(a, i);
       const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
-      if (!whole && i < rows) reinterpret_cast<float2 *>(a.part)[at] = make_float2(ref, l);
+      if (!whole && half == 0 && i < rows) reinterpret_cast<float2 *>(a.part)[at] = make_float2(ref, l);
 #pragma unroll 1
-      for (int d = 0; d < D; d += 32) {
+      for (int d = half * (D / 2); d < (int)(half + 1) * (D / 2); d += 32) {
         uint32_t o[32];
         tmem_ld32(tmem + lanes + P::kO + d, o);
         tmem_wait_ld(o);
@@ -610,28 +618,30 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       constexpr int kPairs = kTokens / 32, kShare = kWiden / kPairs;  // warps of a pair of blocks
       constexpr int kMine = D / 32 / kShare;                          // pieces of a warp
       const uint32_t g = lane >> 2, c = lane & 3;
-      const uint32_t ww = warp - 4, pair = ww % kPairs, p0 = ww / kPairs * kMine;
-      // Blocks from the run's first tile on, 32 at a time in the lanes: record pair (~0: nothing to
-      // read) and scales.
-      struct Entry {
-        uint64_t rec;
-        float ks, vs;
-      };
-      auto entry = [&](uint32_t s) -> Entry {
-        Entry e{~0ull, 0.0f, 0.0f};
-        s += t0 * kTileBlocks;
-        if (s >= min(pr.blocks, t1 * kTileBlocks)) return e;
-        const PageDiv div(a.c.page_tokens);
-        const uint32_t x = first + s, in = div.page(x), page = a.c.table[(size_t)pr.seq * a.c.max_pages + in];
-        if (page >= a.c.num_pages) {
-          raise_error(a.err, kDevBadSlot);
-          return e;
+      const uint32_t ww = warp - kSoft, pair = ww % kPairs, p0 = ww / kPairs * kMine;
+      // The warp's blocks of 16 tiles, one a lane, from the problem's tile t0 + `from` on.
+      uint32_t *const record = sh.record[ww];
+      auto look_up = [&](uint32_t from) {
+        const uint32_t n = from + lane / 2, s = (t0 + n) * kTileBlocks + 2 * pair + lane % 2;
+        const uint32_t at = 2 * n % 64 + lane % 2;
+        uint32_t rec = kNoRecord;
+        if (t0 + n < t1 && s < pr.blocks) {
+          const PageDiv div(a.c.page_tokens);
+          const uint32_t x = first + s, in = div.page(x), page = a.c.table[(size_t)pr.seq * a.c.max_pages + in];
+          if (page < a.c.num_pages)
+            rec = (page * a.c.num_kv + pr.head) * div.per + (x - in * div.per);
+          else
+            raise_error(a.err, kDevBadSlot);
         }
-        e.rec = ((uint64_t)page * a.c.num_kv + pr.head) * div.per + (x - in * div.per);
-        const float2 f = *reinterpret_cast<const float2 *>(a.c.scale + 2 * e.rec);
-        e.ks = f.x;
-        e.vs = f.y;
-        return e;
+        __syncwarp();
+        record[at] = rec;
+        if (p0 == 0) {
+          float2 f = make_float2(0.0f, 0.0f);
+          if (rec != kNoRecord) f = *reinterpret_cast<const float2 *>(a.c.scale + 2 * (size_t)rec);
+          const int e = kv8_scale_exponent(f.y);
+          sh.facts[pair][at] = make_float4(f.x, (float)e, exp2_int(-e), rec != kNoRecord ? 1.0f : 0.0f);
+        }
+        __syncwarp();
       };
       // K: lanes with odd g take the pieces of a pair in the other order, so that a store's eight
       // lanes meet all banks.  A piece's store goes to the lane's offset with bits 5 and 6 turned by
@@ -642,50 +652,37 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       const uint32_t fg = (g >> 1) | ((g & 1) << 2);
       const uint32_t v_lane = pair / 2 * (D * 128) + (32 * p0 + fg) * 128 + ((((pair & 1) * 4 + c) ^ fg) << 4);
       uint4 raw_k[2][kMine], raw_v[2][kMine];  // a tile ahead
-      auto fetch_k = [&](uint64_t rec, int h) {
-        const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + rec * (32 * D) + 512 * p0 + 16 * lane;
-        const int turn = swap ? 512 : 0;
+      const uint8_t *const data = static_cast<const uint8_t *>(a.c.data), *const no_block = reinterpret_cast<const uint8_t *>(g_no_block);
+      const uint32_t k_off = 512 * p0 + 16 * lane + (swap ? 512 : 0), v_off = 16 * D + 512 * p0 + 16 * lane;
+      const int k_turn = swap ? -512 : 512;
+      auto records = [&](uint32_t n) { return *reinterpret_cast<const uint2 *>(record + 2 * n % 64); };
+      auto fetch_k = [&](uint32_t rec, int h) {
+        const uint8_t *src = (rec != kNoRecord ? data + (size_t)rec * (32 * D) : no_block) + k_off;
 #pragma unroll
-        for (int p = 0; p < kMine; ++p) {
-          raw_k[h][p] = make_uint4(0, 0, 0, 0);
-          if (rec != ~0ull) raw_k[h][p] = *reinterpret_cast<const uint4 *>(src + 512 * p + (p & 1 ? -turn : turn));
-        }
+        for (int p = 0; p < kMine; ++p) raw_k[h][p] = *reinterpret_cast<const uint4 *>(src + p / 2 * 1024 + (p & 1) * k_turn);
       };
-      auto fetch_v = [&](uint64_t rec, int h) {
-        const uint8_t *src = static_cast<const uint8_t *>(a.c.data) + rec * (32 * D) + 16 * D + 512 * p0 + 16 * lane;
+      auto fetch_v = [&](uint32_t rec, int h) {
+        const uint8_t *src = (rec != kNoRecord ? data + (size_t)rec * (32 * D) : no_block) + v_off;
 #pragma unroll
-        for (int p = 0; p < kMine; ++p) {
-          raw_v[h][p] = make_uint4(0, 0, 0, 0);
-          if (rec != ~0ull) raw_v[h][p] = *reinterpret_cast<const uint4 *>(src + 512 * p);
-        }
+        for (int p = 0; p < kMine; ++p) raw_v[h][p] = *reinterpret_cast<const uint4 *>(src + 512 * p);
       };
-      Entry cur = entry(lane), nxt = entry(32 + lane);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint64_t rec = __shfl_sync(0xffffffffu, cur.rec, 2 * pair + h);
-        fetch_k(rec, h);
-        fetch_v(rec, h);
+      look_up(0);
+      {
+        const uint2 rec = records(0);
+        fetch_k(rec.x, 0);
+        fetch_k(rec.y, 1);
+        fetch_v(rec.x, 0);
+        fetch_v(rec.y, 1);
       }
       put_q<T, D>(a, pr, q_tile, sh.row_mul);
       __syncthreads();
+      // K of a tile, then V of the one before: K of the next tile waits for no softmax.
 #pragma unroll 1
-      for (uint32_t t = t0; t < t1; ++t) {
-        const uint32_t tile = tiles + (t - t0);
-        // this tile's blocks are entries j .. of cur, the next one's of cur or nxt
-        const uint32_t j = (t - t0) * kTileBlocks % 32;
-        if (j == 0 && t > t0) {
-          cur = nxt;
-          nxt = entry((t - t0) * kTileBlocks + 32 + lane);
-        }
-        uint64_t ahead[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          ahead[h] = __shfl_sync(0xffffffffu, j + kTileBlocks < 32 ? cur.rec : nxt.rec, (j + kTileBlocks + 2 * pair + h) % 32);
-        if (tile >= kStages) {  // the tiles' last contents have been read
-          wait(bars.s_done(tile - kStages), (tile - kStages) / 2);
-          wait(bars.pv_done(tile - kStages), (tile - kStages) / 2);
-        }
-        const uint32_t k_at = k_tile(tile);
+      for (uint32_t n = 0; n <= n_tiles; ++n) {
+        if (n % 16 == 8) look_up(n + 8);
+        if (n < n_tiles) {
+        const uint32_t tile = tiles + n, k_at = k_tile(tile);
+        if (tile >= kStages) wait(bars.s_done(tile - kStages), (tile - kStages) / 2);  // K has been read
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -700,13 +697,18 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
             e4m3x4_f16(raw_k[h][p].w, x[2], x[3]);
             st_shared16(at8, x);
           }
-          fetch_k(ahead[h], h);
         }
-        if (p0 == 0 && (uint32_t)lane - j - 2 * pair < 2) {
-          const int e = kv8_scale_exponent(cur.vs);
-          sh.block[tile & 1][lane - j] = make_float4(cur.ks, (float)e, exp2_int(-e), cur.rec != ~0ull ? 1.0f : 0.0f);
+        fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bars.k_full(tile));
+        const uint2 rec = records(n + 1);
+        fetch_k(rec.x, 0);
+        fetch_k(rec.y, 1);
         }
-        if (is_mixed(t)) {
+        if (n > 0) {
+        const uint32_t tile = tiles + n - 1;
+        if (tile >= kStages) wait(bars.pv_done(tile - kStages), (tile - kStages) / 2);  // V has been read
+        if (is_mixed(t0 + n - 1)) {
           // A NaN would reach rows that do not see its token through 0 x NaN: it is taken out, and
           // its token marked for the rows that do.
           if (ww == 0 && lane < kPairs) sh.nan_mask[tile & 1][lane] = 0;
@@ -743,17 +745,20 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         }
         fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
         __syncwarp();
-        if (lane == 0) mbar_arrive(bars.kv_full(tile));
-        fetch_v(ahead[0], 0);
-        fetch_v(ahead[1], 1);
+        if (lane == 0) mbar_arrive(bars.v_full(tile));
+        const uint2 rec = records(n);
+        fetch_v(rec.x, 0);
+        fetch_v(rec.y, 1);
+        }
       }
     } else {
       // ================================================================ the products
       auto product_s = [&](uint32_t tile) {
-        wait(bars.kv_full(tile), tile / 2);
+        wait(bars.k_full(tile), tile / 2);
         __syncwarp();
         tc_fence_after();
         if (elect_one()) {
+          mbar_arrive(bars.s_done(tile));  // (passes on what the widening warps wrote for the softmax)
 #pragma unroll
           for (int w = 0; w < kTerms; ++w)
             issue_ss<D / 16>(tmem + tile % kS * kTokens, q_tile + w * P::kQTerm, kRows * 128, k_tile(tile), kTokens * 128,
@@ -767,8 +772,8 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
 #pragma unroll 1
       for (uint32_t j = 0; j < n_tiles; ++j) {
         const uint32_t tile = tiles + j;
-        // beside this tile's softmax, unless K and V have one tile only
-        if (kStages == 2 && j + 1 < n_tiles) product_s(tile + 1);
+        if (j + 1 < n_tiles) product_s(tile + 1);  // beside this tile's softmax
+        wait(bars.v_full(tile), tile / 2);
         wait(bars.p_full(tile), tile / 2);
         __syncwarp();
         tc_fence_after();
@@ -780,7 +785,6 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
           umma_commit(bars.pv_done(tile));
         }
         __syncwarp();
-        if (kStages == 1 && j + 1 < n_tiles) product_s(tile + 1);
       }
     }
     tiles += n_tiles;
@@ -803,9 +807,10 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
   if (threadIdx.x == 0) {
     const PromptBars bars(smem_u32(sh.bars));
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bars.kv_full(i), P::kWiden);
-      mbar_init(bars.p_full(i), 4);
-      mbar_init(bars.s_done(i), 1);
+      mbar_init(bars.k_full(i), P::kWiden);
+      mbar_init(bars.v_full(i), P::kWiden);
+      mbar_init(bars.p_full(i), kSoft);
+      mbar_init(bars.s_done(i), 2);
       mbar_init(bars.pv_done(i), 1);
     }
     sh.abort_flag = 0;
@@ -820,9 +825,9 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
   tc_fence_after();
   pdl_launch_dependents();
   pdl_wait();
-  if (warp < 4)
+  if (warp < kSoft)
     prompt_role<T, D, kSoftmax>(a, smem_raw, sh);
-  else if (warp < 4 + P::kWiden)
+  else if (warp < kSoft + P::kWiden)
     prompt_role<T, D, kWidenKv>(a, smem_raw, sh);
   else
     prompt_role<T, D, kProducts>(a, smem_raw, sh);
