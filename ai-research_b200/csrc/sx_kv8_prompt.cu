@@ -7,22 +7,28 @@
 // tensor memory, P goes back there as f16 over S and is the second product's A operand.  e4m3 is
 // exact in f16, so K and V are widened on the way to shared memory; f32 rows split Q and P into two
 // f16 terms, with twice the products.  Warps:
-//   0 .. 3   softmax, a thread per row: the row of S from tensor memory, P back.  The maximum that the
-//            exponentials refer to moves only when it grows by 2^8; the row of O is then rescaled in
-//            tensor memory.
-//   4 ..     widen K and V.  A warp takes a pair of blocks (32 tokens): the cache's 16-byte pieces
+//   0 .. 7   softmax, two threads per row, each for half of a tile's 64 keys: their part of the row of S
+//            from tensor memory, P back.  The maximum that the exponentials refer to moves only when it
+//            grows by 2^8, which the two warps of a row vote on; the row of O is then rescaled in tensor
+//            memory.
+//   8 ..     widen K and V.  A warp takes a pair of blocks (32 tokens): the cache's 16-byte pieces
 //            become 16-byte stores of the 128-byte-swizzled tiles for a fitting order of the tokens
 //            (tile position 32 q + 8 (t % 8 / 2) + 4 half + 2 (t / 8) + t % 2) and of V's elements
 //            (tile row 32 p + 8 (d % 4) + f(d % 32 / 4), f a permutation of 8).  The softmax undoes
 //            the first in its masks and scales, the output the second: both are register indexes.
+//            K is a tile ahead of V, so that no widening waits for the softmax before it.
 //   last     cuts the CTA's run into problems, one ahead, and issues the products.
-// Four warps a role hide little, so what runs seldom is out of line, loops stay loops (unrolled
-// throughout the kernel spent 20 cycles an instruction, fetching), and what describes a problem is in
-// shared memory instead of registers that would be spilled.
-// Bound by shared memory (the tiles' stores and the products' reads) and exponentials (16 a cycle
-// and SM, as many as a product of head size 128 takes cycles).  Two S, K and V tiles let a tile's first
-// product, and the widening for it, run beside the softmax of the one before; up to head size 128 two
-// CTAs share an SM.
+// Two S, K and V tiles let a tile's first product, and the widening for it, run beside the softmax of the
+// one before; up to head size 128 two CTAs share an SM.
+//
+// What bounds it is the roles' own instructions: at head size 128 a CTA's tile takes 2300 cycles, of
+// which the tensor cores work 650.  Code size and spills count for as much as instructions (a kernel
+// unrolled throughout spent 20 cycles an instruction, fetching), so what runs seldom is out of line, loops
+// stay loops, and what describes a problem or a block is in shared memory.  Measured: 4 prompts of 4096
+// tokens behind 4096 (16 heads of 128, 8 kv heads, bf16) 528 us, 770 TFLOP/s; 4 of 2048 tokens with head
+// size 256 144 us.  Four softmax warps with whole rows took 684 us for the first, a shared barrier for K
+// and V 585.  A second look ahead for pages and scales, and Q brought by the roles that wait for it, were
+// slower (576 and 600 us): more code.
 //
 // Work is the line of sx_kv8_attn.cu with problems of their own length: row group k of a sequence
 // sees pos0 + 128 (k + 1) / G keys at most, so the line counts keys x G, whose sums are closed
@@ -51,7 +57,8 @@ struct PromptShape {
   static constexpr int kTerms = SPLIT ? 2 : 1;
   static constexpr int kQTerm = (int)kRows * D * 2;
   static constexpr int kTile = kTokens * D * 2;
-  static constexpr int kSmem = kTerms * kQTerm + kStages * 2 * kTile + 1024;        // + alignment
+  static constexpr int kStaged = kTokens * D;                             // a tile's V as it comes
+  static constexpr int kSmem = kTerms * kQTerm + kStages * 2 * kTile + kStaged + 1024;  // + alignment
   // tensor memory columns: S tiles (P over them), low terms of P, O
   static constexpr int kLow = kS * kTokens;
   static constexpr int kO = kLow + (SPLIT ? kS * kTokens / 2 : 0);
@@ -77,6 +84,12 @@ struct GroupCost {
   }
 };
 
+SX_DEV void ld_shared16(uint32_t src, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];\n"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(src)
+               : "memory");
+}
 SX_DEV void st_shared16(uint32_t dst, const uint32_t (&v)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
                : "memory");
@@ -144,7 +157,7 @@ struct Problem {
 };
 
 // What the CTA's threads share.
-template <int TOKENS>
+template <int TOKENS, int WIDEN>
 struct PromptShared {
   uint64_t bars[10];
   uint32_t tmem_slot, last_flag, abort_flag;
@@ -155,7 +168,7 @@ struct PromptShared {
   float row_top[2][kRows], row_sum[2][kRows];  // of the two halves of a tile's keys
   // The blocks of 32 tiles: of a widening warp the record pairs (kNoRecord: nothing to read); of a pair
   // of blocks of a tile {k scale, log2(v scale), 1 / v scale, there}.
-  uint32_t record[8][64];
+  uint32_t record[WIDEN][64];
   float4 facts[TOKENS / 32][64];
 };
 
@@ -446,7 +459,7 @@ SX_DEV void issue_ts(uint32_t d, uint32_t a_col, uint32_t b_tile, uint32_t b_pan
 
 // One role's way through the CTA's problems.
 template <typename T, int D, Role ROLE>
-SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<PromptShape<D, sizeof(T) == 4>::kTokens> &sh) {
+SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<PromptShape<D, sizeof(T) == 4>::kTokens, PromptShape<D, sizeof(T) == 4>::kWiden> &sh) {
   constexpr bool kSplit = sizeof(T) == 4;
   using P = PromptShape<D, kSplit>;
   constexpr int kTokens = P::kTokens, kS = P::kS, kWiden = P::kWiden, kTerms = P::kTerms, kStages = P::kStages;
@@ -651,7 +664,9 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
                               ((kMine >= 2 ? swap : p0 & 1) << 6) + ((c ^ (g & 1)) << 4);
       const uint32_t fg = (g >> 1) | ((g & 1) << 2);
       const uint32_t v_lane = pair / 2 * (D * 128) + (32 * p0 + fg) * 128 + ((((pair & 1) * 4 + c) ^ fg) << 4);
-      uint4 raw_k[2][kMine], raw_v[2][kMine];  // a tile ahead
+      // A tile ahead: K in registers, V in shared memory (each lane reads what it had fetched).
+      uint4 raw_k[2][kMine];
+      const uint32_t v_stage = q_tile + kTerms * P::kQTerm + 2 * kStages * P::kTile + ww * (2 * kMine * 512) + 16 * lane;
       const uint8_t *const data = static_cast<const uint8_t *>(a.c.data), *const no_block = reinterpret_cast<const uint8_t *>(g_no_block);
       const uint32_t k_off = 512 * p0 + 16 * lane + (swap ? 512 : 0), v_off = 16 * D + 512 * p0 + 16 * lane;
       const int k_turn = swap ? -512 : 512;
@@ -664,7 +679,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       auto fetch_v = [&](uint32_t rec, int h) {
         const uint8_t *src = (rec != kNoRecord ? data + (size_t)rec * (32 * D) : no_block) + v_off;
 #pragma unroll
-        for (int p = 0; p < kMine; ++p) raw_v[h][p] = *reinterpret_cast<const uint4 *>(src + 512 * p);
+        for (int p = 0; p < kMine; ++p) cp_async16(v_stage + (h * kMine + p) * 512, src + 512 * p);
       };
       look_up(0);
       {
@@ -673,6 +688,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         fetch_k(rec.y, 1);
         fetch_v(rec.x, 0);
         fetch_v(rec.y, 1);
+        cp_async_commit();
       }
       put_q<T, D>(a, pr, q_tile, sh.row_mul);
       __syncthreads();
@@ -708,47 +724,49 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         if (n > 0) {
         const uint32_t tile = tiles + n - 1;
         if (tile >= kStages) wait(bars.pv_done(tile - kStages), (tile - kStages) / 2);  // V has been read
-        if (is_mixed(t0 + n - 1)) {
-          // A NaN would reach rows that do not see its token through 0 x NaN: it is taken out, and
-          // its token marked for the rows that do.
+        const bool mixed = is_mixed(t0 + n - 1);
+        uint32_t nan_bits = 0;
+        if (mixed) {
           if (ww == 0 && lane < kPairs) sh.nan_mask[tile & 1][lane] = 0;
           asm volatile("bar.sync 1, %0;\n" ::"n"(kWiden * 32) : "memory");
-          uint32_t bits = 0;
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int p = 0; p < kMine; ++p) {
-              uint32_t w[4] = {raw_v[h][p].x, raw_v[h][p].y, raw_v[h][p].z, raw_v[h][p].w};
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint32_t n = (((w[k] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
-                w[k] &= ~(n * 0xFFu);
-                // bytes are tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9 of block h
-                bits |= ((n & 1u) | ((n >> 7) & 2u) | ((n >> 8) & 0x100u) | ((n >> 15) & 0x200u)) << (2 * c + 16 * h);
-              }
-              raw_v[h][p] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          if (bits) atomicOr(&sh.nan_mask[tile & 1][pair], bits);
         }
+        cp_async_wait<0>();
         const uint32_t v_at = v_tile(tile) + v_lane;
-#pragma unroll
+#pragma unroll 1
         for (int p = 0; p < kMine; ++p) {
-          const uint32_t wa[4] = {raw_v[0][p].x, raw_v[0][p].y, raw_v[0][p].z, raw_v[0][p].w};
-          const uint32_t wb[4] = {raw_v[1][p].x, raw_v[1][p].y, raw_v[1][p].z, raw_v[1][p].w};
+          uint32_t w[2][4];
+          ld_shared16(v_stage + p * 512, w[0]);
+          ld_shared16(v_stage + (kMine + p) * 512, w[1]);
+          if (mixed) {
+            // A NaN would reach rows that do not see its token through 0 x NaN: it is taken out, and
+            // its token marked for the rows that do.
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              uint32_t &x = w[k / 4][k % 4];
+              const uint32_t m = (((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+              x &= ~(m * 0xFFu);
+              // bytes are tokens 2 c, 2 c + 1, 2 c + 8, 2 c + 9 of a block
+              nan_bits |= ((m & 1u) | ((m >> 7) & 2u) | ((m >> 8) & 0x100u) | ((m >> 15) & 0x200u)) << (2 * c + k / 4 * 16);
+            }
+          }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {  // element 4 g + k: row 8 k + f(g) of the piece
             uint32_t x[4];
-            e4m3x4_f16(wa[k], x[0], x[1]);
-            e4m3x4_f16(wb[k], x[2], x[3]);
+            e4m3x4_f16(w[0][k], x[0], x[1]);
+            e4m3x4_f16(w[1][k], x[2], x[3]);
             st_shared16(v_at + p * 4096 + k * 1024, x);
           }
         }
+        if (nan_bits) atomicOr(&sh.nan_mask[tile & 1][pair], nan_bits);
         fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.v_full(tile));
-        const uint2 rec = records(n);
-        fetch_v(rec.x, 0);
-        fetch_v(rec.y, 1);
+        if (n < n_tiles) {
+          const uint2 rec = records(n);
+          fetch_v(rec.x, 0);
+          fetch_v(rec.y, 1);
+          cp_async_commit();
+        }
         }
       }
     } else {
@@ -802,7 +820,7 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
     kv8_prompt_kernel(const __grid_constant__ Kv8AttnArgs a) {
   using P = PromptShape<D, sizeof(T) == 4>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ PromptShared<P::kTokens> sh;
+  __shared__ PromptShared<P::kTokens, P::kWiden> sh;
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
     const PromptBars bars(smem_u32(sh.bars));
