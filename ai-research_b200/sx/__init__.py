@@ -103,19 +103,19 @@ class KV8(C.Structure):
                                   "head_dim")]
 
     def __init__(self, data, scale, table, page_tokens: int, num_kv: int, head_dim: int):
-        page = page_tokens * num_kv * 2 * head_dim
-        num_pages = data.numel() * data.element_size() // page
-        if num_pages * page != data.numel() * data.element_size():
+        num_pages, rest = divmod(data.nbytes, page_tokens * num_kv * 2 * head_dim)
+        if rest:
             raise ValueError("KV8: data does not hold whole pages")
-        if scale.numel() != num_pages * num_kv * (page_tokens // 16) * 2 or scale.element_size() != 4:
+        if scale.numel() != num_pages * num_kv * (page_tokens // 16) * 2 or scale.itemsize != 4:
             raise ValueError("KV8: scale must hold one f32 per record")
-        if table.dim() != 2 or table.element_size() != 4:
+        shape = table.shape
+        if len(shape) != 2 or table.itemsize != 4:
             raise ValueError("KV8: table must be [num_seqs][max_pages] 32-bit page ids")
         if not (data.is_contiguous() and scale.is_contiguous() and table.is_contiguous()):
             raise ValueError("KV8: data, scale and table must be contiguous")
         self._keep = (data, scale, table)
-        super().__init__(_ptr(data), _ptr(scale), _ptr(table), num_pages, page_tokens,
-                         table.shape[1], table.shape[0], num_kv, head_dim)
+        super().__init__(data.data_ptr(), scale.data_ptr(), table.data_ptr(), num_pages,
+                         page_tokens, shape[1], shape[0], num_kv, head_dim)
 
 
 class TpShard(C.Structure):
@@ -378,14 +378,14 @@ def check(status: int) -> None:
 
 def _ptr(a) -> int | None:
     """Device or host address of a numpy array, torch tensor or raw int."""
-    if a is None:
-        return None
-    if isinstance(a, int):
+    if a is None or isinstance(a, int):
         return a
+    try:
+        return a.data_ptr()  # (asked without looking: a small call's host time is its addresses)
+    except AttributeError:
+        pass
     if isinstance(a, np.ndarray):
         return a.ctypes.data
-    if hasattr(a, "data_ptr"):
-        return a.data_ptr()
     raise TypeError(f"cannot take the address of {type(a)}")
 
 
