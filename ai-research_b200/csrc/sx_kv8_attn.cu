@@ -32,7 +32,9 @@ namespace {
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr uint32_t kOverhead = 8;  // blocks a problem's start and end are worth
+constexpr uint32_t kMergeSteps = 3;  // steps (a block a warp) that a merge over CTAs is worth
 constexpr float kPOffset = 10.0f;
+constexpr uint32_t kMaxParts = 32, kPartGroup = 16;  // merged at once; of a first level
 
 SX_DEV uint32_t movmatrix_trans(uint32_t v) {
   uint32_t r;
@@ -71,11 +73,12 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
   constexpr bool kSplit = sizeof(T) == 4;
   using S = DecShape<D, NT, kSplit>;
   constexpr int kSub = S::kSub, kStages = S::kStages, kPieces = S::kPieces, kRows = S::kRows;
+  constexpr uint32_t kStep = kDecWarps * kSub;  // blocks that the CTA takes at a time
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t full_bar[kDecWarps * kStages];
   __shared__ uint32_t last_flag;
   __shared__ float row_mul[kRows], wm[kDecWarps][kRows], wl[kDecWarps][kRows];
-  __shared__ float fac[kDecWarps][kRows], row_inv[kRows];
+  __shared__ float fac[kMaxParts][kRows], row_inv[kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   uint8_t *const qf = smem + S::kArea;
   uint8_t *const ring = smem + warp * S::kRing;
@@ -93,6 +96,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
   auto problems_of = [&](const Kv8Rows &r) {
     return (r.n * a.gqa + kRows - 1) / kRows * a.c.num_kv;
   };
+  uint32_t longest = 0, problems = 0;  // of this lane's sequences
   auto cost = [&](uint32_t b) -> uint64_t {
     Kv8Rows r;
     if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r)) {
@@ -101,10 +105,13 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
     }
     uint32_t first, count;
     seen_blocks(r, a.window, &first, &count);
+    longest = max(longest, count);
+    problems += problems_of(r);
     return r.n ? (uint64_t)(count + kOverhead) * problems_of(r) : 0;
   };
   uint64_t begin, end, run, at;  // at: where the sequence of the next problem starts
   uint32_t b;
+  bool uncut;  // problems are not cut: each goes to the CTA in whose run it starts
   {
     const uint32_t per = (a.c.num_seqs + 31) / 32;
     const uint32_t b0 = lane * per, b1 = min(a.c.num_seqs, b0 + per);
@@ -118,7 +125,10 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
     }
     const uint64_t total = __shfl_sync(0xffffffffu, incl, 31);
     run = (total + gridDim.x - 1) / gridDim.x;
-    run = run > a.min_run ? run : a.min_run;
+    run = run > kStep ? run : kStep;
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    problems = __reduce_add_sync(0xffffffffu, problems);
+    uncut = longest <= kMergeSteps * kStep + (problems <= gridDim.x ? run : 0);
     begin = run * blockIdx.x;
     end = begin + run < total ? begin + run : total;
     if (begin >= end) return;
@@ -137,7 +147,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
   bool fresh = true;  // the first sequence: its first problems may lie before the run
   bool merged = false;
   for (; at < end; at += count + kOverhead, --left, ++problem) {
-    while (left == 0) {  // the next sequence with rows
+    while (left == 0 && b < a.c.num_seqs) {  // the next sequence with rows
       const bool ok = kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r);
       ++b;
       if (!ok || r.n == 0) continue;
@@ -151,8 +161,13 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
         fresh = false;
       }
     }
-    const uint32_t s0 = begin > at ? (uint32_t)(begin - at) : 0;
-    const uint32_t s1 = end - at < count ? (uint32_t)(end - at) : count;
+    if (left == 0) break;  // (the counts changed under the call)
+    uint32_t s0 = begin > at ? (uint32_t)(begin - at) : 0;
+    uint32_t s1 = end - at < count ? (uint32_t)(end - at) : count;
+    if (uncut) {
+      if (s0 != 0) continue;
+      s1 = count;
+    }
     if (s0 >= s1) continue;  // only its overhead lies in the run
     const uint32_t groups = (r.n * a.gqa + kRows - 1) / kRows;
     const uint32_t h = problem / groups, row0 = problem % groups * kRows;  // packed rows
@@ -553,49 +568,65 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
       }
     }
     if (!whole) {
-      // CTAs c0 .. c1 hold parts of this problem; c0 counts them
+      // CTAs c0 .. c1 hold parts of this problem, and the last to arrive merges them: up to 2 kPartGroup
+      // at once, more by groups first, each into its first part's place.  They count at words of CTAs
+      // inside the problem, which no other problem starts in.
       const uint32_t c0 = (uint32_t)(at / run), c1 = (uint32_t)((at + count - 1) / run);
       const uint32_t slot0 = 2 * c0 + (at > run * c0 ? 1 : 0);
-      __syncthreads();
-      if (threadIdx.x == 0) last_flag = arrive_acq_rel(a.cnt + c0) == c1 - c0;
-      __syncthreads();
-      if (last_flag) {
-        auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : 2 * (c0 + k); };
-        const uint32_t n = c1 - c0 + 1;
-        // one warp per row for the maxima, then all threads over the rows' elements
+      const uint32_t parts = c1 - c0 + 1, k0 = (blockIdx.x - c0) / kPartGroup * kPartGroup;
+      auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : 2 * (c0 + k); };
+      bool last = parts <= kMaxParts;  // the level is the last one
+      uint32_t from = last ? 0 : k0, each = 1, n = last ? parts : min(kPartGroup, parts - k0);
+      uint32_t *word = a.cnt + c0 + (from ? from - 1 : 0);
+#pragma unroll 1
+      for (;;) {
+        __syncthreads();
+        if (threadIdx.x == 0) last_flag = arrive_acq_rel(word) == n - 1;
+        __syncthreads();
+        if (!last_flag) break;
+        if (threadIdx.x == 0) *word = 0;
+        // a warp per row for the maxima, a lane per part; then all threads over the rows' elements
         for (uint32_t i = warp; i < rows; i += kDecWarps) {
-          float m = -INFINITY, l = 0.0f;
-          for (uint32_t k = lane; k < n; k += 32) m = fmaxf(m, __ldcg(part_ml + ((size_t)slot_of(k) * kRows + i) * 2));
-          m = warp_max(m);
-          for (uint32_t k = lane; k < n; k += 32) {
-            const float *ml = part_ml + ((size_t)slot_of(k) * kRows + i) * 2;
-            const float mk = __ldcg(ml);
-            l += __ldcg(ml + 1) * (mk == -INFINITY ? 0.0f : ex2(mk - m));
-          }
-          l = warp_sum(l);
+          float2 ml = make_float2(-INFINITY, 0.0f);
+          if ((uint32_t)lane < n)
+            ml = __ldcg(reinterpret_cast<const float2 *>(part_ml) + (size_t)slot_of(from + lane * each) * kRows + i);
+          const float m = warp_max(ml.x), f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m), l = warp_sum(ml.y * f);
+          fac[lane][i] = f;
           if (lane == 0) {
             wm[0][i] = m;
-            row_inv[i] = l == 0.0f ? 0.0f : 1.0f / l;
+            wl[0][i] = l;
           }
         }
         __syncthreads();
         for (uint32_t x = threadIdx.x; x < rows * (D / 4); x += kDecThreads) {
           const uint32_t i = x / (D / 4), d = x % (D / 4) * 4;
-          const float m = wm[0][i];
           float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll 8
           for (uint32_t k = 0; k < n; ++k) {
-            const float mk = __ldcg(part_ml + ((size_t)slot_of(k) * kRows + i) * 2);
-            const float f = mk == -INFINITY ? 0.0f : ex2(mk - m);
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_o + ((size_t)slot_of(k) * kRows + i) * D + d));
+            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_o + ((size_t)slot_of(from + k * each) * kRows + i) * D + d));
+            const float f = fac[k][i];
             sum.x = fmaf(v.x, f, sum.x);
             sum.y = fmaf(v.y, f, sum.y);
             sum.z = fmaf(v.z, f, sum.z);
             sum.w = fmaf(v.w, f, sum.w);
           }
-          const float inv = row_inv[i], y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
-          store_vec<T, 4>(out_row(i) + d, y);
+          if (last) {
+            const float l = wl[0][i], inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+            store_vec<T, 4>(out_row(i) + d, y);
+          } else {
+            *reinterpret_cast<float4 *>(part_o + ((size_t)slot_of(from) * kRows + i) * D + d) = sum;
+          }
         }
-        if (threadIdx.x == 0) a.cnt[c0] = 0;
+        if (last) break;
+        if (threadIdx.x < rows)
+          reinterpret_cast<float2 *>(part_ml)[(size_t)slot_of(from) * kRows + threadIdx.x] =
+              make_float2(wm[0][threadIdx.x], wl[0][threadIdx.x]);
+        last = true;
+        from = 0;
+        each = kPartGroup;
+        n = (parts + kPartGroup - 1) / kPartGroup;
+        word = a.cnt + c0 + 1;
       }
     }
     merged = true;
@@ -612,13 +643,13 @@ DecVariant variant() {
   using S = DecShape<D, NT, sizeof(T) == 4>;
   return {kv8_decode_kernel<T, D, NT>, (uint32_t)S::kSmem, (uint32_t)S::kCtas};
 }
-// Variant i (0, 1, 2: 8, 16, 32 packed rows) of a head size: the output of 8 NT rows takes
-// D NT / 4 registers per thread, of which there may be 128.
+// Variant i (0, 1: 8, 16 packed rows) of a head size: the output of 8 NT rows takes D NT / 4 registers
+// per thread, of which there may be 128.
 template <typename T>
 DecVariant variant(uint32_t d, uint32_t i) {
   switch (d) {
-    case 64: return i == 0 ? variant<T, 64, 1>() : i == 1 ? variant<T, 64, 2>() : variant<T, 64, 4>();
-    case 128: return i == 0 ? variant<T, 128, 1>() : i == 1 ? variant<T, 128, 2>() : variant<T, 128, 4>();
+    case 64: return i == 0 ? variant<T, 64, 1>() : variant<T, 64, 2>();
+    case 128: return i == 0 ? variant<T, 128, 1>() : variant<T, 128, 2>();
     case 256: return i == 0 ? variant<T, 256, 1>() : variant<T, 256, 2>();
     default: return variant<T, 512, 1>();
   }
@@ -627,18 +658,16 @@ DecVariant dec_variant(sx_dtype t, uint32_t d, uint32_t i) {
   return t == SX_F32 ? variant<float>(d, i) : variant<__nv_bfloat16>(d, i);
 }
 
-constexpr uint32_t kMinRun = 32;  // blocks, a problem's overhead included
-
 }  // namespace
 
-// Two parts per CTA of the decode kernel: up to 32 rows of {m, l}, and 4096 output values with one
+// Two parts per CTA of the decode kernel: up to 16 rows of {m, l}, and 4096 output values with one
 // CTA per SM, half as many with two.
-size_t kv8_part_bytes(int num_sms) { return (size_t)2 * num_sms * (2 * 32 * 2 + 4096) * sizeof(float); }
+size_t kv8_part_bytes(int num_sms) { return (size_t)2 * num_sms * (2 * 16 * 2 + 4096) * sizeof(float); }
 
 cudaError_t prepare_kv8_attn() {
   for (uint32_t d : {64u, 128u, 256u, 512u})
     for (sx_dtype t : {SX_F32, SX_BF16})
-      for (uint32_t i = 0; i < 3; ++i) {
+      for (uint32_t i = 0; i < 2; ++i) {
         const DecVariant v = dec_variant(t, d, i);
         const cudaError_t e = cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem);
         if (e != cudaSuccess) return e;
@@ -682,7 +711,6 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
   a.num_q = num_q;
   a.window = window;
   a.gqa = num_q / c->num_kv;
-  a.min_run = sx::kMinRun;
   a.scale = scale;
   a.part = e->kv8_part;
   a.cnt = e->kv8_cnt;
@@ -691,8 +719,8 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
   const uint64_t avg = (uint64_t)((tokens + c->num_seqs - 1) / c->num_seqs) * a.gqa;
   if (avg > 16 && c->head_dim <= 256)
     return sx_host_cuda_status(sx::launch_kv8_prompt(a, t, e->num_sms, e->stream), "kv8_attn launch");
-  const sx::DecVariant v = sx::dec_variant(t, c->head_dim, avg <= 8 ? 0 : avg <= 16 ? 1 : 2);
+  const sx::DecVariant v = sx::dec_variant(t, c->head_dim, avg <= 8 ? 0 : 1);
   return sx_host_cuda_status(
-      sx::launch_chained(v.fn, dim3(e->num_sms * v.ctas), dim3(sx::kDecThreads), v.smem, e->stream, 1, a),
+      sx::launch_chained(v.fn, dim3(std::min(e->num_sms * v.ctas, sx::kMaxParts * sx::kPartGroup)), dim3(sx::kDecThreads), v.smem, e->stream, 1, a),
       "kv8_attn launch");
 }
