@@ -67,18 +67,99 @@ struct DecShape {
   static constexpr int kSmem = kArea + kQ;
 };
 
+// What the CTA's threads share beside the rings.
+template <int ROWS>
+struct DecShared {
+  uint32_t last_flag;
+  float row_mul[ROWS], row_inv[ROWS];
+  float wm[kDecWarps][ROWS], wl[kDecWarps][ROWS];  // maxima and sums of the warps
+  float fac[kMaxParts][ROWS];                      // what a warp's, or a part's, output counts
+};
+
+// A problem that several CTAs hold parts of.
+struct Parts {
+  uint32_t c0, parts, slot0;  // its first CTA, how many, where the first part is
+  uint32_t r0, row0, rows, head;
+  SX_DEV uint32_t slot(uint32_t k) const { return k == 0 ? slot0 : 2 * (c0 + k); }
+};
+
+// Merges a problem's parts, by the last CTA to arrive: up to kMaxParts at once, more by groups first,
+// each into its first part's place.  They count at words of CTAs inside the problem, which no other
+// problem starts in.  Out of line: it would cost the loop registers.
+template <typename T, int D, int ROWS>
+__device__ __noinline__ void merge_parts(const Kv8AttnArgs &a, const Parts w, DecShared<ROWS> &sh) {
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float2 *const part_ml = reinterpret_cast<float2 *>(a.part);
+  float *const part_o = a.part + (size_t)2 * gridDim.x * ROWS * 2;
+  bool last = w.parts <= kMaxParts;  // the level is the last one
+  uint32_t from = last ? 0 : (blockIdx.x - w.c0) / kPartGroup * kPartGroup, each = 1;
+  uint32_t n = last ? w.parts : min(kPartGroup, w.parts - from);
+  uint32_t *word = a.cnt + w.c0 + (from ? from - 1 : 0);
+#pragma unroll 1
+  for (;;) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.last_flag = arrive_acq_rel(word) == n - 1;
+    __syncthreads();
+    if (!sh.last_flag) return;
+    if (threadIdx.x == 0) *word = 0;
+    // a warp per row for the maxima, a lane per part; then all threads over the rows' elements
+    for (uint32_t i = warp; i < w.rows; i += kDecWarps) {
+      float2 ml = make_float2(-INFINITY, 0.0f);
+      if (lane < n) ml = __ldcg(part_ml + (size_t)w.slot(from + lane * each) * ROWS + i);
+      const float m = warp_max(ml.x), f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m), l = warp_sum(ml.y * f);
+      sh.fac[lane][i] = f;
+      if (lane == 0) {
+        sh.wm[0][i] = m;
+        sh.wl[0][i] = l;
+      }
+    }
+    __syncthreads();
+    for (uint32_t x = threadIdx.x; x < w.rows * (D / 4); x += kDecThreads) {
+      const uint32_t i = x / (D / 4), d = x % (D / 4) * 4;
+      float4 sum = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+      for (uint32_t k = 0; k < n; ++k) {
+        const float4 v =
+            __ldcg(reinterpret_cast<const float4 *>(part_o + ((size_t)w.slot(from + k * each) * ROWS + i) * D + d));
+        const float f = sh.fac[k][i];
+        sum.x = fmaf(v.x, f, sum.x);
+        sum.y = fmaf(v.y, f, sum.y);
+        sum.z = fmaf(v.z, f, sum.z);
+        sum.w = fmaf(v.w, f, sum.w);
+      }
+      if (last) {
+        const float l = sh.wl[0][i], inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+        const uint32_t pr = w.row0 + i;
+        store_vec<T, 4>(static_cast<T *>(a.out) + (size_t)(w.r0 + pr / a.gqa) * a.out_ld +
+                            (size_t)(w.head * a.gqa + pr % a.gqa) * D + d, y);
+      } else {
+        *reinterpret_cast<float4 *>(part_o + ((size_t)w.slot(from) * ROWS + i) * D + d) = sum;
+      }
+    }
+    if (last) return;
+    if (threadIdx.x < w.rows)
+      part_ml[(size_t)w.slot(from) * ROWS + threadIdx.x] = make_float2(sh.wm[0][threadIdx.x], sh.wl[0][threadIdx.x]);
+    last = true;
+    from = 0;
+    each = kPartGroup;
+    n = (w.parts + kPartGroup - 1) / kPartGroup;
+    word = a.cnt + w.c0 + 1;
+  }
+}
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>::kCtas))
-    kv8_decode_kernel(Kv8AttnArgs a) {
+    kv8_decode_kernel(const __grid_constant__ Kv8AttnArgs a) {
   constexpr bool kSplit = sizeof(T) == 4;
   using S = DecShape<D, NT, kSplit>;
   constexpr int kSub = S::kSub, kStages = S::kStages, kPieces = S::kPieces, kRows = S::kRows;
   constexpr uint32_t kStep = kDecWarps * kSub;  // blocks that the CTA takes at a time
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t full_bar[kDecWarps * kStages];
-  __shared__ uint32_t last_flag;
-  __shared__ float row_mul[kRows], wm[kDecWarps][kRows], wl[kDecWarps][kRows];
-  __shared__ float fac[kMaxParts][kRows], row_inv[kRows];
+  __shared__ DecShared<kRows> sh;
+  float (&row_mul)[kRows] = sh.row_mul, (&row_inv)[kRows] = sh.row_inv;
+  float (&wm)[kDecWarps][kRows] = sh.wm, (&wl)[kDecWarps][kRows] = sh.wl, (&fac)[kMaxParts][kRows] = sh.fac;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   uint8_t *const qf = smem + S::kArea;
   uint8_t *const ring = smem + warp * S::kRing;
@@ -568,72 +649,14 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
       }
     }
     if (!whole) {
-      // CTAs c0 .. c1 hold parts of this problem, and the last to arrive merges them: up to 2 kPartGroup
-      // at once, more by groups first, each into its first part's place.  They count at words of CTAs
-      // inside the problem, which no other problem starts in.
       const uint32_t c0 = (uint32_t)(at / run), c1 = (uint32_t)((at + count - 1) / run);
-      const uint32_t slot0 = 2 * c0 + (at > run * c0 ? 1 : 0);
-      const uint32_t parts = c1 - c0 + 1, k0 = (blockIdx.x - c0) / kPartGroup * kPartGroup;
-      auto slot_of = [&](uint32_t k) { return k == 0 ? slot0 : 2 * (c0 + k); };
-      bool last = parts <= kMaxParts;  // the level is the last one
-      uint32_t from = last ? 0 : k0, each = 1, n = last ? parts : min(kPartGroup, parts - k0);
-      uint32_t *word = a.cnt + c0 + (from ? from - 1 : 0);
-#pragma unroll 1
-      for (;;) {
-        __syncthreads();
-        if (threadIdx.x == 0) last_flag = arrive_acq_rel(word) == n - 1;
-        __syncthreads();
-        if (!last_flag) break;
-        if (threadIdx.x == 0) *word = 0;
-        // a warp per row for the maxima, a lane per part; then all threads over the rows' elements
-        for (uint32_t i = warp; i < rows; i += kDecWarps) {
-          float2 ml = make_float2(-INFINITY, 0.0f);
-          if ((uint32_t)lane < n)
-            ml = __ldcg(reinterpret_cast<const float2 *>(part_ml) + (size_t)slot_of(from + lane * each) * kRows + i);
-          const float m = warp_max(ml.x), f = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m), l = warp_sum(ml.y * f);
-          fac[lane][i] = f;
-          if (lane == 0) {
-            wm[0][i] = m;
-            wl[0][i] = l;
-          }
-        }
-        __syncthreads();
-        for (uint32_t x = threadIdx.x; x < rows * (D / 4); x += kDecThreads) {
-          const uint32_t i = x / (D / 4), d = x % (D / 4) * 4;
-          float4 sum = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-          for (uint32_t k = 0; k < n; ++k) {
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_o + ((size_t)slot_of(from + k * each) * kRows + i) * D + d));
-            const float f = fac[k][i];
-            sum.x = fmaf(v.x, f, sum.x);
-            sum.y = fmaf(v.y, f, sum.y);
-            sum.z = fmaf(v.z, f, sum.z);
-            sum.w = fmaf(v.w, f, sum.w);
-          }
-          if (last) {
-            const float l = wl[0][i], inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const float y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
-            store_vec<T, 4>(out_row(i) + d, y);
-          } else {
-            *reinterpret_cast<float4 *>(part_o + ((size_t)slot_of(from) * kRows + i) * D + d) = sum;
-          }
-        }
-        if (last) break;
-        if (threadIdx.x < rows)
-          reinterpret_cast<float2 *>(part_ml)[(size_t)slot_of(from) * kRows + threadIdx.x] =
-              make_float2(wm[0][threadIdx.x], wl[0][threadIdx.x]);
-        last = true;
-        from = 0;
-        each = kPartGroup;
-        n = (parts + kPartGroup - 1) / kPartGroup;
-        word = a.cnt + c0 + 1;
-      }
+      merge_parts<T, D, kRows>(a, Parts{c0, c1 - c0 + 1, 2 * c0 + (at > run * c0 ? 1 : 0), r.r0, row0, rows, h}, sh);
     }
     merged = true;
   }
 }
 
-using AttnKernel = void (*)(Kv8AttnArgs);
+using AttnKernel = void (*)(const Kv8AttnArgs);
 struct DecVariant {
   AttnKernel fn;
   uint32_t smem, ctas;
