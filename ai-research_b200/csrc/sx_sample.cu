@@ -3,7 +3,7 @@
 //
 // Both walk rows of a vocabulary (1 MiB at 262144 tokens) and are bound by reading them, so a row
 // is spread over a thread-block cluster: its CTAs exchange one partial result each through
-// distributed shared memory, and the row is read once.
+// distributed shared memory, and the row is read once.  Many long rows take two passes instead.
 #include "sx_common.cuh"
 #include "sx_host.h"
 #include "sx_launch.cuh"
@@ -159,6 +159,76 @@ __global__ void __launch_bounds__(kSampleThreads) probs_kernel(ProbsArgs a) {
       store4(p, i, end, ap, make_float4(e.x * inv, e.y * inv, e.z * inv, e.w * inv));
     }
   }
+}
+
+// Many long rows in two passes: {max, sum} of every chunk of a row, then the division, with the logits
+// from L2 (126 MB; the chunks read last come first).  Clusters of 16 CTAs leave SMs empty and run in
+// waves that wait for their sums; here every CTA streams.  40 rows of 262144: 19.1 us, of which 13.0
+// are the bytes at the measured copy rate, the rest two launches' starts and ends.
+constexpr int kChunkThreads = 256, kChunkVecs = 8;
+constexpr uint32_t kChunk = kChunkThreads * 4 * kChunkVecs;
+
+SX_DEV void load_chunk(const ProbsArgs &a, const float *z, uint32_t i0, float4 (&x)[kChunkVecs]) {
+  const bool az = aligned16(z);
+#pragma unroll
+  for (int k = 0; k < kChunkVecs; ++k) x[k] = load4(z, i0 + k * kChunkThreads * 4, a.n, az, -INFINITY);
+}
+SX_DEV float max_of(const float4 (&x)[kChunkVecs]) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < kChunkVecs; ++k) m = fmaxf(fmaxf(m, fmaxf(x[k].x, x[k].y)), fmaxf(x[k].z, x[k].w));
+  return m;
+}
+
+__global__ void __launch_bounds__(kChunkThreads) probs_chunk_kernel(ProbsArgs a, uint32_t chunks, float2 *part) {
+  __shared__ float2 red[kChunkThreads / 32];
+  const uint32_t row = blockIdx.x / chunks, i0 = blockIdx.x % chunks * kChunk + threadIdx.x * 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_wait();
+  pdl_launch_dependents();  // after the wait: the next pass may read logits before this one ends
+  float4 x[kChunkVecs];
+  load_chunk(a, a.z + (size_t)row * a.z_ld, i0, x);
+  const float m = warp_max(max_of(x)), top = m == -INFINITY ? 0.0f : m;
+  float s = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kChunkVecs; ++k)
+    s += (ex2((x[k].x - top) * a.c) + ex2((x[k].y - top) * a.c)) + (ex2((x[k].z - top) * a.c) + ex2((x[k].w - top) * a.c));
+  s = warp_sum(s);
+  if (lane == 0) red[warp] = make_float2(m, s);
+  __syncthreads();
+  if (warp == 0) {
+    const float2 v = lane < kChunkThreads / 32 ? red[lane] : make_float2(-INFINITY, 0.0f);
+    const float all = warp_max(v.x);
+    const float sum = warp_sum(v.y * (v.x == -INFINITY ? 1.0f : ex2((v.x - all) * a.c)));
+    if (lane == 0) part[blockIdx.x] = make_float2(all, sum);
+  }
+}
+
+__global__ void __launch_bounds__(kChunkThreads) probs_divide_kernel(ProbsArgs a, uint32_t chunks, const float2 *part) {
+  const uint32_t block = gridDim.x - 1 - blockIdx.x, row = block / chunks;
+  const uint32_t i0 = block % chunks * kChunk + threadIdx.x * 4;
+  const uint32_t lane = threadIdx.x & 31;
+  float4 x[kChunkVecs];
+  load_chunk(a, a.z + (size_t)row * a.z_ld, i0, x);
+  pdl_launch_dependents();
+  pdl_wait();
+  float m = -INFINITY, s = 0.0f;
+  for (uint32_t k = lane; k < chunks; k += 32) {  // (the same order in every warp)
+    const float2 v = __ldcg(part + (size_t)row * chunks + k);
+    const float top = fmaxf(m, v.x);
+    s = s * (m == -INFINITY ? 1.0f : ex2((m - top) * a.c)) + v.y * (v.x == -INFINITY ? 1.0f : ex2((v.x - top) * a.c));
+    m = top;
+  }
+  const float all = warp_max(m), top = all == -INFINITY ? 0.0f : all;
+  const float sum = warp_sum(s * (m == -INFINITY ? 1.0f : ex2((m - all) * a.c)));
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // -inf alone stays 0; a NaN or +inf made the sum NaN
+  float *p = a.p + (size_t)row * a.p_ld;
+  const bool ap = aligned16(p);
+#pragma unroll
+  for (int k = 0; k < kChunkVecs; ++k)
+    store4(p, i0 + k * kChunkThreads * 4, a.n, ap,
+           make_float4(ex2((x[k].x - top) * a.c) * inv, ex2((x[k].y - top) * a.c) * inv,
+                       ex2((x[k].z - top) * a.c) * inv, ex2((x[k].w - top) * a.c) * inv));
 }
 
 // ---------------------------------------------------------------------------------------
@@ -364,6 +434,11 @@ ProbsVariant probs_variant(uint32_t n) {
   return {n <= ctas * (8 * 2048) ? probs_kernel<8> : probs_kernel<0>, ctas};
 }
 
+// Rows of four CTAs and more that do not all fit at once (two CTAs an SM, less what clusters leave
+// empty) take two passes: 40 rows of 262144 19.1 us for 25.6, 18 rows 11.2 for 14.8, 100 rows of 65536
+// 14.0 for 16.7; those that fit one, 10 rows of 262144 7.0 us either way, 40 of 65536 6.9.
+constexpr uint32_t kTwoPassCtas = 4;
+
 }  // namespace
 
 cudaError_t prepare_sample_kernels() {
@@ -399,6 +474,21 @@ SX_API sx_status sx_dispatch_probs(sx_engine *e, const float *logits, uint32_t l
   sx::ProbsArgs a{logits, probs, logits_ld ? logits_ld : n, probs_ld ? probs_ld : n, n,
                   1.4426950408889634f / temperature};
   const sx::ProbsVariant v = sx::probs_variant(n);
+  if (v.ctas >= sx::kTwoPassCtas && 2ull * rows * v.ctas > 3ull * e->num_sms) {
+    const uint32_t chunks = (n + sx::kChunk - 1) / sx::kChunk;
+    float2 *const part = reinterpret_cast<float2 *>(e->kv8_part);
+    const uint32_t most = (uint32_t)(sx::kv8_part_bytes(e->num_sms) / sizeof(float2)) / chunks;
+    for (uint32_t r = 0; r < rows && ce == cudaSuccess; r += most) {
+      sx::ProbsArgs b = a;
+      b.z += (size_t)r * a.z_ld;
+      b.p += (size_t)r * a.p_ld;
+      const dim3 grid(std::min(most, rows - r) * chunks), block(sx::kChunkThreads);
+      ce = sx::launch_chained(sx::probs_chunk_kernel, grid, block, 0, e->stream, 1, b, chunks, part);
+      if (ce == cudaSuccess)
+        ce = sx::launch_chained(sx::probs_divide_kernel, grid, block, 0, e->stream, 1, b, chunks, (const float2 *)part);
+    }
+    return sx_host_cuda_status(ce, "probs launch");
+  }
   return sx_host_cuda_status(
       sx::launch_chained(v.fn, dim3(rows * v.ctas), dim3(sx::kSampleThreads), 0, e->stream, v.ctas, a),
       "probs launch");

@@ -185,6 +185,19 @@ def test_attn_long_and_ragged(eng, dtype, d):
     check_attn(eng, dtype, 8, 4, d, 64, [1, 1, 1, 2], [40001, 3, 12345, 777], seed=9)
 
 
+@pytest.mark.parametrize("dtype,d,lens", [("f32", 64, [150000]), ("bf16", 64, [700, 90001, 0, 40000]), ("f32", 256, [60001, 9])])
+def test_attn_many_parts_of_a_problem(eng, dtype, d, lens):
+    """Long enough that over 32 CTAs share a problem, which merge in two levels."""
+    news = [min(n, 1) for n in lens]
+    for _ in range(3):  # the arrival counters are left at 0
+        check_attn(eng, dtype, 4, 1, d, 64, news, lens, seed=12)
+
+
+@pytest.mark.parametrize("lens", [[640], [250] * 40, [700, 1, 0, 33] * 30, [500] * 200])
+def test_attn_problems_cut_and_uncut(eng, lens):
+    check_attn(eng, "bf16", 8, 2, 128, 32, [min(n, 1) for n in lens], lens, seed=13)
+
+
 @pytest.mark.parametrize("dtype,d,hq", [("f32", 64, 8), ("bf16", 128, 16)])
 def test_attn_one_long_prompt(eng, dtype, d, hq):
     check_attn(eng, dtype, hq, 2, d, 64, [700, 1], [2100, 5], seed=10)

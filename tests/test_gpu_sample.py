@@ -78,6 +78,42 @@ def test_probs_special_values(eng, n):
     check_probs(eng, z)
 
 
+@pytest.mark.parametrize("n,rows,ld", [(65537, 40, 65537), (131072, 60, 131076), (262144, 20, 262147), (300001, 20, 300004)])
+def test_probs_many_long_rows(eng, n, rows, ld):
+    z = torch.randn(rows, n, device="cuda") * 3
+    z[1] = -math.inf
+    z[2, : n // 2] = -math.inf
+    z[3, n // 3] = math.nan
+    z[4, n - 1] = math.inf
+    z[5] = torch.finfo(torch.float32).min
+    check_probs(eng, z, 0.8, ld)
+    check_probs(eng, z, 0.8, ld, inplace=True)
+
+
+def test_probs_many_long_rows_repeat_in_a_graph(eng):
+    z = torch.randn(24, 262144, device="cuda")
+    want, out = torch.empty_like(z), torch.empty_like(z)
+    eng.probs(z, want, 24, 262144)
+    eng.sync()
+    s = torch.cuda.Stream()
+    try:
+        with torch.cuda.stream(s):
+            eng.set_stream(s.cuda_stream)
+            eng.probs(z, out, 24, 262144)
+            s.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                for _ in range(4):
+                    eng.probs(z, out, 24, 262144)
+            for _ in range(3):
+                out.zero_()
+                g.replay()
+                s.synchronize()
+                assert torch.equal(out, want)
+    finally:
+        eng.set_stream(sx.STREAM_LEGACY)
+
+
 def test_probs_refusals(eng):
     z = torch.zeros(2, 8, device="cuda")
     for kw in (dict(logits=None), dict(probs=None), dict(n=0), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=math.nan),
