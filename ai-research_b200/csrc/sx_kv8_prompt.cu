@@ -160,15 +160,14 @@ struct Problem {
 template <int TOKENS, int WIDEN>
 struct PromptShared {
   uint64_t bars[10];
-  uint32_t tmem_slot, last_flag, abort_flag;
+  uint32_t tmem_slot, abort_flag;
   uint32_t nan_mask[2][TOKENS / 32];
   Problem problem[2];
   float row_mul[kRows];
-  float2 row_merge[kRows];
   float row_top[2][kRows], row_sum[2][kRows];  // of the two halves of a tile's keys
   // The blocks of 32 tiles: of a widening warp the record pairs (kNoRecord: nothing to read); of a pair
   // of blocks of a tile {k scale, log2(v scale), 1 / v scale, there}.
-  uint32_t record[WIDEN][64];
+  alignas(8) uint32_t record[WIDEN][64];  // (read by twos)
   float4 facts[TOKENS / 32][64];
 };
 
@@ -381,56 +380,89 @@ __device__ __noinline__ void put_q(const Kv8AttnArgs &a, const Problem &w, uint3
   fence_proxy_async();  // generic-proxy stores -> the tensor core's reads
 }
 
-// The last CTA to finish a part of a problem merges the parts: a thread per row for the maxima and the
-// sums, then all threads over the rows' values, four at a time with their loads in flight together.
+// What a part's CTA leaves for the merge: where the problem's parts are, and which it is.
+struct PromptPart {
+  uint32_t parts, part, slot0, c0;  // parts 0: there is none
+  uint32_t r0, row0, rows, head;
+};
+// The workspace: {m, l} of [2 CTAs][128 rows], [2 CTAs][128 rows][D], [2 CTAs] of the above.
+SX_DEV float *part_values(const Kv8AttnArgs &a, uint32_t ctas) { return a.part + (size_t)2 * ctas * kRows * 2; }
+template <int D>
+SX_DEV PromptPart *part_list(const Kv8AttnArgs &a, uint32_t ctas) {
+  return reinterpret_cast<PromptPart *>(part_values(a, ctas) + (size_t)2 * ctas * kRows * D);
+}
+
+// The parts of cut problems, by a second kernel (the last CTA to arrive alone would read them at 17 bytes
+// a cycle, 15 us for 9 parts of 40 rows of 256): CTA j takes part j's share of its problem's rows.
+// Threads: D / 4 columns x kSubs.  A sub takes a row, or with many parts every kSubs-th part of one, and
+// they meet in shared memory.
+constexpr int kMergeThreads = 512;
+constexpr uint32_t kShareParts = 16;
+
+struct Merged {
+  float m, l;
+  float4 o;
+  SX_DEV void add(float mk, float lk, float4 v) {
+    const float top = fmaxf(m, mk);  // a part that saw nothing has -inf and weight 0
+    const float f = m == -INFINITY ? 0.0f : ex2(m - top), g = mk == -INFINITY ? 0.0f : ex2(mk - top);
+    m = top;
+    l = fmaf(l, f, lk * g);
+    o = make_float4(fmaf(o.x, f, v.x * g), fmaf(o.y, f, v.y * g), fmaf(o.z, f, v.z * g), fmaf(o.w, f, v.w * g));
+  }
+};
+
 template <typename T, int D>
-__device__ __noinline__ void merge_parts(const Kv8AttnArgs &a, const Problem &w, float2 (&row)[kRows]) {
-  const float2 *ml = reinterpret_cast<const float2 *>(a.part);
-  const float *po = a.part + (size_t)2 * gridDim.x * kRows * 2;
-  const uint32_t n = w.parts, rows = w.rows;
-  auto slot_of = [&](uint32_t k) { return k == 0 ? w.slot0 : 2 * (w.c0 + k); };
-  if (threadIdx.x < rows) {
-    float m = -INFINITY, l = 0.0f;
-#pragma unroll 4
-    for (uint32_t k = 0; k < n; ++k) {
-      const float2 v = __ldcg(ml + (size_t)slot_of(k) * kRows + threadIdx.x);
-      const float top = fmaxf(m, v.x);  // a part that saw nothing has -inf and weight 0
-      l = l * (m == -INFINITY ? 0.0f : ex2(m - top)) + v.y * (v.x == -INFINITY ? 0.0f : ex2(v.x - top));
-      m = top;
-    }
-    row[threadIdx.x] = make_float2(m, l == 0.0f ? 0.0f : 1.0f / l);
-  }
-  __syncthreads();
-  constexpr uint32_t kCols = D / 4;
+__global__ void __launch_bounds__(kMergeThreads) kv8_prompt_merge_kernel(const __grid_constant__ Kv8AttnArgs a, uint32_t ctas) {
+  constexpr uint32_t kItems = D / 4, kSubs = kMergeThreads / kItems, kBatch = 4;
+  __shared__ Merged red[kMergeThreads];
+  pdl_launch_dependents();
+  pdl_wait();
+  const PromptPart w = part_list<D>(a, ctas)[blockIdx.x];
+  if (w.parts == 0) return;
+  const float2 *const part_ml = reinterpret_cast<const float2 *>(a.part);
+  const float *const part_o = part_values(a, ctas);
+  const uint32_t item = threadIdx.x % kItems, sub = threadIdx.x / kItems;
+  const bool share = w.parts > kShareParts;
+  const uint32_t i0 = w.rows * w.part / w.parts, i1 = w.rows * (w.part + 1) / w.parts;
+  const uint32_t first = share ? sub : 0, step = share ? kSubs : 1, rows = share ? 1 : kSubs;
 #pragma unroll 1
-  for (uint32_t x0 = threadIdx.x; x0 < rows * kCols; x0 += 4 * blockDim.x) {
-    float4 sum[4];
+  for (uint32_t ii = i0; ii < i1; ii += rows) {
+    const uint32_t i = share ? ii : ii + sub;
+    Merged sum{-INFINITY, 0.0f, make_float4(0.0f, 0.0f, 0.0f, 0.0f)};
+#pragma unroll 1
+    for (uint32_t k0 = first; k0 < w.parts && i < i1; k0 += kBatch * step) {
+      float4 v[kBatch];
+      float2 ml[kBatch];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) sum[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 2
-    for (uint32_t k = 0; k < n; ++k) {
-      const size_t base = (size_t)slot_of(k) * kRows;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint32_t x = min(x0 + u * blockDim.x, rows * kCols - 1), i = x / kCols;
-        const float mk = __ldcg(&ml[base + i].x);
-        const float4 v = __ldcg(reinterpret_cast<const float4 *>(po + (base + i) * D + x % kCols * 4));
-        const float f = mk == -INFINITY ? 0.0f : ex2(mk - row[i].x);
-        sum[u].x = fmaf(v.x, f, sum[u].x);
-        sum[u].y = fmaf(v.y, f, sum[u].y);
-        sum[u].z = fmaf(v.z, f, sum[u].z);
-        sum[u].w = fmaf(v.w, f, sum[u].w);
+      for (uint32_t u = 0; u < kBatch; ++u) {
+        const uint32_t k = min(k0 + u * step, w.parts - 1);
+        const size_t at = (size_t)(k == 0 ? w.slot0 : 2 * (w.c0 + k)) * kRows + i;
+        v[u] = *reinterpret_cast<const float4 *>(part_o + at * D + 4 * item);
+        ml[u] = part_ml[at];
       }
-    }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t x = x0 + u * blockDim.x, i = x / kCols;
-      if (x >= rows * kCols) break;
-      const float f = row[i].y, y[4] = {sum[u].x * f, sum[u].y * f, sum[u].z * f, sum[u].w * f};
-      store_vec<T, 4>(static_cast<T *>(a.out) + w.row(a, i) * a.out_ld + w.col(a, i) + x % kCols * 4, y);
+      for (uint32_t u = 0; u < kBatch; ++u)
+        if (k0 + u * step < w.parts) sum.add(ml[u].x, ml[u].y, v[u]);
+    }
+    if (share) {
+      __syncthreads();  // the row before has been added up
+      red[threadIdx.x] = sum;
+      __syncthreads();
+      if (sub == 0)
+#pragma unroll 1
+        for (uint32_t u = 1; u < kSubs; ++u) {
+          const Merged x = red[u * kItems + item];
+          sum.add(x.m, x.l, x.o);
+        }
+    }
+    if (i < i1 && (!share || sub == 0)) {
+      const float inv = sum.l == 0.0f ? 0.0f : 1.0f / sum.l;
+      const float y[4] = {sum.o.x * inv, sum.o.y * inv, sum.o.z * inv, sum.o.w * inv};
+      const uint32_t pr = w.row0 + i;
+      store_vec<T, 4>(static_cast<T *>(a.out) + (size_t)(w.r0 + pr / a.gqa) * a.out_ld +
+                          (size_t)(w.head * a.gqa + pr % a.gqa) * D + 4 * item, y);
     }
   }
-  if (threadIdx.x == 0) a.cnt[w.c0] = 0;
 }
 
 // One product by one thread of the warp that calls it: STEPS of 16 along K, A from shared memory
@@ -476,6 +508,9 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
   };
   Schedule plan;
   if constexpr (ROLE == kProducts) {
+    PromptPart *const list = part_list<D>(a, gridDim.x) + 2 * blockIdx.x;
+    if (lane < 2) list[lane].parts = 0;
+    __syncwarp();
     plan.start(a, kTokens);
     plan.next(a, kTileBlocks, sh.problem[0]);
   }
@@ -593,7 +628,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       tc_fence_after();
       const bool whole = pr.parts == 1;
       const size_t at = (size_t)pr.slot * kRows + i;
-      float *const po = a.part + (size_t)2 * gridDim.x * kRows * 2 + at * D;
+      float *const po = part_values(a, gridDim.x) + at * D;
       T *const out = static_cast<T *>(a.out) + pr.row(a, i) * a.out_ld + pr.col(a, i);
       const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
       if (!whole && half == 0 && i < rows) reinterpret_cast<float2 *>(a.part)[at] = make_float2(ref, l);
@@ -786,6 +821,9 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         __syncwarp();
       };
       product_s(tiles);
+      if (pr.parts > 1 && lane == 0)
+        part_list<D>(a, gridDim.x)[pr.slot] =
+            PromptPart{pr.parts, blockIdx.x - pr.c0, pr.slot0, pr.c0, pr.r0, pr.row0, pr.rows, pr.head};
       plan.next(a, kTileBlocks, sh.problem[(np + 1) & 1]);  // (read by all after the barrier below)
 #pragma unroll 1
       for (uint32_t j = 0; j < n_tiles; ++j) {
@@ -806,12 +844,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       }
     }
     tiles += n_tiles;
-    __syncthreads();  // Q, the tiles and O are free; the parts are written, and the next problem
-    if (pr.parts > 1) {
-      if (threadIdx.x == 0) sh.last_flag = arrive_acq_rel(a.cnt + pr.c0) == pr.parts - 1;
-      __syncthreads();
-      if (sh.last_flag) merge_parts<T, D>(a, pr, sh.row_merge);
-    }
+    __syncthreads();  // Q, the tiles and O are free, and the next problem is there
   }
 }
 
@@ -858,14 +891,16 @@ __global__ void __launch_bounds__((PromptShape<D, sizeof(T) == 4>::kThreads), (P
 }
 
 using PromptKernel = void (*)(const Kv8AttnArgs);
+using PromptMerge = void (*)(const Kv8AttnArgs, uint32_t);
 struct PromptVariant {
   PromptKernel fn;
+  PromptMerge merge;
   uint32_t smem, ctas, threads;
 };
 template <typename T, int D>
 PromptVariant prompt_variant() {
   using P = PromptShape<D, sizeof(T) == 4>;
-  return {kv8_prompt_kernel<T, D>, (uint32_t)P::kSmem, (uint32_t)P::kCtas, (uint32_t)P::kThreads};
+  return {kv8_prompt_kernel<T, D>, kv8_prompt_merge_kernel<T, D>, (uint32_t)P::kSmem, (uint32_t)P::kCtas, (uint32_t)P::kThreads};
 }
 PromptVariant prompt_variant(sx_dtype t, uint32_t d) {
   if (t == SX_F32)
@@ -887,12 +922,17 @@ cudaError_t prepare_kv8_prompt() {
 }
 
 // Two parts per CTA of 128 rows: {m, l}, and 128 (two CTAs per SM) or 256 output values a row.
-size_t kv8_prompt_part_bytes(int num_sms) { return (size_t)2 * num_sms * kRows * (2 * 2 + 256) * sizeof(float); }
+size_t kv8_prompt_part_bytes(int num_sms) {
+  return (size_t)2 * num_sms * (kRows * (2 * 2 + 256) * sizeof(float) + 2 * sizeof(PromptPart));
+}
 
 cudaError_t launch_kv8_prompt(Kv8AttnArgs a, sx_dtype t, int num_sms, cudaStream_t s) {
   const PromptVariant v = prompt_variant(t, a.c.head_dim);
   a.min_run = 6;  // tiles: shorter runs cost more to merge than they save
-  return launch_chained(v.fn, dim3(num_sms * v.ctas), dim3(v.threads), v.smem, s, 1, a);
+  const uint32_t ctas = num_sms * v.ctas;
+  const cudaError_t e = launch_chained(v.fn, dim3(ctas), dim3(v.threads), v.smem, s, 1, a);
+  if (e != cudaSuccess) return e;
+  return launch_chained(v.merge, dim3(2 * ctas), dim3(kMergeThreads), 0, s, 1, a, ctas);
 }
 
 }  // namespace sx
