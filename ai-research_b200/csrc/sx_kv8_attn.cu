@@ -55,11 +55,9 @@ struct DecShape {
   static constexpr int kRows = 8 * NT;
   static constexpr int kPieces = D / 32;
   static constexpr int kCtas = D * NT <= 256 ? 2 : 1;         // per SM
-  static constexpr int kSub = D * NT >= 256 ? 1 : 256 / (D * NT);  // blocks a warp takes at a time
   static constexpr int kRecord = 16 * D;
-  static constexpr int kStageBytes = kSub * kRecord;
   static constexpr int kRing = (kCtas == 2 ? 12 : 24) * 1024; // of one warp
-  static constexpr int kStages = kRing / kStageBytes;
+  static constexpr int kStages = kRing / kRecord;
   static constexpr int kLdO = D + 4;
   static constexpr int kMerge = kDecWarps * kRows * kLdO * 4; // shares the rings' memory
   static constexpr int kArea = kDecWarps * kRing > kMerge ? kDecWarps * kRing : kMerge;
@@ -153,8 +151,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
     kv8_decode_kernel(const __grid_constant__ Kv8AttnArgs a) {
   constexpr bool kSplit = sizeof(T) == 4;
   using S = DecShape<D, NT, kSplit>;
-  constexpr int kSub = S::kSub, kStages = S::kStages, kPieces = S::kPieces, kRows = S::kRows;
-  constexpr uint32_t kStep = kDecWarps * kSub;  // blocks that the CTA takes at a time
+  constexpr int kStages = S::kStages, kPieces = S::kPieces, kRows = S::kRows;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t full_bar[kDecWarps * kStages];
   __shared__ DecShared<kRows> sh;
@@ -206,10 +203,10 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
     }
     const uint64_t total = __shfl_sync(0xffffffffu, incl, 31);
     run = (total + gridDim.x - 1) / gridDim.x;
-    run = run > kStep ? run : kStep;
+    run = run > (uint32_t)kDecWarps ? run : (uint32_t)kDecWarps;
     longest = __reduce_max_sync(0xffffffffu, longest);
     problems = __reduce_add_sync(0xffffffffu, problems);
-    uncut = longest <= kMergeSteps * kStep + (problems <= gridDim.x ? run : 0);
+    uncut = longest <= kMergeSteps * kDecWarps + (problems <= gridDim.x ? run : 0);
     begin = run * blockIdx.x;
     end = begin + run < total ? begin + run : total;
     if (begin >= end) return;
@@ -258,16 +255,17 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
 
     // ---- copies: entry j is the warp's j-th block of the segment, 32 entries at a time in lanes
     const uint32_t *table = a.c.table + (size_t)(b - 1) * a.c.max_pages;
-    const uint32_t steps = (s1 - s0 + kDecWarps * kSub - 1) / (kDecWarps * kSub);
-    auto block_of = [&](uint32_t j) { return s0 + (j / kSub * kDecWarps + warp) * kSub + j % kSub; };
+    const uint32_t steps = (s1 - s0 + kDecWarps - 1 - warp) / kDecWarps;  // of this warp
+    const uint32_t busy = min((uint32_t)kDecWarps, s1 - s0);              // warps with any
+    auto block_of = [&](uint32_t j) { return s0 + j * kDecWarps + warp; };
     struct Entry {
       uint64_t rec;  // record pair index; ~0: nothing to read
       float ks, vs;
     };
     auto entry = [&](uint32_t j) -> Entry {
       Entry e{~0ull, 0.0f, 1.0f};
+      if (j >= steps) return e;
       const uint32_t s = block_of(j);
-      if (s >= s1) return e;
       const uint32_t blk = first + s;
       const uint32_t page = table[blk * kKv8Block / a.c.page_tokens];
       if (page >= a.c.num_pages) {
@@ -301,17 +299,15 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
     uint32_t batch = 0;     // cur holds entries [32 batch, + 32)
     uint32_t to_issue = 0;  // next record to issue: 2 step (K), 2 step + 1 (V)
     auto issue = [&]() {
-      const uint32_t j0 = to_issue / 2 * kSub;
-      const Entry &e = j0 / 32 == batch ? cur : nxt;
-      const bool mine = (uint32_t)lane - j0 % 32 < (uint32_t)kSub && e.rec != ~0ull;
-      const uint32_t n = __popc(__ballot_sync(0xffffffffu, mine));
-      const uint32_t st = issued % kStages;
-      if (lane == 0) mbar_arrive_expect_tx(bar_u + 8 * st, n * S::kRecord);
-      __syncwarp();
-      if (mine)
-        bulk_g2s(ring_u + st * S::kStageBytes + (lane - j0 % 32) * S::kRecord,
-                 static_cast<const uint8_t *>(a.c.data) + (2 * e.rec + (to_issue & 1)) * S::kRecord,
-                 S::kRecord, bar_u + 8 * st);
+      const uint32_t j = to_issue / 2, st = issued % kStages;
+      const Entry &e = j / 32 == batch ? cur : nxt;
+      if ((uint32_t)lane == j % 32) {
+        const bool there = e.rec != ~0ull;
+        mbar_arrive_expect_tx(bar_u + 8 * st, there ? S::kRecord : 0);
+        if (there)
+          bulk_g2s(ring_u + st * S::kRecord, static_cast<const uint8_t *>(a.c.data) + (2 * e.rec + (to_issue & 1)) * S::kRecord,
+                   S::kRecord, bar_u + 8 * st);
+      }
       ++issued;
       ++to_issue;
     };
@@ -375,26 +371,18 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
     const uint32_t all_lo = a.window && pos0 + tok_hi >= a.window ? pos0 + tok_hi - a.window + 1 : 0;
 
     for (uint32_t step = 0; step < steps; ++step) {
-      const uint32_t j0 = step * kSub;
-      if (j0 / 32 != batch) {
+      if (step / 32 != batch) {
         cur = nxt;
         ++batch;
         nxt = entry(32 * (batch + 1) + lane);
       }
-      float ks[kSub], vs[kSub];
-      bool have[kSub];
-#pragma unroll
-      for (int i = 0; i < kSub; ++i) {
-        const int src = (int)(j0 % 32) + i;
-        ks[i] = __shfl_sync(0xffffffffu, cur.ks, src);
-        vs[i] = __shfl_sync(0xffffffffu, cur.vs, src);
-        have[i] = __shfl_sync(0xffffffffu, (int)(cur.rec != ~0ull), src) != 0;
-      }
+      const float ks = __shfl_sync(0xffffffffu, cur.ks, step % 32), vs = __shfl_sync(0xffffffffu, cur.vs, step % 32);
+      const bool have = __shfl_sync(0xffffffffu, (int)(cur.rec != ~0ull), step % 32) != 0;
       auto stage = [&]() -> uint8_t * {  // the next record, once it is there
         const uint32_t st = taken % kStages;
         if (!mbar_wait_bounded(bar_u + 8 * st, (taken / kStages) & 1)) raise_error(a.err, kDevWaitTimeout);
         ++taken;
-        return ring + st * S::kStageBytes;
+        return ring + st * S::kRecord;
       };
       auto release = [&]() {  // a record has been read: its stage takes the next copy
         __syncwarp();
@@ -404,105 +392,88 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
 
       // ---- S^T = K Q^T
       // (two chains of accumulators: an MMA's result is 24 cycles away)
-      float s[kSub][NT][2][4];
+      float s[NT][2][4];
 #pragma unroll
-      for (int i = 0; i < kSub; ++i)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int w = 0; w < 2; ++w)
 #pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s[i][t][w][k] = 0.0f;
+          for (int k = 0; k < 4; ++k) s[t][w][k] = 0.0f;
 #pragma unroll
       for (int p = 0; p < kPieces; ++p) {
-        uint4 q[NT][kSplit ? 2 : 1];
+        const uint4 k4 = *reinterpret_cast<const uint4 *>(kr + p * 512 + lane * 16);
+        uint32_t a0[4], a1[4];
+        e4m3x4_f16(k4.x, a0[0], a0[2]);
+        e4m3x4_f16(k4.y, a1[0], a1[2]);
+        e4m3x4_f16(k4.z, a0[1], a0[3]);
+        e4m3x4_f16(k4.w, a1[1], a1[3]);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int w = 0; w < (kSplit ? 2 : 1); ++w)
-            q[t][w] = *reinterpret_cast<const uint4 *>(qf + w * (S::kQ / 2) + (t * kPieces + p) * 512 + lane * 16);
-#pragma unroll
-        for (int i = 0; i < kSub; ++i) {
-          const uint4 k4 = *reinterpret_cast<const uint4 *>(kr + i * S::kRecord + p * 512 + lane * 16);
-          uint32_t a0[4], a1[4];
-          e4m3x4_f16(k4.x, a0[0], a0[2]);
-          e4m3x4_f16(k4.y, a1[0], a1[2]);
-          e4m3x4_f16(k4.z, a0[1], a0[3]);
-          e4m3x4_f16(k4.w, a1[1], a1[3]);
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int w = 0; w < (kSplit ? 2 : 1); ++w) {
-              mma_f16_16816(s[i][t][0], a0, q[t][w].x, q[t][w].y);
-              mma_f16_16816(s[i][t][1], a1, q[t][w].z, q[t][w].w);
-            }
-        }
+          for (int w = 0; w < (kSplit ? 2 : 1); ++w) {
+            const uint4 q = *reinterpret_cast<const uint4 *>(qf + w * (S::kQ / 2) + (t * kPieces + p) * 512 + lane * 16);
+            mma_f16_16816(s[t][0], a0, q.x, q.y);
+            mma_f16_16816(s[t][1], a1, q.z, q.w);
+          }
       }
 
       release();
 
       // ---- scores, masks, running maximum
       uint8_t *const vr = stage();
-      float lv[kSub], top[NT][2];
+      float top[NT][2];
+      const float lv = (float)kv8_scale_exponent(vs);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) top[t][0] = top[t][1] = -INFINITY;
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int i = 0; i < kSub; ++i) {
-        lv[i] = (float)kv8_scale_exponent(vs[i]);
+        for (int k = 0; k < 4; ++k) s[t][0][k] = fmaf((s[t][0][k] + s[t][1][k]) * ks, mul[t][k & 1], lv);
+      const uint32_t key0 = (first + block_of(step)) * kKv8Block;
+      if (!have || key0 < all_lo || key0 + kKv8Block - 1 > all_hi) {
+        // Some row does not see all of the block.  A token no row sees is taken out of V (its
+        // bytes may be anything); one whose V holds a NaN is taken out too and makes the
+        // rows that do see it NaN.
+        uint32_t nan = 0;
+        uint4 *const own = reinterpret_cast<uint4 *>(vr) + lane;  // + 32 p
+        if (have) {
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p) {
+            const uint4 v = own[32 * p];
+            nan |= ((v.x & 0x7F7F7F7Fu) + 0x01010101u) | ((v.y & 0x7F7F7F7Fu) + 0x01010101u) |
+                   ((v.z & 0x7F7F7F7Fu) + 0x01010101u) | ((v.w & 0x7F7F7F7Fu) + 0x01010101u);
+          }
+          nan &= 0x80808080u;
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) nan |= __shfl_xor_sync(0xffffffffu, nan, w);
+        } else {
+          nan = 0x80808080u;  // nothing was read: whatever the stage holds goes
+        }
+        if (__any_sync(0xffffffffu, nan != 0)) {
+          const uint32_t keep = ~((nan >> 7) * 0xFFu);
+#pragma unroll
+          for (int p = 0; p < kPieces; ++p) {
+            uint4 v = own[32 * p];
+            v.x &= keep; v.y &= keep; v.z &= keep; v.w &= keep;
+            own[32 * p] = v;
+          }
+          fence_proxy_async();  // before the stage's next copy
+        }
+        // token g is byte g % 2 of the lanes with c = g / 2, token g + 8 two bytes on
+        const uint32_t nan_g = __shfl_sync(0xffffffffu, nan, g / 2) >> (8 * (g & 1));
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            s[i][t][0][k] = fmaf((s[i][t][0][k] + s[i][t][1][k]) * ks[i], mul[t][k & 1], lv[i]);
+            const uint32_t key = key0 + g + (k >> 1) * 8;
+            const bool seen = have && key >= see_lo[t][k & 1] && key <= see_hi[t][k & 1];
+            float x = s[t][0][k];
+            if ((nan_g >> (16 * (k >> 1))) & 0x80u) x = NAN;
+            s[t][0][k] = seen ? x : -INFINITY;
           }
-        const uint32_t key0 = (first + block_of(j0 + i)) * kKv8Block;
-        if (!have[i] || key0 < all_lo || key0 + kKv8Block - 1 > all_hi) {
-          // Some row does not see all of the block.  A token no row sees is taken out of V (its
-          // bytes may be anything); one whose V holds a NaN is taken out too and makes the
-          // rows that do see it NaN.
-          uint32_t nan = 0;
-          uint4 *const own = reinterpret_cast<uint4 *>(vr + i * S::kRecord) + lane;  // + 32 p
-          if (have[i]) {
-#pragma unroll
-            for (int p = 0; p < kPieces; ++p) {
-              const uint4 v = own[32 * p];
-              nan |= ((v.x & 0x7F7F7F7Fu) + 0x01010101u) | ((v.y & 0x7F7F7F7Fu) + 0x01010101u) |
-                     ((v.z & 0x7F7F7F7Fu) + 0x01010101u) | ((v.w & 0x7F7F7F7Fu) + 0x01010101u);
-            }
-            nan &= 0x80808080u;
-#pragma unroll
-            for (int w = 4; w < 32; w <<= 1) nan |= __shfl_xor_sync(0xffffffffu, nan, w);
-          } else {
-            nan = 0x80808080u;  // nothing was read: whatever the stage holds goes
-          }
-          if (__any_sync(0xffffffffu, nan != 0)) {
-            const uint32_t keep = ~((nan >> 7) * 0xFFu);
-#pragma unroll
-            for (int p = 0; p < kPieces; ++p) {
-              uint4 v = own[32 * p];
-              v.x &= keep; v.y &= keep; v.z &= keep; v.w &= keep;
-              own[32 * p] = v;
-            }
-            fence_proxy_async();  // before the stage's next copy
-          }
-          // token g is byte g % 2 of the lanes with c = g / 2, token g + 8 two bytes on
-          const uint32_t nan_g = __shfl_sync(0xffffffffu, nan, g / 2) >> (8 * (g & 1));
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t key = key0 + g + (k >> 1) * 8;
-              const bool seen = have[i] && key >= see_lo[t][k & 1] && key <= see_hi[t][k & 1];
-              float x = s[i][t][0][k];
-              if ((nan_g >> (16 * (k >> 1))) & 0x80u) x = NAN;
-              s[i][t][0][k] = seen ? x : -INFINITY;
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) top[t][k & 1] = fmaxf(top[t][k & 1], s[i][t][0][k]);
       }
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) top[t][k] = fmaxf(s[t][0][k], s[t][0][k + 2]);
       bool moved = false;
       float shift[NT][2];
 #pragma unroll
@@ -535,46 +506,41 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
       }
 
       // ---- P^T as B operands
-      uint32_t pb[kSub][NT][kSplit ? 2 : 1][2];
+      uint32_t pb[NT][kSplit ? 2 : 1][2];
+      const float unv = ex2(-lv);
 #pragma unroll
-      for (int i = 0; i < kSub; ++i) {
-        const float unv = ex2(-lv[i]);
+      for (int t = 0; t < NT; ++t) {
+        float pr[4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float pr[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) pr[k] = ex2(s[i][t][0][k] - shift[t][k & 1]);
-          ls[t][0] = fmaf(pr[0] + pr[2], unv, ls[t][0]);
-          ls[t][1] = fmaf(pr[1] + pr[3], unv, ls[t][1]);
-          const uint32_t p0 = pack_f16(pr[0], pr[1]), p1 = pack_f16(pr[2], pr[3]);
-          pb[i][t][0][0] = movmatrix_trans(p0);
-          pb[i][t][0][1] = movmatrix_trans(p1);
-          if constexpr (kSplit) {
-            pb[i][t][1][0] = movmatrix_trans(pack_f16_rest(pr[0], pr[1], p0));
-            pb[i][t][1][1] = movmatrix_trans(pack_f16_rest(pr[2], pr[3], p1));
-          }
+        for (int k = 0; k < 4; ++k) pr[k] = ex2(s[t][0][k] - shift[t][k & 1]);
+        ls[t][0] = fmaf(pr[0] + pr[2], unv, ls[t][0]);
+        ls[t][1] = fmaf(pr[1] + pr[3], unv, ls[t][1]);
+        const uint32_t p0 = pack_f16(pr[0], pr[1]), p1 = pack_f16(pr[2], pr[3]);
+        pb[t][0][0] = movmatrix_trans(p0);
+        pb[t][0][1] = movmatrix_trans(p1);
+        if constexpr (kSplit) {
+          pb[t][1][0] = movmatrix_trans(pack_f16_rest(pr[0], pr[1], p0));
+          pb[t][1][1] = movmatrix_trans(pack_f16_rest(pr[2], pr[3], p1));
         }
       }
 
       // ---- O^T += V^T P^T
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p)
+      for (int p = 0; p < kPieces; ++p) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(vr + p * 512 + lane * 16);
+        uint32_t a0[4], a1[4];
+        e4m3x4_f16(v.x, a0[0], a0[2]);
+        e4m3x4_f16(v.y, a0[1], a0[3]);
+        e4m3x4_f16(v.z, a1[0], a1[2]);
+        e4m3x4_f16(v.w, a1[1], a1[3]);
 #pragma unroll
-        for (int i = 0; i < kSub; ++i) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(vr + i * S::kRecord + p * 512 + lane * 16);
-          uint32_t a0[4], a1[4];
-          e4m3x4_f16(v.x, a0[0], a0[2]);
-          e4m3x4_f16(v.y, a0[1], a0[3]);
-          e4m3x4_f16(v.z, a1[0], a1[2]);
-          e4m3x4_f16(v.w, a1[1], a1[3]);
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int w = 0; w < (kSplit ? 2 : 1); ++w) {
-              mma_f16_16816(o[p][0][t], a0, pb[i][t][w][0], pb[i][t][w][1]);
-              mma_f16_16816(o[p][1][t], a1, pb[i][t][w][0], pb[i][t][w][1]);
-            }
-        }
+          for (int w = 0; w < (kSplit ? 2 : 1); ++w) {
+            mma_f16_16816(o[p][0][t], a0, pb[t][w][0], pb[t][w][1]);
+            mma_f16_16816(o[p][1][t], a1, pb[t][w][0], pb[t][w][1]);
+          }
+      }
       release();
     }
 
@@ -593,14 +559,16 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
       }
     __syncthreads();  // every warp's ring is free
     float *const mo = reinterpret_cast<float *>(smem);
+    if ((uint32_t)warp < busy) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p)
+        for (int p = 0; p < kPieces; ++p)
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
-          *reinterpret_cast<float4 *>(mo + (size_t)(warp * kRows + 8 * t + 2 * c + k) * S::kLdO + 32 * p + 4 * g) =
-              make_float4(o[p][0][t][k], o[p][0][t][k + 2], o[p][1][t][k], o[p][1][t][k + 2]);
+          for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<float4 *>(mo + (size_t)(warp * kRows + 8 * t + 2 * c + k) * S::kLdO + 32 * p + 4 * g) =
+                make_float4(o[p][0][t][k], o[p][0][t][k + 2], o[p][1][t][k], o[p][1][t][k + 2]);
+    }
     const bool whole = s0 == 0 && s1 == count;
     // a problem that starts inside the run, or at its head: at most one of each leaves a part
     const uint32_t slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
@@ -632,8 +600,8 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
     for (uint32_t x = threadIdx.x; x < rows * (D / 4); x += kDecThreads) {
       const uint32_t i = x / (D / 4), d = x % (D / 4) * 4;
       float4 sum = make_float4(0, 0, 0, 0);
-#pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) {
+#pragma unroll 4
+      for (uint32_t w = 0; w < busy; ++w) {
         const float4 v = *reinterpret_cast<const float4 *>(mo + (size_t)(w * kRows + i) * S::kLdO + d);
         const float f = fac[w][i];
         sum.x = fmaf(v.x, f, sum.x);
