@@ -706,9 +706,18 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
   a.part = e->kv8_part;
   a.cnt = e->kv8_cnt;
   a.err = e->err_dev;
-  // Packed rows of an average sequence: past 16 the tcgen05 form, which takes 128 at a time.
+  // Packed rows of an average sequence: past 16 the tcgen05 form, which takes 128 at a time, where there
+  // may be enough to do.  It costs 18 (head size 128) to 21 us (256) before its first tile and this one 6
+  // to 8; a block for 16 rows takes an SM 0.28 us here, and 64 keys for up to 128 rows 1.0 to 1.8 us
+  // there.  The table's width (and the window) bounds the keys, which are on the device.  40 rows of 30
+  // sequences of up to 540 keys: 14.2 us here, 29.4 there (head size 256); of 32 sequences of 8000: 63 and
+  // 43.
+  const uint64_t rows = (uint64_t)tokens * a.gqa;
   const uint64_t avg = (uint64_t)((tokens + c->num_seqs - 1) / c->num_seqs) * a.gqa;
-  if (avg > 16 && c->head_dim <= 256)
+  uint64_t keys = (uint64_t)c->max_pages * c->page_tokens;
+  if (window) keys = std::min<uint64_t>(keys, (uint64_t)window + tokens / c->num_seqs);
+  const bool little = (rows / 16 + c->num_seqs) * c->num_kv * (keys + 128) <= 800ull * e->num_sms;
+  if (avg > 16 && c->head_dim <= 256 && !little)
     return sx_host_cuda_status(sx::launch_kv8_prompt(a, t, e->num_sms, e->stream), "kv8_attn launch");
   const sx::DecVariant v = sx::dec_variant(t, c->head_dim, avg <= 8 ? 0 : 1);
   return sx_host_cuda_status(

@@ -21,6 +21,24 @@ def eng():
     e.close()
 
 
+# Attention of more than 16 packed rows has two forms, and the table's width decides with the rows.
+BOTH_FORMS = """drafts prompts window one_long_prompt strided_rows magnitudes scales_far_apart nan_in_masked_places
+nan_value_only rows_outside_sequences_stay bad_page_masks_and_reports prompts_repeat_bit_for_bit
+repeats_bit_for_bit_on_any_stream_and_in_a_graph scale_zero_and_negative""".split()
+
+
+def pytest_generate_tests(metafunc):
+    if metafunc.function.__name__.removeprefix("test_attn_") in BOTH_FORMS:
+        metafunc.parametrize("table_width", [0, 100000], indirect=True, ids=["narrow", "wide"])
+
+
+@pytest.fixture(autouse=True)
+def table_width(request):
+    Cache.spare_columns = getattr(request, "param", 0)
+    yield
+    Cache.spare_columns = 0
+
+
 # ------------------------------------------------------------------------- the cache in 64 bits
 def codes():
     out = []
@@ -41,6 +59,8 @@ def places(d):
 class Cache:
     """A pool with every page in use: sequences' pages in shuffled order, the rest of the table bad."""
 
+    spare_columns = 0  # of the table: its width says how much there may be to do
+
     def __init__(self, lens, page, hkv, d, seed, first=None, spare=2, fill=1.0):
         g = torch.Generator().manual_seed(seed)
         self.page, self.hkv, self.d, self.lens = page, hkv, d, lens
@@ -48,7 +68,7 @@ class Cache:
         need = [max(0, -(-n // page) - f) for n, f in zip(lens, first)]
         self.pages = sum(need) + spare
         order = torch.randperm(self.pages, generator=g).tolist()
-        width = max([1] + [-(-n // page) for n in lens]) + 1
+        width = max([1] + [-(-n // page) for n in lens]) + 1 + Cache.spare_columns
         rows = []
         for n, f in zip(need, first):
             rows.append([-1] * f + [order.pop() for _ in range(n)] + [-1] * (width - n - f))
