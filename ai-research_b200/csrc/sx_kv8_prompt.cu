@@ -24,15 +24,18 @@
 // What bounds it is the roles' own instructions: at head size 128 a CTA's tile takes 2300 cycles, of
 // which the tensor cores work 650.  Code size and spills count for as much as instructions (a kernel
 // unrolled throughout spent 20 cycles an instruction, fetching), so what runs seldom is out of line, loops
-// stay loops, and what describes a problem or a block is in shared memory.  Measured: 4 prompts of 4096
-// tokens behind 4096 (16 heads of 128, 8 kv heads, bf16) 528 us, 770 TFLOP/s; 4 of 2048 tokens with head
-// size 256 144 us.  Four softmax warps with whole rows took 684 us for the first, a shared barrier for K
-// and V 585.  A second look ahead for pages and scales, and Q brought by the roles that wait for it, were
-// slower (576 and 600 us): more code.
+// stay loops, and what describes a problem or a block is in shared memory.  Measured: 4 prompts of up to
+// 4096 tokens behind 4096 (16 q and 8 kv heads of 128, bf16) 531 us, 760 TFLOP/s or 45 % of the measured
+// rate, at the 1.5 GHz that the power cap leaves; 4 of 2048 tokens with head size 256 132 us; 5 drafts of
+// 32 sequences on up to 16000 keys (8 q heads, 1 kv head of 256) 73.5 us, where 30 tiles a CTA take 37 and
+// cutting the line, bringing Q, the output and the merge the rest.  Four softmax warps with whole rows took
+// 684 us for the first, one barrier for K and V 585.  A second look ahead for pages and scales, and Q
+// brought by the roles that wait for it, were slower (576 and 600 us): more code.
 //
 // Work is the line of sx_kv8_attn.cu with problems of their own length: row group k of a sequence
 // sees pos0 + 128 (k + 1) / G keys at most, so the line counts keys x G, whose sums are closed
-// forms; a tile belongs to the CTA in whose run its first key lies.
+// forms; a tile belongs to the CTA in whose run its first key lies.  Parts of cut problems meet in a
+// second kernel.
 #include "sx_host.h"
 #include "sx_kv8.cuh"
 #include "sx_launch.cuh"

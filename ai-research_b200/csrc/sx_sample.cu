@@ -4,6 +4,8 @@
 // Both walk rows of a vocabulary (1 MiB at 262144 tokens) and are bound by reading them, so a row
 // is spread over a thread-block cluster: its CTAs exchange one partial result each through
 // distributed shared memory, and the row is read once.  Many long rows take two passes instead.
+// Measured, rows of 262144: probabilities of one row 4.6 us, of 40 rows 19.1 (4.4 TB/s); verification of
+// 4 drafts for one sequence 7.2 us, for 64 sequences 26.5 (5.1 TB/s, 78 % of the measured copy rate).
 #include "sx_common.cuh"
 #include "sx_host.h"
 #include "sx_launch.cuh"
