@@ -557,3 +557,13 @@ extern "C" SX_API sx_status sx_dispatch_kv8_append(
                          sx::append_smem(c->head_dim, rotary_dim), e->stream, 1, a),
       "kv8_append launch");
 }
+
+extern "C" SX_API sx_status sx_dispatch_kv8_append_args(sx_engine *e, const sx_kv8_append_args *a) {
+  if (!a) {
+    sx_host_set_error("kv8_append: null arguments");
+    return SX_ERR_INVALID;
+  }
+  return sx_dispatch_kv8_append(e, &a->cache, (sx_dtype)a->dtype, a->q_in, a->k_in, a->v_in, a->q_ld, a->k_ld, a->v_ld,
+                                a->q_norm_w, a->k_norm_w, a->q_out, a->row_start, a->kv_len, a->tokens, a->num_q,
+                                a->inv_freq, a->rotary_dim, a->flags, a->eps);
+}

@@ -734,3 +734,12 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
       sx::launch_chained(v.fn, dim3(std::min(e->num_sms * v.ctas, sx::kMaxParts * sx::kPartGroup)), dim3(sx::kDecThreads), v.smem, e->stream, 1, a),
       "kv8_attn launch");
 }
+
+extern "C" SX_API sx_status sx_dispatch_kv8_attn_args(sx_engine *e, const sx_kv8_attn_args *a) {
+  if (!a) {
+    sx_host_set_error("kv8_attn: null arguments");
+    return SX_ERR_INVALID;
+  }
+  return sx_dispatch_kv8_attn(e, &a->cache, (sx_dtype)a->dtype, a->q, a->out, a->q_ld, a->out_ld, a->row_start,
+                              a->kv_len, a->tokens, a->num_q, a->window, a->scale);
+}

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import weakref
 from pathlib import Path
 
@@ -106,7 +107,7 @@ class KV8(C.Structure):
         num_pages, rest = divmod(data.nbytes, page_tokens * num_kv * 2 * head_dim)
         if rest:
             raise ValueError("KV8: data does not hold whole pages")
-        if scale.numel() != num_pages * num_kv * (page_tokens // 16) * 2 or scale.itemsize != 4:
+        if scale.nbytes != num_pages * num_kv * (page_tokens // 16) * 8 or scale.itemsize != 4:
             raise ValueError("KV8: scale must hold one f32 per record")
         shape = table.shape
         if len(shape) != 2 or table.itemsize != 4:
@@ -114,8 +115,15 @@ class KV8(C.Structure):
         if not (data.is_contiguous() and scale.is_contiguous() and table.is_contiguous()):
             raise ValueError("KV8: data, scale and table must be contiguous")
         self._keep = (data, scale, table)
-        super().__init__(data.data_ptr(), scale.data_ptr(), table.data_ptr(), num_pages,
+        _CACHE.pack_into(self, 0, data.data_ptr(), scale.data_ptr(), table.data_ptr(), num_pages,
                          page_tokens, shape[1], shape[0], num_kv, head_dim)
+
+
+# The fields of sx_kv8, and those of sx_kv8_append_args and sx_kv8_attn_args after their cache: packed,
+# as ctypes takes a tenth of a microsecond for each field and argument.
+_CACHE = struct.Struct("@3Q6I")
+_APPEND_ARGS = struct.Struct("@9Q8If")
+_ATTN_ARGS = struct.Struct("@4Q6If")
 
 
 class TpShard(C.Structure):
@@ -327,6 +335,8 @@ _SIGS = {
     "sx_pages_table": (_P, [_P]),
     "sx_dispatch_kv8_append": (_S, [_P, C.POINTER(KV8), _I, _P, _P, _P, _U32, _U32, _U32, _P, _P,
                                     _P, _P, _P, _U32, _U32, _P, _U32, _U32, _F]),
+    "sx_dispatch_kv8_append_args": (_S, [_P, C.c_char_p]),
+    "sx_dispatch_kv8_attn_args": (_S, [_P, C.c_char_p]),
     "sx_dispatch_kv8_attn": (_S, [_P, C.POINTER(KV8), _I, _P, _P, _U32, _U32, _P, _P, _U32, _U32,
                                   _U32, _F]),
     "sx_dispatch_probs": (_S, [_P, _P, _U32, _P, _U32, _U32, _U32, _F]),
@@ -656,21 +666,25 @@ class Engine:
                    k_eq_v=False, eps=1e-6, q_ld=0, k_ld=0, v_ld=0):
         """sx_dispatch_kv8_append: norm, rotation and quantised append of `tokens` rows (row
         strides in elements; 0: contiguous rows)."""
-        kv = cache.num_kv * cache.head_dim
-        check(lib().sx_dispatch_kv8_append(
-            self.h, C.byref(cache), dtype, _ptr(q_in), _ptr(k_in), _ptr(v_in),
-            q_ld or num_q * cache.head_dim, k_ld or kv, v_ld or kv, _ptr(q_norm_w),
-            _ptr(k_norm_w), _ptr(q_out), _ptr(row_start), _ptr(kv_len), tokens, num_q,
-            _ptr(inv_freq), rotary_dim,
-            (KV8_V_NORM if v_norm else 0) | (KV8_K_EQ_V if k_eq_v else 0), eps))
+        d = cache.head_dim
+        kv = cache.num_kv * d
+        status = lib().sx_dispatch_kv8_append_args(self.h, bytes(cache) + _APPEND_ARGS.pack(
+            _ptr(q_in) or 0, _ptr(k_in) or 0, _ptr(v_in) or 0, _ptr(q_norm_w) or 0,
+            _ptr(k_norm_w) or 0, _ptr(q_out) or 0, _ptr(row_start) or 0, _ptr(kv_len) or 0,
+            _ptr(inv_freq) or 0, dtype, q_ld or num_q * d, k_ld or kv, v_ld or kv, tokens, num_q,
+            rotary_dim, (KV8_V_NORM if v_norm else 0) | (KV8_K_EQ_V if k_eq_v else 0), eps))
+        if status:
+            check(status)
 
     def kv8_attn(self, cache: "KV8", dtype, q, out, row_start, kv_len, tokens, num_q, scale,
                  window=0, q_ld=0, out_ld=0):
         """sx_dispatch_kv8_attn: attention of `tokens` rows over the paged 8-bit cache."""
         row = num_q * cache.head_dim
-        check(lib().sx_dispatch_kv8_attn(
-            self.h, C.byref(cache), dtype, _ptr(q), _ptr(out), q_ld or row, out_ld or row,
-            _ptr(row_start), _ptr(kv_len), tokens, num_q, window, scale))
+        status = lib().sx_dispatch_kv8_attn_args(self.h, bytes(cache) + _ATTN_ARGS.pack(
+            _ptr(q) or 0, _ptr(out) or 0, _ptr(row_start) or 0, _ptr(kv_len) or 0, dtype,
+            q_ld or row, out_ld or row, tokens, num_q, window, scale))
+        if status:
+            check(status)
 
     def probs(self, logits, probs, rows, n, temperature=1.0, logits_ld=0, probs_ld=0):
         """sx_dispatch_probs: softmax(logits / temperature) of f32 rows."""

@@ -607,6 +607,29 @@ SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, sx_dtype t,
                                       uint32_t tokens, uint32_t num_q, uint32_t window,
                                       float scale);
 
+/* The two calls with their arguments in one block, for bindings that pay for each argument (Python's
+ * ctypes: 2 us of a 10 us append). */
+typedef struct {
+  sx_kv8 cache;
+  const void *q_in, *k_in, *v_in;
+  const float *q_norm_w, *k_norm_w;
+  void *q_out;
+  const uint32_t *row_start, *kv_len;
+  const float *inv_freq;
+  uint32_t dtype, q_ld, k_ld, v_ld, tokens, num_q, rotary_dim, flags;
+  float eps;
+} sx_kv8_append_args;
+typedef struct {
+  sx_kv8 cache;
+  const void *q;
+  void *out;
+  const uint32_t *row_start, *kv_len;
+  uint32_t dtype, q_ld, out_ld, tokens, num_q, window;
+  float scale;
+} sx_kv8_attn_args;
+SX_API sx_status sx_dispatch_kv8_append_args(sx_engine *e, const sx_kv8_append_args *a);
+SX_API sx_status sx_dispatch_kv8_attn_args(sx_engine *e, const sx_kv8_attn_args *a);
+
 /* probs[r] = softmax(logits[r] / temperature) for `rows` rows of n f32 (strides in floats, 0: n);
  * temperature 1e-30 .. 1e30.  A row of -inf alone gives zeros; a NaN or +inf gives NaN.  In place allowed
  * when the strides are equal. */
