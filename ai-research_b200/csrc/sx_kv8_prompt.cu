@@ -69,8 +69,10 @@ struct PromptShape {
   static_assert(kO + D <= 512 && kCols * kCtas <= 512, "tensor memory");
 };
 
-// What starting and ending a problem costs, in tiles (10 000 cycles, and a tile takes 3000).
-constexpr uint32_t kPromptOver = 3;
+// What starting and ending a problem costs, in tiles (10 000 cycles, and a tile takes 3000); what cutting
+// one costs, a second start and an end that leaves a part (3 prompts of 361 tokens, head size 256 and a
+// window of 191: 27.8 us uncut, 42.5 cut; 4 of 1500 in a window of 300, head size 128: 48.8 and 60.4).
+constexpr uint32_t kPromptOver = 3, kCutTiles = 16;
 
 // Costs on the line: keys x G of a row group, at most `cap` with a window, plus `over`.
 struct GroupCost {
@@ -199,6 +201,7 @@ struct Schedule {
   uint64_t unit, begin, end, length, at, step;  // at: where the problem starts, step: its length
   uint32_t b, left, head, group;                // next sequence; problems left of the one before
   bool fresh;  // the first sequence: its first problems may lie before the run
+  bool uncut;  // problems go whole to the CTA in whose run they start
   Kv8Rows r;
   GroupCost gc;
 
@@ -210,7 +213,7 @@ struct Schedule {
     k.groups = (x.n * a.gqa + kRows - 1) / kRows;
     return k;
   }
-  SX_DEV uint64_t cost(const Kv8AttnArgs &a, uint32_t i) const {
+  SX_DEV uint64_t cost(const Kv8AttnArgs &a, uint32_t i, uint32_t &problems, uint64_t &longest) const {
     Kv8Rows x;
     if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, i, &x)) {
       if (blockIdx.x == 0) raise_error(a.err, kDevBadParams);
@@ -218,6 +221,8 @@ struct Schedule {
     }
     if (x.n == 0) return 0;
     const GroupCost k = cost_of(a, x);
+    problems += k.groups * a.c.num_kv;
+    longest = max(longest, k.of(k.groups - 1) - k.over);
     return k.before(k.groups) * a.c.num_kv;
   }
   __device__ __noinline__ void start(const Kv8AttnArgs &a, uint32_t tokens) {
@@ -225,8 +230,9 @@ struct Schedule {
     unit = (uint64_t)a.gqa * tokens;
     const uint32_t per = (a.c.num_seqs + 31) / 32;
     const uint32_t b0 = lane * per, b1 = min(a.c.num_seqs, b0 + per);
-    uint64_t mine = 0;
-    for (uint32_t i = b0; i < b1; ++i) mine += cost(a, i);
+    uint64_t mine = 0, longest = 0;
+    uint32_t problems = 0;
+    for (uint32_t i = b0; i < b1; ++i) mine += cost(a, i, problems, longest);
     uint64_t incl = mine;
 #pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
@@ -236,13 +242,17 @@ struct Schedule {
     const uint64_t total = __shfl_sync(0xffffffffu, incl, 31);
     length = (total + gridDim.x - 1) / gridDim.x;
     length = length > a.min_run * unit ? length : a.min_run * unit;
+    problems = __reduce_add_sync(0xffffffffu, problems);
+#pragma unroll 1
+    for (int o = 16; o > 0; o >>= 1) longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, o));
+    uncut = longest <= kCutTiles * unit + (problems <= gridDim.x ? length : 0);
     begin = length * blockIdx.x;
     end = begin + length < total ? begin + length : total;
     const uint32_t who = min(31, __popc(__ballot_sync(0xffffffffu, incl <= begin)));
     at = incl - mine;
     b = b0;
     if (lane == (int)who && begin < end)
-      for (uint64_t n; (n = cost(a, b)) <= begin - at; at += n) ++b;
+      for (uint64_t n; (n = cost(a, b, problems, longest)) <= begin - at; at += n) ++b;
     at = __shfl_sync(0xffffffffu, at, who);
     b = __shfl_sync(0xffffffffu, b, who);
     if (begin >= end) at = end;  // no run for this CTA
@@ -302,10 +312,12 @@ struct Schedule {
       p.t0 = begin > at ? (uint32_t)((begin - at + unit - 1) / unit) : 0;
       const uint64_t until = (end - at + unit - 1) / unit;
       p.t1 = until < count ? (uint32_t)until : count;
+      if (uncut) p.t1 = p.t0 == 0 ? count : 0;
       if (p.t0 >= p.t1) continue;  // no tile starts in the run
       // CTAs c0 .. c1 hold parts of this problem
       p.c0 = (uint32_t)(at / length);
       p.parts = (uint32_t)((at + (count - 1) * unit) / length) - p.c0 + 1;
+      if (uncut) p.parts = 1;
       p.slot = 2 * blockIdx.x + (at > begin ? 1 : 0);
       p.slot0 = 2 * p.c0 + (at > length * p.c0 ? 1 : 0);
       p.more = 1;
