@@ -22,16 +22,16 @@
 // bulk copies (a K or a V record a stage) and its own maximum, sum and output; they merge in shared
 // memory at the end of a problem, and CTAs that share a problem through the workspace: the last to
 // arrive merges (its order is that of the CTAs, so results repeat).  Runs are of 8 blocks at least, one
-// per warp (640 keys of one head of 256: 11.9 us; with 16 or 32, or uncut, 14.0).  Problems of up to three
+// per warp (640 keys of one head of 256: 11.6 us; with 16 or 32, or uncut, 2 more).  Problems of up to three
 // such steps more than a run are not cut, since a merge costs as much (16 rows in a window of 512:
-// 20.3 us; cut 25.3).
+// 19.3 us; cut 25.3).
 //
-// Measured: 64 rows on up to 8192 keys (16 q and 8 kv heads of 256, bf16) 199 us, 5.5 TB/s or 85 % of the
+// Measured: 64 rows on up to 8192 keys (16 q and 8 kv heads of 256, bf16) 187 us, 5.8 TB/s or 90 % of the
 // measured copy rate, the rest being starts and ends of 512 problems, where a CTA's copies run dry; 131k
-// keys of 8 heads of 128 for one f32 row 58 us (72 %); heads of 512 95 %, of 128 77 %, of 64 51 % (a block
-// of 16 tokens costs as many instructions of softmax for a quarter of the bytes).  Two or four blocks a
-// warp at a time were slower below 256: 116 us for 110 with head size 128, 15.9 for 5.5 on 127 keys with
-// 64.
+// keys of 8 heads of 128 for one f32 row 55 us (76 %); batches of heads of 512 100 %, of 128 79 %, of 64
+// 50 % (a block of 16 tokens costs as many instructions of softmax for a quarter of the bytes).  Two or
+// four blocks a warp at a time were slower below 256: 116 us for 110 with head size 128, 15.9 for 5.5 on
+// 127 keys with 64.  So were three or four CTAs an SM (89 and 106 us for 84 with 64).
 #include "sx_host.h"
 #include "sx_kv8.cuh"
 #include "sx_launch.cuh"
@@ -66,7 +66,10 @@ struct DecShape {
   static constexpr int kPieces = D / 32;
   static constexpr int kCtas = D * NT <= 256 ? 2 : 1;         // per SM
   static constexpr int kRecord = 16 * D;
-  static constexpr int kRing = (kCtas == 2 ? 12 : 24) * 1024; // of one warp
+  // Of one warp: an SM has 128 KB on their way, three times what the copy rate needs.  Half as much again
+  // only queues, and every other load behind it: 12 and 24 KB took 200 us for 187 in full batches of 256,
+  // 177 for 168 with 512.
+  static constexpr int kRing = (kCtas == 2 ? 8 : 16) * 1024;
   static constexpr int kStages = kRing / kRecord;
   static constexpr int kLdO = D + 4;
   static constexpr int kMerge = kDecWarps * kRows * kLdO * 4; // shares the rings' memory
