@@ -26,7 +26,7 @@
 // unrolled throughout spent 20 cycles an instruction, fetching), so what runs seldom is out of line, loops
 // stay loops, and what describes a problem or a block is in shared memory.  Measured: 4 prompts of up to
 // 4096 tokens behind 4096 (16 q and 8 kv heads of 128, bf16) 531 us, 760 TFLOP/s or 45 % of the measured
-// rate, at the 1.5 GHz that the power cap leaves; 4 of 2048 tokens with head size 256 132 us; 5 drafts of
+// rate, at the 1.5 GHz that the power cap leaves; 4 of 2048 tokens with head size 256 128 us; 5 drafts of
 // 32 sequences on up to 16000 keys (8 q heads, 1 kv head of 256) 73.5 us, where 30 tiles a CTA take 37 and
 // cutting the line, bringing Q, the output and the merge the rest.  Four softmax warps with whole rows took
 // 684 us for the first, one barrier for K and V 585.  A second look ahead for pages and scales, and Q
@@ -646,18 +646,59 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       float *const po = part_values(a, gridDim.x) + at * D;
       T *const out = static_cast<T *>(a.out) + pr.row(a, i) * a.out_ld + pr.col(a, i);
       const float inv = whole ? (l == 0.0f ? 0.0f : 1.0f / l) : 1.0f;
+      // Whole rows with one CTA an SM go 64 bytes at a time through shared memory (over the K tiles, which
+      // have been read), so that four lanes store them together: a lane's own row is a line of its own
+      // for every 16 bytes.  (Prompts of 2048 with head size 256 128 us for 133; with two CTAs the
+      // registers cost the loop more, 547 us for 534 in the long prompts.)
+      constexpr bool kTogether = P::kCtas == 1;
+      constexpr uint32_t kPiece = 64 / sizeof(T);
+      T *dst[4];  // the rows that this lane stores then
+      if constexpr (kTogether) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          dst[k] = reinterpret_cast<T *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(out), 8 * k + lane / 4)) +
+                   lane % 4 * (kPiece / 4);
+      }
+      const uint32_t stage = k_tile(0) + warp * (32 * 80);
       if (!whole && half == 0 && i < rows) reinterpret_cast<float2 *>(a.part)[at] = make_float2(ref, l);
 #pragma unroll 1
-      for (int d = half * (D / 2); d < (int)(half + 1) * (D / 2); d += 32) {
+      for (int d = half * (D / 2); d < (int)(half + 1) * (D / 2) && 32u * (warp & 3) < rows; d += 32) {
         uint32_t o[32];
         tmem_ld32(tmem + lanes + P::kO + d, o);
         tmem_wait_ld(o);
-        if (i < rows) {
-          // element 4 g + i of the piece is column 8 i + f(g), f(g) = g / 2 + 4 (g % 2)
-          float y[32];
+        // element 4 g + i of the piece is column 8 i + f(g), f(g) = g / 2 + 4 (g % 2)
+        float y[32];
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            y[k] = __uint_as_float(o[8 * (k & 3) + ((k >> 2) >> 1) + 4 * ((k >> 2) & 1)]) * inv;
+        for (int k = 0; k < 32; ++k)
+          y[k] = __uint_as_float(o[8 * (k & 3) + ((k >> 2) >> 1) + 4 * ((k >> 2) & 1)]) * inv;
+        if (kTogether && whole) {
+#pragma unroll
+          for (uint32_t h = 0; h < 32; h += kPiece) {
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+              uint32_t w[4];
+#pragma unroll
+              for (uint32_t e = 0; e < 4; ++e) {
+                if constexpr (kSplit) {
+                  w[e] = __float_as_uint(y[h + 4 * k + e]);
+                } else {
+                  const __nv_bfloat162 b = __floats2bfloat162_rn(y[8 * k + 2 * e], y[8 * k + 2 * e + 1]);
+                  w[e] = *reinterpret_cast<const uint32_t *>(&b);
+                }
+              }
+              st_shared16(stage + lane * 80 + 16 * k, w);
+            }
+            __syncwarp();
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+              uint32_t w[4];
+              ld_shared16(stage + (8 * k + lane / 4) * 80 + 16 * (lane % 4), w);
+              if (32 * (warp & 3) + 8 * k + lane / 4 < rows)
+                *reinterpret_cast<uint4 *>(dst[k] + d + h) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            __syncwarp();
+          }
+        } else if (i < rows) {
           if (whole) {
             constexpr int kVec = 16 / (int)sizeof(T);
 #pragma unroll
