@@ -41,7 +41,10 @@ namespace {
 
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
-constexpr uint32_t kOverhead = 8;  // blocks a problem's start and end are worth
+// Blocks that starting and ending a problem is worth.  With 8, 16, 24, 32 and 48: full batches of head size
+// 256 186, 180, 181, 180 and 183 us, of 128 106, 99, 91, 90 and 91, drafts of two heads of 256 115, 108, 93,
+// 90 and 93.
+constexpr uint32_t kOverhead = 32;
 constexpr uint32_t kMergeSteps = 3;  // steps (a block a warp) that a merge over CTAs is worth
 constexpr float kPOffset = 10.0f;
 constexpr uint32_t kMaxParts = 32, kPartGroup = 16;  // merged at once; of a first level
