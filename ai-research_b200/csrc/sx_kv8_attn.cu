@@ -26,10 +26,10 @@
 // such steps more than a run are not cut, since a merge costs as much (16 rows in a window of 512:
 // 19.3 us; cut 25.3).
 //
-// Measured: 64 rows on up to 8192 keys (16 q and 8 kv heads of 256, bf16) 187 us, 5.8 TB/s or 90 % of the
+// Measured: 64 rows on up to 8192 keys (16 q and 8 kv heads of 256, bf16) 180 us, 6.0 TB/s or 94 % of the
 // measured copy rate, the rest being starts and ends of 512 problems, where a CTA's copies run dry; 131k
-// keys of 8 heads of 128 for one f32 row 55 us (76 %); batches of heads of 512 100 %, of 128 79 %, of 64
-// 50 % (a block of 16 tokens costs as many instructions of softmax for a quarter of the bytes).  Two or
+// keys of 8 heads of 128 for one f32 row 53 us (79 %); batches of heads of 512 102 %, of 128 93 %, of 64
+// 57 % (a block of 16 tokens costs as many instructions of softmax for a quarter of the bytes).  Two or
 // four blocks a warp at a time were slower below 256: 116 us for 110 with head size 128, 15.9 for 5.5 on
 // 127 keys with 64.  So were three or four CTAs an SM (89 and 106 us for 84 with 64).
 #include "sx_host.h"

@@ -25,12 +25,12 @@
 // which the tensor cores work 650.  Code size and spills count for as much as instructions (a kernel
 // unrolled throughout spent 20 cycles an instruction, fetching), so what runs seldom is out of line, loops
 // stay loops, and what describes a problem or a block is in shared memory.  Measured: 4 prompts of up to
-// 4096 tokens behind 4096 (16 q and 8 kv heads of 128, bf16) 531 us, 760 TFLOP/s or 45 % of the measured
-// rate, at the 1.5 GHz that the power cap leaves; 4 of 2048 tokens with head size 256 128 us; 5 drafts of
-// 32 sequences on up to 16000 keys (8 q heads, 1 kv head of 256) 73.5 us, where 30 tiles a CTA take 37 and
+// 4096 tokens behind 4096 (16 q and 8 kv heads of 128, bf16) 520 us, 780 TFLOP/s or 46 % of the measured
+// rate, at the 1.5 GHz that the power cap leaves; 4 of 2048 tokens with head size 256 111.5 us; 5 drafts of
+// 32 sequences on up to 16000 keys (8 q heads, 1 kv head of 256) 58.5 us, where 30 tiles a CTA take 37 and
 // cutting the line, bringing Q, the output and the merge the rest.  Four softmax warps with whole rows took
 // 684 us for the first, one barrier for K and V 585.  A second look ahead for pages and scales, and Q
-// brought by the roles that wait for it, were slower (576 and 600 us): more code.
+// brought by the roles that wait for it, were slower by 5 and 10 %: more code.
 //
 // Work is the line of sx_kv8_attn.cu with problems of their own length: row group k of a sequence
 // sees pos0 + 128 (k + 1) / G keys at most, so the line counts keys x G, whose sums are closed
@@ -69,10 +69,11 @@ struct PromptShape {
   static_assert(kO + D <= 512 && kCols * kCtas <= 512, "tensor memory");
 };
 
-// What starting and ending a problem costs, in tiles (10 000 cycles, and a tile takes 3000); what cutting
-// one costs, a second start and an end that leaves a part (3 prompts of 361 tokens, head size 256 and a
-// window of 191: 27.8 us uncut, 42.5 cut; 4 of 1500 in a window of 300, head size 128: 48.8 and 60.4).
-constexpr uint32_t kPromptOver = 3, kCutTiles = 16;
+// What starting and ending a problem costs, in tiles of 2400 cycles (with 3, 6, 8, 10 and 16: drafts over
+// 16000 keys 74, 60, 58.5, 57.5 and 59 us; prompts of 2048 with head size 256 129, 115, 111.5, 113 and 122).
+// What cutting one costs, a second start and an end that leaves a part (4 prompts of 1500 in a window of
+// 300, head size 128: 48.8 us uncut, 60.4 cut).
+constexpr uint32_t kPromptOver = 8, kCutTiles = 16;
 
 // Costs on the line: keys x G of a row group, at most `cap` with a window, plus `over`.
 struct GroupCost {
