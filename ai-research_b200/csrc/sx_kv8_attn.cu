@@ -723,11 +723,11 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
   a.cnt = e->kv8_cnt;
   a.err = e->err_dev;
   // Packed rows of an average sequence: past 16 the tcgen05 form, which takes 128 at a time, where there
-  // may be enough to do.  It costs 18 (head size 128) to 21 us (256) before its first tile and this one 6
-  // to 8; a block for 16 rows takes an SM 0.28 us here, and 64 keys for up to 128 rows 1.0 to 1.8 us
-  // there.  The table's width (and the window) bounds the keys, which are on the device.  40 rows of 30
-  // sequences of up to 540 keys: 14.2 us here, 29.4 there (head size 256); of 32 sequences of 8000: 63 and
-  // 43.
+  // may be enough to do: its smallest call takes 12.5 (head size 128) to 14 us (256), this form's 7 to 8, but
+  // this one reads a key once for 16 rows.  The table's width (and the window) bounds the keys, which are
+  // on the device.  40 rows of 30 sequences of up to 540 keys 14.3 us here, 23.3 there (head size 256); of
+  // 32 sequences of 8000 49.7 and 37.9; at the limit, 64 rows and 2 kv heads of 30 sequences of 540 keys,
+  // 28.0 and 23.5 (256), 18.1 and 20.3 (128).
   const uint64_t rows = (uint64_t)tokens * a.gqa;
   const uint64_t avg = (uint64_t)((tokens + c->num_seqs - 1) / c->num_seqs) * a.gqa;
   uint64_t keys = (uint64_t)c->max_pages * c->page_tokens;
