@@ -22,13 +22,13 @@
 // bulk copies (a K or a V record a stage) and its own maximum, sum and output; they merge in shared
 // memory at the end of a problem, and CTAs that share a problem through the workspace: the last to
 // arrive merges (its order is that of the CTAs, so results repeat).  Runs are of 8 blocks at least, one
-// per warp (640 keys of one head of 256: 11.6 us; with 16 or 32, or uncut, 2 more).  Problems of up to three
+// per warp (640 keys of one head of 256: 11.8 us; with 16 or 32, or uncut, 2 more).  Problems of up to three
 // such steps more than a run are not cut, since a merge costs as much (16 rows in a window of 512:
-// 19.3 us; cut 25.3).
+// 20 us; cut 25.3).
 //
 // Measured: 64 rows on up to 8192 keys (16 q and 8 kv heads of 256, bf16) 180 us, 6.0 TB/s or 94 % of the
 // measured copy rate, the rest being starts and ends of 512 problems, where a CTA's copies run dry; 131k
-// keys of 8 heads of 128 for one f32 row 53 us (79 %); batches of heads of 512 102 %, of 128 93 %, of 64
+// keys of 8 heads of 128 for one f32 row 54.5 us (76 %); batches of heads of 512 102 %, of 128 93 %, of 64
 // 57 % (a block of 16 tokens costs as many instructions of softmax for a quarter of the bytes).  Two or
 // four blocks a warp at a time were slower below 256: 116 us for 110 with head size 128, 15.9 for 5.5 on
 // 127 keys with 64.  So were three or four CTAs an SM (89 and 106 us for 84 with 64).
@@ -408,11 +408,14 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
 
       // ---- S^T = K Q^T
       // (two chains of accumulators: an MMA's result is 24 cycles away)
-      float s[NT][2][4];
+      // (the small terms apart: the tensor core cuts off a sum's last bits at every addition, and one chain
+      // for both left 1.6e-6 of one f32 row's output on 640 keys for 0.4e-6, at 1 to 4 % less time)
+      constexpr int kChains = kSplit ? 4 : 2;
+      float s[NT][kChains][4];
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
+        for (int w = 0; w < kChains; ++w)
 #pragma unroll
           for (int k = 0; k < 4; ++k) s[t][w][k] = 0.0f;
 #pragma unroll
@@ -428,8 +431,8 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
 #pragma unroll
           for (int w = 0; w < (kSplit ? 2 : 1); ++w) {
             const uint4 q = *reinterpret_cast<const uint4 *>(qf + w * (S::kQ / 2) + (t * kPieces + p) * 512 + lane * 16);
-            mma_f16_16816(s[t][0], a0, q.x, q.y);
-            mma_f16_16816(s[t][1], a1, q.z, q.w);
+            mma_f16_16816(s[t][2 * w], a0, q.x, q.y);
+            mma_f16_16816(s[t][2 * w + 1], a1, q.z, q.w);
           }
       }
 
@@ -442,7 +445,11 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[t][0][k] = fmaf((s[t][0][k] + s[t][1][k]) * ks, mul[t][k & 1], lv);
+        for (int k = 0; k < 4; ++k) {
+          float x = s[t][0][k] + s[t][1][k];
+          if constexpr (kSplit) x += s[t][2][k] + s[t][3][k];
+          s[t][0][k] = fmaf(x * ks, mul[t][k & 1], lv);
+        }
       const uint32_t key0 = (first + block_of(step)) * kKv8Block;
       if (!have || key0 < all_lo || key0 + kKv8Block - 1 > all_hi) {
         // Some row does not see all of the block.  A token no row sees is taken out of V (its
