@@ -13,26 +13,17 @@
 
 #include "../../include/sx.h"
 #include "sx_common.cuh"
+#include "sx_kv8_units.h"
 
 namespace sx {
 
-constexpr int kKv8Block = 16;      // tokens per record
 constexpr int kKv8MinExp = -60, kKv8MaxExp = 60;
 constexpr uint32_t kKv8MaxSeqs = 4096;
 
-// Rows of sequence b: [r0, r0 + n), its length with them.
-struct Kv8Rows {
-  uint32_t r0, n, len;
-};
-
-// False when the rows or the length do not fit (include/sx.h: the sequence is skipped).
+// Rows of sequence b; false when they do not fit.
 SX_DEV bool kv8_rows(const sx_kv8 &c, const uint32_t *row_start, const uint32_t *kv_len,
                      uint32_t tokens, uint32_t b, Kv8Rows *r) {
-  const uint32_t r0 = row_start[b], r1 = row_start[b + 1];
-  r->r0 = r0;
-  r->n = r1 - r0;
-  r->len = kv_len[b];
-  return r0 <= r1 && r1 <= tokens && r->n <= r->len && r->len <= c.max_pages * c.page_tokens;
+  return kv8_rows_fit(row_start[b], row_start[b + 1], kv_len[b], tokens, c.max_pages * c.page_tokens, r);
 }
 
 // The last b < n with key(b) <= u (0 if there is none); key rises with b.  A whole warp calls it:

@@ -5,11 +5,9 @@
 //   q', k' = R(pos) (x / rms(x) * gain),  v' = v / rms(v),  stored = rn_e4m3(x' 2^-e),
 //   e = min { e : max |record| <= 448 2^e }
 //
-// A record belongs to one CTA, which sees all of its new tokens, so the scale needs no atomics:
-// unit u is one 16-token block of one sequence, a CTA takes one unit and a group of kv heads with
-// their q heads.  With sequence b's rows at row_start[b], units row_start[b] / 16 + 2 b .. belong to
-// it: n rows touch at most n / 16 + 2 blocks, so the grid follows from the row and sequence counts
-// alone and nothing is read back.
+// A record belongs to one CTA, which sees all of its new tokens, so the scale needs no atomics: a CTA
+// takes one unit (sx_kv8_units.h), a 16-token block of one sequence, and a group of kv heads with their
+// q heads.  The grid follows from the row and sequence counts alone and nothing is read back.
 //
 // Bound by the rows' bytes, and close behind by instructions: a vector of 256 has 45 cycles of an SM
 // at the copy rate.  Half a warp takes a vector (a token of the unit each, when all 16 are new):
@@ -217,9 +215,7 @@ SX_DEV void transpose4(uint32_t (&w)[4]) {
   w[3] = prmt(c, d, 0x7632);
 }
 
-// One 16-token block of one sequence.
-struct Unit {
-  uint32_t row0, cnt, t0;  // its new rows, how many, the first one's place in the block
+struct Unit : Kv8Unit {
   uint32_t page, in_page;  // page and block of the page
 };
 
@@ -380,6 +376,15 @@ SX_DEV void append_heads(const AppendArgs &a, const Unit &u, uint32_t h0, uint32
   }
 }
 
+// The owners' search needs a row_start that rises, up to `tokens`: the grid's last CTA looks at all of it.
+// (In every CTA that took 5 % of long prompts' time and 0.5 us of a small call's 6.3.)
+__device__ __noinline__ void report_falls(const uint32_t *row_start, uint32_t seqs, uint32_t tokens, uint32_t *err) {
+  for (uint32_t i = threadIdx.x; i < seqs; i += kAppThreads) {
+    const uint32_t r0 = row_start[i], r1 = row_start[i + 1];
+    if (r0 > r1 || r1 > tokens) raise_error(err, kDevBadParams);
+  }
+}
+
 template <typename T, int D, TurnMode MODE>
 __global__ void __launch_bounds__(kAppThreads, D * sizeof(T) <= 512 ? 4 : D <= 256 ? 3 : 2)
     kv8_append_kernel(AppendArgs a) {
@@ -389,23 +394,20 @@ __global__ void __launch_bounds__(kAppThreads, D * sizeof(T) <= 512 ? 4 : D <= 2
   pdl_wait();
 
   const uint32_t u = blockIdx.x;
-  const uint32_t b = warp_last_le(a.c.num_seqs, u, [&](uint32_t i) { return a.row_start[i] / 16 + 2 * i; });
+  if (u == gridDim.x - 1) {
+    report_falls(a.row_start, a.c.num_seqs, a.tokens, a.err);
+    return;
+  }
+  const uint32_t b = warp_last_le(a.c.num_seqs, u, [&](uint32_t i) { return kv8_unit_base(a.row_start[i], i); });
   Kv8Rows r;
   if (!kv8_rows(a.c, a.row_start, a.kv_len, a.tokens, b, &r)) {
     if (threadIdx.x == 0) raise_error(a.err, kDevBadParams);
     return;
   }
-  const uint32_t pos0 = r.len - r.n;  // position of the sequence's first new row
-  const uint32_t rel = u - (r.r0 / 16 + 2 * b);
-  const uint32_t blk = pos0 / kKv8Block + rel;
-  if (r.n == 0 || blk * kKv8Block >= r.len) return;
-  const uint32_t lo = max(pos0, blk * kKv8Block), hi = min(r.len, (blk + 1) * kKv8Block);
   Unit unit;
-  unit.row0 = r.r0 + (lo - pos0);
-  unit.cnt = hi - lo;
-  unit.t0 = lo % kKv8Block;
-  unit.page = a.c.table[(size_t)b * a.c.max_pages + blk * kKv8Block / a.c.page_tokens];
-  unit.in_page = blk % (a.c.page_tokens / kKv8Block);
+  if (!kv8_unit(r, u - kv8_unit_base(r.r0, b), &unit)) return;
+  unit.page = a.c.table[(size_t)b * a.c.max_pages + unit.block * kKv8Block / a.c.page_tokens];
+  unit.in_page = unit.block % (a.c.page_tokens / kKv8Block);
   if (unit.page >= a.c.num_pages) {
     if (threadIdx.x == 0) raise_error(a.err, kDevBadSlot);
     return;
@@ -413,11 +415,11 @@ __global__ void __launch_bounds__(kAppThreads, D * sizeof(T) <= 512 ? 4 : D <= 2
 
   float *const q_w = reinterpret_cast<float *>(sh + append_tile_bytes(D, MODE == kTurnMemory)), *const k_w = q_w + D;
   float *const angles = k_w + D;
-  const uint32_t half = a.rot / 2;
+  const uint32_t half = a.rot / 2, pos = unit.block * kKv8Block + unit.t0;
   for (uint32_t i = threadIdx.x; i < unit.cnt * half; i += blockDim.x) {
     const uint32_t t = i / half, f = i - t * half;
     float s, c;
-    sincosf(__fmul_rn((float)(lo + t), a.inv_freq[f]), &s, &c);
+    sincosf(__fmul_rn((float)(pos + t), a.inv_freq[f]), &s, &c);
     angles[t * a.rot + f] = c;
     angles[t * a.rot + half + f] = s;
   }
@@ -546,12 +548,12 @@ extern "C" SX_API sx_status sx_dispatch_kv8_append(
   a.err = e->err_dev;
   // All kv heads of a unit in one CTA compute its angles once; with few units the heads are spread
   // until every SM has work.
-  const uint32_t units = tokens / sx::kKv8Block + 2 * c->num_seqs;
+  const uint32_t units = sx::kv8_unit_count(tokens, c->num_seqs);
   a.heads_per_cta = c->num_kv;
   while (a.heads_per_cta > 1 && (uint64_t)units * ((c->num_kv + a.heads_per_cta - 1) / a.heads_per_cta) <
                                     12ull * e->num_sms)
     a.heads_per_cta = (a.heads_per_cta + 1) / 2;
-  const dim3 grid(units, (c->num_kv + a.heads_per_cta - 1) / a.heads_per_cta);
+  const dim3 grid(units + 1, (c->num_kv + a.heads_per_cta - 1) / a.heads_per_cta);
   return sx_host_cuda_status(
       sx::launch_chained(sx::append_kernel(t, c->head_dim, rotary_dim / 2), grid, dim3(sx::kAppThreads),
                          sx::append_smem(c->head_dim, rotary_dim), e->stream, 1, a),

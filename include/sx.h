@@ -578,9 +578,11 @@ typedef struct {
  * over what it holds; when new tokens raise it the older ones are rounded again to the new scale
  * (exact but for e4m3 subnormals), and a record whose first token is new starts empty: its scale
  * is the new tokens' and the slots after them hold zeros.  A NaN is stored as NaN and an infinity
- * as the largest value.  Sequences whose rows or length do not fit (row_start falling or past
- * `tokens`, more rows than kv_len, kv_len past the table, page id >= num_pages) are skipped and
- * raise SX_ERR_DEVICE at the next sx_engine_sync.  One call must not name a page twice among the
+ * as the largest value.  Rows before row_start[0] and past the last sequence's belong to nobody:
+ * a part of a larger batch keeps its place in the row arrays.  Sequences whose rows or length do not
+ * fit (falling or past `tokens`, more rows than kv_len, kv_len past the table, page id >= num_pages)
+ * are skipped and raise SX_ERR_DEVICE at the next sx_engine_sync; where row_start falls, other
+ * sequences of that call may be left out too, in whole or in part.  One call must not name a page twice among the
  * pages it writes.  Vectors 16-byte aligned, strides multiples of 16 bytes. */
 SX_API sx_status sx_dispatch_kv8_append(sx_engine *e, const sx_kv8 *c, sx_dtype t,
                                         const void *q_in, const void *k_in, const void *v_in,

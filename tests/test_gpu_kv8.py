@@ -676,3 +676,61 @@ def test_append_refusals(eng):
         assert e.value.status == sx.SX_ERR_INVALID, bad
     call(tokens=0)
     eng.sync()
+
+
+@pytest.mark.parametrize("rot", [0, 64])
+@pytest.mark.parametrize("lead", [1, 15, 16, 17, 32, 100])
+def test_append_rows_before_the_first_sequence(eng, lead, rot):
+    """A part of a batch: row_start does not begin at 0, and the rows before it belong to nobody."""
+    news, lens, d, hq, hkv = [1, 20, 3], [150, 120, 64], 64, 4, 2
+    n = sum(news)
+    a, b = (Cache(lens, 16, hkv, d, 1, spare=0) for _ in range(2))
+    qkv = torch.randn(lead + n, (hq + 2 * hkv) * d, device="cuda")
+    freq = torch.tensor([1e4 ** (-2 * i / max(rot, 1)) for i in range(rot // 2)], device="cuda")
+    start, kv_len, _ = rows_of(news, lens)
+    qa, qb = torch.full((n, hq * d), 5.0, device="cuda"), torch.full((lead + n, hq * d), 5.0, device="cuda")
+
+    def call(c, rows, q_out, start, tokens):
+        eng.kv8_append(c.kv8(), 0, rows, rows[:, hq * d:], rows[:, (hq + hkv) * d:], q_out, start, kv_len, tokens, hq,
+                       freq if rot else None, rot, q_ld=qkv.shape[1], k_ld=qkv.shape[1], v_ld=qkv.shape[1])
+
+    call(a, qkv[lead:], qa, start, n)
+    call(b, qkv, qb, start + lead, lead + n)
+    eng.sync()
+    assert torch.equal(a.data, b.data) and torch.equal(a.scale, b.scale)
+    assert torch.equal(qa, qb[lead:]) and (qb[:lead] == 5.0).all()
+
+
+@pytest.mark.parametrize("start,lens,tokens", [([0, 1000, 1010, 0, 16], [1000, 400, 3, 16], 1010), ([40, 0, 5], [60, 9], 40), ([1000, 1001], [2000], 8)])
+def test_append_falling_rows_are_reported(eng, start, lens, tokens):
+    """A record is as it was, or as an append of its sequence alone leaves it, where the sequence's rows fit."""
+    d = 64
+    a, b, was = (Cache(lens, 16, 1, d, 3) for _ in range(3))
+    k = torch.randn(tokens, d, device="cuda")
+    eng.kv8_append(a.kv8(), 0, None, k, k, None, ints(start), ints(lens), tokens, 0, None, 0)
+    with pytest.raises(sx.SxError) as e:
+        eng.sync()
+    assert e.value.status == sx.SX_ERR_DEVICE
+    for i, (r0, r1) in enumerate(zip(start, start[1:])):
+        if r0 <= r1 <= tokens:
+            c = sx.KV8(b.data, b.scale, b.table[i:i + 1], 16, 1, d)
+            eng.kv8_append(c, 0, None, k, k, None, ints([r0, r1]), ints(lens[i:i + 1]), tokens, 0, None, 0)
+    eng.sync()
+    as_it_was = (a.data == was.data).all(-1) & (a.scale == was.scale)
+    appended = (a.data == b.data).all(-1) & (a.scale == b.scale)
+    assert (as_it_was | appended).all()
+
+
+@pytest.mark.parametrize("wide", [0, 100000])
+@pytest.mark.parametrize("new,lead", [(1, 16), (1, 100), (40, 33)])
+def test_attn_of_rows_before_the_first_sequence(eng, new, lead, wide):
+    lens, d = [150, 64], 64
+    Cache.spare_columns = wide  # (put back by the fixture)
+    c = Cache(lens, 16, 2, d, 1)
+    q = torch.randn(lead + 2 * new, 4 * d, device="cuda")
+    start, kv_len, _ = rows_of([new, new], lens)
+    a, b = torch.empty(2 * new, 4 * d, device="cuda"), torch.full_like(q, 3.0)
+    eng.kv8_attn(c.kv8(), 0, q[lead:], a, start, kv_len, 2 * new, 4, 0.1)
+    eng.kv8_attn(c.kv8(), 0, q, b, start + lead, kv_len, lead + 2 * new, 4, 0.1)
+    eng.sync()
+    assert (a - b[lead:]).abs().max() <= 1e-4 and (b[:lead] == 3.0).all()
