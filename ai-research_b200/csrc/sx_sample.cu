@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) verify_kernel(VerifyArgs a)
     if (total == 0) continue;  // the same in every CTA
     none = false;
     const uint64_t before = warp_sum_u64((uint32_t)lane < rank ? ps : 0) + before_warp;
-    const uint64_t u = (uint64_t)(us * 16777216.0f);
+    const uint64_t u = (uint64_t)(fminf(fmaxf(us, 0.0f), 1.0f - 0x1p-24f) * 16777216.0f);  // (a NaN is 0)
     const uint64_t goal = (total >> 24) * u + (((total & 0xFFFFFFull) * u) >> 24);
     if (before <= goal && goal < before + mine) {  // this warp's run
       const uint32_t who = __popc(__ballot_sync(0xffffffffu, before + incl <= goal));

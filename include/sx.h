@@ -649,7 +649,8 @@ SX_API sx_status sx_dispatch_probs(sx_engine *e, const float *logits, uint32_t l
  * token is drawn with u_sample[b] in [0, 1) from max(p - q, 0) of the first refused place, or from
  * row n_draft[b] when all were accepted: with weights floor(min(w, 1) 2^38) (NaN and negative: 0),
  * their sum S and goal floor(S floor(u 2^24) / 2^24), the first index whose cumulative weight
- * exceeds the goal -- whole numbers, so no order of summation changes the token.  Where the
+ * exceeds the goal (u of 1 and more, which a generator over (0, 1] gives, counts as 1 - 2^-24, one
+ * below 0 and a NaN as 0) -- whole numbers, so no order of summation changes the token.  Where the
  * difference has no weight the target's row itself is used, and SX_NO_TOKEN where that has none.
  * out[b][0 .. drafts]: the accepted tokens, the drawn one, then SX_NO_TOKEN; accepted[b]: how many
  * were accepted.  A token id >= vocab is refused; n_draft[b] > drafts counts as drafts; both

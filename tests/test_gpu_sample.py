@@ -326,6 +326,18 @@ def test_verify_and_probs_in_a_graph(eng):
         assert np.array_equal(out.cpu().numpy().view(np.uint32), want_out) and acc.tolist() == want_acc.tolist()
 
 
+@pytest.mark.parametrize("v", [1, 100, 32001])
+@pytest.mark.parametrize("u,counts_as", [(1.0, 1 - 2.0 ** -24), (1.5, 1 - 2.0 ** -24), (math.inf, 1 - 2.0 ** -24), (-1.0, 0.0), (-0.0, 0.0), (math.nan, 0.0)])
+def test_verify_draws_with_any_number(eng, v, u, counts_as):
+    """u outside [0, 1) draws the nearest token: every place of out is written."""
+    p, q, tok, ua, us = drawn_inputs(3, 2, v, 13)
+    us[:] = counts_as
+    want = check_verify(eng, p, q, tok, ua, us)
+    us[:] = u
+    got = run_verify(eng, p, q, tok, ua, us)
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
 def test_verify_refusals(eng):
     p, q, tok, ua, us = drawn_inputs(2, 2, 50, 11)
     out, acc = torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
