@@ -78,6 +78,7 @@ SX_API sx_status sx_pages_extend(sx_pages *p, uint32_t seq, uint32_t len) {
 SX_API sx_status sx_pages_truncate(sx_pages *p, uint32_t seq, uint32_t len) {
   if (!p || seq >= p->len.size()) return bad("pages_truncate: no such sequence");
   if (len > p->len[seq]) return bad("pages_truncate: longer than the sequence");
+  if (len == p->len[seq] && len > 0) return SX_OK;  // (0 ends it, released pages or not)
   uint32_t *row = row_of(p, seq);
   const uint32_t keep = pages_of(p, len);
   if (len > 0 && keep <= p->first[seq])

@@ -69,6 +69,21 @@ def test_pages_truncate_past_a_released_page_is_refused():
     assert p.free_count == 8
 
 
+def test_pages_truncate_to_the_same_length_changes_nothing():
+    """A step whose drafts all stand takes nothing back, also when a window has passed every full page."""
+    p = sx.Pages(8, 16, 1, 8)
+    p.extend(0, 64)
+    p.release_before(0, 64)
+    before = p.table()
+    p.truncate(0, 64)
+    assert np.array_equal(before, p.table()) and p.length(0) == 64 and p.free_count == 8
+    p.extend(0, 65)
+    assert p.table()[0].tolist()[:4] == [sx.NO_PAGE] * 4 and p.table()[0, 4] < 8
+    p.truncate(0, 0)
+    p.truncate(0, 0)
+    assert p.free_count == 8
+
+
 @pytest.mark.parametrize("args", [(0, 16, 1, 1), (4, 0, 1, 1), (4, 24, 1, 1), (4, 2048, 1, 1), (4, 16, 0, 1),
                                   (4, 16, 1, 0), (4, 1024, 1, 1 << 21)])
 def test_pages_bad_geometry(args):
