@@ -616,6 +616,7 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
       size_t o_pbar = take(256);
       size_t o_kpart = take(std::max(sx::kv8_part_bytes(e->num_sms), sx::kv8_prompt_part_bytes(e->num_sms)));
       size_t o_kcnt = take((size_t)e->num_sms * 2 * 4);
+      size_t o_probs = take(sx::kProbsPartBytes);
       e->scratch_bytes = off;
       st = cuda_status(cudaMalloc(&e->scratch, e->scratch_bytes), "engine scratch");
       if (st) break;
@@ -631,6 +632,7 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
       e->persist_bar = reinterpret_cast<uint32_t *>(b + o_pbar);
       e->kv8_part = reinterpret_cast<float *>(b + o_kpart);
       e->kv8_cnt = reinterpret_cast<uint32_t *>(b + o_kcnt);
+      e->probs_part = reinterpret_cast<float2 *>(b + o_probs);
       st = cuda_status(cudaMemset(e->scratch, 0, e->scratch_bytes), "engine scratch zero");
       if (st) break;
     }

@@ -39,6 +39,7 @@ struct sx_engine {
   uint32_t *persist_bar = nullptr;  // grid-barrier arrival word of the persistent kernel
   float *kv8_part = nullptr;     // paged 8-bit attention: parts of problems split over CTAs
   uint32_t *kv8_cnt = nullptr;   // and their arrival counters, one per CTA
+  float2 *probs_part = nullptr;  // probabilities: parts of long rows
   int num_sms = 148;
   std::mutex freq_mu;
   std::map<std::pair<uint32_t, uint32_t>, float *> inv_freq;  // (rot, theta bits)

@@ -343,8 +343,9 @@ size_t kv8_part_bytes(int num_sms);
 // its form for many rows per kv head (sx_kv8_prompt.cu); the arguments are in sx_kv8.cuh
 cudaError_t prepare_kv8_prompt();
 size_t kv8_prompt_part_bytes(int num_sms);
-// Probabilities and verification (sx_sample.cu)
+// Probabilities and verification (sx_sample.cu): scratch for the {max, sum} of long rows' chunks
 cudaError_t prepare_sample_kernels();
+constexpr size_t kProbsPartBytes = 512 * 1024;  // 2048 rows of 262144, 32 of the longest
 
 // Batch-prefill Q4_0 projection GEMM (sx_prefill.cu): y[t][n] = x[t][:] . bf16(deq(w[n][:]))
 cudaError_t prepare_prefill_kernel();

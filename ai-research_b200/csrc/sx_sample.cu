@@ -478,8 +478,8 @@ SX_API sx_status sx_dispatch_probs(sx_engine *e, const float *logits, uint32_t l
   const sx::ProbsVariant v = sx::probs_variant(n);
   if (v.ctas >= sx::kTwoPassCtas && 2ull * rows * v.ctas > 3ull * e->num_sms) {
     const uint32_t chunks = (n + sx::kChunk - 1) / sx::kChunk;
-    float2 *const part = reinterpret_cast<float2 *>(e->kv8_part);
-    const uint32_t most = (uint32_t)(sx::kv8_part_bytes(e->num_sms) / sizeof(float2)) / chunks;
+    float2 *const part = e->probs_part;
+    const uint32_t most = (uint32_t)(sx::kProbsPartBytes / sizeof(float2)) / chunks;
     for (uint32_t r = 0; r < rows && ce == cudaSuccess; r += most) {
       sx::ProbsArgs b = a;
       b.z += (size_t)r * a.z_ld;

@@ -114,6 +114,58 @@ def test_probs_many_long_rows_repeat_in_a_graph(eng):
         eng.set_stream(sx.STREAM_LEGACY)
 
 
+@pytest.mark.parametrize("rows,n", [(3000, 65537), (40, (1 << 24) - 3)])
+def test_probs_more_rows_than_one_pass_holds(eng, rows, n):
+    """Row by row against a softmax in 64 bits, at places of every pass over the rows."""
+    z = torch.randn(rows, 4096, device="cuda")
+    z = z.repeat(1, -(-n // 4096))[:, :n].contiguous()
+    z[:, -1] = torch.arange(rows, device="cuda") % 7
+    out = torch.empty_like(z)
+    eng.probs(z, out, rows, n)
+    eng.sync()
+    for r in list(range(0, rows, max(1, rows // 40))) + [rows - 1]:
+        want = torch.softmax(z[r].double(), -1)
+        assert ((out[r] - want).abs() <= want * 2.0 ** -19).all(), r
+
+
+def test_probs_beside_attention(eng):
+    """Captured in two graphs, long rows' probabilities and an attention that is cut over CTAs may run at
+    the same time: they work in memory of their own."""
+    d, n = 128, 6000
+    data = torch.randint(0, 120, (n // 16, 2, 1, 2, 16 * d), dtype=torch.uint8, device="cuda")
+    scale = torch.full((n // 16, 2, 1, 2), 2.0 ** -6, device="cuda")
+    table = torch.arange(n // 16, dtype=torch.int32, device="cuda")[None]
+    cache = sx.KV8(data, scale, table, 16, 2, d)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    z = torch.randn(24, 262144, device="cuda")
+    for new in (1, 100):
+        q = torch.randn(new, 8 * d, device="cuda")
+        start, kv_len, out, p = ints(0, new), ints(n), torch.empty_like(q), torch.empty_like(z)
+        eng.kv8_attn(cache, sx.DTYPE_F32, q, out, start, kv_len, new, 8, d ** -0.5)
+        eng.probs(z, p, 24, 262144)
+        eng.sync()
+        want_out, want_p = out.clone(), p.clone()
+        streams, graphs = [torch.cuda.Stream() for _ in range(2)], [torch.cuda.CUDAGraph() for _ in range(2)]
+        try:
+            for s, g, call in zip(streams, graphs, (lambda: eng.kv8_attn(cache, sx.DTYPE_F32, q, out, start, kv_len, new, 8, d ** -0.5),
+                                                    lambda: eng.probs(z, p, 24, 262144))):
+                with torch.cuda.graph(g, stream=s):
+                    eng.set_stream(s.cuda_stream)
+                    for _ in range(20):
+                        call()
+        finally:
+            eng.set_stream(sx.STREAM_LEGACY)
+        for _ in range(5):
+            out.zero_()
+            p.zero_()
+            torch.cuda.synchronize()
+            for s, g in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want_out) and torch.equal(p, want_p)
+
+
 def test_probs_refusals(eng):
     z = torch.zeros(2, 8, device="cuda")
     for kw in (dict(logits=None), dict(probs=None), dict(n=0), dict(temperature=0.0), dict(temperature=-1.0), dict(temperature=math.nan),
