@@ -589,6 +589,8 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
                      "capture stream");
     if (st) break;
     e->stream = e->own_stream;
+    st = cuda_status(cudaEventCreateWithFlags(&e->order, cudaEventDisableTiming), "stream order event");
+    if (st) break;
     st = cuda_status(cudaHostAlloc((void **)&e->err_host, sizeof(uint32_t), cudaHostAllocMapped),
                      "error word");
     if (st) break;
@@ -675,6 +677,7 @@ SX_API void sx_engine_destroy(sx_engine *e) {
   for (auto &kv : e->inv_freq) cudaFree(kv.second);
   if (e->scratch) cudaFree(e->scratch);
   if (e->err_host) cudaFreeHost(e->err_host);
+  if (e->order) cudaEventDestroy(e->order);
   if (e->capture_stream) cudaStreamDestroy(e->capture_stream);
   if (e->own_stream) cudaStreamDestroy(e->own_stream);
   delete e;
@@ -682,7 +685,31 @@ SX_API void sx_engine_destroy(sx_engine *e) {
 
 SX_API sx_status sx_engine_set_stream(sx_engine *e, void *cuda_stream) {
   SX_CHECK_ARG(e, "engine: null");
-  e->stream = cuda_stream ? (cudaStream_t)cuda_stream : e->own_stream;
+  const cudaStream_t from = e->stream, to = cuda_stream ? (cudaStream_t)cuda_stream : e->own_stream;
+  if (e->scratch_used && from != to) {
+    // Streams in capture neither wait for work outside nor record for it.
+    auto plain = [](cudaStream_t s) {
+      cudaStreamCaptureStatus c;
+      const bool ok = cudaStreamIsCapturing(s, &c) == cudaSuccess && c == cudaStreamCaptureStatusNone;
+      if (!ok) cudaGetLastError();
+      return ok;
+    };
+    auto follow = [&](cudaStream_t s, cudaStream_t after) {
+      if (s == after) return cudaSuccess;
+      const cudaError_t ce = cudaEventRecord(e->order, after);
+      return ce == cudaSuccess ? cudaStreamWaitEvent(s, e->order, 0) : ce;
+    };
+    SX_TRY_CUDA(cudaSetDevice(e->device), "cudaSetDevice");
+    const bool from_plain = plain(from), to_plain = plain(to);
+    const cudaStream_t next = to_plain ? to : from_plain ? from : nullptr;  // what waits for `left`
+    if (next && e->left) {
+      SX_TRY_CUDA(follow(next, e->left), "stream order");
+      e->left = nullptr;
+    }
+    if (from_plain && to_plain) SX_TRY_CUDA(follow(to, from), "stream order");
+    if (from_plain && !to_plain) e->left = from;
+  }
+  e->stream = to;
   return SX_OK;
 }
 SX_API void *sx_engine_stream(sx_engine *e) { return e ? (void *)e->stream : nullptr; }
@@ -690,7 +717,9 @@ SX_API void *sx_engine_stream(sx_engine *e) { return e ? (void *)e->stream : nul
 SX_API sx_status sx_engine_sync(sx_engine *e) {
   SX_CHECK_ARG(e, "engine: null");
   SX_TRY_CUDA(cudaSetDevice(e->device), "cudaSetDevice");
-  return wait_stream(e, e->stream, 60000000000ull);
+  const sx_status st = wait_stream(e, e->stream, 60000000000ull);
+  if (!e->left && st != SX_ERR_TIMEOUT && st != SX_ERR_CUDA) e->scratch_used = false;
+  return st;
 }
 
 // ---------------------------------------------------------------------------------------

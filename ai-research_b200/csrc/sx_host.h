@@ -40,6 +40,10 @@ struct sx_engine {
   float *kv8_part = nullptr;     // paged 8-bit attention: parts of problems split over CTAs
   uint32_t *kv8_cnt = nullptr;   // and their arrival counters, one per CTA
   float2 *probs_part = nullptr;  // probabilities: parts of long rows
+  // Calls that work in kv8_part or probs_part must not overlap: sx_engine_set_stream orders them.
+  bool scratch_used = false;     // by a call that sx_engine_sync has not waited for
+  cudaEvent_t order = nullptr;
+  cudaStream_t left = nullptr;   // left for a stream in capture, which could not wait for it
   int num_sms = 148;
   std::mutex freq_mu;
   std::map<std::pair<uint32_t, uint32_t>, float *> inv_freq;  // (rot, theta bits)

@@ -728,6 +728,7 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
   a.scale = scale;
   a.part = e->kv8_part;
   a.cnt = e->kv8_cnt;
+  e->scratch_used = true;
   a.err = e->err_dev;
   // Packed rows of an average sequence: past 16 the tcgen05 form, which takes 128 at a time, where there
   // may be enough to do: its smallest call takes 12.5 (head size 128) to 14 us (256), this form's 7 to 8, but

@@ -435,6 +435,12 @@ __global__ void __launch_bounds__(kMergeThreads) kv8_prompt_merge_kernel(const _
   pdl_wait();
   const PromptPart w = part_list<D>(a, ctas)[blockIdx.x];
   if (w.parts == 0) return;
+  // (what another call's parts left here, had one run at the same time, ends as an error)
+  if (w.part >= w.parts || w.c0 + w.parts > ctas || w.slot0 >= 2 * ctas || w.rows - 1 >= kRows || w.head >= a.c.num_kv ||
+      w.r0 >= a.tokens || (w.row0 + w.rows - 1) / a.gqa >= a.tokens - w.r0) {
+    if (threadIdx.x == 0) raise_error(a.err, kDevBadParams);
+    return;
+  }
   const float2 *const part_ml = reinterpret_cast<const float2 *>(a.part);
   const float *const part_o = part_values(a, ctas);
   const uint32_t item = threadIdx.x % kItems, sub = threadIdx.x / kItems;

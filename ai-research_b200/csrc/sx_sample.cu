@@ -479,6 +479,7 @@ SX_API sx_status sx_dispatch_probs(sx_engine *e, const float *logits, uint32_t l
   if (v.ctas >= sx::kTwoPassCtas && 2ull * rows * v.ctas > 3ull * e->num_sms) {
     const uint32_t chunks = (n + sx::kChunk - 1) / sx::kChunk;
     float2 *const part = e->probs_part;
+    e->scratch_used = true;
     const uint32_t most = (uint32_t)(sx::kProbsPartBytes / sizeof(float2)) / chunks;
     for (uint32_t r = 0; r < rows && ce == cudaSuccess; r += most) {
       sx::ProbsArgs b = a;

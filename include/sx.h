@@ -102,7 +102,9 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
                                   sx_engine **out);
 /* GpuEngine.deinit (kernels.zig:70-78) */
 SX_API void sx_engine_destroy(sx_engine *e);
-/* Run subsequent work on an external cudaStream_t (NULL restores the engine's own). */
+/* Run subsequent work on an external cudaStream_t (NULL restores the engine's own).  Where a
+ * sx_dispatch_kv8_attn or sx_dispatch_probs has run since the last sx_engine_sync, the new stream waits
+ * for the one it replaces, which must still exist; streams in capture are left out of this. */
 SX_API sx_status sx_engine_set_stream(sx_engine *e, void *cuda_stream);
 SX_API void *sx_engine_stream(sx_engine *e);
 /* Wait for the engine stream, then report any device-side error word. */
@@ -521,6 +523,11 @@ SX_API sx_status sx_model_create_tp(sx_engine *e, const sx_model_config *cfg, sx
  * logits into probabilities (sx_dispatch_probs) and checks the drafted tokens against them
  * (sx_dispatch_verify).  All four are asynchronous on the engine stream, allocate nothing and
  * can be captured in a CUDA graph; lengths, page ids and tokens are read on the device.
+ *
+ * Attention, and probabilities of many long rows, work in memory of the engine (40 MB and 0.5 MB,
+ * apart from one another).  Two calls of the same kind on one engine must not overlap on the GPU: on
+ * one stream, and over sx_engine_set_stream, they do not; graphs that hold such calls must not be
+ * replayed beside one another or beside direct calls.  Engines of their own may overlap.
  * ------------------------------------------------------------------------------------- */
 /* Page bookkeeping (host): which pages of a pool hold which sequence.  Only ids live here. */
 typedef struct sx_pages sx_pages;

@@ -1,5 +1,6 @@
 """The paged 8-bit KV cache: append with rotation and quantisation, and attention over it, against
 restatements in 64 bits that follow the layout's byte formulas."""
+import ctypes
 import math
 
 import pytest
@@ -734,3 +735,85 @@ def test_attn_of_rows_before_the_first_sequence(eng, new, lead, wide):
     eng.kv8_attn(c.kv8(), 0, q, b, start + lead, kv_len, lead + 2 * new, 4, 0.1)
     eng.sync()
     assert (a - b[lead:]).abs().max() <= 1e-4 and (b[:lead] == 3.0).all()
+
+
+def parallel_calls(eng):
+    """An attention of each form that is cut over CTAs, and long rows' probabilities: calls that work in
+    the engine's memory, and their outputs."""
+    d, n = 128, 6000
+    c, calls = Cache([n], 16, 2, d, 5), []
+    for new in (1, 100):
+        q, (start, kv_len, _) = torch.randn(new, 8 * d, device="cuda"), rows_of([new], [n])
+        out = torch.empty_like(q)
+        calls.append((lambda q=q, out=out, start=start, kv_len=kv_len, new=new:
+                      eng.kv8_attn(c.kv8(), 0, q, out, start, kv_len, new, 8, d ** -0.5), out))
+    z = torch.randn(24, 262144, device="cuda")
+    p = torch.empty_like(z)
+    calls.append((lambda: eng.probs(z, p, 24, 262144), p))
+    return calls
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_calls_follow_one_another_over_streams(eng, which):
+    """A call after set_stream begins when the one before it, on the other stream, has ended."""
+    call, out = parallel_calls(eng)[which]
+    call()
+    eng.sync()
+    want = out.clone()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    try:
+        first, second = torch.cuda.Event(), torch.cuda.Event()
+        for s, done in zip(streams, (first, second)):
+            eng.set_stream(s.cuda_stream)
+            with torch.cuda.stream(s):
+                if done is first:
+                    torch.cuda._sleep(200_000_000)  # a tenth of a second
+                call()
+                done.record()
+        second.synchronize()
+        assert first.query()
+        # a capture between them: the stream in capture cannot wait, the next one does
+        eng.set_stream(streams[0].cuda_stream)
+        with torch.cuda.stream(streams[0]):
+            torch.cuda._sleep(200_000_000)
+            call()
+            first.record()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(streams[1]):
+            g.capture_begin(capture_error_mode="thread_local")
+            eng.set_stream(streams[1].cuda_stream)
+            call()
+            g.capture_end()
+        eng.set_stream(streams[2].cuda_stream)
+        with torch.cuda.stream(streams[2]):
+            call()
+            second.record()
+        second.synchronize()
+        assert first.query()
+        eng.sync()
+        with torch.cuda.stream(streams[1]):
+            out.zero_()
+            g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    finally:
+        torch.cuda.synchronize()
+        eng.sync()
+        eng.set_stream(sx.STREAM_LEGACY)
+
+
+def test_a_stream_may_go_after_a_sync(eng):
+    """Nothing is asked of the stream that is left once sx_engine_sync has waited for it."""
+    call, out = parallel_calls(eng)[0]
+    made, lib = ctypes.c_void_p(), ctypes.CDLL("libcudart.so.12")  # (torch's own streams are never destroyed)
+    assert lib.cudaStreamCreateWithFlags(ctypes.byref(made), 1) == 0
+    eng.set_stream(made.value)
+    call()
+    eng.sync()
+    assert lib.cudaStreamDestroy(made) == 0
+    eng.set_stream(sx.STREAM_LEGACY)
+    want = out.clone()
+    call()
+    eng.sync()
+    assert torch.equal(out, want)
