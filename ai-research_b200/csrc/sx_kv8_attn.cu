@@ -10,10 +10,15 @@
 // along the lanes' rows and enters the second with tokens along K: movmatrix transposes it.
 //
 // Values: e4m3 is exact in f16.  q is scaled by a power of two per row to at most 2 and split into
-// two f16 terms (22 bits) for f32 rows; bf16 rows need one.  The running maximum m is that of
-// x + log2(v scale), x the score in log2 units, so that p' = 2^(x + log2(v scale) - m + 10) is at
-// most 2^10, carries the V record's scale and keeps 14 binades of subnormal-free f16 below the
-// largest contribution; the softmax's sum takes p' / v scale in f32.
+// two f16 terms (22 bits) for f32 rows; bf16 rows need one.  The reference m is the running maximum of
+// x + log2(v scale), x the score in log2 units, rounded up to a whole number: p' = 2^(x + log2(v scale) -
+// m + 15) is at most 2^15 and carries the V record's scale, and what changes m is an exact power of two.
+// The softmax's sum takes p' / v scale in f32.  f16 holds 22 bits of a p' down to 2^-3 (two terms; 11 bits
+// down to 2^-14 with one) and multiples of 2^-24 below.
+//
+// A record's scale may be far above the values that a row sees in it: its largest value may be masked, or
+// have no weight.  m would then leave nothing of the p' of other records.  Where scales fall by more than
+// 2^kFar the output is scaled up and m lowered to the record's own, as far as f32 holds the output.
 //
 // Split: the batch's work is a line of 16-token blocks -- for each sequence, kv head and group of
 // packed rows the blocks it sees and kOverhead more, for what starting and ending it costs -- cut
@@ -46,7 +51,9 @@ constexpr int kDecThreads = kDecWarps * 32;
 // 90 and 93.
 constexpr uint32_t kOverhead = 32;
 constexpr uint32_t kMergeSteps = 3;  // steps (a block a warp) that a merge over CTAs is worth
-constexpr float kPOffset = 10.0f;
+constexpr float kPOffset = 15.0f;
+constexpr float kFar = 16.0f;     // p' of a scale this far below is 2^-1 at its largest: 22 bits of multiples of 2^-24
+constexpr int kLargest = 100;     // exponent up to which an output is scaled up
 constexpr uint32_t kMaxParts = 32, kPartGroup = 16;  // merged at once; of a first level
 
 SX_DEV uint32_t movmatrix_trans(uint32_t v) {
@@ -361,6 +368,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
     __syncthreads();
 
     float o[kPieces][2][NT][4], mx[NT][2], ls[NT][2], mul[NT][2];
+    float lmax = -INFINITY;  // the largest log2(v scale) that mx may stand for
     uint32_t see_lo[NT][2], see_hi[NT][2];  // keys [lo, hi] of this lane's packed rows
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -448,7 +456,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
         for (int k = 0; k < 4; ++k) {
           float x = s[t][0][k] + s[t][1][k];
           if constexpr (kSplit) x += s[t][2][k] + s[t][3][k];
-          s[t][0][k] = fmaf(x * ks, mul[t][k & 1], lv);
+          s[t][0][k] = x * ks * mul[t][k & 1];
         }
       const uint32_t key0 = (first + block_of(step)) * kKv8Block;
       if (!have || key0 < all_lo || key0 + kKv8Block - 1 > all_hi) {
@@ -497,6 +505,43 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int k = 0; k < 2; ++k) top[t][k] = fmaxf(s[t][0][k], s[t][0][k + 2]);
+      if (lv < lmax - kFar && have) {
+        // mx may stand for a scale far above this one's: down to what this record's own would be
+        bool later = false;  // a row that sees nothing of it: its mx stays
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float m = top[t][k], big = ls[t][k];
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt) big = fmaxf(big, fmaxf(fabsf(o[p][mt][t][k]), fabsf(o[p][mt][t][k + 2])));
+#pragma unroll
+            for (int w = 4; w < 32; w <<= 1) {
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+              big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, w));
+            }
+            const int room = kLargest + 127 - (int)(__float_as_uint(big) >> 23);
+            const float down = fminf(mx[t][k] - ceilf(m + lv), (float)min(room, 126));
+            if (m == -INFINITY) {
+              later |= mx[t][k] != -INFINITY;
+            } else if (down > 0.0f) {
+              const float f = exp2_int((int)down);
+              mx[t][k] -= (float)(int)down;
+              ls[t][k] *= f;
+#pragma unroll
+              for (int p = 0; p < kPieces; ++p)
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt) {
+                  o[p][mt][t][k] *= f;
+                  o[p][mt][t][k + 2] *= f;
+                }
+            }
+          }
+        if (!__any_sync(0xffffffffu, later)) lmax = lv;
+      }
+      if (have) lmax = fmaxf(lmax, lv);
       bool moved = false;
       float shift[NT][2];
 #pragma unroll
@@ -506,9 +551,9 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
           float m = top[t][k];
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-          top[t][k] = fmaxf(m, mx[t][k]);
+          top[t][k] = fmaxf(ceilf(m + lv), mx[t][k]);
           moved |= top[t][k] != mx[t][k];
-          shift[t][k] = top[t][k] == -INFINITY ? 0.0f : top[t][k] - kPOffset;
+          shift[t][k] = top[t][k] == -INFINITY ? 0.0f : lv - (top[t][k] - kPOffset);
         }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -535,7 +580,7 @@ __global__ void __launch_bounds__(kDecThreads, (DecShape<D, NT, sizeof(T) == 4>:
       for (int t = 0; t < NT; ++t) {
         float pr[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) pr[k] = ex2(s[t][0][k] - shift[t][k & 1]);
+        for (int k = 0; k < 4; ++k) pr[k] = ex2(s[t][0][k] + shift[t][k & 1]);
         ls[t][0] = fmaf(pr[0] + pr[2], unv, ls[t][0]);
         ls[t][1] = fmaf(pr[1] + pr[3], unv, ls[t][1]);
         const uint32_t p0 = pack_f16(pr[0], pr[1]), p1 = pack_f16(pr[2], pr[3]);

@@ -10,14 +10,18 @@
 //   0 .. 7   softmax, two threads per row, each for half of a tile's 64 keys: their part of the row of S
 //            from tensor memory, P back.  The maximum that the exponentials refer to moves only when it
 //            grows by 2^8, which the two warps of a row vote on; the row of O is then rescaled in tensor
-//            memory.
+//            memory.  P's exponent is kOffset where the reference is.  f16 holds 22 bits of a P down to 2^-3
+//            (two terms; 11 bits down to 2^-14 with one) and multiples of 2^-24 below: enough while V's
+//            scales are within 2^kFar of the problem's largest.  What is further below is added to O in f32
+//            (add_far).
 //   8 ..     widen K and V.  A warp takes a pair of blocks (32 tokens): the cache's 16-byte pieces
 //            become 16-byte stores of the 128-byte-swizzled tiles for a fitting order of the tokens
 //            (tile position 32 q + 8 (t % 8 / 2) + 4 half + 2 (t / 8) + t % 2) and of V's elements
 //            (tile row 32 p + 8 (d % 4) + f(d % 32 / 4), f a permutation of 8).  The softmax undoes
 //            the first in its masks and scales, the output the second: both are register indexes.
 //            K is a tile ahead of V, so that no widening waits for the softmax before it.
-//   last     cuts the CTA's run into problems, one ahead, and issues the products.
+//   last     cuts the CTA's run into problems, one ahead, issues the products, and says which tiles have
+//            records that are far below.
 // Two S, K and V tiles let a tile's first product, and the widening for it, run beside the softmax of the
 // one before; up to head size 128 two CTAs share an SM.
 //
@@ -46,7 +50,7 @@ namespace {
 
 constexpr uint32_t kRows = 128;      // packed rows of a problem
 constexpr int kSoft = 8;             // softmax warps
-constexpr float kPromptOffset = 6.0f, kSlack = 8.0f;
+constexpr float kSlack = 8.0f, kOffset = 15.0f - kSlack;  // P is at most 2^15
 constexpr float kMinScale = 1.17549435e-38f;  // a product with a masked -inf stays that
 
 template <int D, bool SPLIT>
@@ -58,6 +62,7 @@ struct PromptShape {
   static constexpr int kWiden = kCtas == 2 ? 4 : 8;                       // warps that widen
   static constexpr int kThreads = (kSoft + kWiden + 1) * 32;
   static constexpr int kTerms = SPLIT ? 2 : 1;
+  static constexpr float kFar = SPLIT ? 10.0f : 20.0f;                    // P of the largest is 2^-3, 2^-13 there
   static constexpr int kQTerm = (int)kRows * D * 2;
   static constexpr int kTile = kTokens * D * 2;
   static constexpr int kStaged = kTokens * D;                             // a tile's V as it comes
@@ -145,6 +150,80 @@ __device__ __noinline__ void rescale_row(uint32_t col, int cols, float f) {
   }
 }
 
+// column k of a half is token 16 (k / 4 % 2) + 8 (k / 2 % 2) + 2 (k / 8) + k % 2 of it, record k / 4 % 2
+SX_DEV constexpr uint32_t key_bit(int k) { return 1u << (16 * ((k >> 2) & 1) + 8 * ((k >> 1) & 1) + 2 * (k >> 3) + (k & 1)); }
+
+// A tile's records whose log2(v scale) is under `below`: their part of this thread's row of O, in f32 from
+// the scores at s_col and the f16 tile of V, by both halves of a row in turn.  `facts`: shared memory of the
+// half's two records'.  Their scores, and those of keys that `vis` lacks, are -inf afterwards.  Returns their
+// part of the softmax's sum.  It takes 30 tiles' time: scales of one head that differ by over 2^10 are no
+// ordinary values.  Out of line, and plain values for arguments: references to what the loop reads took 15 %
+// of long prompts' time, and the call itself takes 4 % with head size 128 (bf16), 1 to 2 % elsewhere.
+template <int D>
+__device__ __noinline__ float add_far(uint32_t o_col, uint32_t v_tile, uint32_t s_col, uint32_t vis, uint32_t facts, float mul,
+                                      float ref, float below, bool begin) {
+  const uint32_t half = threadIdx.x / kRows, pair_bar = 2 + ((threadIdx.x >> 5) & 3);
+  uint32_t s[32], b[2][4];
+  float x[32], l = 0.0f;
+  ld_shared16(facts, b[0]);
+  ld_shared16(facts + 16, b[1]);
+  tmem_ld32(s_col, s);
+  tmem_wait_ld(s);
+  const float shift = ref == -INFINITY ? 0.0f : ref - kOffset;
+  auto factor = [&](int h) { return fmaxf(__uint_as_float(b[h][0]) * mul, kMinScale); };
+  auto offset = [&](int h) {
+    const float lv = __uint_as_float(b[h][1]);
+    return lv < below && lv > (float)kKv8MinExp ? lv - shift : -INFINITY;
+  };
+  const float2 km = make_float2(factor(0), factor(1)), off = make_float2(offset(0), offset(1));
+  const float2 unv = make_float2(__uint_as_float(b[0][2]), __uint_as_float(b[1][2]));
+#pragma unroll
+  for (int k = 0; k < 32; ++k) {
+    const bool second = (k >> 2) & 1;
+    const float add = second ? off.y : off.x;
+    if (!(vis & key_bit(k))) s[k] = 0xFF800000u;
+    x[k] = add != -INFINITY ? ex2(fmaf(__uint_as_float(s[k]), second ? km.y : km.x, add)) : 0.0f;
+    l = fmaf(x[k], second ? unv.y : unv.x, l);
+    if (add != -INFINITY) s[k] = 0xFF800000u;
+  }
+  tmem_st16(s_col, *reinterpret_cast<const uint32_t(*)[16]>(s));
+  tmem_st16(s_col + 16, *reinterpret_cast<const uint32_t(*)[16]>(s + 16));
+  if (begin) {  // zeros in O
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s[k] = 0;
+#pragma unroll 1
+    for (int d = half * (D / 2); d < (int)(half + 1) * (D / 2); d += 16)
+      tmem_st16(o_col + d, *reinterpret_cast<const uint32_t(*)[16]>(s));
+  }
+  tmem_wait_st();
+#pragma unroll 1
+  for (uint32_t turn = 0; turn < 2; ++turn) {
+    tc_fence_before();
+    pair_any(pair_bar, false);
+    tc_fence_after();
+    if (turn == half) {
+#pragma unroll 1
+      for (int d = 0; d < D; ++d) {
+        float o = __uint_as_float(tmem_ld1(o_col + d));
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t v[4];
+          ld_shared16(v_tile + d * 128 + (((4 * half + c) ^ (d & 7)) << 4), v);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&v[k]));
+            o = fmaf(x[8 * c + 2 * k], y.x, fmaf(x[8 * c + 2 * k + 1], y.y, o));
+          }
+        }
+        tmem_st1(o_col + d, __float_as_uint(o));
+      }
+      tmem_wait_st();
+    }
+  }
+  tc_fence_before();
+  return l;
+}
+
 enum Role { kSoftmax, kWidenKv, kProducts };
 
 // 128 packed rows of one sequence and kv head, and the tiles [t0, t1) of their keys that this CTA takes.
@@ -162,6 +241,8 @@ struct Problem {
   }
 };
 
+enum : uint32_t { kGone = 1, kApart = 2 };
+
 // What the CTA's threads share.
 template <int TOKENS, int WIDEN>
 struct PromptShared {
@@ -175,6 +256,10 @@ struct PromptShared {
   // of blocks of a tile {k scale, log2(v scale), 1 / v scale, there}.
   alignas(8) uint32_t record[WIDEN][64];  // (read by twos)
   float4 facts[TOKENS / 32][64];
+  // Of an even or odd tile: whether it has records that are not there or are far below (kGone, kApart), and
+  // what log2(v scale) is far below.
+  uint32_t odd_records[2];
+  float far_below[2];
 };
 
 // A wait that runs out ends the CTA's waiting altogether: what follows runs through on whatever is
@@ -563,6 +648,16 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       const uint32_t pos = pr.pos0 + (pr.row0 + min(i, rows - 1)) / a.gqa;
       const uint32_t see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_hi = pos + 1;
       float ref = -INFINITY, l = 0.0f;
+      // bit = token of this thread's half of a tile: the keys that its row sees, and that are there
+      auto visible = [&](uint32_t t) {
+        const uint32_t k0 = (first + t * kTileBlocks) * kKv8Block + 32 * half;
+        const uint32_t lo = see_lo > k0 ? see_lo - k0 : 0, hi = see_hi > k0 ? see_hi - k0 : 0;
+        uint32_t vis = lo < 32 && hi > lo ? (hi < 32 ? (1u << hi) - 1 : ~0u) & (~0u << lo) : 0;
+        const float4 *const block = sh.facts[half] + 2 * (t - t0) % 64;
+        if (block[0].w == 0.0f) vis &= 0xFFFF0000u;
+        if (block[1].w == 0.0f) vis &= 0x0000FFFFu;
+        return vis;
+      };
 #pragma unroll 1
       for (uint32_t t = t0; t < t1; ++t) {
         const uint32_t tile = tiles + (t - t0), s_col = tmem + lanes + tile % kS * kTokens;
@@ -575,20 +670,15 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         tmem_ld32(s_col + 32 * half, s);
         // block 2 half holds columns k with k / 4 even, block 2 half + 1 the others
         const float4 *const block = sh.facts[half] + 2 * (t - t0) % 64;
-        const bool gone0 = block[0].w == 0.0f, gone1 = block[1].w == 0.0f;
+        const uint32_t odd = sh.odd_records[tile & 1];
         const float km[2] = {fmaxf(block[0].x * mul, kMinScale), fmaxf(block[1].x * mul, kMinScale)};
         tmem_wait_ld(s);
-        if (mixed || gone0 || gone1) {  // some row does not see all of the tile, or a block is not there
-          const uint32_t k0 = (first + t * kTileBlocks) * kKv8Block + 32 * half;
-          const uint32_t lo = see_lo > k0 ? see_lo - k0 : 0, hi = see_hi > k0 ? see_hi - k0 : 0;
-          uint32_t vis = lo < 32 && hi > lo ? (hi < 32 ? (1u << hi) - 1 : ~0u) & (~0u << lo) : 0;
-          if (gone0) vis &= 0xFFFF0000u;
-          if (gone1) vis &= 0x0000FFFFu;
+        if (mixed || (odd & kGone)) {  // some row does not see all of the tile, or a block is not there
+          const uint32_t vis = visible(t);
           if (mixed && (sh.nan_mask[tile & 1][half] & vis)) l = NAN;
-          // column k is token 16 (k / 4 % 2) + 8 (k / 2 % 2) + 2 (k / 8) + k % 2
 #pragma unroll
           for (int k = 0; k < 32; ++k)
-            if (!(vis & (1u << (16 * ((k >> 2) & 1) + 8 * ((k >> 1) & 1) + 2 * (k >> 3) + (k & 1))))) s[k] = 0xFF800000u;
+            if (!(vis & key_bit(k))) s[k] = 0xFF800000u;
         }
         // -- the largest x + log2(v scale)
         float m[2] = {-INFINITY, -INFINITY};
@@ -600,7 +690,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         // -- one that outgrew the reference: rescale the row.  The vote also says that both halves of
         // the row have been read, which P overwrites.
         auto grows = [&] { return top > ref + kSlack || (ref == -INFINITY && top > ref); };
-        if (pair_any(pair_bar, grows())) {
+        if (pair_any(pair_bar, grows() || (odd & kApart))) {
           sh.row_top[half][i] = top;
           pair_any(pair_bar, false);
           top = fmaxf(top, sh.row_top[half ^ 1][i]);
@@ -615,8 +705,17 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
             rescale_row(tmem + lanes + P::kO + half * (D / 2), D / 2, f);
             tmem_wait_st();
           }
+          if (odd & kApart) {
+            wait(bars.v_full(tile), tile / 2);
+            __syncwarp();
+            l += add_far<D>(tmem + lanes + P::kO, v_tile(tile), s_col + 32 * half, visible(t), smem_u32(block), mul, ref,
+                            sh.far_below[tile & 1], t == t0);
+            tmem_ld32(s_col + 32 * half, s);  // (again, rather than kept over the call)
+            tmem_wait_ld(s);
+            pair_any(pair_bar, false);  // (both halves have, before either's P)
+          }
         }
-        const float shift = ref == -INFINITY ? 0.0f : ref - kPromptOffset;
+        const float shift = ref == -INFINITY ? 0.0f : ref - kOffset;
         const float off[2] = {block[0].y - shift, block[1].y - shift};
         float sum[2] = {0.0f, 0.0f};
         uint32_t hi[16];
@@ -749,7 +848,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         if (p0 == 0) {
           float2 f = make_float2(0.0f, 0.0f);
           if (rec != kNoRecord) f = *reinterpret_cast<const float2 *>(a.c.scale + 2 * (size_t)rec);
-          const int e = kv8_scale_exponent(f.y);
+          const int e = rec != kNoRecord ? kv8_scale_exponent(f.y) : kKv8MinExp;
           sh.facts[pair][at] = make_float4(f.x, (float)e, exp2_int(-e), rec != kNoRecord ? 1.0f : 0.0f);
         }
         __syncwarp();
@@ -869,9 +968,25 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       }
     } else {
       // ================================================================ the products
+      // Records whose scale is far below the problem's largest so far are added apart: the softmax's
+      // reference may stand for a value of that scale which is masked or has no weight, and nothing of
+      // their P would be left.  (The least scale is that of zeros, or nearly: those may go.)
+      int most = -128;
       auto product_s = [&](uint32_t tile) {
         wait(bars.k_full(tile), tile / 2);
         __syncwarp();
+        {
+          const float4 f = sh.facts[lane / 2 % 2][2 * (tile - tiles) % 64 + lane % 2];
+          const bool gone = __any_sync(0xffffffffu, f.w == 0.0f);
+          most = max(most, __reduce_max_sync(0xffffffffu, f.w != 0.0f ? (int)f.y : -128));
+          const float below = (float)most - P::kFar;
+          const bool apart = __any_sync(0xffffffffu, f.y < below && f.y > (float)kKv8MinExp);
+          if (lane == 0) {
+            sh.odd_records[tile & 1] = (gone ? kGone : 0) | (apart ? kApart : 0);
+            sh.far_below[tile & 1] = below;
+          }
+          __syncwarp();
+        }
         tc_fence_after();
         if (elect_one()) {
           mbar_arrive(bars.s_done(tile));  // (passes on what the widening warps wrote for the softmax)
@@ -884,6 +999,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         __syncwarp();
       };
       product_s(tiles);
+      const bool begun = (sh.odd_records[tiles & 1] & kApart) != 0;  // O: add_far has
       if (pr.parts > 1 && lane == 0)
         part_list<D>(a, gridDim.x)[pr.slot] =
             PromptPart{pr.parts, blockIdx.x - pr.c0, pr.slot0, pr.c0, pr.r0, pr.row0, pr.rows, pr.head};
@@ -900,7 +1016,7 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
 #pragma unroll
           for (int w = 0; w < kTerms; ++w)
             issue_ts<kTokens / 16>(tmem + P::kO, tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens),
-                                   v_tile(tile), D * 128, umma_idesc_f16(kRows, D), j > 0 || w > 0);
+                                   v_tile(tile), D * 128, umma_idesc_f16(kRows, D), j > 0 || w > 0 || begun);
           umma_commit(bars.pv_done(tile));
         }
         __syncwarp();

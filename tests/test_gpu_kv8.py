@@ -24,7 +24,7 @@ def eng():
 
 # Attention of more than 16 packed rows has two forms, and the table's width decides with the rows.
 BOTH_FORMS = """drafts prompts window one_long_prompt strided_rows magnitudes scales_far_apart nan_in_masked_places
-nan_value_only rows_outside_sequences_stay bad_page_masks_and_reports prompts_repeat_bit_for_bit
+nan_value_only large_values_without_weight scales_at_random rows_outside_sequences_stay bad_page_masks_and_reports prompts_repeat_bit_for_bit
 repeats_bit_for_bit_on_any_stream_and_in_a_graph scale_zero_and_negative""".split()
 
 
@@ -253,6 +253,80 @@ def test_attn_scales_far_apart(eng):
     check_attn(eng, "f32", 2, 1, 64, 16, [1, 4], [256, 64], cache=cache)
     cache.scale[..., 1] = 2.0 ** -60
     check_attn(eng, "f32", 2, 1, 64, 16, [1, 4], [256, 64], cache=cache)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256, 512])
+@pytest.mark.parametrize("new", [1, 5, 140])
+@pytest.mark.parametrize("kind", ["past_the_end", "before_the_window", "later_row", "no_weight", "no_weight_first", "every_other", "all_but_one"])
+def test_attn_large_values_without_weight(eng, dtype, d, new, kind):
+    """A record's scale may come from a value that a row does not see, or that has no weight in it: what
+    the row sees beside it keeps its precision.  (A refused draft, a token that a window has left, an
+    outlier that nothing attends to.)  The other tokens of such a record hold zeros, which is what a scale
+    so far above them leaves of them."""
+    code, dt = DT[dtype]
+    total, window = 409 + new, 150 if kind == "before_the_window" else 0
+    cache = Cache([total], 32, 1, d, 17)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    base = torch.randn(d, device="cuda", generator=g)
+    q = (base + 0.1 * torch.randn(new, 4, d, device="cuda", generator=g)).reshape(new, 4 * d).to(dt)
+    start, kv_len, _ = rows_of([new], [total])
+    dz = want_attn(cache, q, [new], [total], 4, d ** -0.5, window)[2]  # (before: what is added has no weight)
+    in_k, in_v = (x.reshape(16, d) for x in places(d))
+
+    def record(pos, exponent, large=None):
+        page, slot = int(cache.table[0, pos // 32]), pos % 32 // 16
+        cache.data[page, 0, slot, 1] = 0
+        cache.scale[page, 0, slot, 1] = 2.0 ** exponent
+        if large is not None:
+            cache.data[page, 0, slot, 1, in_v[large % 16]] = 0x7E
+        return page, slot
+
+    if kind == "past_the_end":
+        record(total - 1, 50, total | 15)
+    elif kind == "before_the_window":
+        first = total - new - window + 1  # the first key that some row sees
+        record(first, 50, first - 1 if first % 16 else None)
+    elif kind == "later_row":
+        record(total - 1, 50, total - 1)
+    elif kind in ("no_weight", "no_weight_first"):
+        pos = 3 if kind == "no_weight_first" else 200
+        page, slot = record(pos, 50, pos)
+        cache.data[page, 0, slot, 0] = 0
+        cache.scale[page, 0, slot, 0] = 0.25
+        cache.data[page, 0, slot, 0, in_k[pos % 16]] = torch.where(base > 0, 0xFE, 0x7E).to(torch.uint8)
+    elif kind == "every_other":
+        for pos in range(0, total, 32):
+            record(pos, 60)
+    else:
+        for pos in range(0, total, 16):
+            if pos != 112:
+                record(pos, 60)
+        cache.scale[int(cache.table[0, 3]), 0, 1, 1] = 2.0 ** -50
+    out = torch.empty_like(q)
+    eng.kv8_attn(cache.kv8(), code, q, out, start, kv_len, new, 4, d ** -0.5, window=window)
+    eng.sync()
+    want, mass, _ = want_attn(cache, q, [new], [total], 4, d ** -0.5, window)
+    tol = tolerance(dtype, want, mass, dz, d)
+    bad = ~((out.double() - want).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), float(((out.double() - want).abs() / tol).max()), bad.nonzero()[:3].tolist())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128, 256, 512])
+@pytest.mark.parametrize("new", [1, 5, 140])
+def test_attn_scales_at_random(eng, dtype, d, new):
+    """V records with scales anywhere in 2^-40 .. 2^40 and, every third of them, zeros in half of their
+    elements: each element of the output is as near as its own terms allow."""
+    cache = Cache([500 + new, 90 + new], 32, 2, d, 21)
+    g = torch.Generator(device="cuda").manual_seed(9)
+    cache.scale[..., 1] = torch.exp2(torch.randint(-40, 41, cache.scale.shape[:-1], device="cuda", generator=g).float())
+    cut = places(d)[1].reshape(16, d)[:, : d // 2].reshape(-1)
+    hit = torch.rand(cache.scale.shape[:-1], device="cuda", generator=g) < 1 / 3
+    v = cache.data[..., 1, :]
+    v[..., cut] = torch.where(hit[..., None], 0, v[..., cut])
+    cache.data[..., 1, :] = v
+    check_attn(eng, dtype, 8, 2, d, 32, [new, new], [500 + new, 90 + new], cache=cache)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
