@@ -24,7 +24,7 @@ def eng():
 
 # Attention of more than 16 packed rows has two forms, and the table's width decides with the rows.
 BOTH_FORMS = """drafts prompts window one_long_prompt strided_rows magnitudes scales_far_apart nan_in_masked_places
-nan_value_only large_values_without_weight scales_at_random rows_outside_sequences_stay bad_page_masks_and_reports prompts_repeat_bit_for_bit
+nan_value_only large_values_without_weight scales_at_random chunks_beside_single_tokens rows_outside_sequences_stay bad_page_masks_and_reports prompts_repeat_bit_for_bit
 repeats_bit_for_bit_on_any_stream_and_in_a_graph scale_zero_and_negative""".split()
 
 
@@ -224,6 +224,43 @@ def test_attn_one_long_prompt(eng, dtype, d, hq):
     check_attn(eng, dtype, hq, 2, d, 64, [700, 1], [2100, 5], seed=10)
 
 
+@pytest.mark.parametrize("dtype,d,hkv", [("f32", 64, 4), ("bf16", 64, 4), ("f32", 128, 2), ("bf16", 256, 2)])
+def test_attn_many_tiles_of_a_problem_on_one_cta(eng, dtype, d, hkv):
+    """More problems than CTAs, of 44 tiles of 64 keys each: a CTA's tables of a problem's records wrap."""
+    n = 75 if d < 256 else 80
+    lens = [2816 - (7 * i) % 50 for i in range(n)]
+    check_attn(eng, dtype, 8 * hkv, hkv, d, 64, [16] * n, lens, seed=14)
+
+
+@pytest.mark.parametrize("dtype,d,total", [("f32", 64, 60001), ("bf16", 128, 100000), ("bf16", 256, 40011), ("f32", 256, 60000)])
+@pytest.mark.parametrize("new", [5, 16])
+def test_attn_many_parts_of_packed_rows(eng, dtype, d, total, new):
+    """One session's drafts on a long context: over a hundred CTAs hold parts of one problem."""
+    for _ in range(2):
+        check_attn(eng, dtype, 8, 1, d, 64, [new], [total], seed=15)
+
+
+@pytest.mark.parametrize("dtype,d", [("f32", 64), ("bf16", 128), ("bf16", 256), ("f32", 512)])
+@pytest.mark.parametrize("chunk", [60, 700])
+def test_attn_chunks_beside_single_tokens(eng, dtype, d, chunk):
+    """A batch that decodes most of its sequences and takes a prompt's chunk in two: one call for all."""
+    news = [1, 1, chunk, 0, 1, 1, 5, 1, chunk // 2] + [1] * 20
+    lens = [900, 1, chunk + 1500, 40, 17, 3000, 64, 333, chunk // 2] + [100 + 37 * i for i in range(20)]
+    check_attn(eng, dtype, 8, 2, d, 32, news, lens, seed=16)
+    check_attn(eng, dtype, 8, 2, d, 32, news, lens, seed=16, window=100)
+
+
+@pytest.mark.parametrize("dtype,d", [("f32", 64), ("bf16", 128), ("bf16", 256)])
+def test_attn_scales_at_random_over_many_tiles(eng, dtype, d):
+    lens, new = [6000, 3000], 40
+    cache = Cache(lens, 32, 1, d, 22)
+    g = torch.Generator(device="cuda").manual_seed(10)
+    far = torch.rand(cache.scale.shape[:-1], device="cuda", generator=g) < 0.05
+    up = torch.randint(-30, 31, far.shape, device="cuda", generator=g)
+    cache.scale[..., 1] *= torch.exp2(torch.where(far, up, 0).float())
+    check_attn(eng, dtype, 8, 1, d, 32, [new, new], lens, cache=cache)
+
+
 def test_attn_many_sequences(eng):
     lens = [(i * 37) % 200 for i in range(300)]
     check_attn(eng, "bf16", 4, 2, 64, 16, [min(n, 1) for n in lens], lens, seed=11)
@@ -253,6 +290,31 @@ def test_attn_scales_far_apart(eng):
     check_attn(eng, "f32", 2, 1, 64, 16, [1, 4], [256, 64], cache=cache)
     cache.scale[..., 1] = 2.0 ** -60
     check_attn(eng, "f32", 2, 1, 64, 16, [1, 4], [256, 64], cache=cache)
+
+
+@pytest.mark.parametrize("d,new,rows_form", [(64, 1, 39), (128, 2, 39), (256, 1, 39), (512, 1, 39), (64, 5, 32), (256, 5, 32)])
+@pytest.mark.parametrize("depth", [20.3, 25.4, 28.7])
+def test_attn_one_dominant_key_and_many_small_ones(eng, d, new, rows_form, depth):
+    """Equal p of 2^-depth err alike: each by 2^-22 of itself, and by the last bit that f16 leaves beside
+    the dominant one, 2^-39 (2^-32 with many rows per kv head); `total` of them add up."""
+    total = 100000
+    cache = Cache([total], 64, 1, d, 23)
+    cache.data[:, :, :, 0] = 0  # K: scores of 0
+    cache.data[:, :, :, 1] = 0x3E  # V: 1.75 scale
+    cache.scale[..., 1] = 1.0
+    page, slot, t = int(cache.table[0, 100]), 1, 5
+    in_k, in_v = (x.reshape(16, d) for x in places(d))
+    cache.data[page, 0, slot, 0, in_k[t]] = 0x38  # 1
+    cache.data[page, 0, slot, 1, in_v[t]] = 0xB8  # -1
+    cache.scale[page, 0, slot, 0] = 1.0
+    q = torch.full((new, 8 * d), depth * math.log(2) / math.sqrt(d), device="cuda")
+    start, kv_len, _ = rows_of([new], [total])
+    out = torch.empty_like(q)
+    eng.kv8_attn(cache.kv8(), 0, q, out, start, kv_len, new, 8, d ** -0.5)
+    eng.sync()
+    want, mass, dz = want_attn(cache, q, [new], [total], 8, d ** -0.5, 0)
+    tol = tolerance("f32", want, mass, dz, d) + 1.75 * total * 2.0 ** -rows_form
+    assert ((out.double() - want).abs() <= tol).all(), float(((out.double() - want).abs() / tol).max())
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
