@@ -76,3 +76,37 @@ def test_speculate(drafts, temperature):
     assert pages.free_count == per * len(lens)
     pages.close()
     eng.close()
+
+
+@pytest.mark.parametrize("drafts,temperature", [(0, 1.0), (1, 0.7), (4, 1.0)])
+def test_speculate_every_session_against_plain_attention(drafts, temperature):
+    """What the cache holds for every session, cut to the tokens asked for, gives the next row of a plain
+    forward pass over them (the bound is that of the test above)."""
+    eng = sx.Engine(0)
+    eng.set_stream(sx.STREAM_LEGACY)
+    lens, tokens, page, per = [1, 2, 17, 100, 200], 24, 16, 24
+    pages = sx.Pages(per * len(lens), page, len(lens), per)
+    target = speculate.Target(eng, pages, layers=2, hidden=256, q_heads=8, kv_heads=2, head_dim=64, vocab=1000,
+                              num_pages=per * len(lens), page_tokens=page)
+    rng = np.random.default_rng(3)
+    prompts = [rng.integers(0, 1000, n) for n in lens]
+    got, hits, tried = speculate.generate(eng, target, prompts, tokens, drafts, temperature)
+    eng.sync()
+    compared = 0
+    for b, prompt in enumerate(prompts):
+        seq = np.concatenate([prompt, got[b]])
+        # the cache holds all but the newest token at least; more where a lucky session ran ahead
+        n = min(pages.length(b), len(seq))
+        assert n >= len(seq) - 1
+        pages.truncate(b, n - 1)
+        pages.extend(b, n)
+        news = [0] * len(prompts)
+        news[b] = 1
+        row = target.rows(torch.as_tensor(seq[n - 1:n], device="cuda"), news)[0].float()
+        want = dense_rows(target, torch.as_tensor(seq[:n], device="cuda"))[-1].float()
+        assert (row - want).norm() <= 0.05 * want.norm()
+        compared += 1
+    assert compared == len(prompts)
+    eng.sync()
+    pages.close()
+    eng.close()
