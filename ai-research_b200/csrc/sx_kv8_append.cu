@@ -560,6 +560,7 @@ extern "C" SX_API sx_status sx_dispatch_kv8_append(
       "kv8_append launch");
 }
 
+extern "C" SX_API uint32_t sx_kv8_append_args_bytes(void) { return (uint32_t)sizeof(sx_kv8_append_args); }
 extern "C" SX_API sx_status sx_dispatch_kv8_append_args(sx_engine *e, const sx_kv8_append_args *a) {
   if (!a) {
     sx_host_set_error("kv8_append: null arguments");

@@ -794,6 +794,7 @@ extern "C" SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, 
       "kv8_attn launch");
 }
 
+extern "C" SX_API uint32_t sx_kv8_attn_args_bytes(void) { return (uint32_t)sizeof(sx_kv8_attn_args); }
 extern "C" SX_API sx_status sx_dispatch_kv8_attn_args(sx_engine *e, const sx_kv8_attn_args *a) {
   if (!a) {
     sx_host_set_error("kv8_attn: null arguments");

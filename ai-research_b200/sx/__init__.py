@@ -335,6 +335,8 @@ _SIGS = {
     "sx_pages_table": (_P, [_P]),
     "sx_dispatch_kv8_append": (_S, [_P, C.POINTER(KV8), _I, _P, _P, _P, _U32, _U32, _U32, _P, _P,
                                     _P, _P, _P, _U32, _U32, _P, _U32, _U32, _F]),
+    "sx_kv8_append_args_bytes": (_U32, []),
+    "sx_kv8_attn_args_bytes": (_U32, []),
     "sx_dispatch_kv8_append_args": (_S, [_P, C.c_char_p]),
     "sx_dispatch_kv8_attn_args": (_S, [_P, C.c_char_p]),
     "sx_dispatch_kv8_attn": (_S, [_P, C.POINTER(KV8), _I, _P, _P, _U32, _U32, _P, _P, _U32, _U32,
@@ -366,11 +368,23 @@ def lib():
         fn = getattr(L, name)
         fn.restype = res
         fn.argtypes = args
-    if L.sx_model_config_bytes() != C.sizeof(ModelConfig):
-        raise ImportError(f"{path}: sx_model_config is {L.sx_model_config_bytes()} bytes, this "
-                          f"binding's mirror {C.sizeof(ModelConfig)}: rebuild the library")
+    _check_layouts(L, path)
     _lib = L
     return L
+
+
+def _check_layouts(L, path) -> None:
+    """Structs that the binding lays out itself are as long as the library's."""
+    def packed(tail):  # a cache, the tail, and C's padding to 8 bytes
+        return -(-(C.sizeof(KV8) + tail.size) // 8) * 8
+
+    for name, ours in (("sx_model_config", C.sizeof(ModelConfig)),
+                       ("sx_kv8_append_args", packed(_APPEND_ARGS)),
+                       ("sx_kv8_attn_args", packed(_ATTN_ARGS))):
+        theirs = getattr(L, name + "_bytes")()
+        if theirs != ours:
+            raise ImportError(f"{path}: {name} is {theirs} bytes, this binding's mirror {ours}: "
+                              "rebuild the library")
 
 
 def declared_symbols() -> list[str]:

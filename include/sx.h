@@ -640,6 +640,9 @@ typedef struct {
   uint32_t dtype, q_ld, out_ld, tokens, num_q, window;
   float scale;
 } sx_kv8_attn_args;
+/* sizeof of the two blocks, for bindings that lay them out themselves to compare with */
+SX_API uint32_t sx_kv8_append_args_bytes(void);
+SX_API uint32_t sx_kv8_attn_args_bytes(void);
 SX_API sx_status sx_dispatch_kv8_append_args(sx_engine *e, const sx_kv8_append_args *a);
 SX_API sx_status sx_dispatch_kv8_attn_args(sx_engine *e, const sx_kv8_attn_args *a);
 
