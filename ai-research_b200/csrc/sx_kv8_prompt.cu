@@ -70,6 +70,13 @@ struct PromptShape {
   // tensor memory columns: S tiles (P over them), low terms of P, O
   static constexpr int kLow = kS * kTokens;
   static constexpr int kO = kLow + (SPLIT ? kS * kTokens / 2 : 0);
+  static constexpr int kTotal = SPLIT && kCtas == 1 && kO + 2 * D <= 512 ? kO + D : 0;  // sums of O (fold_row), where there is room
+  // Tiles after which f32 rows' O is added to a sum apart.  The tensor core cuts products off at the last bit
+  // of the sum so far, always toward zero: a bias that grows with the sum's length, 9e-6 of the output on
+  // 6000 keys of equal weight (head size 256) and 2.3e-5 on 31000, where the products' f32 sums err by 1.6e-6.
+  // Sums of 8 tiles leave 1.7e-6 on any length, of 16 2.6e-6, of 4 (in tensor memory) 0.9e-6.  f32 prompts
+  // and drafts take 10 to 13 % more time for it; bf16 rows round by 2^-9 at the end and go without.
+  static constexpr uint32_t kFold = kTotal ? 4 : 8;
   static constexpr int kCols = kO + D <= 256 ? 256 : 512;
   static_assert(kO + D <= 512 && kCols * kCtas <= 512, "tensor memory");
 };
@@ -224,6 +231,77 @@ __device__ __noinline__ float add_far(uint32_t o_col, uint32_t v_tile, uint32_t 
   return l;
 }
 
+// f32 rows: this thread's half of its row of O, `cols` columns from o_col on, is added to a sum whose
+// reference is in shared memory at ref_at: in tensor memory at t_col (0: there is no room), or in the
+// workspace at `acc`, a row every kRows floats.  Only this thread touches it, so additions are in order; in
+// the workspace they are left to L2 while the reference stays.  A whole warp calls it.
+SX_DEV float ref_factor(float was, float ref) { return was == ref ? 1.0f : was == -INFINITY ? 0.0f : ex2(was - ref); }
+SX_DEV float ld_shared_f32(uint32_t at) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+SX_DEV void st_shared_f32(uint32_t at, float v) { asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(at), "f"(v) : "memory"); }
+template <bool IN_TMEM>
+__device__ __noinline__ void fold_row(uint32_t o_col, uint32_t t_col, int cols, float *acc, uint32_t ref_at, float ref, bool first) {
+  const float f = first ? 1.0f : ref_factor(ld_shared_f32(ref_at), ref);
+  st_shared_f32(ref_at, ref);
+  const bool moved = __any_sync(0xffffffffu, f != 1.0f);
+#pragma unroll 1
+  for (int d = 0; d < cols; d += 16, acc += 16 * kRows) {
+    uint32_t o[16];
+    tmem_ld16(o_col + d, o);
+    if constexpr (IN_TMEM) {
+      uint32_t t[16];
+      tmem_ld16(t_col + d, t);
+      tmem_wait_ld(o);
+      tmem_wait_ld(t);
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        o[k] = first ? o[k] : __float_as_uint(fmaf(__uint_as_float(t[k]), f, __uint_as_float(o[k])));
+      tmem_st16(t_col + d, o);
+    } else if (first) {
+      tmem_wait_ld(o);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) __stcg(acc + k * kRows, __uint_as_float(o[k]));
+    } else if (!moved) {
+      tmem_wait_ld(o);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) atomicAdd(acc + k * kRows, __uint_as_float(o[k]));
+    } else {
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = __ldcg(acc + k * kRows);
+      tmem_wait_ld(o);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) __stcg(acc + k * kRows, fmaf(v[k], f, __uint_as_float(o[k])));
+    }
+  }
+  if constexpr (IN_TMEM) tmem_wait_st();
+}
+// and at a problem's end the sum to O
+template <bool IN_TMEM>
+__device__ __noinline__ void unfold_row(uint32_t o_col, uint32_t t_col, int cols, const float *acc, uint32_t ref_at, float ref) {
+  const float f = ref_factor(ld_shared_f32(ref_at), ref);
+#pragma unroll 2
+  for (int d = 0; d < cols; d += 16, acc += 16 * kRows) {
+    uint32_t o[16], v[16];
+    if constexpr (IN_TMEM) {
+      tmem_ld16(t_col + d, v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__ldcg(acc + k * kRows));
+    }
+    tmem_ld16(o_col + d, o);
+    tmem_wait_ld(o);
+    if constexpr (IN_TMEM) tmem_wait_ld(v);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(fmaf(__uint_as_float(v[k]), f, __uint_as_float(o[k])));
+    tmem_st16(o_col + d, o);
+  }
+  tmem_wait_st();
+}
+
 enum Role { kSoftmax, kWidenKv, kProducts };
 
 // 128 packed rows of one sequence and kv head, and the tiles [t0, t1) of their keys that this CTA takes.
@@ -252,6 +330,7 @@ struct PromptShared {
   Problem problem[2];
   float row_mul[kRows];
   float row_top[2][kRows], row_sum[2][kRows];  // of the two halves of a tile's keys
+  float fold_ref[2][kRows];                    // of the sum of earlier tiles' O
   // The blocks of 32 tiles: of a widening warp the record pairs (kNoRecord: nothing to read); of a pair
   // of blocks of a tile {k scale, log2(v scale), 1 / v scale, there}.
   alignas(8) uint32_t record[WIDEN][64];  // (read by twos)
@@ -648,6 +727,8 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       const uint32_t pos = pr.pos0 + (pr.row0 + min(i, rows - 1)) / a.gqa;
       const uint32_t see_lo = a.window && pos >= a.window ? pos - a.window + 1 : 0, see_hi = pos + 1;
       float ref = -INFINITY, l = 0.0f;
+      auto fold_at = [&] { return part_values(a, gridDim.x) + ((size_t)pr.slot * D + half * (D / 2)) * kRows + i; };
+      const uint32_t fold_ref = smem_u32(&sh.fold_ref[half][i]);
       // bit = token of this thread's half of a tile: the keys that its row sees, and that are there
       auto visible = [&](uint32_t t) {
         const uint32_t k0 = (first + t * kTileBlocks) * kKv8Block + 32 * half;
@@ -736,6 +817,16 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         }
         l = fmaf(sum[0], block[0].z, fmaf(sum[1], block[1].z, l));
         tmem_wait_st();
+        if constexpr (kSplit) {
+          if (t != t0 && (t - t0) % P::kFold == 0) {  // O of the tiles before; this tile's begins anew
+            wait(bars.pv_done(tile - 1), (tile - 1) / 2);
+            __syncwarp();
+            tc_fence_after();
+            if (32u * (warp & 3) < rows)
+              fold_row<P::kTotal != 0>(tmem + lanes + P::kO + half * (D / 2), tmem + lanes + P::kTotal + half * (D / 2), D / 2, fold_at(),
+                                       fold_ref, ref, t - t0 == P::kFold);
+          }
+        }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(bars.p_full(tile));
@@ -747,6 +838,12 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
       wait(bars.pv_done(tiles + n_tiles - 1), (tiles + n_tiles - 1) / 2);
       __syncwarp();
       tc_fence_after();
+      if (kSplit && n_tiles > P::kFold) {
+        if (32u * (warp & 3) < rows)
+          unfold_row<P::kTotal != 0>(tmem + lanes + P::kO + half * (D / 2), tmem + lanes + P::kTotal + half * (D / 2), D / 2, fold_at(),
+                                     fold_ref, ref);
+        asm volatile("bar.sync 6, %0;\n" ::"n"(kSoft * 32) : "memory");  // parts go where the sums are
+      }
       const bool whole = pr.parts == 1;
       const size_t at = (size_t)pr.slot * kRows + i;
       float *const po = part_values(a, gridDim.x) + at * D;
@@ -991,15 +1088,15 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         if (elect_one()) {
           mbar_arrive(bars.s_done(tile));  // (passes on what the widening warps wrote for the softmax)
 #pragma unroll
-          for (int w = 0; w < kTerms; ++w)
+          for (int w = kTerms - 1; w >= 0; --w)  // (the small terms first: what is cut off goes by the sum so far)
             issue_ss<D / 16>(tmem + tile % kS * kTokens, q_tile + w * P::kQTerm, kRows * 128, k_tile(tile), kTokens * 128,
-                             umma_idesc_f16(kRows, kTokens), w > 0);
+                             umma_idesc_f16(kRows, kTokens), w < kTerms - 1);
           umma_commit(bars.s_done(tile));
         }
         __syncwarp();
       };
       product_s(tiles);
-      const bool begun = (sh.odd_records[tiles & 1] & kApart) != 0;  // O: add_far has
+      const bool begun = (sh.odd_records[tiles & 1] & kApart) != 0;
       if (pr.parts > 1 && lane == 0)
         part_list<D>(a, gridDim.x)[pr.slot] =
             PromptPart{pr.parts, blockIdx.x - pr.c0, pr.slot0, pr.c0, pr.r0, pr.row0, pr.rows, pr.head};
@@ -1012,11 +1109,13 @@ SX_DEV void prompt_role(const Kv8AttnArgs &a, uint8_t *smem_raw, PromptShared<Pr
         wait(bars.p_full(tile), tile / 2);
         __syncwarp();
         tc_fence_after();
+        // a sum of tiles begins with zeros, but the first where add_far has begun it
+        const bool add = kSplit && j % P::kFold == 0 && j > 0 ? false : j > 0 || begun;
         if (elect_one()) {
 #pragma unroll
           for (int w = 0; w < kTerms; ++w)
             issue_ts<kTokens / 16>(tmem + P::kO, tmem + (w ? P::kLow + tile % kS * (kTokens / 2) : tile % kS * kTokens),
-                                   v_tile(tile), D * 128, umma_idesc_f16(kRows, D), j > 0 || w > 0 || begun);
+                                   v_tile(tile), D * 128, umma_idesc_f16(kRows, D), add || w > 0);
           umma_commit(bars.pv_done(tile));
         }
         __syncwarp();

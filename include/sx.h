@@ -612,7 +612,8 @@ SX_API sx_status sx_dispatch_kv8_append(sx_engine *e, const sx_kv8 *c, sx_dtype 
  * V scale (2^-39 with up to 16 rows per kv head): one dominant key and n small ones of the same value may
  * be n times that apart from the exact sum.  A V scale far above the others' takes nothing from them,
  * whether the value that it comes from is masked, has no weight or dominates; with many rows per kv head,
- * records whose scale is over 2^10 (SX_BF16: 2^20) below another's take some 30 times as long.  Vectors 16-byte aligned, strides multiples of
+ * records whose scale is over 2^10 (SX_BF16: 2^20) below another's take some 30 times as long.  SX_F32 outputs are within about 2e-6 of
+ * the exact ones (2-norm, measured on up to 100000 keys of equal weight).  Vectors 16-byte aligned, strides multiples of
  * 16 bytes; num_q a multiple of num_kv, at most 64 q heads per kv head. */
 SX_API sx_status sx_dispatch_kv8_attn(sx_engine *e, const sx_kv8 *c, sx_dtype t, const void *q,
                                       void *out, uint32_t q_ld, uint32_t out_ld,

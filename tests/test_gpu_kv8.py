@@ -292,6 +292,47 @@ def test_attn_scales_far_apart(eng):
     check_attn(eng, "f32", 2, 1, 64, 16, [1, 4], [256, 64], cache=cache)
 
 
+@pytest.mark.parametrize("d,hkv,news,lens", [(64, 4, [1000, 900], [31000, 20000]), (128, 4, [1000, 900], [31000, 20000]), (256, 2, [1000, 900], [31000, 20000]),
+                                             (256, 8, [1] * 48, [8192 - 5 * i for i in range(48)]), (64, 8, [1] * 96, [8192 - 5 * i for i in range(96)])])
+def test_attn_f32_sums_do_not_wear_off(eng, d, hkv, news, lens):
+    """Keys of about equal weight and values of either sign: the tensor core cuts products off at 2^-24 of the
+    sum so far, toward zero, so that a sum of n loses sqrt(n) 2^-24 of itself.  Sums are of 512 keys at
+    most before they are added in f32: 1.4e-6, twice that for the sum's spread, and 1e-6 for the scores."""
+    cache = Cache([64], 64, hkv, d, 24)  # (for its methods; the pool is made on the GPU)
+    pages = [-(-n // 64) for n in lens]
+    g = torch.Generator(device="cuda").manual_seed(11)
+    total = sum(pages)
+    cache.data = (torch.randn(total, hkv, 4, 2, 16 * d, device="cuda", generator=g) * 60).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.uint8)
+    cache.scale = torch.full((total, hkv, 4, 2), 2.0 ** -6, device="cuda")
+    cache.table = torch.full((len(lens), max(pages)), -1, dtype=torch.int32, device="cuda")
+    order = torch.randperm(total, device="cuda", generator=g).to(torch.int32)
+    at = 0
+    for b, n in enumerate(pages):
+        cache.table[b, :n] = order[at:at + n]
+        at += n
+    q = torch.randn(sum(news), 2 * hkv * d, device="cuda", generator=g)
+    out = torch.empty_like(q)
+    start, kv_len, _ = rows_of(news, lens)
+    eng.kv8_attn(cache.kv8(), 0, q, out, start, kv_len, sum(news), 2 * hkv, d ** -0.5)
+    eng.sync()
+    # every tenth row is enough
+    keep = torch.arange(0, sum(news), 10 if max(news) > 1 else 1, device="cuda")
+    off = norm = 0.0
+    row = 0
+    for b, (n, m) in enumerate(zip(news, lens)):
+        mine = keep[(keep >= row) & (keep < row + n)]
+        if len(mine):
+            k, v = cache.values(b, m)
+            hide = torch.arange(m, device="cuda")[None] > (m - n + mine - row)[:, None]
+            for h in range(2 * hkv):
+                z = (q[mine, h * d:(h + 1) * d].double() @ k[:, h // 2].T * d ** -0.5).masked_fill_(hide, -math.inf)
+                want = torch.softmax(z, -1) @ v[:, h // 2]
+                off += float((out[mine, h * d:(h + 1) * d] - want).square().sum())
+                norm += float(want.square().sum())
+        row += n
+    assert math.sqrt(off / norm) <= 4e-6, math.sqrt(off / norm)
+
+
 @pytest.mark.parametrize("d,new,rows_form", [(64, 1, 39), (128, 2, 39), (256, 1, 39), (512, 1, 39), (64, 5, 32), (256, 5, 32)])
 @pytest.mark.parametrize("depth", [20.3, 25.4, 28.7])
 def test_attn_one_dominant_key_and_many_small_ones(eng, d, new, rows_form, depth):
