@@ -17,8 +17,10 @@
 // once per unit.  K and V stay in registers until the block's maxima have met in shared memory, are
 // converted by their owners, and leave through a byte tile that turns rows of tokens into the
 // record's pieces.  Measured: 64 prompts of 16 to 512 tokens (16 q and 8 kv heads of 256, bf16) 135 us,
-// 4.2 TB/s or 65 % of the measured copy rate; one token of 8 sessions 6.3 us, the latency of its chain of
-// loads (rows and lengths, page ids, the records' old bytes and scales).
+// 4.2 TB/s or 65 % of the measured copy rate, with 59 % of the issue slots used and warps that wait for their
+// loads most (4.0 of the stalls per issue, at the 46 % of an SM's warps that registers leave); one token of 8
+// sessions 6.5 us, the latency of its chain of loads (rows and lengths, page ids, the records' old bytes and
+// scales).
 #include "sx_host.h"
 #include "sx_kv8.cuh"
 #include "sx_launch.cuh"

@@ -27,16 +27,19 @@
 // bulk copies (a K or a V record a stage) and its own maximum, sum and output; they merge in shared
 // memory at the end of a problem, and CTAs that share a problem through the workspace: the last to
 // arrive merges (its order is that of the CTAs, so results repeat).  Runs are of 8 blocks at least, one
-// per warp (640 keys of one head of 256: 11.8 us; with 16 or 32, or uncut, 2 more).  Problems of up to three
+// per warp (640 keys of one head of 256: 11.9 us; with 16 or 32, or uncut, 2 more).  Problems of up to three
 // such steps more than a run are not cut, since a merge costs as much (16 rows in a window of 512:
-// 20 us; cut 25.3).
+// 20.4 us; cut 5 more).
 //
-// Measured: 64 rows on up to 8192 keys (16 q and 8 kv heads of 256, bf16) 180 us, 6.0 TB/s or 94 % of the
+// Measured: 64 rows on up to 8192 keys (16 q and 8 kv heads of 256, bf16) 179 us, 6.1 TB/s or 94 % of the
 // measured copy rate, the rest being starts and ends of 512 problems, where a CTA's copies run dry; 131k
-// keys of 8 heads of 128 for one f32 row 54.5 us (76 %); batches of heads of 512 102 %, of 128 93 %, of 64
-// 57 % (a block of 16 tokens costs as many instructions of softmax for a quarter of the bytes).  Two or
-// four blocks a warp at a time were slower below 256: 116 us for 110 with head size 128, 15.9 for 5.5 on
-// 127 keys with 64.  So were three or four CTAs an SM (89 and 106 us for 84 with 64).
+// keys of 8 heads of 128 for one f32 row 56.4 us (74 %); batches of heads of 512 101 %, of 128 92 %, of 64
+// 56 % (a block of 16 tokens costs as many instructions of softmax for a quarter of the bytes); of f32 rows
+// 99, 77 and 51 %; of 16 f32 rows per kv head 41 % (128, where 16 rows' output and scores spill) and 48 % (256).  A window
+// of 512 leaves 128 of 296 CTAs work, and a warp's ring two records: each of the five steps waits for its
+// own (20.4 us, floor 5.3).  Two or four blocks a warp at a time were slower below 256: 15.9 us for 5.5 on
+// 127 keys with 64, 5 % in full batches of 128.  So were three or four CTAs an SM (6 and 26 % in full
+// batches of 64).
 #include "sx_host.h"
 #include "sx_kv8.cuh"
 #include "sx_launch.cuh"

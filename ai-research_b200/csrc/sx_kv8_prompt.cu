@@ -29,11 +29,12 @@
 // which the tensor cores work 650.  Code size and spills count for as much as instructions (a kernel
 // unrolled throughout spent 20 cycles an instruction, fetching), so what runs seldom is out of line, loops
 // stay loops, and what describes a problem or a block is in shared memory.  Measured: 4 prompts of up to
-// 4096 tokens behind 4096 (16 q and 8 kv heads of 128, bf16) 520 us, 780 TFLOP/s or 46 % of the measured
-// rate, at the 1.5 GHz that the power cap leaves; 4 of 2048 tokens with head size 256 111.5 us; 5 drafts of
-// 32 sequences on up to 16000 keys (8 q heads, 1 kv head of 256) 58.5 us, where 30 tiles a CTA take 37 and
-// cutting the line, bringing Q, the output and the merge the rest.  Four softmax warps with whole rows took
-// 684 us for the first, one barrier for K and V 585.  A second look ahead for pages and scales, and Q
+// 4096 tokens behind 4096 (16 q and 8 kv heads of 128, bf16) 545 us, 743 TFLOP/s or 44 % of the measured
+// rate, at the 1.5 GHz that the power cap leaves (565 in a long row of calls); 4 of 2048 tokens with head size
+// 256 111.7 us (f32 rows 168.6); 5 drafts of 32 sequences on up to 16000 keys (8 q heads, 1 kv head of 256)
+// 58 us (f32 84), where 30 tiles a CTA take 37 -- 88 of a tile's 128 rows are padding -- and cutting the
+// line, bringing Q, the output and the merge the rest.  Four softmax warps with whole rows took a third more for
+// the first, one barrier for K and V an eighth.  A second look ahead for pages and scales, and Q
 // brought by the roles that wait for it, were slower by 5 and 10 %: more code.
 //
 // Work is the line of sx_kv8_attn.cu with problems of their own length: row group k of a sequence
