@@ -73,6 +73,21 @@ struct ProbsArgs {
   float c;
 };
 
+// A sum of many terms whose rounding is carried along: rows of 2^24 logits leave chains of 64 (two passes) to
+// 512 additions, which err alike where a row repeats itself (by 1e-6 of all its probabilities in two passes).
+struct LongSum {
+  float s = 0.0f, rest = 0.0f;
+  SX_DEV void scale(float f) {
+    s *= f;
+    rest *= f;
+  }
+  SX_DEV void add(float x) {
+    const float y = __fadd_rn(x, rest), t = __fadd_rn(s, y);
+    rest = __fsub_rn(y, __fsub_rn(t, s));
+    s = t;
+  }
+};
+
 // NV > 0: a thread holds NV float4 of the row in registers, so the row is read once; NV = 0: rows
 // of any length, read a second time (from L2) for the division.
 template <int NV>
@@ -104,16 +119,18 @@ __global__ void __launch_bounds__(kSampleThreads) probs_kernel(ProbsArgs a) {
     for (int k = 0; k < NV; ++k) m = fmaxf(fmaxf(m, fmaxf(x[k].x, x[k].y)), fmaxf(x[k].z, x[k].w));
   } else {
     const uint32_t end = min(a.n, (rank + 1) * seg);
+    LongSum sum;
     for (uint32_t i = i0; i < end; i += kSampleThreads * 4) {
       const float4 v = load4(z, i, end, az, -INFINITY);
       const float t = fmaxf(m, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
       if (t > m) {
-        s *= m == -INFINITY ? 0.0f : ex2((m - t) * a.c);
+        sum.scale(m == -INFINITY ? 0.0f : ex2((m - t) * a.c));
         m = t;
       }
       const float4 e = exps(v, local(m));
-      s += (e.x + e.y) + (e.z + e.w);
+      sum.add((e.x + e.y) + (e.z + e.w));
     }
+    s = sum.s;
   }
   const float mine = m;
   m = warp_max(m);
@@ -214,15 +231,17 @@ __global__ void __launch_bounds__(kChunkThreads) probs_divide_kernel(ProbsArgs a
   load_chunk(a, a.z + (size_t)row * a.z_ld, i0, x);
   pdl_launch_dependents();
   pdl_wait();
-  float m = -INFINITY, s = 0.0f;
+  float m = -INFINITY;
+  LongSum s;
   for (uint32_t k = lane; k < chunks; k += 32) {  // (the same order in every warp)
     const float2 v = __ldcg(part + (size_t)row * chunks + k);
     const float top = fmaxf(m, v.x);
-    s = s * (m == -INFINITY ? 1.0f : ex2((m - top) * a.c)) + v.y * (v.x == -INFINITY ? 1.0f : ex2((v.x - top) * a.c));
+    s.scale(m == -INFINITY ? 1.0f : ex2((m - top) * a.c));
+    s.add(v.y * (v.x == -INFINITY ? 1.0f : ex2((v.x - top) * a.c)));
     m = top;
   }
   const float all = warp_max(m), top = all == -INFINITY ? 0.0f : all;
-  const float sum = warp_sum(s * (m == -INFINITY ? 1.0f : ex2((m - all) * a.c)));
+  const float sum = warp_sum(s.s * (m == -INFINITY ? 1.0f : ex2((m - all) * a.c)));
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // -inf alone stays 0; a NaN or +inf made the sum NaN
   float *p = a.p + (size_t)row * a.p_ld;
   const bool ap = aligned16(p);

@@ -128,6 +128,20 @@ def test_probs_more_rows_than_one_pass_holds(eng, rows, n):
         assert ((out[r] - want).abs() <= want * 2.0 ** -19).all(), r
 
 
+@pytest.mark.parametrize("rows,n", [(1, (1 << 24) - 3), (2, 3_000_001), (24, (1 << 24) - 3)])
+def test_probs_long_rows_that_repeat_themselves(eng, rows, n):
+    """Equal parts err alike, and a plain chain of additions with them: 512 of 2^-25 in one pass, 64 in two."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    z = torch.randn(rows, 4096, device="cuda", generator=g).repeat(1, -(-n // 4096))[:, :n].contiguous()
+    out = torch.empty_like(z)
+    eng.probs(z, out, rows, n)
+    eng.sync()
+    for r in range(rows):
+        want = torch.softmax(z[r].double(), -1)
+        # the sum alone: what all of a row's probabilities have in common
+        assert abs(float(((out[r] - want) / want).mean())) <= 2.0 ** -21, r
+
+
 def test_probs_beside_attention(eng):
     """Captured in two graphs, long rows' probabilities and an attention that is cut over CTAs may run at
     the same time: they work in memory of their own."""
