@@ -610,8 +610,9 @@ SX_API sx_status sx_dispatch_kv8_append(sx_engine *e, const sx_kv8 *c, sx_dtype 
  * operands with f32 sums: e4m3 is exact in f16; q and p are split into two f16 terms for SX_F32
  * (22 bits) and rounded to f16 for SX_BF16.  A p also errs by up to 2^-32 of the row's largest p times
  * V scale (2^-39 with up to 16 rows per kv head): one dominant key and n small ones of the same value may
- * be n times that apart from the exact sum.  A V scale far above the others' takes nothing from them,
- * whether the value that it comes from is masked, has no weight or dominates; with many rows per kv head,
+ * be n times that apart from the exact sum.  A V scale far above the others' takes nothing from them
+ * (but from records of the least scale, 2^-60), whether the value that it comes from is masked, has no
+ * weight or dominates; with many rows per kv head,
  * records whose scale is over 2^10 (SX_BF16: 2^20) below another's take some 30 times as long.  SX_F32 outputs are within about 2e-6 of
  * the exact ones (2-norm, measured on up to 100000 keys of equal weight).  Vectors 16-byte aligned, strides multiples of
  * 16 bytes; num_q a multiple of num_kv, at most 64 q heads per kv head. */
