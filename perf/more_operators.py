@@ -133,7 +133,8 @@ def _rms(x):
 def _to_codes(u):
     top = u.abs().amax(-1, keepdim=True)
     top = torch.where(top >= TINY, top, 0.0)
-    return torch.round(u * torch.where(top > 0, 127.0 / top, 0.0)).to(torch.int8), top / 127.0
+    step = torch.full_like(top, 127.0) / top  # (one rounding: a number over a tensor is a reciprocal and a product)
+    return torch.round(u * torch.where(top > 0, step, 0.0)).to(torch.int8), top / 127.0
 
 
 def _plain_quantize(s):
