@@ -37,6 +37,7 @@ ENGINE_KV_F32 = 1
 
 DTYPE_F32 = 0
 DTYPE_BF16 = 1
+DTYPE_I8 = 2  # residual_norm's y
 KV8_K_EQ_V = 1
 KV8_V_NORM = 2
 NO_PAGE = 0xFFFFFFFF
@@ -124,6 +125,8 @@ class KV8(C.Structure):
 _CACHE = struct.Struct("@3Q6I")
 _APPEND_ARGS = struct.Struct("@9Q8If")
 _ATTN_ARGS = struct.Struct("@4Q6If")
+# sx_quantize_i8_args, sx_residual_norm_args, sx_gemm_i8_args, sx_gate_up_i8_args
+_I8_ARGS = tuple(map(struct.Struct, ("@4Q5If", "@7Q8I2f", "@5Q7I", "@7Q7I")))
 
 
 class TpShard(C.Structure):
@@ -344,6 +347,11 @@ _SIGS = {
     "sx_dispatch_probs": (_S, [_P, _P, _U32, _P, _U32, _U32, _U32, _F]),
     "sx_dispatch_verify": (_S, [_P, _P, _U32, _P, _U32, _P, _P, _P, _P, _P, _P, _U32, _U32,
                                 _U32]),
+    "sx_i8_args_bytes": (_U32, [_U32]),
+    "sx_dispatch_quantize_i8": (_S, [_P, C.c_char_p]),
+    "sx_dispatch_residual_norm": (_S, [_P, C.c_char_p]),
+    "sx_dispatch_gemm_i8": (_S, [_P, C.c_char_p]),
+    "sx_dispatch_gate_up_i8": (_S, [_P, C.c_char_p]),
     "sx_archive_create": (_S, [_P, _U32, _P, C.POINTER(_P)]),
     "sx_archive_destroy": (None, [_P]),
     "sx_archive_integrate": (_S, [_P, _P, _U64, _P, _P]),
@@ -385,6 +393,10 @@ def _check_layouts(L, path) -> None:
         if theirs != ours:
             raise ImportError(f"{path}: {name} is {theirs} bytes, this binding's mirror {ours}: "
                               "rebuild the library")
+    for i, block in enumerate(_I8_ARGS):
+        if L.sx_i8_args_bytes(i) != -(-block.size // 8) * 8:
+            raise ImportError(f"{path}: block {i} of the int8 operators' arguments has another "
+                              "length than this binding's mirror: rebuild the library")
 
 
 def declared_symbols() -> list[str]:
@@ -711,6 +723,44 @@ class Engine:
         check(lib().sx_dispatch_verify(
             self.h, _ptr(target), target_ld, _ptr(draft), draft_ld, _ptr(tok), _ptr(n_draft),
             _ptr(u_accept), _ptr(u_sample), _ptr(out), _ptr(accepted), seqs, drafts, vocab))
+
+    # --- the feed-forward block in 8-bit whole numbers
+    def quantize_i8(self, dtype, x, q, scale, rows, n, norm_w=None, eps=1e-6, x_ld=0, q_ld=0):
+        """sx_dispatch_quantize_i8: rows of x (normalised with the gain norm_w, or as they are) to
+        int8 codes and one scale each (row strides in elements; 0: contiguous rows)."""
+        status = lib().sx_dispatch_quantize_i8(self.h, _I8_ARGS[0].pack(
+            _ptr(x) or 0, _ptr(norm_w) or 0, _ptr(q) or 0, _ptr(scale) or 0, dtype, x_ld or n,
+            q_ld or n, rows, n, eps))
+        if status:
+            check(status)
+
+    def residual_norm(self, x, r_dtype, r, x_out, y_dtype, y, rows, n, post_w=None, pre_w=None,
+                      scalar=1.0, eps=1e-6, y_scale=None, x_ld=0, r_ld=0, x_out_ld=0, y_ld=0):
+        """sx_dispatch_residual_norm: x_out = (x + rms(r) * post_w) * scalar and
+        y = rms(x_out) * pre_w, in f32, bf16 or (y_scale) int8; y None: x_out alone."""
+        status = lib().sx_dispatch_residual_norm(self.h, _I8_ARGS[1].pack(
+            _ptr(x) or 0, _ptr(r) or 0, _ptr(post_w) or 0, _ptr(pre_w) or 0, _ptr(x_out) or 0,
+            _ptr(y) or 0, _ptr(y_scale) or 0, r_dtype, y_dtype, x_ld or n, r_ld or n,
+            x_out_ld or n, y_ld or n, rows, n, scalar, eps))
+        if status:
+            check(status)
+
+    def gemm_i8(self, x, x_scale, w, w_scale, dtype, y, t, n, k, x_ld=0, w_ld=0, y_ld=0):
+        """sx_dispatch_gemm_i8: y[t][n] = x_scale[t] w_scale[n] sum_k x[t][k] w[n][k]."""
+        status = lib().sx_dispatch_gemm_i8(self.h, _I8_ARGS[2].pack(
+            _ptr(x) or 0, _ptr(x_scale) or 0, _ptr(w) or 0, _ptr(w_scale) or 0, _ptr(y) or 0, dtype,
+            x_ld or k, w_ld or k, y_ld or n, t, n, k))
+        if status:
+            check(status)
+
+    def gate_up_i8(self, x, x_scale, wg, wg_scale, wu, wu_scale, dtype, y, t, n, k, x_ld=0, w_ld=0,
+                   y_ld=0):
+        """sx_dispatch_gate_up_i8: gelu_tanh(gate) * up of two such products."""
+        status = lib().sx_dispatch_gate_up_i8(self.h, _I8_ARGS[3].pack(
+            _ptr(x) or 0, _ptr(x_scale) or 0, _ptr(wg) or 0, _ptr(wu) or 0, _ptr(wg_scale) or 0,
+            _ptr(wu_scale) or 0, _ptr(y) or 0, dtype, x_ld or k, w_ld or k, y_ld or n, t, n, k))
+        if status:
+            check(status)
 
     def unpack_q4(self, w_packed, out, m, k):
         check(lib().sx_dispatch_unpack_q4(self.h, _ptr(w_packed), _ptr(out), m, k))

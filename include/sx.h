@@ -550,7 +550,7 @@ SX_API uint32_t sx_pages_free_count(const sx_pages *p);
  * device before the step that uses it. */
 SX_API const uint32_t *sx_pages_table(const sx_pages *p);
 
-typedef enum { SX_F32 = 0, SX_BF16 = 1 } sx_dtype;
+typedef enum { SX_F32 = 0, SX_BF16 = 1, SX_I8 = 2 /* sx_dispatch_residual_norm's y only */ } sx_dtype;
 
 /* A paged 8-bit cache of one layer in device memory.  Every 16 tokens of one kv head are a K
  * record and a V record of 16 head_dim e4m3 bytes; a stored value is its e4m3 number times the
@@ -676,6 +676,85 @@ SX_API sx_status sx_dispatch_verify(sx_engine *e, const float *target, uint32_t 
                                     const uint32_t *n_draft, const float *u_accept,
                                     const float *u_sample, uint32_t *out, uint32_t *accepted,
                                     uint32_t seqs, uint32_t drafts, uint32_t vocab);
+
+/* ---------------------------------------------------------------------------------------
+ * The feed-forward block of a layer in 8-bit whole numbers (new: the reference multiplies Q4_0 and
+ * Q8_0 blocks by f32 activations).  Both operands of a product are int8: a row of activations and a
+ * row of weights (an output channel) have one f32 scale each, made by sx_dispatch_quantize_i8, and
+ * sums of products are whole numbers in 32 bits, so their order does not matter:
+ *
+ *   residual_norm -> gate_up_i8 -> quantize_i8 -> gemm_i8 -> residual_norm
+ *
+ * All four are asynchronous on the engine stream, use no memory but their arguments' and can be
+ * captured in a CUDA graph; calls on streams of their own may overlap.  Arguments come in one block; a
+ * row stride `*_ld` counts elements.  0 rows are no work.  Inputs and outputs must not overlap but
+ * where it says so.
+ * ------------------------------------------------------------------------------------- */
+/* Rows to codes: u = x (norm_w NULL) or x * norm_w, f32 products; a = the largest |u| of the row;
+ *   q = u * (127 / a) rounded to the nearest whole number, ties to even (quotient and product in f32),
+ *   scale = a / 127, with norm_w times 1 / sqrt(mean(x^2) + eps):
+ * q * scale is the row, or its RMS norm with the gain norm_w (whose own factor cancels out of q).  Rows
+ * whose a is below 2^-100 count as zeros (codes and scale 0); a row that holds a NaN or an infinity, or
+ * with norm_w one whose squares' sum passes f32, has codes 0 and scale NaN, so what is computed from it
+ * is NaN.  Rows of a weight matrix make the codes of its output channels.  n a multiple of 16, below
+ * 131072; x 16-byte aligned with a stride of 16 bytes' multiple, q likewise; norm_w 16-byte aligned. */
+typedef struct {
+  const void *x;       /* [rows] of n, dtype SX_F32 or SX_BF16 */
+  const float *norm_w; /* [n] or NULL                          */
+  int8_t *q;           /* [rows] of n                          */
+  float *scale;        /* [rows]                               */
+  uint32_t dtype, x_ld, q_ld, rows, n;
+  float eps;
+} sx_quantize_i8_args;
+SX_API sx_status sx_dispatch_quantize_i8(sx_engine *e, const sx_quantize_i8_args *a);
+
+/* The seam of two blocks, per row:
+ *   h = r / sqrt(mean(r^2) + eps) * post_w   (post_w NULL: h = r)
+ *   x_out = (x + h) * scalar
+ *   y = x_out / sqrt(mean(x_out^2) + eps) * pre_w
+ * in f32; y in y_dtype, SX_I8 as sx_dispatch_quantize_i8 of x_out with gain pre_w (scales to y_scale,
+ * else NULL).  y NULL: x_out alone, without pre_w.  x_out may be x.  Sizes and alignment as there. */
+typedef struct {
+  const float *x;       /* [rows] of n: the residual stream             */
+  const void *r;        /* [rows] of n, r_dtype: what the block computed */
+  const float *post_w;  /* [n] or NULL                                  */
+  const float *pre_w;   /* [n]                                          */
+  float *x_out;         /* [rows] of n                                  */
+  void *y;              /* [rows] of n, y_dtype                         */
+  float *y_scale;       /* [rows], with SX_I8                           */
+  uint32_t r_dtype, y_dtype, x_ld, r_ld, x_out_ld, y_ld, rows, n;
+  float scalar, eps;
+} sx_residual_norm_args;
+SX_API sx_status sx_dispatch_residual_norm(sx_engine *e, const sx_residual_norm_args *a);
+
+/* y[t][n] = (float) (sum_k x[t][k] w[n][k]) * x_scale[t] * w_scale[n], rounded to dtype once.
+ * k a multiple of 16, below 131072 (so that sums of any codes, -128 too, stay below 2^31); x and w
+ * 16-byte aligned with strides that are multiples of 16; y aligned to its elements, any stride.  Bytes
+ * between a row's end and its stride are not used.  t and n below 2^31. */
+typedef struct {
+  const int8_t *x;      /* [t] of k */
+  const float *x_scale; /* [t]      */
+  const int8_t *w;      /* [n] of k */
+  const float *w_scale; /* [n]      */
+  void *y;              /* [t] of n, dtype SX_F32 or SX_BF16 */
+  uint32_t dtype, x_ld, w_ld, y_ld, t, n, k;
+} sx_gemm_i8_args;
+SX_API sx_status sx_dispatch_gemm_i8(sx_engine *e, const sx_gemm_i8_args *a);
+
+/* y = gelu_tanh(g) * u, g and u as sx_dispatch_gemm_i8 of (wg, wg_scale) and (wu, wu_scale) in f32,
+ * gelu_tanh(g) = g / 2 (1 + tanh(0.7978845608 (g + 0.044715 g^3))).  Limits as there. */
+typedef struct {
+  const int8_t *x;
+  const float *x_scale;
+  const int8_t *wg, *wu; /* [n] of k each, row stride w_ld */
+  const float *wg_scale, *wu_scale;
+  void *y;
+  uint32_t dtype, x_ld, w_ld, y_ld, t, n, k;
+} sx_gate_up_i8_args;
+SX_API sx_status sx_dispatch_gate_up_i8(sx_engine *e, const sx_gate_up_i8_args *a);
+/* sizeof of the blocks above (0 quantize_i8, 1 residual_norm, 2 gemm_i8, 3 gate_up_i8), for bindings that
+ * lay them out themselves to compare with */
+SX_API uint32_t sx_i8_args_bytes(uint32_t which);
 
 #ifdef __cplusplus
 }
