@@ -1,8 +1,15 @@
 // sx_i8_gemm.cu -- products of int8 rows on the tcgen05 tensor cores (include/sx.h, sx_dispatch_gemm_i8 and
 // sx_dispatch_gate_up_i8).
 //
-// A CTA takes 128 rows of x and 128 columns of y: the tiles come by TMA, 128 codes of K a stage, and
-// tcgen05.mma (kind::i8) sums them in 32 bits in tensor memory.  gate_up: 64 columns of each matrix.
+// Two CTAs of a cluster take a tile of 256 rows of x and BN columns of y (gate_up: BN / 2 of each matrix), 128
+// rows in the tensor memory of each: tcgen05.mma of the pair (kind::i8, 32-bit sums) reads 128 rows of x and half
+// of the columns' weights from each CTA's shared memory, so both operands are fetched once per pair.  The grid is
+// one pair per two SMs, which goes through the tiles; tensor memory holds two tiles' sums, so that one is
+// scaled and stored while the next is summed.  Warps of a CTA:
+//   0       TMA: 128 codes of K a stage, completing on the leader's barrier
+//   1       the leader's issues the products and commits stages and sums to both CTAs
+//   2 .. 5  sums to values, 32 rows each, staged in shared memory and stored by TMA (rows of y that do not
+//           begin and end on 16 bytes: by lanes)
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -16,25 +23,79 @@
 namespace sx {
 namespace {
 
-constexpr uint32_t kBM = 128, kBN = 128, kBK = 128, kStages = 4;
-constexpr uint32_t kATile = kBM * kBK, kBTile = kBN * kBK, kStage = kATile + kBTile;
-constexpr uint32_t kSmem = kStages * kStage + 1024;
-constexpr int kThreads = 6 * 32;
+constexpr uint32_t kBM = 256, kBK = 128;        // of a pair
+constexpr uint32_t kHalf = kBM / 2;             // rows of a CTA
+constexpr int kEpiWarps = 4, kThreads = (2 + kEpiWarps) * 32;
+constexpr uint32_t kBox = 4096;                 // 32 rows of 128 bytes of y
+constexpr uint32_t kTmemCols = 512, kAccCols = 256;
+constexpr uint32_t kGroup = 8;                  // tiles of rows that are taken together, for L2
 
-SX_DEV void tma_load_2d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
+template <uint32_t BN>
+struct PairShape {
+  static constexpr uint32_t kATile = kHalf * kBK, kBTile = BN / 2 * kBK, kStage = kATile + kBTile;
+  static constexpr uint32_t kStages = 196608 / kStage;
+  static constexpr uint32_t kSmem = kStages * kStage + kEpiWarps * 2 * kBox + 1024;  // + alignment
+};
+
+// ---- TMA, cluster and pair wrappers
+SX_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+SX_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+// the address of a shared-memory word of this CTA in CTA `rank` of the cluster
+SX_DEV uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+SX_DEV void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+}
+// 2-D tiled load into this CTA's shared memory that completes on a barrier of either CTA of the pair
+SX_DEV void tma_load_pair(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], "
       "[%1, {%2, %3}], [%4];\n" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-// D[tmem] (+)= A[smem desc] . B[smem desc]^T of int8, 32 of K
-SX_DEV void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+SX_DEV void tma_store_2d(const CUtensorMap *map, int32_t x, int32_t y, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(src)
+               : "memory");
+}
+SX_DEV void bulk_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
+template <int N>
+SX_DEV void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
+}
+SX_DEV void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
+
+SX_DEV void tmem_alloc_pair(uint32_t dst_smem, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(dst_smem), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+}
+SX_DEV void tmem_dealloc_pair(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(cols) : "memory");
+}
+// D[tmem] (+)= A[smem desc] . B[smem desc]^T of int8, 32 of K, A and B from both CTAs of the pair
+SX_DEV void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
+}
+// arrive once on the barrier at this place in both CTAs when every operation this thread issued has completed
+SX_DEV void umma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
+               "h"((uint16_t)3)
+               : "memory");
 }
 // Instruction descriptor: D s32, A and B s8, both K-major, N >> 3, M >> 4.
 constexpr uint32_t umma_idesc_i8(uint32_t m, uint32_t n) {
@@ -42,39 +103,56 @@ constexpr uint32_t umma_idesc_i8(uint32_t m, uint32_t n) {
 }
 
 struct Maps {
-  CUtensorMap x, w[2];
+  CUtensorMap x, w[2], y;
 };
+struct Tiles {
+  uint32_t rows, cols, all;  // tiles of rows and of columns
+  uint32_t lanes;            // rows of y do not begin and end on 16 bytes: lanes store them
+};
+// Tile i: kGroup tiles of rows go through all columns together, so what runs at a time reads few of either.
+SX_DEV void tile_at(const Tiles &g, uint32_t i, uint32_t *row, uint32_t *col) {
+  const uint32_t band = i / (kGroup * g.cols), in = i - band * kGroup * g.cols;
+  const uint32_t high = min(kGroup, g.rows - band * kGroup);
+  *col = in / high;
+  *row = band * kGroup + in % high;
+}
 
-template <typename T, bool GATED>
-__global__ void __launch_bounds__(kThreads, 1) gemm_i8_kernel(const __grid_constant__ Maps maps, const __grid_constant__ I8Args a) {
+template <typename T, bool GATED, uint32_t BN>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_i8_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ I8Args a, const __grid_constant__ Tiles g) {
+  using S = PairShape<BN>;
+  constexpr uint32_t kStages = S::kStages, kCols = GATED ? BN / 2 : BN;  // columns of y
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kStages + 1];
+  __shared__ __align__(8) uint64_t bars[2 * kStages + 4];
   __shared__ uint32_t tmem_slot, abort_flag;
-  constexpr uint32_t kCols = GATED ? kBN / 2 : kBN;  // of y
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __shared__ __align__(16) float col_scale[kEpiWarps][GATED ? 2 : 1][32];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_rank();
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u, bar0 = smem_u32(bars);
-  auto full = [&](uint32_t s) { return bar0 + 8 * s; };
-  auto empty = [&](uint32_t s) { return bar0 + 8 * (kStages + s); };
-  const uint32_t done = bar0 + 16 * kStages;
-  const uint32_t m0 = blockIdx.x * kBM, n0 = blockIdx.y * kCols, steps = (a.k + kBK - 1) / kBK;
+  auto full = [&](uint32_t s) { return bar0 + 8 * s; };                   // the leader's: both CTAs' copies
+  auto empty = [&](uint32_t s) { return bar0 + 8 * (kStages + s); };      // each CTA's
+  auto sums_full = [&](uint32_t c) { return bar0 + 8 * (2 * kStages + c); };
+  auto sums_empty = [&](uint32_t c) { return bar0 + 8 * (2 * kStages + 2 + c); };  // the leader's
   volatile uint32_t *const stop = &abort_flag;
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < kStages; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    mbar_init(done, 1);
+    for (uint32_t c = 0; c < 2; ++c) {
+      mbar_init(sums_full(c), 1);
+      mbar_init(sums_empty(c), 2 * kEpiWarps);
+    }
     abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 0) {
-    tmem_alloc(smem_u32(&tmem_slot), kBN);
-    tmem_relinquish();
-  }
+  __syncwarp();
+  if (warp == 0) tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
   tc_fence_before();
   __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  // A wait that runs out ends this CTA's waiting: what follows is skipped, and the error word says so.
   auto wait = [&](uint32_t bar, uint32_t parity) {
     if (*stop) return false;
     if (mbar_wait_bounded(bar, parity & 1)) return true;
@@ -82,66 +160,145 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_i8_kernel(const __grid_const
     raise_error(a.err, kDevWaitTimeout);
     return false;
   };
+  const uint32_t pair = blockIdx.x / 2, pairs = gridDim.x / 2, steps = (a.k + kBK - 1) / kBK;
   pdl_launch_dependents();
   pdl_wait();
-  uint32_t issued = 0;
+  uint32_t it = 0;  // stages used, over all tiles
   if (warp == 0 && lane == 0) {
-    for (uint32_t i = 0; i < steps; ++i) {
-      const uint32_t s = i % kStages, st = base + s * kStage;
-      if (i >= kStages && !wait(empty(s), i / kStages - 1)) break;
-      mbar_arrive_expect_tx(full(s), kStage);
-      tma_load_2d(st, &maps.x, i * kBK, m0, full(s));
-      tma_load_2d(st + kATile, &maps.w[0], i * kBK, n0, full(s));
-      if constexpr (GATED) tma_load_2d(st + kATile + kBTile / 2, &maps.w[1], i * kBK, n0, full(s));
-      issued = i + 1;
+    for (uint32_t i = pair; i < g.all; i += pairs) {
+      uint32_t row, col;
+      tile_at(g, i, &row, &col);
+      const int32_t x_row = row * kBM + rank * kHalf;
+      const int32_t w_row = GATED ? col * kCols : col * kCols + rank * (BN / 2);
+      const CUtensorMap *const w = GATED && rank ? &maps.w[1] : &maps.w[0];
+      bool ok = true;
+      for (uint32_t k = 0; k < steps; ++k, ++it) {
+        const uint32_t s = it % kStages, at = base + s * S::kStage, bar = in_cta(full(s), 0);
+        if (it >= kStages && !(ok = wait(empty(s), it / kStages - 1))) break;
+        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * S::kStage);
+        tma_load_pair(at, &maps.x, k * kBK, x_row, bar);
+        tma_load_pair(at + S::kATile, w, k * kBK, w_row, bar);
+      }
+      if (!ok) break;
     }
-  } else if (warp == 1 && lane == 0) {
-    for (uint32_t i = 0; i < steps; ++i) {
-      const uint32_t s = i % kStages, st = base + s * kStage;
-      if (!wait(full(s), i / kStages)) break;
+  } else if (warp == 1 && lane == 0 && rank == 0) {
+    uint32_t n = 0;
+    for (uint32_t i = pair; i < g.all; i += pairs, ++n) {
+      const uint32_t d = tmem + n % 2 * kAccCols;
+      if (n >= 2 && !wait(sums_empty(n & 1), n / 2 - 1)) break;
       tc_fence_after();
-      const uint64_t x = umma_desc_sw128(st), w = umma_desc_sw128(st + kATile);
+      bool ok = true;
+      for (uint32_t k = 0; k < steps; ++k, ++it) {
+        const uint32_t s = it % kStages, at = base + s * S::kStage;
+        if (!(ok = wait(full(s), it / kStages))) break;
+        tc_fence_after();
+        const uint64_t x = umma_desc_sw128(at), w = umma_desc_sw128(at + S::kATile);
 #pragma unroll
-      for (uint32_t k = 0; k < kBK / 32; ++k) umma_i8(tmem, x + 2 * k, w + 2 * k, umma_idesc_i8(kBM, kBN), i > 0 || k > 0);
-      umma_commit(empty(s));
+        for (uint32_t j = 0; j < kBK / 32; ++j) umma_i8_pair(d, x + 2 * j, w + 2 * j, umma_idesc_i8(kBM, BN), k > 0 || j > 0);
+        umma_commit_pair(empty(s));
+      }
+      if (!ok) break;
+      umma_commit_pair(sums_full(n & 1));
     }
-    umma_commit(done);
   } else if (warp >= 2) {
-    const uint32_t q = warp & 3, t = m0 + 32 * q + lane;
-    const bool ok = wait(done, 0);
-    __syncwarp();
-    tc_fence_after();
-    if (__all_sync(0xffffffffu, ok)) {
-      const float xs = t < a.t ? a.x_scale[t] : 0.0f;
-      T *const y = static_cast<T *>(a.y) + (size_t)min(t, a.t - 1) * a.y_ld;
+    const uint32_t q = warp & 3, boxes = base + kStages * S::kStage + (warp - 2) * 2 * kBox;
+    float(&cs)[GATED ? 2 : 1][32] = col_scale[warp - 2];
+    constexpr uint32_t kBoxCols = 128 / sizeof(T);
+    uint32_t n = 0, stored = 0;
+    for (uint32_t i = pair; i < g.all; i += pairs, ++n) {
+      uint32_t row, col;
+      tile_at(g, i, &row, &col);
+      const uint32_t t0 = row * kBM + rank * kHalf + 32 * q, n0 = col * kCols, src = tmem + ((32 * q) << 16) + n % 2 * kAccCols;
+      const float xs = t0 + lane < a.t ? a.x_scale[t0 + lane] : 0.0f;
+      const bool ok = wait(sums_full(n & 1), n / 2);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
 #pragma unroll 1
       for (uint32_t c = 0; c < kCols; c += 32) {
-        uint32_t r[32], u[32];
-        tmem_ld32(tmem + ((32 * q) << 16) + c, r);
-        if constexpr (GATED) tmem_ld32(tmem + ((32 * q) << 16) + kBN / 2 + c, u);
+        uint32_t r[32], u[GATED ? 32 : 1];
+        tmem_ld32(src + c, r);
+        if constexpr (GATED) tmem_ld32(src + BN / 2 + c, u);
+        const uint32_t nc = n0 + c + lane;
+        __syncwarp();  // the scales of the columns before have been read
+        cs[0][lane] = nc < a.n ? a.w_scale[0][nc] : 0.0f;
+        if constexpr (GATED) cs[1][lane] = nc < a.n ? a.w_scale[1][nc] : 0.0f;
+        const uint32_t box = boxes + stored % 2 * kBox, half = sizeof(T) == 2 ? c / 32 % 2 : 0;
+        if (half == 0) {
+          if (lane == 0) bulk_wait_read<1>();  // the store from this box before has read it
+        }
+        __syncwarp();
         tmem_wait_ld(r);
         if constexpr (GATED) tmem_wait_ld(u);
+        float v[32];
 #pragma unroll
         for (uint32_t j = 0; j < 32; ++j) {
-          const uint32_t n = n0 + c + j;
-          if (t < a.t && n < a.n) {
-            float v = i8_value((int32_t)r[j], xs, a.w_scale[0][n]);
-            if constexpr (GATED) v = i8_gated(v, i8_value((int32_t)u[j], xs, a.w_scale[1][n]));
-            y[n] = i8_out<T>(v);
-          }
+          v[j] = i8_value((int32_t)r[j], xs, cs[0][j]);
+          if constexpr (GATED) v[j] = i8_gated(v[j], i8_value((int32_t)u[j], xs, cs[GATED ? 1 : 0][j]));
         }
+        const uint32_t line = box + lane * 128, sw = lane & 7;
+#pragma unroll
+        for (uint32_t j = 0; j < 32 * sizeof(T) / 16; ++j) {
+          uint32_t w[4];
+#pragma unroll
+          for (uint32_t e = 0; e < 4; ++e) {
+            if constexpr (sizeof(T) == 4) {
+              w[e] = __float_as_uint(v[4 * j + e]);
+            } else {
+              const __nv_bfloat162 b = __floats2bfloat162_rn(v[8 * j + 2 * e], v[8 * j + 2 * e + 1]);
+              w[e] = *reinterpret_cast<const uint32_t *>(&b);
+            }
+          }
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};\n" ::"r"(line + (((half * 4 + j) ^ sw) << 4)), "r"(w[0]), "r"(w[1]),
+                       "r"(w[2]), "r"(w[3])
+                       : "memory");
+        }
+        if (sizeof(T) == 2 && half == 0 && c + 32 < kCols) continue;
+        const uint32_t c0 = n0 + c - half * 32;
+        if (!g.lanes) {
+          fence_proxy_async();  // generic-proxy writes -> the TMA engine's reads
+          __syncwarp();
+          if (lane == 0 && c0 < a.n && t0 < a.t) {
+            tma_store_2d(&maps.y, (int32_t)c0, (int32_t)t0, box);  // (not what is past t and n)
+            bulk_commit();
+          }
+        } else {
+          __syncwarp();
+#pragma unroll 1
+          for (uint32_t rr = 0; rr < 32 && t0 + rr < a.t; ++rr) {
+            T *const y = static_cast<T *>(a.y) + (size_t)(t0 + rr) * a.y_ld;
+            for (uint32_t e = lane; e < kBoxCols && c0 + e < a.n; e += 32) {
+              const uint32_t at = box + rr * 128 + (((e * (uint32_t)sizeof(T) / 16) ^ (rr & 7)) << 4) + e * (uint32_t)sizeof(T) % 16;
+              if constexpr (sizeof(T) == 4) {
+                float f;
+                asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(f) : "r"(at) : "memory");
+                y[c0 + e] = f;
+              } else {
+                uint16_t h;
+                asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(h) : "r"(at) : "memory");
+                y[c0 + e] = __ushort_as_bfloat16(h);
+              }
+            }
+          }
+          __syncwarp();
+        }
+        ++stored;
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(in_cta(sums_empty(n & 1), 0));
     }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0 && lane == 0 && *stop)  // a stopped CTA waits (bounded) for the copies that it issued
-    for (uint32_t s = 0; s < kStages; ++s)
-      if (issued > s) mbar_wait_bounded(full(s), ((issued - 1 - s) / kStages) & 1);
+  if (threadIdx.x == 0 && rank == 0 && *stop)  // a stopped pair waits (bounded) for the copies that it issued
+    for (uint32_t s = 0; s < kStages && s < it; ++s) mbar_wait_bounded(full(s), ((it - 1 - s) / kStages) & 1);
   __syncwarp();
+  cluster_sync();  // no CTA leaves while the other's products, copies or arrivals may reach it
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, kBN);
+    tmem_dealloc_pair(tmem, kTmemCols);
   }
 }
 
@@ -157,32 +314,58 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
-// rows of k codes, in boxes of `box` rows x 128 codes
-bool encode_rows(CUtensorMap *map, const int8_t *p, uint32_t rows, uint32_t k, uint32_t ld, uint32_t box_rows) {
-  auto encode = tensor_map_encoder();
-  const cuuint64_t dims[2] = {k, rows}, strides[1] = {ld};
-  const cuuint32_t box[2] = {kBK, box_rows}, one[2] = {1, 1};
-  return encode && encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+bool encode(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t cols, uint64_t rows, uint64_t ld_bytes, uint32_t box_cols,
+            uint32_t box_rows) {
+  auto fn = tensor_map_encoder();
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld_bytes};
+  const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
+  return fn && fn(map, type, 2, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <bool GATED>
-cudaError_t launch_gemm(uint32_t dtype, const I8Args &a, cudaStream_t s) {
-  Maps maps;
-  constexpr uint32_t cols = GATED ? kBN / 2 : kBN;
-  if (!encode_rows(&maps.x, a.x, a.t, a.k, a.x_ld, kBM) || !encode_rows(&maps.w[0], a.w[0], a.n, a.k, a.w_ld, cols)) return cudaErrorInvalidValue;
-  if (GATED && !encode_rows(&maps.w[1], a.w[1], a.n, a.k, a.w_ld, cols)) return cudaErrorInvalidValue;
-  auto kern = dtype == SX_F32 ? gemm_i8_kernel<float, GATED> : gemm_i8_kernel<__nv_bfloat16, GATED>;
-  return launch_chained(kern, dim3((a.t + kBM - 1) / kBM, (a.n + cols - 1) / cols), dim3(kThreads), kSmem, s, 1, maps, a);
+using PairKernel = void (*)(const Maps, const I8Args, const Tiles);
+struct PairVariant {
+  PairKernel fn;
+  uint32_t bn, smem;
+};
+template <typename T, bool GATED>
+PairVariant pair_variant(uint32_t bn) {
+  return {gemm_i8_pair_kernel<T, GATED, 256>, 256, PairShape<256>::kSmem};
+}
+PairVariant pair_variant(uint32_t dtype, bool gated, uint32_t bn) {
+  if (dtype == SX_F32) return gated ? pair_variant<float, true>(bn) : pair_variant<float, false>(bn);
+  return gated ? pair_variant<__nv_bfloat16, true>(bn) : pair_variant<__nv_bfloat16, false>(bn);
+}
+
+cudaError_t launch_pair(uint32_t dtype, bool gated, const I8Args &a, int num_sms, cudaStream_t s) {
+  const PairVariant v = pair_variant(dtype, gated, 256);
+  const uint32_t cols = gated ? v.bn / 2 : v.bn, es = dtype == SX_F32 ? 4 : 2;
+  Tiles g;
+  g.rows = (a.t + kBM - 1) / kBM;
+  g.cols = (a.n + cols - 1) / cols;
+  g.all = g.rows * g.cols;
+  // (a TMA store writes whole 16 bytes, those of a row's end too)
+  g.lanes = ((uintptr_t)a.y | (uintptr_t)a.y_ld * es | (uintptr_t)a.n * es) % 16 != 0;
+  Maps maps{};
+  bool ok = encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.k, a.t, a.x_ld, kBK, kHalf);
+  for (int i = 0; i < (gated ? 2 : 1); ++i) ok = ok && encode(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, v.bn / 2);
+  if (!g.lanes)
+    ok = ok && encode(&maps.y, dtype == SX_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.n, a.t,
+                      (uint64_t)a.y_ld * es, 128 / es, 32);
+  if (!ok) return cudaErrorInvalidValue;
+  return launch_chained(v.fn, dim3(2 * std::min<uint32_t>(g.all, num_sms / 2)), dim3(kThreads), v.smem, s, 2, maps, a, g);
 }
 
 }  // namespace
 
 cudaError_t prepare_gemm_i8() {
-  for (auto k : {gemm_i8_kernel<float, false>, gemm_i8_kernel<float, true>, gemm_i8_kernel<__nv_bfloat16, false>, gemm_i8_kernel<__nv_bfloat16, true>}) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem);
-    if (e != cudaSuccess) return e;
-  }
+  for (uint32_t dtype : {SX_F32, SX_BF16})
+    for (bool gated : {false, true})
+      for (uint32_t bn : {256u}) {
+        const PairVariant v = pair_variant(dtype, gated, bn);
+        const cudaError_t e = cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem);
+        if (e != cudaSuccess) return e;
+      }
   return cudaSuccess;
 }
 
@@ -210,12 +393,13 @@ sx_status dispatch_i8(const char *what, sx_engine *e, uint32_t dtype, sx::I8Args
   if (al % 16 != 0) return bad("x and weights must be 16-byte aligned and their strides multiples of 16");
   if ((uintptr_t)a.y % (dtype == SX_F32 ? 4 : 2) != 0) return bad("y must be aligned to its elements");
   if (a.t >= (1u << 31) || a.n >= (1u << 31)) return bad("t and n must be below 2^31");
+  if ((uint64_t)a.t * a.n >= (1ull << 42)) return bad("t * n must be below 2^42");  // (tiles are counted in 32 bits)
   if (!e) return bad("null engine");
   if (a.t == 0) return SX_OK;
   const cudaError_t ce = cudaSetDevice(e->device);
   if (ce != cudaSuccess) return sx_host_cuda_status(ce, "cudaSetDevice");
   a.err = e->err_dev;
-  return sx_host_cuda_status(gated ? sx::launch_gemm<true>(dtype, a, e->stream) : sx::launch_gemm<false>(dtype, a, e->stream), what);
+  return sx_host_cuda_status(sx::launch_pair(dtype, gated, a, e->num_sms, e->stream), what);
 }
 
 }  // namespace
