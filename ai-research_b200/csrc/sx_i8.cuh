@@ -32,4 +32,8 @@ SX_DEV float i8_out<float>(float v) { return v; }
 template <>
 SX_DEV __nv_bfloat16 i8_out<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+constexpr uint32_t kI8GemvRows = 16;  // up to which the weights are streamed
+cudaError_t prepare_gemv_i8();
+cudaError_t launch_gemv_i8(uint32_t dtype, bool gated, const I8Args &a, int num_sms, cudaStream_t s);
+
 }  // namespace sx

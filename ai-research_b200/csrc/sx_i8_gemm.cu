@@ -302,6 +302,201 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// ---- few rows of x, or few tiles: weights as the rows of the products
+// 128 columns of y (rows of weights) are the M of the product and up to 256 rows of x its N, so that no row of the
+// tensor memory is spent on rows of x that are not there; the CTAs of a cluster share a tile, each with a part of
+// K, and each then adds up what all of them have of its share of the rows of x (whole numbers, in any order).
+constexpr uint32_t kWRows = 128, kWTile = kWRows * kBK;
+struct SplitShape {
+  uint32_t tok;        // rows of x of a tile: a multiple of 16
+  uint32_t stages, cluster, tmem_cols;
+};
+
+SX_DEV void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+      : "memory");
+}
+SX_DEV void tma_load_2d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
+      "[%1, {%2, %3}], [%4];\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+SX_DEV void tma_prefetch_2d(const CUtensorMap *map, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y)
+               : "memory");
+}
+
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(kThreads)
+    gemm_i8_split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ I8Args a, const __grid_constant__ SplitShape p) {
+  constexpr uint32_t kMats = GATED ? 2 : 1, kMaxStages = 12;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 1];
+  __shared__ uint32_t tmem_slot, abort_flag;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x % p.cluster;
+  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u, bar0 = smem_u32(bars), stage_bytes = kMats * kWTile + p.tok * kBK;
+  auto full = [&](uint32_t s) { return bar0 + 8 * s; };
+  auto empty = [&](uint32_t s) { return bar0 + 8 * (kMaxStages + s); };
+  const uint32_t done = bar0 + 16 * kMaxStages;
+  const uint32_t n0 = blockIdx.x / p.cluster * kWRows, t0 = blockIdx.y * p.tok;
+  const uint32_t all = (a.k + kBK - 1) / kBK, k0 = all * rank / p.cluster, steps = all * (rank + 1) / p.cluster - k0;
+  volatile uint32_t *const stop = &abort_flag;
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < p.stages; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    mbar_init(done, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+    // asked into L2 while the kernel before this one ends
+    for (uint32_t i = 0; i < steps && i < p.stages; ++i)
+#pragma unroll
+      for (uint32_t m = 0; m < kMats; ++m) tma_prefetch_2d(&maps.w[m], (k0 + i) * kBK, n0);
+  }
+  __syncwarp();
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&tmem_slot), p.tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    if (*stop) return false;
+    if (mbar_wait_bounded(bar, parity & 1)) return true;
+    *stop = 1;
+    raise_error(a.err, kDevWaitTimeout);
+    return false;
+  };
+  pdl_launch_dependents();
+  pdl_wait();
+  uint32_t issued = 0;
+  bool ok = true;
+  if (warp == 0 && lane == 0) {
+    for (uint32_t i = 0, s = 0, round = 0; i < steps; ++i) {
+      const uint32_t at = base + s * stage_bytes;
+      if (round > 0 && !wait(empty(s), round - 1)) break;
+      mbar_arrive_expect_tx(full(s), stage_bytes);
+#pragma unroll
+      for (uint32_t m = 0; m < kMats; ++m) tma_load_2d(at + m * kWTile, &maps.w[m], (k0 + i) * kBK, n0, full(s));
+      tma_load_2d(at + kMats * kWTile, &maps.x, (k0 + i) * kBK, t0, full(s));
+      issued = i + 1;
+      if (++s == p.stages) s = 0, ++round;
+    }
+  } else if (warp == 1 && lane == 0) {
+    const uint32_t idesc = umma_idesc_i8(kWRows, p.tok);
+    for (uint32_t i = 0, s = 0, round = 0; i < steps; ++i) {
+      const uint32_t at = base + s * stage_bytes;
+      if (!wait(full(s), round)) break;
+      tc_fence_after();
+      const uint64_t x = umma_desc_sw128(at + kMats * kWTile);
+#pragma unroll
+      for (uint32_t m = 0; m < kMats; ++m) {
+        const uint64_t w = umma_desc_sw128(at + m * kWTile);
+#pragma unroll
+        for (uint32_t j = 0; j < kBK / 32; ++j) umma_i8(tmem + m * p.tok, w + 2 * j, x + 2 * j, idesc, i > 0 || j > 0);
+      }
+      umma_commit(empty(s));
+      if (++s == p.stages) s = 0, ++round;
+    }
+    umma_commit(done);
+  }
+  const uint32_t q = warp & 3, n = n0 + 32 * q + lane, src = tmem + ((32 * q) << 16);
+  const uint32_t rows = min(p.tok, a.t - t0);  // of x
+  float ws[kMats];
+#pragma unroll
+  for (uint32_t m = 0; m < kMats; ++m) ws[m] = n < a.n ? a.w_scale[m][n] : 0.0f;
+  auto value = [&](int32_t g, int32_t u, float xs) {
+    float v = i8_value(g, xs, ws[0]);
+    if constexpr (GATED) v = i8_gated(v, i8_value(u, xs, ws[kMats - 1]));
+    return i8_out<T>(v);
+  };
+  if (warp >= 2) {
+    ok = wait(done, 0);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+  }
+  if (p.cluster == 1) {
+    if (warp >= 2 && ok) {
+#pragma unroll 1
+      for (uint32_t c = 0; c < rows; c += 16) {
+        uint32_t r[16], u[16];
+        tmem_ld16(src + c, r);
+        if constexpr (GATED) tmem_ld16(src + p.tok + c, u);
+        const float xs = c + lane < rows ? a.x_scale[t0 + c + lane] : 0.0f;
+        tmem_wait_ld(r);
+        if constexpr (GATED) tmem_wait_ld(u);
+        T *const y = static_cast<T *>(a.y) + (size_t)(t0 + c) * a.y_ld + n;
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j) {
+          const T v = value((int32_t)r[j], (int32_t)u[GATED ? j : 0], __shfl_sync(0xffffffffu, xs, j));
+          if (c + j < rows && n < a.n) y[(size_t)j * a.y_ld] = v;
+        }
+      }
+    }
+  } else {
+    // Rows of x, by eights, are shared out over the cluster.  A CTA's shared memory takes all parts of its own,
+    // over its tiles: [CTA][matrix][row of x][128].
+    __syncwarp();
+    cluster_sync();  // all tiles have been read
+    auto share = [&](uint32_t r) { return p.tok / 8 * r / p.cluster * 8; };
+    const uint32_t most = (p.tok / 8 + p.cluster - 1) / p.cluster * 8, part = kMats * most * kWRows * 4;
+    if (warp >= 2) {
+#pragma unroll 1
+      for (uint32_t i = 1; i <= p.cluster; ++i) {
+        const uint32_t to = (rank + i) % p.cluster, c0 = share(to), c1 = min(rows, share(to + 1));
+        const uint32_t dst = in_cta(base + rank * part, to) + (32 * q + lane) * 4;
+#pragma unroll 1
+        for (uint32_t c = c0; c < c1; c += 8)
+#pragma unroll
+          for (uint32_t m = 0; m < kMats; ++m) {
+            uint32_t r[8];
+            tmem_ld8(src + m * p.tok + c, r);
+#pragma unroll
+            for (uint32_t j = 0; j < 8; ++j)
+              if (c + j < c1)
+                asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(dst + (m * most + c - c0 + j) * kWRows * 4), "r"(r[j]) : "memory");
+          }
+      }
+    }
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 2 && ok) {
+      const uint32_t c0 = share(rank), c1 = min(rows, share(rank + 1));
+#pragma unroll 4
+      for (uint32_t c = c0; c < c1; ++c) {
+        int32_t sum[2] = {0, 0};
+#pragma unroll
+        for (uint32_t m = 0; m < kMats; ++m)
+#pragma unroll 1
+          for (uint32_t i = 0; i < p.cluster; ++i) {
+            int32_t v;
+            asm volatile("ld.shared.s32 %0, [%1];\n" : "=r"(v) : "r"(base + i * part + ((m * most + c - c0) * kWRows + 32 * q + lane) * 4) : "memory");
+            sum[m] += v;
+          }
+        const T v = value(sum[0], sum[1], a.x_scale[t0 + c]);
+        if (n < a.n) static_cast<T *>(a.y)[(size_t)(t0 + c) * a.y_ld + n] = v;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && *stop)  // a stopped CTA waits (bounded) for the copies that it issued
+    for (uint32_t s = 0; s < p.stages && s < issued; ++s) mbar_wait_bounded(full(s), ((issued - 1 - s) / p.stages) & 1);
+  __syncwarp();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, p.tmem_cols);
+  }
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
@@ -356,9 +551,45 @@ cudaError_t launch_pair(uint32_t dtype, bool gated, const I8Args &a, int num_sms
   return launch_chained(v.fn, dim3(2 * std::min<uint32_t>(g.all, num_sms / 2)), dim3(kThreads), v.smem, s, 2, maps, a, g);
 }
 
+using SplitKernel = void (*)(const Maps, const I8Args, const SplitShape);
+SplitKernel split_kernel(uint32_t dtype, bool gated) {
+  if (dtype == SX_F32) return gated ? gemm_i8_split_kernel<float, true> : gemm_i8_split_kernel<float, false>;
+  return gated ? gemm_i8_split_kernel<__nv_bfloat16, true> : gemm_i8_split_kernel<__nv_bfloat16, false>;
+}
+constexpr uint32_t kSplitRows = 512;
+constexpr uint32_t kSplitSmem = 220 * 1024, kSplitSmemTwo = 108 * 1024;  // one CTA an SM, two
+
+cudaError_t launch_split(uint32_t dtype, bool gated, const I8Args &a, int num_sms, cudaStream_t s) {
+  const uint32_t mats = gated ? 2 : 1, most = gated ? 128 : 256, sms = num_sms;
+  SplitShape p;
+  uint32_t t_tiles = (a.t + most - 1) / most;
+  const uint32_t n_tiles = (a.n + kWRows - 1) / kWRows;
+  p.tok = ((a.t + t_tiles - 1) / t_tiles + 15) / 16 * 16;
+  t_tiles = (a.t + p.tok - 1) / p.tok;
+  const uint32_t tiles = n_tiles * t_tiles, steps = (a.k + kBK - 1) / kBK;
+  p.cluster = 1;
+  while (p.cluster < 8 && 2 * p.cluster * tiles <= sms && 2 * p.cluster * 2 <= steps) p.cluster *= 2;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < mats * p.tok) p.tmem_cols *= 2;
+  const uint32_t room = tiles * p.cluster <= sms ? kSplitSmem : kSplitSmemTwo, stage = mats * kWTile + p.tok * kBK;
+  p.stages = std::min(12u, (room - 1024) / stage);
+  const uint32_t parts = p.cluster > 1 ? p.cluster * mats * ((p.tok / 8 + p.cluster - 1) / p.cluster * 8) * kWRows * 4 : 0;
+  const uint32_t smem = std::max(p.stages * stage, parts) + 1024;
+  Maps maps{};
+  bool ok = encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.k, a.t, a.x_ld, kBK, p.tok);
+  for (uint32_t i = 0; i < mats; ++i) ok = ok && encode(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, kWRows);
+  if (!ok) return cudaErrorInvalidValue;
+  return launch_chained(split_kernel(dtype, gated), dim3(n_tiles * p.cluster, t_tiles), dim3(kThreads), smem, s, p.cluster, maps, a, p);
+}
+
 }  // namespace
 
 cudaError_t prepare_gemm_i8() {
+  for (uint32_t dtype : {SX_F32, SX_BF16})
+    for (bool gated : {false, true}) {
+      const cudaError_t e = cudaFuncSetAttribute(split_kernel(dtype, gated), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSplitSmem);
+      if (e != cudaSuccess) return e;
+    }
   for (uint32_t dtype : {SX_F32, SX_BF16})
     for (bool gated : {false, true})
       for (uint32_t bn : {256u}) {
@@ -366,7 +597,7 @@ cudaError_t prepare_gemm_i8() {
         const cudaError_t e = cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem);
         if (e != cudaSuccess) return e;
       }
-  return cudaSuccess;
+  return prepare_gemv_i8();
 }
 
 }  // namespace sx
@@ -399,7 +630,9 @@ sx_status dispatch_i8(const char *what, sx_engine *e, uint32_t dtype, sx::I8Args
   const cudaError_t ce = cudaSetDevice(e->device);
   if (ce != cudaSuccess) return sx_host_cuda_status(ce, "cudaSetDevice");
   a.err = e->err_dev;
-  return sx_host_cuda_status(sx::launch_pair(dtype, gated, a, e->num_sms, e->stream), what);
+  return sx_host_cuda_status(a.t <= sx::kI8GemvRows ? sx::launch_gemv_i8(dtype, gated, a, e->num_sms, e->stream)
+                             : a.t <= sx::kSplitRows ? sx::launch_split(dtype, gated, a, e->num_sms, e->stream)
+                                                     : sx::launch_pair(dtype, gated, a, e->num_sms, e->stream), what);
 }
 
 }  // namespace
