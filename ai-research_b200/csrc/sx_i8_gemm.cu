@@ -8,7 +8,7 @@
 // scaled and stored while the next is summed.  Warps of a CTA:
 //   0       TMA: 128 codes of K a stage, completing on the leader's barrier
 //   1       the leader's issues the products and commits stages and sums to both CTAs
-//   2 .. 5  sums to values, 32 rows each, staged in shared memory and stored by TMA (rows of y that do not
+//   2 .. 9  sums to values, 32 rows each and every other box of columns, staged in shared memory and stored by TMA (rows of y that do not
 //           begin and end on 16 bytes: by lanes)
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -17,6 +17,7 @@
 
 #include "sx_host.h"
 #include "sx_i8.cuh"
+#include "sx_kv8.cuh"
 #include "sx_launch.cuh"
 #include "sx_tcgen05.cuh"
 
@@ -25,7 +26,7 @@ namespace {
 
 constexpr uint32_t kBM = 256, kBK = 128;        // of a pair
 constexpr uint32_t kHalf = kBM / 2;             // rows of a CTA
-constexpr int kEpiWarps = 4, kThreads = (2 + kEpiWarps) * 32;
+constexpr int kEpiWarps = 8, kThreads = (2 + kEpiWarps) * 32;
 constexpr uint32_t kBox = 4096;                 // 32 rows of 128 bytes of y
 constexpr uint32_t kTmemCols = 512, kAccCols = 256;
 constexpr uint32_t kGroup = 8;                  // tiles of rows that are taken together, for L2
@@ -34,8 +35,17 @@ template <uint32_t BN>
 struct PairShape {
   static constexpr uint32_t kATile = kHalf * kBK, kBTile = BN / 2 * kBK, kStage = kATile + kBTile;
   static constexpr uint32_t kStages = 196608 / kStage;
-  static constexpr uint32_t kSmem = kStages * kStage + kEpiWarps * 2 * kBox + 1024;  // + alignment
+  static constexpr uint32_t kData = kStages * kStage + kEpiWarps * kBox;
 };
+// What the CTA's threads share behind the stages and boxes: no static shared memory beside them, so that they begin
+// on the 1024 bytes that the swizzle asks for, with room for a little less than that.
+template <uint32_t STAGES, int MATS>
+struct PairShared {
+  float col_scale[kEpiWarps][MATS][32];
+  uint64_t bars[2 * STAGES + 4];
+  uint32_t tmem_slot, abort_flag;
+};
+constexpr uint32_t kMaxSmem = 227 * 1024;
 
 // ---- TMA, cluster and pair wrappers
 SX_DEV uint32_t cluster_rank() {
@@ -62,6 +72,10 @@ SX_DEV void tma_load_pair(uint32_t dst, const CUtensorMap *map, int32_t x, int32
       "[%1, {%2, %3}], [%4];\n" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
+}
+SX_DEV void tma_prefetch_2d(const CUtensorMap *map, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y)
+               : "memory");
 }
 SX_DEV void tma_store_2d(const CUtensorMap *map, int32_t x, int32_t y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
@@ -122,12 +136,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     gemm_i8_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ I8Args a, const __grid_constant__ Tiles g) {
   using S = PairShape<BN>;
   constexpr uint32_t kStages = S::kStages, kCols = GATED ? BN / 2 : BN;  // columns of y
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * kStages + 4];
-  __shared__ uint32_t tmem_slot, abort_flag;
-  __shared__ __align__(16) float col_scale[kEpiWarps][GATED ? 2 : 1][32];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_rank();
-  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u, bar0 = smem_u32(bars);
+  using Shared = PairShared<kStages, GATED ? 2 : 1>;
+  static_assert(S::kData + sizeof(Shared) <= kMaxSmem, "shared memory");
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u, skip = base - smem_u32(smem_raw);
+  if (skip + S::kData + sizeof(Shared) > kMaxSmem) {  // (alike in all CTAs: never where shared memory is laid out as it is)
+    raise_error(a.err, kDevBadParams);
+    return;
+  }
+  Shared &sh = *reinterpret_cast<Shared *>(smem_raw + skip + S::kData);
+  uint32_t &tmem_slot = sh.tmem_slot, &abort_flag = sh.abort_flag;
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_rank(), bar0 = smem_u32(sh.bars);
   auto full = [&](uint32_t s) { return bar0 + 8 * s; };                   // the leader's: both CTAs' copies
   auto empty = [&](uint32_t s) { return bar0 + 8 * (kStages + s); };      // each CTA's
   auto sums_full = [&](uint32_t c) { return bar0 + 8 * (2 * kStages + c); };
@@ -161,6 +180,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     return false;
   };
   const uint32_t pair = blockIdx.x / 2, pairs = gridDim.x / 2, steps = (a.k + kBK - 1) / kBK;
+  if (threadIdx.x == 0 && pair < g.all) {  // the first weights are asked into L2 while the kernel before this one ends
+    uint32_t row, col;
+    tile_at(g, pair, &row, &col);
+    for (uint32_t k = 0; k < steps && k < kStages; ++k)
+      tma_prefetch_2d(GATED && rank ? &maps.w[1] : &maps.w[0], k * kBK, GATED ? col * kCols : col * kCols + rank * (BN / 2));
+  }
+  __syncwarp();
   pdl_launch_dependents();
   pdl_wait();
   uint32_t it = 0;  // stages used, over all tiles
@@ -201,31 +227,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       umma_commit_pair(sums_full(n & 1));
     }
   } else if (warp >= 2) {
-    const uint32_t q = warp & 3, boxes = base + kStages * S::kStage + (warp - 2) * 2 * kBox;
-    float(&cs)[GATED ? 2 : 1][32] = col_scale[warp - 2];
-    constexpr uint32_t kBoxCols = 128 / sizeof(T);
-    uint32_t n = 0, stored = 0;
+    constexpr uint32_t kBoxCols = 128 / sizeof(T), kPer = kBoxCols / 32;  // columns of a box, loads of 32 of them
+    constexpr uint32_t kBoxes = kCols / kBoxCols, kMine = (kBoxes + 1) / 2 * kPer;  // of a tile; of a warp, loads
+    static_assert(kCols % kBoxCols == 0, "whole boxes");
+    const uint32_t q = warp & 3, odd = (warp - 2) / 4, box = base + kStages * S::kStage + (warp - 2) * kBox;
+    float(&cs)[GATED ? 2 : 1][32] = sh.col_scale[warp - 2];
+    auto first = [&](uint32_t i) { return (odd + 2 * (i / kPer)) * kBoxCols + i % kPer * 32; };  // column of load i
+    uint32_t n = 0;
     for (uint32_t i = pair; i < g.all; i += pairs, ++n) {
       uint32_t row, col;
       tile_at(g, i, &row, &col);
       const uint32_t t0 = row * kBM + rank * kHalf + 32 * q, n0 = col * kCols, src = tmem + ((32 * q) << 16) + n % 2 * kAccCols;
       const float xs = t0 + lane < a.t ? a.x_scale[t0 + lane] : 0.0f;
+      float ws[GATED ? 2 : 1][kMine];  // scales of the columns, a lane each: here before the sums are
+#pragma unroll
+      for (uint32_t m = 0; m < (GATED ? 2 : 1); ++m)
+#pragma unroll
+        for (uint32_t k = 0; k < kMine; ++k) {
+          const uint32_t nc = n0 + first(k) + lane;
+          ws[m][k] = first(k) < kCols && nc < a.n ? a.w_scale[m][nc] : 0.0f;
+        }
       const bool ok = wait(sums_full(n & 1), n / 2);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
 #pragma unroll 1
-      for (uint32_t c = 0; c < kCols; c += 32) {
+      for (uint32_t k = 0; k < kMine && first(k) < kCols; ++k) {
+        const uint32_t c = first(k);
         uint32_t r[32], u[GATED ? 32 : 1];
         tmem_ld32(src + c, r);
         if constexpr (GATED) tmem_ld32(src + BN / 2 + c, u);
-        const uint32_t nc = n0 + c + lane;
         __syncwarp();  // the scales of the columns before have been read
-        cs[0][lane] = nc < a.n ? a.w_scale[0][nc] : 0.0f;
-        if constexpr (GATED) cs[1][lane] = nc < a.n ? a.w_scale[1][nc] : 0.0f;
-        const uint32_t box = boxes + stored % 2 * kBox, half = sizeof(T) == 2 ? c / 32 % 2 : 0;
-        if (half == 0) {
-          if (lane == 0) bulk_wait_read<1>();  // the store from this box before has read it
+#pragma unroll
+        for (uint32_t m = 0; m < (GATED ? 2 : 1); ++m) {
+          cs[m][lane] = ws[m][0];
+#pragma unroll
+          for (uint32_t w = 0; w + 1 < kMine; ++w) ws[m][w] = ws[m][w + 1];
         }
+        const uint32_t half = k % kPer;
+        if (half == 0 && lane == 0) bulk_wait_read<0>();  // the box's store before has read it
         __syncwarp();
         tmem_wait_ld(r);
         if constexpr (GATED) tmem_wait_ld(u);
@@ -252,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        "r"(w[2]), "r"(w[3])
                        : "memory");
         }
-        if (sizeof(T) == 2 && half == 0 && c + 32 < kCols) continue;
+        if (half + 1 < kPer) continue;
         const uint32_t c0 = n0 + c - half * 32;
         if (!g.lanes) {
           fence_proxy_async();  // generic-proxy writes -> the TMA engine's reads
@@ -281,7 +320,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           __syncwarp();
         }
-        ++stored;
       }
       tc_fence_before();
       __syncwarp();
@@ -305,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---- few rows of x, or few tiles: weights as the rows of the products
 // 128 columns of y (rows of weights) are the M of the product and up to 256 rows of x its N, so that no row of the
 // tensor memory is spent on rows of x that are not there; the CTAs of a cluster share a tile, each with a part of
-// K, and each then adds up what all of them have of its share of the rows of x (whole numbers, in any order).
+// K, and each then adds up what all of them have of every so-manieth row of x (whole numbers, in any order).
 constexpr uint32_t kWRows = 128, kWTile = kWRows * kBK;
 struct SplitShape {
   uint32_t tok;        // rows of x of a tile: a multiple of 16
@@ -326,11 +364,6 @@ SX_DEV void tma_load_2d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-SX_DEV void tma_prefetch_2d(const CUtensorMap *map, int32_t x, int32_t y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y)
-               : "memory");
-}
-
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(kThreads)
     gemm_i8_split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ I8Args a, const __grid_constant__ SplitShape p) {
@@ -378,7 +411,7 @@ __global__ void __launch_bounds__(kThreads)
   pdl_launch_dependents();
   pdl_wait();
   uint32_t issued = 0;
-  bool ok = true;
+  bool ok = false;
   if (warp == 0 && lane == 0) {
     for (uint32_t i = 0, s = 0, round = 0; i < steps; ++i) {
       const uint32_t at = base + s * stage_bytes;
@@ -408,84 +441,80 @@ __global__ void __launch_bounds__(kThreads)
     }
     umma_commit(done);
   }
-  const uint32_t q = warp & 3, n = n0 + 32 * q + lane, src = tmem + ((32 * q) << 16);
-  const uint32_t rows = min(p.tok, a.t - t0);  // of x
-  float ws[kMats];
-#pragma unroll
-  for (uint32_t m = 0; m < kMats; ++m) ws[m] = n < a.n ? a.w_scale[m][n] : 0.0f;
-  auto value = [&](int32_t g, int32_t u, float xs) {
-    float v = i8_value(g, xs, ws[0]);
-    if constexpr (GATED) v = i8_gated(v, i8_value(u, xs, ws[kMats - 1]));
-    return i8_out<T>(v);
-  };
+  // ---- sums to shared memory, over the tiles: [row of x][matrix][128]
+  const uint32_t rows = min(p.tok, a.t - t0), epi = warp - 2;  // rows of x
   if (warp >= 2) {
     ok = wait(done, 0);
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
-  }
-  if (p.cluster == 1) {
-    if (warp >= 2 && ok) {
+    const uint32_t q = warp & 3, src = tmem + ((32 * q) << 16), dst = base + (32 * q + lane) * 4;
 #pragma unroll 1
-      for (uint32_t c = 0; c < rows; c += 16) {
-        uint32_t r[16], u[16];
-        tmem_ld16(src + c, r);
-        if constexpr (GATED) tmem_ld16(src + p.tok + c, u);
-        const float xs = c + lane < rows ? a.x_scale[t0 + c + lane] : 0.0f;
-        tmem_wait_ld(r);
-        if constexpr (GATED) tmem_wait_ld(u);
-        T *const y = static_cast<T *>(a.y) + (size_t)(t0 + c) * a.y_ld + n;
+    for (uint32_t c = epi / 4 * 16; c < rows; c += 32)
 #pragma unroll
-        for (uint32_t j = 0; j < 16; ++j) {
-          const T v = value((int32_t)r[j], (int32_t)u[GATED ? j : 0], __shfl_sync(0xffffffffu, xs, j));
-          if (c + j < rows && n < a.n) y[(size_t)j * a.y_ld] = v;
+      for (uint32_t m = 0; m < kMats; ++m) {
+        uint32_t r[16];
+        tmem_ld16(src + m * p.tok + c, r);
+        tmem_wait_ld(r);
+#pragma unroll
+        for (uint32_t j = 0; j < 16; ++j)
+          asm volatile("st.shared.b32 [%0], %1;\n" ::"r"(dst + ((c + j) * kMats + m) * kWRows * 4), "r"(r[j]) : "memory");
+      }
+  }
+  __syncwarp();
+  if (p.cluster > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  // ---- a warp takes a row of x, four columns a lane; a CTA's rows are every p.cluster-th
+  if (warp >= 2 && ok) {
+    const uint32_t n = n0 + 4 * lane;
+    float ws[kMats][4];
+#pragma unroll
+    for (uint32_t m = 0; m < kMats; ++m)
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) ws[m][j] = n + j < a.n ? a.w_scale[m][n + j] : 0.0f;
+    const uint32_t es = sizeof(T);
+    const bool wide = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)a.y_ld * es) % (4 * es)) == 0 && n + 4 <= a.n;
+#pragma unroll 2
+    for (uint32_t c = rank + p.cluster * epi; c < rows; c += p.cluster * kEpiWarps) {
+      const float xs = a.x_scale[t0 + c];
+      int32_t sum[kMats][4];
+#pragma unroll
+      for (uint32_t m = 0; m < kMats; ++m)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) sum[m][j] = 0;
+      const uint32_t at = base + c * kMats * kWRows * 4 + lane * 16;
+      for (uint32_t i = 0; i < p.cluster; ++i) {
+        const uint32_t from = p.cluster > 1 ? in_cta(at, i) : at;
+#pragma unroll
+        for (uint32_t m = 0; m < kMats; ++m) {
+          int32_t v[4];
+          asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];\n"
+                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                       : "r"(from + m * kWRows * 4)
+                       : "memory");
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j) sum[m][j] += v[j];
         }
       }
-    }
-  } else {
-    // Rows of x, by eights, are shared out over the cluster.  A CTA's shared memory takes all parts of its own,
-    // over its tiles: [CTA][matrix][row of x][128].
-    __syncwarp();
-    cluster_sync();  // all tiles have been read
-    auto share = [&](uint32_t r) { return p.tok / 8 * r / p.cluster * 8; };
-    const uint32_t most = (p.tok / 8 + p.cluster - 1) / p.cluster * 8, part = kMats * most * kWRows * 4;
-    if (warp >= 2) {
-#pragma unroll 1
-      for (uint32_t i = 1; i <= p.cluster; ++i) {
-        const uint32_t to = (rank + i) % p.cluster, c0 = share(to), c1 = min(rows, share(to + 1));
-        const uint32_t dst = in_cta(base + rank * part, to) + (32 * q + lane) * 4;
-#pragma unroll 1
-        for (uint32_t c = c0; c < c1; c += 8)
+      float v[4];
 #pragma unroll
-          for (uint32_t m = 0; m < kMats; ++m) {
-            uint32_t r[8];
-            tmem_ld8(src + m * p.tok + c, r);
-#pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-              if (c + j < c1)
-                asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(dst + (m * most + c - c0 + j) * kWRows * 4), "r"(r[j]) : "memory");
-          }
+      for (uint32_t j = 0; j < 4; ++j) {
+        v[j] = i8_value(sum[0][j], xs, ws[0][j]);
+        if constexpr (GATED) v[j] = i8_gated(v[j], i8_value(sum[kMats - 1][j], xs, ws[kMats - 1][j]));
       }
-    }
-    __syncwarp();
-    cluster_sync();
-    if (warp >= 2 && ok) {
-      const uint32_t c0 = share(rank), c1 = min(rows, share(rank + 1));
-#pragma unroll 4
-      for (uint32_t c = c0; c < c1; ++c) {
-        int32_t sum[2] = {0, 0};
+      T *const y = static_cast<T *>(a.y) + (size_t)(t0 + c) * a.y_ld + n;
+      if (wide) {
+        store_vec<T, 4>(y, v);
+      } else {
 #pragma unroll
-        for (uint32_t m = 0; m < kMats; ++m)
-#pragma unroll 1
-          for (uint32_t i = 0; i < p.cluster; ++i) {
-            int32_t v;
-            asm volatile("ld.shared.s32 %0, [%1];\n" : "=r"(v) : "r"(base + i * part + ((m * most + c - c0) * kWRows + 32 * q + lane) * 4) : "memory");
-            sum[m] += v;
-          }
-        const T v = value(sum[0], sum[1], a.x_scale[t0 + c]);
-        if (n < a.n) static_cast<T *>(a.y)[(size_t)(t0 + c) * a.y_ld + n] = v;
+        for (uint32_t j = 0; j < 4; ++j)
+          if (n + j < a.n) y[j] = i8_out<T>(v[j]);
       }
     }
   }
+  __syncwarp();
+  if (p.cluster > 1) cluster_sync();  // the others have read this CTA's sums
   tc_fence_before();
   __syncthreads();
   if (threadIdx.x == 0 && *stop)  // a stopped CTA waits (bounded) for the copies that it issued
@@ -521,11 +550,11 @@ bool encode(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t 
 using PairKernel = void (*)(const Maps, const I8Args, const Tiles);
 struct PairVariant {
   PairKernel fn;
-  uint32_t bn, smem;
+  uint32_t bn;
 };
 template <typename T, bool GATED>
 PairVariant pair_variant(uint32_t bn) {
-  return {gemm_i8_pair_kernel<T, GATED, 256>, 256, PairShape<256>::kSmem};
+  return {gemm_i8_pair_kernel<T, GATED, 256>, 256};
 }
 PairVariant pair_variant(uint32_t dtype, bool gated, uint32_t bn) {
   if (dtype == SX_F32) return gated ? pair_variant<float, true>(bn) : pair_variant<float, false>(bn);
@@ -548,7 +577,7 @@ cudaError_t launch_pair(uint32_t dtype, bool gated, const I8Args &a, int num_sms
     ok = ok && encode(&maps.y, dtype == SX_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.n, a.t,
                       (uint64_t)a.y_ld * es, 128 / es, 32);
   if (!ok) return cudaErrorInvalidValue;
-  return launch_chained(v.fn, dim3(2 * std::min<uint32_t>(g.all, num_sms / 2)), dim3(kThreads), v.smem, s, 2, maps, a, g);
+  return launch_chained(v.fn, dim3(2 * std::min<uint32_t>(g.all, num_sms / 2)), dim3(kThreads), kMaxSmem, s, 2, maps, a, g);
 }
 
 using SplitKernel = void (*)(const Maps, const I8Args, const SplitShape);
@@ -573,8 +602,7 @@ cudaError_t launch_split(uint32_t dtype, bool gated, const I8Args &a, int num_sm
   while (p.tmem_cols < mats * p.tok) p.tmem_cols *= 2;
   const uint32_t room = tiles * p.cluster <= sms ? kSplitSmem : kSplitSmemTwo, stage = mats * kWTile + p.tok * kBK;
   p.stages = std::min(12u, (room - 1024) / stage);
-  const uint32_t parts = p.cluster > 1 ? p.cluster * mats * ((p.tok / 8 + p.cluster - 1) / p.cluster * 8) * kWRows * 4 : 0;
-  const uint32_t smem = std::max(p.stages * stage, parts) + 1024;
+  const uint32_t smem = std::max(p.stages * stage, p.tok * mats * kWRows * 4) + 1024;  // the stages, then the sums
   Maps maps{};
   bool ok = encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.k, a.t, a.x_ld, kBK, p.tok);
   for (uint32_t i = 0; i < mats; ++i) ok = ok && encode(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, kWRows);
@@ -594,7 +622,7 @@ cudaError_t prepare_gemm_i8() {
     for (bool gated : {false, true})
       for (uint32_t bn : {256u}) {
         const PairVariant v = pair_variant(dtype, gated, bn);
-        const cudaError_t e = cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem);
+        const cudaError_t e = cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
         if (e != cudaSuccess) return e;
       }
   return prepare_gemv_i8();
