@@ -14,6 +14,7 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "sx_host.h"
 #include "sx_i8.cuh"
@@ -24,6 +25,7 @@
 namespace sx {
 namespace {
 
+constexpr uint32_t kSplitRows = 512, BNSEL = 256;
 constexpr uint32_t kBM = 256, kBK = 128;        // of a pair
 constexpr uint32_t kHalf = kBM / 2;             // rows of a CTA
 constexpr int kEpiWarps = 8, kThreads = (2 + kEpiWarps) * 32;
@@ -364,6 +366,13 @@ SX_DEV void tma_load_2d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+SX_DEV void ld_shared_v4(uint32_t src, int32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
+}
+SX_DEV void ld_cluster_v4(uint32_t src, int32_t (&v)[4]) {
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(src) : "memory");
+}
+
 template <typename T, bool GATED>
 __global__ void __launch_bounds__(kThreads)
     gemm_i8_split_kernel(const __grid_constant__ Maps maps, const __grid_constant__ I8Args a, const __grid_constant__ SplitShape p) {
@@ -443,6 +452,10 @@ __global__ void __launch_bounds__(kThreads)
   }
   // ---- sums to shared memory, over the tiles: [row of x][matrix][128]
   const uint32_t rows = min(p.tok, a.t - t0), epi = warp - 2;  // rows of x
+  // This warp's rows of x further on, and the scale of the lane-th of them: here before the sums are.
+  const uint32_t mine = rank + p.cluster * epi, apart = p.cluster * kEpiWarps;
+  static_assert(32 * kEpiWarps >= 256, "a lane for each of a warp's rows");
+  const float xs_mine = warp >= 2 && mine + lane * apart < rows ? a.x_scale[t0 + mine + lane * apart] : 0.0f;
   if (warp >= 2) {
     ok = wait(done, 0);
     ok = __all_sync(0xffffffffu, ok);
@@ -465,38 +478,18 @@ __global__ void __launch_bounds__(kThreads)
     cluster_sync();
   else
     __syncthreads();
-  // ---- a warp takes a row of x, four columns a lane; a CTA's rows are every p.cluster-th
+  // ---- a warp takes rows of x, four columns a lane; a CTA's rows are every p.cluster-th
   if (warp >= 2 && ok) {
-    const uint32_t n = n0 + 4 * lane;
+    const uint32_t n = n0 + 4 * lane, at = base + lane * 16;
     float ws[kMats][4];
 #pragma unroll
     for (uint32_t m = 0; m < kMats; ++m)
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) ws[m][j] = n + j < a.n ? a.w_scale[m][n + j] : 0.0f;
-    const uint32_t es = sizeof(T);
-    const bool wide = ((reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)a.y_ld * es) % (4 * es)) == 0 && n + 4 <= a.n;
-#pragma unroll 2
-    for (uint32_t c = rank + p.cluster * epi; c < rows; c += p.cluster * kEpiWarps) {
-      const float xs = a.x_scale[t0 + c];
-      int32_t sum[kMats][4];
-#pragma unroll
-      for (uint32_t m = 0; m < kMats; ++m)
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) sum[m][j] = 0;
-      const uint32_t at = base + c * kMats * kWRows * 4 + lane * 16;
-      for (uint32_t i = 0; i < p.cluster; ++i) {
-        const uint32_t from = p.cluster > 1 ? in_cta(at, i) : at;
-#pragma unroll
-        for (uint32_t m = 0; m < kMats; ++m) {
-          int32_t v[4];
-          asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];\n"
-                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                       : "r"(from + m * kWRows * 4)
-                       : "memory");
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j) sum[m][j] += v[j];
-        }
-      }
+    constexpr uint32_t es = sizeof(T);
+    const bool wide = (reinterpret_cast<uintptr_t>(a.y) | (uintptr_t)a.y_ld * es) % (4 * es) == 0 && n + 4 <= a.n;
+    auto store = [&](uint32_t c, uint32_t nth, const int32_t (&sum)[kMats][4]) {
+      const float xs = __shfl_sync(0xffffffffu, xs_mine, nth);
       float v[4];
 #pragma unroll
       for (uint32_t j = 0; j < 4; ++j) {
@@ -511,7 +504,49 @@ __global__ void __launch_bounds__(kThreads)
         for (uint32_t j = 0; j < 4; ++j)
           if (n + j < a.n) y[j] = i8_out<T>(v[j]);
       }
-    }
+    };
+    // (a load's result is hundreds of cycles away: all CTAs' parts of a row, or several rows, at a time)
+    auto rows_of = [&](auto parts, auto at_once) {
+      constexpr uint32_t kParts = decltype(parts)::value, kOnce = decltype(at_once)::value;
+#pragma unroll 1
+      for (uint32_t c = mine, nth = 0; c < rows; c += kOnce * apart, nth += kOnce) {
+        int32_t v[kOnce][kParts][kMats][4];
+#pragma unroll
+        for (uint32_t o = 0; o < kOnce; ++o) {
+          const uint32_t row = min(c + o * apart, rows - 1) * kMats * kWRows * 4 + at;
+#pragma unroll
+          for (uint32_t i = 0; i < kParts; ++i)
+#pragma unroll
+            for (uint32_t m = 0; m < kMats; ++m)
+              if constexpr (kParts == 1)
+                ld_shared_v4(row + m * kWRows * 4, v[o][i][m]);
+              else
+                ld_cluster_v4(in_cta(row + m * kWRows * 4, i), v[o][i][m]);
+        }
+#pragma unroll
+        for (uint32_t o = 0; o < kOnce; ++o) {
+#pragma unroll
+          for (uint32_t i = 1; i < kParts; ++i)
+#pragma unroll
+            for (uint32_t m = 0; m < kMats; ++m)
+#pragma unroll
+              for (uint32_t j = 0; j < 4; ++j) v[o][0][m][j] += v[o][i][m][j];
+          if (c + o * apart < rows) store(c + o * apart, nth + o, v[o][0]);
+        }
+      }
+    };
+    using One = std::integral_constant<uint32_t, 1>;
+    using Two = std::integral_constant<uint32_t, 2>;
+    using Four = std::integral_constant<uint32_t, 4>;
+    using Eight = std::integral_constant<uint32_t, 8>;
+    if (p.cluster == 1)
+      rows_of(One{}, Four{});
+    else if (p.cluster == 2)
+      rows_of(Two{}, Two{});
+    else if (p.cluster == 4)
+      rows_of(Four{}, One{});
+    else
+      rows_of(Eight{}, One{});
   }
   __syncwarp();
   if (p.cluster > 1) cluster_sync();  // the others have read this CTA's sums
@@ -554,6 +589,7 @@ struct PairVariant {
 };
 template <typename T, bool GATED>
 PairVariant pair_variant(uint32_t bn) {
+  if (bn == 128) return {gemm_i8_pair_kernel<T, GATED, 128>, 128};
   return {gemm_i8_pair_kernel<T, GATED, 256>, 256};
 }
 PairVariant pair_variant(uint32_t dtype, bool gated, uint32_t bn) {
@@ -562,7 +598,7 @@ PairVariant pair_variant(uint32_t dtype, bool gated, uint32_t bn) {
 }
 
 cudaError_t launch_pair(uint32_t dtype, bool gated, const I8Args &a, int num_sms, cudaStream_t s) {
-  const PairVariant v = pair_variant(dtype, gated, 256);
+  const PairVariant v = pair_variant(dtype, gated, BNSEL);
   const uint32_t cols = gated ? v.bn / 2 : v.bn, es = dtype == SX_F32 ? 4 : 2;
   Tiles g;
   g.rows = (a.t + kBM - 1) / kBM;
@@ -585,7 +621,6 @@ SplitKernel split_kernel(uint32_t dtype, bool gated) {
   if (dtype == SX_F32) return gated ? gemm_i8_split_kernel<float, true> : gemm_i8_split_kernel<float, false>;
   return gated ? gemm_i8_split_kernel<__nv_bfloat16, true> : gemm_i8_split_kernel<__nv_bfloat16, false>;
 }
-constexpr uint32_t kSplitRows = 512;
 constexpr uint32_t kSplitSmem = 220 * 1024, kSplitSmemTwo = 108 * 1024;  // one CTA an SM, two
 
 cudaError_t launch_split(uint32_t dtype, bool gated, const I8Args &a, int num_sms, cudaStream_t s) {
@@ -620,7 +655,7 @@ cudaError_t prepare_gemm_i8() {
     }
   for (uint32_t dtype : {SX_F32, SX_BF16})
     for (bool gated : {false, true})
-      for (uint32_t bn : {256u}) {
+      for (uint32_t bn : {128u, 256u}) {
         const PairVariant v = pair_variant(dtype, gated, bn);
         const cudaError_t e = cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
         if (e != cudaSuccess) return e;
