@@ -55,6 +55,11 @@ SX_DEV uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
   return r;
 }
+SX_DEV bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+  return p != 0;
+}
 SX_DEV void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
@@ -118,6 +123,15 @@ constexpr uint32_t umma_idesc_i8(uint32_t m, uint32_t n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 
+// A wait that runs out ends this CTA's waiting: what follows is skipped, and the error word says so.
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile uint32_t *stop, uint32_t *err) {
+  if (*stop) return false;
+  if (mbar_wait_bounded(bar, parity)) return true;
+  *stop = 1;
+  raise_error(err, kDevWaitTimeout);
+  return false;
+}
+
 struct Maps {
   CUtensorMap x, w[2], y;
 };
@@ -173,14 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  // A wait that runs out ends this CTA's waiting: what follows is skipped, and the error word says so.
-  auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (*stop) return false;
-    if (mbar_wait_bounded(bar, parity & 1)) return true;
-    *stop = 1;
-    raise_error(a.err, kDevWaitTimeout);
-    return false;
-  };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity & 1) || wait_longer(bar, parity & 1, stop, a.err); };
   const uint32_t pair = blockIdx.x / 2, pairs = gridDim.x / 2, steps = (a.k + kBK - 1) / kBK;
   if (threadIdx.x == 0 && pair < g.all) {  // the first weights are asked into L2 while the kernel before this one ends
     uint32_t row, col;
@@ -192,7 +199,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
   uint32_t it = 0;  // stages used, over all tiles
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {  // (the whole warp, so that addresses are the same in all lanes; one thread issues)
+    const uint32_t leader_full = in_cta(full(0), 0);
     for (uint32_t i = pair; i < g.all; i += pairs) {
       uint32_t row, col;
       tile_at(g, i, &row, &col);
@@ -201,32 +209,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       const CUtensorMap *const w = GATED && rank ? &maps.w[1] : &maps.w[0];
       bool ok = true;
       for (uint32_t k = 0; k < steps; ++k, ++it) {
-        const uint32_t s = it % kStages, at = base + s * S::kStage, bar = in_cta(full(s), 0);
-        if (it >= kStages && !(ok = wait(empty(s), it / kStages - 1))) break;
-        if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * S::kStage);
-        tma_load_pair(at, &maps.x, k * kBK, x_row, bar);
-        tma_load_pair(at + S::kATile, w, k * kBK, w_row, bar);
+        const uint32_t s = it % kStages, at = base + s * S::kStage, bar = leader_full + 8 * s;
+        if (it >= kStages && !(ok = __all_sync(0xffffffffu, wait(empty(s), it / kStages - 1)))) break;
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * S::kStage);
+          tma_load_pair(at, &maps.x, k * kBK, x_row, bar);
+          tma_load_pair(at + S::kATile, w, k * kBK, w_row, bar);
+        }
+        __syncwarp();
       }
       if (!ok) break;
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
+  } else if (warp == 1 && rank == 0) {
+    // (the whole warp, so that descriptors are the same in all lanes; one thread issues)
     uint32_t n = 0;
     for (uint32_t i = pair; i < g.all; i += pairs, ++n) {
       const uint32_t d = tmem + n % 2 * kAccCols;
-      if (n >= 2 && !wait(sums_empty(n & 1), n / 2 - 1)) break;
+      if (n >= 2 && !__all_sync(0xffffffffu, wait(sums_empty(n & 1), n / 2 - 1))) break;
       tc_fence_after();
       bool ok = true;
       for (uint32_t k = 0; k < steps; ++k, ++it) {
         const uint32_t s = it % kStages, at = base + s * S::kStage;
-        if (!(ok = wait(full(s), it / kStages))) break;
+        if (!(ok = __all_sync(0xffffffffu, wait(full(s), it / kStages)))) break;
         tc_fence_after();
         const uint64_t x = umma_desc_sw128(at), w = umma_desc_sw128(at + S::kATile);
+        if (elect_one()) {
 #pragma unroll
-        for (uint32_t j = 0; j < kBK / 32; ++j) umma_i8_pair(d, x + 2 * j, w + 2 * j, umma_idesc_i8(kBM, BN), k > 0 || j > 0);
-        umma_commit_pair(empty(s));
+          for (uint32_t j = 0; j < kBK / 32; ++j) umma_i8_pair(d, x + 2 * j, w + 2 * j, umma_idesc_i8(kBM, BN), k > 0 || j > 0);
+          umma_commit_pair(empty(s));
+          if (k + 1 == steps) umma_commit_pair(sums_full(n & 1));
+        }
+        __syncwarp();
       }
       if (!ok) break;
-      umma_commit_pair(sums_full(n & 1));
     }
   } else if (warp >= 2) {
     constexpr uint32_t kBoxCols = 128 / sizeof(T), kPer = kBoxCols / 32;  // columns of a box, loads of 32 of them
@@ -410,45 +425,45 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  auto wait = [&](uint32_t bar, uint32_t parity) {
-    if (*stop) return false;
-    if (mbar_wait_bounded(bar, parity & 1)) return true;
-    *stop = 1;
-    raise_error(a.err, kDevWaitTimeout);
-    return false;
-  };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity & 1) || wait_longer(bar, parity & 1, stop, a.err); };
   pdl_launch_dependents();
   pdl_wait();
   uint32_t issued = 0;
   bool ok = false;
-  if (warp == 0 && lane == 0) {
+  if (warp == 0) {  // (whole warps, so that addresses are the same in all lanes; one thread issues)
     for (uint32_t i = 0, s = 0, round = 0; i < steps; ++i) {
       const uint32_t at = base + s * stage_bytes;
-      if (round > 0 && !wait(empty(s), round - 1)) break;
-      mbar_arrive_expect_tx(full(s), stage_bytes);
+      if (round > 0 && !__all_sync(0xffffffffu, wait(empty(s), round - 1))) break;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(full(s), stage_bytes);
 #pragma unroll
-      for (uint32_t m = 0; m < kMats; ++m) tma_load_2d(at + m * kWTile, &maps.w[m], (k0 + i) * kBK, n0, full(s));
-      tma_load_2d(at + kMats * kWTile, &maps.x, (k0 + i) * kBK, t0, full(s));
+        for (uint32_t m = 0; m < kMats; ++m) tma_load_2d(at + m * kWTile, &maps.w[m], (k0 + i) * kBK, n0, full(s));
+        tma_load_2d(at + kMats * kWTile, &maps.x, (k0 + i) * kBK, t0, full(s));
+      }
+      __syncwarp();
       issued = i + 1;
       if (++s == p.stages) s = 0, ++round;
     }
-  } else if (warp == 1 && lane == 0) {
+  } else if (warp == 1) {
     const uint32_t idesc = umma_idesc_i8(kWRows, p.tok);
     for (uint32_t i = 0, s = 0, round = 0; i < steps; ++i) {
       const uint32_t at = base + s * stage_bytes;
-      if (!wait(full(s), round)) break;
+      if (!__all_sync(0xffffffffu, wait(full(s), round))) break;
       tc_fence_after();
       const uint64_t x = umma_desc_sw128(at + kMats * kWTile);
+      if (elect_one()) {
 #pragma unroll
-      for (uint32_t m = 0; m < kMats; ++m) {
-        const uint64_t w = umma_desc_sw128(at + m * kWTile);
+        for (uint32_t m = 0; m < kMats; ++m) {
+          const uint64_t w = umma_desc_sw128(at + m * kWTile);
 #pragma unroll
-        for (uint32_t j = 0; j < kBK / 32; ++j) umma_i8(tmem + m * p.tok, w + 2 * j, x + 2 * j, idesc, i > 0 || j > 0);
+          for (uint32_t j = 0; j < kBK / 32; ++j) umma_i8(tmem + m * p.tok, w + 2 * j, x + 2 * j, idesc, i > 0 || j > 0);
+        }
+        umma_commit(empty(s));
+        if (i + 1 == steps) umma_commit(done);
       }
-      umma_commit(empty(s));
+      __syncwarp();
       if (++s == p.stages) s = 0, ++round;
     }
-    umma_commit(done);
   }
   // ---- sums to shared memory, over the tiles: [row of x][matrix][128]
   const uint32_t rows = min(p.tok, a.t - t0), epi = warp - 2;  // rows of x
