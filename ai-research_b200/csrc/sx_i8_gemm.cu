@@ -287,9 +287,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (GATED) tmem_wait_ld(u);
         float v[32];
 #pragma unroll
-        for (uint32_t j = 0; j < 32; ++j) {
-          v[j] = i8_value((int32_t)r[j], xs, cs[0][j]);
-          if constexpr (GATED) v[j] = i8_gated(v[j], i8_value((int32_t)u[j], xs, cs[GATED ? 1 : 0][j]));
+        for (uint32_t j = 0; j < 32; j += 2) {
+          float2 y = i8_value2((int32_t)r[j], (int32_t)r[j + 1], xs, *reinterpret_cast<const float2 *>(&cs[0][j]));
+          if constexpr (GATED)
+            y = i8_gated2(y, i8_value2((int32_t)u[j], (int32_t)u[j + 1], xs, *reinterpret_cast<const float2 *>(&cs[1][j])));
+          v[j] = y.x;
+          v[j + 1] = y.y;
         }
         const uint32_t line = box + lane * 128, sw = lane & 7;
 #pragma unroll
