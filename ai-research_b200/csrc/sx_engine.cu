@@ -662,7 +662,7 @@ SX_API sx_status sx_engine_create(int device, sx_quant_mode mode, uint32_t flags
     if (st) break;
     st = cuda_status(sx::prepare_sample_kernels(), "probability kernel attributes");
     if (st) break;
-    st = cuda_status(sx::prepare_gemm_i8(), "int8 product kernel attributes");
+    st = cuda_status(sx::prepare_gemm_i8(e->i8_clusters), "int8 product kernel attributes");
   } while (0);
   if (st != SX_OK) {
     sx_engine_destroy(e);

@@ -47,6 +47,7 @@ struct sx_engine {
   int num_sms = 148;
   std::mutex freq_mu;
   std::map<std::pair<uint32_t, uint32_t>, float *> inv_freq;  // (rot, theta bits)
+  uint32_t i8_clusters[4] = {0, 0, 0, 0};  // clusters of 1, 2, 4, 8 CTAs, an SM each, that run at a time
 };
 
 struct sx_buffer {

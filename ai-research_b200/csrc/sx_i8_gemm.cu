@@ -13,6 +13,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -25,13 +26,11 @@
 namespace sx {
 namespace {
 
-constexpr uint32_t kSplitRows = 512, BNSEL = 256;
 constexpr uint32_t kBM = 256, kBK = 128;        // of a pair
 constexpr uint32_t kHalf = kBM / 2;             // rows of a CTA
 constexpr int kEpiWarps = 8, kThreads = (2 + kEpiWarps) * 32;
 constexpr uint32_t kBox = 4096;                 // 32 rows of 128 bytes of y
 constexpr uint32_t kTmemCols = 512, kAccCols = 256;
-constexpr uint32_t kGroup = 8;                  // tiles of rows that are taken together, for L2
 
 template <uint32_t BN>
 struct PairShape {
@@ -132,19 +131,33 @@ __device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile
   return false;
 }
 
+template <typename T>
+SX_DEV T ld_shared(uint32_t src) {
+  if constexpr (sizeof(T) == 4) {
+    float f;
+    asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(f) : "r"(src) : "memory");
+    return f;
+  } else {
+    uint16_t h;
+    asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(h) : "r"(src) : "memory");
+    return __ushort_as_bfloat16(h);
+  }
+}
+
 struct Maps {
   CUtensorMap x, w[2], y;
 };
 struct Tiles {
   uint32_t rows, cols, all;  // tiles of rows and of columns
+  uint32_t group;            // tiles of rows that go through all columns together
   uint32_t lanes;            // rows of y do not begin and end on 16 bytes: lanes store them
 };
-// Tile i: kGroup tiles of rows go through all columns together, so what runs at a time reads few of either.
+// Tile i: what runs at a time reads few rows of either matrix, and the rows of x of a group stay in L2 meanwhile.
 SX_DEV void tile_at(const Tiles &g, uint32_t i, uint32_t *row, uint32_t *col) {
-  const uint32_t band = i / (kGroup * g.cols), in = i - band * kGroup * g.cols;
-  const uint32_t high = min(kGroup, g.rows - band * kGroup);
+  const uint32_t band = i / (g.group * g.cols), in = i - band * g.group * g.cols;
+  const uint32_t high = min(g.group, g.rows - band * g.group);
   *col = in / high;
-  *row = band * kGroup + in % high;
+  *row = band * g.group + in % high;
 }
 
 template <typename T, bool GATED, uint32_t BN>
@@ -250,20 +263,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t q = warp & 3, odd = (warp - 2) / 4, box = base + kStages * S::kStage + (warp - 2) * kBox;
     float(&cs)[GATED ? 2 : 1][32] = sh.col_scale[warp - 2];
     auto first = [&](uint32_t i) { return (odd + 2 * (i / kPer)) * kBoxCols + i % kPer * 32; };  // column of load i
-    uint32_t n = 0;
-    for (uint32_t i = pair; i < g.all; i += pairs, ++n) {
+    // Scales of a tile, a row's and the columns' a lane each: a tile ahead, as they come from L2.
+    struct Scales {
+      uint32_t t0, n0;
+      float x, w[GATED ? 2 : 1][kMine];
+    };
+    auto scales_of = [&](uint32_t i, Scales &sc) {
+      if (i >= g.all) return;
       uint32_t row, col;
       tile_at(g, i, &row, &col);
-      const uint32_t t0 = row * kBM + rank * kHalf + 32 * q, n0 = col * kCols, src = tmem + ((32 * q) << 16) + n % 2 * kAccCols;
-      const float xs = t0 + lane < a.t ? a.x_scale[t0 + lane] : 0.0f;
-      float ws[GATED ? 2 : 1][kMine];  // scales of the columns, a lane each: here before the sums are
+      sc.t0 = row * kBM + rank * kHalf + 32 * q;
+      sc.n0 = col * kCols;
+      sc.x = sc.t0 + lane < a.t ? a.x_scale[sc.t0 + lane] : 0.0f;
 #pragma unroll
       for (uint32_t m = 0; m < (GATED ? 2 : 1); ++m)
 #pragma unroll
         for (uint32_t k = 0; k < kMine; ++k) {
-          const uint32_t nc = n0 + first(k) + lane;
-          ws[m][k] = first(k) < kCols && nc < a.n ? a.w_scale[m][nc] : 0.0f;
+          const uint32_t nc = sc.n0 + first(k) + lane;
+          sc.w[m][k] = first(k) < kCols && nc < a.n ? a.w_scale[m][nc] : 0.0f;
         }
+    };
+    uint32_t n = 0;
+    Scales next;
+    scales_of(pair, next);
+    for (uint32_t i = pair; i < g.all; i += pairs, ++n) {
+      Scales now = next;
+      scales_of(i + pairs, next);
+      const uint32_t t0 = now.t0, n0 = now.n0, src = tmem + ((32 * q) << 16) + n % 2 * kAccCols;
+      const float xs = now.x;
+      float(&ws)[GATED ? 2 : 1][kMine] = now.w;
       const bool ok = wait(sums_full(n & 1), n / 2);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
@@ -322,21 +350,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           __syncwarp();
+          constexpr uint32_t kOnce = 8;
 #pragma unroll 1
-          for (uint32_t rr = 0; rr < 32 && t0 + rr < a.t; ++rr) {
-            T *const y = static_cast<T *>(a.y) + (size_t)(t0 + rr) * a.y_ld;
-            for (uint32_t e = lane; e < kBoxCols && c0 + e < a.n; e += 32) {
-              const uint32_t at = box + rr * 128 + (((e * (uint32_t)sizeof(T) / 16) ^ (rr & 7)) << 4) + e * (uint32_t)sizeof(T) % 16;
-              if constexpr (sizeof(T) == 4) {
-                float f;
-                asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(f) : "r"(at) : "memory");
-                y[c0 + e] = f;
-              } else {
-                uint16_t h;
-                asm volatile("ld.shared.u16 %0, [%1];\n" : "=h"(h) : "r"(at) : "memory");
-                y[c0 + e] = __ushort_as_bfloat16(h);
+          for (uint32_t r0 = 0; r0 < 32 && t0 + r0 < a.t; r0 += kOnce) {
+            T v[kOnce][kPer];
+#pragma unroll
+            for (uint32_t rr = 0; rr < kOnce; ++rr)
+#pragma unroll
+              for (uint32_t e = 0; e < kPer; ++e) {
+                const uint32_t c = e * 32 + lane, row = r0 + rr;
+                v[rr][e] = ld_shared<T>(box + row * 128 + (((c * (uint32_t)sizeof(T) / 16) ^ (row & 7)) << 4) + c * (uint32_t)sizeof(T) % 16);
               }
-            }
+#pragma unroll
+            for (uint32_t rr = 0; rr < kOnce; ++rr)
+#pragma unroll
+              for (uint32_t e = 0; e < kPer; ++e)
+                if (t0 + r0 + rr < a.t && c0 + e * 32 + lane < a.n)
+                  static_cast<T *>(a.y)[(size_t)(t0 + r0 + rr) * a.y_ld + c0 + e * 32 + lane] = v[rr][e];
           }
           __syncwarp();
         }
@@ -615,23 +645,53 @@ PairVariant pair_variant(uint32_t dtype, bool gated, uint32_t bn) {
   return gated ? pair_variant<__nv_bfloat16, true>(bn) : pair_variant<__nv_bfloat16, false>(bn);
 }
 
-cudaError_t launch_pair(uint32_t dtype, bool gated, const I8Args &a, int num_sms, cudaStream_t s) {
-  const PairVariant v = pair_variant(dtype, gated, BNSEL);
-  const uint32_t cols = gated ? v.bn / 2 : v.bn, es = dtype == SX_F32 ? 4 : 2;
+
+struct PairPlan {
+  uint32_t bn;
   Tiles g;
-  g.rows = (a.t + kBM - 1) / kBM;
-  g.cols = (a.n + cols - 1) / cols;
-  g.all = g.rows * g.cols;
+  float us;
+};
+constexpr uint64_t kGroupBytes = 32u << 20;
+
+// Tiles of 256 columns, or of 128 where that leaves half of the pairs without one.  The time, by what was
+// measured: 5 us beside the steps of 128 of K, and those 0.30 us, 0.42 at the clock that the power cap leaves in
+// long calls; with 128 columns 4.2 and 0.27 us.  Tiles with little K wait for their values (2.7 us each), and lanes store
+// for 2.5 us longer.
+PairPlan pair_plan(uint32_t dtype, bool gated, const I8Args &a, uint32_t sms) {
+  PairPlan p{256, {}, 0.0f};
+  const uint32_t pairs = sms / 2, es = dtype == SX_F32 ? 4 : 2, steps = (a.k + kBK - 1) / kBK;
+  const uint64_t rows = (a.t + kBM - 1) / kBM;
+  auto cols = [&](uint32_t bn) -> uint64_t {
+    const uint32_t c = gated ? bn / 2 : bn;
+    return (a.n + c - 1) / c;
+  };
+  if (2 * rows * cols(256) <= pairs) p.bn = 128;
+  p.g.rows = (uint32_t)rows;
+  p.g.cols = (uint32_t)cols(p.bn);
+  p.g.all = p.g.rows * p.g.cols;
+  // Rows of x that stay in L2 while the columns' weights go by: the more there are, the fewer times that weights which
+  // do not fit L2 come from memory (118 MB of gate and up, 16896 rows of 3840: 8, 16, 32 tiles 1466, 1419, 1400 us), but
+  // not past what L2 keeps (16384 rows of 15360: 696, 725, 788).
+  p.g.group = (uint32_t)std::min<uint64_t>(32, std::max<uint64_t>(1, kGroupBytes / ((uint64_t)kBM * a.k)));
   // (a TMA store writes whole 16 bytes, those of a row's end too)
-  g.lanes = ((uintptr_t)a.y | (uintptr_t)a.y_ld * es | (uintptr_t)a.n * es) % 16 != 0;
+  p.g.lanes = ((uintptr_t)a.y | (uintptr_t)a.y_ld * es | (uintptr_t)a.n * es) % 16 != 0;
+  const uint32_t waves = (p.g.all + pairs - 1) / pairs;
+  p.us = p.bn == 128 ? 4.2f + 0.27f * steps : 5.0f + waves * std::max((waves > 2 ? 0.42f : 0.30f) * steps, 2.7f);
+  if (p.g.lanes) p.us += waves * 2.5f;
+  return p;
+}
+
+cudaError_t launch_pair(uint32_t dtype, bool gated, const I8Args &a, const PairPlan &p, uint32_t sms, cudaStream_t s) {
+  const PairVariant v = pair_variant(dtype, gated, p.bn);
+  const uint32_t es = dtype == SX_F32 ? 4 : 2;
   Maps maps{};
   bool ok = encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.k, a.t, a.x_ld, kBK, kHalf);
   for (int i = 0; i < (gated ? 2 : 1); ++i) ok = ok && encode(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, v.bn / 2);
-  if (!g.lanes)
+  if (!p.g.lanes)
     ok = ok && encode(&maps.y, dtype == SX_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.n, a.t,
                       (uint64_t)a.y_ld * es, 128 / es, 32);
   if (!ok) return cudaErrorInvalidValue;
-  return launch_chained(v.fn, dim3(2 * std::min<uint32_t>(g.all, num_sms / 2)), dim3(kThreads), kMaxSmem, s, 2, maps, a, g);
+  return launch_chained(v.fn, dim3(2 * std::min(p.g.all, sms / 2)), dim3(kThreads), kMaxSmem, s, 2, maps, a, p.g);
 }
 
 using SplitKernel = void (*)(const Maps, const I8Args, const SplitShape);
@@ -641,36 +701,78 @@ SplitKernel split_kernel(uint32_t dtype, bool gated) {
 }
 constexpr uint32_t kSplitSmem = 220 * 1024, kSplitSmemTwo = 108 * 1024;  // one CTA an SM, two
 
-cudaError_t launch_split(uint32_t dtype, bool gated, const I8Args &a, int num_sms, cudaStream_t s) {
-  const uint32_t mats = gated ? 2 : 1, most = gated ? 128 : 256, sms = num_sms;
+
+struct SplitPlan {
   SplitShape p;
-  uint32_t t_tiles = (a.t + most - 1) / most;
-  const uint32_t n_tiles = (a.n + kWRows - 1) / kWRows;
-  p.tok = ((a.t + t_tiles - 1) / t_tiles + 15) / 16 * 16;
-  t_tiles = (a.t + p.tok - 1) / p.tok;
-  const uint32_t tiles = n_tiles * t_tiles, steps = (a.k + kBK - 1) / kBK;
-  p.cluster = 1;
-  while (p.cluster < 8 && 2 * p.cluster * tiles <= sms && 2 * p.cluster * 2 <= steps) p.cluster *= 2;
-  p.tmem_cols = 32;
-  while (p.tmem_cols < mats * p.tok) p.tmem_cols *= 2;
-  const uint32_t room = tiles * p.cluster <= sms ? kSplitSmem : kSplitSmemTwo, stage = mats * kWTile + p.tok * kBK;
-  p.stages = std::min(12u, (room - 1024) / stage);
-  const uint32_t smem = std::max(p.stages * stage, p.tok * mats * kWRows * 4) + 1024;  // the stages, then the sums
+  uint32_t n_tiles, t_tiles, smem;
+  float us;
+};
+// The time, by what was measured: 3.3 us, the stages at 110 KB a us and SM or the weights at 6.2 TB/s, whichever is
+// longer, and 13 ns for each row of a tile and matrix.
+SplitPlan split_plan(bool gated, const I8Args &a, const uint32_t (&clusters)[4]) {
+  const uint32_t mats = gated ? 2 : 1, most = gated ? 128 : 256, steps = (a.k + kBK - 1) / kBK;
+  SplitPlan s{};
+  s.t_tiles = (a.t + most - 1) / most;
+  s.n_tiles = (a.n + kWRows - 1) / kWRows;
+  s.p.tok = ((a.t + s.t_tiles - 1) / s.t_tiles + 15) / 16 * 16;
+  s.t_tiles = (a.t + s.p.tok - 1) / s.p.tok;
+  const uint64_t tiles = (uint64_t)s.n_tiles * s.t_tiles;
+  const uint32_t stage = mats * kWTile + s.p.tok * kBK;
+  s.p.cluster = 1;
+  for (uint32_t i = 1; i < 4 && tiles <= clusters[i] && (2u << i) <= steps; ++i) s.p.cluster = 1u << i;
+  s.p.tmem_cols = 32;
+  while (s.p.tmem_cols < mats * s.p.tok) s.p.tmem_cols *= 2;
+  const uint32_t sums = s.p.tok * mats * kWRows * 4;
+  const bool two = tiles > clusters[0];  // CTAs an SM, where there are more than SMs
+  s.p.stages = std::min(12u, ((two ? kSplitSmemTwo : kSplitSmem) - 1024) / stage);
+  s.smem = std::max(s.p.stages * stage, sums) + 1024;  // the stages, then the sums
+  const float waves = tiles <= clusters[0] ? 1.0f : (float)((tiles + clusters[0] - 1) / clusters[0]);
+  const float load = (float)((steps + s.p.cluster - 1) / s.p.cluster) * (float)stage * (1.0f / 110e3f);
+  const float memory = (float)mats * (float)a.n * (float)a.k * (1.0f / 6.2e6f);
+  s.us = 3.3f + std::max(waves * load, memory) + waves * 0.013f * (float)(s.p.tok * mats);
+  return s;
+}
+
+cudaError_t launch_split(uint32_t dtype, bool gated, const I8Args &a, const SplitPlan &p, cudaStream_t s) {
   Maps maps{};
-  bool ok = encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.k, a.t, a.x_ld, kBK, p.tok);
-  for (uint32_t i = 0; i < mats; ++i) ok = ok && encode(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, kWRows);
+  bool ok = encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.k, a.t, a.x_ld, kBK, p.p.tok);
+  for (int i = 0; i < (gated ? 2 : 1); ++i) ok = ok && encode(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, kWRows);
   if (!ok) return cudaErrorInvalidValue;
-  return launch_chained(split_kernel(dtype, gated), dim3(n_tiles * p.cluster, t_tiles), dim3(kThreads), smem, s, p.cluster, maps, a, p);
+  return launch_chained(split_kernel(dtype, gated), dim3(p.n_tiles * p.p.cluster, p.t_tiles), dim3(kThreads), p.smem, s, p.p.cluster, maps, a, p.p);
+}
+
+// Few rows or few tiles: weights as the rows of the products; else tiles of pairs.
+cudaError_t launch_tiles(uint32_t dtype, bool gated, const I8Args &a, int num_sms, const uint32_t (&clusters)[4], cudaStream_t s) {
+  const PairPlan pair = pair_plan(dtype, gated, a, num_sms);
+  const SplitPlan split = split_plan(gated, a, clusters);
+  if (split.t_tiles <= 65535 && split.us < pair.us) return launch_split(dtype, gated, a, split, s);
+  return launch_pair(dtype, gated, a, pair, num_sms, s);
 }
 
 }  // namespace
 
-cudaError_t prepare_gemm_i8() {
+cudaError_t prepare_gemm_i8(uint32_t (&clusters)[4]) {
   for (uint32_t dtype : {SX_F32, SX_BF16})
     for (bool gated : {false, true}) {
       const cudaError_t e = cudaFuncSetAttribute(split_kernel(dtype, gated), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSplitSmem);
       if (e != cudaSuccess) return e;
     }
+  for (uint32_t i = 0; i < 4; ++i) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 1u << i;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(1u << i);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kSplitSmem;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, split_kernel(SX_F32, false), &cfg);
+    if (e != cudaSuccess) return e;
+    if (n > 0) clusters[i] = (uint32_t)n;
+  }
   for (uint32_t dtype : {SX_F32, SX_BF16})
     for (bool gated : {false, true})
       for (uint32_t bn : {128u, 256u}) {
@@ -712,8 +814,7 @@ sx_status dispatch_i8(const char *what, sx_engine *e, uint32_t dtype, sx::I8Args
   if (ce != cudaSuccess) return sx_host_cuda_status(ce, "cudaSetDevice");
   a.err = e->err_dev;
   return sx_host_cuda_status(a.t <= sx::kI8GemvRows ? sx::launch_gemv_i8(dtype, gated, a, e->num_sms, e->stream)
-                             : a.t <= sx::kSplitRows ? sx::launch_split(dtype, gated, a, e->num_sms, e->stream)
-                                                     : sx::launch_pair(dtype, gated, a, e->num_sms, e->stream), what);
+                                                     : sx::launch_tiles(dtype, gated, a, e->num_sms, e->i8_clusters, e->stream), what);
 }
 
 }  // namespace

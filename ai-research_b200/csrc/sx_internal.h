@@ -342,7 +342,8 @@ cudaError_t prepare_kv8_attn();
 size_t kv8_part_bytes(int num_sms);
 // its form for many rows per kv head (sx_kv8_prompt.cu); the arguments are in sx_kv8.cuh
 cudaError_t prepare_kv8_prompt();
-cudaError_t prepare_gemm_i8();
+// clusters: how many of 1, 2, 4, 8 CTAs with all of an SM's shared memory run at a time
+cudaError_t prepare_gemm_i8(uint32_t (&clusters)[4]);
 size_t kv8_prompt_part_bytes(int num_sms);
 // Probabilities and verification (sx_sample.cu): scratch for the {max, sum} of long rows' chunks
 cudaError_t prepare_sample_kernels();
