@@ -93,47 +93,69 @@ SX_DEV float code_factor(uint32_t top, float sq_sum, float inv, bool norm, float
   return a >= kTiny ? 127.0f / a : 0.0f;
 }
 
-template <typename T>
+// G: groups of 8 elements that a thread holds; 0: rows too long for registers are read again (from L2).
+template <typename T, uint32_t G>
 __global__ void __launch_bounds__(kMaxThreads) quantize_i8_kernel(const __grid_constant__ RowsArgs a) {
   __shared__ RowRed red;
   pdl_launch_dependents();
   pdl_wait();
   const size_t row = blockIdx.x;
   const T *const in = static_cast<const T *>(a.in) + row * a.in_ld;
+  int8_t *const q = static_cast<int8_t *>(a.y) + row * a.y_ld;
   uint32_t top = 0;
   float sum = 0.0f;
-  auto group = [&](uint32_t d, float (&u)[8], bool first) {
-    load8(in + d, u);
+  // u of a group, from x there
+  auto gained = [&](uint32_t d, float (&u)[8]) {
     if (!a.w) return;
     float w[8];
     load8(a.w + d, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (first) sum = fmaf(u[i], u[i], sum);
-      u[i] = __fmul_rn(u[i], w[i]);
-    }
+    for (int i = 0; i < 8; ++i) u[i] = __fmul_rn(u[i], w[i]);
   };
-  for (uint32_t d = 8 * threadIdx.x; d < a.n; d += 8 * blockDim.x) {
-    float u[8];
-    group(d, u, true);
+  auto measure = [&](uint32_t d, float (&u)[8]) {
+    if (a.w)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(u[i], u[i], sum);
+    gained(d, u);
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(u[i]) & 0x7FFFFFFFu);
+  };
+  const uint32_t d0 = 8 * threadIdx.x, step = 8 * blockDim.x;
+  float u[G ? G : 1][8];
+  if constexpr (G > 0) {
+#pragma unroll
+    for (uint32_t g = 0; g < G; ++g)
+      if (d0 + g * step < a.n) load8(in + d0 + g * step, u[g]);
+#pragma unroll
+    for (uint32_t g = 0; g < G; ++g)
+      if (d0 + g * step < a.n) measure(d0 + g * step, u[g]);
+  } else {
+    for (uint32_t d = d0; d < a.n; d += step) {
+      load8(in + d, u[0]);
+      measure(d, u[0]);
+    }
   }
   row_reduce(red, top, sum);
   float scale;
   const float inv = a.w ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : 1.0f;
   const float mul = code_factor(top, sum, inv, a.w != nullptr, &scale);
   if (threadIdx.x == 0) a.scale[row] = scale;
-  for (uint32_t d = 8 * threadIdx.x; d < a.n; d += 8 * blockDim.x) {
-    float u[8];
-    group(d, u, false);
-    store_codes(static_cast<int8_t *>(a.y) + row * a.y_ld + d, u, mul);
+  if constexpr (G > 0) {
+#pragma unroll
+    for (uint32_t g = 0; g < G; ++g)
+      if (d0 + g * step < a.n) store_codes(q + d0 + g * step, u[g], mul);
+  } else {
+    for (uint32_t d = d0; d < a.n; d += step) {
+      load8(in + d, u[0]);
+      gained(d, u[0]);
+      store_codes(q + d, u[0], mul);
+    }
   }
 }
 
 enum RowOut { kOutNone, kOutF32, kOutBf16, kOutI8 };
 
-template <typename T, RowOut OUT>
+template <typename T, RowOut OUT, uint32_t G>
 __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const __grid_constant__ RowsArgs a) {
   __shared__ RowRed red[2];
   pdl_launch_dependents();
@@ -142,34 +164,61 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const __grid
   const T *const r = static_cast<const T *>(a.in) + row * a.in_ld;
   const float *const x = a.x + row * a.x_ld;
   float *const x_out = a.x_out + row * a.x_out_ld;
+  const uint32_t d0 = 8 * threadIdx.x, step = 8 * blockDim.x;
+  constexpr uint32_t kHeld = G ? G : 1;
+  float h[kHeld][8], v[kHeld][8];
   uint32_t top = 0;
   float sum = 0.0f, post = 1.0f;
-  if (a.post_w) {
-    for (uint32_t d = 8 * threadIdx.x; d < a.n; d += 8 * blockDim.x) {
-      float h[8];
-      load8(r + d, h);
+  if constexpr (G > 0) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(h[i], h[i], sum);
+    for (uint32_t g = 0; g < G; ++g)
+      if (d0 + g * step < a.n) {
+        load8(r + d0 + g * step, h[g]);
+        load8(x + d0 + g * step, v[g]);
+      }
+  }
+  auto squares = [&](const float (&u)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum = fmaf(u[i], u[i], sum);
+  };
+  if (a.post_w) {
+    if constexpr (G > 0) {
+#pragma unroll
+      for (uint32_t g = 0; g < G; ++g)
+        if (d0 + g * step < a.n) squares(h[g]);
+    } else {
+      for (uint32_t d = d0; d < a.n; d += step) {
+        load8(r + d, h[0]);
+        squares(h[0]);
+      }
     }
     row_reduce(red[0], top, sum);
     post = 1.0f / sqrtf(sum / (float)a.n + a.eps);
     sum = 0.0f;
   }
-  for (uint32_t d = 8 * threadIdx.x; d < a.n; d += 8 * blockDim.x) {
-    float h[8], v[8], w[8];
-    load8(r + d, h);
-    load8(x + d, v);
+  // the new residual of a group in u, from x there
+  auto residual = [&](uint32_t d, const float (&t)[8], float (&u)[8]) {
+    float w[8];
     if (a.post_w) load8(a.post_w + d, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = (v[i] + (a.post_w ? h[i] * post * w[i] : h[i])) * a.scalar;
-      sum = fmaf(v[i], v[i], sum);
-    }
-    store8(x_out + d, v);
+    for (int i = 0; i < 8; ++i) u[i] = (u[i] + (a.post_w ? t[i] * post * w[i] : t[i])) * a.scalar;
+    store8(x_out + d, u);
+    squares(u);
     if constexpr (OUT == kOutI8) {
       load8(a.w + d, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(__fmul_rn(v[i], w[i])) & 0x7FFFFFFFu);
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(__fmul_rn(u[i], w[i])) & 0x7FFFFFFFu);
+    }
+  };
+  if constexpr (G > 0) {
+#pragma unroll
+    for (uint32_t g = 0; g < G; ++g)
+      if (d0 + g * step < a.n) residual(d0 + g * step, h[g], v[g]);
+  } else {
+    for (uint32_t d = d0; d < a.n; d += step) {
+      load8(r + d, h[0]);
+      load8(x + d, v[0]);
+      residual(d, h[0], v[0]);
     }
   }
   if constexpr (OUT == kOutNone) return;
@@ -181,36 +230,61 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const __grid
     mul = code_factor(top, sum, inv, true, &scale);
     if (threadIdx.x == 0) a.scale[row] = scale;
   }
-  for (uint32_t d = 8 * threadIdx.x; d < a.n; d += 8 * blockDim.x) {
-    float v[8], w[8];
-    load8(x_out + d, v);
+  auto normed = [&](uint32_t d, float (&u)[8]) {
+    float w[8];
     load8(a.w + d, w);
     if constexpr (OUT == kOutI8) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(v[i], w[i]);
-      store_codes(static_cast<int8_t *>(a.y) + row * a.y_ld + d, v, mul);
+      for (int i = 0; i < 8; ++i) u[i] = __fmul_rn(u[i], w[i]);
+      store_codes(static_cast<int8_t *>(a.y) + row * a.y_ld + d, u, mul);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
+      for (int i = 0; i < 8; ++i) u[i] = u[i] * inv * w[i];
       if constexpr (OUT == kOutF32)
-        store8(static_cast<float *>(a.y) + row * a.y_ld + d, v);
+        store8(static_cast<float *>(a.y) + row * a.y_ld + d, u);
       else
-        store8(static_cast<__nv_bfloat16 *>(a.y) + row * a.y_ld + d, v);
+        store8(static_cast<__nv_bfloat16 *>(a.y) + row * a.y_ld + d, u);
+    }
+  };
+  if constexpr (G > 0) {
+#pragma unroll
+    for (uint32_t g = 0; g < G; ++g)
+      if (d0 + g * step < a.n) normed(d0 + g * step, v[g]);
+  } else {
+    for (uint32_t d = d0; d < a.n; d += step) {
+      load8(x_out + d, v[0]);
+      normed(d, v[0]);
     }
   }
 }
 
 using RowsKernel = void (*)(const RowsArgs);
 
-cudaError_t launch_rows(RowsKernel k, const RowsArgs &a, cudaStream_t s) {
-  const uint32_t threads = std::min(kMaxThreads, (a.n / 8 + 31) / 32 * 32);
+// Groups of 8 that a thread holds: one where rows are few (more threads end sooner), else up to `most`; 0 past
+// kMaxThreads times that.
+uint32_t groups_of(uint32_t n, uint32_t rows, uint32_t most, uint32_t sms) {
+  const uint32_t groups = n / 8;
+  uint32_t g = rows <= 2 * sms || groups <= 32 ? 1 : most;
+  while (g < most && groups > g * kMaxThreads) g *= 2;
+  return groups > g * kMaxThreads ? 0 : g;
+}
+cudaError_t launch_rows(RowsKernel k, const RowsArgs &a, uint32_t g, cudaStream_t s) {
+  const uint32_t each = 8 * (g ? g : 1), threads = std::min(kMaxThreads, ((a.n + each - 1) / each + 31) / 32 * 32);
   return launch_chained(k, dim3(a.rows), dim3(threads), 0, s, 1, a);
 }
 
 template <typename T>
-RowsKernel residual_kernel(bool none, uint32_t y_dtype) {
-  if (none) return residual_norm_kernel<T, kOutNone>;
-  return y_dtype == SX_F32 ? residual_norm_kernel<T, kOutF32> : y_dtype == SX_BF16 ? residual_norm_kernel<T, kOutBf16> : residual_norm_kernel<T, kOutI8>;
+RowsKernel quantize_kernel(uint32_t g) {
+  return g == 0 ? quantize_i8_kernel<T, 0> : g == 1 ? quantize_i8_kernel<T, 1> : g == 2 ? quantize_i8_kernel<T, 2> : quantize_i8_kernel<T, 4>;
+}
+template <typename T, RowOut OUT>
+RowsKernel residual_kernel(uint32_t g) {
+  return g == 0 ? residual_norm_kernel<T, OUT, 0> : g == 1 ? residual_norm_kernel<T, OUT, 1> : residual_norm_kernel<T, OUT, 2>;
+}
+template <typename T>
+RowsKernel residual_kernel(bool none, uint32_t y_dtype, uint32_t g) {
+  if (none) return residual_kernel<T, kOutNone>(g);
+  return y_dtype == SX_F32 ? residual_kernel<T, kOutF32>(g) : y_dtype == SX_BF16 ? residual_kernel<T, kOutBf16>(g) : residual_kernel<T, kOutI8>(g);
 }
 
 uint32_t bytes_of(uint32_t dtype) { return dtype == SX_F32 ? 4 : dtype == SX_BF16 ? 2 : 1; }
@@ -251,8 +325,9 @@ SX_API sx_status sx_dispatch_quantize_i8(sx_engine *e, const sx_quantize_i8_args
   r.rows = a->rows;
   r.n = a->n;
   r.eps = a->eps;
+  const uint32_t g = sx::groups_of(a->n, a->rows, 4, e->num_sms);
   return sx_host_cuda_status(
-      sx::launch_rows(a->dtype == SX_F32 ? sx::quantize_i8_kernel<float> : sx::quantize_i8_kernel<__nv_bfloat16>, r, e->stream),
+      sx::launch_rows(a->dtype == SX_F32 ? sx::quantize_kernel<float>(g) : sx::quantize_kernel<__nv_bfloat16>(g), r, g, e->stream),
       "quantize_i8 launch");
 }
 
@@ -302,9 +377,10 @@ SX_API sx_status sx_dispatch_residual_norm(sx_engine *e, const sx_residual_norm_
   r.scalar = a->scalar;
   r.eps = a->eps;
   const bool none = a->y == nullptr;
+  const uint32_t g = sx::groups_of(a->n, a->rows, 2, e->num_sms);
   return sx_host_cuda_status(
-      sx::launch_rows(a->r_dtype == SX_F32 ? sx::residual_kernel<float>(none, a->y_dtype) : sx::residual_kernel<__nv_bfloat16>(none, a->y_dtype),
-                      r, e->stream),
+      sx::launch_rows(a->r_dtype == SX_F32 ? sx::residual_kernel<float>(none, a->y_dtype, g) : sx::residual_kernel<__nv_bfloat16>(none, a->y_dtype, g),
+                      r, g, e->stream),
       "residual_norm launch");
 }
 
