@@ -27,20 +27,37 @@ struct RowsArgs {
   float scalar, eps;
 };
 
+// 8 elements as they are in memory, and as f32
 template <typename T>
-SX_DEV void load8(const T *p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    load_vec<T, 8>(p, v);
-  } else {
-    float a[4], b[4];
-    load_vec<T, 4>(p, a);
-    load_vec<T, 4>(p + 4, b);
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+};
+template <typename T>
+SX_DEV void load_raw(const T *p, Raw8<T> &r) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = a[i];
-      v[4 + i] = b[i];
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = reinterpret_cast<const uint4 *>(p)[i];
+}
+template <typename T>
+SX_DEV void unpack8(const Raw8<T> &r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+    const uint32_t w[4] = {r.v[i].x, r.v[i].y, r.v[i].z, r.v[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (sizeof(T) == 4) {
+        v[4 * i + k] = __uint_as_float(w[k]);
+      } else {
+        v[2 * k] = __uint_as_float(w[k] << 16);
+        v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+      }
     }
   }
+}
+template <typename T>
+SX_DEV void load8(const T *p, float (&v)[8]) {
+  Raw8<T> r;
+  load_raw(p, r);
+  unpack8(r, v);
 }
 template <typename T>
 SX_DEV void store8(T *p, const float (&v)[8]) {
@@ -52,15 +69,28 @@ SX_DEV void store8(T *p, const float (&v)[8]) {
     store_vec<T, 4>(p + 4, b);
   }
 }
+// Codes of 8 values: adding 1.5 2^23 rounds a value of up to 127 to a whole number, ties to even, which is then the
+// sum's low byte.  mul 0: a row without values, whatever its elements.
 SX_DEV void store_codes(int8_t *p, const float (&u)[8], float mul) {
-  uint32_t w[2];
+  constexpr float kMagic = 12582912.0f;
+  uint32_t w[2] = {0, 0};
+  if (mul != 0.0f) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    w[h] = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[h] |= ((uint32_t)__float2int_rn(__fmul_rn(u[4 * h + i], mul)) & 0xFFu) << (8 * i);
+    for (int h = 0; h < 2; ++h) {
+      // (products apart: a paired one and the sum after it would become one operation, with one rounding)
+      const float2 c = make_float2(kMagic, kMagic);
+      const float2 x = add2(make_float2(__fmul_rn(u[4 * h], mul), __fmul_rn(u[4 * h + 1], mul)), c);
+      const float2 y = add2(make_float2(__fmul_rn(u[4 * h + 2], mul), __fmul_rn(u[4 * h + 3], mul)), c);
+      w[h] = prmt(prmt(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040), prmt(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040), 0x5410);
+    }
   }
   *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+}
+// the larger of top and |x|, a NaN where there is one
+SX_DEV float top_of(float top, float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(top), "f"(fabsf(x)));
+  return r;
 }
 
 // The largest `top` and the sum of `sum` over the CTA.
@@ -68,11 +98,13 @@ struct RowRed {
   uint32_t top[32];
   float sum[32];
 };
+// WARP: a row has a warp, else the CTA.
+template <bool WARP>
 SX_DEV void row_reduce(RowRed &red, uint32_t &top, float &sum) {
   const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   top = __reduce_max_sync(0xffffffffu, top);
   sum = warp_sum(sum);
-  if (warps == 1) return;
+  if (WARP || warps == 1) return;
   if (lane == 0) {
     red.top[warp] = top;
     red.sum[warp] = sum;
@@ -80,6 +112,17 @@ SX_DEV void row_reduce(RowRed &red, uint32_t &top, float &sum) {
   __syncthreads();
   top = __reduce_max_sync(0xffffffffu, lane < warps ? red.top[lane] : 0u);
   sum = warp_sum(lane < warps ? red.sum[lane] : 0.0f);
+}
+// This thread's row, its first element and how far its next are
+struct Place {
+  size_t row;
+  uint32_t d0, step;
+};
+constexpr uint32_t kWarpRows = 8;  // rows of a CTA with WARP
+template <bool WARP>
+SX_DEV Place place() {
+  if (WARP) return {(size_t)blockIdx.x * kWarpRows + (threadIdx.x >> 5), 8 * (threadIdx.x & 31), 8 * 32};
+  return {blockIdx.x, 8 * threadIdx.x, 8 * blockDim.x};
 }
 
 // What a row's codes are multiplied by, and its scale.
@@ -94,86 +137,99 @@ SX_DEV float code_factor(uint32_t top, float sq_sum, float inv, bool norm, float
 }
 
 // G: groups of 8 elements that a thread holds; 0: rows too long for registers are read again (from L2).
-template <typename T, uint32_t G>
-__global__ void __launch_bounds__(kMaxThreads) quantize_i8_kernel(const __grid_constant__ RowsArgs a) {
+template <typename T, bool WARP, uint32_t G>
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads) quantize_i8_kernel(const __grid_constant__ RowsArgs a) {
   __shared__ RowRed red;
   pdl_launch_dependents();
   pdl_wait();
-  const size_t row = blockIdx.x;
-  const T *const in = static_cast<const T *>(a.in) + row * a.in_ld;
-  int8_t *const q = static_cast<int8_t *>(a.y) + row * a.y_ld;
-  uint32_t top = 0;
-  float sum = 0.0f;
+  const Place p = place<WARP>();
+  if (WARP && p.row >= a.rows) return;
+  const uint32_t d0 = p.d0, step = p.step;
+  const T *const in = static_cast<const T *>(a.in) + p.row * a.in_ld;
+  int8_t *const q = static_cast<int8_t *>(a.y) + p.row * a.y_ld;
+  float top = 0.0f, sum = 0.0f, u[8];
   // u of a group, from x there
-  auto gained = [&](uint32_t d, float (&u)[8]) {
+  auto gained = [&](uint32_t d) {
     if (!a.w) return;
     float w[8];
     load8(a.w + d, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) u[i] = __fmul_rn(u[i], w[i]);
   };
-  auto measure = [&](uint32_t d, float (&u)[8]) {
+  auto measure = [&](uint32_t d) {
     if (a.w)
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum = fmaf(u[i], u[i], sum);
-    gained(d, u);
+    gained(d);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(u[i]) & 0x7FFFFFFFu);
+    for (int i = 0; i < 8; ++i) top = top_of(top, u[i]);
   };
-  const uint32_t d0 = 8 * threadIdx.x, step = 8 * blockDim.x;
-  float u[G ? G : 1][8];
+  Raw8<T> held[G ? G : 1];
   if constexpr (G > 0) {
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
-      if (d0 + g * step < a.n) load8(in + d0 + g * step, u[g]);
+      if (d0 + g * step < a.n) load_raw(in + d0 + g * step, held[g]);
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
-      if (d0 + g * step < a.n) measure(d0 + g * step, u[g]);
+      if (d0 + g * step < a.n) {
+        unpack8(held[g], u);
+        measure(d0 + g * step);
+      }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
-      load8(in + d, u[0]);
-      measure(d, u[0]);
+      load8(in + d, u);
+      measure(d);
     }
   }
-  row_reduce(red, top, sum);
+  uint32_t bits = __float_as_uint(top) & 0x7FFFFFFFu;  // (their order is the values', with infinity and NaN on top)
+  row_reduce<WARP>(red, bits, sum);
   float scale;
   const float inv = a.w ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : 1.0f;
-  const float mul = code_factor(top, sum, inv, a.w != nullptr, &scale);
-  if (threadIdx.x == 0) a.scale[row] = scale;
+  const float mul = code_factor(bits, sum, inv, a.w != nullptr, &scale);
+  if (d0 == 0) a.scale[p.row] = scale;
   if constexpr (G > 0) {
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
-      if (d0 + g * step < a.n) store_codes(q + d0 + g * step, u[g], mul);
+      if (d0 + g * step < a.n) {
+        unpack8(held[g], u);
+        gained(d0 + g * step);
+        store_codes(q + d0 + g * step, u, mul);
+      }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
-      load8(in + d, u[0]);
-      gained(d, u[0]);
-      store_codes(q + d, u[0], mul);
+      load8(in + d, u);
+      gained(d);
+      store_codes(q + d, u, mul);
     }
   }
 }
 
 enum RowOut { kOutNone, kOutF32, kOutBf16, kOutI8 };
 
-template <typename T, RowOut OUT, uint32_t G>
-__global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const __grid_constant__ RowsArgs a) {
+// (f32 rows with four groups a thread read r again: 64 registers of a row's would leave one CTA an SM)
+template <typename T, RowOut OUT, bool WARP, uint32_t G>
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads) residual_norm_kernel(const __grid_constant__ RowsArgs a) {
   __shared__ RowRed red[2];
   pdl_launch_dependents();
   pdl_wait();
-  const size_t row = blockIdx.x;
+  const Place p = place<WARP>();
+  const size_t row = p.row;
+  if (WARP && row >= a.rows) return;
   const T *const r = static_cast<const T *>(a.in) + row * a.in_ld;
   const float *const x = a.x + row * a.x_ld;
   float *const x_out = a.x_out + row * a.x_out_ld;
-  const uint32_t d0 = 8 * threadIdx.x, step = 8 * blockDim.x;
+  const uint32_t d0 = p.d0, step = p.step;
   constexpr uint32_t kHeld = G ? G : 1;
-  float h[kHeld][8], v[kHeld][8];
-  uint32_t top = 0;
-  float sum = 0.0f, post = 1.0f;
+  constexpr bool kAgain = !WARP && G == 4 && sizeof(T) == 4;
+  Raw8<T> held[kAgain ? 1 : kHeld];
+  float h[8], v[kHeld][8];
+  uint32_t bits = 0;
+  float top = 0.0f, sum = 0.0f, post = 1.0f;
   if constexpr (G > 0) {
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
       if (d0 + g * step < a.n) {
-        load8(r + d0 + g * step, h[g]);
+        if constexpr (!kAgain) load_raw(r + d0 + g * step, held[g]);
         load8(x + d0 + g * step, v[g]);
       }
   }
@@ -185,14 +241,20 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const __grid
     if constexpr (G > 0) {
 #pragma unroll
       for (uint32_t g = 0; g < G; ++g)
-        if (d0 + g * step < a.n) squares(h[g]);
+        if (d0 + g * step < a.n) {
+          if constexpr (kAgain)
+            load8(r + d0 + g * step, h);
+          else
+            unpack8(held[g], h);
+          squares(h);
+        }
     } else {
       for (uint32_t d = d0; d < a.n; d += step) {
-        load8(r + d, h[0]);
-        squares(h[0]);
+        load8(r + d, h);
+        squares(h);
       }
     }
-    row_reduce(red[0], top, sum);
+    row_reduce<WARP>(red[0], bits, sum);
     post = 1.0f / sqrtf(sum / (float)a.n + a.eps);
     sum = 0.0f;
   }
@@ -207,28 +269,35 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const __grid
     if constexpr (OUT == kOutI8) {
       load8(a.w + d, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(__fmul_rn(u[i], w[i])) & 0x7FFFFFFFu);
+      for (int i = 0; i < 8; ++i) top = top_of(top, __fmul_rn(u[i], w[i]));
     }
   };
   if constexpr (G > 0) {
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
-      if (d0 + g * step < a.n) residual(d0 + g * step, h[g], v[g]);
+      if (d0 + g * step < a.n) {
+        if constexpr (kAgain)
+          load8(r + d0 + g * step, h);
+        else
+          unpack8(held[g], h);
+        residual(d0 + g * step, h, v[g]);
+      }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
-      load8(r + d, h[0]);
+      load8(r + d, h);
       load8(x + d, v[0]);
-      residual(d, h[0], v[0]);
+      residual(d, h, v[0]);
     }
   }
   if constexpr (OUT == kOutNone) return;
-  row_reduce(red[1], top, sum);
+  bits = __float_as_uint(top) & 0x7FFFFFFFu;
+  row_reduce<WARP>(red[1], bits, sum);
   const float inv = 1.0f / sqrtf(sum / (float)a.n + a.eps);
   float mul = 0.0f;
   if constexpr (OUT == kOutI8) {
     float scale;
-    mul = code_factor(top, sum, inv, true, &scale);
-    if (threadIdx.x == 0) a.scale[row] = scale;
+    mul = code_factor(bits, sum, inv, true, &scale);
+    if (d0 == 0) a.scale[row] = scale;
   }
   auto normed = [&](uint32_t d, float (&u)[8]) {
     float w[8];
@@ -260,31 +329,53 @@ __global__ void __launch_bounds__(kMaxThreads) residual_norm_kernel(const __grid
 
 using RowsKernel = void (*)(const RowsArgs);
 
-// Groups of 8 that a thread holds: one where rows are few (more threads end sooner), else up to `most`; 0 past
-// kMaxThreads times that.
-uint32_t groups_of(uint32_t n, uint32_t rows, uint32_t most, uint32_t sms) {
+// How rows are laid over threads.
+struct RowsPlan {
+  bool warp;
+  uint32_t g, threads, ctas;
+};
+// Few rows: a CTA each with a thread for every 8 elements, which ends soonest.  Many short ones: a warp each, as CTAs
+// start at most one a ns (60000 rows of 256 as CTAs 63 us).  Else a CTA each, up to `most` groups a thread.
+RowsPlan rows_plan(uint32_t n, uint32_t rows, uint32_t warp_most, uint32_t most, uint32_t sms) {
   const uint32_t groups = n / 8;
-  uint32_t g = rows <= 2 * sms || groups <= 32 ? 1 : most;
-  while (g < most && groups > g * kMaxThreads) g *= 2;
-  return groups > g * kMaxThreads ? 0 : g;
-}
-cudaError_t launch_rows(RowsKernel k, const RowsArgs &a, uint32_t g, cudaStream_t s) {
-  const uint32_t each = 8 * (g ? g : 1), threads = std::min(kMaxThreads, ((a.n + each - 1) / each + 31) / 32 * 32);
-  return launch_chained(k, dim3(a.rows), dim3(threads), 0, s, 1, a);
+  RowsPlan p{false, 1, 0, rows};
+  if (rows > 2 * sms && groups <= 32 * warp_most) {
+    p.warp = true;
+    while (groups > 32 * p.g) p.g *= 2;
+    p.threads = 32 * kWarpRows;
+    p.ctas = (rows + kWarpRows - 1) / kWarpRows;
+    return p;
+  }
+  if (rows > 2 * sms && groups > 128) p.g = std::min(rows > 32 * sms || groups > 1024 ? 4u : 2u, most);
+  while (p.g < most && groups > p.g * kMaxThreads) p.g *= 2;
+  if (groups > p.g * kMaxThreads) p.g = 0;
+  const uint32_t each = p.g ? p.g : 1;
+  p.threads = std::min(kMaxThreads, ((groups + each - 1) / each + 31) / 32 * 32);
+  return p;
 }
 
+using RowsKernel = void (*)(const RowsArgs);
 template <typename T>
-RowsKernel quantize_kernel(uint32_t g) {
-  return g == 0 ? quantize_i8_kernel<T, 0> : g == 1 ? quantize_i8_kernel<T, 1> : g == 2 ? quantize_i8_kernel<T, 2> : quantize_i8_kernel<T, 4>;
+RowsKernel quantize_kernel(const RowsPlan &p) {
+  if (p.warp) {
+    if constexpr (sizeof(T) == 2)
+      if (p.g == 8) return quantize_i8_kernel<T, true, 8>;
+    return p.g == 1 ? quantize_i8_kernel<T, true, 1> : p.g == 2 ? quantize_i8_kernel<T, true, 2> : quantize_i8_kernel<T, true, 4>;
+  }
+  return p.g == 0 ? quantize_i8_kernel<T, false, 0> : p.g == 1 ? quantize_i8_kernel<T, false, 1>
+       : p.g == 2 ? quantize_i8_kernel<T, false, 2> : quantize_i8_kernel<T, false, 4>;
 }
 template <typename T, RowOut OUT>
-RowsKernel residual_kernel(uint32_t g) {
-  return g == 0 ? residual_norm_kernel<T, OUT, 0> : g == 1 ? residual_norm_kernel<T, OUT, 1> : residual_norm_kernel<T, OUT, 2>;
+RowsKernel residual_kernel(const RowsPlan &p) {
+  if (p.warp)
+    return p.g == 1 ? residual_norm_kernel<T, OUT, true, 1> : p.g == 2 ? residual_norm_kernel<T, OUT, true, 2> : residual_norm_kernel<T, OUT, true, 4>;
+  return p.g == 0 ? residual_norm_kernel<T, OUT, false, 0> : p.g == 1 ? residual_norm_kernel<T, OUT, false, 1>
+       : p.g == 2 ? residual_norm_kernel<T, OUT, false, 2> : residual_norm_kernel<T, OUT, false, 4>;
 }
 template <typename T>
-RowsKernel residual_kernel(bool none, uint32_t y_dtype, uint32_t g) {
-  if (none) return residual_kernel<T, kOutNone>(g);
-  return y_dtype == SX_F32 ? residual_kernel<T, kOutF32>(g) : y_dtype == SX_BF16 ? residual_kernel<T, kOutBf16>(g) : residual_kernel<T, kOutI8>(g);
+RowsKernel residual_kernel(bool none, uint32_t y_dtype, const RowsPlan &p) {
+  if (none) return residual_kernel<T, kOutNone>(p);
+  return y_dtype == SX_F32 ? residual_kernel<T, kOutF32>(p) : y_dtype == SX_BF16 ? residual_kernel<T, kOutBf16>(p) : residual_kernel<T, kOutI8>(p);
 }
 
 uint32_t bytes_of(uint32_t dtype) { return dtype == SX_F32 ? 4 : dtype == SX_BF16 ? 2 : 1; }
@@ -325,9 +416,9 @@ SX_API sx_status sx_dispatch_quantize_i8(sx_engine *e, const sx_quantize_i8_args
   r.rows = a->rows;
   r.n = a->n;
   r.eps = a->eps;
-  const uint32_t g = sx::groups_of(a->n, a->rows, 4, e->num_sms);
-  return sx_host_cuda_status(
-      sx::launch_rows(a->dtype == SX_F32 ? sx::quantize_kernel<float>(g) : sx::quantize_kernel<__nv_bfloat16>(g), r, g, e->stream),
+  const sx::RowsPlan p = sx::rows_plan(a->n, a->rows, a->dtype == SX_F32 ? 4 : 8, 4, e->num_sms);
+  const sx::RowsKernel k = a->dtype == SX_F32 ? sx::quantize_kernel<float>(p) : sx::quantize_kernel<__nv_bfloat16>(p);
+  return sx_host_cuda_status(sx::launch_chained(k, dim3(p.ctas), dim3(p.threads), 0, e->stream, 1, r),
       "quantize_i8 launch");
 }
 
@@ -377,10 +468,10 @@ SX_API sx_status sx_dispatch_residual_norm(sx_engine *e, const sx_residual_norm_
   r.scalar = a->scalar;
   r.eps = a->eps;
   const bool none = a->y == nullptr;
-  const uint32_t g = sx::groups_of(a->n, a->rows, 2, e->num_sms);
+  const sx::RowsPlan p = sx::rows_plan(a->n, a->rows, 4, a->n > 8192 ? 4 : 2, e->num_sms);
   return sx_host_cuda_status(
-      sx::launch_rows(a->r_dtype == SX_F32 ? sx::residual_kernel<float>(none, a->y_dtype, g) : sx::residual_kernel<__nv_bfloat16>(none, a->y_dtype, g),
-                      r, g, e->stream),
+      sx::launch_chained(a->r_dtype == SX_F32 ? sx::residual_kernel<float>(none, a->y_dtype, p) : sx::residual_kernel<__nv_bfloat16>(none, a->y_dtype, p),
+                         dim3(p.ctas), dim3(p.threads), 0, e->stream, 1, r),
       "residual_norm launch");
 }
 
