@@ -627,7 +627,7 @@ bool encode(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t 
   const cuuint64_t dims[2] = {cols, rows}, strides[1] = {ld_bytes};
   const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
   return fn && fn(map, type, 2, const_cast<void *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 using PairKernel = void (*)(const Maps, const I8Args, const Tiles);
@@ -656,7 +656,7 @@ constexpr uint64_t kGroupBytes = 32u << 20;
 // Tiles of 256 columns, or of 128 where that leaves half of the pairs without one.  The time, by what was
 // measured: 5 us beside the steps of 128 of K, and those 0.30 us, 0.42 at the clock that the power cap leaves in
 // long calls; with 128 columns 4.2 and 0.27 us.  Tiles with little K wait for their values (2.7 us each), and lanes store
-// for 2.5 us longer.
+// for 1 us longer.  Weights that L2 does not hold come at 5 TB/s.
 PairPlan pair_plan(uint32_t dtype, bool gated, const I8Args &a, uint32_t sms) {
   PairPlan p{256, {}, 0.0f};
   const uint32_t pairs = sms / 2, es = dtype == SX_F32 ? 4 : 2, steps = (a.k + kBK - 1) / kBK;
@@ -676,8 +676,9 @@ PairPlan pair_plan(uint32_t dtype, bool gated, const I8Args &a, uint32_t sms) {
   // (a TMA store writes whole 16 bytes, those of a row's end too)
   p.g.lanes = ((uintptr_t)a.y | (uintptr_t)a.y_ld * es | (uintptr_t)a.n * es) % 16 != 0;
   const uint32_t waves = (p.g.all + pairs - 1) / pairs;
-  p.us = p.bn == 128 ? 4.2f + 0.27f * steps : 5.0f + waves * std::max((waves > 2 ? 0.42f : 0.30f) * steps, 2.7f);
-  if (p.g.lanes) p.us += waves * 2.5f;
+  const float memory = (gated ? 2.0f : 1.0f) * (float)a.n * (float)a.k * (1.0f / 5.0e6f);
+  p.us = p.bn == 128 ? 4.2f + std::max(0.27f * steps, memory) : 5.0f + std::max(waves * std::max((waves > 2 ? 0.42f : 0.30f) * steps, 2.7f), memory);
+  if (p.g.lanes) p.us += waves * 1.0f;
   return p;
 }
 
@@ -726,10 +727,13 @@ SplitPlan split_plan(bool gated, const I8Args &a, const uint32_t (&clusters)[4])
   const bool two = tiles > clusters[0];  // CTAs an SM, where there are more than SMs
   s.p.stages = std::min(12u, ((two ? kSplitSmemTwo : kSplitSmem) - 1024) / stage);
   s.smem = std::max(s.p.stages * stage, sums) + 1024;  // the stages, then the sums
-  const float waves = tiles <= clusters[0] ? 1.0f : (float)((tiles + clusters[0] - 1) / clusters[0]);
-  const float load = (float)((steps + s.p.cluster - 1) / s.p.cluster) * (float)stage * (1.0f / 110e3f);
+  const float waves = !two ? 1.0f : s.smem <= kSplitSmemTwo ? (float)tiles / (float)clusters[0] : (float)((tiles + clusters[0] - 1) / clusters[0]);
+  const float ragged = (a.w_ld | a.x_ld) % 128 != 0 ? 1.4f : 1.0f;  // rows that begin inside a line
+  const float load = ragged * (float)((steps + s.p.cluster - 1) / s.p.cluster) * (float)stage * (1.0f / 110e3f);
   const float memory = (float)mats * (float)a.n * (float)a.k * (1.0f / 6.2e6f);
-  s.us = 3.3f + std::max(waves * load, memory) + waves * 0.013f * (float)(s.p.tok * mats);
+  const float values = 0.013f * (float)(s.p.tok * mats);
+  // (CTAs that have an SM for themselves start when the ones before have ended)
+  s.us = two && s.smem > kSplitSmemTwo ? waves * (3.3f + load + values) : 3.3f + std::max(waves * load, memory) + waves * values;
   return s;
 }
 
@@ -813,7 +817,10 @@ sx_status dispatch_i8(const char *what, sx_engine *e, uint32_t dtype, sx::I8Args
   const cudaError_t ce = cudaSetDevice(e->device);
   if (ce != cudaSuccess) return sx_host_cuda_status(ce, "cudaSetDevice");
   a.err = e->err_dev;
-  return sx_host_cuda_status(a.t <= sx::kI8GemvRows ? sx::launch_gemv_i8(dtype, gated, a, e->num_sms, e->stream)
+  // Streaming the weights; many short rows of them are few steps for each of its CTAs (32768 x 1024: 1 row 9.7 us, as
+  // tiles 8.1; 16 rows 11.9, 8.0; 32768 x 4096: 1 row 22.7 us).
+  const bool stream = a.t <= sx::kI8GemvRows && (a.k > 2048 || a.n <= (gated ? 48u : 96u) * (uint32_t)e->num_sms);
+  return sx_host_cuda_status(stream ? sx::launch_gemv_i8(dtype, gated, a, e->num_sms, e->stream)
                                                      : sx::launch_tiles(dtype, gated, a, e->num_sms, e->i8_clusters, e->stream), what);
 }
 
