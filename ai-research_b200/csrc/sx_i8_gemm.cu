@@ -1,7 +1,7 @@
 // sx_i8_gemm.cu -- products of int8 rows on the tcgen05 tensor cores (include/sx.h, sx_dispatch_gemm_i8 and
 // sx_dispatch_gate_up_i8).
 //
-// Two CTAs of a cluster take a tile of 256 rows of x and BN columns of y (gate_up: BN / 2 of each matrix), 128
+// Two CTAs of a cluster take a tile of 256 rows of x and 256 columns of y (gate_up: 128 of each matrix), 128
 // rows in the tensor memory of each: tcgen05.mma of the pair (kind::i8, 32-bit sums) reads 128 rows of x and half
 // of the columns' weights from each CTA's shared memory, so both operands are fetched once per pair.  The grid is
 // one pair per two SMs, which goes through the tiles; tensor memory holds two tiles' sums, so that one is
@@ -26,24 +26,20 @@
 namespace sx {
 namespace {
 
-constexpr uint32_t kBM = 256, kBK = 128;        // of a pair
+constexpr uint32_t kBM = 256, kBN = 256, kBK = 128;  // of a pair
 constexpr uint32_t kHalf = kBM / 2;             // rows of a CTA
 constexpr int kEpiWarps = 8, kThreads = (2 + kEpiWarps) * 32;
 constexpr uint32_t kBox = 4096;                 // 32 rows of 128 bytes of y
-constexpr uint32_t kTmemCols = 512, kAccCols = 256;
+constexpr uint32_t kTmemCols = 512;             // two tiles' sums
 
-template <uint32_t BN>
-struct PairShape {
-  static constexpr uint32_t kATile = kHalf * kBK, kBTile = BN / 2 * kBK, kStage = kATile + kBTile;
-  static constexpr uint32_t kStages = 196608 / kStage;
-  static constexpr uint32_t kData = kStages * kStage + kEpiWarps * kBox;
-};
+constexpr uint32_t kATile = kHalf * kBK, kBTile = kBN / 2 * kBK, kStage = kATile + kBTile, kStages = 196608 / kStage;
+constexpr uint32_t kData = kStages * kStage + kEpiWarps * kBox;
 // What the CTA's threads share behind the stages and boxes: no static shared memory beside them, so that they begin
 // on the 1024 bytes that the swizzle asks for, with room for a little less than that.
-template <uint32_t STAGES, int MATS>
+template <int MATS>
 struct PairShared {
   float col_scale[kEpiWarps][MATS][32];
-  uint64_t bars[2 * STAGES + 4];
+  uint64_t bars[2 * kStages + 4];
   uint32_t tmem_slot, abort_flag;
 };
 constexpr uint32_t kMaxSmem = 227 * 1024;
@@ -145,35 +141,45 @@ SX_DEV T ld_shared(uint32_t src) {
 }
 
 struct Maps {
-  CUtensorMap x, w[2], y;
+  CUtensorMap x, w[2], part[2], y;  // part: the weights in boxes for a part of a tile
 };
 struct Tiles {
-  uint32_t rows, cols, all;  // tiles of rows and of columns
-  uint32_t group;            // tiles of rows that go through all columns together
-  uint32_t lanes;            // rows of y do not begin and end on 16 bytes: lanes store them
+  uint32_t rows, cols;  // tiles of rows and of columns
+  uint32_t group;       // tiles of rows that go through all columns together
+  uint32_t whole;       // tiles taken whole; those after them in 2^part parts, by columns
+  uint32_t part, units; // units: whole tiles and parts
+  uint32_t lanes;       // rows of y do not begin and end on 16 bytes: lanes store them
+};
+// What a pair takes at a time: columns [part, + 1) of 2^lg of a tile
+struct Unit {
+  uint32_t row, col, lg, part;
 };
 // Tile i: what runs at a time reads few rows of either matrix, and the rows of x of a group stay in L2 meanwhile.
-SX_DEV void tile_at(const Tiles &g, uint32_t i, uint32_t *row, uint32_t *col) {
-  const uint32_t band = i / (g.group * g.cols), in = i - band * g.group * g.cols;
+SX_DEV Unit unit_at(const Tiles &g, uint32_t i) {
+  Unit u;
+  u.lg = i < g.whole ? 0 : g.part;
+  const uint32_t tile = i < g.whole ? i : g.whole + ((i - g.whole) >> u.lg);
+  u.part = (i - g.whole) & ((1u << u.lg) - 1);
+  const uint32_t band = tile / (g.group * g.cols), in = tile - band * g.group * g.cols;
   const uint32_t high = min(g.group, g.rows - band * g.group);
-  *col = in / high;
-  *row = band * g.group + in % high;
+  u.col = in / high;
+  u.row = band * g.group + in % high;
+  return u;
 }
 
-template <typename T, bool GATED, uint32_t BN>
+template <typename T, bool GATED>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_i8_pair_kernel(const __grid_constant__ Maps maps, const __grid_constant__ I8Args a, const __grid_constant__ Tiles g) {
-  using S = PairShape<BN>;
-  constexpr uint32_t kStages = S::kStages, kCols = GATED ? BN / 2 : BN;  // columns of y
-  using Shared = PairShared<kStages, GATED ? 2 : 1>;
-  static_assert(S::kData + sizeof(Shared) <= kMaxSmem, "shared memory");
+  constexpr uint32_t kCols = GATED ? kBN / 2 : kBN;  // columns of y of a tile
+  using Shared = PairShared<GATED ? 2 : 1>;
+  static_assert(kData + sizeof(Shared) <= kMaxSmem, "shared memory");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u, skip = base - smem_u32(smem_raw);
-  if (skip + S::kData + sizeof(Shared) > kMaxSmem) {  // (alike in all CTAs: never where shared memory is laid out as it is)
+  if (skip + kData + sizeof(Shared) > kMaxSmem) {  // (alike in all CTAs: never where shared memory is laid out as it is)
     raise_error(a.err, kDevBadParams);
     return;
   }
-  Shared &sh = *reinterpret_cast<Shared *>(smem_raw + skip + S::kData);
+  Shared &sh = *reinterpret_cast<Shared *>(smem_raw + skip + kData);
   uint32_t &tmem_slot = sh.tmem_slot, &abort_flag = sh.abort_flag;
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = cluster_rank(), bar0 = smem_u32(sh.bars);
   auto full = [&](uint32_t s) { return bar0 + 8 * s; };                   // the leader's: both CTAs' copies
@@ -202,11 +208,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = tmem_slot;
   auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_try_wait(bar, parity & 1) || wait_longer(bar, parity & 1, stop, a.err); };
   const uint32_t pair = blockIdx.x / 2, pairs = gridDim.x / 2, steps = (a.k + kBK - 1) / kBK;
-  if (threadIdx.x == 0 && pair < g.all) {  // the first weights are asked into L2 while the kernel before this one ends
-    uint32_t row, col;
-    tile_at(g, pair, &row, &col);
-    for (uint32_t k = 0; k < steps && k < kStages; ++k)
-      tma_prefetch_2d(GATED && rank ? &maps.w[1] : &maps.w[0], k * kBK, GATED ? col * kCols : col * kCols + rank * (BN / 2));
+  // this CTA's first row of weights of a unit, and the copies that bring its rows
+  auto w_row = [&](const Unit &u) -> int32_t { return u.col * kCols + u.part * (kCols >> u.lg) + (GATED ? 0 : rank * (kBN / 2 >> u.lg)); };
+  auto w_map = [&](const Unit &u) { return u.lg ? &maps.part[GATED ? rank : 0] : &maps.w[GATED ? rank : 0]; };
+  if (threadIdx.x == 0 && pair < g.units) {  // the first weights are asked into L2 while the kernel before this one ends
+    const Unit u = unit_at(g, pair);
+    for (uint32_t k = 0; k < steps && k < kStages; ++k) tma_prefetch_2d(w_map(u), k * kBK, w_row(u));
   }
   __syncwarp();
   pdl_launch_dependents();
@@ -214,20 +221,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t it = 0;  // stages used, over all tiles
   if (warp == 0) {  // (the whole warp, so that addresses are the same in all lanes; one thread issues)
     const uint32_t leader_full = in_cta(full(0), 0);
-    for (uint32_t i = pair; i < g.all; i += pairs) {
-      uint32_t row, col;
-      tile_at(g, i, &row, &col);
-      const int32_t x_row = row * kBM + rank * kHalf;
-      const int32_t w_row = GATED ? col * kCols : col * kCols + rank * (BN / 2);
-      const CUtensorMap *const w = GATED && rank ? &maps.w[1] : &maps.w[0];
+    for (uint32_t i = pair; i < g.units; i += pairs) {
+      const Unit u = unit_at(g, i);
+      const int32_t x_row = u.row * kBM + rank * kHalf, w0 = w_row(u);
+      const CUtensorMap *const w = w_map(u);
+      const uint32_t bytes = 2 * (kATile + (kBTile >> u.lg));  // of both CTAs
       bool ok = true;
       for (uint32_t k = 0; k < steps; ++k, ++it) {
-        const uint32_t s = it % kStages, at = base + s * S::kStage, bar = leader_full + 8 * s;
+        const uint32_t s = it % kStages, at = base + s * kStage, bar = leader_full + 8 * s;
         if (it >= kStages && !(ok = __all_sync(0xffffffffu, wait(empty(s), it / kStages - 1)))) break;
         if (elect_one()) {
-          if (rank == 0) mbar_arrive_expect_tx(full(s), 2 * S::kStage);
+          if (rank == 0) mbar_arrive_expect_tx(full(s), bytes);
           tma_load_pair(at, &maps.x, k * kBK, x_row, bar);
-          tma_load_pair(at + S::kATile, w, k * kBK, w_row, bar);
+          tma_load_pair(at + kATile, w, k * kBK, w0, bar);
         }
         __syncwarp();
       }
@@ -236,19 +242,19 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1 && rank == 0) {
     // (the whole warp, so that descriptors are the same in all lanes; one thread issues)
     uint32_t n = 0;
-    for (uint32_t i = pair; i < g.all; i += pairs, ++n) {
-      const uint32_t d = tmem + n % 2 * kAccCols;
+    for (uint32_t i = pair; i < g.units; i += pairs, ++n) {
+      const uint32_t d = tmem + n % 2 * kBN, idesc = umma_idesc_i8(kBM, kBN >> (i < g.whole ? 0 : g.part));
       if (n >= 2 && !__all_sync(0xffffffffu, wait(sums_empty(n & 1), n / 2 - 1))) break;
       tc_fence_after();
       bool ok = true;
       for (uint32_t k = 0; k < steps; ++k, ++it) {
-        const uint32_t s = it % kStages, at = base + s * S::kStage;
+        const uint32_t s = it % kStages, at = base + s * kStage;
         if (!(ok = __all_sync(0xffffffffu, wait(full(s), it / kStages)))) break;
         tc_fence_after();
-        const uint64_t x = umma_desc_sw128(at), w = umma_desc_sw128(at + S::kATile);
+        const uint64_t x = umma_desc_sw128(at), w = umma_desc_sw128(at + kATile);
         if (elect_one()) {
 #pragma unroll
-          for (uint32_t j = 0; j < kBK / 32; ++j) umma_i8_pair(d, x + 2 * j, w + 2 * j, umma_idesc_i8(kBM, BN), k > 0 || j > 0);
+          for (uint32_t j = 0; j < kBK / 32; ++j) umma_i8_pair(d, x + 2 * j, w + 2 * j, idesc, k > 0 || j > 0);
           umma_commit_pair(empty(s));
           if (k + 1 == steps) umma_commit_pair(sums_full(n & 1));
         }
@@ -260,20 +266,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t kBoxCols = 128 / sizeof(T), kPer = kBoxCols / 32;  // columns of a box, loads of 32 of them
     constexpr uint32_t kBoxes = kCols / kBoxCols, kMine = (kBoxes + 1) / 2 * kPer;  // of a tile; of a warp, loads
     static_assert(kCols % kBoxCols == 0, "whole boxes");
-    const uint32_t q = warp & 3, odd = (warp - 2) / 4, box = base + kStages * S::kStage + (warp - 2) * kBox;
+    const uint32_t q = warp & 3, odd = (warp - 2) / 4, box = base + kStages * kStage + (warp - 2) * kBox;
     float(&cs)[GATED ? 2 : 1][32] = sh.col_scale[warp - 2];
     auto first = [&](uint32_t i) { return (odd + 2 * (i / kPer)) * kBoxCols + i % kPer * 32; };  // column of load i
     // Scales of a tile, a row's and the columns' a lane each: a tile ahead, as they come from L2.
     struct Scales {
-      uint32_t t0, n0;
+      uint32_t t0, n0, lg;
       float x, w[GATED ? 2 : 1][kMine];
     };
     auto scales_of = [&](uint32_t i, Scales &sc) {
-      if (i >= g.all) return;
-      uint32_t row, col;
-      tile_at(g, i, &row, &col);
-      sc.t0 = row * kBM + rank * kHalf + 32 * q;
-      sc.n0 = col * kCols;
+      if (i >= g.units) return;
+      const Unit u = unit_at(g, i);
+      sc.t0 = u.row * kBM + rank * kHalf + 32 * q;
+      sc.n0 = u.col * kCols + u.part * (kCols >> u.lg);
+      sc.lg = u.lg;
       sc.x = sc.t0 + lane < a.t ? a.x_scale[sc.t0 + lane] : 0.0f;
 #pragma unroll
       for (uint32_t m = 0; m < (GATED ? 2 : 1); ++m)
@@ -286,21 +292,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t n = 0;
     Scales next;
     scales_of(pair, next);
-    for (uint32_t i = pair; i < g.all; i += pairs, ++n) {
+    for (uint32_t i = pair; i < g.units; i += pairs, ++n) {
       Scales now = next;
       scales_of(i + pairs, next);
-      const uint32_t t0 = now.t0, n0 = now.n0, src = tmem + ((32 * q) << 16) + n % 2 * kAccCols;
+      const uint32_t t0 = now.t0, n0 = now.n0, src = tmem + ((32 * q) << 16) + n % 2 * kBN, cols = kCols >> now.lg;
       const float xs = now.x;
       float(&ws)[GATED ? 2 : 1][kMine] = now.w;
       const bool ok = wait(sums_full(n & 1), n / 2);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
 #pragma unroll 1
-      for (uint32_t k = 0; k < kMine && first(k) < kCols; ++k) {
+      for (uint32_t k = 0; k < kMine && first(k) < cols; ++k) {
         const uint32_t c = first(k);
         uint32_t r[32], u[GATED ? 32 : 1];
         tmem_ld32(src + c, r);
-        if constexpr (GATED) tmem_ld32(src + BN / 2 + c, u);
+        if constexpr (GATED) tmem_ld32(src + cols + c, u);
         __syncwarp();  // the scales of the columns before have been read
 #pragma unroll
         for (uint32_t m = 0; m < (GATED ? 2 : 1); ++m) {
@@ -631,68 +637,61 @@ bool encode(CUtensorMap *map, CUtensorMapDataType type, const void *p, uint64_t 
 }
 
 using PairKernel = void (*)(const Maps, const I8Args, const Tiles);
-struct PairVariant {
-  PairKernel fn;
-  uint32_t bn;
-};
-template <typename T, bool GATED>
-PairVariant pair_variant(uint32_t bn) {
-  if (bn == 128) return {gemm_i8_pair_kernel<T, GATED, 128>, 128};
-  return {gemm_i8_pair_kernel<T, GATED, 256>, 256};
+PairKernel pair_kernel(uint32_t dtype, bool gated) {
+  if (dtype == SX_F32) return gated ? gemm_i8_pair_kernel<float, true> : gemm_i8_pair_kernel<float, false>;
+  return gated ? gemm_i8_pair_kernel<__nv_bfloat16, true> : gemm_i8_pair_kernel<__nv_bfloat16, false>;
 }
-PairVariant pair_variant(uint32_t dtype, bool gated, uint32_t bn) {
-  if (dtype == SX_F32) return gated ? pair_variant<float, true>(bn) : pair_variant<float, false>(bn);
-  return gated ? pair_variant<__nv_bfloat16, true>(bn) : pair_variant<__nv_bfloat16, false>(bn);
-}
-
 
 struct PairPlan {
-  uint32_t bn;
   Tiles g;
   float us;
 };
 constexpr uint64_t kGroupBytes = 32u << 20;
 
-// Tiles of 256 columns, or of 128 where that leaves half of the pairs without one.  The time, by what was
-// measured: 5 us beside the steps of 128 of K, and those 0.30 us, 0.42 at the clock that the power cap leaves in
-// long calls; with 128 columns 4.2 and 0.27 us.  Tiles with little K wait for their values (2.7 us each), and lanes store
-// for 1 us longer.  Weights that L2 does not hold come at 5 TB/s.
-PairPlan pair_plan(uint32_t dtype, bool gated, const I8Args &a, uint32_t sms) {
-  PairPlan p{256, {}, 0.0f};
-  const uint32_t pairs = sms / 2, es = dtype == SX_F32 ? 4 : 2, steps = (a.k + kBK - 1) / kBK;
-  const uint64_t rows = (a.t + kBM - 1) / kBM;
-  auto cols = [&](uint32_t bn) -> uint64_t {
-    const uint32_t c = gated ? bn / 2 : bn;
-    return (a.n + c - 1) / c;
-  };
-  if (2 * rows * cols(256) <= pairs) p.bn = 128;
-  p.g.rows = (uint32_t)rows;
-  p.g.cols = (uint32_t)cols(p.bn);
-  p.g.all = p.g.rows * p.g.cols;
+// Tiles that are left when all pairs have had as many whole ones are taken in parts of half or a quarter of the
+// columns, so that more pairs have one (768 x 8192 x 3840 23.8 us, in halves 21.4; 1024 x 5000 x 4096 27.2, in quarters
+// 22.2).  The time, by what was measured: 5 us beside the steps of 128 of K, and those
+// 0.30 us, 0.42 at the clock that the power cap leaves in long calls, of a half 0.27.  Tiles with little K wait for
+// their values (2.7 us each), and lanes store for 1 us longer.  Weights that L2 does not hold come at 5 TB/s.
+PairPlan pair_plan(uint32_t dtype, bool gated, const I8Args &a, uint32_t pairs) {
+  PairPlan p{};
+  const uint32_t es = dtype == SX_F32 ? 4 : 2, steps = (a.k + kBK - 1) / kBK, cols = gated ? kBN / 2 : kBN;
+  p.g.rows = (a.t + kBM - 1) / kBM;
+  p.g.cols = (a.n + cols - 1) / cols;
+  const uint32_t all = p.g.rows * p.g.cols, left = all % pairs;
+  p.g.whole = all - left;
+  // (quarters only behind whole tiles: 1024 x 1024 x 1024 in halves 5.5 us, in quarters 6.7; and a box of y is 128
+  // bytes, where a quarter of a gated tile has 32 columns)
+  p.g.part = left * 4 <= pairs && p.g.whole > 0 && !(gated && es == 2) ? 2 : left * 2 <= pairs ? 1 : 0;
+  if (left == 0) p.g.part = 0;
+  p.g.units = p.g.whole + (left << p.g.part);
   // Rows of x that stay in L2 while the columns' weights go by: the more there are, the fewer times that weights which
   // do not fit L2 come from memory (118 MB of gate and up, 16896 rows of 3840: 8, 16, 32 tiles 1466, 1419, 1400 us), but
   // not past what L2 keeps (16384 rows of 15360: 696, 725, 788).
   p.g.group = (uint32_t)std::min<uint64_t>(32, std::max<uint64_t>(1, kGroupBytes / ((uint64_t)kBM * a.k)));
   // (a TMA store writes whole 16 bytes, those of a row's end too)
   p.g.lanes = ((uintptr_t)a.y | (uintptr_t)a.y_ld * es | (uintptr_t)a.n * es) % 16 != 0;
-  const uint32_t waves = (p.g.all + pairs - 1) / pairs;
   const float memory = (gated ? 2.0f : 1.0f) * (float)a.n * (float)a.k * (1.0f / 5.0e6f);
-  p.us = p.bn == 128 ? 4.2f + std::max(0.27f * steps, memory) : 5.0f + std::max(waves * std::max((waves > 2 ? 0.42f : 0.30f) * steps, 2.7f), memory);
+  const float turns = (float)(all / pairs), waves = turns + (left ? 1.0f : 0.0f);
+  const float step = waves > 2.0f ? 0.42f : 0.30f, last = left == 0 ? 0.0f : std::max((p.g.part == 2 ? 0.5f : p.g.part == 1 ? 0.65f : 1.0f) * step * steps, p.g.part ? 1.5f : 2.7f);
+  p.us = (turns > 0.0f || p.g.part == 0 ? 5.0f : 4.2f) + std::max(turns * std::max(step * steps, 2.7f) + last, memory);
   if (p.g.lanes) p.us += waves * 1.0f;
   return p;
 }
 
-cudaError_t launch_pair(uint32_t dtype, bool gated, const I8Args &a, const PairPlan &p, uint32_t sms, cudaStream_t s) {
-  const PairVariant v = pair_variant(dtype, gated, p.bn);
+cudaError_t launch_pair(uint32_t dtype, bool gated, const I8Args &a, const PairPlan &p, uint32_t pairs, cudaStream_t s) {
   const uint32_t es = dtype == SX_F32 ? 4 : 2;
   Maps maps{};
   bool ok = encode(&maps.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, a.k, a.t, a.x_ld, kBK, kHalf);
-  for (int i = 0; i < (gated ? 2 : 1); ++i) ok = ok && encode(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, v.bn / 2);
+  for (int i = 0; i < (gated ? 2 : 1); ++i) {
+    if (p.g.whole || !p.g.part) ok = ok && encode(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, kBN / 2);
+    if (p.g.part) ok = ok && encode(&maps.part[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, kBN / 2 >> p.g.part);
+  }
   if (!p.g.lanes)
     ok = ok && encode(&maps.y, dtype == SX_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.n, a.t,
                       (uint64_t)a.y_ld * es, 128 / es, 32);
   if (!ok) return cudaErrorInvalidValue;
-  return launch_chained(v.fn, dim3(2 * std::min(p.g.all, sms / 2)), dim3(kThreads), kMaxSmem, s, 2, maps, a, p.g);
+  return launch_chained(pair_kernel(dtype, gated), dim3(2 * std::min(p.g.units, pairs)), dim3(kThreads), kMaxSmem, s, 2, maps, a, p.g);
 }
 
 using SplitKernel = void (*)(const Maps, const I8Args, const SplitShape);
@@ -746,11 +745,11 @@ cudaError_t launch_split(uint32_t dtype, bool gated, const I8Args &a, const Spli
 }
 
 // Few rows or few tiles: weights as the rows of the products; else tiles of pairs.
-cudaError_t launch_tiles(uint32_t dtype, bool gated, const I8Args &a, int num_sms, const uint32_t (&clusters)[4], cudaStream_t s) {
-  const PairPlan pair = pair_plan(dtype, gated, a, num_sms);
+cudaError_t launch_tiles(uint32_t dtype, bool gated, const I8Args &a, const uint32_t (&clusters)[4], cudaStream_t s) {
+  const PairPlan pair = pair_plan(dtype, gated, a, clusters[1]);
   const SplitPlan split = split_plan(gated, a, clusters);
   if (split.t_tiles <= 65535 && split.us < pair.us) return launch_split(dtype, gated, a, split, s);
-  return launch_pair(dtype, gated, a, pair, num_sms, s);
+  return launch_pair(dtype, gated, a, pair, clusters[1], s);
 }
 
 }  // namespace
@@ -775,15 +774,13 @@ cudaError_t prepare_gemm_i8(uint32_t (&clusters)[4]) {
     int n = 0;
     const cudaError_t e = cudaOccupancyMaxActiveClusters(&n, split_kernel(SX_F32, false), &cfg);
     if (e != cudaSuccess) return e;
-    if (n > 0) clusters[i] = (uint32_t)n;
+    clusters[i] = (uint32_t)std::max(n, 1);
   }
   for (uint32_t dtype : {SX_F32, SX_BF16})
-    for (bool gated : {false, true})
-      for (uint32_t bn : {128u, 256u}) {
-        const PairVariant v = pair_variant(dtype, gated, bn);
-        const cudaError_t e = cudaFuncSetAttribute(v.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
-        if (e != cudaSuccess) return e;
-      }
+    for (bool gated : {false, true}) {
+      const cudaError_t e = cudaFuncSetAttribute(pair_kernel(dtype, gated), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
+      if (e != cudaSuccess) return e;
+    }
   return prepare_gemv_i8();
 }
 
@@ -821,7 +818,7 @@ sx_status dispatch_i8(const char *what, sx_engine *e, uint32_t dtype, sx::I8Args
   // tiles 8.1; 16 rows 11.9, 8.0; 32768 x 4096: 1 row 22.7 us).
   const bool stream = a.t <= sx::kI8GemvRows && (a.k > 2048 || a.n <= (gated ? 48u : 96u) * (uint32_t)e->num_sms);
   return sx_host_cuda_status(stream ? sx::launch_gemv_i8(dtype, gated, a, e->num_sms, e->stream)
-                                                     : sx::launch_tiles(dtype, gated, a, e->num_sms, e->i8_clusters, e->stream), what);
+                                                     : sx::launch_tiles(dtype, gated, a, e->i8_clusters, e->stream), what);
 }
 
 }  // namespace
