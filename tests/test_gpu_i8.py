@@ -116,6 +116,47 @@ def test_every_small_number_of_rows(eng, t):
     check_gate_up(eng, t, 207, 720, torch.bfloat16, seed=t)
 
 
+# more tiles than run at a time, with few, some and many left over; many groups of rows; many short rows of weights
+MANY = [(2560, 2048, 64), (2600, 2400, 208), (9000, 600, 64), (5000, 4100, 96), (300, 40000, 80), (8, 33000, 528), (16, 30000, 272),
+        (20, 33000, 144), (17000, 64, 64), (1, 70000, 32), (130, 20000, 400), (33000, 40, 48), (1100, 5000, 2064), (700, 900, 131056)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("t,n,k", MANY)
+def test_many_tiles(eng, t, n, k, dtype):
+    check_gemm(eng, t, n, k, dtype, seed=t)
+    if k < 10000:
+        check_gate_up(eng, t, (n + 1) // 2, k, dtype, seed=t)
+
+
+@pytest.mark.parametrize("t,ld", [(3, 1 << 31), (40, 1 << 27), (300, 1 << 24)])
+def test_offsets_past_32_bits(eng, t, ld):
+    """Rows of x and y that lie further apart than 32 bits reach."""
+    n, k, x_ld = 200, 144, ld + 16
+    (x, xs), (w, ws), (wu, us) = operands(t, n, k, 8, gated=True)
+    far = torch.empty(t * x_ld, dtype=torch.int8, device="cuda").view(t, x_ld)
+    far[:, :k] = x
+    want, got = torch.empty(t, n, dtype=torch.bfloat16, device="cuda"), torch.empty(t * (ld + 8), dtype=torch.bfloat16, device="cuda").view(t, ld + 8)
+    eng.gemm_i8(x, xs, w, ws, sx.DTYPE_BF16, want, t, n, k)
+    eng.gemm_i8(far, xs, w, ws, sx.DTYPE_BF16, got, t, n, k, x_ld=x_ld, y_ld=ld + 8)
+    eng.sync()
+    assert torch.equal(got[:, :n], want)
+    eng.gate_up_i8(x, xs, w, ws, wu, us, sx.DTYPE_BF16, want, t, n, k)
+    eng.gate_up_i8(far, xs, w, ws, wu, us, sx.DTYPE_BF16, got, t, n, k, x_ld=x_ld, y_ld=ld + 8)
+    eng.sync()
+    assert torch.equal(got[:, :n], want)
+    del got
+    # weights
+    far_w = far if t <= n else far[:n]
+    rows = far_w.shape[0]
+    far_w[:, :k] = w[:rows]
+    want, got = torch.empty(t, rows, device="cuda"), torch.empty(t, rows, device="cuda")
+    eng.gemm_i8(x, xs, w, ws, sx.DTYPE_F32, want, t, rows, k)
+    eng.gemm_i8(x, xs, far_w, ws, sx.DTYPE_F32, got, t, rows, k, w_ld=x_ld)
+    eng.sync()
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("t,n,k", [(1, 100, 144), (6, 333, 1040), (40, 130, 272), (300, 200, 400), (700, 601, 144)])
 def test_strides(eng, t, n, k, dtype):
@@ -223,6 +264,22 @@ def test_quantize_sizes(eng, n, norm, dtype):
     rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
     for rows in (1, 5, 130 if n < 20000 else 3):
         check_quantize(eng, (rand(rows, n) * rand(rows, 1).exp()).to(dtype), 1 + 0.2 * rand(n) if norm else None)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", [(297, 16), (299, 256), (1001, 272), (333, 512), (301, 784), (303, 1024), (305, 1040), (307, 2048), (309, 2064), (5001, 1552),
+                                    (5003, 3840), (311, 8192), (313, 8208), (315, 16400)])
+def test_many_rows(eng, rows, n, dtype):
+    """Rows as warps and as CTAs, with every number of elements a thread."""
+    g = gen(rows)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    x = (rand(rows, n) * rand(rows, 1).exp()).to(dtype)
+    x[5], x[7, 3], x[9, n - 1], x[11] = 0, math.nan, math.inf, 1
+    check_quantize(eng, x)
+    check_quantize(eng, x, 1 + 0.2 * rand(n))
+    x[[7, 9]] = 0
+    for y_type in (torch.float32, torch.bfloat16, torch.int8, None):
+        check_norm(eng, rand(rows, n), x, 1 + 0.2 * rand(n), 1 + 0.2 * rand(n), 0.5, y_type)
 
 
 def test_quantize_many_rows_and_strides(eng):
@@ -334,6 +391,29 @@ def test_norm_special_rows(eng, n, y_type):
     r[4] = 0
     x[5, n // 2] = 1e5
     check_norm(eng, x, r, torch.ones(n, device="cuda"), torch.ones(n, device="cuda"), 1.0, y_type)
+
+
+@pytest.mark.parametrize("rows,ld", [(3, 1 << 31), (700, 1 << 23)])
+def test_rows_past_32_bits(eng, rows, ld):
+    n = 96
+    g = gen(rows)
+    x = torch.randn(rows, n, device="cuda", generator=g).bfloat16()
+    w = 1 + 0.1 * torch.randn(n, device="cuda", generator=g)
+    far = torch.empty(rows * (ld + 8), dtype=torch.bfloat16, device="cuda").view(rows, ld + 8)
+    far[:, :n] = x
+    q, qf = torch.empty(rows, n, dtype=torch.int8, device="cuda"), torch.empty(rows * (ld + 16), dtype=torch.int8, device="cuda").view(rows, ld + 16)
+    s, sf = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    eng.quantize_i8(sx.DTYPE_BF16, x, q, s, rows, n, norm_w=w)
+    eng.quantize_i8(sx.DTYPE_BF16, far, qf, sf, rows, n, norm_w=w, x_ld=ld + 8, q_ld=ld + 16)
+    eng.sync()
+    assert torch.equal(qf[:, :n], q) and torch.equal(s, sf)
+    xr = torch.randn(rows, n, device="cuda", generator=g)
+    out, y, yf = torch.empty(rows, n, device="cuda"), torch.empty(rows, n, dtype=torch.bfloat16, device="cuda"), far
+    eng.residual_norm(xr, sx.DTYPE_BF16, x, out, sx.DTYPE_BF16, y, rows, n, post_w=w, pre_w=w)
+    first = out.clone()
+    eng.residual_norm(xr, sx.DTYPE_BF16, x, out, sx.DTYPE_BF16, yf, rows, n, post_w=w, pre_w=w, y_ld=ld + 8)
+    eng.sync()
+    assert torch.equal(yf[:, :n], y) and torch.equal(out, first)
 
 
 # ---------------------------------------------------------------------- streams, graphs, a whole block
