@@ -1,15 +1,30 @@
 // sx_i8_gemm.cu -- products of int8 rows on the tcgen05 tensor cores (include/sx.h, sx_dispatch_gemm_i8 and
 // sx_dispatch_gate_up_i8).
 //
-// Two CTAs of a cluster take a tile of 256 rows of x and 256 columns of y (gate_up: 128 of each matrix), 128
-// rows in the tensor memory of each: tcgen05.mma of the pair (kind::i8, 32-bit sums) reads 128 rows of x and half
-// of the columns' weights from each CTA's shared memory, so both operands are fetched once per pair.  The grid is
-// one pair per two SMs, which goes through the tiles; tensor memory holds two tiles' sums, so that one is
-// scaled and stored while the next is summed.  Warps of a CTA:
-//   0       TMA: 128 codes of K a stage, completing on the leader's barrier
+//   y[t][n] = x_scale[t] w_scale[n] sum_k x[t][k] w[n][k]        gate_up: gelu_tanh(y_gate) y_up
+//
+// Sums are whole numbers below 2^31 in 32 bits: no order of summation, split of K or kernel changes them, and a
+// value is rounded three times in f32 (the sum, two scales), then to y's type.
+//
+// Many rows: tiles.  Two CTAs of a cluster take a tile of 256 rows of x and 256 columns of y (gate_up: 128 of each
+// matrix), 128 rows in the tensor memory of each: tcgen05.mma of the pair (kind::i8) reads 128 rows of x and half of
+// the columns' weights from each CTA's shared memory, so both operands are fetched once per pair.  The grid is one
+// pair per two SMs, which goes through the tiles; tensor memory holds two tiles' sums, so that one is scaled and
+// stored while the next is summed.  Warps of a CTA:
+//   0       TMA: 128 codes of K a stage, six stages, completing on the leader's barrier
 //   1       the leader's issues the products and commits stages and sums to both CTAs
-//   2 .. 9  sums to values, 32 rows each and every other box of columns, staged in shared memory and stored by TMA (rows of y that do not
-//           begin and end on 16 bytes: by lanes)
+//   2 .. 9  sums to values, 32 rows each and every other box of columns, staged in shared memory and stored by TMA
+//           (rows of y that do not begin and end on 16 bytes: by lanes)
+// Measured: 16896 x 8192 x 3840 into f32 411 us (box to box up to 433), 2.6 POP/s or 159 % of the measured bf16
+// rate; gate and up of 16896 x 15360 x 3840 1323 us, 3.0 POP/s, 184 %.  What bounds it is the power cap: the clock
+// falls to 1.3 GHz, and bringing tiles from L2 takes nearly as much power as the products.  (Zeros as data leave it
+// at 1.97 GHz, and the same call takes 252 us; products without copies 271, copies without products 243; no stores
+// 351 of 433, stores that stay in L2 395.)  So tiles that read less for a product were tried: 256 x 512 with one set
+// of sums ran at 1.5 GHz and took 391 us for 365, since four stages of 48 KB are too few; 256 x 128 takes 456 for
+// 369.  A thread that issues by itself costs the products of 128 columns a third (516 us for 343, without copies):
+// what is alike in a warp has to be known to be so.
+//
+// Few rows of x, or few tiles: see below.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -411,7 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---- few rows of x, or few tiles: weights as the rows of the products
 // 128 columns of y (rows of weights) are the M of the product and up to 256 rows of x its N, so that no row of the
 // tensor memory is spent on rows of x that are not there; the CTAs of a cluster share a tile, each with a part of
-// K, and each then adds up what all of them have of every so-manieth row of x (whole numbers, in any order).
+// K, and each then adds up what all of them have of every so-manieth row of x: whole numbers, so the order does not
+// matter and no memory but theirs is needed.  It reads the rows of x once for 128 columns, which bounds it from some
+// 100 rows on: 17 rows of 3840 x 15360 13.5 us (4.4 TB/s of weights), 128 rows 16, 256 rows 21, where copies from L2
+// run at 110 KB a us and SM; what starting and ending costs is 3.3 us of each.  Tiles half as deep in shared
+// memory, so that the next call's CTAs find room beside these, took 14.6, 21.5 and 29.8.
 constexpr uint32_t kWRows = 128, kWTile = kWRows * kBK;
 struct SplitShape {
   uint32_t tok;        // rows of x of a tile: a multiple of 16

@@ -7,6 +7,14 @@
 // matrix); its warps take pieces of 64 bytes of K in turn, each through a ring of its own that every lane fills
 // and reads back alone, and their sums meet in shared memory.  Where the rows alone are too few CTAs, those of
 // a cluster share them, each with a part of K.
+//
+// Measured, bound by HBM: 262144 rows of 3840 143 us (7.0 TB/s, 107 % of the measured copy rate); gate and up of one
+// token (118 MB) 20.6 us (5.7 TB/s), 8 tokens 21.3; the down projection of one token (59 MB) 11.6 us (5.1 TB/s), 8
+// tokens 12.6, 16 14.5; 3 us of each are the launch, the first bytes, the cluster's and the CTA's sums.  Three CTAs an
+// SM with three pieces each on their way against two with four: 20.5 and 22.9 us for gate and up, but 13.9 and 11.9
+// for the down projection, whose 240 CTAs all run at once.  Rows of x that are not there are not copied: eight lanes
+// asking for the same bytes of the one row took 14.9 us for 11.9.  All of a CTA's weights asked into L2 at its start
+// took longer (26.9 us for 22.9): they queue ahead of what is needed first.
 #include "sx_host.h"
 #include "sx_i8.cuh"
 #include "sx_launch.cuh"

@@ -1,9 +1,16 @@
 // sx_i8_rows.cu -- rows to int8 codes, and the norms and residual between two blocks (include/sx.h,
 // sx_dispatch_quantize_i8 and sx_dispatch_residual_norm).
 //
-// A row is read once: each thread holds groups of 8 elements, the row's maximum and sum of squares meet
-// in shared memory, and what is written comes from registers.  A code is u * (127 / max|u|) with u = x * w,
-// which has no sum in it, so codes do not depend on how a row is split over threads.
+// A row is read once: each thread holds groups of 8 elements as they came, the row's maximum and sum of squares meet
+// in shared memory (or in the row's warp), and what is written comes from registers.  A code is u * (127 / max|u|)
+// with u = x * w, which has no sum in it, so codes do not depend on how a row is split over threads.  A NaN or an
+// infinity is found in the maximum itself, whose bits are above all others'.
+//
+// Measured, bound by HBM: seam of 16896 rows of 3840 (f32 stream, bf16 in and out) 130 us, 7.0 TB/s or 107 % of the
+// measured copy rate; codes of 2697 x 15360 bf16 26.5 us (4.7 TB/s, 72 %), of 16896 x 3840 36 (5.4 TB/s), of f32 with a
+// gain 58.6 (5.5): CTAs start, wait for a row and end, and two in three bytes are read.  CTAs that go through rows
+// with the next one on its way were slower (45 us for 39, f32 89 for 59: registers), as were a warp for rows of
+// 3840 (45) and more elements a thread.  One row of 3840 takes 1.5 us, with both norms 2.6.
 #include "sx_host.h"
 #include "sx_i8.cuh"
 #include "sx_kv8.cuh"
