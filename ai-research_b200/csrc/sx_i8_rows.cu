@@ -7,10 +7,10 @@
 // infinity is found in the maximum itself, whose bits are above all others'.
 //
 // Measured, bound by HBM: seam of 16896 rows of 3840 (f32 stream, bf16 in and out) 130 us, 7.0 TB/s or 107 % of the
-// measured copy rate; codes of 2697 x 15360 bf16 26.5 us (4.7 TB/s, 72 %), of 16896 x 3840 36 (5.4 TB/s), of f32 with a
-// gain 58.6 (5.5): CTAs start, wait for a row and end, and two in three bytes are read.  CTAs that go through rows
-// with the next one on its way were slower (45 us for 39, f32 89 for 59: registers), as were a warp for rows of
-// 3840 (45) and more elements a thread.  One row of 3840 takes 1.5 us, with both norms 2.6.
+// measured copy rate; codes of 2697 x 15360 bf16 22.3 us (5.6 TB/s, 85 %), of 16896 x 3840 32 (6.1 TB/s), of f32 with a
+// gain 58.6 (5.5): instructions and starts of CTAs count beside the bytes (bf16 magnitudes one at a time took 26.2 and
+// 36 us, codes by conversions 27 and 39).  CTAs that go through rows with the next one on its way were slower (45 us
+// for 39, f32 89 for 59: registers), as were a warp for rows of 3840 (45) and more elements a thread.  One row of 3840 takes 1.5 us, with both norms 2.6.
 #include "sx_host.h"
 #include "sx_i8.cuh"
 #include "sx_kv8.cuh"
@@ -100,6 +100,13 @@ SX_DEV float top_of(float top, float x) {
   return r;
 }
 
+// the larger magnitudes of two bf16s, each of a place
+SX_DEV void top_bits(uint32_t &pair, const uint4 &v) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) asm("max.u16x2 %0, %0, %1;\n" : "+r"(pair) : "r"(w[i] & 0x7FFF7FFFu));
+}
+
 // The largest `top` and the sum of `sum` over the CTA.
 struct RowRed {
   uint32_t top[32];
@@ -144,8 +151,9 @@ SX_DEV float code_factor(uint32_t top, float sq_sum, float inv, bool norm, float
 }
 
 // G: groups of 8 elements that a thread holds; 0: rows too long for registers are read again (from L2).
+// (bf16 rows with four groups a thread: 32 registers, for all threads that an SM takes)
 template <typename T, bool WARP, uint32_t G>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads) quantize_i8_kernel(const __grid_constant__ RowsArgs a) {
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, !WARP && sizeof(T) == 2 && G == 4 ? 2 : 1) quantize_i8_kernel(const __grid_constant__ RowsArgs a) {
   __shared__ RowRed red;
   pdl_launch_dependents();
   pdl_wait();
@@ -176,12 +184,20 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads) quantize_
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
       if (d0 + g * step < a.n) load_raw(in + d0 + g * step, held[g]);
+    if (sizeof(T) == 2 && !a.w) {  // two at a time: the order of bf16's bits is the values' too
+      uint32_t pair = 0;
 #pragma unroll
-    for (uint32_t g = 0; g < G; ++g)
-      if (d0 + g * step < a.n) {
-        unpack8(held[g], u);
-        measure(d0 + g * step);
-      }
+      for (uint32_t g = 0; g < G; ++g)
+        if (d0 + g * step < a.n) top_bits(pair, held[g].v[0]);
+      top = __uint_as_float(max(pair << 16, pair & 0xFFFF0000u));
+    } else {
+#pragma unroll
+      for (uint32_t g = 0; g < G; ++g)
+        if (d0 + g * step < a.n) {
+          unpack8(held[g], u);
+          measure(d0 + g * step);
+        }
+    }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
       load8(in + d, u);
