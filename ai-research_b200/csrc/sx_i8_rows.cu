@@ -7,9 +7,9 @@
 // infinity is found in the maximum itself, whose bits are above all others'.
 //
 // Measured, bound by HBM: seam of 16896 rows of 3840 (f32 stream, bf16 in and out) 130 us, 7.0 TB/s or 107 % of the
-// measured copy rate; codes of 2697 x 15360 bf16 22.3 us (5.6 TB/s, 85 %), of 16896 x 3840 32 (6.1 TB/s), of f32 with a
-// gain 58.6 (5.5): instructions and starts of CTAs count beside the bytes (bf16 magnitudes one at a time took 26.2 and
-// 36 us, codes by conversions 27 and 39).  CTAs that go through rows with the next one on its way were slower (45 us
+// measured copy rate; codes of 2697 x 15360 bf16 20 us (6.2 TB/s, 95 %), of 16896 x 3840 29 (6.7 TB/s), of f32 with a
+// gain 51.6 (6.3): instructions and L1 count beside the bytes (bf16 magnitudes one at a time took 26.2 and 36 us, codes
+// by conversions 27 and 39; gains read again for the codes 58.6).  CTAs that go through rows with the next one on its way were slower (45 us
 // for 39, f32 89 for 59: registers), as were a warp for rows of 3840 (45) and more elements a thread.  One row of 3840 takes 1.5 us, with both norms 2.6.
 #include "sx_host.h"
 #include "sx_i8.cuh"
@@ -150,10 +150,11 @@ SX_DEV float code_factor(uint32_t top, float sq_sum, float inv, bool norm, float
   return a >= kTiny ? 127.0f / a : 0.0f;
 }
 
-// G: groups of 8 elements that a thread holds; 0: rows too long for registers are read again (from L2).
-// (bf16 rows with four groups a thread: 32 registers, for all threads that an SM takes)
-template <typename T, bool WARP, uint32_t G>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, !WARP && sizeof(T) == 2 && G == 4 ? 2 : 1) quantize_i8_kernel(const __grid_constant__ RowsArgs a) {
+// G: groups of 8 elements that a thread holds, as they came or with their GAIN; 0: rows too long for registers are
+// read again (from L2).
+template <typename T, bool GAIN, bool WARP, uint32_t G>
+__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
+    quantize_i8_kernel(const __grid_constant__ RowsArgs a) {
   __shared__ RowRed red;
   pdl_launch_dependents();
   pdl_wait();
@@ -162,67 +163,65 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads, !WARP && 
   const uint32_t d0 = p.d0, step = p.step;
   const T *const in = static_cast<const T *>(a.in) + p.row * a.in_ld;
   int8_t *const q = static_cast<int8_t *>(a.y) + p.row * a.y_ld;
-  float top = 0.0f, sum = 0.0f, u[8];
-  // u of a group, from x there
-  auto gained = [&](uint32_t d) {
-    if (!a.w) return;
-    float w[8];
-    load8(a.w + d, w);
+  constexpr uint32_t kHeld = G ? G : 1;
+  Raw8<T> raw[kHeld];
+  float u[GAIN ? kHeld : 1][8], top = 0.0f, sum = 0.0f;
+  // the group at d, from x in v: with its gain, and counted
+  auto measure = [&](uint32_t d, float (&v)[8]) {
+    if constexpr (GAIN) {
+      float w[8];
+      load8(a.w + d, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = __fmul_rn(u[i], w[i]);
+      for (int i = 0; i < 8; ++i) {
+        sum = fmaf(v[i], v[i], sum);
+        v[i] = __fmul_rn(v[i], w[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = top_of(top, v[i]);
   };
-  auto measure = [&](uint32_t d) {
-    if (a.w)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(u[i], u[i], sum);
-    gained(d);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = top_of(top, u[i]);
-  };
-  Raw8<T> held[G ? G : 1];
   if constexpr (G > 0) {
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
-      if (d0 + g * step < a.n) load_raw(in + d0 + g * step, held[g]);
-    if (sizeof(T) == 2 && !a.w) {  // two at a time: the order of bf16's bits is the values' too
+      if (d0 + g * step < a.n) load_raw(in + d0 + g * step, raw[g]);
+    if constexpr (sizeof(T) == 2 && !GAIN) {  // two at a time: the order of bf16's bits is the values' too
       uint32_t pair = 0;
 #pragma unroll
       for (uint32_t g = 0; g < G; ++g)
-        if (d0 + g * step < a.n) top_bits(pair, held[g].v[0]);
+        if (d0 + g * step < a.n) top_bits(pair, raw[g].v[0]);
       top = __uint_as_float(max(pair << 16, pair & 0xFFFF0000u));
     } else {
 #pragma unroll
       for (uint32_t g = 0; g < G; ++g)
         if (d0 + g * step < a.n) {
-          unpack8(held[g], u);
-          measure(d0 + g * step);
+          unpack8(raw[g], u[GAIN ? g : 0]);
+          measure(d0 + g * step, u[GAIN ? g : 0]);
         }
     }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
-      load8(in + d, u);
-      measure(d);
+      load8(in + d, u[0]);
+      measure(d, u[0]);
     }
   }
   uint32_t bits = __float_as_uint(top) & 0x7FFFFFFFu;  // (their order is the values', with infinity and NaN on top)
   row_reduce<WARP>(red, bits, sum);
   float scale;
-  const float inv = a.w ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : 1.0f;
-  const float mul = code_factor(bits, sum, inv, a.w != nullptr, &scale);
+  const float inv = GAIN ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : 1.0f;
+  const float mul = code_factor(bits, sum, inv, GAIN, &scale);
   if (d0 == 0) a.scale[p.row] = scale;
   if constexpr (G > 0) {
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
       if (d0 + g * step < a.n) {
-        unpack8(held[g], u);
-        gained(d0 + g * step);
-        store_codes(q + d0 + g * step, u, mul);
+        if constexpr (!GAIN) unpack8(raw[g], u[0]);
+        store_codes(q + d0 + g * step, u[GAIN ? g : 0], mul);
       }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
-      load8(in + d, u);
-      gained(d);
-      store_codes(q + d, u, mul);
+      load8(in + d, u[0]);
+      measure(d, u[0]);
+      store_codes(q + d, u[0], mul);
     }
   }
 }
@@ -378,15 +377,19 @@ RowsPlan rows_plan(uint32_t n, uint32_t rows, uint32_t warp_most, uint32_t most,
 }
 
 using RowsKernel = void (*)(const RowsArgs);
-template <typename T>
+template <typename T, bool GAIN>
 RowsKernel quantize_kernel(const RowsPlan &p) {
   if (p.warp) {
-    if constexpr (sizeof(T) == 2)
-      if (p.g == 8) return quantize_i8_kernel<T, true, 8>;
-    return p.g == 1 ? quantize_i8_kernel<T, true, 1> : p.g == 2 ? quantize_i8_kernel<T, true, 2> : quantize_i8_kernel<T, true, 4>;
+    if constexpr (sizeof(T) == 2 && !GAIN)
+      if (p.g == 8) return quantize_i8_kernel<T, GAIN, true, 8>;
+    return p.g == 1 ? quantize_i8_kernel<T, GAIN, true, 1> : p.g == 2 ? quantize_i8_kernel<T, GAIN, true, 2> : quantize_i8_kernel<T, GAIN, true, 4>;
   }
-  return p.g == 0 ? quantize_i8_kernel<T, false, 0> : p.g == 1 ? quantize_i8_kernel<T, false, 1>
-       : p.g == 2 ? quantize_i8_kernel<T, false, 2> : quantize_i8_kernel<T, false, 4>;
+  return p.g == 0 ? quantize_i8_kernel<T, GAIN, false, 0> : p.g == 1 ? quantize_i8_kernel<T, GAIN, false, 1>
+       : p.g == 2 ? quantize_i8_kernel<T, GAIN, false, 2> : quantize_i8_kernel<T, GAIN, false, 4>;
+}
+template <typename T>
+RowsKernel quantize_kernel(const RowsPlan &p, bool gain) {
+  return gain ? quantize_kernel<T, true>(p) : quantize_kernel<T, false>(p);
 }
 template <typename T, RowOut OUT>
 RowsKernel residual_kernel(const RowsPlan &p) {
@@ -439,8 +442,8 @@ SX_API sx_status sx_dispatch_quantize_i8(sx_engine *e, const sx_quantize_i8_args
   r.rows = a->rows;
   r.n = a->n;
   r.eps = a->eps;
-  const sx::RowsPlan p = sx::rows_plan(a->n, a->rows, a->dtype == SX_F32 ? 4 : 8, 4, e->num_sms);
-  const sx::RowsKernel k = a->dtype == SX_F32 ? sx::quantize_kernel<float>(p) : sx::quantize_kernel<__nv_bfloat16>(p);
+  const sx::RowsPlan p = sx::rows_plan(a->n, a->rows, a->dtype == SX_F32 || a->norm_w ? 4 : 8, 4, e->num_sms);
+  const sx::RowsKernel k = a->dtype == SX_F32 ? sx::quantize_kernel<float>(p, a->norm_w) : sx::quantize_kernel<__nv_bfloat16>(p, a->norm_w);
   return sx_host_cuda_status(sx::launch_chained(k, dim3(p.ctas), dim3(p.threads), 0, e->stream, 1, r),
       "quantize_i8 launch");
 }
