@@ -14,7 +14,7 @@
 //   0       TMA: 128 codes of K a stage, six stages, completing on the leader's barrier
 //   1       the leader's issues the products and commits stages and sums to both CTAs
 //   2 .. 9  sums to values, 32 rows each and every other box of columns, staged in shared memory and stored by TMA
-//           (rows of y that do not begin and end on 16 bytes: by lanes)
+//           (rows of y that do not begin on 16 bytes, and ends of rows inside them: by lanes)
 // Measured: 16896 x 8192 x 3840 into f32 411 us (box to box up to 433), 2.6 POP/s or 159 % of the measured bf16
 // rate; gate and up of 16896 x 15360 x 3840 1323 us, 3.0 POP/s, 184 %.  What bounds it is the power cap: the clock
 // falls to 1.3 GHz, and bringing tiles from L2 takes nearly as much power as the products.  (Zeros as data leave it
@@ -79,8 +79,10 @@ SX_DEV uint32_t in_cta(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
+// Nothing in memory is handed over by it, only sums that have been read: a release would wait for the lanes' stores to
+// y too (8192 x 8191 x 512 into bf16 76 us, so 55; gate and up of it into f32 143, 110).
 SX_DEV void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar) : "memory");
 }
 // 2-D tiled load into this CTA's shared memory that completes on a barrier of either CTA of the pair
 SX_DEV void tma_load_pair(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
@@ -170,7 +172,7 @@ struct Tiles {
   uint32_t group;       // tiles of rows that go through all columns together
   uint32_t whole;       // tiles taken whole; those after them in 2^part parts, by columns
   uint32_t part, units; // units: whole tiles and parts
-  uint32_t lanes;       // rows of y do not begin and end on 16 bytes: lanes store them
+  uint32_t boxes;       // boxes of y that end before this column are stored by copies, the others by lanes
   uint32_t far;         // y is more than L2 holds: its lines leave L2 before those of x and the weights
 };
 // What a pair takes at a time: columns [part, + 1) of 2^lg of a tile
@@ -325,6 +327,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool ok = wait(sums_full(n & 1), n / 2);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
+      auto drained = [&] {  // this warp has read its sums
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(in_cta(sums_empty(n & 1), 0));
+      };
+      if (first(0) >= cols) drained();
 #pragma unroll 1
       for (uint32_t k = 0; k < kMine && first(k) < cols; ++k) {
         const uint32_t c = first(k);
@@ -343,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         tmem_wait_ld(r);
         if constexpr (GATED) tmem_wait_ld(u);
+        if (k + 1 == kMine || first(k + 1) >= cols) drained();
         float v[32];
 #pragma unroll
         for (uint32_t j = 0; j < 32; j += 2) {
@@ -371,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (half + 1 < kPer) continue;
         const uint32_t c0 = n0 + c - half * 32;
-        if (!g.lanes) {
+        if (c0 + kBoxCols <= g.boxes) {
           fence_proxy_async();  // generic-proxy writes -> the TMA engine's reads
           __syncwarp();
           if (lane == 0 && c0 < a.n && t0 < a.t) {
@@ -404,9 +413,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(in_cta(sums_empty(n & 1), 0));
     }
     if (lane == 0) bulk_wait_all();
     __syncwarp();
@@ -700,15 +706,18 @@ PairPlan pair_plan(uint32_t dtype, bool gated, const I8Args &a, uint32_t pairs) 
   // do not fit L2 come from memory (118 MB of gate and up, 16896 rows of 3840: 8, 16, 32 tiles 1466, 1419, 1400 us), but
   // not past what L2 keeps (16384 rows of 15360: 696, 725, 788).
   p.g.group = (uint32_t)std::min<uint64_t>(32, std::max<uint64_t>(1, kGroupBytes / ((uint64_t)kBM * a.k)));
-  // (a TMA store writes whole 16 bytes, those of a row's end too)
-  p.g.lanes = ((uintptr_t)a.y | (uintptr_t)a.y_ld * es | (uintptr_t)a.n * es) % 16 != 0;
+  // Copies store rows that begin on 16 bytes, and of those whole 16 bytes: where a row ends inside them, its last box
+  // is left to lanes (8192 x 8191 x 512, rows 8192 apart: f32 67 -> 60 us, bf16 54 -> 36).  Rows that begin anywhere are
+  // the lanes' (8191 apart: 95 and 55 us).  Their stores cut sectors in two; shifted by rows into whole lines, through
+  // registers that keep what is left of a box, they take twelve instructions a row and box for four, and 135 us.
+  p.g.boxes = ((uintptr_t)a.y | (uintptr_t)a.y_ld * es) % 16 != 0 ? 0 : (uint64_t)a.n * es % 16 != 0 ? a.n : ~0u;
   // (16896 x 8192 of f32: 438 -> 433 us; 8192 x 8192 x 512 72.6 -> 69)
   p.g.far = (uint64_t)a.t * a.n * es > (128u << 20);
   const float memory = (gated ? 2.0f : 1.0f) * (float)a.n * (float)a.k * (1.0f / 5.0e6f);
   const float turns = (float)(all / pairs), waves = turns + (left ? 1.0f : 0.0f);
   const float step = waves > 2.0f ? 0.42f : 0.30f, last = left == 0 ? 0.0f : std::max((p.g.part == 2 ? 0.5f : p.g.part == 1 ? 0.65f : 1.0f) * step * steps, p.g.part ? 1.5f : 2.7f);
   p.us = (turns > 0.0f || p.g.part == 0 ? 5.0f : 4.2f) + std::max(turns * std::max(step * steps, 2.7f) + last, memory);
-  if (p.g.lanes) p.us += waves * 1.0f;
+  if (p.g.boxes == 0) p.us += waves * 1.0f;
   return p;
 }
 
@@ -720,7 +729,7 @@ cudaError_t launch_pair(uint32_t dtype, bool gated, const I8Args &a, const PairP
     if (p.g.whole || !p.g.part) ok = ok && encode(&maps.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, kBN / 2);
     if (p.g.part) ok = ok && encode(&maps.part[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, a.w[i], a.k, a.n, a.w_ld, kBK, kBN / 2 >> p.g.part);
   }
-  if (!p.g.lanes)
+  if (p.g.boxes != 0)
     ok = ok && encode(&maps.y, dtype == SX_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.y, a.n, a.t,
                       (uint64_t)a.y_ld * es, 128 / es, 32);
   if (!ok) return cudaErrorInvalidValue;

@@ -166,6 +166,15 @@ def test_strides(eng, t, n, k, dtype):
         check_gate_up(eng, t, n, k, dtype, x_ld=k + 16, w_ld=k + 112, y_ld=n + extra)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("t,n,k", [(300, 1, 64), (2600, 2401, 208), (5000, 2045, 96), (1100, 4999, 272), (4097, 1023, 1040)])
+def test_rows_that_begin_aligned_and_end_anywhere(eng, t, n, k, dtype):
+    """Rows 16 bytes apart or a multiple: nothing is written between a row's end and the next."""
+    for extra in (0, 8):
+        check_gemm(eng, t, n, k, dtype, seed=n, y_ld=(n + 7) // 8 * 8 + extra)
+        check_gate_up(eng, t, n, k, dtype, seed=n, y_ld=(n + 7) // 8 * 8 + extra)
+
+
 @pytest.mark.parametrize("off", [1, 2, 4, 6])
 @pytest.mark.parametrize("t,n", [(3, 64), (64, 256), (300, 512)])
 def test_unaligned_outputs(eng, t, n, off):
