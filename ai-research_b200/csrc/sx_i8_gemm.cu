@@ -687,9 +687,10 @@ constexpr uint64_t kGroupBytes = 32u << 20;
 
 // Tiles that are left when all pairs have had as many whole ones are taken in parts of half or a quarter of the
 // columns, so that more pairs have one (768 x 8192 x 3840 23.8 us, in halves 21.4; 1024 x 5000 x 4096 27.2, in quarters
-// 22.2).  The time, by what was measured: 5 us beside the steps of 128 of K, and those
-// 0.30 us, 0.42 at the clock that the power cap leaves in long calls, of a half 0.27.  Tiles with little K wait for
-// their values (2.7 us each), and lanes store for 1 us longer.  Weights that L2 does not hold come at 5 TB/s.
+// 22.2).  The time, by what was measured: 5 us beside the steps of 128 of K, and those 0.31 us (0.42 and more at the
+// clock that the power cap leaves in calls of 100 us, where there is no other choice), three quarters of it for a half.
+// Tiles with little K wait for their values (2.7 us each), and lanes store for 0.4 us longer.  Weights that L2 does
+// not hold come at 5 TB/s.
 PairPlan pair_plan(uint32_t dtype, bool gated, const I8Args &a, uint32_t pairs) {
   PairPlan p{};
   const uint32_t es = dtype == SX_F32 ? 4 : 2, steps = (a.k + kBK - 1) / kBK, cols = gated ? kBN / 2 : kBN;
@@ -715,9 +716,10 @@ PairPlan pair_plan(uint32_t dtype, bool gated, const I8Args &a, uint32_t pairs) 
   p.g.far = (uint64_t)a.t * a.n * es > (128u << 20);
   const float memory = (gated ? 2.0f : 1.0f) * (float)a.n * (float)a.k * (1.0f / 5.0e6f);
   const float turns = (float)(all / pairs), waves = turns + (left ? 1.0f : 0.0f);
-  const float step = waves > 2.0f ? 0.42f : 0.30f, last = left == 0 ? 0.0f : std::max((p.g.part == 2 ? 0.5f : p.g.part == 1 ? 0.65f : 1.0f) * step * steps, p.g.part ? 1.5f : 2.7f);
-  p.us = (turns > 0.0f || p.g.part == 0 ? 5.0f : 4.2f) + std::max(turns * std::max(step * steps, 2.7f) + last, memory);
-  if (p.g.boxes == 0) p.us += waves * 1.0f;
+  const float ragged = (a.w_ld | a.x_ld) % 128 != 0 ? 1.2f : 1.0f;  // rows that begin inside a line
+  const float step = 0.31f * ragged, last = left == 0 ? 0.0f : std::max((p.g.part == 2 ? 0.5f : p.g.part == 1 ? 0.75f : 1.0f) * step * steps, p.g.part ? 1.5f : 2.7f);
+  p.us = (turns > 0.0f || p.g.part == 0 ? 5.0f : gated ? 3.5f : 4.0f) + std::max(turns * std::max(step * steps, 2.7f) + last, memory);
+  if (p.g.boxes == 0) p.us += waves * 0.4f;
   return p;
 }
 
@@ -769,8 +771,9 @@ SplitPlan split_plan(bool gated, const I8Args &a, const uint32_t (&clusters)[4])
   s.p.stages = std::min(12u, ((two ? kSplitSmemTwo : kSplitSmem) - 1024) / stage);
   s.smem = std::max(s.p.stages * stage, sums) + 1024;  // the stages, then the sums
   const float waves = !two ? 1.0f : s.smem <= kSplitSmemTwo ? (float)tiles / (float)clusters[0] : (float)((tiles + clusters[0] - 1) / clusters[0]);
-  const float ragged = (a.w_ld | a.x_ld) % 128 != 0 ? 1.4f : 1.0f;  // rows that begin inside a line
-  const float load = ragged * (float)((steps + s.p.cluster - 1) / s.p.cluster) * (float)stage * (1.0f / 110e3f);
+  const float ragged = (a.w_ld | a.x_ld) % 128 != 0 ? 1.3f : 1.0f;  // rows that begin inside a line
+  const float few = two && s.p.stages < 3 ? 1.6f : 1.0f;  // (275 x 16078 x 2688, gate and up: 45 us; tiles of pairs 31.5)
+  const float load = few * ragged * (float)((steps + s.p.cluster - 1) / s.p.cluster) * (float)stage * (1.0f / 110e3f);
   const float memory = (float)mats * (float)a.n * (float)a.k * (1.0f / 6.2e6f);
   const float values = 0.013f * (float)(s.p.tok * mats);
   // (CTAs that have an SM for themselves start when the ones before have ended)
