@@ -745,7 +745,6 @@ SplitKernel split_kernel(uint32_t dtype, bool gated) {
 }
 constexpr uint32_t kSplitSmem = 220 * 1024, kSplitSmemTwo = 108 * 1024;  // one CTA an SM, two
 
-
 struct SplitPlan {
   SplitShape p;
   uint32_t n_tiles, t_tiles, smem;
@@ -863,7 +862,7 @@ sx_status dispatch_i8(const char *what, sx_engine *e, uint32_t dtype, sx::I8Args
   // tiles 8.1; 16 rows 11.9, 8.0; 32768 x 4096: 1 row 22.7 us).
   const bool stream = a.t <= sx::kI8GemvRows && (a.k > 2048 || a.n <= (gated ? 48u : 96u) * (uint32_t)e->num_sms);
   return sx_host_cuda_status(stream ? sx::launch_gemv_i8(dtype, gated, a, e->num_sms, e->stream)
-                                                     : sx::launch_tiles(dtype, gated, a, e->i8_clusters, e->stream), what);
+                                    : sx::launch_tiles(dtype, gated, a, e->i8_clusters, e->stream), what);
 }
 
 }  // namespace

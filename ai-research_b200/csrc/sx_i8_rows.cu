@@ -9,8 +9,9 @@
 // Measured, bound by HBM: seam of 16896 rows of 3840 (f32 stream, bf16 in and out) 130 us, 7.0 TB/s or 107 % of the
 // measured copy rate; codes of 2697 x 15360 bf16 20 us (6.2 TB/s, 95 %), of 16896 x 3840 29 (6.7 TB/s), of f32 with a
 // gain 51.6 (6.3): instructions and L1 count beside the bytes (bf16 magnitudes one at a time took 26.2 and 36 us, codes
-// by conversions 27 and 39; gains read again for the codes 58.6).  CTAs that go through rows with the next one on its way were slower (45 us
-// for 39, f32 89 for 59: registers), as were a warp for rows of 3840 (45) and more elements a thread.  One row of 3840 takes 1.5 us, with both norms 2.6.
+// by conversions 27 and 39; gains read again for the codes 58.6).  CTAs that go through rows with the next one on its
+// way were slower (45 us for 39, f32 89 for 59: registers), as were a warp for rows of 3840 (45) and more elements a
+// thread.  One row of 3840 takes 1.5 us, with both norms 2.6.
 #include "sx_host.h"
 #include "sx_i8.cuh"
 #include "sx_kv8.cuh"
@@ -349,8 +350,6 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads) residual_
   }
 }
 
-using RowsKernel = void (*)(const RowsArgs);
-
 // How rows are laid over threads.
 struct RowsPlan {
   bool warp;
@@ -444,8 +443,7 @@ SX_API sx_status sx_dispatch_quantize_i8(sx_engine *e, const sx_quantize_i8_args
   r.eps = a->eps;
   const sx::RowsPlan p = sx::rows_plan(a->n, a->rows, a->dtype == SX_F32 || a->norm_w ? 4 : 8, 4, e->num_sms);
   const sx::RowsKernel k = a->dtype == SX_F32 ? sx::quantize_kernel<float>(p, a->norm_w) : sx::quantize_kernel<__nv_bfloat16>(p, a->norm_w);
-  return sx_host_cuda_status(sx::launch_chained(k, dim3(p.ctas), dim3(p.threads), 0, e->stream, 1, r),
-      "quantize_i8 launch");
+  return sx_host_cuda_status(sx::launch_chained(k, dim3(p.ctas), dim3(p.threads), 0, e->stream, 1, r), "quantize_i8 launch");
 }
 
 SX_API sx_status sx_dispatch_residual_norm(sx_engine *e, const sx_residual_norm_args *a) {
