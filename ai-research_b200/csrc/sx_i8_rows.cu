@@ -8,10 +8,11 @@
 //
 // Measured, bound by HBM: seam of 16896 rows of 3840 (f32 stream, bf16 in and out) 130 us, 7.0 TB/s or 107 % of the
 // measured copy rate; codes of 2697 x 15360 bf16 20 us (6.2 TB/s, 95 %), of 16896 x 3840 29 (6.7 TB/s), of f32 with a
-// gain 51.6 (6.3): instructions and L1 count beside the bytes (bf16 magnitudes one at a time took 26.2 and 36 us, codes
-// by conversions 27 and 39; gains read again for the codes 58.6).  CTAs that go through rows with the next one on its
-// way were slower (45 us for 39, f32 89 for 59: registers), as were a warp for rows of 3840 (45) and more elements a
-// thread.  One row of 3840 takes 1.5 us, with both norms 2.6.
+// gain 49.7 (6.5), of bf16 with one 41 (4.8: registers leave nine rows an SM): instructions and L1 count beside the
+// bytes (bf16 magnitudes one at a time took 26.2 and 36 us, codes by conversions 27 and 39; gains read again for the
+// codes 58.6, two rows at a time for bf16's no faster).  CTAs that go through rows with the next one on its way were
+// slower (45 us for 39, f32 89 for 59: registers), as were a warp for rows of 3840 (45) and more elements a thread.
+// One row of 3840 takes 1.5 us, with both norms 2.6.
 #include "sx_host.h"
 #include "sx_i8.cuh"
 #include "sx_kv8.cuh"
@@ -77,9 +78,16 @@ SX_DEV void store8(T *p, const float (&v)[8]) {
     store_vec<T, 4>(p + 4, b);
   }
 }
+// The same of 4 elements and 4 of 128 elements further, zeros past n: each load of a warp is then one piece of memory.
+// (Of 32 bytes a lane L1 takes twice as long: 16896 x 3840 f32 with a gain 51.5 us, so 49.7; 8000 x 8000 55.4 and 51.1.
+// bf16 rows, half as many bytes for the same gains, are better off in pieces of 16 bytes: 41 and 42.)
+SX_DEV void load_raw_far(const float *p, bool more, Raw8<float> &r) {
+  r.v[0] = *reinterpret_cast<const uint4 *>(p);
+  r.v[1] = more ? *reinterpret_cast<const uint4 *>(p + 128) : make_uint4(0, 0, 0, 0);
+}
 // Codes of 8 values: adding 1.5 2^23 rounds a value of up to 127 to a whole number, ties to even, which is then the
 // sum's low byte.  mul 0: a row without values, whatever its elements.
-SX_DEV void store_codes(int8_t *p, const float (&u)[8], float mul) {
+SX_DEV uint2 codes_of(const float (&u)[8], float mul) {
   constexpr float kMagic = 12582912.0f;
   uint32_t w[2] = {0, 0};
   if (mul != 0.0f) {
@@ -92,7 +100,13 @@ SX_DEV void store_codes(int8_t *p, const float (&u)[8], float mul) {
       w[h] = prmt(prmt(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040), prmt(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040), 0x5410);
     }
   }
-  *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+  return make_uint2(w[0], w[1]);
+}
+SX_DEV void store_codes(int8_t *p, const float (&u)[8], float mul) { *reinterpret_cast<uint2 *>(p) = codes_of(u, mul); }
+SX_DEV void store_codes_far(int8_t *p, bool more, const float (&u)[8], float mul) {
+  const uint2 c = codes_of(u, mul);
+  *reinterpret_cast<uint32_t *>(p) = c.x;
+  if (more) *reinterpret_cast<uint32_t *>(p + 128) = c.y;
 }
 // the larger of top and |x|, a NaN where there is one
 SX_DEV float top_of(float top, float x) {
@@ -161,17 +175,35 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
   pdl_wait();
   const Place p = place<WARP>();
   if (WARP && p.row >= a.rows) return;
-  const uint32_t d0 = p.d0, step = p.step;
+  constexpr bool kFar = GAIN && sizeof(T) == 4;  // a warp's 256 elements as in load_raw_far
+  const uint32_t d0 = kFar ? p.d0 - 4 * (threadIdx.x & 31) : p.d0, step = p.step;
   const T *const in = static_cast<const T *>(a.in) + p.row * a.in_ld;
   int8_t *const q = static_cast<int8_t *>(a.y) + p.row * a.y_ld;
   constexpr uint32_t kHeld = G ? G : 1;
   Raw8<T> raw[kHeld];
   float u[GAIN ? kHeld : 1][8], top = 0.0f, sum = 0.0f;
+  auto load = [&](uint32_t d, Raw8<T> &r) {
+    if constexpr (kFar)
+      load_raw_far(in + d, d + 128 < a.n, r);
+    else
+      load_raw(in + d, r);
+  };
+  auto store = [&](uint32_t d, const float (&v)[8], float mul) {
+    if constexpr (kFar)
+      store_codes_far(q + d, d + 128 < a.n, v, mul);
+    else
+      store_codes(q + d, v, mul);
+  };
   // the group at d, from x in v: with its gain, and counted
   auto measure = [&](uint32_t d, float (&v)[8]) {
     if constexpr (GAIN) {
+      Raw8<float> raw_w;
+      if constexpr (kFar)
+        load_raw_far(a.w + d, d + 128 < a.n, raw_w);
+      else
+        load_raw(a.w + d, raw_w);
       float w[8];
-      load8(a.w + d, w);
+      unpack8(raw_w, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         sum = fmaf(v[i], v[i], sum);
@@ -184,7 +216,7 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
   if constexpr (G > 0) {
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
-      if (d0 + g * step < a.n) load_raw(in + d0 + g * step, raw[g]);
+      if (d0 + g * step < a.n) load(d0 + g * step, raw[g]);
     if constexpr (sizeof(T) == 2 && !GAIN) {  // two at a time: the order of bf16's bits is the values' too
       uint32_t pair = 0;
 #pragma unroll
@@ -201,7 +233,8 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
     }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
-      load8(in + d, u[0]);
+      load(d, raw[0]);
+      unpack8(raw[0], u[0]);
       measure(d, u[0]);
     }
   }
@@ -216,13 +249,14 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
     for (uint32_t g = 0; g < G; ++g)
       if (d0 + g * step < a.n) {
         if constexpr (!GAIN) unpack8(raw[g], u[0]);
-        store_codes(q + d0 + g * step, u[GAIN ? g : 0], mul);
+        store(d0 + g * step, u[GAIN ? g : 0], mul);
       }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
-      load8(in + d, u[0]);
+      load(d, raw[0]);
+      unpack8(raw[0], u[0]);
       measure(d, u[0]);
-      store_codes(q + d, u[0], mul);
+      store(d, u[0], mul);
     }
   }
 }
