@@ -8,7 +8,7 @@
 //
 // Measured, bound by HBM: seam of 16896 rows of 3840 (f32 stream, bf16 in and out) 130 us, 7.0 TB/s or 107 % of the
 // measured copy rate; codes of 2697 x 15360 bf16 20 us (6.2 TB/s, 95 %), of 16896 x 3840 29 (6.7 TB/s), of f32 with a
-// gain 49.7 (6.5), of bf16 with one 41 (4.8: registers leave nine rows an SM): instructions and L1 count beside the
+// gain 49.0 (6.6), of bf16 with one 39.4 (4.9: registers leave eight rows an SM): instructions and L1 count beside the
 // bytes (bf16 magnitudes one at a time took 26.2 and 36 us, codes by conversions 27 and 39; gains read again for the
 // codes 58.6, two rows at a time for bf16's no faster).  CTAs that go through rows with the next one on its way were
 // slower (45 us for 39, f32 89 for 59: registers), as were a warp for rows of 3840 (45) and more elements a thread.
@@ -166,10 +166,10 @@ SX_DEV float code_factor(uint32_t top, float sq_sum, float inv, bool norm, float
 }
 
 // G: groups of 8 elements that a thread holds, as they came or with their GAIN; 0: rows too long for registers are
-// read again (from L2).
+// read again (from L2).  (With 64 registers kMaxThreads fit.  The bound given as threads makes slower code: 2697 x 15360
+// with a gain 36.9 us, so 34.8; bf16 32.8, 30.9.)
 template <typename T, bool GAIN, bool WARP, uint32_t G>
-__global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
-    quantize_i8_kernel(const __grid_constant__ RowsArgs a) {
+__global__ void __maxnreg__(64) quantize_i8_kernel(const __grid_constant__ RowsArgs a) {
   __shared__ RowRed red;
   pdl_launch_dependents();
   pdl_wait();
@@ -182,18 +182,6 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
   constexpr uint32_t kHeld = G ? G : 1;
   Raw8<T> raw[kHeld];
   float u[GAIN ? kHeld : 1][8], top = 0.0f, sum = 0.0f;
-  auto load = [&](uint32_t d, Raw8<T> &r) {
-    if constexpr (kFar)
-      load_raw_far(in + d, d + 128 < a.n, r);
-    else
-      load_raw(in + d, r);
-  };
-  auto store = [&](uint32_t d, const float (&v)[8], float mul) {
-    if constexpr (kFar)
-      store_codes_far(q + d, d + 128 < a.n, v, mul);
-    else
-      store_codes(q + d, v, mul);
-  };
   // the group at d, from x in v: with its gain, and counted
   auto measure = [&](uint32_t d, float (&v)[8]) {
     if constexpr (GAIN) {
@@ -216,7 +204,12 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
   if constexpr (G > 0) {
 #pragma unroll
     for (uint32_t g = 0; g < G; ++g)
-      if (d0 + g * step < a.n) load(d0 + g * step, raw[g]);
+      if (d0 + g * step < a.n) {
+        if constexpr (kFar)
+          load_raw_far(in + d0 + g * step, d0 + g * step + 128 < a.n, raw[g]);
+        else
+          load_raw(in + d0 + g * step, raw[g]);
+      }
     if constexpr (sizeof(T) == 2 && !GAIN) {  // two at a time: the order of bf16's bits is the values' too
       uint32_t pair = 0;
 #pragma unroll
@@ -233,7 +226,10 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
     }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
-      load(d, raw[0]);
+      if constexpr (kFar)
+        load_raw_far(in + d, d + 128 < a.n, raw[0]);
+      else
+        load_raw(in + d, raw[0]);
       unpack8(raw[0], u[0]);
       measure(d, u[0]);
     }
@@ -249,14 +245,23 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads)
     for (uint32_t g = 0; g < G; ++g)
       if (d0 + g * step < a.n) {
         if constexpr (!GAIN) unpack8(raw[g], u[0]);
-        store(d0 + g * step, u[GAIN ? g : 0], mul);
+        if constexpr (kFar)
+          store_codes_far(q + d0 + g * step, d0 + g * step + 128 < a.n, u[g], mul);
+        else
+          store_codes(q + d0 + g * step, u[GAIN ? g : 0], mul);
       }
   } else {
     for (uint32_t d = d0; d < a.n; d += step) {
-      load(d, raw[0]);
+      if constexpr (kFar)
+        load_raw_far(in + d, d + 128 < a.n, raw[0]);
+      else
+        load_raw(in + d, raw[0]);
       unpack8(raw[0], u[0]);
       measure(d, u[0]);
-      store(d, u[0], mul);
+      if constexpr (kFar)
+        store_codes_far(q + d, d + 128 < a.n, u[0], mul);
+      else
+        store_codes(q + d, u[0], mul);
     }
   }
 }
