@@ -154,6 +154,9 @@ SX_DEV Place place() {
   return {blockIdx.x, 8 * threadIdx.x, 8 * blockDim.x};
 }
 
+// 1 / sqrt(mean of squares + eps); a NaN where the squares' sum has passed f32: as 0 it would take a row's values away.
+SX_DEV float inv_rms(float mean) { return mean < INFINITY ? 1.0f / sqrtf(mean) : __uint_as_float(0x7FC00000u); }
+
 // What a row's codes are multiplied by, and its scale.
 SX_DEV float code_factor(uint32_t top, float sq_sum, float inv, bool norm, float *scale) {
   const float a = __uint_as_float(top);
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads) residual_
       }
     }
     row_reduce<WARP>(red[0], bits, sum);
-    post = 1.0f / sqrtf(sum / (float)a.n + a.eps);
+    post = inv_rms(sum / (float)a.n + a.eps);
     sum = 0.0f;
   }
   // the new residual of a group in u, from x there
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(WARP ? kWarpRows * 32 : kMaxThreads) residual_
   if constexpr (OUT == kOutNone) return;
   bits = __float_as_uint(top) & 0x7FFFFFFFu;
   row_reduce<WARP>(red[1], bits, sum);
-  const float inv = 1.0f / sqrtf(sum / (float)a.n + a.eps);
+  const float inv = inv_rms(sum / (float)a.n + a.eps);
   float mul = 0.0f;
   if constexpr (OUT == kOutI8) {
     float scale;

@@ -713,7 +713,9 @@ SX_API sx_status sx_dispatch_quantize_i8(sx_engine *e, const sx_quantize_i8_args
  *   x_out = (x + h) * scalar
  *   y = x_out / sqrt(mean(x_out^2) + eps) * pre_w
  * in f32; y in y_dtype, SX_I8 as sx_dispatch_quantize_i8 of x_out with gain pre_w (scales to y_scale,
- * else NULL).  y NULL: x_out alone, without pre_w.  x_out may be x.  Sizes and alignment as there. */
+ * else NULL).  y NULL: x_out alone, without pre_w.  x_out may be x.  A norm of a row whose squares' sum
+ * passes f32 (one with an infinity, or values above some 1e18) is NaN in all of the row, whatever it is
+ * written as: x_out with post_w, y.  Sizes and alignment as there. */
 typedef struct {
   const float *x;       /* [rows] of n: the residual stream             */
   const void *r;        /* [rows] of n, r_dtype: what the block computed */

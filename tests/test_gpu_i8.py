@@ -591,3 +591,57 @@ def test_rows_do_not_depend_on_their_batch(eng):
         eng.gate_up_i8(x, xs, w, ws, wu, us, sx.DTYPE_F32, b, t, 650, 720)
         eng.sync()
         assert torch.equal(a, y[:t]) and torch.equal(b, z[:t])
+
+
+# rows as CTAs with every number of elements a thread, and as warps
+LAYOUTS = [(9, 64), (9, 3840), (9, 8208), (9, 15360), (9, 40000), (305, 64), (305, 512), (305, 1024), (305, 2048), (305, 8192), (305, 8208), (305, 16400)]
+
+
+def seam(eng, x, r, post, pre, y_type, scalar=0.875, eps=1e-6):
+    rows, n = x.shape
+    out, scale = torch.empty(rows, n, device="cuda"), torch.empty(rows, device="cuda") if y_type == torch.int8 else None
+    y = None if y_type is None else torch.full((rows, n), JUNK, dtype=y_type, device="cuda")
+    eng.residual_norm(x, TYPES[r.dtype], r, out, TYPES.get(y_type, 0), y, rows, n, post_w=post, pre_w=pre, scalar=scalar, eps=eps, y_scale=scale)
+    eng.sync()
+    return out, y, scale
+
+
+def only_nan(y, scale):
+    """Rows of no value: floats that are NaN, or codes 0 with the scale NaN."""
+    return y.isnan().all() if scale is None else (y == 0).all() and scale.isnan().all()
+
+
+@pytest.mark.parametrize("r_type", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", LAYOUTS)
+def test_norm_of_squares_past_f32(eng, rows, n, r_type):
+    """A norm of squares whose sum f32 does not hold is NaN, whatever it is written as, and no other row's."""
+    g = gen(n)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    clean = rand(rows, n), rand(rows, n).to(r_type)
+    clean[1][rows - 1] *= 1e16  # (not past it)
+    clean[0][rows - 2] *= 1e16
+    post, pre = 1 + 0.2 * rand(n), 1 + 0.2 * rand(n)
+    x, r = (v.clone() for v in clean)
+    r[0] *= 1e30
+    r[1, n // 3] = 1e20
+    r[2, 5] = math.inf
+    x[3] *= 1e30
+    x[4, n - 1] = -1e25
+    x[5, 7] = -math.inf
+    for y_type in (torch.float32, torch.bfloat16, torch.int8, None):
+        for w in (post, None):
+            check_norm(eng, *clean, w, pre, 0.875, y_type)
+            want, want_y, want_scale = seam(eng, *clean, w, pre, y_type)
+            out, y, scale = seam(eng, x, r, w, pre, y_type)
+            assert torch.equal(out[6:], want[6:])
+            if w is not None:
+                assert out[:3].isnan().all()
+                assert torch.equal(out[5].isinf(), x[5].isinf()) and torch.equal(out[5, 8:], want[5, 8:])
+            else:
+                assert torch.equal(out[:6], (x[:6] + r[:6].float()) * 0.875)
+            assert ((out[3:5] - x[3:5] * 0.875).abs() <= x[3:5].abs() * 2 * F + (want[3:5] - clean[0][3:5] * 0.875).abs() + 1e-6).all()
+            if y_type is None:
+                continue
+            assert torch.equal(y[6:], want_y[6:]) and only_nan(y[:6], None if scale is None else scale[:6])
+            if scale is not None:
+                assert torch.equal(scale[6:], want_scale[6:])
