@@ -154,10 +154,13 @@ SX_DEV Place place() {
   return {blockIdx.x, 8 * threadIdx.x, 8 * blockDim.x};
 }
 
-// 1 / sqrt(mean of squares + eps); a NaN where the squares' sum has passed f32: as 0 it would take a row's values away.
-SX_DEV float inv_rms(float mean) { return mean < INFINITY ? 1.0f / sqrtf(mean) : __uint_as_float(0x7FC00000u); }
+// 1 / sqrt(mean of squares + eps); a NaN where that is no normal number of f32: a sum of squares that has passed f32 would
+// take a row's values away as 0, and below 2^-126 squares are rounded by a 2^-149, which shows in their sum.
+SX_DEV float inv_rms(float mean) {
+  return __float_as_uint(mean) - 0x00800000u < 0x7F000000u ? 1.0f / sqrtf(mean) : __uint_as_float(0x7FC00000u);
+}
 
-// What a row's codes are multiplied by, and its scale.
+// What a row's codes are multiplied by, and its scale (inv: inv_rms with a norm, or 1).
 SX_DEV float code_factor(uint32_t top, float sq_sum, float inv, bool norm, float *scale) {
   const float a = __uint_as_float(top);
   if (top >= kInf || (norm && !(sq_sum < INFINITY))) {
@@ -240,7 +243,7 @@ __global__ void __maxnreg__(64) quantize_i8_kernel(const __grid_constant__ RowsA
   uint32_t bits = __float_as_uint(top) & 0x7FFFFFFFu;  // (their order is the values', with infinity and NaN on top)
   row_reduce<WARP>(red, bits, sum);
   float scale;
-  const float inv = GAIN ? 1.0f / sqrtf(sum / (float)a.n + a.eps) : 1.0f;
+  const float inv = GAIN ? inv_rms(sum / (float)a.n + a.eps) : 1.0f;
   const float mul = code_factor(bits, sum, inv, GAIN, &scale);
   if (d0 == 0) a.scale[p.row] = scale;
   if constexpr (G > 0) {

@@ -696,8 +696,10 @@ SX_API sx_status sx_dispatch_verify(sx_engine *e, const float *target, uint32_t 
  * q * scale is the row, or its RMS norm with the gain norm_w (whose own factor cancels out of q).  Rows
  * whose a is below 2^-100 count as zeros (codes and scale 0); a row that holds a NaN or an infinity, or
  * with norm_w one whose squares' sum passes f32, has codes 0 and scale NaN, so what is computed from it
- * is NaN.  Rows of a weight matrix make the codes of its output channels.  n a multiple of 16, below
- * 131072; x 16-byte aligned with a stride of 16 bytes' multiple, q likewise; norm_w 16-byte aligned. */
+ * is NaN.  Of the others the scale is NaN where mean(x^2) + eps is below 2^-126, which no eps from there
+ * on lets happen (squares that small are rounded away).  Rows of a weight matrix make the codes of its
+ * output channels.  n a multiple of 16, below 131072; x 16-byte aligned with a stride of 16 bytes'
+ * multiple, q likewise; norm_w 16-byte aligned. */
 typedef struct {
   const void *x;       /* [rows] of n, dtype SX_F32 or SX_BF16 */
   const float *norm_w; /* [n] or NULL                          */
@@ -713,9 +715,10 @@ SX_API sx_status sx_dispatch_quantize_i8(sx_engine *e, const sx_quantize_i8_args
  *   x_out = (x + h) * scalar
  *   y = x_out / sqrt(mean(x_out^2) + eps) * pre_w
  * in f32; y in y_dtype, SX_I8 as sx_dispatch_quantize_i8 of x_out with gain pre_w (scales to y_scale,
- * else NULL).  y NULL: x_out alone, without pre_w.  x_out may be x.  A norm of a row whose squares' sum
- * passes f32 (one with an infinity, or values above some 1e18) is NaN in all of the row, whatever it is
- * written as: x_out with post_w, y.  Sizes and alignment as there. */
+ * else NULL).  y NULL: x_out alone, without pre_w.  x_out may be x.  A norm is NaN in all of a row,
+ * whatever that is written as (x_out with post_w, y), where the squares' sum passes f32, as with an
+ * infinity, or mean + eps is below 2^-126, which no eps from there on lets happen: squares that small are
+ * rounded away.  Sizes and alignment as there. */
 typedef struct {
   const float *x;       /* [rows] of n: the residual stream             */
   const void *r;        /* [rows] of n, r_dtype: what the block computed */

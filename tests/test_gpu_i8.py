@@ -645,3 +645,45 @@ def test_norm_of_squares_past_f32(eng, rows, n, r_type):
             assert torch.equal(y[6:], want_y[6:]) and only_nan(y[:6], None if scale is None else scale[:6])
             if scale is not None:
                 assert torch.equal(scale[6:], want_scale[6:])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,n", LAYOUTS)
+def test_squares_below_f32(eng, rows, n, dtype):
+    """Rows whose squares are nothing in f32: any eps of a normal number is enough for them; with less they are NaN (codes,
+    where values are below 2^-100: zeros)."""
+    g = gen(n)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    post, pre, zeros, ones = 1 + 0.2 * rand(n), 1 + 0.2 * rand(n), torch.zeros(rows, n, device="cuda"), torch.ones(rows, n, device="cuda")
+    x = rand(rows, n)
+    x[:3] *= torch.tensor([1e-15, 1e-17, 1e-18], device="cuda")[:, None]
+    x[rows - 1] *= 1e-18
+    for eps in (0.0, 1e-40):
+        check_quantize(eng, x.to(dtype), pre, eps=eps)
+        for y_type in (torch.float32, torch.bfloat16, torch.int8, None):
+            check_norm(eng, x, zeros.to(dtype), None, pre, 0.5, y_type, eps=eps)
+            check_norm(eng, zeros, x.to(dtype), post, pre, 0.5, y_type, eps=eps)
+    small = x.clone()
+    small[3:7] = rand(4, n) * torch.tensor([1e-20, 1e-25, 1e-29, 1e-36], device="cuda")[:, None]
+    small[7] = 0
+    for eps in (2.0 ** -126, 1e-30):
+        check_quantize(eng, small.to(dtype), pre, eps=eps)
+        for y_type in (torch.float32, torch.bfloat16, torch.int8, None):
+            check_norm(eng, small, zeros.to(dtype), None, pre, 0.5, y_type, eps=eps)
+            check_norm(eng, ones, small.to(dtype), post, pre, 0.5, y_type, eps=eps)
+    for eps in (0.0, 1e-41):
+        q, scale = torch.full((rows, n), JUNK, dtype=torch.int8, device="cuda"), torch.full((rows,), 9.0, device="cuda")
+        eng.quantize_i8(TYPES[dtype], small.to(dtype), q, scale, rows, n, norm_w=pre, eps=eps)
+        eng.sync()
+        assert scale[3:6].isnan().all() and (q[6:8] == 0).all() and (scale[6:8] == 0).all()
+        assert scale[:3].isfinite().all() and scale[8:].isfinite().all() and (q[8:].abs().amax(-1) == 127).all()
+        for y_type in (torch.float32, torch.bfloat16, torch.int8):
+            out, y, scale = seam(eng, small, zeros.to(dtype), None, pre, y_type, eps=eps)
+            assert torch.equal(out, small * 0.875)
+            if scale is None:
+                assert only_nan(y[3:8], None) and y[:3].isfinite().all() and y[8:].isfinite().all()
+            else:
+                assert scale[3:6].isnan().all() and (y[6:8] == 0).all() and (scale[6:8] == 0).all()
+                assert scale[:3].isfinite().all() and scale[8:].isfinite().all()
+            out = seam(eng, ones, small.to(dtype), post, pre, y_type, eps=eps)[0]
+            assert out[3:8].isnan().all() and out[:3].isfinite().all() and out[8:].isfinite().all()
