@@ -687,3 +687,11 @@ def test_squares_below_f32(eng, rows, n, dtype):
                 assert scale[:3].isfinite().all() and scale[8:].isfinite().all()
             out = seam(eng, ones, small.to(dtype), post, pre, y_type, eps=eps)[0]
             assert out[3:8].isnan().all() and out[:3].isfinite().all() and out[8:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype,t", [(torch.float32, 4200), (torch.bfloat16, 8400)], ids=["f32", "bf16"])
+@pytest.mark.parametrize("n,y_ld", [(8200, 8200), (8201, 8208)])
+def test_results_that_l2_does_not_hold(eng, t, n, y_ld, dtype):
+    """More than 128 MB of y: its lines leave L2 first; whole rows, and rows that end inside 16 bytes."""
+    check_gemm(eng, t, n, 80, dtype, seed=n, y_ld=y_ld)
+    check_gate_up(eng, t, n, 80, dtype, seed=n, y_ld=y_ld)
