@@ -695,3 +695,30 @@ def test_results_that_l2_does_not_hold(eng, t, n, y_ld, dtype):
     """More than 128 MB of y: its lines leave L2 first; whole rows, and rows that end inside 16 bytes."""
     check_gemm(eng, t, n, 80, dtype, seed=n, y_ld=y_ld)
     check_gate_up(eng, t, n, 80, dtype, seed=n, y_ld=y_ld)
+
+
+@pytest.mark.parametrize("t,n", [(4, 70), (16, 70), (40, 300), (400, 300)])
+def test_infinite_scales_of_columns(eng, t, n):
+    """An infinite scale makes its column infinite, by the sums' signs; NaN where there is 0 to multiply."""
+    k = 320
+    (x, xs), (w, ws), (wu, us) = operands(t, n, k, 3, gated=True)
+    x[1] = 0
+    xs[2] = 0
+    ws[7], us[9] = math.inf, math.inf
+    y, z = torch.empty(t, n, device="cuda"), torch.empty(t, n, device="cuda")
+    eng.gemm_i8(x, xs, w, ws, sx.DTYPE_F32, y, t, n, k)
+    eng.gate_up_i8(x, xs, w, ws, wu, us, sx.DTYPE_F32, z, t, n, k)
+    eng.sync()
+    s, su = sums(x, w), sums(x, wu)
+    inf = torch.tensor(math.inf, device="cuda", dtype=torch.float64)
+    sign = torch.where(xs > 0, s[:, 7].sign(), 0.0)
+    assert torch.equal(y[:, 7].double().nan_to_num(0.0, math.inf, -math.inf), torch.where(sign == 0, 0.0, sign * inf))
+    assert torch.equal(y[:, 7].isnan(), sign == 0)
+    # an infinite gate opens or, below, is infinity times nothing; an infinite `up` has the gate's sign times its own
+    up = torch.where(xs > 0, su[:, 7].sign(), 0.0)
+    lost = (sign <= 0) | (up == 0)
+    assert torch.equal(z[:, 7].isnan(), lost) and torch.equal(z[:, 7].double()[~lost], (up * inf)[~lost])
+    both = torch.where(xs > 0, s[:, 9].sign() * su[:, 9].sign(), 0.0)
+    assert torch.equal(z[:, 9].isnan(), both == 0) and torch.equal(z[:, 9].double()[both != 0], (both * inf)[both != 0])
+    cols = [j for j in range(n) if j not in (7, 9)]
+    assert y[:, cols].isfinite().all() and z[:, cols].isfinite().all() and y[:, 9].isfinite().all()
