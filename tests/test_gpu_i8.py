@@ -722,3 +722,40 @@ def test_infinite_scales_of_columns(eng, t, n):
     assert torch.equal(z[:, 9].isnan(), both == 0) and torch.equal(z[:, 9].double()[both != 0], (both * inf)[both != 0])
     cols = [j for j in range(n) if j not in (7, 9)]
     assert y[:, cols].isfinite().all() and z[:, cols].isfinite().all() and y[:, 9].isfinite().all()
+
+
+@pytest.mark.parametrize("t", [1, 16, 50, 300])
+def test_captures_with_inputs_of_their_own(eng, t):
+    """Two captures of blocks whose weights are the same, replayed at once: each has its own input's results."""
+    blocks = [Block(eng, t, 512, 1040, 1) for _ in range(2)]
+    graphs, streams = [], [torch.cuda.Stream() for _ in blocks]
+    try:
+        for b, s in zip(blocks, streams):
+            eng.set_stream(s.cuda_stream)
+            with torch.cuda.stream(s):
+                b.run()
+                s.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=s):
+                    b.run()
+                graphs.append(g)
+    finally:
+        eng.set_stream(sx.STREAM_LEGACY)
+    torch.cuda.synchronize()
+    for i, b in enumerate(blocks):
+        b.x.normal_(generator=gen(100 * i + t))
+        b.attn.normal_(generator=gen(100 * i + t + 50))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    replayed = [(b.x1.clone(), b.h.clone(), b.out.clone(), b.y.clone()) for b in blocks]
+    for x, y in zip(*replayed):
+        assert not torch.equal(x, y)
+    for b, r in zip(blocks, replayed):
+        b.run()
+        eng.sync()
+        for x, y in zip((b.x1, b.h, b.out, b.y), r):
+            assert torch.equal(x, y)
