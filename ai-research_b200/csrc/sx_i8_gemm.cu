@@ -844,7 +844,7 @@ sx_status dispatch_i8(const char *what, sx_engine *e, uint32_t dtype, sx::I8Args
     al |= (uintptr_t)a.w[i];
     if ((uintptr_t)a.w_scale[i] % 4 != 0) return bad("scales must be aligned to their elements");
   }
-  if (!a.x || !a.x_scale || !a.y) return bad("null x, x_scale or y");
+  if (a.t && (!a.x || !a.x_scale || !a.y)) return bad("null x, x_scale or y");  // (an empty tensor has no address)
   if ((uintptr_t)a.x_scale % 4 != 0) return bad("scales must be aligned to their elements");
   if (a.k == 0 || a.k % 16 != 0 || a.k >= sx::kI8MaxK) return bad("k must be a multiple of 16, above 0 and below 131072");
   if (a.n == 0) return bad("n must be above 0");

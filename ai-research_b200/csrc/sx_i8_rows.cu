@@ -464,7 +464,7 @@ SX_API sx_status sx_dispatch_quantize_i8(sx_engine *e, const sx_quantize_i8_args
   };
   if (!a) return bad("null arguments");
   if (a->dtype != SX_F32 && a->dtype != SX_BF16) return bad("dtype must be SX_F32 or SX_BF16");
-  if (!a->x || !a->q || !a->scale) return bad("null x, q or scale");
+  if (a->rows && (!a->x || !a->q || !a->scale)) return bad("null x, q or scale");  // (an empty tensor has no address)
   if (a->n == 0 || a->n % 16 != 0 || a->n >= sx::kI8MaxK) return bad("n must be a multiple of 16, above 0 and below 131072");
   if (a->x_ld < a->n || a->q_ld < a->n) return bad("row strides are shorter than a row");
   if (!sx::aligned(a->x, a->x_ld, a->dtype) || !sx::aligned(a->q, a->q_ld, SX_I8) || (uintptr_t)a->norm_w % 16 != 0)
@@ -498,13 +498,13 @@ SX_API sx_status sx_dispatch_residual_norm(sx_engine *e, const sx_residual_norm_
   };
   if (!a) return bad("null arguments");
   if (a->r_dtype != SX_F32 && a->r_dtype != SX_BF16) return bad("r_dtype must be SX_F32 or SX_BF16");
-  if (!a->x || !a->r || !a->x_out) return bad("null x, r or x_out");
+  if (a->rows && (!a->x || !a->r || !a->x_out)) return bad("null x, r or x_out");
   if (a->n == 0 || a->n % 16 != 0 || a->n >= sx::kI8MaxK) return bad("n must be a multiple of 16, above 0 and below 131072");
   if (a->x_ld < a->n || a->r_ld < a->n || a->x_out_ld < a->n) return bad("row strides are shorter than a row");
   if (!sx::aligned(a->x, a->x_ld, SX_F32) || !sx::aligned(a->r, a->r_ld, a->r_dtype) || !sx::aligned(a->x_out, a->x_out_ld, SX_F32) ||
       (uintptr_t)a->post_w % 16 != 0)
     return bad("rows and gains must be 16-byte aligned and strides multiples of 16 bytes");
-  if (a->x_out == a->x && a->x_out_ld != a->x_ld) return bad("x_out may be x with the same stride only");
+  if (a->rows && a->x_out == a->x && a->x_out_ld != a->x_ld) return bad("x_out may be x with the same stride only");
   if (a->y) {
     if (a->y_dtype != SX_F32 && a->y_dtype != SX_BF16 && a->y_dtype != SX_I8) return bad("y_dtype must be SX_F32, SX_BF16 or SX_I8");
     if (!a->pre_w) return bad("null pre_w");

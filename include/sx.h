@@ -687,8 +687,8 @@ SX_API sx_status sx_dispatch_verify(sx_engine *e, const float *target, uint32_t 
  *
  * All four are asynchronous on the engine stream, use no memory but their arguments' and can be
  * captured in a CUDA graph; calls on streams of their own may overlap.  Arguments come in one block; a
- * row stride `*_ld` counts elements.  0 rows are no work.  Inputs and outputs must not overlap but
- * where it says so.
+ * row stride `*_ld` counts elements.  0 rows are no work, and their pointers may be NULL.  Inputs and
+ * outputs must not overlap but where it says so.
  * ------------------------------------------------------------------------------------- */
 /* Rows to codes: u = x (norm_w NULL) or x * norm_w, f32 products; a = the largest |u| of the row;
  *   q = u * (127 / a) rounded to the nearest whole number, ties to even (quotient and product in f32),

@@ -164,3 +164,19 @@ def test_no_arguments_at_all():
     for call in ("quantize_i8", "residual_norm", "gemm_i8", "gate_up_i8"):
         assert getattr(sx.lib(), "sx_dispatch_" + call)(None, None) == sx.SX_ERR_INVALID
         assert "null arguments" in sx.last_error()
+
+
+@pytest.mark.parametrize("call,args", [
+    ("quantize_i8", dict(Q, rows=0, x=None, q=None, scale=None)), ("quantize_i8", dict(Q, rows=0, x=None, q=None, scale=None, norm_w=E)),
+    ("residual_norm", dict(N, rows=0, x=None, r=None, x_out=None, y=None)),
+    ("residual_norm", dict(N, rows=0, x=None, r=None, x_out=None, y=None, y_scale=None, y_dtype=2, x_ld=72)),
+    ("gemm_i8", dict(P, t=0, x=None, x_scale=None, y=None)), ("gate_up_i8", dict(U, t=0, x=None, x_scale=None, y=None)),
+])
+def test_no_rows_have_no_addresses(engine, call, args):
+    """Tensors of no rows have no memory, and the call no work: nothing but the engine is missed."""
+    assert refusal(engine, call, args) == "null engine"
+
+
+@pytest.mark.parametrize("call,args", [("gemm_i8", dict(P, t=0, w=None)), ("gate_up_i8", dict(U, t=0, wu_scale=None))])
+def test_weights_are_there_without_rows_too(engine, call, args):
+    assert "null weights" in refusal(engine, call, args)
