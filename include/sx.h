@@ -735,7 +735,7 @@ SX_API sx_status sx_dispatch_residual_norm(sx_engine *e, const sx_residual_norm_
 /* y[t][n] = (float) (sum_k x[t][k] w[n][k]) * x_scale[t] * w_scale[n], rounded to dtype once.
  * k a multiple of 16, below 131072 (so that sums of any codes, -128 too, stay below 2^31); x and w
  * 16-byte aligned with strides that are multiples of 16; y aligned to its elements, any stride.  Bytes
- * between a row's end and its stride are not used.  t and n below 2^31. */
+ * between a row's end and its stride are not used.  t and n below 2^31, t * n below 2^42. */
 typedef struct {
   const int8_t *x;      /* [t] of k */
   const float *x_scale; /* [t]      */

@@ -180,3 +180,11 @@ def test_no_rows_have_no_addresses(engine, call, args):
 @pytest.mark.parametrize("call,args", [("gemm_i8", dict(P, t=0, w=None)), ("gate_up_i8", dict(U, t=0, wu_scale=None))])
 def test_weights_are_there_without_rows_too(engine, call, args):
     assert "null weights" in refusal(engine, call, args)
+
+
+@pytest.mark.parametrize("call,args", [("gemm_i8", P), ("gate_up_i8", U)])
+def test_the_largest_results(engine, call, args):
+    """Tiles are counted in 32 bits: t * n below 2^42."""
+    for t, n in ((1 << 21, 1 << 21), (1 << 30, 1 << 12)):
+        assert "2^42" in refusal(engine, call, dict(args, t=t, n=n, y_ld=n))
+        assert refusal(engine, call, dict(args, t=t - 1, n=n, y_ld=n)) == "null engine"
