@@ -20,8 +20,9 @@ struct I8Args {
 // A sum as the value it stands for.  (Operations are spelled out here and below: all kernels round alike, so a
 // row of a product does not depend on which of them computes it.)
 SX_DEV float i8_value(int32_t sum, float x_scale, float w_scale) { return __fmul_rn(__fmul_rn((float)sum, x_scale), w_scale); }
-// gelu_tanh(g) * u: g / 2 (1 + tanh z) = g / (1 + e^-2z), z = 0.7978845608 (g + 0.044715 g^3); e^-2z overflows where
-// the quotient is 0 in f32
+// gelu_tanh(g) * u: g / 2 (1 + tanh z) = g / (1 + e^-2z), z = 0.7978845608 (g + 0.044715 g^3).  The reciprocal is 0 where it
+// would be below f32's normal numbers, from a sum of 2^126 on (g below -10): that takes at most 2^-126 |g u| away.  Above,
+// e^-2z carries its exponent's rounding: some 9 + 17 |z| steps of 2^-23 in all.
 constexpr float kGelu1 = -2.0f * 0.7978845608f * 1.4426950408889634f, kGelu3 = kGelu1 * 0.044715f;  // of g, g^3 in log2 e^-2z
 SX_DEV float i8_ex2(float x) {
   float r;

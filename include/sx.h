@@ -747,7 +747,8 @@ typedef struct {
 SX_API sx_status sx_dispatch_gemm_i8(sx_engine *e, const sx_gemm_i8_args *a);
 
 /* y = gelu_tanh(g) * u, g and u as sx_dispatch_gemm_i8 of (wg, wg_scale) and (wu, wu_scale) in f32,
- * gelu_tanh(g) = g / 2 (1 + tanh(0.7978845608 (g + 0.044715 g^3))).  Limits as there. */
+ * gelu_tanh(g) = g / 2 (1 + tanh(0.7978845608 (g + 0.044715 g^3))); 0 where that is below 2^-126 |g|
+ * (g below -10).  Limits as there. */
 typedef struct {
   const int8_t *x;
   const float *x_scale;

@@ -759,3 +759,24 @@ def test_captures_with_inputs_of_their_own(eng, t):
         eng.sync()
         for x, y in zip((b.x1, b.h, b.out, b.y), r):
             assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("t", [1, 9, 40, 300])
+def test_gates_that_are_nothing(eng, t):
+    """Around g = -10 the gate leaves f32's normal numbers: off by at most 2^-126 |g u| there, and never by more below."""
+    n, k = 2048, 16
+    x = torch.ones(t, k, dtype=torch.int8, device="cuda")
+    wg, wu = -torch.ones(n, k, dtype=torch.int8, device="cuda"), torch.ones(n, k, dtype=torch.int8, device="cuda")
+    xs = torch.ones(t, device="cuda")
+    gs = torch.linspace(9.0, 11.0, n, device="cuda") / 16
+    us = torch.full((n,), 2.0 ** 90 / 16, device="cuda")
+    y = torch.empty(t, n, device="cuda")
+    eng.gate_up_i8(x, xs, wg, gs, wu, us, sx.DTYPE_F32, y, t, n, k)
+    eng.sync()
+    g, u = -16 * gs.double(), 2.0 ** 90
+    z = (0.7978845608 * (g + 0.044715 * g ** 3)).abs()
+    want = gelu(g) * u
+    # (as in check_gate_up, g and u exact here but for g's own rounding; the reciprocal's 0 takes 2^-126 |g u|)
+    tol = want.abs() * (18 + 33 * z) * F + (g * u).abs() * 2.0 ** -126
+    assert ((y.double() - want).abs() <= tol).all()
+    assert (y[:, g < -10.01] == 0).all() and (y[:, g > -9.99] != 0).all()
