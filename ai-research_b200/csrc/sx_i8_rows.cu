@@ -6,13 +6,14 @@
 // with u = x * w, which has no sum in it, so codes do not depend on how a row is split over threads.  A NaN or an
 // infinity is found in the maximum itself, whose bits are above all others'.
 //
-// Measured, bound by HBM: seam of 16896 rows of 3840 (f32 stream, bf16 in and out) 130 us, 7.0 TB/s or 107 % of the
-// measured copy rate; codes of 2697 x 15360 bf16 20 us (6.2 TB/s, 95 %), of 16896 x 3840 29 (6.7 TB/s), of f32 with a
-// gain 49.0 (6.6), of bf16 with one 39.4 (4.9: registers leave eight rows an SM): instructions and L1 count beside the
-// bytes (bf16 magnitudes one at a time took 26.2 and 36 us, codes by conversions 27 and 39; gains read again for the
-// codes 58.6, two rows at a time for bf16's no faster).  CTAs that go through rows with the next one on its way were
-// slower (45 us for 39, f32 89 for 59: registers), as were a warp for rows of 3840 (45) and more elements a thread.
-// One row of 3840 takes 1.5 us, with both norms 2.6.
+// Measured, bound by HBM: seam of 16896 rows of 3840 (f32 stream, bf16 in and out, 12 bytes an element) 135 us, 5.8 TB/s
+// or 88 % of the measured copy rate, with L1 77 % busy beside it; into codes 146 us, 75 %; codes of 2697 x 15360 bf16 20 us
+// (6.2 TB/s, 95 %), of 16896 x 3840 29 (6.6 TB/s), of f32 with a gain 49 (6.6), of bf16 with one 44 (4.4: registers leave
+// eight rows an SM) and of 2697 x 15360 32.5 (3.8: two): instructions and L1 count beside the bytes (bf16 magnitudes one at
+// a time took 26.2 and 36 us, codes by conversions 27 and 39; gains read again for the codes 58.6 for f32's 51.4, two rows
+// at a time for bf16's no faster).  CTAs that go through rows with the next one on its way were slower (45 us for 39, f32
+// 89 for 59: registers), as were a warp for rows of 3840 (45) and more elements a thread.  One row of 3840 takes 1.5 us,
+// with a gain 1.9, with both norms 3.0.
 #include "sx_host.h"
 #include "sx_i8.cuh"
 #include "sx_kv8.cuh"
