@@ -655,11 +655,6 @@ __global__ void __launch_bounds__(kMergeThreads) kv8_prompt_merge_kernel(const _
 // One product by one thread of the warp that calls it: STEPS of 16 along K, A from shared memory
 // (a_tile) or tensor memory (a_col); 32 bytes of a swizzled row per step, a panel of 64 elements every
 // four.  The whole warp comes here so that descriptors are the same in all lanes.
-SX_DEV bool elect_one() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
-  return p != 0;
-}
 template <int STEPS>
 SX_DEV void issue_ss(uint32_t d, uint32_t a_tile, uint32_t a_panel, uint32_t b_tile, uint32_t b_panel, uint32_t idesc,
                      bool add) {

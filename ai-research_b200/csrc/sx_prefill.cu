@@ -23,15 +23,11 @@
 //                    memory and store Y with TMA.
 // Every mbarrier wait is bounded; a wait that runs out records kDevWaitTimeout, the CTA stops
 // issuing, drains what it already issued and frees its TMEM.
-#include <cuda.h>
-#include <cudaTypedefs.h>
-
-#include <mutex>
-
 #include "sx_common.cuh"
 #include "sx_host.h"
 #include "sx_internal.h"
 #include "sx_tcgen05.cuh"
+#include "sx_tma.cuh"
 
 namespace sx {
 
@@ -47,33 +43,6 @@ constexpr uint32_t kStageBytes = kATile + kBTile + ((kRaw + 1023) & ~1023u);
 constexpr uint32_t kPrefillSmem = kStages * kStageBytes + 2048;  // + alignment, barriers
 constexpr uint32_t kTmemCols = 512;                     // two 128 x 256 f32 accumulators
 static_assert(kDqWarps * 8192 <= kStages * kStageBytes, "epilogue staging reuses the stages");
-
-// ---- TMA wrappers ----
-// 2-D tiled TMA load of box (x = k, y = token row) into this CTA's own shared memory
-SX_DEV void tma_load_2d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], "
-      "[%1, {%2, %3}], [%4];\n" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-      : "memory");
-}
-
-// 2-D tiled TMA store of a shared-memory box to global memory (rows/columns past the tensor's
-// extent are not written), tracked by the issuing thread's bulk async-group
-SX_DEV void tma_store_2d(const CUtensorMap *map, int32_t x, int32_t y, uint32_t src) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
-          reinterpret_cast<uint64_t>(map)),
-      "r"(x), "r"(y), "r"(src)
-      : "memory");
-}
-SX_DEV void bulk_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
-// the shared-memory source of all but the newest N committed groups has been read
-template <int N>
-SX_DEV void bulk_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
-}
-SX_DEV void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 
 // Instruction descriptor: D f32, A and B bf16, both K-major, N >> 3, M >> 4.
 constexpr uint32_t umma_idesc_bf16(int m, int n) {
@@ -304,21 +273,6 @@ __global__ void __launch_bounds__(kPThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
-}
-
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link)
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void *p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  });
-  return fn;
 }
 
 }  // namespace
