@@ -716,9 +716,10 @@ SX_API sx_status sx_dispatch_quantize_i8(sx_engine *e, const sx_quantize_i8_args
  *   y = x_out / sqrt(mean(x_out^2) + eps) * pre_w
  * in f32; y in y_dtype, SX_I8 as sx_dispatch_quantize_i8 of x_out with gain pre_w (scales to y_scale,
  * else NULL).  y NULL: x_out alone, without pre_w.  x_out may be x.  A norm is NaN in all of a row,
- * whatever that is written as (x_out with post_w, y), where the squares' sum passes f32, as with an
- * infinity, or mean + eps is below 2^-126, which no eps from there on lets happen: squares that small are
- * rounded away.  Sizes and alignment as there. */
+ * whatever that is written as (x_out with post_w, y; SX_I8 by its scale), where the squares' sum passes
+ * f32, as with an infinity, or mean + eps is below 2^-126, which no eps from there on lets happen: squares
+ * that small are rounded away.  (Codes of rows that count as zeros are zeros there too.)  Sizes and
+ * alignment as there. */
 typedef struct {
   const float *x;       /* [rows] of n: the residual stream             */
   const void *r;        /* [rows] of n, r_dtype: what the block computed */
